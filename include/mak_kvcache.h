@@ -603,6 +603,150 @@ MAK_API int mak_ipc_export(const void* ptr, void* handle_out, int64_t* offset_ou
 MAK_API int mak_ipc_import(const void* handle, int64_t offset, void** ptr_out);
 MAK_API int mak_ipc_release(const void* handle);
 
+/* ---- block-scaled 8-bit caches: attention and the writer ------------------- */
+
+/* Code types of a block-scaled cache. */
+#define MAK_CODE_INT8 0 /* signed codes, the writer makes -127 .. 127 */
+#define MAK_CODE_E4M3 1 /* OCP E4M3 (torch.float8_e4m3fn), the writer makes |v| <= 448 */
+
+/*
+ * A block-scaled cache: codes [num_blocks][num_heads][head_dim][block_size]
+ * (the tile layout, one byte per element, the last two axes contiguous) and one
+ * float per (block, head).  The value of a code is code * scale.
+ */
+typedef struct mak_block_cache_desc {
+  void* key;
+  void* value;
+  float* key_scale;
+  float* value_scale;
+  int64_t key_stride_block, key_stride_head;     /* bytes, multiples of 16 */
+  int64_t value_stride_block, value_stride_head; /* bytes, multiples of 16 */
+  int64_t key_scale_stride_block, key_scale_stride_head;     /* elements */
+  int64_t value_scale_stride_block, value_scale_stride_head; /* elements */
+  const int32_t* block_tables; /* [num_seqs][max_blocks], row stride table_stride */
+  const int32_t* context_lens; /* tokens of each sequence, those of this call included */
+  const int32_t* cu_seqlens;   /* [num_seqs + 1] rows of each sequence in the packed tensors; NULL: one row each */
+  int64_t table_stride;
+  int64_t num_blocks, num_seqs, max_blocks, num_rows;
+  int32_t num_heads, head_dim, block_size, code_type;
+} mak_block_cache_desc;
+
+typedef struct mak_block_attn_desc {
+  mak_block_cache_desc cache;
+  const void* q; /* [num_rows][num_q_heads][head_dim], head_dim contiguous */
+  void* out;     /* same shape, same dtype */
+  float* lse;    /* [num_rows][num_q_heads] contiguous, or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_stride_row, q_stride_head, out_stride_row, out_stride_head; /* elements */
+  int32_t num_q_heads, q_dtype, causal, window; /* window 0: none */
+  float scale;
+  int32_t reserved;
+} mak_block_attn_desc;
+
+/* Bytes of the workspace of mak_block_attention: independent of the call's sizes.
+ * It is zeroed once by the caller and then kept for calls that follow one another
+ * on one stream (the kernels leave its counters at zero). */
+MAK_API int64_t mak_block_attention_workspace_bytes(void);
+
+/*
+ * out[r, h] = softmax(scale * q[r, h] . K^T) V over the tokens that row r sees.
+ * Row r of sequence s is its (r - cu_seqlens[s])-th row of this call, at
+ * position context_lens[s] - (rows of s) + that index; it sees tokens up to its
+ * own position (causal) or all of them, and with window > 0 (causal only) the
+ * last `window` of those.  A row that sees nothing gives zeros and lse = -inf.
+ * Block ids outside [0, num_blocks) are skipped like tokens outside the sequence.
+ */
+MAK_API int mak_block_attention(const mak_block_attn_desc* desc, void* stream);
+
+/*
+ * Quantise k / v rows [num_rows][num_heads][head_dim] into the last positions of
+ * their sequences (context_lens counts them).  Per (block, head) and per K and V:
+ * m = max |x| over the finite values that the call writes there (0 when below
+ * 2^-100); the scale becomes m / 127 (INT8) or m / 448 (E4M3) where the call
+ * writes the block's first position, else the larger of that and the old scale,
+ * and the codes that stay are rounded again to a scale that grew.  Non-finite
+ * values are stored as 0.  Positions behind the last token of a block that the
+ * call begins are zeroed; other positions of the block keep their value.
+ */
+MAK_API int mak_block_append(const mak_block_cache_desc* cache, const void* k, const void* v, int64_t k_stride_row,
+                             int64_t k_stride_head, int64_t v_stride_row, int64_t v_stride_head, int32_t dtype, void* stream);
+
+/* ---- pages of a cache ------------------------------------------------------- */
+
+/*
+ * Page bookkeeping on the device: block_tables int32 [num_rows][max_blocks] (-1 =
+ * none), context_lens int32 [num_rows], ref_counts int32 [num_pages] (0 = free).
+ * Page ids and rows outside their ranges are skipped.  New pages are the free
+ * ones of lowest index, given out in the order of the requests.
+ */
+typedef struct mak_pages_desc {
+  int32_t* block_tables;
+  int32_t* context_lens;
+  int32_t* ref_counts;
+  int64_t table_stride;
+  int64_t num_rows, max_blocks, num_pages;
+  int64_t block_size;
+} mak_pages_desc;
+
+/* Planes that pages are copied in: page p of plane i lives at ptrs[i] + p * strides[i] (bytes), sizes[i] bytes long.
+ * The three are HOST arrays. */
+typedef struct mak_pages_planes {
+  const uint64_t* ptrs;
+  const int64_t* strides;
+  const int64_t* sizes;
+  int64_t num_planes;
+} mak_pages_planes;
+
+/* Row children[i] becomes a copy of row parents[i]: full pages are shared, a part-filled last page is copied into a new
+ * one.  Where no page is free the child ends at its last full page and missing[0] counts it.  `moves` is scratch of
+ * 2 * n + 2 int32.  No row may be a parent and a child of one call. */
+MAK_API int mak_pages_fork(const mak_pages_desc* pages, const mak_pages_planes* planes, const int32_t* parents,
+                           const int32_t* children, int64_t n, int32_t* missing, int32_t* moves, void* stream);
+
+/* Give rows[i] the pages for new_tokens[i] more tokens (context_lens grow by them).  Where pages run out the row grows to
+ * its last page's end and missing[0] counts the tokens that found no place. */
+MAK_API int mak_pages_grow(const mak_pages_desc* pages, const int32_t* rows, const int32_t* new_tokens, int64_t n,
+                           int32_t* missing, void* stream);
+
+/* Drop rows[i]: each of its pages loses one reference, its entries become -1, its length 0. */
+MAK_API int mak_pages_free(const mak_pages_desc* pages, const int32_t* rows, int64_t n, void* stream);
+
+/* Move the pages in use to indexes 0 .. live[0] - 1 (those already there stay), with tables and counts.  `scratch` is
+ * 3 * num_pages + 2 int32. */
+MAK_API int mak_pages_compact(const mak_pages_desc* pages, const mak_pages_planes* planes, int32_t* live, int32_t* scratch,
+                              void* stream);
+
+/* Copy page src[i] to page dst[i] in every plane (a pair with an id out of range is skipped; no page may be both a source
+ * and a destination, nor a destination twice). */
+MAK_API int mak_pages_copy(const mak_pages_planes* planes, int64_t num_pages, const int32_t* src, const int32_t* dst, int64_t n,
+                           void* stream);
+
+/* ---- rotary positions with several axes ------------------------------------- */
+
+#define MAK_ROPE_MAX_PAIRS 256
+
+typedef struct mak_rope_axes_desc {
+  const void* q; /* [tokens][q_heads][head_dim], head_dim contiguous */
+  const void* k; /* [tokens][k_heads][head_dim] or NULL */
+  void* q_out;
+  void* k_out;
+  const void* positions; /* [axes][tokens], int32 or int64, row stride pos_stride */
+  const float* cos;      /* [max_positions][rot_dim / 2], row stride cos_stride */
+  const float* sin;
+  int64_t tokens, max_positions;
+  int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head;
+  int64_t qo_stride_token, qo_stride_head, ko_stride_token, ko_stride_head; /* elements */
+  int64_t pos_stride, cos_stride, sin_stride;
+  int32_t q_heads, k_heads, head_dim, rot_dim;
+  int32_t dtype, pos_dtype, axes, interleaved, inverse, reserved;
+  uint8_t pair_axis[MAK_ROPE_MAX_PAIRS]; /* axis of each pair */
+} mak_rope_axes_desc;
+
+/* Pair j of each head turns by the angle of row positions[pair_axis[j]][t] (inverse = 1: by its negative, which is the
+ * gradient); columns past rot_dim are copied.  Tokens with a position outside the table keep that pair unchanged. */
+MAK_API int mak_rope_axes(const mak_rope_axes_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

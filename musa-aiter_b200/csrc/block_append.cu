@@ -1,0 +1,303 @@
+// The writer of a block-scaled 8-bit cache: k / v rows into the last positions of
+// their sequences, each (block, head) tile with one scale.
+//
+// Mathematics.  m = max |x| over the finite values written to the tile;
+// s = m / Qmax for a tile the call begins, else max(s_old, m / Qmax);
+// code = round(x / s), and where s grew the codes that stay become
+// round(code * (s_old / s)).  Every step is an IEEE operation in 32 bits (the
+// quotient x / s by reciprocal, remainder and one correction, which rounds
+// exactly: P. Markstein, IA-64 and Elementary Functions, 2000).
+//
+// Layout.  One warp owns one tile [head_dim][block_size] of K or V, so nothing is
+// shared and a tile is read at most once and written once.  A lane holds
+// head_dim / 32 neighbouring dims of 16 tokens: its loads are a piece of a token's
+// row, its stores whole 16-byte pieces of the tile's rows.
+#include "block_attn.cuh"
+
+namespace mak {
+
+int check_block_cache(const mak_block_cache_desc& c, const char* name);
+
+namespace {
+
+constexpr int kWarpsPerBlock = 4;
+
+struct AppendParams {
+  uint8_t* cache[2];
+  float* scale[2];
+  const void* x[2];
+  int64_t c_sb[2], c_sh[2], s_sb[2], s_sh[2], x_sr[2], x_sh[2];
+  const int32_t* tables;
+  const int32_t* ctx_lens;
+  const int32_t* starts;
+  int64_t table_stride, num_blocks, items;
+  int32_t num_seqs, max_blocks, num_rows, nh, bs_log2;
+};
+
+// Loads N neighbouring values of one row as float; non-finite values become 0.
+template <int DT, int N>
+__device__ __forceinline__ void load_values(const void* base, int64_t at, float (&x)[N]) {
+  if constexpr (DT == MAK_DT_F32) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 f = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(base) + at + i));
+      x[i] = f.x;
+      x[i + 1] = f.y;
+    }
+  } else {
+    uint32_t w[N / 2];
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if constexpr (N == 2) {
+      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    } else if constexpr (N == 4) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x, w[1] = v.y;
+    } else {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      if constexpr (DT == MAK_DT_BF16) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) x[i] = 0.f;
+}
+
+template <int CODE>
+__device__ __forceinline__ float code_value(uint32_t byte) {
+  if constexpr (CODE == MAK_CODE_INT8) {
+    return static_cast<float>(static_cast<int>(static_cast<int8_t>(byte)));
+  } else {
+    uint32_t h;
+    asm("{\n .reg .b16 a;\n cvt.u16.u32 a, %1;\n cvt.rn.f16x2.e4m3x2 %0, a;\n}" : "=r"(h) : "r"(byte));
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(h)));
+  }
+}
+
+// Four values to four code bytes.
+template <int CODE>
+__device__ __forceinline__ uint32_t to_codes(const float (&v)[4]) {
+  if constexpr (CODE == MAK_CODE_INT8) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // adding 1.5 * 2^23 rounds to a whole number in the low bits
+      b[i] = __float_as_uint(fminf(fmaxf(v[i], -127.f), 127.f) + 12582912.f);
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  } else {
+    uint32_t r;
+    asm("{\n .reg .b16 l, h;\n cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n"
+        " mov.b32 %0, {l, h};\n}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]));
+    return r;
+  }
+}
+
+template <int HD, int CODE, int DT>
+__global__ void __launch_bounds__(32 * kWarpsPerBlock) block_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kDims = HD / 32;
+  constexpr float kMost = CODE == MAK_CODE_INT8 ? 127.f : 448.f;
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t unit = blockIdx.x * static_cast<int64_t>(kWarpsPerBlock) + (threadIdx.x >> 5);
+  if (unit >= p.items * p.nh * 2) return;
+  const int kv = static_cast<int>(unit & 1);
+  const int head = static_cast<int>((unit >> 1) % p.nh);
+  const int64_t item = (unit >> 1) / p.nh;
+  const int bs = 1 << p.bs_log2;
+
+  // Slots floor(starts[s] / bs) + 2 s ... belong to sequence s: at least as many as it
+  // can touch blocks, whatever its position.
+  int s, row0, rows, nth;
+  if (p.starts == nullptr) {
+    s = static_cast<int>(item), row0 = s, rows = 1, nth = 0;
+  } else {
+    int lo = 0, n = p.num_seqs;  // the last s in [lo, lo + n) with slot(s) <= item
+    while (n > 1) {
+      const int step = (n + 31) >> 5;
+      const int at = lo + lane * step;
+      bool ok = false;
+      if (at < lo + n) ok = (max(__ldg(p.starts + at), 0) >> p.bs_log2) + 2 * static_cast<int64_t>(at) <= item;
+      const uint32_t votes = __ballot_sync(0xffffffffu, ok);
+      const int k = votes == 0 ? 0 : 31 - __clz(votes);
+      const int end = lo + n;
+      lo += k * step;
+      n = min(step, end - lo);
+    }
+    s = lo;
+    row0 = max(__ldg(p.starts + s), 0);
+    rows = min(__ldg(p.starts + s + 1), p.num_rows) - row0;
+    nth = static_cast<int>(item - (row0 >> p.bs_log2) - 2 * static_cast<int64_t>(s));
+  }
+  const int64_t ctx = __ldg(p.ctx_lens + s);
+  const int64_t first = ctx - rows;  // position of the call's first row
+  if (rows <= 0 || first < 0) return;
+  const int64_t block = (first >> p.bs_log2) + nth;
+  const int64_t start = block << p.bs_log2;
+  if (start >= ctx || block >= p.max_blocks) return;
+  const int page = __ldg(p.tables + s * p.table_stride + block);
+  if (page < 0 || page >= p.num_blocks) return;
+  const bool begun = start >= first;
+  const int off0 = begun ? 0 : static_cast<int>(first - start);  // offsets [off0, off1) are written
+  const int off1 = static_cast<int>(min(ctx - start, static_cast<int64_t>(bs)));
+  const void* x = p.x[kv];
+  // element of offset o, this lane's dims: xat + o * row stride
+  const int64_t xat = (row0 + start - first) * p.x_sr[kv] + head * p.x_sh[kv] + lane * kDims;
+  uint8_t* tile = p.cache[kv] + page * p.c_sb[kv] + head * p.c_sh[kv] + static_cast<int64_t>(lane * kDims) * bs;
+  float* sp = p.scale[kv] + page * p.s_sb[kv] + head * p.s_sh[kv];
+
+  float old = 0.f;
+  if (!begun) {
+    old = *sp;
+    if (!(old > 0.f) || old == INFINITY) old = 0.f;
+  }
+  float top = 0.f;
+#pragma unroll 4
+  for (int o = off0; o < off1; ++o) {
+    float v[kDims];
+    load_values<DT, kDims>(x, xat + o * p.x_sr[kv], v);
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) top = fmaxf(top, fabsf(v[i]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float mine = top < 0x1p-100f ? 0.f : __fdiv_rn(top, kMost);
+  const float now = fmaxf(old, mine);
+  const bool grew = now > old;
+  if (lane == 0 && (begun || grew || old == 0.f)) *sp = now;
+  const float safe = now > 0.f ? now : 1.f;
+  const float ratio = grew ? __fdiv_rn(old, safe) : 1.f;
+  const float inv = __frcp_rn(safe);
+  const bool direct = safe < 0x1p-60f || safe > 0x1p60f;  // the remainder could underflow
+
+  for (int c0 = 0; c0 < bs; c0 += 16) {
+    const bool fresh = c0 < off1 && c0 + 16 > off0;
+    if (!fresh && !begun && !(grew)) continue;
+    uint32_t w[kDims][4];
+    if (begun) {
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) {
+        const uint4 t = *reinterpret_cast<const uint4*>(tile + static_cast<int64_t>(i) * bs + c0);
+        w[i][0] = t.x, w[i][1] = t.y, w[i][2] = t.z, w[i][3] = t.w;
+      }
+      if (grew) {
+#pragma unroll
+        for (int i = 0; i < kDims; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) v[b] = __fmul_rn(code_value<CODE>((w[i][q] >> (8 * b)) & 0xffu), ratio);
+            w[i][q] = to_codes<CODE>(v);
+          }
+      }
+    }
+    if (fresh) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float v[4][kDims];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const int o = c0 + 4 * q + b;
+#pragma unroll
+          for (int i = 0; i < kDims; ++i) v[b][i] = 0.f;
+          if (o >= off0 && o < off1) load_values<DT, kDims>(x, xat + o * p.x_sr[kv], v[b]);
+        }
+        uint32_t mask = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+          if (c0 + 4 * q + b >= off0 && c0 + 4 * q + b < off1) mask |= 0xffu << (8 * b);
+#pragma unroll
+        for (int i = 0; i < kDims; ++i) {
+          float y[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            if (direct) {
+              y[b] = __fdiv_rn(v[b][i], safe);
+            } else {
+              const float q0 = __fmul_rn(v[b][i], inv);
+              y[b] = __fmaf_rn(__fmaf_rn(-q0, safe, v[b][i]), inv, q0);
+            }
+          }
+          w[i][q] = (w[i][q] & ~mask) | (to_codes<CODE>(y) & mask);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDims; ++i)
+      *reinterpret_cast<uint4*>(tile + static_cast<int64_t>(i) * bs + c0) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+  }
+}
+
+template <int HD, int CODE>
+int launch_append(const AppendParams& p, int dtype, dim3 grid, cudaStream_t st) {
+  const dim3 block(32 * kWarpsPerBlock);
+  const char* name = "mak_block_append";
+  if (dtype == MAK_DT_F16) return launch_pdl(name, block_append_kernel<HD, CODE, MAK_DT_F16>, grid, block, 0, st, p);
+  if (dtype == MAK_DT_BF16) return launch_pdl(name, block_append_kernel<HD, CODE, MAK_DT_BF16>, grid, block, 0, st, p);
+  return launch_pdl(name, block_append_kernel<HD, CODE, MAK_DT_F32>, grid, block, 0, st, p);
+}
+
+template <int HD>
+int launch_append_code(const AppendParams& p, int code, int dtype, dim3 grid, cudaStream_t st) {
+  return code == MAK_CODE_INT8 ? launch_append<HD, MAK_CODE_INT8>(p, dtype, grid, st)
+                               : launch_append<HD, MAK_CODE_E4M3>(p, dtype, grid, st);
+}
+
+}  // namespace
+}  // namespace mak
+
+using namespace mak;
+
+extern "C" int mak_block_append(const mak_block_cache_desc* cache, const void* k, const void* v, int64_t k_stride_row,
+                                int64_t k_stride_head, int64_t v_stride_row, int64_t v_stride_head, int32_t dtype, void* stream) {
+  const char* name = "mak_block_append";
+  if (cache == nullptr) return fail(MAK_E_INVALID, "%s: null descriptor", name);
+  const mak_block_cache_desc& c = *cache;
+  if (int rc = check_block_cache(c, name)) return rc;
+  if (dtype != MAK_DT_F16 && dtype != MAK_DT_BF16 && dtype != MAK_DT_F32)
+    return fail(MAK_E_UNSUPPORTED, "%s: k / v must be float16, bfloat16 or float32", name);
+  if (c.num_seqs == 0 || c.num_rows == 0) return MAK_OK;
+  if (k == nullptr || v == nullptr) return fail(MAK_E_INVALID, "%s: null k or v", name);
+  const uint64_t align = 16 / dtype_bytes(dtype);
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) ||
+      (static_cast<uint64_t>(k_stride_row | k_stride_head | v_stride_row | v_stride_head) & (align - 1)))
+    return fail(MAK_E_INVALID, "%s: k / v need 16-byte aligned rows", name);
+  AppendParams p = {};
+  p.cache[0] = static_cast<uint8_t*>(c.key), p.cache[1] = static_cast<uint8_t*>(c.value);
+  p.scale[0] = c.key_scale, p.scale[1] = c.value_scale;
+  p.x[0] = k, p.x[1] = v;
+  p.c_sb[0] = c.key_stride_block, p.c_sb[1] = c.value_stride_block;
+  p.c_sh[0] = c.key_stride_head, p.c_sh[1] = c.value_stride_head;
+  p.s_sb[0] = c.key_scale_stride_block, p.s_sb[1] = c.value_scale_stride_block;
+  p.s_sh[0] = c.key_scale_stride_head, p.s_sh[1] = c.value_scale_stride_head;
+  p.x_sr[0] = k_stride_row, p.x_sr[1] = v_stride_row;
+  p.x_sh[0] = k_stride_head, p.x_sh[1] = v_stride_head;
+  p.tables = c.block_tables, p.ctx_lens = c.context_lens, p.starts = c.cu_seqlens;
+  p.table_stride = c.table_stride, p.num_blocks = c.num_blocks;
+  p.num_seqs = static_cast<int32_t>(c.num_seqs), p.max_blocks = static_cast<int32_t>(c.max_blocks);
+  p.num_rows = static_cast<int32_t>(c.num_rows), p.nh = c.num_heads;
+  p.bs_log2 = c.block_size == 16 ? 4 : c.block_size == 32 ? 5 : c.block_size == 64 ? 6 : 7;
+  p.items = c.cu_seqlens == nullptr ? c.num_seqs : (c.num_rows >> p.bs_log2) + 2 * c.num_seqs;
+  const int64_t blocks = (p.items * p.nh * 2 + kWarpsPerBlock - 1) / kWarpsPerBlock;
+  if (blocks > 0x7fffffff) return fail(MAK_E_UNSUPPORTED, "%s: too many rows for one call", name);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  cudaStream_t st = as_stream(stream);
+  if (c.head_dim == 64) return launch_append_code<64>(p, c.code_type, dtype, grid, st);
+  if (c.head_dim == 128) return launch_append_code<128>(p, c.code_type, dtype, grid, st);
+  return launch_append_code<256>(p, c.code_type, dtype, grid, st);
+}

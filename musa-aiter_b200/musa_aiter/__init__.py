@@ -8,7 +8,10 @@ rejected (there is no CPU fallback).
 
 from .version import __version__
 from . import registry, dispatch
+from .ops.block_cache import kv_append_block_scaled, paged_attention_block_scaled
 from .ops.cache import apply_rope, apply_rope_to_key_cache, copy_to_kv_cache
+from .ops.pages import kv_pages_compact, kv_pages_copy, kv_pages_fork, kv_pages_free, kv_pages_grow
+from .ops.rope_axes import apply_rope_axes, apply_rope_axes_backward
 from .ops.kv_layout import KVFormatFacts, KVLayoutKind, KVLayoutSpec, KVOrganization, KVScaleKind
 from .ops.kv_transfer_plan import (
     KVTransferEntry,

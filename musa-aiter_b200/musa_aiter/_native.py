@@ -272,6 +272,16 @@ _PROTOTYPES = {
             c_void_p,
         ],
     ),
+    # descriptors of the calls below are packed bytes
+    "mak_block_attention_workspace_bytes": (c_int64, []),
+    "mak_block_attention": (c_int32, [c_void_p, c_void_p]),
+    "mak_block_append": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p]),
+    "mak_pages_fork": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "mak_pages_grow": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "mak_pages_free": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p]),
+    "mak_pages_compact": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mak_pages_copy": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "mak_rope_axes": (c_int32, [c_void_p, c_void_p]),
 }
 
 _LOCK = threading.Lock()

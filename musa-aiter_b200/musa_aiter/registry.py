@@ -120,6 +120,21 @@ for _name, _status, _dtypes, _desc, _notes in _KVCACHE:
 _CACHE = [
     ("apply_rope", "b200", _FLOAT, "RoPE with the reference's per-operation rounding.", ()),
     ("apply_rope_to_key_cache", "b200", _FLOAT, "Apply RoPE in place to selected paged key-cache slots.", ()),
+    ("apply_rope_axes", "b200", _HALF, "RoPE with one position per axis (time, height, width), q and k in one launch.", ()),
+    ("apply_rope_axes_backward", "b200", _HALF, "Gradient of apply_rope_axes.", ()),
+    ("kv_append_block_scaled", "b200", _FLOAT, "Quantising write into an 8-bit cache with one scale per block and head.", ()),
 ]
 for _name, _status, _dtypes, _desc, _notes in _CACHE:
     register(OperatorCapability(_name, "cache", _status, _dtypes, ("cuda",), (BACKEND,), _desc, _notes, ("handwritten-cuda-sm100a",)))
+
+# Operators of this build on top of the reference's families.
+_EXTRA = [
+    ("paged_attention_block_scaled", "attention", _HALF, "Attention over a paged 8-bit cache with one scale per block and head."),
+    ("kv_pages_copy", "pages", ("any",), "Copy pages within every plane of a cache, one launch."),
+    ("kv_pages_fork", "pages", ("any",), "Continue sequences in new rows: full pages shared, part-filled ones copied."),
+    ("kv_pages_grow", "pages", ("int32",), "Hand out pages for new tokens."),
+    ("kv_pages_free", "pages", ("int32",), "Return the pages of ended sequences."),
+    ("kv_pages_compact", "pages", ("any",), "Move the pages in use to the lowest indexes."),
+]
+for _name, _family, _dtypes, _desc in _EXTRA:
+    register(OperatorCapability(_name, _family, "b200", _dtypes, ("cuda",), (BACKEND,), _desc, (), ("handwritten-cuda-sm100a",)))
