@@ -533,6 +533,8 @@ constexpr int64_t kCounterBytes = (2 * kMaxGrid * 4 + 255) / 256 * 256;
 
 }  // namespace
 
+int launch_block_attn_tc(const BlockAttnParams& p, int head_dim, int code, cudaStream_t st);
+
 int check_block_cache(const mak_block_cache_desc& c, const char* name) {
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
     return fail(MAK_E_UNSUPPORTED, "%s: head_dim must be 64, 128 or 256, got %d", name, c.head_dim);
@@ -611,6 +613,7 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
   cudaStream_t st = as_stream(stream);
   // Rows that share a cache head, on average: more than 8 fill a second set of columns.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
+  if (rows >= 64 && c.head_dim <= 128) return launch_block_attn_tc(p, c.head_dim, c.code_type, st);
   const bool wide = rows > 8 && c.head_dim < 256;
   if (c.head_dim == 64) return wide ? launch_rows_code<64, 2>(p, c.code_type, st) : launch_rows_code<64, 1>(p, c.code_type, st);
   if (c.head_dim == 128) return wide ? launch_rows_code<128, 2>(p, c.code_type, st) : launch_rows_code<128, 1>(p, c.code_type, st);
