@@ -47,12 +47,14 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// Asynchronous 16-byte copy to shared memory; bytes = 0 stores zeros and reads nothing.
+__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Tiles of a unit of sequence v (at least one, so that empty rows are written).
@@ -68,17 +70,22 @@ __device__ __forceinline__ int64_t seq_work(const BlockAttnParams& p, const SeqV
   return groups * p.nh * unit_tiles(v);
 }
 
+// Each lane's loads go through its own slots of a ring: the lane that copies 16 bytes
+// in is the one that reads them, so no barrier is needed, and the loads in flight cost
+// no registers.  The ring holds the K (or V) share of one tile: while K is consumed V of
+// the same tile takes its slots, and K of the next tile takes V's.
 template <int HD, int NT>
 struct Smem {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kPStride = kTile * 2 + 16;  // bytes between rows of the weights
+  static constexpr int kPStride = 64 * 2 + 16;  // bytes between rows of the weights of 64 tokens
   union {
-    uint8_t weights[kWarps][kRows * kPStride];
+    uint4 ring[kWarps][HD / 4][32];
     float acc[kWarps][kRows][HD + 1];
   };
+  uint8_t weights[kWarps][kRows * kPStride];
+  alignas(16) __half q[kRows][HD + 16];
   float m[kWarps][kRows];
   float l[kWarps][kRows];
-  alignas(16) __half q[kRows][HD + 16];
   float qscale[kRows];
   int64_t scan[kWarps];
   int64_t begin_base;
@@ -87,10 +94,12 @@ struct Smem {
 };
 
 template <int HD, int NT, int CODE>
-__global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128 ? 4 : 2))
+__global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
     block_attn_rows_kernel(const __grid_constant__ BlockAttnParams p) {
   constexpr int kRows = 8 * NT;
-  __shared__ Smem<HD, NT> sm;
+  constexpr int kSteps = HD / 16;  // groups of 4 loads of one lane per tile of K (and of V)
+  extern __shared__ __align__(16) uint8_t raw[];
+  Smem<HD, NT>& sm = *reinterpret_cast<Smem<HD, NT>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   pdl_wait();
@@ -252,21 +261,65 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
     const uint8_t* vbase = p.value + head * p.v_sh;
     const int bs = 1 << p.bs_log2;
     const int tile0 = v.hi > v.lo ? v.lo / kTile : 0;
-
-    for (int t = ta + warp; t < tb; t += kWarps) {
-      const int tok = (tile0 + t) * kTile;
-      if (tok >= any_hi || tok + kTile <= any_lo) continue;
-      // this lane's 16 tokens of K: chunk g
-      const int kt = tok + 16 * g;
+    // tiles of this warp: t, t + kWarps, ... below t_end, all of which some row sees
+    int t = ta + warp, t_end = tb;
+    if (any_hi > any_lo) {
+      t_end = min(t_end, (any_hi + kTile - 1) / kTile - tile0);
+      const int skip = any_lo / kTile - tile0 - t;
+      if (skip > 0) t += (skip + kWarps - 1) / kWarps * kWarps;
+    } else {
+      t_end = 0;
+    }
+    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(&sm.ring[warp][0][lane]));
+    // Block of this lane's 16 tokens of K (chunk g) of tile i, -1 where there is none.
+    auto find = [&](int i) {
+      const int kt = (tile0 + i) * kTile + 16 * g;
       int page = -1;
-      if (kt < any_hi && kt + 16 > any_lo) page = __ldg(table + (kt >> p.bs_log2));
-      if (page >= p.num_blocks) page = -1;
-      const uint8_t* kp = kbase + page * p.k_sb + (kt & (bs - 1)) + static_cast<int64_t>(c) * bs;
-      float ksc = 0.f, vsc = 0.f;
-      if (page >= 0) {
-        ksc = __ldg(p.key_scale + page * p.ks_sb + head * p.ks_sh);
-        vsc = __ldg(p.value_scale + page * p.vs_sb + head * p.vs_sh);
+      if (i < t_end && kt < any_hi && kt + 16 > any_lo) page = __ldg(table + (kt >> p.bs_log2));
+      return page >= p.num_blocks ? -1 : page;
+    };
+    int page = find(t), page1 = find(t + kWarps);
+    float ksc = 0.f, vsc = 0.f;
+    auto scales = [&](int pg, float* a, float* b) {
+      *a = *b = 0.f;
+      if (pg >= 0) {
+        *a = __ldg(p.key_scale + pg * p.ks_sb + head * p.ks_sh);
+        *b = __ldg(p.value_scale + pg * p.vs_sb + head * p.vs_sh);
       }
+    };
+    const int in_block = (16 * g) & (bs - 1);  // a tile starts at a block's start
+    const uint8_t* kp = page >= 0 ? kbase + page * p.k_sb + in_block + c * bs : kbase;
+    uint32_t kn = page >= 0 ? 16 : 0;
+    if (t < t_end) {
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks) {
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) copy_async(ring + (4 * ks + jj) * 512, kp + (16 * ks + 4 * jj) * (kn ? bs : 0), kn);
+        copy_commit();
+      }
+      scales(page, &ksc, &vsc);
+    }
+
+    for (; t < t_end; t += kWarps) {
+      const int tok = (tile0 + t) * kTile;
+      const int kt = tok + 16 * g;
+      // V of this tile: chunk 4 hf + c
+      const uint8_t* vp[2];
+      uint32_t vn[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int vpage = __shfl_sync(0xffffffffu, page, (4 * hf + c) * 4);
+        vn[hf] = vpage >= 0 ? 16 : 0;
+        vp[hf] = vpage >= 0 ? vbase + vpage * p.v_sb + ((64 * hf + 16 * c) & (bs - 1)) + g * bs : vbase;
+      }
+      // the next tile
+      const int page2 = find(t + 2 * kWarps);
+      const bool more = t + kWarps < t_end;
+      const uint8_t* kp1 = page1 >= 0 ? kbase + page1 * p.k_sb + in_block + c * bs : kbase;
+      const uint32_t kn1 = page1 >= 0 ? 16 : 0;
+      float ksc1, vsc1;
+      scales(page1, &ksc1, &vsc1);
+
       float s[NT][8][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -275,13 +328,11 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[n][i][e] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
+      for (int ks = 0; ks < kSteps; ++ks) {
+        copy_wait<kSteps - 1>();
         uint4 x[4];
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          x[jj] = make_uint4(0, 0, 0, 0);
-          if (page >= 0) x[jj] = ldg_stream(kp + static_cast<int64_t>(16 * ks + 4 * jj) * bs);
-        }
+        for (int jj = 0; jj < 4; ++jj) x[jj] = sm.ring[warp][4 * ks + jj][lane];
 #pragma unroll
         for (int wd = 0; wd < 4; ++wd) {
           const uint32_t x0 = (&x[0].x)[wd], x1 = (&x[1].x)[wd], x2 = (&x[2].x)[wd], x3 = (&x[3].x)[wd];
@@ -297,6 +348,14 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
             mma_f16(s[n][2 * wd + 1], b[0], b[1], b[2], b[3], qf[n][ks][0], qf[n][ks][1]);
           }
         }
+        // the slots just read take the V loads that will be the kSteps-th to be waited for from here
+        const int hf = ks / (kSteps / 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = 16 * (2 * (ks % (kSteps / 2)) + (e >> 1)) + 8 * (e & 1);
+          copy_async(ring + (4 * ks + e) * 512, vp[hf] + row * (vn[hf] ? bs : 0), vn[hf]);
+        }
+        copy_commit();
       }
       // s[n][i][2 * r + e]: token kt + 2 i + r, column 2 c + e
       const bool whole = tok >= all_lo && tok + kTile <= all_hi;
@@ -307,9 +366,9 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
       const float vkeep = vnew > vref ? vref / vnew : 1.f;
       const float vfac = vnew > 0.f ? vsc / vnew * 32768.f : 0.f;
       vref = vnew;
-      uint8_t* wrow = sm.weights[warp];
       bool moved = false;
       float keep[NT][2];
+      uint32_t wt[NT][2][8];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float f[2] = {qs[n][0] * ksc, qs[n][1] * ksc};
@@ -338,18 +397,11 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
           moved |= keep[n][e] != 1.f;
           m[n][e] = mn;
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float w8 = exp2_fast(s[n][i][2 * r + e] - ms);
-              l[n][e] += w8;
-              s[n][i][2 * r + e] = w8 * vfac;
-            }
-          uint4* dst = reinterpret_cast<uint4*>(wrow + (n * 8 + 2 * c + e) * Smem<HD, NT>::kPStride + g * 32);
-          dst[0] = make_uint4(pack_f16(s[n][0][e], s[n][0][2 + e]), pack_f16(s[n][1][e], s[n][1][2 + e]),
-                              pack_f16(s[n][2][e], s[n][2][2 + e]), pack_f16(s[n][3][e], s[n][3][2 + e]));
-          dst[1] = make_uint4(pack_f16(s[n][4][e], s[n][4][2 + e]), pack_f16(s[n][5][e], s[n][5][2 + e]),
-                              pack_f16(s[n][6][e], s[n][6][2 + e]), pack_f16(s[n][7][e], s[n][7][2 + e]));
+          for (int i = 0; i < 8; ++i) {
+            const float w0 = exp2_fast(s[n][i][e] - ms), w1 = exp2_fast(s[n][i][2 + e] - ms);
+            l[n][e] += w0 + w1;
+            wt[n][e][i] = pack_f16(w0 * vfac, w1 * vfac);
+          }
         }
       }
       if (__any_sync(0xffffffffu, moved)) {
@@ -360,50 +412,72 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[n][i][e] *= keep[n][e & 1];
       }
-      __syncwarp();
+      uint8_t* wrow = sm.weights[warp];
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const int vt = tok + 64 * hf + 16 * c;
-        const int vpage = __shfl_sync(0xffffffffu, page, (4 * hf + c) * 4);
-        const uint8_t* vp = vbase + vpage * p.v_sb + (vt & (bs - 1)) + static_cast<int64_t>(g) * bs;
+        // weights of 64 tokens from the score layout to the operand layout
+        if ((g >> 2) == hf) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint4* dst = reinterpret_cast<uint4*>(wrow + (n * 8 + 2 * c + e) * Smem<HD, NT>::kPStride + (g & 3) * 32);
+              dst[0] = make_uint4(wt[n][e][0], wt[n][e][1], wt[n][e][2], wt[n][e][3]);
+              dst[1] = make_uint4(wt[n][e][4], wt[n][e][5], wt[n][e][6], wt[n][e][7]);
+            }
+        }
+        __syncwarp();
         uint32_t pf[NT][4][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          const uint4* src = reinterpret_cast<const uint4*>(wrow + (n * 8 + g) * Smem<HD, NT>::kPStride + (4 * hf + c) * 32);
+          const uint4* src = reinterpret_cast<const uint4*>(wrow + (n * 8 + g) * Smem<HD, NT>::kPStride + c * 32);
           const uint4 a = src[0], b = src[1];
           pf[n][0][0] = a.x, pf[n][0][1] = a.y, pf[n][1][0] = a.z, pf[n][1][1] = a.w;
           pf[n][2][0] = b.x, pf[n][2][1] = b.y, pf[n][3][0] = b.z, pf[n][3][1] = b.w;
         }
+        __syncwarp();
         // tokens of this chunk that some row sees; the others' codes may be anything and count as 0
+        const int vt = tok + 64 * hf + 16 * c;
         const int first = any_lo - vt, last = any_hi - vt;
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-          uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-          if (vpage >= 0) {
-            x0 = ldg_stream(vp + static_cast<int64_t>(16 * i) * bs);
-            x1 = ldg_stream(vp + static_cast<int64_t>(16 * i + 8) * bs);
-          }
+        for (int i2 = 0; i2 < kSteps / 2; ++i2) {
+          const int ks = hf * (kSteps / 2) + i2;
+          copy_wait<kSteps - 1>();
+          uint4 x[4];
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint32_t y0 = (&x0.x)[q4], y1 = (&x1.x)[q4];
-            if (!whole) {
-              uint32_t mask = 0;
+          for (int e = 0; e < 4; ++e) x[e] = sm.ring[warp][4 * ks + e][lane];
 #pragma unroll
-              for (int b = 0; b < 4; ++b)
-                if (4 * q4 + b >= first && 4 * q4 + b < last) mask |= 0xffu << (8 * b);
-              y0 &= mask;
-              y1 &= mask;
+          for (int i1 = 0; i1 < 2; ++i1) {
+            const int i = 2 * i2 + i1;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint32_t y0 = (&x[2 * i1].x)[q4], y1 = (&x[2 * i1 + 1].x)[q4];
+              if (!whole) {
+                uint32_t mask = 0;
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                  if (4 * q4 + b >= first && 4 * q4 + b < last) mask |= 0xffu << (8 * b);
+                y0 &= mask;
+                y1 &= mask;
+              }
+              uint32_t a[4];
+              codes4_to_f16<CODE>(y0, &a[0], &a[2]);
+              codes4_to_f16<CODE>(y1, &a[1], &a[3]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma_f16(acc[n][i], a[0], a[1], a[2], a[3], pf[n][q4][0], pf[n][q4][1]);
             }
-            uint32_t a[4];
-            codes4_to_f16<CODE>(y0, &a[0], &a[2]);
-            codes4_to_f16<CODE>(y1, &a[1], &a[3]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(acc[n][i], a[0], a[1], a[2], a[3], pf[n][q4][0], pf[n][q4][1]);
           }
+          if (more) {
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) copy_async(ring + (4 * ks + jj) * 512, kp1 + (16 * ks + 4 * jj) * (kn1 ? bs : 0), kn1);
+          }
+          copy_commit();
         }
       }
-      __syncwarp();
+      page = page1, page1 = page2;
+      ksc = ksc1, vsc = vsc1;
     }
+    copy_wait<0>();
 
     // ---- join the warps --------------------------------------------------------
 #pragma unroll
@@ -412,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
-    __syncthreads();  // the weights are read, their space takes the accumulators
+    __syncthreads();  // the ring is read, its space takes the accumulators
     const float unit_scale = vref * (1.f / 32768.f);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -478,30 +552,39 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
       __syncthreads();
       if (sm.last) {
         __threadfence();
-        for (int idx = tid; idx < live * HD; idx += kThreads) {
-          const int r = idx / HD, d = idx % HD;
-          float mx = -INFINITY, o = 0.f, sum = 0.f;
+        for (int idx = tid; idx < live * (HD / 4); idx += kThreads) {
+          const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+          float mx = -INFINITY, sum = 0.f;
+          float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
           for (int b = first_block; b <= last_block; ++b) {
             const float* src = p.partial + (2 * static_cast<int64_t>(b) + (unit_w0 > b * chunk ? 1 : 0)) * kStep;
             const float pm = __ldcg(src + kRows * HD + r), pl = __ldcg(src + kRows * HD + kRows + r);
-            const float po = __ldcg(src + r * HD + d);
+            const float4 po = __ldcg(reinterpret_cast<const float4*>(src + r * HD + d));
             const float mn = fmaxf(mx, pm);
             const float ms = mn == -INFINITY ? 0.f : mn;
             const float k0 = exp2_fast(mx - ms), k1 = exp2_fast(pm - ms);
-            o = o * k0 + po * k1;
+            o[0] = o[0] * k0 + po.x * k1;
+            o[1] = o[1] * k0 + po.y * k1;
+            o[2] = o[2] * k0 + po.z * k1;
+            o[3] = o[3] * k0 + po.w * k1;
             sum = sum * k0 + pl * k1;
             mx = mn;
           }
           const int i = (row0 + r) / p.group, j = head * p.group + (row0 + r) % p.group;
-          const float y = sum > 0.f || sum != sum ? o / sum : 0.f;
+          const bool some = sum > 0.f || sum != sum;
           const int64_t at = (v.first + i) * p.o_sr + j * p.o_sh + d;
-          if (p.q_bf16)
-            reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
-          else
-            reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(y);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float y = some ? o[e] / sum : 0.f;
+            if (p.q_bf16)
+              reinterpret_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(y);
+            else
+              reinterpret_cast<__half*>(p.out)[at + e] = __float2half_rn(y);
+          }
           if (d == 0 && p.lse != nullptr)
             p.lse[static_cast<int64_t>(v.first + i) * p.nh * p.group + j] =
-                sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+                some ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
         }
         if (tid == 0) p.counters[slot0] = 0;
       }
@@ -513,15 +596,22 @@ __global__ void __launch_bounds__(kThreads, HD == 64 ? 4 : (NT == 1 && HD == 128
 template <int HD, int NT, int CODE>
 int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
   const void* fn = reinterpret_cast<const void*>(&block_attn_rows_kernel<HD, NT, CODE>);
+  constexpr int kBytes = sizeof(Smem<HD, NT>);
   static int per_sm = 0;
   if (per_sm == 0) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(block_attn_rows_kernel<HD, NT, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return cuda_fail(e, "mak_block_attention");
+    }
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kThreads, 0) != cudaSuccess || n <= 0) n = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kThreads, kBytes) != cudaSuccess || n <= 0) n = 1;
     per_sm = n;
   }
   int grid = per_sm * sm_count();
   if (grid > kMaxGrid) grid = kMaxGrid;
-  return launch_pdl("mak_block_attention", block_attn_rows_kernel<HD, NT, CODE>, dim3(grid), dim3(kThreads), 0, st, p);
+  return launch_pdl("mak_block_attention", block_attn_rows_kernel<HD, NT, CODE>, dim3(grid), dim3(kThreads), kBytes, st, p);
 }
 
 template <int HD, int NT>
