@@ -72,14 +72,18 @@ __device__ __forceinline__ int64_t seq_work(const BlockAttnParams& p, const SeqV
 
 // Each lane's loads go through its own slots of a ring: the lane that copies 16 bytes
 // in is the one that reads them, so no barrier is needed, and the loads in flight cost
-// no registers.  The ring holds the K (or V) share of one tile: while K is consumed V of
-// the same tile takes its slots, and K of the next tile takes V's.
+// no registers.  Loads come in groups of 4 per lane, head_dim / 16 groups for K of a tile
+// and as many for V; each group that is consumed makes room for the one kRing further on,
+// so V follows K and K of the next tile follows V.  The loops are rolled as far as the
+// accumulators allow: unrolled whole, waiting for instructions cost more than the work.
+constexpr int kRing = 4;  // groups
+
 template <int HD, int NT>
 struct Smem {
   static constexpr int kRows = 8 * NT;
   static constexpr int kPStride = 64 * 2 + 16;  // bytes between rows of the weights of 64 tokens
   union {
-    uint4 ring[kWarps][HD / 4][32];
+    uint4 ring[kWarps][4 * kRing][32];
     float acc[kWarps][kRows][HD + 1];
   };
   uint8_t weights[kWarps][kRows * kPStride];
@@ -213,18 +217,11 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
       }
     }
     __syncthreads();
-    uint32_t qf[NT][HD / 16][2];
     float qs[NT][2];
     int lo[NT][2], hi[NT][2];
     int all_lo = 0, all_hi = 0x7fffffff, any_lo = 0x7fffffff, any_hi = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        const uint2 f = *reinterpret_cast<const uint2*>(&sm.q[n * 8 + g][ks * 16 + c * 4]);
-        qf[n][ks][0] = f.x;
-        qf[n][ks][1] = f.y;
-      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = n * 8 + 2 * c + e;
@@ -290,11 +287,17 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
     const int in_block = (16 * g) & (bs - 1);  // a tile starts at a block's start
     const uint8_t* kp = page >= 0 ? kbase + page * p.k_sb + in_block + c * bs : kbase;
     uint32_t kn = page >= 0 ? 16 : 0;
+    // group i of K: rows 16 i + 4 jj + c of this lane's chunk
+    auto load_k = [&](int slot, int i, const uint8_t* from, uint32_t bytes) {
+      const uint8_t* at = from + (bytes ? 16 * i * bs : 0);
+      const int step = bytes ? 4 * bs : 0;
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) copy_async(ring + (4 * slot + jj) * 512, at + jj * step, bytes);
+    };
     if (t < t_end) {
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) {
-#pragma unroll
-        for (int jj = 0; jj < 4; ++jj) copy_async(ring + (4 * ks + jj) * 512, kp + (16 * ks + 4 * jj) * (kn ? bs : 0), kn);
+      for (int i = 0; i < kRing; ++i) {
+        load_k(i, i, kp, kn);
         copy_commit();
       }
       scales(page, &ksc, &vsc);
@@ -327,35 +330,48 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
         for (int i = 0; i < 8; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[n][i][e] = 0.f;
+      // group i of V: rows 32 pair + 8 e + g of chunk 4 hf + c
+      auto load_v = [&](int slot, int hf, int pair) {
+        const uint8_t* at = hf ? vp[1] : vp[0];
+        const uint32_t bytes = hf ? vn[1] : vn[0];
+        const int step = bytes ? 8 * bs : 0;
+        at += 4 * pair * step;
 #pragma unroll
-      for (int ks = 0; ks < kSteps; ++ks) {
-        copy_wait<kSteps - 1>();
-        uint4 x[4];
+        for (int e = 0; e < 4; ++e) copy_async(ring + (4 * slot + e) * 512, at + e * step, bytes);
+      };
+#pragma unroll 1
+      for (int k0 = 0; k0 < kSteps; k0 += kRing) {
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) x[jj] = sm.ring[warp][4 * ks + jj][lane];
+        for (int u = 0; u < kRing; ++u) {
+          const int ks = k0 + u;
+          copy_wait<kRing - 1>();
+          uint4 x[4];
 #pragma unroll
-        for (int wd = 0; wd < 4; ++wd) {
-          const uint32_t x0 = (&x[0].x)[wd], x1 = (&x[1].x)[wd], x2 = (&x[2].x)[wd], x3 = (&x[3].x)[wd];
-          uint32_t a[4], b[4];
-          // tokens 4 wd, 4 wd + 1 -> row pair (g, g + 8) of tile 2 wd
-          codes4_to_f16<CODE>(__byte_perm(x0, x1, 0x5140), &a[0], &a[1]);
-          codes4_to_f16<CODE>(__byte_perm(x2, x3, 0x5140), &a[2], &a[3]);
-          codes4_to_f16<CODE>(__byte_perm(x0, x1, 0x7362), &b[0], &b[1]);
-          codes4_to_f16<CODE>(__byte_perm(x2, x3, 0x7362), &b[2], &b[3]);
+          for (int jj = 0; jj < 4; ++jj) x[jj] = sm.ring[warp][4 * u + jj][lane];
+          uint2 qf[NT];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_f16(s[n][2 * wd], a[0], a[1], a[2], a[3], qf[n][ks][0], qf[n][ks][1]);
-            mma_f16(s[n][2 * wd + 1], b[0], b[1], b[2], b[3], qf[n][ks][0], qf[n][ks][1]);
+          for (int n = 0; n < NT; ++n) qf[n] = *reinterpret_cast<const uint2*>(&sm.q[n * 8 + g][ks * 16 + c * 4]);
+#pragma unroll
+          for (int wd = 0; wd < 4; ++wd) {
+            const uint32_t x0 = (&x[0].x)[wd], x1 = (&x[1].x)[wd], x2 = (&x[2].x)[wd], x3 = (&x[3].x)[wd];
+            uint32_t a[4], b[4];
+            // tokens 4 wd, 4 wd + 1 -> row pair (g, g + 8) of tile 2 wd
+            codes4_to_f16<CODE>(__byte_perm(x0, x1, 0x5140), &a[0], &a[1]);
+            codes4_to_f16<CODE>(__byte_perm(x2, x3, 0x5140), &a[2], &a[3]);
+            codes4_to_f16<CODE>(__byte_perm(x0, x1, 0x7362), &b[0], &b[1]);
+            codes4_to_f16<CODE>(__byte_perm(x2, x3, 0x7362), &b[2], &b[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma_f16(s[n][2 * wd], a[0], a[1], a[2], a[3], qf[n].x, qf[n].y);
+              mma_f16(s[n][2 * wd + 1], b[0], b[1], b[2], b[3], qf[n].x, qf[n].y);
+            }
           }
+          if (k0 + kRing < kSteps)
+            load_k(u, ks + kRing, kp, kn);
+          else
+            load_v(u, u / (kSteps / 2), u % (kSteps / 2));
+          copy_commit();
         }
-        // the slots just read take the V loads that will be the kSteps-th to be waited for from here
-        const int hf = ks / (kSteps / 2);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = 16 * (2 * (ks % (kSteps / 2)) + (e >> 1)) + 8 * (e & 1);
-          copy_async(ring + (4 * ks + e) * 512, vp[hf] + row * (vn[hf] ? bs : 0), vn[hf]);
-        }
-        copy_commit();
       }
       // s[n][i][2 * r + e]: token kt + 2 i + r, column 2 c + e
       const bool whole = tok >= all_lo && tok + kTile <= all_hi;
@@ -413,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
             for (int e = 0; e < 4; ++e) acc[n][i][e] *= keep[n][e & 1];
       }
       uint8_t* wrow = sm.weights[warp];
-#pragma unroll
+#pragma unroll 1
       for (int hf = 0; hf < 2; ++hf) {
         // weights of 64 tokens from the score layout to the operand layout
         if ((g >> 2) == hf) {
@@ -441,11 +457,12 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
         const int first = any_lo - vt, last = any_hi - vt;
 #pragma unroll
         for (int i2 = 0; i2 < kSteps / 2; ++i2) {
-          const int ks = hf * (kSteps / 2) + i2;
-          copy_wait<kSteps - 1>();
+          // HD 64 has two groups to a half: their slots go by the half
+          const int slot = kSteps / 2 >= kRing ? i2 % kRing : hf * (kSteps / 2) + i2;
+          copy_wait<kRing - 1>();
           uint4 x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = sm.ring[warp][4 * ks + e][lane];
+          for (int e = 0; e < 4; ++e) x[e] = sm.ring[warp][4 * slot + e][lane];
 #pragma unroll
           for (int i1 = 0; i1 < 2; ++i1) {
             const int i = 2 * i2 + i1;
@@ -467,14 +484,16 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
               for (int n = 0; n < NT; ++n) mma_f16(acc[n][i], a[0], a[1], a[2], a[3], pf[n][q4][0], pf[n][q4][1]);
             }
           }
-          if (more) {
-#pragma unroll
-            for (int jj = 0; jj < 4; ++jj) copy_async(ring + (4 * ks + jj) * 512, kp1 + (16 * ks + 4 * jj) * (kn1 ? bs : 0), kn1);
-          }
+          const int next = hf * (kSteps / 2) + i2 + kRing;  // group of V, or past the last one of the next tile's K
+          if (next < kSteps)
+            load_v(slot, next / (kSteps / 2), next % (kSteps / 2));
+          else if (more)
+            load_k(slot, next - kSteps, kp1, kn1);
           copy_commit();
         }
       }
       page = page1, page1 = page2;
+      kp = kp1, kn = kn1;
       ksc = ksc1, vsc = vsc1;
     }
     copy_wait<0>();
@@ -609,9 +628,14 @@ int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kThreads, kBytes) != cudaSuccess || n <= 0) n = 1;
     per_sm = n;
   }
-  int grid = per_sm * sm_count();
+  int64_t grid = per_sm * sm_count();
   if (grid > kMaxGrid) grid = kMaxGrid;
-  return launch_pdl("mak_block_attention", block_attn_rows_kernel<HD, NT, CODE>, dim3(grid), dim3(kThreads), kBytes, st, p);
+  // no more blocks than there can be work for: kWarps tiles each
+  const int64_t seq_tiles = ((static_cast<int64_t>(p.max_blocks) << p.bs_log2) + kTile - 1) / kTile + 1;
+  const int64_t groups = static_cast<int64_t>(p.num_rows) * p.group / (8 * NT) + p.num_seqs;
+  const int64_t most = (groups * p.nh * seq_tiles + kWarps - 1) / kWarps;
+  if (most < grid) grid = most;
+  return launch_pdl("mak_block_attention", block_attn_rows_kernel<HD, NT, CODE>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kBytes, st, p);
 }
 
 template <int HD, int NT>
