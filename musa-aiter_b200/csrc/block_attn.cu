@@ -3,59 +3,79 @@
 //
 // Mathematics.  With codes k, v and scales a, b per (block, head):
 //   S[t] = scale * a(t) * (q . k[t]),   o = sum_t 2^(S'[t] - m) b(t) v[t] / sum_t 2^(S'[t] - m)
-// with S' = S * log2(e) and the running maximum m.  The matrix instructions see
-// the codes themselves, exact in f16; a multiplies a finished product and b the
-// weight of a token, both in 32 bits, so a scale costs one multiplication per
-// token and not one per element.
+// with S' = S * log2(e).  The 8-bit tensor cores see the codes as they lie in the cache, so no
+// code is ever converted: what multiplies them is split into three 8-bit terms instead, and
+// there is little of that (a handful of rows of q, and their weights).
+//   E4M3: x = x1 + x2 / 16 + x3 / 256 ... with x1 = e4m3(x), x2 = e4m3(16 (x - x1)), ...: each term
+//     rounds off 2^-4 of what it is given, three leave 2^-12 of a value, or 2^-18 in all.
+//     A row of q is scaled to a maximum in [2^7, 2^8) (three terms), weights to at most 2^8 (four).
+//   int8: x = x1 2^16 + x2 2^8 + x3, a whole number in balanced base 256: q to a maximum in
+//     [2^21, 2^22), weights to 127 * 2^24 (four digits).  The products are summed exactly in s32.
+// So q (bf16: 8 bits, f16: 11) goes in exactly but for values below 2^-13 of its row's largest,
+// and a weight is good to 2^-12 of itself or 2^-30 of its tile's largest.  The fourth term is free:
+// 8 rows with three terms would be 24 columns, and the tensor cores want a multiple of 16.
+// Each 128-token tile has its own maximum, largest V scale and product with V; tiles are joined
+// in 32-bit registers, so the tensor cores' accumulators never need rescaling.
 //
-// q in f16: a row of bf16 is multiplied by a power of two that brings its
-// largest magnitude to [2^14, 2^15); values that fall out of f16's normal range
-// by that are below 2^-28 of the largest and err by at most 2^-39 of it.
-// Weights in f16: p * b(t) / b_max * 2^15, at most 2^15, rounded once (2^-12
-// relative); b_max is the largest scale met so far and rescales with m.  The
-// sum of the weights is taken in 32 bits before that rounding.
+// Layout.  Tokens are the M axis of the scores (A = K, MN-major: tokens contiguous) and head_dim
+// the M axis of the products (A = V, K-major: tokens contiguous again); the rows of q (heads that
+// share a cache head, times the rows of a sequence), term by term, are N.  A block of the
+// cache is a [head_dim][block_size] byte tile, which for block_size 16 is exactly the tensor
+// core's unswizzled operand layout (one contiguous bulk copy) and for 32 to 128 its 32- to
+// 128-byte swizzled one (one TMA box).
 //
-// Layout.  A warp takes 128 tokens at a time.  K is the A operand of
-// m16n8k16 with tokens as rows and V the A operand with head_dim as rows; the
-// rows of q (the heads that share a cache head, times the rows of a sequence)
-// are the 8 columns.  A lane's 16-byte load is 16 tokens of one head_dim row,
-// so neighbouring lanes cover 4 rows of K (8 of V) in full sectors, and since
-// the order of the contracted index is free as long as both operands agree, the
-// loaded bytes become fragments in place: no shared memory for K or V.
-//
-// Work.  All (sequence, head, row group) units laid end to end as 128-token
-// tiles are cut into equal runs, one per block, whatever the lengths; a block
-// finds its run from the lengths alone.  A unit cut by that leaves partial sums
-// (maximum, sum, accumulators) and the last block to arrive joins them.
+// Work.  All (sequence, head, row group) units laid end to end as 128-token tiles are cut into
+// equal runs, one per thread block, whatever the lengths; a block finds its run from the lengths
+// alone.  A unit cut by that leaves partial sums (maximum, sum, accumulators) and the last block
+// to arrive joins them.  Roles: warps 0-3 softmax (a thread per token, then per head_dim row),
+// warp 4 copies, warp 5 issues the tensor cores; two tiles are in flight between them.
+#include <cuda.h>
+
 #include "block_attn.cuh"
+#include "tcgen05.cuh"
 
 namespace mak {
 namespace {
 
-constexpr int kTile = 128;       // tokens per warp step
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxGrid = 148 * 8;  // blocks of the largest grid; the workspace has two partial sums for each
+constexpr int kTile = 128;  // tokens per step
+constexpr int kThreads = 192;
+constexpr int kSoft = 128;  // threads of the softmax warps
+constexpr int kMaxGrid = 148 * 4;  // blocks of the largest grid; the workspace has two partial sums for each
 constexpr int kMaxRows = 16;
 constexpr int kMaxDim = 256;
+constexpr int kMinChunk = 2;  // tiles per block that are worth another block
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
+template <int HD, int ROWS>
+struct Cfg {
+  static constexpr int kN = 4 * ROWS;              // columns of the products
+  static constexpr int kParts = HD == 256 ? 2 : 1; // 128-row parts of head_dim
+  static constexpr int kStages = HD == 64 ? 4 : HD == 128 && ROWS == 8 ? 3 : 2;
+  static constexpr int kTileBytes = HD * kTile;
+  static constexpr int kTmem = 2 * kN * (1 + kParts) <= 128 ? 128 : 2 * kN * (1 + kParts) <= 256 ? 256 : 512;
+};
 
-// Asynchronous 16-byte copy to shared memory; bytes = 0 stores zeros and reads nothing.
-__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
+template <int HD, int ROWS>
+struct Smem {
+  using C = Cfg<HD, ROWS>;
+  // V first: with head_dim 64 the products read 128 rows from it, the last 64 past a tile's end
+  alignas(1024) uint8_t v[C::kStages][C::kTileBytes];
+  alignas(1024) uint8_t k[C::kStages][C::kTileBytes];
+  alignas(1024) uint8_t p[2][C::kN * kTile];
+  uint8_t q[C::kN * HD];
+  alignas(16) float ks[8][8], vs[8][8];  // scales per 16 tokens, tile number mod 8
+  uint32_t have[8];                      // bit c: 16-token piece c has a block
+  alignas(16) float wmax[2][4][ROWS];
+  alignas(16) float row_scale[ROWS];
+  int row_lo[ROWS], row_hi[ROWS];
+  float lsum[4][ROWS];
+  alignas(8) uint64_t k_full[C::kStages], k_empty[C::kStages], v_full[C::kStages], v_empty[C::kStages];
+  uint64_t q_full, s_full[2], p_full[2], o_full[2], spare;
+  int64_t scan[4];
+  int64_t begin_base;
+  int begin_seq;
+  uint32_t tmem;
+  int gave_up, last;
+};
 
 // Tiles of a unit of sequence v (at least one, so that empty rows are written).
 __device__ __forceinline__ int unit_tiles(const SeqView& v) {
@@ -63,584 +83,734 @@ __device__ __forceinline__ int unit_tiles(const SeqView& v) {
   return t1 > t0 ? t1 - t0 : 1;
 }
 
-template <int NROWS>
+template <int ROWS>
 __device__ __forceinline__ int64_t seq_work(const BlockAttnParams& p, const SeqView& v) {
   if (v.rows == 0) return 0;
-  const int64_t groups = (static_cast<int64_t>(v.rows) * p.group + NROWS - 1) / NROWS;
+  const int64_t groups = (static_cast<int64_t>(v.rows) * p.group + ROWS - 1) / ROWS;
   return groups * p.nh * unit_tiles(v);
 }
 
-// Each lane's loads go through its own slots of a ring: the lane that copies 16 bytes
-// in is the one that reads them, so no barrier is needed, and the loads in flight cost
-// no registers.  Loads come in groups of 4 per lane, head_dim / 16 groups for K of a tile
-// and as many for V; each group that is consumed makes room for the one kRing further on,
-// so V follows K and K of the next tile follows V.  The loops are rolled as far as the
-// accumulators allow: unrolled whole, waiting for instructions cost more than the work.
-constexpr int kRing = 4;  // groups
-
-template <int HD, int NT>
-struct Smem {
-  static constexpr int kRows = 8 * NT;
-  static constexpr int kPStride = 64 * 2 + 16;  // bytes between rows of the weights of 64 tokens
-  union {
-    uint4 ring[kWarps][4 * kRing][32];
-    float acc[kWarps][kRows][HD + 1];
-  };
-  uint8_t weights[kWarps][kRows * kPStride];
-  alignas(16) __half q[kRows][HD + 16];
-  float m[kWarps][kRows];
-  float l[kWarps][kRows];
-  float qscale[kRows];
-  int64_t scan[kWarps];
-  int64_t begin_base;
-  int begin_seq;
-  int last;
+// A block's run of work, unit by unit; every warp walks it for itself.
+struct Walk {
+  int64_t w, w_end, base;
+  int seq;
+};
+struct Unit {
+  SeqView v;
+  int seq, head, row0, live;          // rows row0 .. row0 + live of the sequence (row i * group + j: row i, query head j)
+  int tiles, ta, tb;                  // of the unit's tiles this block has [ta, tb)
+  int t_first, t_last;                // absolute tiles of those that some row sees
+  int any_lo, any_hi, all_lo, all_hi; // tokens that some / all rows see
+  int64_t w0;
 };
 
-template <int HD, int NT, int CODE>
-__global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : NT == 1 ? 3 : 2)
-    block_attn_rows_kernel(const __grid_constant__ BlockAttnParams p) {
-  constexpr int kRows = 8 * NT;
-  constexpr int kSteps = HD / 16;  // groups of 4 loads of one lane per tile of K (and of V)
-  extern __shared__ __align__(16) uint8_t raw[];
-  Smem<HD, NT>& sm = *reinterpret_cast<Smem<HD, NT>*>(raw);
+template <int ROWS>
+__device__ __forceinline__ bool next_unit(const BlockAttnParams& p, Walk& k, Unit& u) {
+  if (k.w >= k.w_end) return false;
+  SeqView v = seq_view(p, k.seq);
+  int64_t sw = seq_work<ROWS>(p, v);
+  while (k.w >= k.base + sw) {
+    k.base += sw;
+    v = seq_view(p, ++k.seq);
+    sw = seq_work<ROWS>(p, v);
+  }
+  u.v = v;
+  u.seq = k.seq;
+  u.tiles = unit_tiles(v);
+  const int64_t rel = k.w - k.base;
+  const int64_t unit = (rel >> 31) == 0 ? static_cast<uint32_t>(rel) / static_cast<uint32_t>(u.tiles) : rel / u.tiles;
+  u.w0 = k.base + unit * u.tiles;
+  u.ta = static_cast<int>(k.w - u.w0);
+  u.tb = static_cast<int>(min(k.w_end - u.w0, static_cast<int64_t>(u.tiles)));
+  const int rows_total = v.rows * p.group;
+  const uint32_t groups = (rows_total + ROWS - 1) / ROWS;
+  u.head = static_cast<int>(static_cast<uint32_t>(unit) / groups);
+  u.row0 = static_cast<int>(static_cast<uint32_t>(unit) % groups) * ROWS;
+  u.live = min(ROWS, rows_total - u.row0);
+  int lo1, hi0;
+  row_range(p, v, u.row0 / p.group, &u.any_lo, &hi0);
+  row_range(p, v, (u.row0 + u.live - 1) / p.group, &lo1, &u.any_hi);
+  u.all_lo = lo1;
+  u.all_hi = hi0;
+  const int tile0 = v.hi > v.lo ? v.lo / kTile : 0;
+  u.t_first = u.t_last = 0;
+  if (u.any_hi > u.any_lo) {
+    u.t_first = max(tile0 + u.ta, u.any_lo / kTile);
+    u.t_last = max(u.t_first, min(tile0 + u.tb, (u.any_hi + kTile - 1) / kTile));
+  }
+  k.w = u.w0 + u.tb;
+  return true;
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Two values (E4M3: at most 448) to their terms, low byte of t[i] the first value's.
+template <int TERMS>
+__device__ __forceinline__ void split_e4m3(float x, float y, uint32_t (&t)[TERMS]) {
+#pragma unroll
+  for (int i = 0; i < TERMS; ++i) {
+    uint16_t b;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(y), "f"(x));
+    t[i] = b;
+    if (i + 1 < TERMS) {
+      uint32_t h;
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(b));
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      x = (x - f.x) * 16.f;
+      y = (y - f.y) * 16.f;
+    }
+  }
+}
+// Whole number below 127.4 * 2^24 to its balanced base-256 digits, highest in byte 3.
+__device__ __forceinline__ uint32_t split_int8(float x) {
+  return (static_cast<uint32_t>(__float2int_rn(x)) + 0x808080u) ^ 0x808080u;
+}
+
+// The terms' products to their sum: in units of the last digit (int8) or of the first term (E4M3).
+template <int CODE, int TERMS>
+__device__ __forceinline__ float join_terms(const uint32_t (&t)[TERMS]) {
+  float x = 0.f;
+  if constexpr (CODE == MAK_CODE_INT8) {
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) x = fmaf(x, 256.f, static_cast<float>(static_cast<int>(t[i])));
+  } else {
+#pragma unroll
+    for (int i = TERMS - 1; i >= 0; --i) x = fmaf(x, 1.f / 16.f, __uint_as_float(t[i]));
+  }
+  return x;
+}
+
+template <int HD, int ROWS, int CODE>
+__global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
+    block_attn_rows_kernel(const __grid_constant__ BlockAttnParams p, const __grid_constant__ CUtensorMap kmap,
+                           const __grid_constant__ CUtensorMap vmap) {
+  using C = Cfg<HD, ROWS>;
+  constexpr int kST = C::kStages;
+  extern __shared__ uint8_t raw[];
+  Smem<HD, ROWS>& sm = *reinterpret_cast<Smem<HD, ROWS>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, c = lane & 3;
   pdl_wait();
   pdl_trigger();
 
   // ---- the run of this block ------------------------------------------------
-  const int per = (p.num_seqs + kThreads - 1) / kThreads;
-  const int s0 = min(tid * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
-  int64_t mine = 0;
-  for (int s = s0; s < s1; ++s) mine += seq_work<kRows>(p, seq_view(p, s));
-  int64_t incl = mine;
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 31) sm.scan[warp] = incl;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) incl += sm.scan[w];
-    total += sm.scan[w];
-  }
-  int64_t chunk = (total + gridDim.x - 1) / gridDim.x;
-  if (chunk < kWarps) chunk = kWarps;  // a tile for each warp before another block joins
-  const int64_t w_begin = blockIdx.x * chunk;
-  const int64_t w_end = min(w_begin + chunk, total);
-  if (w_begin >= w_end) return;
-  if (incl - mine <= w_begin && w_begin < incl) {
-    int64_t base = incl - mine;
-    for (int s = s0; s < s1; ++s) {
-      const int64_t w = seq_work<kRows>(p, seq_view(p, s));
-      if (w_begin < base + w) {
-        sm.begin_seq = s;
-        sm.begin_base = base;
-        break;
+  Walk walk;
+  int64_t chunk;
+  {
+    const int per = (p.num_seqs + kSoft - 1) / kSoft;
+    const int s0 = min(tid * per, p.num_seqs), s1 = warp < 4 ? min(s0 + per, p.num_seqs) : s0;
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) mine += seq_work<ROWS>(p, seq_view(p, s));
+    int64_t incl = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31 && warp < 4) sm.scan[warp] = incl;
+    if (tid == kSoft) {
+      sm.gave_up = 0;
+      for (int i = 0; i < kST; ++i) {
+        mbar_init(&sm.k_full[i], 1);
+        mbar_init(&sm.k_empty[i], 1);
+        mbar_init(&sm.v_full[i], 1);
+        mbar_init(&sm.v_empty[i], 1);
       }
-      base += w;
+      mbar_init(&sm.q_full, 4);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.s_full[i], 1);
+        mbar_init(&sm.p_full[i], 4);
+        mbar_init(&sm.o_full[i], 1);
+      }
+      mbar_init(&sm.spare, 1);
+      mbar_init_fence();
+    }
+    __syncthreads();
+    int64_t total = 0;
+    for (int x = 0; x < 4; ++x) {
+      if (x < warp) incl += sm.scan[x];
+      total += sm.scan[x];
+    }
+    chunk = (total >> 31) == 0 ? (static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x : (total + gridDim.x - 1) / gridDim.x;
+    if (chunk < kMinChunk) chunk = kMinChunk;
+    walk.w = blockIdx.x * chunk;
+    walk.w_end = min(walk.w + chunk, total);
+    if (walk.w >= walk.w_end) return;
+    if (warp < 4 && incl - mine <= walk.w && walk.w < incl) {
+      int64_t base = incl - mine;
+      for (int s = s0; s < s1; ++s) {
+        const int64_t w = seq_work<ROWS>(p, seq_view(p, s));
+        if (walk.w < base + w) {
+          sm.begin_seq = s;
+          sm.begin_base = base;
+          break;
+        }
+        base += w;
+      }
     }
   }
+  if (warp == 5) tmem_alloc<C::kTmem>(&sm.tmem);
+  // q has no fourth term
+  for (int i = tid; i < ROWS * HD / 4; i += kThreads) reinterpret_cast<uint32_t*>(sm.q + 3 * ROWS * HD)[i] = 0;
+  fence_async_shared();
+  tc_fence_before();
   __syncthreads();
-  int seq = sm.begin_seq;
-  int64_t base = sm.begin_base;
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  walk.seq = sm.begin_seq;
+  walk.base = sm.begin_base;
+  const int64_t w_begin = walk.w;
+  volatile int* gave_up = &sm.gave_up;
+  const int bs = 1 << p.bs_log2;
+  Unit u;
 
-  int64_t w = w_begin;
-  while (w < w_end) {
-    SeqView v = seq_view(p, seq);
-    int64_t sw = seq_work<kRows>(p, v);
-    while (w >= base + sw) {
-      base += sw;
-      v = seq_view(p, ++seq);
-      sw = seq_work<kRows>(p, v);
-    }
-    const int tiles = unit_tiles(v);
-    const int64_t unit = (w - base) / tiles;
-    const int64_t unit_w0 = base + unit * tiles;
-    const int ta = static_cast<int>(w - unit_w0);
-    const int tb = static_cast<int>(min(w_end - unit_w0, static_cast<int64_t>(tiles)));
-    const int rows_total = v.rows * p.group;
-    const int groups = (rows_total + kRows - 1) / kRows;
-    const int head = static_cast<int>(unit / groups);
-    const int row0 = static_cast<int>(unit % groups) * kRows;  // row i * group + j: row i, query head j of the group
-
-    // ---- q rows: f16, contracted index in fragment order ---------------------
-    __syncthreads();  // the last unit's readers are done
-    {
-      constexpr int kLanes = HD / 8;            // lanes of one row
-      constexpr int kPass = kThreads / kLanes;  // rows at once
-      const int part = tid % kLanes;
+  if (warp < 4) {
+    // ---- softmax ----------------------------------------------------------------
+    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+    const int piece = tid >> 4;  // 16-token piece of this thread's token
+    uint32_t it = 0;
+    bool ok = true;
+    while (next_unit<ROWS>(p, walk, u)) {
+      const int n = u.t_last - u.t_first;
+      if (n > 0) {
+        // rows of q: three 8-bit terms each; a row's threads are neighbours
+        constexpr int kPer = HD * ROWS / kSoft;  // values of a thread
+        constexpr int kRowThreads = kSoft / ROWS;
+        const int r = tid / kRowThreads, d0 = tid % kRowThreads * kPer;
+        uint32_t w[kPer / 2];
 #pragma unroll
-      for (int r0 = 0; r0 < kRows; r0 += kPass) {
-        const int r = r0 + tid / kLanes;
-        const bool on = r < kRows && row0 + r < rows_total;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (on) {
-          const int i = (row0 + r) / p.group, j = (row0 + r) % p.group;
-          raw = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (v.first + i) * p.q_sr +
-                                                     (head * p.group + j) * p.q_sh + part * 8));
+        for (int e = 0; e < kPer / 2; ++e) w[e] = 0;
+        const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) % p.group;
+        if (r < u.live) {
+          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (u.v.first + i) * p.q_sr + j * p.q_sh + d0;
+#pragma unroll
+          for (int e = 0; e < kPer / 4; ++e) {
+            const uint2 x = __ldg(reinterpret_cast<const uint2*>(src) + e);
+            w[2 * e] = x.x, w[2 * e + 1] = x.y;
+          }
         }
-        float x[8];
-        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-        float top = 0.f;
+        float x[kPer], top = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < kPer / 2; ++e) {
           if (p.q_bf16) {
-            x[2 * e] = __uint_as_float(words[e] << 16);
-            x[2 * e + 1] = __uint_as_float(words[e] & 0xffff0000u);
+            x[2 * e] = __uint_as_float(w[e] << 16);
+            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
           } else {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[e]));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
             x[2 * e] = f.x;
             x[2 * e + 1] = f.y;
           }
           top = fmaxf(top, fmaxf(fabsf(x[2 * e]), fabsf(x[2 * e + 1])));
+          if (x[2 * e] != x[2 * e] || x[2 * e + 1] != x[2 * e + 1]) top = INFINITY;
         }
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        // 2^up brings top to [2^14, 2^15); bf16 only, f16 is taken as it is
-        int up = 0;
-        if (p.q_bf16 && top > 0.f && top < __uint_as_float(0x7f800000u)) up = 14 - (ilogbf(top));
+        for (int o = kRowThreads / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        constexpr int kTop = CODE == MAK_CODE_INT8 ? 21 : 7;
+        const int up = top > 0.f && top < INFINITY ? kTop - ilogbf(top) : 0;
         const int up1 = up / 2, up2 = up - up1;  // two steps: 2^up itself may leave the exponent range
         const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up1) << 23);
         const float f2 = __uint_as_float(static_cast<uint32_t>(127 + up2) << 23);
-        if (r < kRows) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            // d = 16 ks + 4 jj + cc sits at 16 ks + 4 cc + jj
-            const int d = part * 8 + e;
-            sm.q[r][(d & ~15) + (d & 3) * 4 + ((d >> 2) & 3)] = __float2half_rn(x[e] * f1 * f2);
+        for (int e = 0; e < kPer; e += 4) {
+          float y[4];
+#pragma unroll
+          for (int b = 0; b < 4; ++b) y[b] = x[e + b] * f1 * f2;
+          uint32_t t[3];
+          if constexpr (CODE == MAK_CODE_INT8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) v[b] = split_int8(y[b]);
+#pragma unroll
+            for (int z = 0; z < 3; ++z) {
+              const uint32_t pick = (2 - z) | ((6 - z) << 4);  // byte 2 - z of both
+              t[z] = __byte_perm(__byte_perm(v[0], v[1], pick), __byte_perm(v[2], v[3], pick), 0x5410);
+            }
+          } else {
+            uint32_t a[3], b[3];
+            split_e4m3(y[0], y[1], a);
+            split_e4m3(y[2], y[3], b);
+#pragma unroll
+            for (int z = 0; z < 3; ++z) t[z] = a[z] | (b[z] << 16);
           }
-          if (part == 0) sm.qscale[r] = ldexpf(p.scale_log2, -up);
+#pragma unroll
+          for (int z = 0; z < 3; ++z) {
+            const int col = z * ROWS + r, d = d0 + e;
+            *reinterpret_cast<uint32_t*>(sm.q + (col >> 3) * (HD * 8) + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = t[z];
+          }
         }
+        if (d0 == 0) {
+          sm.row_scale[r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
+          int lo = 0, hi = 0;
+          if (r < u.live) row_range(p, u.v, i, &lo, &hi);
+          sm.row_lo[r] = lo;
+          sm.row_hi[r] = hi;
+        }
+        fence_async_shared();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full);
+        soft_sync();
       }
-    }
-    __syncthreads();
-    float qs[NT][2];
-    int lo[NT][2], hi[NT][2];
-    int all_lo = 0, all_hi = 0x7fffffff, any_lo = 0x7fffffff, any_hi = 0;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = n * 8 + 2 * c + e;
-        qs[n][e] = sm.qscale[r];
-        lo[n][e] = hi[n][e] = 0;
-        if (row0 + r < rows_total) row_range(p, v, (row0 + r) / p.group, &lo[n][e], &hi[n][e]);
-      }
-    }
-    {  // tokens that all rows of the group see, and that any sees
-      const int i0 = row0 / p.group, i1 = min(row0 + kRows, rows_total) - 1;
-      int l0, h0, l1, h1;
-      row_range(p, v, i0, &l0, &h0);
-      row_range(p, v, i1 / p.group, &l1, &h1);
-      all_lo = l1;
-      all_hi = h0;
-      any_lo = l0;
-      any_hi = h1;
-    }
 
-    float acc[NT][HD / 16][4];
-    float m[NT][2], l[NT][2];
+      float acc[C::kParts][ROWS], m[ROWS], l[ROWS], keep[ROWS], gain[ROWS];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int r = 0; r < ROWS; ++r) {
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[n][i][e] = 0.f;
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
-    }
-    float vref = 0.f;
-    const int32_t* table = p.tables + seq * p.table_stride;
-    const uint8_t* kbase = p.key + head * p.k_sh;
-    const uint8_t* vbase = p.value + head * p.v_sh;
-    const int bs = 1 << p.bs_log2;
-    const int tile0 = v.hi > v.lo ? v.lo / kTile : 0;
-    // tiles of this warp: t, t + kWarps, ... below t_end, all of which some row sees
-    int t = ta + warp, t_end = tb;
-    if (any_hi > any_lo) {
-      t_end = min(t_end, (any_hi + kTile - 1) / kTile - tile0);
-      const int skip = any_lo / kTile - tile0 - t;
-      if (skip > 0) t += (skip + kWarps - 1) / kWarps * kWarps;
-    } else {
-      t_end = 0;
-    }
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(&sm.ring[warp][0][lane]));
-    // Block of this lane's 16 tokens of K (chunk g) of tile i, -1 where there is none.
-    auto find = [&](int i) {
-      const int kt = (tile0 + i) * kTile + 16 * g;
-      int page = -1;
-      if (i < t_end && kt < any_hi && kt + 16 > any_lo) page = __ldg(table + (kt >> p.bs_log2));
-      return page >= p.num_blocks ? -1 : page;
-    };
-    int page = find(t), page1 = find(t + kWarps);
-    float ksc = 0.f, vsc = 0.f;
-    auto scales = [&](int pg, float* a, float* b) {
-      *a = *b = 0.f;
-      if (pg >= 0) {
-        *a = __ldg(p.key_scale + pg * p.ks_sb + head * p.ks_sh);
-        *b = __ldg(p.value_scale + pg * p.vs_sb + head * p.vs_sh);
+        for (int h = 0; h < C::kParts; ++h) acc[h][r] = 0.f;
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        keep[r] = gain[r] = 0.f;
       }
-    };
-    const int in_block = (16 * g) & (bs - 1);  // a tile starts at a block's start
-    const uint8_t* kp = page >= 0 ? kbase + page * p.k_sb + in_block + c * bs : kbase;
-    uint32_t kn = page >= 0 ? 16 : 0;
-    // group i of K: rows 16 i + 4 jj + c of this lane's chunk
-    auto load_k = [&](int slot, int i, const uint8_t* from, uint32_t bytes) {
-      const uint8_t* at = from + (bytes ? 16 * i * bs : 0);
-      const int step = bytes ? 4 * bs : 0;
+      // the product with V of tile x joins the sums
+      auto collect = [&](uint32_t x) {
+        if (!mbar_wait_warp(&sm.o_full[x & 1], (x >> 1) & 1, gave_up)) return false;
+        if (HD == 64 && warp >= 2) return true;
+        tc_fence_after();
 #pragma unroll
-      for (int jj = 0; jj < 4; ++jj) copy_async(ring + (4 * slot + jj) * 512, at + jj * step, bytes);
-    };
-    if (t < t_end) {
+        for (int h = 0; h < C::kParts; ++h) {
+          uint32_t o[4][ROWS];
+          const uint32_t at = tmem + lanes + 2 * C::kN + (2 * h + (x & 1)) * C::kN;
 #pragma unroll
-      for (int i = 0; i < kRing; ++i) {
-        load_k(i, i, kp, kn);
-        copy_commit();
-      }
-      scales(page, &ksc, &vsc);
-    }
-
-    for (; t < t_end; t += kWarps) {
-      const int tok = (tile0 + t) * kTile;
-      const int kt = tok + 16 * g;
-      // V of this tile: chunk 4 hf + c
-      const uint8_t* vp[2];
-      uint32_t vn[2];
+          for (int z = 0; z < 4; ++z) tmem_ld(at + z * ROWS, o[z]);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int vpage = __shfl_sync(0xffffffffu, page, (4 * hf + c) * 4);
-        vn[hf] = vpage >= 0 ? 16 : 0;
-        vp[hf] = vpage >= 0 ? vbase + vpage * p.v_sb + ((64 * hf + 16 * c) & (bs - 1)) + g * bs : vbase;
-      }
-      // the next tile
-      const int page2 = find(t + 2 * kWarps);
-      const bool more = t + kWarps < t_end;
-      const uint8_t* kp1 = page1 >= 0 ? kbase + page1 * p.k_sb + in_block + c * bs : kbase;
-      const uint32_t kn1 = page1 >= 0 ? 16 : 0;
-      float ksc1, vsc1;
-      scales(page1, &ksc1, &vsc1);
-
-      float s[NT][8][4];
+          for (int z = 0; z < 4; ++z) tmem_wait(o[z]);
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][i][e] = 0.f;
-      // group i of V: rows 32 pair + 8 e + g of chunk 4 hf + c
-      auto load_v = [&](int slot, int hf, int pair) {
-        const uint8_t* at = hf ? vp[1] : vp[0];
-        const uint32_t bytes = hf ? vn[1] : vn[0];
-        const int step = bytes ? 8 * bs : 0;
-        at += 4 * pair * step;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) copy_async(ring + (4 * slot + e) * 512, at + e * step, bytes);
+          for (int r = 0; r < ROWS; ++r) {
+            const uint32_t t[4] = {o[0][r], o[1][r], o[2][r], o[3][r]};
+            acc[h][r] = acc[h][r] * keep[r] + join_terms<CODE>(t) * gain[r];
+          }
+        }
+        return true;
       };
-#pragma unroll 1
-      for (int k0 = 0; k0 < kSteps; k0 += kRing) {
+      // A warp that gave up goes through the same barriers as the others, without waiting for anything else.
+      for (int t = 0; t < n; ++t) {
+        const uint32_t x = it + t;
+        ok = ok && mbar_wait_warp(&sm.s_full[x & 1], (x >> 1) & 1, gave_up);
+        tc_fence_after();
+        float s[ROWS];
+        {
+          uint32_t o[3][ROWS];
+          const uint32_t at = tmem + lanes + (x & 1) * C::kN;
 #pragma unroll
-        for (int u = 0; u < kRing; ++u) {
-          const int ks = k0 + u;
-          copy_wait<kRing - 1>();
-          uint4 x[4];
+          for (int z = 0; z < 3; ++z) tmem_ld(at + z * ROWS, o[z]);
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) x[jj] = sm.ring[warp][4 * u + jj][lane];
-          uint2 qf[NT];
+          for (int z = 0; z < 3; ++z) tmem_wait(o[z]);
+          const float ks = sm.ks[x & 7][piece];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) qf[n] = *reinterpret_cast<const uint2*>(&sm.q[n * 8 + g][ks * 16 + c * 4]);
-#pragma unroll
-          for (int wd = 0; wd < 4; ++wd) {
-            const uint32_t x0 = (&x[0].x)[wd], x1 = (&x[1].x)[wd], x2 = (&x[2].x)[wd], x3 = (&x[3].x)[wd];
-            uint32_t a[4], b[4];
-            // tokens 4 wd, 4 wd + 1 -> row pair (g, g + 8) of tile 2 wd
-            codes4_to_f16<CODE>(__byte_perm(x0, x1, 0x5140), &a[0], &a[1]);
-            codes4_to_f16<CODE>(__byte_perm(x2, x3, 0x5140), &a[2], &a[3]);
-            codes4_to_f16<CODE>(__byte_perm(x0, x1, 0x7362), &b[0], &b[1]);
-            codes4_to_f16<CODE>(__byte_perm(x2, x3, 0x7362), &b[2], &b[3]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              mma_f16(s[n][2 * wd], a[0], a[1], a[2], a[3], qf[n].x, qf[n].y);
-              mma_f16(s[n][2 * wd + 1], b[0], b[1], b[2], b[3], qf[n].x, qf[n].y);
-            }
-          }
-          if (k0 + kRing < kSteps)
-            load_k(u, ks + kRing, kp, kn);
-          else
-            load_v(u, u / (kSteps / 2), u % (kSteps / 2));
-          copy_commit();
-        }
-      }
-      // s[n][i][2 * r + e]: token kt + 2 i + r, column 2 c + e
-      const bool whole = tok >= all_lo && tok + kTile <= all_hi;
-      float vmax = fabsf(vsc);
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-      const float vnew = fmaxf(vref, vmax);
-      const float vkeep = vnew > vref ? vref / vnew : 1.f;
-      const float vfac = vnew > 0.f ? vsc / vnew * 32768.f : 0.f;
-      vref = vnew;
-      bool moved = false;
-      float keep[NT][2];
-      uint32_t wt[NT][2][8];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float f[2] = {qs[n][0] * ksc, qs[n][1] * ksc};
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = s[n][i][e] * f[e & 1];
-            if (!whole || page < 0) {
-              const int at = kt + 2 * i + (e >> 1);
-              if (page < 0 || at < lo[n][e & 1] || at >= hi[n][e & 1]) x = -INFINITY;
-            }
-            s[n][i][e] = x;
-            top[e & 1] = fmaxf(top[e & 1], x);
-          }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
-          const float mn = fmaxf(m[n][e], top[e]);
-          const float ms = mn == -INFINITY ? 0.f : mn;
-          keep[n][e] = exp2_fast(m[n][e] - ms);
-          l[n][e] *= keep[n][e];
-          keep[n][e] *= vkeep;
-          moved |= keep[n][e] != 1.f;
-          m[n][e] = mn;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float w0 = exp2_fast(s[n][i][e] - ms), w1 = exp2_fast(s[n][i][2 + e] - ms);
-            l[n][e] += w0 + w1;
-            wt[n][e][i] = pack_f16(w0 * vfac, w1 * vfac);
+          for (int r = 0; r < ROWS; ++r) {
+            const uint32_t t[3] = {o[0][r], o[1][r], o[2][r]};
+            s[r] = join_terms<CODE>(t) * (sm.row_scale[r] * ks);
           }
         }
-      }
-      if (__any_sync(0xffffffffu, moved)) {
+        const int tok0 = (u.t_first + t) * kTile;
+        const uint32_t have = sm.have[x & 7];
+        if (tok0 < u.all_lo || tok0 + kTile > u.all_hi || have != 0xffu) {
+          const bool there = (have >> piece) & 1;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int r = 0; r < ROWS; ++r)
+            if (!there || tok0 + tid < sm.row_lo[r] || tok0 + tid >= sm.row_hi[r]) s[r] = -INFINITY;
+        }
+        float top[ROWS];
 #pragma unroll
-          for (int i = 0; i < HD / 16; ++i)
+        for (int r = 0; r < ROWS; ++r) top[r] = warp_max(s[r]);
+        if (lane == 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][i][e] *= keep[n][e & 1];
-      }
-      uint8_t* wrow = sm.weights[warp];
-#pragma unroll 1
-      for (int hf = 0; hf < 2; ++hf) {
-        // weights of 64 tokens from the score layout to the operand layout
-        if ((g >> 2) == hf) {
+          for (int r = 0; r < ROWS; r += 4)
+            *reinterpret_cast<float4*>(&sm.wmax[x & 1][warp][r]) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
+        }
+        soft_sync();
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int r = 0; r < ROWS; r += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(&sm.wmax[x & 1][w][r]);
+            top[r] = fmaxf(top[r], o.x);
+            top[r + 1] = fmaxf(top[r + 1], o.y);
+            top[r + 2] = fmaxf(top[r + 2], o.z);
+            top[r + 3] = fmaxf(top[r + 3], o.w);
+          }
+        const float vs = sm.vs[x & 7][piece];
+        float vtop = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) vtop = fmaxf(vtop, fabsf(sm.vs[x & 7][c]));
+        constexpr float kFull = CODE == MAK_CODE_INT8 ? 127.f * 16777216.f : 256.f;
+        const float weight = vtop > 0.f ? vs / vtop * kFull : 0.f;
+        // the tile before this one, whose factors are still in keep / gain
+        if (t > 0) ok = ok && collect(x - 1);
+        uint8_t* dst = sm.p[x & 1] + piece * 128 + (tid & 15);
+#pragma unroll
+        for (int r = 0; r < ROWS; r += 2) {
+          float y[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mt = top[r + e], mn = fmaxf(m[r + e], mt);
+            const float ms = mn == -INFINITY ? 0.f : mn;
+            const float old = exp2_fast(m[r + e] - ms), add = exp2_fast(mt - ms);
+            const float w = exp2_fast(s[r + e] - (mt == -INFINITY ? 0.f : mt));
+            l[r + e] = l[r + e] * old + w * add;
+            keep[r + e] = old;
+            gain[r + e] = add * vtop * (1.f / kFull);
+            m[r + e] = mn;
+            y[e] = w * weight;
+          }
+          if constexpr (CODE == MAK_CODE_INT8) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              uint4* dst = reinterpret_cast<uint4*>(wrow + (n * 8 + 2 * c + e) * Smem<HD, NT>::kPStride + (g & 3) * 32);
-              dst[0] = make_uint4(wt[n][e][0], wt[n][e][1], wt[n][e][2], wt[n][e][3]);
-              dst[1] = make_uint4(wt[n][e][4], wt[n][e][5], wt[n][e][6], wt[n][e][7]);
-            }
-        }
-        __syncwarp();
-        uint32_t pf[NT][4][2];
+              const uint32_t v = split_int8(y[e]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint4* src = reinterpret_cast<const uint4*>(wrow + (n * 8 + g) * Smem<HD, NT>::kPStride + c * 32);
-          const uint4 a = src[0], b = src[1];
-          pf[n][0][0] = a.x, pf[n][0][1] = a.y, pf[n][1][0] = a.z, pf[n][1][1] = a.w;
-          pf[n][2][0] = b.x, pf[n][2][1] = b.y, pf[n][3][0] = b.z, pf[n][3][1] = b.w;
-        }
-        __syncwarp();
-        // tokens of this chunk that some row sees; the others' codes may be anything and count as 0
-        const int vt = tok + 64 * hf + 16 * c;
-        const int first = any_lo - vt, last = any_hi - vt;
-#pragma unroll
-        for (int i2 = 0; i2 < kSteps / 2; ++i2) {
-          // HD 64 has two groups to a half: their slots go by the half
-          const int slot = kSteps / 2 >= kRing ? i2 % kRing : hf * (kSteps / 2) + i2;
-          copy_wait<kRing - 1>();
-          uint4 x[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = sm.ring[warp][4 * slot + e][lane];
-#pragma unroll
-          for (int i1 = 0; i1 < 2; ++i1) {
-            const int i = 2 * i2 + i1;
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              uint32_t y0 = (&x[2 * i1].x)[q4], y1 = (&x[2 * i1 + 1].x)[q4];
-              if (!whole) {
-                uint32_t mask = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                  if (4 * q4 + b >= first && 4 * q4 + b < last) mask |= 0xffu << (8 * b);
-                y0 &= mask;
-                y1 &= mask;
+              for (int z = 0; z < 4; ++z) {
+                const int col = z * ROWS + r + e;
+                dst[(col >> 3) * 1024 + (col & 7) * 16] = static_cast<uint8_t>(v >> (8 * (3 - z)));
               }
-              uint32_t a[4];
-              codes4_to_f16<CODE>(y0, &a[0], &a[2]);
-              codes4_to_f16<CODE>(y1, &a[1], &a[3]);
+            }
+          } else {
+            uint32_t v[4];
+            split_e4m3(y[0], y[1], v);
 #pragma unroll
-              for (int n = 0; n < NT; ++n) mma_f16(acc[n][i], a[0], a[1], a[2], a[3], pf[n][q4][0], pf[n][q4][1]);
+            for (int z = 0; z < 4; ++z) {
+              const int col = z * ROWS + r;
+              dst[(col >> 3) * 1024 + (col & 7) * 16] = static_cast<uint8_t>(v[z]);
+              dst[((col + 1) >> 3) * 1024 + ((col + 1) & 7) * 16] = static_cast<uint8_t>(v[z] >> 8);
             }
           }
-          const int next = hf * (kSteps / 2) + i2 + kRing;  // group of V, or past the last one of the next tile's K
-          if (next < kSteps)
-            load_v(slot, next / (kSteps / 2), next % (kSteps / 2));
-          else if (more)
-            load_k(slot, next - kSteps, kp1, kn1);
-          copy_commit();
         }
+        // E4M3: codes that no row sees may be NaN, which a weight of zero does not cancel
+        if (CODE == MAK_CODE_E4M3 && (tok0 < u.any_lo || tok0 + kTile > u.any_hi || have != 0xffu)) {
+          const uint32_t slot = x % kST;
+          ok = ok && mbar_wait_warp(&sm.v_full[slot], (x / kST) & 1, gave_up);
+          for (int d = tid; d < HD; d += kSoft)
+            for (int c = 0; c < 8; ++c) {
+              const int ct = tok0 + 16 * c;
+              const bool there = (have >> c) & 1;
+              if (there && ct >= u.any_lo && ct + 16 <= u.any_hi) continue;
+              const int per_line = bs >> 4;  // 16-byte pieces of a line
+              const int swz = p.bs_log2 == 7 ? d & 7 : p.bs_log2 == 6 ? (d >> 1) & 3 : p.bs_log2 == 5 ? (d >> 2) & 1 : 0;
+              uint4* at = reinterpret_cast<uint4*>(sm.v[slot] + (c / per_line) * (HD * bs) + d * bs + (((c % per_line) ^ swz) << 4));
+              uint4 v = *at;
+              uint32_t* words = &v.x;
+#pragma unroll
+              for (int b = 0; b < 4; ++b) {
+                uint32_t mask = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (there && ct + 4 * b + e >= u.any_lo && ct + 4 * b + e < u.any_hi) mask |= 0xffu << (8 * e);
+                words[b] &= mask;
+              }
+              *at = v;
+            }
+        }
+        fence_async_shared();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[x & 1]);
       }
-      page = page1, page1 = page2;
-      kp = kp1, kn = kn1;
-      ksc = ksc1, vsc = vsc1;
-    }
-    copy_wait<0>();
+      if (ok && n > 0) ok = collect(it + n - 1);
+      it += n;
 
-    // ---- join the warps --------------------------------------------------------
+      // ---- this block's share of the unit -----------------------------------------
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
-    __syncthreads();  // the ring is read, its space takes the accumulators
-    const float unit_scale = vref * (1.f / 32768.f);
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          sm.acc[warp][n * 8 + 2 * c + (e & 1)][16 * i + g + 8 * (e >> 1)] = acc[n][i][e] * unit_scale;
-      if (g == 0) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          sm.m[warp][n * 8 + 2 * c + e] = m[n][e];
-          sm.l[warp][n * 8 + 2 * c + e] = l[n][e];
+      for (int r = 0; r < ROWS; ++r) {
+        if (!ok) {  // a block that gave up leaves NaN, not stale memory
+          l[r] = __uint_as_float(0x7fffffffu);
+          m[r] = 0.f;
         }
-      }
-    }
-    __syncthreads();
-    const bool single = ta == 0 && tb == tiles;
-    const int first_block = static_cast<int>(unit_w0 / chunk);
-    const int last_block = static_cast<int>((unit_w0 + tiles - 1) / chunk);
-    const int live = min(kRows, rows_total - row0);
-    constexpr int kStep = kRows * (HD + 2);  // floats of one partial sum
-    float* part = nullptr;
-    if (!single) part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (unit_w0 > w_begin ? 1 : 0)) * kStep;
-    for (int idx = tid; idx < live * HD; idx += kThreads) {
-      const int r = idx / HD, d = idx % HD;
-      float mx = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) mx = fmaxf(mx, sm.m[x][r]);
-      const float ms = mx == -INFINITY ? 0.f : mx;
-      float o = 0.f, sum = 0.f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) {
-        const float k = exp2_fast(sm.m[x][r] - ms);
-        o += k * sm.acc[x][r][d];
-        sum += k * sm.l[x][r];
+        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+        if (lane == 0) sm.lsum[warp][r] = l[r];
       }
-      if (single) {
-        const int i = (row0 + r) / p.group, j = head * p.group + (row0 + r) % p.group;
-        const float y = sum > 0.f || sum != sum ? o / sum : 0.f;
-        const int64_t at = (v.first + i) * p.o_sr + j * p.o_sh + d;
+      soft_sync();
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) l[r] = sm.lsum[0][r] + sm.lsum[1][r] + sm.lsum[2][r] + sm.lsum[3][r];
+      auto put = [&](int r, int d, float y) {
+        const int row = u.row0 + r;
+        const int64_t at = (u.v.first + row / p.group) * p.o_sr + (u.head * p.group + row % p.group) * p.o_sh + d;
         if (p.q_bf16)
           reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
         else
           reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(y);
-        if (d == 0 && p.lse != nullptr)
-          p.lse[static_cast<int64_t>(v.first + i) * p.nh * p.group + j] =
+      };
+      auto put_lse = [&](int r, float mx, float sum) {
+        const int row = u.row0 + r;
+        if (p.lse != nullptr)
+          p.lse[static_cast<int64_t>(u.v.first + row / p.group) * p.nh * p.group + u.head * p.group + row % p.group] =
               sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
-      } else {
-        part[r * HD + d] = o;
-        if (d == 0) {
-          part[kRows * HD + r] = mx;
-          part[kRows * HD + kRows + r] = sum;
-        }
-      }
-    }
-    if (!single) {
-      __threadfence();
-      __syncthreads();
-      const int slot0 = 2 * first_block + (unit_w0 > first_block * chunk ? 1 : 0);
-      const int blocks = last_block - first_block + 1;
-      if (tid == 0) sm.last = atomicAdd(p.counters + slot0, 1) == blocks - 1;
-      __syncthreads();
-      if (sm.last) {
-        __threadfence();
-        for (int idx = tid; idx < live * (HD / 4); idx += kThreads) {
-          const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
-          float mx = -INFINITY, sum = 0.f;
-          float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-          for (int b = first_block; b <= last_block; ++b) {
-            const float* src = p.partial + (2 * static_cast<int64_t>(b) + (unit_w0 > b * chunk ? 1 : 0)) * kStep;
-            const float pm = __ldcg(src + kRows * HD + r), pl = __ldcg(src + kRows * HD + kRows + r);
-            const float4 po = __ldcg(reinterpret_cast<const float4*>(src + r * HD + d));
-            const float mn = fmaxf(mx, pm);
-            const float ms = mn == -INFINITY ? 0.f : mn;
-            const float k0 = exp2_fast(mx - ms), k1 = exp2_fast(pm - ms);
-            o[0] = o[0] * k0 + po.x * k1;
-            o[1] = o[1] * k0 + po.y * k1;
-            o[2] = o[2] * k0 + po.z * k1;
-            o[3] = o[3] * k0 + po.w * k1;
-            sum = sum * k0 + pl * k1;
-            mx = mn;
-          }
-          const int i = (row0 + r) / p.group, j = head * p.group + (row0 + r) % p.group;
-          const bool some = sum > 0.f || sum != sum;
-          const int64_t at = (v.first + i) * p.o_sr + j * p.o_sh + d;
+      };
+      constexpr int kStep = ROWS * (HD + 2);  // floats of one partial sum
+      if (u.ta == 0 && u.tb == u.tiles) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = some ? o[e] / sum : 0.f;
-            if (p.q_bf16)
-              reinterpret_cast<__nv_bfloat16*>(p.out)[at + e] = __float2bfloat16_rn(y);
-            else
-              reinterpret_cast<__half*>(p.out)[at + e] = __float2half_rn(y);
+        for (int r = 0; r < ROWS; ++r) {
+          if (r < u.live) {
+            const float inv = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
+#pragma unroll
+            for (int h = 0; h < C::kParts; ++h)
+              if (HD >= 128 || tid < HD) put(r, h * 128 + tid, acc[h][r] * inv);
+            if (tid == 0) put_lse(r, m[r], l[r]);
           }
-          if (d == 0 && p.lse != nullptr)
-            p.lse[static_cast<int64_t>(v.first + i) * p.nh * p.group + j] =
-                some ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
         }
-        if (tid == 0) p.counters[slot0] = 0;
+        soft_sync();  // lsum is read
+      } else {
+        float* part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (u.w0 > w_begin ? 1 : 0)) * kStep;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+          for (int h = 0; h < C::kParts; ++h)
+            if (HD >= 128 || tid < HD) part[r * HD + h * 128 + tid] = acc[h][r];
+          if (tid == 0) {
+            part[ROWS * HD + r] = m[r];
+            part[ROWS * HD + ROWS + r] = l[r];
+          }
+        }
+        __threadfence();
+        soft_sync();
+        const int first_block = static_cast<int>(u.w0 / chunk), last_block = static_cast<int>((u.w0 + u.tiles - 1) / chunk);
+        const int slot0 = 2 * first_block + (u.w0 > first_block * chunk ? 1 : 0);
+        if (tid == 0) sm.last = atomicAdd(p.counters + slot0, 1) == last_block - first_block;
+        soft_sync();
+        if (sm.last) {
+          __threadfence();
+          for (int idx = tid; idx < u.live * (HD / 4); idx += kSoft) {
+            const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+            float mx = -INFINITY, sum = 0.f;
+            float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int b = first_block; b <= last_block; ++b) {
+              const float* src = p.partial + (2 * static_cast<int64_t>(b) + (u.w0 > b * chunk ? 1 : 0)) * kStep;
+              const float pm = __ldcg(src + ROWS * HD + r), pl = __ldcg(src + ROWS * HD + ROWS + r);
+              const float4 po = __ldcg(reinterpret_cast<const float4*>(src + r * HD + d));
+              const float mn = fmaxf(mx, pm);
+              const float ms = mn == -INFINITY ? 0.f : mn;
+              const float k0 = exp2_fast(mx - ms), k1 = exp2_fast(pm - ms);
+              o[0] = o[0] * k0 + po.x * k1;
+              o[1] = o[1] * k0 + po.y * k1;
+              o[2] = o[2] * k0 + po.z * k1;
+              o[3] = o[3] * k0 + po.w * k1;
+              sum = sum * k0 + pl * k1;
+              mx = mn;
+            }
+            const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) put(r, d + e, o[e] * inv);
+            if (d == 0) put_lse(r, mx, sum);
+          }
+          if (tid == 0) p.counters[slot0] = 0;
+        }
       }
     }
-    w = unit_w0 + tb;
+  } else if (warp == 4) {
+    // ---- copies: block ids and scales for four tiles at a time, a lane per 16 tokens ---------
+    const int mine = lane >> 3, piece = lane & 7;
+    const int per_line = bs >> 4;
+    const uint32_t bytes = HD * bs;
+    int gt = 0, count = 0, head = 0, next_count = 0, next_head = 0;
+    int page = -1, next_page = -1;
+    float ks = 0.f, vs = 0.f, next_ks = 0.f, next_vs = 0.f;
+    u.t_last = 0;
+    // the next batch of at most four tiles of one unit; 0 at the end
+    auto look_ahead = [&]() {
+      next_count = 0;
+      while (gt >= u.t_last) {
+        if (!next_unit<ROWS>(p, walk, u)) return;
+        gt = u.t_first;
+      }
+      next_count = min(4, u.t_last - gt);
+      next_head = u.head;
+      const int tok = ((gt + mine) * kTile + 16 * piece) & ~(bs - 1);  // the block's first token
+      next_page = -1;
+      if (mine < next_count && tok < u.any_hi && tok + bs > u.any_lo)
+        next_page = __ldg(p.tables + u.seq * p.table_stride + (tok >> p.bs_log2));
+      if (next_page >= p.num_blocks) next_page = -1;
+      next_ks = next_vs = 0.f;
+      if (next_page >= 0) {
+        next_ks = __ldg(p.key_scale + next_page * p.ks_sb + next_head * p.ks_sh);
+        next_vs = __ldg(p.value_scale + next_page * p.vs_sb + next_head * p.vs_sh);
+      }
+      gt += next_count;
+    };
+    look_ahead();
+    uint32_t it = 0, k_sent = 0, v_sent = 0;
+    bool ok = true;
+    while (next_count > 0 && ok) {
+      count = next_count, head = next_head, page = next_page, ks = next_ks, vs = next_vs;
+      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+      for (int j = 0; j < count; ++j, ++it) {
+        const uint32_t slot = it % kST, parity = ((it / kST) & 1) ^ 1;
+        const bool issue = mine == j && page >= 0 && piece % per_line == 0;
+        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, issue));
+        ok = mbar_wait_warp(&sm.k_empty[slot], parity, gave_up);
+        if (!ok) break;
+        if (issue) {
+          const uint32_t to = smem_addr(sm.k[slot]) + piece * (HD * 16);
+          if (p.bs_log2 == 4)
+            bulk_load(to, p.key + page * p.k_sb + head * p.k_sh, bytes, &sm.k_full[slot]);
+          else
+            tensor_load(to, &kmap, head, page, &sm.k_full[slot]);
+        }
+        if (mine == j) {
+          sm.ks[it & 7][piece] = ks;
+          sm.vs[it & 7][piece] = vs;
+          if (piece == 0) sm.have[it & 7] = (there >> (8 * j)) & 0xffu;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect(&sm.k_full[slot], boxes * bytes);
+        ++k_sent;
+        if (j == 0) look_ahead();
+        ok = mbar_wait_warp(&sm.v_empty[slot], parity, gave_up);
+        if (!ok) break;
+        if (issue) {
+          const uint32_t to = smem_addr(sm.v[slot]) + piece * (HD * 16);
+          if (p.bs_log2 == 4)
+            bulk_load(to, p.value + page * p.v_sb + head * p.v_sh, bytes, &sm.v_full[slot]);
+          else
+            tensor_load(to, &vmap, head, page, &sm.v_full[slot]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect(&sm.v_full[slot], boxes * bytes);
+        ++v_sent;
+      }
+    }
+    // copies in flight end before the block does
+    for (uint32_t i = k_sent > kST ? k_sent - kST : 0; i < k_sent; ++i)
+      for (uint32_t z = 0; z < kWaitLimit && !mbar_try(&sm.k_full[i % kST], (i / kST) & 1); ++z) {
+      }
+    for (uint32_t i = v_sent > kST ? v_sent - kST : 0; i < v_sent; ++i)
+      for (uint32_t z = 0; z < kWaitLimit && !mbar_try(&sm.v_full[i % kST], (i / kST) & 1); ++z) {
+      }
+  } else if (lane == 0) {
+    // ---- the tensor cores ---------------------------------------------------------
+    constexpr int kFmt = CODE == MAK_CODE_INT8 ? 1 : 0, kAcc = CODE == MAK_CODE_INT8 ? 2 : 1;
+    constexpr uint32_t kQk = instr_desc(C::kN, kAcc, kFmt, true, false), kPv = instr_desc(C::kN, kAcc, kFmt, false, false);
+    const int line = p.bs_log2;
+    // K: lines of 8 head_dim rows, then blocks; V: the same lines as rows of M
+    const uint32_t k_lbo = line == 4 ? 128 : HD * bs, k_sbo = line == 4 ? HD * 16 : 8 * bs;
+    const uint32_t v_lbo = line == 4 ? HD * 16 : 16, v_sbo = 8 * bs;
+    auto mma = [&](uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+      if constexpr (CODE == MAK_CODE_INT8)
+        mma_ss_i8(d, a, b, idesc, add);
+      else
+        mma_ss_f8(d, a, b, idesc, add);
+    };
+    uint32_t it = 0, units = 0;
+    bool ok = true;
+    auto scores = [&](uint32_t x) {
+      const uint32_t slot = x % kST;
+      if (!mbar_wait(&sm.k_full[slot], (x / kST) & 1, gave_up)) return false;
+      tc_fence_after();
+      const uint32_t ka = smem_addr(sm.k[slot]), qa = smem_addr(sm.q);
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)
+        mma(tmem + (x & 1) * C::kN, smem_desc(ka + i * 32 * bs, k_lbo, k_sbo, line), smem_desc(qa + i * 256, 128, HD * 8, 0), kQk, i > 0);
+      tc_commit(&sm.s_full[x & 1]);
+      tc_commit(&sm.k_empty[slot]);
+      return true;
+    };
+    while (ok && next_unit<ROWS>(p, walk, u)) {
+      const int n = u.t_last - u.t_first;
+      if (n == 0) continue;
+      ok = mbar_wait(&sm.q_full, units & 1, gave_up);
+      ++units;
+      for (int t = 0; t < 2 && t < n && ok; ++t) ok = scores(it + t);
+      for (int t = 0; t < n && ok; ++t) {
+        const uint32_t x = it + t, slot = x % kST;
+        ok = mbar_wait(&sm.p_full[x & 1], (x >> 1) & 1, gave_up) && mbar_wait(&sm.v_full[slot], (x / kST) & 1, gave_up);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = smem_addr(sm.v[slot]), pa = smem_addr(sm.p[x & 1]);
+#pragma unroll
+        for (int h = 0; h < C::kParts; ++h)
+#pragma unroll
+          for (int i = 0; i < kTile / 32; ++i)
+            mma(tmem + 2 * C::kN + (2 * h + (x & 1)) * C::kN,
+                smem_desc(va + h * 128 * bs + ((32 * i) >> line) * (HD * bs) + ((32 * i) & (bs - 1)), v_lbo, v_sbo, line),
+                smem_desc(pa + i * 256, 128, 1024, 0), kPv, i > 0);
+        tc_commit(&sm.o_full[x & 1]);
+        tc_commit(&sm.v_empty[slot]);
+        if (t + 2 < n) ok = scores(x + 2);
+      }
+      it += n;
+    }
+    if (!ok) {  // let what was issued end before the TMEM is given back
+      tc_commit(&sm.spare);
+      for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free<C::kTmem>(tmem);
   }
 }
 
-template <int HD, int NT, int CODE>
+// [num_blocks][num_heads][head_dim][block_size] bytes, boxes of one head of one block, lines swizzled.
+int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (encode == nullptr) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess || fn == nullptr) {
+      (void)cudaGetLastError();
+      return fail(MAK_E_CUDA, "mak_block_attention: no cuTensorMapEncodeTiled in this driver");
+    }
+    encode = reinterpret_cast<Encode>(fn);
+  }
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(bs), static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(nh),
+                              static_cast<cuuint64_t>(num_blocks)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(bs), static_cast<cuuint64_t>(sh), static_cast<cuuint64_t>(sb)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(bs), static_cast<cuuint32_t>(hd), 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle =
+      bs == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bs == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, steps,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(MAK_E_INVALID, "mak_block_attention: the cache's strides make no tensor map (%d)", static_cast<int>(rc));
+  return MAK_OK;
+}
+
+template <int HD, int ROWS, int CODE>
 int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
-  const void* fn = reinterpret_cast<const void*>(&block_attn_rows_kernel<HD, NT, CODE>);
-  constexpr int kBytes = sizeof(Smem<HD, NT>);
+  const auto kernel = block_attn_rows_kernel<HD, ROWS, CODE>;
+  constexpr int kBytes = sizeof(Smem<HD, ROWS>) + 1024;
+  static_assert(kBytes <= (HD == 256 ? 227 : 113) * 1024, "blocks per SM");
   static int per_sm = 0;
   if (per_sm == 0) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(block_attn_rows_kernel<HD, NT, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (e != cudaSuccess) {
       (void)cudaGetLastError();
       return cuda_fail(e, "mak_block_attention");
     }
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, kThreads, kBytes) != cudaSuccess || n <= 0) n = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, kBytes) != cudaSuccess || n <= 0) n = 1;
+    // TMEM has 512 columns, and a block whose allocation has to wait for another's end gains nothing
+    if (n * Cfg<HD, ROWS>::kTmem > 512) n = 512 / Cfg<HD, ROWS>::kTmem;
     per_sm = n;
+  }
+  CUtensorMap maps[2] = {};
+  if (p.bs_log2 > 4 && p.num_blocks > 0) {
+    if (int rc = cache_map(&maps[0], p.key, p.k_sb, p.k_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2)) return rc;
+    if (int rc = cache_map(&maps[1], p.value, p.v_sb, p.v_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2)) return rc;
   }
   int64_t grid = per_sm * sm_count();
   if (grid > kMaxGrid) grid = kMaxGrid;
-  // no more blocks than there can be work for: kWarps tiles each
+  // no more blocks than there can be work for
   const int64_t seq_tiles = ((static_cast<int64_t>(p.max_blocks) << p.bs_log2) + kTile - 1) / kTile + 1;
-  const int64_t groups = static_cast<int64_t>(p.num_rows) * p.group / (8 * NT) + p.num_seqs;
-  const int64_t most = (groups * p.nh * seq_tiles + kWarps - 1) / kWarps;
+  const int64_t groups = static_cast<int64_t>(p.num_rows) * p.group / ROWS + p.num_seqs;
+  const int64_t most = (groups * p.nh * seq_tiles + kMinChunk - 1) / kMinChunk;
   if (most < grid) grid = most;
-  return launch_pdl("mak_block_attention", block_attn_rows_kernel<HD, NT, CODE>, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kBytes, st, p);
+  return launch_pdl("mak_block_attention", kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), kBytes, st, p, maps[0], maps[1]);
 }
 
-template <int HD, int NT>
+template <int HD, int ROWS>
 int launch_rows_code(const BlockAttnParams& p, int code, cudaStream_t st) {
-  return code == MAK_CODE_INT8 ? launch_rows<HD, NT, MAK_CODE_INT8>(p, st) : launch_rows<HD, NT, MAK_CODE_E4M3>(p, st);
+  return code == MAK_CODE_INT8 ? launch_rows<HD, ROWS, MAK_CODE_INT8>(p, st) : launch_rows<HD, ROWS, MAK_CODE_E4M3>(p, st);
 }
 
 constexpr int64_t kCounterBytes = (2 * kMaxGrid * 4 + 255) / 256 * 256;
@@ -729,7 +899,7 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
   if (rows >= 64 && c.head_dim <= 128) return launch_block_attn_tc(p, c.head_dim, c.code_type, st);
   const bool wide = rows > 8 && c.head_dim < 256;
-  if (c.head_dim == 64) return wide ? launch_rows_code<64, 2>(p, c.code_type, st) : launch_rows_code<64, 1>(p, c.code_type, st);
-  if (c.head_dim == 128) return wide ? launch_rows_code<128, 2>(p, c.code_type, st) : launch_rows_code<128, 1>(p, c.code_type, st);
-  return launch_rows_code<256, 1>(p, c.code_type, st);
+  if (c.head_dim == 64) return wide ? launch_rows_code<64, 16>(p, c.code_type, st) : launch_rows_code<64, 8>(p, c.code_type, st);
+  if (c.head_dim == 128) return wide ? launch_rows_code<128, 16>(p, c.code_type, st) : launch_rows_code<128, 8>(p, c.code_type, st);
+  return launch_rows_code<256, 8>(p, c.code_type, st);
 }

@@ -22,6 +22,7 @@
 // Scores and weights share TMEM columns: the product with V of a tile is issued
 // before the next scores of the same rows overwrite them.
 #include "block_attn.cuh"
+#include "tcgen05.cuh"
 
 namespace mak {
 namespace {
@@ -29,97 +30,7 @@ namespace {
 constexpr int kTile = 128;                // tokens per step
 constexpr int kUnitRows = 256;            // rows of a block
 constexpr int kThreads = 512;
-constexpr uint32_t kWaitLimit = 1u << 22; // polls of a barrier before the block gives up
 constexpr float kLazy = 8.f;              // log2 growth of a row's maximum that is tolerated
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-
-__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(b)) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(smem_addr(b)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// False when the barrier did not complete within the limit, or another role gave up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* gave_up) {
-  for (uint32_t i = 0; i < kWaitLimit; ++i) {
-    if (mbar_try(b, parity)) return true;
-    if ((i & 255) == 255 && *gave_up) return false;
-  }
-  *gave_up = 1;
-  return false;
-}
-
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t* b) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(b)) : "memory");
-}
-__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// D (TMEM, f32) = or += A (shared memory) * B (shared memory)
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(add)
-      : "memory");
-}
-// D (TMEM, f32) = or += A (TMEM) * B (shared memory)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(add)
-      : "memory");
-}
-
-#define MAK_R8(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3]), "=r"(a[i + 4]), "=r"(a[i + 5]), "=r"(a[i + 6]), "=r"(a[i + 7])
-#define MAK_W8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
-
-__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
-      "%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : MAK_R8(v, 0), MAK_R8(v, 8), MAK_R8(v, 16), MAK_R8(v, 24)
-      : "r"(at));
-}
-#define MAK_RW8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
-// Waits for this thread's loads from TMEM; the registers are named so that nothing uses them before.
-__device__ __forceinline__ void tmem_wait32(uint32_t (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" : MAK_RW8(v, 0), MAK_RW8(v, 8), MAK_RW8(v, 16), MAK_RW8(v, 24)::"memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::MAK_W8(v, 0),
-      MAK_W8(v, 8), MAK_W8(v, 16), MAK_W8(v, 24), "r"(at)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MAK_W8(v, 0),
-      MAK_W8(v, 8), "r"(at)
-      : "memory");
-}
-
-// Shared-memory matrix descriptor: 128-byte swizzle, strides in bytes.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t at, uint32_t lbo, uint32_t sbo) {
-  return static_cast<uint64_t>((at >> 4) & 0x3fff) | (static_cast<uint64_t>((lbo >> 4) & 0x3fff) << 16) |
-         (static_cast<uint64_t>((sbo >> 4) & 0x3fff) << 32) | (1ull << 46) | (2ull << 61);
-}
-// Instruction descriptor: f16 x f16 -> f32, M = 128.
-constexpr uint32_t instr_desc(int n, bool b_mn_major) {
-  return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(128 >> 4) << 24);
-}
 
 template <int HD>
 struct TcSmem {
@@ -180,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
         mbar_init(&sm.p_full[i], 4);
         mbar_init(&sm.o_full[i], 1);
       }
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      mbar_init_fence();
     }
   }
   __syncthreads();
@@ -190,8 +101,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
   const int64_t row0 = static_cast<int64_t>(sm.unit_tile) * kUnitRows;
   if (row0 >= rows_total) return;
   if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    tmem_alloc<512>(&sm.tmem);
   }
   const int live = static_cast<int>(min(static_cast<int64_t>(kUnitRows), rows_total - row0));
   const int halves = live > 128 ? 2 : 1;
@@ -283,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int t = 0; t < tiles; ++t) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm.s_full[half], t & 1, gave_up));
+        ok = mbar_wait_warp(&sm.s_full[half], t & 1, gave_up);
         if (!ok) break;
         tc_fence_after();
         const int tok = (t0 + t) * kTile;
@@ -295,8 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t x[32];
-          tmem_ld32(s_at + c * 32, x);
-          tmem_wait32(x);
+          tmem_ld(s_at + c * 32, x);
+          tmem_wait(x);
           const float f0 = kf[2 * c] * qs, f1 = kf[2 * c + 1] * qs;
           if (whole) {
 #pragma unroll
@@ -319,11 +229,11 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c) {
               uint32_t x[32];
-              tmem_ld32(o_at + c * 32, x);
-              tmem_wait32(x);
+              tmem_ld(o_at + c * 32, x);
+              tmem_wait(x);
 #pragma unroll
               for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
-              tmem_st32(o_at + c * 32, x);
+              tmem_st(o_at + c * 32, x);
             }
           }
         }
@@ -331,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t x[32], y[16];
-          tmem_ld32(s_at + c * 32, x);
-          tmem_wait32(x);
+          tmem_ld(s_at + c * 32, x);
+          tmem_wait(x);
           const float f0 = kf[2 * c] * qs, f1 = kf[2 * c + 1] * qs;
           const float v0 = vf[2 * c], v1 = vf[2 * c + 1];
 #pragma unroll
@@ -349,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
             l += a + b;
             y[e >> 1] = pack_f16(a * w, b * w);
           }
-          tmem_st16(s_at + c * 16, y);
+          tmem_st(s_at + c * 16, y);
         }
         tc_wait_st();
         tc_fence_before();
@@ -357,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
         if (lane == 0) mbar_arrive(&sm.p_full[half]);
       }
       if (ok && tiles > 0) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sm.o_full[half], 0, gave_up));
+        ok = mbar_wait_warp(&sm.o_full[half], 0, gave_up);
         tc_fence_after();
       }
       // a block that gave up leaves NaN, not stale memory
@@ -369,8 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t x[32];
         if (tiles > 0 && ok) {
-          tmem_ld32(o_at + c * 32, x);
-          tmem_wait32(x);
+          tmem_ld(o_at + c * 32, x);
+          tmem_wait(x);
         }
         if (on) {
           uint32_t y[16];
@@ -474,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
     for (int t = 0; t < tiles; ++t) {
       const int st = t & 1;
       const uint32_t parity = ((t >> 1) & 1) ^ 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&sm.k_empty[st], parity, gave_up))) break;
+      if (!mbar_wait_warp(&sm.k_empty[st], parity, gave_up)) break;
       // the factors of tile t - 4 were last read before tile t - 2's scores were issued
       if (dlo == 0 && w < 2) {
         sm.kfac[t & 3][chunk] = ks;
@@ -492,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
       page = next_page;
       if (t + 1 < tiles) fetch(kb, p.k_sb, t + 1, page, kx);
       next_page = find(t + 2);
-      if (!__all_sync(0xffffffffu, mbar_wait(&sm.v_empty[st], parity, gave_up))) break;
+      if (!mbar_wait_warp(&sm.v_empty[st], parity, gave_up)) break;
       store(sm.v[st], t, vx);
       fence_async_shared();
       __syncwarp();
@@ -504,13 +414,13 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
     }
   } else if (warp == 12 && lane == 0 && tiles > 0) {
     // ---- the tensor cores ---------------------------------------------------------
-    constexpr uint32_t kQk = instr_desc(kTile, true), kPv = instr_desc(HD, false);
+    constexpr uint32_t kQk = instr_desc(kTile, 1, 0, false, true), kPv = instr_desc(HD, 1, 0, false, false);
     auto scores = [&](int half, int st) {
       const uint32_t qa = smem_addr(sm.q[half]), ka = smem_addr(sm.k[st]);
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
-        mma_ss(tmem + half * 128, smem_desc(qa + (ks >> 2) * 16384 + (ks & 3) * 32, 16, 1024),
-               smem_desc(ka + ks * 2048, HD * 128, 1024), kQk, ks > 0);
+        mma_ss_f16(tmem + half * 128, smem_desc(qa + (ks >> 2) * 16384 + (ks & 3) * 32, 16, 1024, 7),
+               smem_desc(ka + ks * 2048, HD * 128, 1024, 7), kQk, ks > 0);
       tc_commit(&sm.s_full[half]);
     };
     bool ok = true;
@@ -532,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
         const uint32_t va = smem_addr(sm.v[st]);
 #pragma unroll
         for (int ks = 0; ks < kTile / 16; ++ks)
-          mma_ts(tmem + 256 + half * HD, tmem + half * 128 + ks * 8, smem_desc(va + (ks >> 2) * (HD * 128) + (ks & 3) * 32, 16, 1024),
+          mma_ts_f16(tmem + 256 + half * HD, tmem + half * 128 + ks * 8, smem_desc(va + (ks >> 2) * (HD * 128) + (ks & 3) * 32, 16, 1024, 7),
                  kPv, t > 0 || ks > 0);
         if (half == halves - 1) tc_commit(&sm.v_empty[st]);
         if (t + 1 < tiles) {
@@ -554,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
   if (warp == 12) {
     __syncwarp();
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    tmem_free<512>(tmem);
   }
 }
 
