@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
                            const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<HD, ROWS>;
   constexpr int kST = C::kStages;
-  extern __shared__ uint8_t raw[];
-  Smem<HD, ROWS>& sm = *reinterpret_cast<Smem<HD, ROWS>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Smem<HD, ROWS>& sm = *reinterpret_cast<Smem<HD, ROWS>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_trigger();
@@ -602,73 +602,77 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
   } else if (warp == 4) {
     // ---- copies: block ids and scales for four tiles at a time, a lane per 16 tokens ---------
     const int mine = lane >> 3, piece = lane & 7;
-    const int per_line = bs >> 4;
-    const uint32_t bytes = HD * bs;
-    int gt = 0, count = 0, head = 0, next_count = 0, next_head = 0;
-    int page = -1, next_page = -1;
-    float ks = 0.f, vs = 0.f, next_ks = 0.f, next_vs = 0.f;
+    const uint32_t per_line = bs >> 4, bytes = HD * bs;
+    const bool leads = piece % per_line == 0;  // issues its block's copies
+    const uint32_t k_to = smem_addr(sm.k) + piece * (HD * 16), v_to = smem_addr(sm.v) + piece * (HD * 16);
+    struct Batch {
+      int count, head, page;
+      float ks, vs;
+      const uint8_t *k, *v;
+    } next;
+    int gt = 0;
     u.t_last = 0;
-    // the next batch of at most four tiles of one unit; 0 at the end
+    // the next batch of at most four tiles of one unit; none at the end
     auto look_ahead = [&]() {
-      next_count = 0;
+      next.count = 0;
       while (gt >= u.t_last) {
         if (!next_unit<ROWS>(p, walk, u)) return;
         gt = u.t_first;
       }
-      next_count = min(4, u.t_last - gt);
-      next_head = u.head;
+      next.count = min(4, u.t_last - gt);
+      next.head = u.head;
       const int tok = ((gt + mine) * kTile + 16 * piece) & ~(bs - 1);  // the block's first token
-      next_page = -1;
-      if (mine < next_count && tok < u.any_hi && tok + bs > u.any_lo)
-        next_page = __ldg(p.tables + u.seq * p.table_stride + (tok >> p.bs_log2));
-      if (next_page >= p.num_blocks) next_page = -1;
-      next_ks = next_vs = 0.f;
-      if (next_page >= 0) {
-        next_ks = __ldg(p.key_scale + next_page * p.ks_sb + next_head * p.ks_sh);
-        next_vs = __ldg(p.value_scale + next_page * p.vs_sb + next_head * p.vs_sh);
+      next.page = -1;
+      if (mine < next.count && tok < u.any_hi && tok + bs > u.any_lo)
+        next.page = __ldg(p.tables + u.seq * p.table_stride + (tok >> p.bs_log2));
+      if (next.page >= p.num_blocks) next.page = -1;
+      next.ks = next.vs = 0.f;
+      if (next.page >= 0) {
+        next.ks = __ldg(p.key_scale + next.page * p.ks_sb + next.head * p.ks_sh);
+        next.vs = __ldg(p.value_scale + next.page * p.vs_sb + next.head * p.vs_sh);
+        next.k = p.key + next.page * p.k_sb + next.head * p.k_sh;
+        next.v = p.value + next.page * p.v_sb + next.head * p.v_sh;
       }
-      gt += next_count;
+      gt += next.count;
     };
     look_ahead();
-    uint32_t it = 0, k_sent = 0, v_sent = 0;
+    uint32_t it = 0, slot = 0, parity = 1, k_sent = 0, v_sent = 0;
     bool ok = true;
-    while (next_count > 0 && ok) {
-      count = next_count, head = next_head, page = next_page, ks = next_ks, vs = next_vs;
-      const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-      for (int j = 0; j < count; ++j, ++it) {
-        const uint32_t slot = it % kST, parity = ((it / kST) & 1) ^ 1;
-        const bool issue = mine == j && page >= 0 && piece % per_line == 0;
-        const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, issue));
+    while (next.count > 0 && ok) {
+      const Batch b = next;
+      const uint32_t there = __ballot_sync(0xffffffffu, b.page >= 0);
+      const uint32_t led = __ballot_sync(0xffffffffu, b.page >= 0 && leads);
+      for (int j = 0; j < b.count; ++j, ++it) {
+        const bool issue = mine == j && b.page >= 0 && leads;
+        const uint32_t expect = __popc((led >> (8 * j)) & 0xffu) * bytes;
         ok = mbar_wait_warp(&sm.k_empty[slot], parity, gave_up);
         if (!ok) break;
         if (issue) {
-          const uint32_t to = smem_addr(sm.k[slot]) + piece * (HD * 16);
           if (p.bs_log2 == 4)
-            bulk_load(to, p.key + page * p.k_sb + head * p.k_sh, bytes, &sm.k_full[slot]);
+            bulk_load(k_to + slot * C::kTileBytes, b.k, bytes, &sm.k_full[slot]);
           else
-            tensor_load(to, &kmap, head, page, &sm.k_full[slot]);
+            tensor_load(k_to + slot * C::kTileBytes, &kmap, b.head, b.page, &sm.k_full[slot]);
         }
         if (mine == j) {
-          sm.ks[it & 7][piece] = ks;
-          sm.vs[it & 7][piece] = vs;
+          sm.ks[it & 7][piece] = b.ks;
+          sm.vs[it & 7][piece] = b.vs;
           if (piece == 0) sm.have[it & 7] = (there >> (8 * j)) & 0xffu;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect(&sm.k_full[slot], boxes * bytes);
+        if (lane == 0) mbar_arrive_expect(&sm.k_full[slot], expect);
         ++k_sent;
         if (j == 0) look_ahead();
         ok = mbar_wait_warp(&sm.v_empty[slot], parity, gave_up);
         if (!ok) break;
         if (issue) {
-          const uint32_t to = smem_addr(sm.v[slot]) + piece * (HD * 16);
           if (p.bs_log2 == 4)
-            bulk_load(to, p.value + page * p.v_sb + head * p.v_sh, bytes, &sm.v_full[slot]);
+            bulk_load(v_to + slot * C::kTileBytes, b.v, bytes, &sm.v_full[slot]);
           else
-            tensor_load(to, &vmap, head, page, &sm.v_full[slot]);
+            tensor_load(v_to + slot * C::kTileBytes, &vmap, b.head, b.page, &sm.v_full[slot]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_expect(&sm.v_full[slot], boxes * bytes);
+        if (lane == 0) mbar_arrive_expect(&sm.v_full[slot], expect);
         ++v_sent;
+        if (++slot == kST) slot = 0, parity ^= 1;
       }
     }
     // copies in flight end before the block does
@@ -692,18 +696,25 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       else
         mma_ss_f8(d, a, b, idesc, add);
     };
+    // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
+    const uint64_t k_desc = smem_desc(smem_addr(sm.k), k_lbo, k_sbo, line), q_desc = smem_desc(smem_addr(sm.q), 128, HD * 8, 0);
+    const uint64_t v_desc = smem_desc(smem_addr(sm.v), v_lbo, v_sbo, line), p_desc = smem_desc(smem_addr(sm.p), 128, 1024, 0);
+    constexpr uint32_t kTileStep = C::kTileBytes / 16;
+    uint32_t v_step[kTile / 32];  // 32 tokens of V each
+#pragma unroll
+    for (int i = 0; i < kTile / 32; ++i) v_step[i] = (((32 * i) >> line) * (HD * bs) + ((32 * i) & (bs - 1))) >> 4;
     uint32_t it = 0, units = 0;
+    uint32_t k_slot = 0, k_parity = 0, v_slot = 0, v_parity = 0;
     bool ok = true;
     auto scores = [&](uint32_t x) {
-      const uint32_t slot = x % kST;
-      if (!mbar_wait(&sm.k_full[slot], (x / kST) & 1, gave_up)) return false;
+      if (!mbar_wait(&sm.k_full[k_slot], k_parity, gave_up)) return false;
       tc_fence_after();
-      const uint32_t ka = smem_addr(sm.k[slot]), qa = smem_addr(sm.q);
+      const uint64_t kd = k_desc + k_slot * kTileStep;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i)
-        mma(tmem + (x & 1) * C::kN, smem_desc(ka + i * 32 * bs, k_lbo, k_sbo, line), smem_desc(qa + i * 256, 128, HD * 8, 0), kQk, i > 0);
+      for (int i = 0; i < HD / 32; ++i) mma(tmem + (x & 1) * C::kN, kd + i * 2 * bs, q_desc + i * 16, kQk, i > 0);
       tc_commit(&sm.s_full[x & 1]);
-      tc_commit(&sm.k_empty[slot]);
+      tc_commit(&sm.k_empty[k_slot]);
+      if (++k_slot == kST) k_slot = 0, k_parity ^= 1;
       return true;
     };
     while (ok && next_unit<ROWS>(p, walk, u)) {
@@ -713,20 +724,19 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       ++units;
       for (int t = 0; t < 2 && t < n && ok; ++t) ok = scores(it + t);
       for (int t = 0; t < n && ok; ++t) {
-        const uint32_t x = it + t, slot = x % kST;
-        ok = mbar_wait(&sm.p_full[x & 1], (x >> 1) & 1, gave_up) && mbar_wait(&sm.v_full[slot], (x / kST) & 1, gave_up);
+        const uint32_t x = it + t;
+        ok = mbar_wait(&sm.v_full[v_slot], v_parity, gave_up) && mbar_wait(&sm.p_full[x & 1], (x >> 1) & 1, gave_up);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t va = smem_addr(sm.v[slot]), pa = smem_addr(sm.p[x & 1]);
+        const uint64_t vd = v_desc + v_slot * kTileStep, pd = p_desc + (x & 1) * (C::kN * kTile / 16);
 #pragma unroll
         for (int h = 0; h < C::kParts; ++h)
 #pragma unroll
           for (int i = 0; i < kTile / 32; ++i)
-            mma(tmem + 2 * C::kN + (2 * h + (x & 1)) * C::kN,
-                smem_desc(va + h * 128 * bs + ((32 * i) >> line) * (HD * bs) + ((32 * i) & (bs - 1)), v_lbo, v_sbo, line),
-                smem_desc(pa + i * 256, 128, 1024, 0), kPv, i > 0);
+            mma(tmem + 2 * C::kN + (2 * h + (x & 1)) * C::kN, vd + h * 8 * bs + v_step[i], pd + i * 16, kPv, i > 0);
         tc_commit(&sm.o_full[x & 1]);
-        tc_commit(&sm.v_empty[slot]);
+        tc_commit(&sm.v_empty[v_slot]);
+        if (++v_slot == kST) v_slot = 0, v_parity ^= 1;
         if (t + 2 < n) ok = scores(x + 2);
       }
       it += n;
@@ -778,17 +788,17 @@ int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int
 template <int HD, int ROWS, int CODE>
 int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
   const auto kernel = block_attn_rows_kernel<HD, ROWS, CODE>;
-  constexpr int kBytes = sizeof(Smem<HD, ROWS>) + 1024;
-  static_assert(kBytes <= (HD == 256 ? 227 : 113) * 1024, "blocks per SM");
+  constexpr int kBytes = sizeof(Smem<HD, ROWS>);
+  static_assert(kBytes <= (HD == 256 ? 227 : 113) * 1024, "blocks per SM");  // 228 KB less 1 KB per block
   static int per_sm = 0;
   if (per_sm == 0) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     if (e != cudaSuccess) {
       (void)cudaGetLastError();
       return cuda_fail(e, "mak_block_attention");
     }
-    int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kThreads, kBytes) != cudaSuccess || n <= 0) n = 1;
+    int n = HD == 256 ? 1 : 2;
     // TMEM has 512 columns, and a block whose allocation has to wait for another's end gains nothing
     if (n * Cfg<HD, ROWS>::kTmem > 512) n = 512 / Cfg<HD, ROWS>::kTmem;
     per_sm = n;
