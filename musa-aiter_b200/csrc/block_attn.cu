@@ -14,8 +14,8 @@
 // So q (bf16: 8 bits, f16: 11) goes in exactly but for values below 2^-13 of its row's largest,
 // and a weight is good to 2^-12 of itself or 2^-30 of its tile's largest.  The fourth term is free:
 // 8 rows with three terms would be 24 columns, and the tensor cores want a multiple of 16.
-// Each 128-token tile has its own maximum, largest V scale and product with V; tiles are joined
-// in 32-bit registers, so the tensor cores' accumulators never need rescaling.
+// Each step of one or two 128-token tiles has its own maximum, largest V scale and product with V;
+// steps are joined in 32-bit registers, so the tensor cores' accumulators never need rescaling.
 //
 // Layout.  Tokens are the M axis of the scores (A = K, MN-major: tokens contiguous) and head_dim
 // the M axis of the products (A = V, K-major: tokens contiguous again); the rows of q (heads that
@@ -28,7 +28,7 @@
 // equal runs, one per thread block, whatever the lengths; a block finds its run from the lengths
 // alone.  A unit cut by that leaves partial sums (maximum, sum, accumulators) and the last block
 // to arrive joins them.  Roles: warps 0-3 softmax (a thread per token, then per head_dim row),
-// warp 4 copies, warp 5 issues the tensor cores; two tiles are in flight between them.
+// warp 4 copies, warp 5 issues the tensor cores; two steps are in flight between them.
 #include <cuda.h>
 
 #include "block_attn.cuh"
@@ -44,32 +44,42 @@ constexpr int kMaxGrid = 148 * 4;  // blocks of the largest grid; the workspace 
 constexpr int kMaxRows = 16;
 constexpr int kMaxDim = 256;
 constexpr int kMinChunk = 2;  // tiles per block that are worth another block
+// A unit's beginning and end (its rows of q, its result) take a block about as long as this many tiles.
+constexpr int kUnitCost = 3;
 
 template <int HD, int ROWS>
 struct Cfg {
   static constexpr int kN = 4 * ROWS;              // columns of the products
   static constexpr int kParts = HD == 256 ? 2 : 1; // 128-row parts of head_dim
-  static constexpr int kStages = HD == 64 ? 4 : HD == 128 && ROWS == 8 ? 3 : 2;
+  static constexpr int kStep = ROWS == 8 ? 2 : 1;  // tiles of one softmax step
+  // Tiles of K and V in shared memory.  Scores are taken as soon as K is there; V waits for the
+  // weights, a step of it held and a step on its way.
+  static constexpr int kKs = HD == 64 ? 4 : 2;
+  static constexpr int kVs = HD == 64 ? 6 : ROWS == 8 ? 4 : 3;
   static constexpr int kTileBytes = HD * kTile;
-  static constexpr int kTmem = 2 * kN * (1 + kParts) <= 128 ? 128 : 2 * kN * (1 + kParts) <= 256 ? 256 : 512;
+  static constexpr int kScores = 0, kOut = 2 * kStep * kN;  // TMEM columns: two steps' scores, one product
+  static constexpr int kCols = kOut + kParts * kN;
+  static constexpr int kTmem = kCols <= 128 ? 128 : kCols <= 256 ? 256 : 512;
 };
 
 template <int HD, int ROWS>
 struct Smem {
   using C = Cfg<HD, ROWS>;
   // V first: with head_dim 64 the products read 128 rows from it, the last 64 past a tile's end
-  alignas(1024) uint8_t v[C::kStages][C::kTileBytes];
-  alignas(1024) uint8_t k[C::kStages][C::kTileBytes];
-  alignas(1024) uint8_t p[2][C::kN * kTile];
+  alignas(1024) uint8_t v[C::kVs][C::kTileBytes];
+  alignas(1024) uint8_t k[C::kKs][C::kTileBytes];
+  alignas(1024) uint8_t p[C::kN * kTile * C::kStep];
   uint8_t q[C::kN * HD];
-  alignas(16) float ks[8][8], vs[8][8];  // scales per 16 tokens, tile number mod 8
-  uint32_t have[8];                      // bit c: 16-token piece c has a block
+  alignas(16) float ks[16][8], vs[16][8];  // scales per 16 tokens, tile number mod 16
+  uint32_t have[16];                       // bit c: 16-token piece c has a block
+  int page[16][8], head[16];               // for the copies of V, which follow those of K
   alignas(16) float wmax[2][4][ROWS];
   alignas(16) float row_scale[ROWS];
   int row_lo[ROWS], row_hi[ROWS];
+  alignas(8) int64_t row_out[ROWS], row_lse[ROWS];  // places of the results
   float lsum[4][ROWS];
-  alignas(8) uint64_t k_full[C::kStages], k_empty[C::kStages], v_full[C::kStages], v_empty[C::kStages];
-  uint64_t q_full, s_full[2], p_full[2], o_full[2], spare;
+  alignas(8) uint64_t k_full[C::kKs], k_empty[C::kKs], v_full[C::kVs], v_empty[C::kVs];
+  uint64_t q_full, s_full[2], p_full, o_full, spare;
   int64_t scan[4];
   int64_t begin_base;
   int begin_seq;
@@ -84,61 +94,83 @@ __device__ __forceinline__ int unit_tiles(const SeqView& v) {
 }
 
 template <int ROWS>
+__device__ __forceinline__ int row_groups(const BlockAttnParams& p, const SeqView& v) {
+  return (v.rows * p.group + ROWS - 1) / ROWS;
+}
+template <int ROWS>
 __device__ __forceinline__ int64_t seq_work(const BlockAttnParams& p, const SeqView& v) {
-  if (v.rows == 0) return 0;
-  const int64_t groups = (static_cast<int64_t>(v.rows) * p.group + ROWS - 1) / ROWS;
-  return groups * p.nh * unit_tiles(v);
+  return static_cast<int64_t>(row_groups<ROWS>(p, v)) * p.nh * (unit_tiles(v) + kUnitCost);
 }
 
-// A block's run of work, unit by unit; every warp walks it for itself.
+// A block's run [w, w_end) of work, unit by unit; every warp walks it for itself.  A unit of n
+// tiles is kUnitCost + n steps long, its tiles being the last ones.
 struct Walk {
-  int64_t w, w_end, base;
-  int seq;
+  SeqView v;
+  int seq, head, group, groups, tiles;  // the unit that begins at w0
+  int64_t w, w_end, w0;
 };
 struct Unit {
-  SeqView v;
-  int seq, head, row0, live;          // rows row0 .. row0 + live of the sequence (row i * group + j: row i, query head j)
+  int seq;
+  int head, row0, live;               // rows row0 .. row0 + live (row i * group + j: row i, query head j)
   int tiles, ta, tb;                  // of the unit's tiles this block has [ta, tb)
   int t_first, t_last;                // absolute tiles of those that some row sees
   int any_lo, any_hi, all_lo, all_hi; // tokens that some / all rows see
-  int64_t w0;
+  int64_t w_tiles;                    // where the unit's tiles begin
+  SeqView v;
 };
 
 template <int ROWS>
+__device__ __forceinline__ void begin_walk(const BlockAttnParams& p, Walk& k, int seq, int64_t base) {
+  k.seq = seq;
+  k.v = seq_view(p, seq);
+  k.tiles = unit_tiles(k.v);
+  k.groups = row_groups<ROWS>(p, k.v);
+  const int64_t rel = k.w - base;
+  const uint32_t len = k.tiles + kUnitCost;
+  const int64_t unit = (rel >> 32) == 0 ? static_cast<uint32_t>(rel) / len : rel / len;
+  k.w0 = base + unit * len;
+  k.head = static_cast<int>(static_cast<uint32_t>(unit) / static_cast<uint32_t>(k.groups));
+  k.group = static_cast<int>(unit - static_cast<int64_t>(k.head) * k.groups);
+}
+
+// The next unit of which this block has any tiles.
+template <int ROWS>
 __device__ __forceinline__ bool next_unit(const BlockAttnParams& p, Walk& k, Unit& u) {
-  if (k.w >= k.w_end) return false;
-  SeqView v = seq_view(p, k.seq);
-  int64_t sw = seq_work<ROWS>(p, v);
-  while (k.w >= k.base + sw) {
-    k.base += sw;
-    v = seq_view(p, ++k.seq);
-    sw = seq_work<ROWS>(p, v);
+  for (;;) {
+    if (k.w >= k.w_end) return false;
+    u.ta = static_cast<int>(max(k.w - k.w0 - kUnitCost, static_cast<int64_t>(0)));
+    u.tb = static_cast<int>(min(k.w_end - k.w0 - kUnitCost, static_cast<int64_t>(k.tiles)));
+    u.seq = k.seq;
+    u.v = k.v;
+    u.tiles = k.tiles;
+    u.head = k.head;
+    u.row0 = k.group * ROWS;
+    u.w_tiles = k.w0 + kUnitCost;
+    k.w0 += kUnitCost + k.tiles;
+    k.w = k.w0;
+    if (k.w < k.w_end && ++k.group == k.groups) {
+      k.group = 0;
+      if (++k.head == p.nh) {
+        k.head = 0;
+        do {
+          k.v = seq_view(p, ++k.seq);
+        } while (k.v.rows == 0);
+        k.tiles = unit_tiles(k.v);
+        k.groups = row_groups<ROWS>(p, k.v);
+      }
+    }
+    if (u.tb > u.ta) break;
   }
-  u.v = v;
-  u.seq = k.seq;
-  u.tiles = unit_tiles(v);
-  const int64_t rel = k.w - k.base;
-  const int64_t unit = (rel >> 31) == 0 ? static_cast<uint32_t>(rel) / static_cast<uint32_t>(u.tiles) : rel / u.tiles;
-  u.w0 = k.base + unit * u.tiles;
-  u.ta = static_cast<int>(k.w - u.w0);
-  u.tb = static_cast<int>(min(k.w_end - u.w0, static_cast<int64_t>(u.tiles)));
-  const int rows_total = v.rows * p.group;
-  const uint32_t groups = (rows_total + ROWS - 1) / ROWS;
-  u.head = static_cast<int>(static_cast<uint32_t>(unit) / groups);
-  u.row0 = static_cast<int>(static_cast<uint32_t>(unit) % groups) * ROWS;
-  u.live = min(ROWS, rows_total - u.row0);
-  int lo1, hi0;
-  row_range(p, v, u.row0 / p.group, &u.any_lo, &hi0);
-  row_range(p, v, (u.row0 + u.live - 1) / p.group, &lo1, &u.any_hi);
-  u.all_lo = lo1;
-  u.all_hi = hi0;
+  const SeqView& v = u.v;
+  u.live = min(ROWS, v.rows * p.group - u.row0);
+  row_range(p, v, u.row0 / p.group, &u.any_lo, &u.all_hi);
+  row_range(p, v, (u.row0 + u.live - 1) / p.group, &u.all_lo, &u.any_hi);
   const int tile0 = v.hi > v.lo ? v.lo / kTile : 0;
   u.t_first = u.t_last = 0;
   if (u.any_hi > u.any_lo) {
     u.t_first = max(tile0 + u.ta, u.any_lo / kTile);
     u.t_last = max(u.t_first, min(tile0 + u.tb, (u.any_hi + kTile - 1) / kTile));
   }
-  k.w = u.w0 + u.tb;
   return true;
 }
 
@@ -190,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     block_attn_rows_kernel(const __grid_constant__ BlockAttnParams p, const __grid_constant__ CUtensorMap kmap,
                            const __grid_constant__ CUtensorMap vmap) {
   using C = Cfg<HD, ROWS>;
-  constexpr int kST = C::kStages;
+  constexpr int kKs = C::kKs, kVs = C::kVs;
   extern __shared__ __align__(1024) uint8_t raw[];
   Smem<HD, ROWS>& sm = *reinterpret_cast<Smem<HD, ROWS>*>(raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -213,18 +245,19 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     if (lane == 31 && warp < 4) sm.scan[warp] = incl;
     if (tid == kSoft) {
       sm.gave_up = 0;
-      for (int i = 0; i < kST; ++i) {
+      for (int i = 0; i < kKs; ++i) {
         mbar_init(&sm.k_full[i], 1);
         mbar_init(&sm.k_empty[i], 1);
+      }
+      for (int i = 0; i < kVs; ++i) {
         mbar_init(&sm.v_full[i], 1);
         mbar_init(&sm.v_empty[i], 1);
       }
       mbar_init(&sm.q_full, 4);
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&sm.s_full[i], 1);
-        mbar_init(&sm.p_full[i], 4);
-        mbar_init(&sm.o_full[i], 1);
-      }
+      mbar_init(&sm.s_full[0], 1);
+      mbar_init(&sm.s_full[1], 1);
+      mbar_init(&sm.p_full, 4);
+      mbar_init(&sm.o_full, 1);
       mbar_init(&sm.spare, 1);
       mbar_init_fence();
     }
@@ -242,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     if (warp < 4 && incl - mine <= walk.w && walk.w < incl) {
       int64_t base = incl - mine;
       for (int s = s0; s < s1; ++s) {
-        const int64_t w = seq_work<ROWS>(p, seq_view(p, s));
+        const int64_t w = seq_work<ROWS>(p, seq_view(p, s));  // zero for a sequence without rows
         if (walk.w < base + w) {
           sm.begin_seq = s;
           sm.begin_base = base;
@@ -260,30 +293,42 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  walk.seq = sm.begin_seq;
-  walk.base = sm.begin_base;
+  begin_walk<ROWS>(p, walk, sm.begin_seq, sm.begin_base);
   const int64_t w_begin = walk.w;
   volatile int* gave_up = &sm.gave_up;
   const int bs = 1 << p.bs_log2;
   Unit u;
+  auto block_of = [&](int64_t w) {
+    return (w >> 32) == 0 && (chunk >> 32) == 0 ? static_cast<uint32_t>(w) / static_cast<uint32_t>(chunk) : w / chunk;
+  };
 
   if (warp < 4) {
     // ---- softmax ----------------------------------------------------------------
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     const int piece = tid >> 4;  // 16-token piece of this thread's token
-    uint32_t it = 0;
+    uint32_t it = 0, tiles_done = 0;  // steps and tiles before this unit
     bool ok = true;
     while (next_unit<ROWS>(p, walk, u)) {
       const int n = u.t_last - u.t_first;
+      const int steps = (n + C::kStep - 1) / C::kStep;
+      // a row's threads are neighbours
+      constexpr int kPer = HD * ROWS / kSoft;  // values of a thread
+      constexpr int kRowThreads = kSoft / ROWS;
+      const int r = tid / kRowThreads, d0 = tid % kRowThreads * kPer;
+      const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) - i * p.group;
+      if (d0 == 0) {
+        int lo = 0, hi = 0;
+        if (r < u.live) row_range(p, u.v, i, &lo, &hi);
+        sm.row_lo[r] = lo;
+        sm.row_hi[r] = hi;
+        sm.row_out[r] = (u.v.first + i) * p.o_sr + j * p.o_sh;
+        sm.row_lse[r] = static_cast<int64_t>(u.v.first + i) * p.nh * p.group + j;
+      }
       if (n > 0) {
-        // rows of q: three 8-bit terms each; a row's threads are neighbours
-        constexpr int kPer = HD * ROWS / kSoft;  // values of a thread
-        constexpr int kRowThreads = kSoft / ROWS;
-        const int r = tid / kRowThreads, d0 = tid % kRowThreads * kPer;
+        // rows of q: three 8-bit terms each
         uint32_t w[kPer / 2];
 #pragma unroll
         for (int e = 0; e < kPer / 2; ++e) w[e] = 0;
-        const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) % p.group;
         if (r < u.live) {
           const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (u.v.first + i) * p.q_sr + j * p.q_sh + d0;
 #pragma unroll
@@ -341,13 +386,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             *reinterpret_cast<uint32_t*>(sm.q + (col >> 3) * (HD * 8) + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = t[z];
           }
         }
-        if (d0 == 0) {
-          sm.row_scale[r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
-          int lo = 0, hi = 0;
-          if (r < u.live) row_range(p, u.v, i, &lo, &hi);
-          sm.row_lo[r] = lo;
-          sm.row_hi[r] = hi;
-        }
+        if (d0 == 0) sm.row_scale[r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
         fence_async_shared();
         tc_fence_before();
         __syncwarp();
@@ -355,231 +394,252 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         soft_sync();
       }
 
-      float acc[C::kParts][ROWS], m[ROWS], l[ROWS], keep[ROWS], gain[ROWS];
+      float acc[C::kParts][ROWS], m[ROWS], l[ROWS], gain[ROWS];
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
+      for (int z = 0; z < ROWS; ++z) {
 #pragma unroll
-        for (int h = 0; h < C::kParts; ++h) acc[h][r] = 0.f;
-        m[r] = -INFINITY;
-        l[r] = 0.f;
-        keep[r] = gain[r] = 0.f;
+        for (int h = 0; h < C::kParts; ++h) acc[h][z] = 0.f;
+        m[z] = -INFINITY;
+        l[z] = 0.f;
+        gain[z] = 0.f;
       }
-      // the product with V of tile x joins the sums
+      // the product with V of step x joins the sums
       auto collect = [&](uint32_t x) {
-        if (!mbar_wait_warp(&sm.o_full[x & 1], (x >> 1) & 1, gave_up)) return false;
+        if (!mbar_wait_warp(&sm.o_full, x & 1, gave_up)) return false;
         if (HD == 64 && warp >= 2) return true;
         tc_fence_after();
 #pragma unroll
         for (int h = 0; h < C::kParts; ++h) {
           uint32_t o[4][ROWS];
-          const uint32_t at = tmem + lanes + 2 * C::kN + (2 * h + (x & 1)) * C::kN;
+          const uint32_t at = tmem + lanes + C::kOut + h * C::kN;
 #pragma unroll
           for (int z = 0; z < 4; ++z) tmem_ld(at + z * ROWS, o[z]);
 #pragma unroll
           for (int z = 0; z < 4; ++z) tmem_wait(o[z]);
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            const uint32_t t[4] = {o[0][r], o[1][r], o[2][r], o[3][r]};
-            acc[h][r] = acc[h][r] * keep[r] + join_terms<CODE>(t) * gain[r];
+          for (int z = 0; z < ROWS; ++z) {
+            const uint32_t t[4] = {o[0][z], o[1][z], o[2][z], o[3][z]};
+            acc[h][z] += join_terms<CODE>(t) * gain[z];
           }
         }
         return true;
       };
       // A warp that gave up goes through the same barriers as the others, without waiting for anything else.
-      for (int t = 0; t < n; ++t) {
-        const uint32_t x = it + t;
+      for (int t = 0; t < steps; ++t) {
+        const uint32_t x = it + t, tile = tiles_done + t * C::kStep;
+        const int count = min(C::kStep, n - t * C::kStep);  // tiles of this step
         ok = ok && mbar_wait_warp(&sm.s_full[x & 1], (x >> 1) & 1, gave_up);
         tc_fence_after();
-        float s[ROWS];
-        {
+        float s[C::kStep][ROWS];
+        float top[ROWS], vtop = 0.f, vs[C::kStep];
+        const int tok0 = (u.t_first + t * C::kStep) * kTile;
+#pragma unroll
+        for (int y = 0; y < C::kStep; ++y) {
           uint32_t o[3][ROWS];
-          const uint32_t at = tmem + lanes + (x & 1) * C::kN;
+          const uint32_t at = tmem + lanes + C::kScores + ((x & 1) * C::kStep + y) * C::kN;
 #pragma unroll
           for (int z = 0; z < 3; ++z) tmem_ld(at + z * ROWS, o[z]);
 #pragma unroll
           for (int z = 0; z < 3; ++z) tmem_wait(o[z]);
-          const float ks = sm.ks[x & 7][piece];
+          const uint32_t k = (tile + y) & 15;
+          const float ks = sm.ks[k][piece];
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r) {
-            const uint32_t t[3] = {o[0][r], o[1][r], o[2][r]};
-            s[r] = join_terms<CODE>(t) * (sm.row_scale[r] * ks);
+          for (int z = 0; z < ROWS; ++z) {
+            const uint32_t t3[3] = {o[0][z], o[1][z], o[2][z]};
+            s[y][z] = join_terms<CODE>(t3) * (sm.row_scale[z] * ks);
+          }
+          vs[y] = sm.vs[k][piece];
+          const int tk = tok0 + y * kTile;
+          const uint32_t have = y < count ? sm.have[k] : 0u;
+          if (tk < u.all_lo || tk + kTile > u.all_hi || have != 0xffu) {
+            const bool there = (have >> piece) & 1;
+            if (!there) vs[y] = 0.f;
+#pragma unroll
+            for (int z = 0; z < ROWS; ++z)
+              if (!there || tk + tid < sm.row_lo[z] || tk + tid >= sm.row_hi[z]) s[y][z] = -INFINITY;
+          }
+          if (y < count) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) vtop = fmaxf(vtop, fabsf(sm.vs[k][c]));
           }
         }
-        const int tok0 = (u.t_first + t) * kTile;
-        const uint32_t have = sm.have[x & 7];
-        if (tok0 < u.all_lo || tok0 + kTile > u.all_hi || have != 0xffu) {
-          const bool there = (have >> piece) & 1;
 #pragma unroll
-          for (int r = 0; r < ROWS; ++r)
-            if (!there || tok0 + tid < sm.row_lo[r] || tok0 + tid >= sm.row_hi[r]) s[r] = -INFINITY;
-        }
-        float top[ROWS];
-#pragma unroll
-        for (int r = 0; r < ROWS; ++r) top[r] = warp_max(s[r]);
+        for (int z = 0; z < ROWS; ++z) top[z] = warp_max(C::kStep == 2 ? fmaxf(s[0][z], s[C::kStep - 1][z]) : s[0][z]);
         if (lane == 0) {
 #pragma unroll
-          for (int r = 0; r < ROWS; r += 4)
-            *reinterpret_cast<float4*>(&sm.wmax[x & 1][warp][r]) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
+          for (int z = 0; z < ROWS; z += 4)
+            *reinterpret_cast<float4*>(&sm.wmax[x & 1][warp][z]) = make_float4(top[z], top[z + 1], top[z + 2], top[z + 3]);
         }
         soft_sync();
 #pragma unroll
         for (int w = 0; w < 4; ++w)
 #pragma unroll
-          for (int r = 0; r < ROWS; r += 4) {
-            const float4 o = *reinterpret_cast<const float4*>(&sm.wmax[x & 1][w][r]);
-            top[r] = fmaxf(top[r], o.x);
-            top[r + 1] = fmaxf(top[r + 1], o.y);
-            top[r + 2] = fmaxf(top[r + 2], o.z);
-            top[r + 3] = fmaxf(top[r + 3], o.w);
+          for (int z = 0; z < ROWS; z += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(&sm.wmax[x & 1][w][z]);
+            top[z] = fmaxf(top[z], o.x);
+            top[z + 1] = fmaxf(top[z + 1], o.y);
+            top[z + 2] = fmaxf(top[z + 2], o.z);
+            top[z + 3] = fmaxf(top[z + 3], o.w);
           }
-        const float vs = sm.vs[x & 7][piece];
-        float vtop = 0.f;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) vtop = fmaxf(vtop, fabsf(sm.vs[x & 7][c]));
         constexpr float kFull = CODE == MAK_CODE_INT8 ? 127.f * 16777216.f : 256.f;
-        const float weight = vtop > 0.f ? vs / vtop * kFull : 0.f;
-        // the tile before this one, whose factors are still in keep / gain
+        const float weight = vtop > 0.f ? kFull / vtop : 0.f;
+        // The step before: its product also is the last reader of the weights' place.
         if (t > 0) ok = ok && collect(x - 1);
-        uint8_t* dst = sm.p[x & 1] + piece * 128 + (tid & 15);
+        uint8_t* dst = sm.p + piece * 128 + (tid & 15);
 #pragma unroll
-        for (int r = 0; r < ROWS; r += 2) {
-          float y[2];
+        for (int z = 0; z < ROWS; z += 2) {
+          float w[C::kStep][2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mt = top[r + e], mn = fmaxf(m[r + e], mt);
-            const float ms = mn == -INFINITY ? 0.f : mn;
-            const float old = exp2_fast(m[r + e] - ms), add = exp2_fast(mt - ms);
-            const float w = exp2_fast(s[r + e] - (mt == -INFINITY ? 0.f : mt));
-            l[r + e] = l[r + e] * old + w * add;
-            keep[r + e] = old;
-            gain[r + e] = add * vtop * (1.f / kFull);
-            m[r + e] = mn;
-            y[e] = w * weight;
-          }
-          if constexpr (CODE == MAK_CODE_INT8) {
+            const float mt = top[z + e], mn = fmaxf(m[z + e], mt);
+            const float ms = mn == -INFINITY ? 0.f : mn, mz = mt == -INFINITY ? 0.f : mt;
+            const float old = exp2_fast(m[z + e] - ms), add = exp2_fast(mt - ms);
+            float sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t v = split_int8(y[e]);
-#pragma unroll
-              for (int z = 0; z < 4; ++z) {
-                const int col = z * ROWS + r + e;
-                dst[(col >> 3) * 1024 + (col & 7) * 16] = static_cast<uint8_t>(v >> (8 * (3 - z)));
-              }
+            for (int y = 0; y < C::kStep; ++y) {
+              w[y][e] = exp2_fast(s[y][z + e] - mz);
+              sum += w[y][e];
+              w[y][e] *= vs[y] * weight;
             }
-          } else {
-            uint32_t v[4];
-            split_e4m3(y[0], y[1], v);
+            l[z + e] = l[z + e] * old + sum * add;
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              const int col = z * ROWS + r;
-              dst[(col >> 3) * 1024 + (col & 7) * 16] = static_cast<uint8_t>(v[z]);
-              dst[((col + 1) >> 3) * 1024 + ((col + 1) & 7) * 16] = static_cast<uint8_t>(v[z] >> 8);
+            for (int h = 0; h < C::kParts; ++h) acc[h][z + e] *= old;
+            gain[z + e] = add * vtop * (1.f / kFull);
+            m[z + e] = mn;
+          }
+#pragma unroll
+          for (int y = 0; y < C::kStep; ++y) {
+            // column (term, row), token: 8 columns x 16 tokens are 128 bytes
+            uint8_t* to = dst + y * 1024;
+            if constexpr (CODE == MAK_CODE_INT8) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t v = split_int8(w[y][e]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const int col = c * ROWS + z + e;
+                  to[(col >> 3) * (1024 * C::kStep) + (col & 7) * 16] = static_cast<uint8_t>(v >> (8 * (3 - c)));
+                }
+              }
+            } else {
+              uint32_t v[4];
+              split_e4m3(w[y][0], w[y][1], v);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const int col = c * ROWS + z;
+                to[(col >> 3) * (1024 * C::kStep) + (col & 7) * 16] = static_cast<uint8_t>(v[c]);
+                to[((col + 1) >> 3) * (1024 * C::kStep) + ((col + 1) & 7) * 16] = static_cast<uint8_t>(v[c] >> 8);
+              }
             }
           }
         }
         // E4M3: codes that no row sees may be NaN, which a weight of zero does not cancel
-        if (CODE == MAK_CODE_E4M3 && (tok0 < u.any_lo || tok0 + kTile > u.any_hi || have != 0xffu)) {
-          const uint32_t slot = x % kST;
-          ok = ok && mbar_wait_warp(&sm.v_full[slot], (x / kST) & 1, gave_up);
-          for (int d = tid; d < HD; d += kSoft)
-            for (int c = 0; c < 8; ++c) {
-              const int ct = tok0 + 16 * c;
-              const bool there = (have >> c) & 1;
-              if (there && ct >= u.any_lo && ct + 16 <= u.any_hi) continue;
-              const int per_line = bs >> 4;  // 16-byte pieces of a line
-              const int swz = p.bs_log2 == 7 ? d & 7 : p.bs_log2 == 6 ? (d >> 1) & 3 : p.bs_log2 == 5 ? (d >> 2) & 1 : 0;
-              uint4* at = reinterpret_cast<uint4*>(sm.v[slot] + (c / per_line) * (HD * bs) + d * bs + (((c % per_line) ^ swz) << 4));
-              uint4 v = *at;
-              uint32_t* words = &v.x;
+        if (CODE == MAK_CODE_E4M3) {
+          for (int y = 0; y < count; ++y) {
+            const int tk = tok0 + y * kTile;
+            const uint32_t have = sm.have[(tile + y) & 15];
+            if (tk >= u.any_lo && tk + kTile <= u.any_hi && have == 0xffu) continue;
+            const uint32_t slot = (tile + y) % kVs;
+            ok = ok && mbar_wait_warp(&sm.v_full[slot], ((tile + y) / kVs) & 1, gave_up);
+            for (int d = tid; d < HD; d += kSoft)
+              for (int c = 0; c < 8; ++c) {
+                const int ct = tk + 16 * c;
+                const bool there = (have >> c) & 1;
+                if (there && ct >= u.any_lo && ct + 16 <= u.any_hi) continue;
+                const int per_line = bs >> 4;  // 16-byte pieces of a line
+                const int swz = p.bs_log2 == 7 ? d & 7 : p.bs_log2 == 6 ? (d >> 1) & 3 : p.bs_log2 == 5 ? (d >> 2) & 1 : 0;
+                uint4* at = reinterpret_cast<uint4*>(sm.v[slot] + (c / per_line) * (HD * bs) + d * bs + (((c % per_line) ^ swz) << 4));
+                uint4 v = *at;
+                uint32_t* words = &v.x;
 #pragma unroll
-              for (int b = 0; b < 4; ++b) {
-                uint32_t mask = 0;
+                for (int b = 0; b < 4; ++b) {
+                  uint32_t mask = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (there && ct + 4 * b + e >= u.any_lo && ct + 4 * b + e < u.any_hi) mask |= 0xffu << (8 * e);
-                words[b] &= mask;
+                  for (int e = 0; e < 4; ++e)
+                    if (there && ct + 4 * b + e >= u.any_lo && ct + 4 * b + e < u.any_hi) mask |= 0xffu << (8 * e);
+                  words[b] &= mask;
+                }
+                *at = v;
               }
-              *at = v;
-            }
+          }
         }
         fence_async_shared();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.p_full[x & 1]);
+        if (lane == 0) mbar_arrive(&sm.p_full);
       }
-      if (ok && n > 0) ok = collect(it + n - 1);
-      it += n;
+      if (ok && n > 0) ok = collect(it + steps - 1);
+      it += steps;
+      tiles_done += n;
 
       // ---- this block's share of the unit -----------------------------------------
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
+      for (int z = 0; z < ROWS; ++z) {
         if (!ok) {  // a block that gave up leaves NaN, not stale memory
-          l[r] = __uint_as_float(0x7fffffffu);
-          m[r] = 0.f;
+          l[z] = __uint_as_float(0x7fffffffu);
+          m[z] = 0.f;
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
-        if (lane == 0) sm.lsum[warp][r] = l[r];
+        for (int o = 16; o > 0; o >>= 1) l[z] += __shfl_xor_sync(0xffffffffu, l[z], o);
+        if (lane == 0) sm.lsum[warp][z] = l[z];
       }
       soft_sync();
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) l[r] = sm.lsum[0][r] + sm.lsum[1][r] + sm.lsum[2][r] + sm.lsum[3][r];
-      auto put = [&](int r, int d, float y) {
-        const int row = u.row0 + r;
-        const int64_t at = (u.v.first + row / p.group) * p.o_sr + (u.head * p.group + row % p.group) * p.o_sh + d;
+      for (int z = 0; z < ROWS; ++z) l[z] = sm.lsum[0][z] + sm.lsum[1][z] + sm.lsum[2][z] + sm.lsum[3][z];
+      auto put = [&](int z, int d, float y) {
+        const int64_t at = sm.row_out[z] + d;
         if (p.q_bf16)
           reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
         else
           reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(y);
       };
-      auto put_lse = [&](int r, float mx, float sum) {
-        const int row = u.row0 + r;
+      auto put_lse = [&](int z, float mx, float sum) {
         if (p.lse != nullptr)
-          p.lse[static_cast<int64_t>(u.v.first + row / p.group) * p.nh * p.group + u.head * p.group + row % p.group] =
-              sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+          p.lse[sm.row_lse[z]] = sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
       };
-      constexpr int kStep = ROWS * (HD + 2);  // floats of one partial sum
+      constexpr int kFloats = ROWS * (HD + 2);  // of one partial sum
       if (u.ta == 0 && u.tb == u.tiles) {
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
-          if (r < u.live) {
-            const float inv = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;
+        for (int z = 0; z < ROWS; ++z) {
+          if (z < u.live) {
+            const float inv = l[z] > 0.f || l[z] != l[z] ? 1.f / l[z] : 0.f;
 #pragma unroll
             for (int h = 0; h < C::kParts; ++h)
-              if (HD >= 128 || tid < HD) put(r, h * 128 + tid, acc[h][r] * inv);
-            if (tid == 0) put_lse(r, m[r], l[r]);
+              if (HD >= 128 || tid < HD) put(z, h * 128 + tid, acc[h][z] * inv);
+            if (tid == z) put_lse(z, m[z], l[z]);
           }
         }
-        soft_sync();  // lsum is read
       } else {
-        float* part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (u.w0 > w_begin ? 1 : 0)) * kStep;
+        float* part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (u.w_tiles > w_begin ? 1 : 0)) * kFloats;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) {
+        for (int z = 0; z < ROWS; ++z) {
 #pragma unroll
           for (int h = 0; h < C::kParts; ++h)
-            if (HD >= 128 || tid < HD) part[r * HD + h * 128 + tid] = acc[h][r];
-          if (tid == 0) {
-            part[ROWS * HD + r] = m[r];
-            part[ROWS * HD + ROWS + r] = l[r];
+            if (HD >= 128 || tid < HD) part[z * HD + h * 128 + tid] = acc[h][z];
+          if (tid == z) {
+            part[ROWS * HD + z] = m[z];
+            part[ROWS * HD + ROWS + z] = l[z];
           }
         }
-        __threadfence();
+        const int first_block = static_cast<int>(block_of(u.w_tiles)), last_block = static_cast<int>(block_of(u.w_tiles + u.tiles - 1));
+        const int slot0 = 2 * first_block + (u.w_tiles > first_block * chunk ? 1 : 0);
         soft_sync();
-        const int first_block = static_cast<int>(u.w0 / chunk), last_block = static_cast<int>((u.w0 + u.tiles - 1) / chunk);
-        const int slot0 = 2 * first_block + (u.w0 > first_block * chunk ? 1 : 0);
-        if (tid == 0) sm.last = atomicAdd(p.counters + slot0, 1) == last_block - first_block;
+        if (tid == 0) {
+          __threadfence();
+          sm.last = atomicAdd(p.counters + slot0, 1) == last_block - first_block;
+          __threadfence();
+        }
         soft_sync();
         if (sm.last) {
-          __threadfence();
           for (int idx = tid; idx < u.live * (HD / 4); idx += kSoft) {
-            const int r = idx / (HD / 4), d = idx % (HD / 4) * 4;
+            const int z = idx / (HD / 4), d = idx % (HD / 4) * 4;
             float mx = -INFINITY, sum = 0.f;
             float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
             for (int b = first_block; b <= last_block; ++b) {
-              const float* src = p.partial + (2 * static_cast<int64_t>(b) + (u.w0 > b * chunk ? 1 : 0)) * kStep;
-              const float pm = __ldcg(src + ROWS * HD + r), pl = __ldcg(src + ROWS * HD + ROWS + r);
-              const float4 po = __ldcg(reinterpret_cast<const float4*>(src + r * HD + d));
+              const float* src = p.partial + (2 * static_cast<int64_t>(b) + (u.w_tiles > b * chunk ? 1 : 0)) * kFloats;
+              const float pm = __ldcg(src + ROWS * HD + z), pl = __ldcg(src + ROWS * HD + ROWS + z);
+              const float4 po = __ldcg(reinterpret_cast<const float4*>(src + z * HD + d));
               const float mn = fmaxf(mx, pm);
               const float ms = mn == -INFINITY ? 0.f : mn;
               const float k0 = exp2_fast(mx - ms), k1 = exp2_fast(pm - ms);
@@ -592,12 +652,13 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             }
             const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) put(r, d + e, o[e] * inv);
-            if (d == 0) put_lse(r, mx, sum);
+            for (int e = 0; e < 4; ++e) put(z, d + e, o[e] * inv);
+            if (d == 0) put_lse(z, mx, sum);
           }
           if (tid == 0) p.counters[slot0] = 0;
         }
       }
+      soft_sync();  // the rows' places and sums are read
     }
   } else if (warp == 4) {
     // ---- copies: block ids and scales for four tiles at a time, a lane per 16 tokens ---------
@@ -608,7 +669,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     struct Batch {
       int count, head, page;
       float ks, vs;
-      const uint8_t *k, *v;
     } next;
     int gt = 0;
     u.t_last = 0;
@@ -630,57 +690,81 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       if (next.page >= 0) {
         next.ks = __ldg(p.key_scale + next.page * p.ks_sb + next.head * p.ks_sh);
         next.vs = __ldg(p.value_scale + next.page * p.vs_sb + next.head * p.vs_sh);
-        next.k = p.key + next.page * p.k_sb + next.head * p.k_sh;
-        next.v = p.value + next.page * p.v_sb + next.head * p.v_sh;
       }
       gt += next.count;
     };
     look_ahead();
-    uint32_t it = 0, slot = 0, parity = 1, k_sent = 0, v_sent = 0;
-    bool ok = true;
-    while (next.count > 0 && ok) {
-      const Batch b = next;
-      const uint32_t there = __ballot_sync(0xffffffffu, b.page >= 0);
-      const uint32_t led = __ballot_sync(0xffffffffu, b.page >= 0 && leads);
-      for (int j = 0; j < b.count; ++j, ++it) {
-        const bool issue = mine == j && b.page >= 0 && leads;
-        const uint32_t expect = __popc((led >> (8 * j)) & 0xffu) * bytes;
-        ok = mbar_wait_warp(&sm.k_empty[slot], parity, gave_up);
-        if (!ok) break;
-        if (issue) {
+    Batch b = next;
+    next.count = 0;
+    bool looked = false;
+    uint32_t k_sent = 0, v_sent = 0, k_slot = 0, k_parity = 1, v_slot = 0, v_parity = 1, idle = 0;
+    int j = 0;
+    // K of tile k_sent and V of tile v_sent, whichever has room; V's blocks are read back from shared memory
+    while (b.count > 0 || v_sent < k_sent) {
+      bool did = false;
+      if (b.count > 0 && k_sent - v_sent < 12 && __all_sync(0xffffffffu, mbar_try(&sm.k_empty[k_slot], k_parity))) {
+        const uint32_t ring = k_sent & 15;
+        const bool on = mine == j && b.page >= 0;
+        const uint32_t there = __ballot_sync(0xffffffffu, on), led = __ballot_sync(0xffffffffu, on && leads);
+        if (on && leads) {
           if (p.bs_log2 == 4)
-            bulk_load(k_to + slot * C::kTileBytes, b.k, bytes, &sm.k_full[slot]);
+            bulk_load(k_to + k_slot * C::kTileBytes, p.key + b.page * p.k_sb + b.head * p.k_sh, bytes, &sm.k_full[k_slot]);
           else
-            tensor_load(k_to + slot * C::kTileBytes, &kmap, b.head, b.page, &sm.k_full[slot]);
+            tensor_load(k_to + k_slot * C::kTileBytes, &kmap, b.head, b.page, &sm.k_full[k_slot]);
         }
         if (mine == j) {
-          sm.ks[it & 7][piece] = b.ks;
-          sm.vs[it & 7][piece] = b.vs;
-          if (piece == 0) sm.have[it & 7] = (there >> (8 * j)) & 0xffu;
+          sm.ks[ring][piece] = b.ks;
+          sm.vs[ring][piece] = b.vs;
+          sm.page[ring][piece] = b.page;
+          if (piece == 0) {
+            sm.have[ring] = there >> (8 * j);
+            sm.head[ring] = b.head;
+          }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect(&sm.k_full[slot], expect);
+        if (lane == 0) mbar_arrive_expect(&sm.k_full[k_slot], __popc(led) * bytes);
         ++k_sent;
-        if (j == 0) look_ahead();
-        ok = mbar_wait_warp(&sm.v_empty[slot], parity, gave_up);
-        if (!ok) break;
-        if (issue) {
-          if (p.bs_log2 == 4)
-            bulk_load(v_to + slot * C::kTileBytes, b.v, bytes, &sm.v_full[slot]);
-          else
-            tensor_load(v_to + slot * C::kTileBytes, &vmap, b.head, b.page, &sm.v_full[slot]);
+        if (++k_slot == kKs) k_slot = 0, k_parity ^= 1;
+        if (!looked) {
+          look_ahead();
+          looked = true;
         }
-        if (lane == 0) mbar_arrive_expect(&sm.v_full[slot], expect);
+        if (++j == b.count) {
+          b = next;
+          j = 0;
+          looked = false;
+        }
+        did = true;
+      }
+      if (v_sent < k_sent && __all_sync(0xffffffffu, mbar_try(&sm.v_empty[v_slot], v_parity))) {
+        const uint32_t ring = v_sent & 15;
+        const int page = lane < 8 && leads ? sm.page[ring][piece] : -1, head = sm.head[ring];
+        const uint32_t led = __ballot_sync(0xffffffffu, page >= 0);
+        if (page >= 0) {
+          if (p.bs_log2 == 4)
+            bulk_load(v_to + v_slot * C::kTileBytes, p.value + page * p.v_sb + head * p.v_sh, bytes, &sm.v_full[v_slot]);
+          else
+            tensor_load(v_to + v_slot * C::kTileBytes, &vmap, head, page, &sm.v_full[v_slot]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect(&sm.v_full[v_slot], __popc(led) * bytes);
         ++v_sent;
-        if (++slot == kST) slot = 0, parity ^= 1;
+        if (++v_slot == kVs) v_slot = 0, v_parity ^= 1;
+        did = true;
+      }
+      if (did) {
+        idle = 0;
+      } else if (++idle >= kWaitLimit || __any_sync(0xffffffffu, (idle & 255) == 255 && *gave_up)) {
+        *gave_up = 1;
+        break;
       }
     }
     // copies in flight end before the block does
-    for (uint32_t i = k_sent > kST ? k_sent - kST : 0; i < k_sent; ++i)
-      for (uint32_t z = 0; z < kWaitLimit && !mbar_try(&sm.k_full[i % kST], (i / kST) & 1); ++z) {
+    for (uint32_t i = k_sent > kKs ? k_sent - kKs : 0; i < k_sent; ++i)
+      for (uint32_t z = 0; z < kWaitLimit && !mbar_try(&sm.k_full[i % kKs], (i / kKs) & 1); ++z) {
       }
-    for (uint32_t i = v_sent > kST ? v_sent - kST : 0; i < v_sent; ++i)
-      for (uint32_t z = 0; z < kWaitLimit && !mbar_try(&sm.v_full[i % kST], (i / kST) & 1); ++z) {
+    for (uint32_t i = v_sent > kVs ? v_sent - kVs : 0; i < v_sent; ++i)
+      for (uint32_t z = 0; z < kWaitLimit && !mbar_try(&sm.v_full[i % kVs], (i / kVs) & 1); ++z) {
       }
   } else if (lane == 0) {
     // ---- the tensor cores ---------------------------------------------------------
@@ -698,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     };
     // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
     const uint64_t k_desc = smem_desc(smem_addr(sm.k), k_lbo, k_sbo, line), q_desc = smem_desc(smem_addr(sm.q), 128, HD * 8, 0);
-    const uint64_t v_desc = smem_desc(smem_addr(sm.v), v_lbo, v_sbo, line), p_desc = smem_desc(smem_addr(sm.p), 128, 1024, 0);
+    const uint64_t v_desc = smem_desc(smem_addr(sm.v), v_lbo, v_sbo, line), p_desc = smem_desc(smem_addr(sm.p), 128, 1024 * C::kStep, 0);
     constexpr uint32_t kTileStep = C::kTileBytes / 16;
     uint32_t v_step[kTile / 32];  // 32 tokens of V each
 #pragma unroll
@@ -706,40 +790,50 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     uint32_t it = 0, units = 0;
     uint32_t k_slot = 0, k_parity = 0, v_slot = 0, v_parity = 0;
     bool ok = true;
-    auto scores = [&](uint32_t x) {
-      if (!mbar_wait(&sm.k_full[k_slot], k_parity, gave_up)) return false;
-      tc_fence_after();
-      const uint64_t kd = k_desc + k_slot * kTileStep;
+    // scores of step x, `count` tiles
+    auto scores = [&](uint32_t x, int count) {
+      for (int y = 0; y < count; ++y) {
+        if (!mbar_wait(&sm.k_full[k_slot], k_parity, gave_up)) return false;
+        tc_fence_after();
+        const uint64_t kd = k_desc + k_slot * kTileStep;
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) mma(tmem + (x & 1) * C::kN, kd + i * 2 * bs, q_desc + i * 16, kQk, i > 0);
+        for (int i = 0; i < HD / 32; ++i)
+          mma(tmem + C::kScores + ((x & 1) * C::kStep + y) * C::kN, kd + i * 2 * bs, q_desc + i * 16, kQk, i > 0);
+        tc_commit(&sm.k_empty[k_slot]);
+        if (++k_slot == kKs) k_slot = 0, k_parity ^= 1;
+      }
       tc_commit(&sm.s_full[x & 1]);
-      tc_commit(&sm.k_empty[k_slot]);
-      if (++k_slot == kST) k_slot = 0, k_parity ^= 1;
       return true;
     };
     while (ok && next_unit<ROWS>(p, walk, u)) {
       const int n = u.t_last - u.t_first;
       if (n == 0) continue;
+      const int steps = (n + C::kStep - 1) / C::kStep;
       ok = mbar_wait(&sm.q_full, units & 1, gave_up);
       ++units;
-      for (int t = 0; t < 2 && t < n && ok; ++t) ok = scores(it + t);
-      for (int t = 0; t < n && ok; ++t) {
+      for (int t = 0; t < 2 && t < steps && ok; ++t) ok = scores(it + t, min(C::kStep, n - t * C::kStep));
+      for (int t = 0; t < steps && ok; ++t) {
         const uint32_t x = it + t;
-        ok = mbar_wait(&sm.v_full[v_slot], v_parity, gave_up) && mbar_wait(&sm.p_full[x & 1], (x >> 1) & 1, gave_up);
+        const int count = min(C::kStep, n - t * C::kStep);
+        for (int y = 0; y < count && ok; ++y) {
+          ok = mbar_wait(&sm.v_full[v_slot], v_parity, gave_up);
+          if (y == 0) ok = ok && mbar_wait(&sm.p_full, x & 1, gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = v_desc + v_slot * kTileStep, pd = p_desc + y * 64;
+#pragma unroll
+          for (int h = 0; h < C::kParts; ++h)
+#pragma unroll
+            for (int i = 0; i < kTile / 32; ++i)
+              mma(tmem + C::kOut + h * C::kN, vd + h * 8 * bs + v_step[i], pd + i * 16, kPv, y > 0 || i > 0);
+          tc_commit(&sm.v_empty[v_slot]);
+          if (++v_slot == kVs) v_slot = 0, v_parity ^= 1;
+        }
         if (!ok) break;
-        tc_fence_after();
-        const uint64_t vd = v_desc + v_slot * kTileStep, pd = p_desc + (x & 1) * (C::kN * kTile / 16);
-#pragma unroll
-        for (int h = 0; h < C::kParts; ++h)
-#pragma unroll
-          for (int i = 0; i < kTile / 32; ++i)
-            mma(tmem + 2 * C::kN + (2 * h + (x & 1)) * C::kN, vd + h * 8 * bs + v_step[i], pd + i * 16, kPv, i > 0);
-        tc_commit(&sm.o_full[x & 1]);
-        tc_commit(&sm.v_empty[v_slot]);
-        if (++v_slot == kST) v_slot = 0, v_parity ^= 1;
-        if (t + 2 < n) ok = scores(x + 2);
+        tc_commit(&sm.o_full);
+        if (t + 2 < steps) ok = scores(x + 2, min(C::kStep, n - (t + 2) * C::kStep));
       }
-      it += n;
+      it += steps;
     }
     if (!ok) {  // let what was issued end before the TMEM is given back
       tc_commit(&sm.spare);
@@ -798,6 +892,8 @@ int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
       (void)cudaGetLastError();
       return cuda_fail(e, "mak_block_attention");
     }
+    // The occupancy query answers 1 for these kernels; two blocks do run where their shared memory,
+    // registers and TMEM columns fit twice (11.7 of 12 warps active on average).
     int n = HD == 256 ? 1 : 2;
     // TMEM has 512 columns, and a block whose allocation has to wait for another's end gains nothing
     if (n * Cfg<HD, ROWS>::kTmem > 512) n = 512 / Cfg<HD, ROWS>::kTmem;
@@ -811,7 +907,7 @@ int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
   int64_t grid = per_sm * sm_count();
   if (grid > kMaxGrid) grid = kMaxGrid;
   // no more blocks than there can be work for
-  const int64_t seq_tiles = ((static_cast<int64_t>(p.max_blocks) << p.bs_log2) + kTile - 1) / kTile + 1;
+  const int64_t seq_tiles = ((static_cast<int64_t>(p.max_blocks) << p.bs_log2) + kTile - 1) / kTile + 1 + kUnitCost;
   const int64_t groups = static_cast<int64_t>(p.num_rows) * p.group / ROWS + p.num_seqs;
   const int64_t most = (groups * p.nh * seq_tiles + kMinChunk - 1) / kMinChunk;
   if (most < grid) grid = most;
