@@ -69,14 +69,15 @@ struct Smem {
   alignas(1024) uint8_t v[C::kVs][C::kTileBytes];
   alignas(1024) uint8_t k[C::kKs][C::kTileBytes];
   alignas(1024) uint8_t p[C::kN * kTile * C::kStep];
-  uint8_t q[C::kN * HD];
+  // The products read four terms of q, of which there are three: what follows makes columns nobody reads.
+  uint8_t q[2][3 * ROWS * HD];  // of this unit and the next
   alignas(16) float ks[16][8], vs[16][8];  // scales per 16 tokens, tile number mod 16
   uint32_t have[16];                       // bit c: 16-token piece c has a block
   int page[16][8], head[16];               // for the copies of V, which follow those of K
   alignas(16) float wmax[2][4][ROWS];
-  alignas(16) float row_scale[ROWS];
-  int row_lo[ROWS], row_hi[ROWS];
-  alignas(8) int64_t row_out[ROWS], row_lse[ROWS];  // places of the results
+  alignas(16) float row_scale[2][ROWS];
+  int row_lo[2][ROWS], row_hi[2][ROWS];
+  alignas(8) int64_t row_out[2][ROWS], row_lse[2][ROWS];  // places of the results
   float lsum[4][ROWS];
   alignas(8) uint64_t k_full[C::kKs], k_empty[C::kKs], v_full[C::kVs], v_empty[C::kVs];
   uint64_t q_full, s_full[2], p_full, o_full, spare;
@@ -286,9 +287,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     }
   }
   if (warp == 5) tmem_alloc<C::kTmem>(&sm.tmem);
-  // q has no fourth term
-  for (int i = tid; i < ROWS * HD / 4; i += kThreads) reinterpret_cast<uint32_t*>(sm.q + 3 * ROWS * HD)[i] = 0;
-  fence_async_shared();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -308,10 +306,8 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     const int piece = tid >> 4;  // 16-token piece of this thread's token
     uint32_t it = 0, tiles_done = 0;  // steps and tiles before this unit
     bool ok = true;
-    while (next_unit<ROWS>(p, walk, u)) {
-      const int n = u.t_last - u.t_first;
-      const int steps = (n + C::kStep - 1) / C::kStep;
-      // a row's threads are neighbours
+    // Rows of a unit: their places, and q as three 8-bit terms.  A row's threads are neighbours.
+    auto stage = [&](const Unit& u, int buf) {
       constexpr int kPer = HD * ROWS / kSoft;  // values of a thread
       constexpr int kRowThreads = kSoft / ROWS;
       const int r = tid / kRowThreads, d0 = tid % kRowThreads * kPer;
@@ -319,13 +315,12 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       if (d0 == 0) {
         int lo = 0, hi = 0;
         if (r < u.live) row_range(p, u.v, i, &lo, &hi);
-        sm.row_lo[r] = lo;
-        sm.row_hi[r] = hi;
-        sm.row_out[r] = (u.v.first + i) * p.o_sr + j * p.o_sh;
-        sm.row_lse[r] = static_cast<int64_t>(u.v.first + i) * p.nh * p.group + j;
+        sm.row_lo[buf][r] = lo;
+        sm.row_hi[buf][r] = hi;
+        sm.row_out[buf][r] = (u.v.first + i) * p.o_sr + j * p.o_sh;
+        sm.row_lse[buf][r] = static_cast<int64_t>(u.v.first + i) * p.nh * p.group + j;
       }
-      if (n > 0) {
-        // rows of q: three 8-bit terms each
+      if (u.t_last > u.t_first) {
         uint32_t w[kPer / 2];
 #pragma unroll
         for (int e = 0; e < kPer / 2; ++e) w[e] = 0;
@@ -383,17 +378,81 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
 #pragma unroll
           for (int z = 0; z < 3; ++z) {
             const int col = z * ROWS + r, d = d0 + e;
-            *reinterpret_cast<uint32_t*>(sm.q + (col >> 3) * (HD * 8) + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = t[z];
+            *reinterpret_cast<uint32_t*>(sm.q[buf] + (col >> 3) * (HD * 8) + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = t[z];
           }
         }
-        if (d0 == 0) sm.row_scale[r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
+        if (d0 == 0) sm.row_scale[buf][r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
         fence_async_shared();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.q_full);
-        soft_sync();
       }
+    };
+    auto put = [&](int buf, int z, int d, float y) {
+      const int64_t at = sm.row_out[buf][z] + d;
+      if (p.q_bf16)
+        reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
+      else
+        reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(y);
+    };
+    auto put_lse = [&](int buf, int z, float mx, float sum) {
+      if (p.lse != nullptr)
+        p.lse[sm.row_lse[buf][z]] = sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+    };
+    constexpr int kFloats = ROWS * (HD + 2);  // of one partial sum
+    // A unit whose partial sum was left: the last of its blocks to get here joins them.  Whether this one
+    // is the last is asked for at once and looked at a unit later.
+    struct {
+      int first, last, slot, live, buf;
+      int64_t w_tiles;
+      int ticket;
+    } open;
+    open.first = -1;
+    auto close = [&]() {
+      if (open.first < 0) return;
+      if (tid == 0) {
+        sm.last = open.ticket == open.last - open.first;
+        __threadfence();
+      }
+      soft_sync();
+      if (sm.last) {
+        for (int idx = tid; idx < open.live * (HD / 4); idx += kSoft) {
+          const int z = idx / (HD / 4), d = idx % (HD / 4) * 4;
+          float mx = -INFINITY, sum = 0.f;
+          float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+          for (int b = open.first; b <= open.last; ++b) {
+            const float* src = p.partial + (2 * static_cast<int64_t>(b) + (open.w_tiles > b * chunk ? 1 : 0)) * kFloats;
+            const float pm = __ldcg(src + ROWS * HD + z), pl = __ldcg(src + ROWS * HD + ROWS + z);
+            const float4 po = __ldcg(reinterpret_cast<const float4*>(src + z * HD + d));
+            const float mn = fmaxf(mx, pm);
+            const float ms = mn == -INFINITY ? 0.f : mn;
+            const float k0 = exp2_fast(mx - ms), k1 = exp2_fast(pm - ms);
+            o[0] = o[0] * k0 + po.x * k1;
+            o[1] = o[1] * k0 + po.y * k1;
+            o[2] = o[2] * k0 + po.z * k1;
+            o[3] = o[3] * k0 + po.w * k1;
+            sum = sum * k0 + pl * k1;
+            mx = mn;
+          }
+          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) put(open.buf, z, d + e, o[e] * inv);
+          if (d == 0) put_lse(open.buf, z, mx, sum);
+        }
+        if (tid == 0) p.counters[open.slot] = 0;
+      }
+      open.first = -1;
+      soft_sync();
+    };
 
+    int buf = 0;
+    bool more = next_unit<ROWS>(p, walk, u);
+    if (more) stage(u, 0);
+    soft_sync();
+    while (more) {
+      const int n = u.t_last - u.t_first;
+      const int steps = (n + C::kStep - 1) / C::kStep;
       float acc[C::kParts][ROWS], m[ROWS], l[ROWS], gain[ROWS];
 #pragma unroll
       for (int z = 0; z < ROWS; ++z) {
@@ -446,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
 #pragma unroll
           for (int z = 0; z < ROWS; ++z) {
             const uint32_t t3[3] = {o[0][z], o[1][z], o[2][z]};
-            s[y][z] = join_terms<CODE>(t3) * (sm.row_scale[z] * ks);
+            s[y][z] = join_terms<CODE>(t3) * (sm.row_scale[buf][z] * ks);
           }
           vs[y] = sm.vs[k][piece];
           const int tk = tok0 + y * kTile;
@@ -456,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             if (!there) vs[y] = 0.f;
 #pragma unroll
             for (int z = 0; z < ROWS; ++z)
-              if (!there || tk + tid < sm.row_lo[z] || tk + tid >= sm.row_hi[z]) s[y][z] = -INFINITY;
+              if (!there || tk + tid < sm.row_lo[buf][z] || tk + tid >= sm.row_hi[buf][z]) s[y][z] = -INFINITY;
           }
           if (y < count) {
 #pragma unroll
@@ -485,53 +544,57 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         const float weight = vtop > 0.f ? kFull / vtop : 0.f;
         // The step before: its product also is the last reader of the weights' place.
         if (t > 0) ok = ok && collect(x - 1);
-        uint8_t* dst = sm.p + piece * 128 + (tid & 15);
+        uint32_t words[C::kStep][4][ROWS / 4];  // weights of this thread's tokens: term, four rows
 #pragma unroll
-        for (int z = 0; z < ROWS; z += 2) {
-          float w[C::kStep][2];
+        for (int z0 = 0; z0 < ROWS; z0 += 4) {
+          float w[C::kStep][4];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float mt = top[z + e], mn = fmaxf(m[z + e], mt);
+          for (int e = 0; e < 4; ++e) {
+            const int z = z0 + e;
+            const float mt = top[z], mn = fmaxf(m[z], mt);
             const float ms = mn == -INFINITY ? 0.f : mn, mz = mt == -INFINITY ? 0.f : mt;
-            const float old = exp2_fast(m[z + e] - ms), add = exp2_fast(mt - ms);
+            const float old = exp2_fast(m[z] - ms), add = exp2_fast(mt - ms);
             float sum = 0.f;
 #pragma unroll
             for (int y = 0; y < C::kStep; ++y) {
-              w[y][e] = exp2_fast(s[y][z + e] - mz);
+              w[y][e] = exp2_fast(s[y][z] - mz);
               sum += w[y][e];
               w[y][e] *= vs[y] * weight;
             }
-            l[z + e] = l[z + e] * old + sum * add;
+            l[z] = l[z] * old + sum * add;
 #pragma unroll
-            for (int h = 0; h < C::kParts; ++h) acc[h][z + e] *= old;
-            gain[z + e] = add * vtop * (1.f / kFull);
-            m[z + e] = mn;
+            for (int h = 0; h < C::kParts; ++h) acc[h][z] *= old;
+            gain[z] = add * vtop * (1.f / kFull);
+            m[z] = mn;
           }
 #pragma unroll
           for (int y = 0; y < C::kStep; ++y) {
-            // column (term, row), token: 8 columns x 16 tokens are 128 bytes
-            uint8_t* to = dst + y * 1024;
             if constexpr (CODE == MAK_CODE_INT8) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint32_t v = split_int8(w[y][e]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  const int col = c * ROWS + z + e;
-                  to[(col >> 3) * (1024 * C::kStep) + (col & 7) * 16] = static_cast<uint8_t>(v >> (8 * (3 - c)));
-                }
-              }
-            } else {
               uint32_t v[4];
-              split_e4m3(w[y][0], w[y][1], v);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = split_int8(w[y][e]);
 #pragma unroll
               for (int c = 0; c < 4; ++c) {
-                const int col = c * ROWS + z;
-                to[(col >> 3) * (1024 * C::kStep) + (col & 7) * 16] = static_cast<uint8_t>(v[c]);
-                to[((col + 1) >> 3) * (1024 * C::kStep) + ((col + 1) & 7) * 16] = static_cast<uint8_t>(v[c] >> 8);
+                const uint32_t pick = (3 - c) | ((7 - c) << 4);  // byte 3 - c of both
+                words[y][c][z0 / 4] = __byte_perm(__byte_perm(v[0], v[1], pick), __byte_perm(v[2], v[3], pick), 0x5410);
               }
+            } else {
+              uint32_t a[4], b[4];
+              split_e4m3(w[y][0], w[y][1], a);
+              split_e4m3(w[y][2], w[y][3], b);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) words[y][c][z0 / 4] = a[c] | (b[c] << 16);
             }
           }
+        }
+        // 16 columns of a token are 16 bytes, the next 16 a step's tokens further on
+#pragma unroll
+        for (int y = 0; y < C::kStep; ++y) {
+          const uint32_t* x4 = &words[y][0][0];
+#pragma unroll
+          for (int c = 0; c < ROWS / 4; ++c)
+            *reinterpret_cast<uint4*>(sm.p + (c * C::kStep * kTile + y * kTile + tid) * 16) =
+                make_uint4(x4[4 * c], x4[4 * c + 1], x4[4 * c + 2], x4[4 * c + 3]);
         }
         // E4M3: codes that no row sees may be NaN, which a weight of zero does not cancel
         if (CODE == MAK_CODE_E4M3) {
@@ -568,6 +631,11 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full);
       }
+      // The next unit's rows, so that the tensor cores begin on it while this one ends.
+      close();
+      const Unit done = u;
+      more = next_unit<ROWS>(p, walk, u);
+      if (more) stage(u, buf ^ 1);
       if (ok && n > 0) ok = collect(it + steps - 1);
       it += steps;
       tiles_done += n;
@@ -586,31 +654,20 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       soft_sync();
 #pragma unroll
       for (int z = 0; z < ROWS; ++z) l[z] = sm.lsum[0][z] + sm.lsum[1][z] + sm.lsum[2][z] + sm.lsum[3][z];
-      auto put = [&](int z, int d, float y) {
-        const int64_t at = sm.row_out[z] + d;
-        if (p.q_bf16)
-          reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(y);
-        else
-          reinterpret_cast<__half*>(p.out)[at] = __float2half_rn(y);
-      };
-      auto put_lse = [&](int z, float mx, float sum) {
-        if (p.lse != nullptr)
-          p.lse[sm.row_lse[z]] = sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
-      };
-      constexpr int kFloats = ROWS * (HD + 2);  // of one partial sum
-      if (u.ta == 0 && u.tb == u.tiles) {
+      if (done.ta == 0 && done.tb == done.tiles) {
 #pragma unroll
         for (int z = 0; z < ROWS; ++z) {
-          if (z < u.live) {
+          if (z < done.live) {
             const float inv = l[z] > 0.f || l[z] != l[z] ? 1.f / l[z] : 0.f;
 #pragma unroll
             for (int h = 0; h < C::kParts; ++h)
-              if (HD >= 128 || tid < HD) put(z, h * 128 + tid, acc[h][z] * inv);
-            if (tid == z) put_lse(z, m[z], l[z]);
+              if (HD >= 128 || tid < HD) put(buf, z, h * 128 + tid, acc[h][z] * inv);
+            if (tid == z) put_lse(buf, z, m[z], l[z]);
           }
         }
+        soft_sync();  // the rows' places and sums are read
       } else {
-        float* part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (u.w_tiles > w_begin ? 1 : 0)) * kFloats;
+        float* part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (done.w_tiles > w_begin ? 1 : 0)) * kFloats;
 #pragma unroll
         for (int z = 0; z < ROWS; ++z) {
 #pragma unroll
@@ -621,45 +678,21 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             part[ROWS * HD + ROWS + z] = l[z];
           }
         }
-        const int first_block = static_cast<int>(block_of(u.w_tiles)), last_block = static_cast<int>(block_of(u.w_tiles + u.tiles - 1));
-        const int slot0 = 2 * first_block + (u.w_tiles > first_block * chunk ? 1 : 0);
+        open.first = static_cast<int>(block_of(done.w_tiles));
+        open.last = static_cast<int>(block_of(done.w_tiles + done.tiles - 1));
+        open.slot = 2 * open.first + (done.w_tiles > open.first * chunk ? 1 : 0);
+        open.live = done.live;
+        open.buf = buf;
+        open.w_tiles = done.w_tiles;
         soft_sync();
         if (tid == 0) {
           __threadfence();
-          sm.last = atomicAdd(p.counters + slot0, 1) == last_block - first_block;
-          __threadfence();
-        }
-        soft_sync();
-        if (sm.last) {
-          for (int idx = tid; idx < u.live * (HD / 4); idx += kSoft) {
-            const int z = idx / (HD / 4), d = idx % (HD / 4) * 4;
-            float mx = -INFINITY, sum = 0.f;
-            float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-            for (int b = first_block; b <= last_block; ++b) {
-              const float* src = p.partial + (2 * static_cast<int64_t>(b) + (u.w_tiles > b * chunk ? 1 : 0)) * kFloats;
-              const float pm = __ldcg(src + ROWS * HD + z), pl = __ldcg(src + ROWS * HD + ROWS + z);
-              const float4 po = __ldcg(reinterpret_cast<const float4*>(src + z * HD + d));
-              const float mn = fmaxf(mx, pm);
-              const float ms = mn == -INFINITY ? 0.f : mn;
-              const float k0 = exp2_fast(mx - ms), k1 = exp2_fast(pm - ms);
-              o[0] = o[0] * k0 + po.x * k1;
-              o[1] = o[1] * k0 + po.y * k1;
-              o[2] = o[2] * k0 + po.z * k1;
-              o[3] = o[3] * k0 + po.w * k1;
-              sum = sum * k0 + pl * k1;
-              mx = mn;
-            }
-            const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) put(z, d + e, o[e] * inv);
-            if (d == 0) put_lse(z, mx, sum);
-          }
-          if (tid == 0) p.counters[slot0] = 0;
+          open.ticket = atomicAdd(p.counters + open.slot, 1);
         }
       }
-      soft_sync();  // the rows' places and sums are read
+      buf ^= 1;
     }
+    close();
   } else if (warp == 4) {
     // ---- copies: block ids and scales for four tiles at a time, a lane per 16 tokens ---------
     const int mine = lane >> 3, piece = lane & 7;
@@ -769,7 +802,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
   } else if (lane == 0) {
     // ---- the tensor cores ---------------------------------------------------------
     constexpr int kFmt = CODE == MAK_CODE_INT8 ? 1 : 0, kAcc = CODE == MAK_CODE_INT8 ? 2 : 1;
-    constexpr uint32_t kQk = instr_desc(C::kN, kAcc, kFmt, true, false), kPv = instr_desc(C::kN, kAcc, kFmt, false, false);
+    constexpr uint32_t kQk = instr_desc(C::kN, kAcc, kFmt, true, false), kPv = instr_desc(C::kN, kAcc, kFmt, false, true);
     const int line = p.bs_log2;
     // K: lines of 8 head_dim rows, then blocks; V: the same lines as rows of M
     const uint32_t k_lbo = line == 4 ? 128 : HD * bs, k_sbo = line == 4 ? HD * 16 : 8 * bs;
@@ -781,13 +814,16 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         mma_ss_f8(d, a, b, idesc, add);
     };
     // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
-    const uint64_t k_desc = smem_desc(smem_addr(sm.k), k_lbo, k_sbo, line), q_desc = smem_desc(smem_addr(sm.q), 128, HD * 8, 0);
-    const uint64_t v_desc = smem_desc(smem_addr(sm.v), v_lbo, v_sbo, line), p_desc = smem_desc(smem_addr(sm.p), 128, 1024 * C::kStep, 0);
+    const uint64_t k_desc = smem_desc(smem_addr(sm.k), k_lbo, k_sbo, line);
+    uint64_t q_desc = 0;
+    const uint64_t v_desc = smem_desc(smem_addr(sm.v), v_lbo, v_sbo, line);
+    const uint64_t p_desc = smem_desc(smem_addr(sm.p), 128, kTile * 16 * C::kStep, 0);
     constexpr uint32_t kTileStep = C::kTileBytes / 16;
     uint32_t v_step[kTile / 32];  // 32 tokens of V each
 #pragma unroll
     for (int i = 0; i < kTile / 32; ++i) v_step[i] = (((32 * i) >> line) * (HD * bs) + ((32 * i) & (bs - 1))) >> 4;
     uint32_t it = 0, units = 0;
+    int buf = 1;  // of q: unit by unit
     uint32_t k_slot = 0, k_parity = 0, v_slot = 0, v_parity = 0;
     bool ok = true;
     // scores of step x, `count` tiles
@@ -807,10 +843,12 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     };
     while (ok && next_unit<ROWS>(p, walk, u)) {
       const int n = u.t_last - u.t_first;
+      buf ^= 1;
       if (n == 0) continue;
       const int steps = (n + C::kStep - 1) / C::kStep;
       ok = mbar_wait(&sm.q_full, units & 1, gave_up);
       ++units;
+      q_desc = smem_desc(smem_addr(sm.q[buf]), 128, HD * 8, 0);
       for (int t = 0; t < 2 && t < steps && ok; ++t) ok = scores(it + t, min(C::kStep, n - t * C::kStep));
       for (int t = 0; t < steps && ok; ++t) {
         const uint32_t x = it + t;
@@ -820,12 +858,12 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
           if (y == 0) ok = ok && mbar_wait(&sm.p_full, x & 1, gave_up);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t vd = v_desc + v_slot * kTileStep, pd = p_desc + y * 64;
+          const uint64_t vd = v_desc + v_slot * kTileStep, pd = p_desc + y * kTile;
 #pragma unroll
           for (int h = 0; h < C::kParts; ++h)
 #pragma unroll
             for (int i = 0; i < kTile / 32; ++i)
-              mma(tmem + C::kOut + h * C::kN, vd + h * 8 * bs + v_step[i], pd + i * 16, kPv, y > 0 || i > 0);
+              mma(tmem + C::kOut + h * C::kN, vd + h * 8 * bs + v_step[i], pd + i * 32, kPv, y > 0 || i > 0);
           tc_commit(&sm.v_empty[v_slot]);
           if (++v_slot == kVs) v_slot = 0, v_parity ^= 1;
         }
