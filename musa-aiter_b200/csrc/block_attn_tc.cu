@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
   volatile int* gave_up = &sm.gave_up;
 
   if (warp < 8) {
+    regs_up<176>();  // with 104 and 56 below: what the block was launched with
     // ---- softmax ----------------------------------------------------------------
     const int half = warp >> 2;
     const int r = tid & 127;
@@ -201,24 +202,45 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
         const float* vf = sm.vfac[t & 3];
         const uint32_t have = (sm.chunks[t & 3] & 0xfu) | ((sm.chunks[t & 3] >> 4) & 0xf0u);
         const bool whole = tok >= all_lo && tok + kTile <= all_hi && have == 0xffu;
-        float top = -INFINITY;
+        // the row's scores stay in registers: scaled, then exponentiated
+        uint32_t x[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t x[32];
-          tmem_ld(s_at + c * 32, x);
-          tmem_wait(x);
-          const float f0 = kf[2 * c] * qs, f1 = kf[2 * c + 1] * qs;
-          if (whole) {
+        for (int c = 0; c < 4; ++c) tmem_ld(s_at + c * 32, x[c]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) top = fmaxf(top, __uint_as_float(x[e]) * (e < 16 ? f0 : f1));
-          } else {
+        for (int c = 0; c < 4; ++c) tmem_wait(x[c]);
+        if (whole) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int at = tok + 32 * c + e;
-              if (at >= lo && at < hi && ((have >> (2 * c + (e >> 4))) & 1)) top = fmaxf(top, __uint_as_float(x[e]) * (e < 16 ? f0 : f1));
+          for (int c = 0; c < 8; ++c) {
+            const float f = kf[c] * qs;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              uint32_t* at = &x[c >> 1][(c & 1) * 16 + e];
+              const float2 y = mul2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(f, f));
+              at[0] = __float_as_uint(y.x);
+              at[1] = __float_as_uint(y.y);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float f = kf[c] * qs;
+            // columns [from, to) of these 16 are seen
+            const int first = tok + 16 * c;
+            const int from = lo - first, to = (have >> c) & 1 ? hi - first : 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              uint32_t& at = x[c >> 1][(c & 1) * 16 + e];
+              at = e >= from && e < to ? __float_as_uint(__uint_as_float(at) * f) : 0xff800000u;
             }
           }
         }
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(x[c][e])), __uint_as_float(x[c][e + 1]));
+        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = fmaxf(m, top);
@@ -226,41 +248,36 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
           m = mn;
           l *= keep;
           if (t > 0) {
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld(o_at + c * 16, o);
+              tmem_wait(o);
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c) {
-              uint32_t x[32];
-              tmem_ld(o_at + c * 32, x);
-              tmem_wait(x);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * keep);
-              tmem_st(o_at + c * 32, x);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmem_st(o_at + c * 16, o);
             }
           }
         }
         const float ms = m == -INFINITY ? 0.f : m;
+        const float2 shift = make_float2(-ms, -ms);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          uint32_t x[32], y[16];
-          tmem_ld(s_at + c * 32, x);
-          tmem_wait(x);
-          const float f0 = kf[2 * c] * qs, f1 = kf[2 * c + 1] * qs;
-          const float v0 = vf[2 * c], v1 = vf[2 * c + 1];
+          uint32_t y[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float f = e < 16 ? f0 : f1, w = e < 16 ? v0 : v1;
-            float a = exp2_fast(fmaf(__uint_as_float(x[e]), f, -ms));
-            float b = exp2_fast(fmaf(__uint_as_float(x[e + 1]), f, -ms));
-            if (!whole) {
-              const int at = tok + 32 * c + e;
-              const bool page = (have >> (2 * c + (e >> 4))) & 1;
-              a = page && at >= lo && at < hi ? a : 0.f;
-              b = page && at + 1 >= lo && at + 1 < hi ? b : 0.f;
-            }
-            l += a + b;
-            y[e >> 1] = pack_f16(a * w, b * w);
+            const float w = vf[2 * c + (e >> 4)];
+            float2 a = add2(make_float2(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), shift);
+            a.x = exp2_fast(a.x);
+            a.y = exp2_fast(a.y);
+            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], a);
+            a = mul2(a, make_float2(w, w));
+            y[e >> 1] = pack_f16(a.x, a.y);
           }
           tmem_st(s_at + c * 16, y);
         }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -313,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
             !ok ? bad : some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
     }
   } else if (warp < 12) {
+    regs_down<104>();
     // ---- codes to f16 in shared memory -------------------------------------------
     const int w = warp - 8;
     const int dlo = lane & 7, chunk = (w & 1) * 4 + (lane >> 3);
@@ -353,18 +371,23 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
             if (kt + 4 * q + b >= any_lo && kt + 4 * q + b < any_hi) mask[q] |= 0xffu << (8 * b);
         }
       }
-#pragma unroll
-      for (int it = 0; it < kIts; ++it) {
+      auto convert = [&](int it, uint4 z) {
         uint32_t y[8];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t word = (&x[it].x)[q];
-          if (edge) word &= mask[q];
-          codes4_to_f16<CODE>(word, &y[2 * q], &y[2 * q + 1]);
-        }
+        codes4_to_f16<CODE>(z.x, &y[0], &y[1]);
+        codes4_to_f16<CODE>(z.y, &y[2], &y[3]);
+        codes4_to_f16<CODE>(z.z, &y[4], &y[5]);
+        codes4_to_f16<CODE>(z.w, &y[6], &y[7]);
         uint8_t* line = dst + to + it * 1024;
         *reinterpret_cast<uint4*>(line + c0) = make_uint4(y[0], y[1], y[2], y[3]);
         *reinterpret_cast<uint4*>(line + c1) = make_uint4(y[4], y[5], y[6], y[7]);
+      };
+      if (edge) {
+#pragma unroll
+        for (int it = 0; it < kIts; ++it)
+          convert(it, make_uint4(x[it].x & mask[0], x[it].y & mask[1], x[it].z & mask[2], x[it].w & mask[3]));
+      } else {
+#pragma unroll
+        for (int it = 0; it < kIts; ++it) convert(it, x[it]);
       }
     };
     auto scales = [&]() {
@@ -412,50 +435,55 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
         scales();
       }
     }
-  } else if (warp == 12 && lane == 0 && tiles > 0) {
-    // ---- the tensor cores ---------------------------------------------------------
-    constexpr uint32_t kQk = instr_desc(kTile, 1, 0, false, true), kPv = instr_desc(HD, 1, 0, false, false);
-    auto scores = [&](int half, int st) {
-      const uint32_t qa = smem_addr(sm.q[half]), ka = smem_addr(sm.k[st]);
+  } else {
+    regs_down<56>();
+    if (warp == 12 && lane == 0 && tiles > 0) {
+      // ---- the tensor cores -------------------------------------------------------
+      constexpr uint32_t kQk = instr_desc(kTile, 1, 0, false, true), kPv = instr_desc(HD, 1, 0, false, false);
+      // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
+      const uint64_t q_desc = smem_desc(smem_addr(sm.q), 16, 1024, 7), k_desc = smem_desc(smem_addr(sm.k), HD * 128, 1024, 7);
+      const uint64_t v_desc = smem_desc(smem_addr(sm.v), 16, 1024, 7);
+      constexpr uint32_t kBuffer = HD * 256 / 16;
+      auto scores = [&](int half, int st) {
+        const uint64_t qd = q_desc + half * kBuffer, kd = k_desc + st * kBuffer;
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-        mma_ss_f16(tmem + half * 128, smem_desc(qa + (ks >> 2) * 16384 + (ks & 3) * 32, 16, 1024, 7),
-               smem_desc(ka + ks * 2048, HD * 128, 1024, 7), kQk, ks > 0);
-      tc_commit(&sm.s_full[half]);
-    };
-    bool ok = true;
-    for (int half = 0; half < halves && ok; ++half) ok = mbar_wait(&sm.q_full[half], 0, gave_up);
-    ok = ok && mbar_wait(&sm.k_full[0], 0, gave_up);
-    if (ok) {
-      tc_fence_after();
-      for (int half = 0; half < halves; ++half) scores(half, 0);
-      tc_commit(&sm.k_empty[0]);
-    }
-    for (int t = 0; t < tiles && ok; ++t) {
-      const int st = t & 1;
-      ok = mbar_wait(&sm.v_full[st], (t >> 1) & 1, gave_up);
-      if (ok && t + 1 < tiles) ok = mbar_wait(&sm.k_full[st ^ 1], ((t + 1) >> 1) & 1, gave_up);
-      for (int half = 0; half < halves && ok; ++half) {
-        ok = mbar_wait(&sm.p_full[half], t & 1, gave_up);
-        if (!ok) break;
+        for (int ks = 0; ks < HD / 16; ++ks)
+          mma_ss_f16(tmem + half * 128, qd + (ks >> 2) * 1024 + (ks & 3) * 2, kd + ks * 128, kQk, ks > 0);
+        tc_commit(&sm.s_full[half]);
+      };
+      bool ok = true;
+      for (int half = 0; half < halves && ok; ++half) ok = mbar_wait(&sm.q_full[half], 0, gave_up);
+      ok = ok && mbar_wait(&sm.k_full[0], 0, gave_up);
+      if (ok) {
         tc_fence_after();
-        const uint32_t va = smem_addr(sm.v[st]);
+        for (int half = 0; half < halves; ++half) scores(half, 0);
+        tc_commit(&sm.k_empty[0]);
+      }
+      for (int t = 0; t < tiles && ok; ++t) {
+        const int st = t & 1;
+        ok = mbar_wait(&sm.v_full[st], (t >> 1) & 1, gave_up);
+        if (ok && t + 1 < tiles) ok = mbar_wait(&sm.k_full[st ^ 1], ((t + 1) >> 1) & 1, gave_up);
+        for (int half = 0; half < halves && ok; ++half) {
+          ok = mbar_wait(&sm.p_full[half], t & 1, gave_up);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = v_desc + st * kBuffer;
 #pragma unroll
-        for (int ks = 0; ks < kTile / 16; ++ks)
-          mma_ts_f16(tmem + 256 + half * HD, tmem + half * 128 + ks * 8, smem_desc(va + (ks >> 2) * (HD * 128) + (ks & 3) * 32, 16, 1024, 7),
-                 kPv, t > 0 || ks > 0);
-        if (half == halves - 1) tc_commit(&sm.v_empty[st]);
-        if (t + 1 < tiles) {
-          scores(half, st ^ 1);
-          if (half == halves - 1) tc_commit(&sm.k_empty[st ^ 1]);
-        } else {
-          tc_commit(&sm.o_full[half]);
+          for (int ks = 0; ks < kTile / 16; ++ks)
+            mma_ts_f16(tmem + 256 + half * HD, tmem + half * 128 + ks * 8, vd + (ks >> 2) * (HD * 8) + (ks & 3) * 2, kPv, t > 0 || ks > 0);
+          if (half == halves - 1) tc_commit(&sm.v_empty[st]);
+          if (t + 1 < tiles) {
+            scores(half, st ^ 1);
+            if (half == halves - 1) tc_commit(&sm.k_empty[st ^ 1]);
+          } else {
+            tc_commit(&sm.o_full[half]);
+          }
         }
       }
-    }
-    if (!ok) {  // let what was issued end before the TMEM is given back
-      tc_commit(&sm.spare);
-      for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
+      if (!ok) {  // let what was issued end before the TMEM is given back
+        tc_commit(&sm.spare);
+        for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
+        }
       }
     }
   }

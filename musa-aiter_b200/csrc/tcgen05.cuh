@@ -51,6 +51,16 @@ __device__ __forceinline__ void tc_commit(uint64_t* b) {
 // Generic writes to shared memory become visible to the tensor cores and the copy engine.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Registers of the threads of a warpgroup from here on.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 template <int COLS>
 __device__ __forceinline__ void tmem_alloc(uint32_t* at) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "n"(COLS) : "memory");
