@@ -29,8 +29,6 @@
 // alone.  A unit cut by that leaves partial sums (maximum, sum, accumulators) and the last block
 // to arrive joins them.  Roles: warps 0-3 softmax (a thread per token, then per head_dim row),
 // warp 4 copies, warp 5 issues the tensor cores; two steps are in flight between them.
-#include <cuda.h>
-
 #include "block_attn.cuh"
 #include "tcgen05.cuh"
 
@@ -888,35 +886,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
   }
 }
 
-// [num_blocks][num_heads][head_dim][block_size] bytes, boxes of one head of one block, lines swizzled.
-int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs) {
-  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static Encode encode = nullptr;
-  if (encode == nullptr) {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
-    if (e != cudaSuccess || fn == nullptr) {
-      (void)cudaGetLastError();
-      return fail(MAK_E_CUDA, "mak_block_attention: no cuTensorMapEncodeTiled in this driver");
-    }
-    encode = reinterpret_cast<Encode>(fn);
-  }
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(bs), static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(nh),
-                              static_cast<cuuint64_t>(num_blocks)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(bs), static_cast<cuuint64_t>(sh), static_cast<cuuint64_t>(sb)};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>(bs), static_cast<cuuint32_t>(hd), 1, 1}, steps[4] = {1, 1, 1, 1};
-  const CUtensorMapSwizzle swizzle =
-      bs == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bs == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
-  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, steps,
-                             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (rc != CUDA_SUCCESS) return fail(MAK_E_INVALID, "mak_block_attention: the cache's strides make no tensor map (%d)", static_cast<int>(rc));
-  return MAK_OK;
-}
-
 template <int HD, int ROWS, int CODE>
 int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
   const auto kernel = block_attn_rows_kernel<HD, ROWS, CODE>;
@@ -939,8 +908,8 @@ int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
   }
   CUtensorMap maps[2] = {};
   if (p.bs_log2 > 4 && p.num_blocks > 0) {
-    if (int rc = cache_map(&maps[0], p.key, p.k_sb, p.k_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2)) return rc;
-    if (int rc = cache_map(&maps[1], p.value, p.v_sb, p.v_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2)) return rc;
+    if (int rc = cache_map(&maps[0], p.key, p.k_sb, p.k_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2, true)) return rc;
+    if (int rc = cache_map(&maps[1], p.value, p.v_sb, p.v_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2, true)) return rc;
   }
   int64_t grid = per_sm * sm_count();
   if (grid > kMaxGrid) grid = kMaxGrid;
@@ -960,6 +929,35 @@ int launch_rows_code(const BlockAttnParams& p, int code, cudaStream_t st) {
 constexpr int64_t kCounterBytes = (2 * kMaxGrid * 4 + 255) / 256 * 256;
 
 }  // namespace
+
+int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs,
+              bool swizzled) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (encode == nullptr) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess || fn == nullptr) {
+      (void)cudaGetLastError();
+      return fail(MAK_E_CUDA, "mak_block_attention: no cuTensorMapEncodeTiled in this driver");
+    }
+    encode = reinterpret_cast<Encode>(fn);
+  }
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(bs), static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(nh),
+                              static_cast<cuuint64_t>(num_blocks)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(bs), static_cast<cuuint64_t>(sh), static_cast<cuuint64_t>(sb)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(bs), static_cast<cuuint32_t>(hd), 1, 1}, steps[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle =
+      !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : bs == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bs == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+  const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, steps,
+                             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(MAK_E_INVALID, "mak_block_attention: the cache's strides make no tensor map (%d)", static_cast<int>(rc));
+  return MAK_OK;
+}
 
 int launch_block_attn_tc(const BlockAttnParams& p, int head_dim, int code, cudaStream_t st);
 

@@ -2,6 +2,7 @@
 // rows and the kernel for many rows share.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -86,6 +87,10 @@ __device__ __forceinline__ void codes4_to_f16(uint32_t w, uint32_t* lo, uint32_t
   }
 }
 
+// [num_blocks][num_heads][head_dim][block_size] bytes as boxes of one head of one block, lines of
+// block_size bytes swizzled or as they are.
+int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool swizzled);
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -93,18 +98,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // Two 32-bit operations in one instruction, each rounded as its scalar form.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
   asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 w, x, y, z;\n mov.b64 w, {%2, %3};\n mov.b64 x, {%4, %5};\n mov.b64 y, {%6, %7};\n fma.rn.f32x2 z, w, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
 

@@ -12,8 +12,9 @@
 // so a K / V tile serves all of them) as two tiles of 128, and walks the cache in
 // tiles of 128 tokens.  Roles:
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row (TMEM lane)
-//   warps 8-11       load codes, convert to f16, store to shared memory
+//   warps 8-11       codes to f16, shared memory to shared memory
 //   warp 12          one thread issues all tcgen05.mma
+//   warp 13          block ids, scales, and the copies of the codes to shared memory
 // While one row tile's scores are exponentiated the tensor cores work for the other.
 //
 // Layout.  The cache tile is [head_dim][tokens], tokens contiguous.  Converted to f16
@@ -37,9 +38,11 @@ struct TcSmem {
   alignas(1024) uint8_t q[2][HD * 256];  // 128 rows: HD / 64 pieces of [128][64]
   alignas(1024) uint8_t k[2][HD * 256];  // 128 tokens: 2 pieces of [HD][64]
   alignas(1024) uint8_t v[2][HD * 256];
-  float kfac[4][8], vfac[4][8];          // per 16 tokens of a tile
-  uint32_t chunks[4];                    // 16-token pieces that have a page: 0-3 in byte 0, 4-7 in byte 1
-  alignas(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], spare;
+  alignas(128) uint8_t k_raw[HD * 128], v_raw[HD * 128];  // codes as they come: [block][HD][block_size]
+  alignas(16) float kfac[4][8], vfac[4][8];  // per 16 tokens of a tile: K scale, weight of a unit of V
+  alignas(16) float vlog[4][8], vinv[4][8];  // log2 and reciprocal of the latter
+  uint32_t have[4], plain[4];                // bit c: piece c has a block; its factors are positive and finite
+  alignas(8) uint64_t kr_full, kr_empty, vr_full, vr_empty, q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], spare;
   uint32_t tmem;
   float vmax[4];
   int unit_seq, unit_tile;
@@ -47,9 +50,11 @@ struct TcSmem {
 };
 
 template <int HD, int CODE>
-__global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid_constant__ BlockAttnParams p) {
-  extern __shared__ uint8_t raw[];
-  TcSmem<HD>& sm = *reinterpret_cast<TcSmem<HD>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~static_cast<uintptr_t>(1023));
+__global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid_constant__ BlockAttnParams p,
+                                                                           const __grid_constant__ CUtensorMap kmap,
+                                                                           const __grid_constant__ CUtensorMap vmap) {
+  extern __shared__ __align__(1024) uint8_t raw[];
+  TcSmem<HD>& sm = *reinterpret_cast<TcSmem<HD>*>(raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   pdl_trigger();
@@ -81,6 +86,10 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
       sm.unit_tile = static_cast<int>(item - row * p.group / kUnitRows - lo);
       sm.gave_up = 0;
       mbar_init(&sm.spare, 1);
+      mbar_init(&sm.kr_full, 1);
+      mbar_init(&sm.vr_full, 1);
+      mbar_init(&sm.kr_empty, 4);
+      mbar_init(&sm.vr_empty, 4);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&sm.q_full[i], 4);
         mbar_init(&sm.k_full[i], 4);
@@ -132,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
   volatile int* gave_up = &sm.gave_up;
 
   if (warp < 8) {
-    regs_up<176>();  // with 104 and 56 below: what the block was launched with
+    regs_up<184>();  // with 80 and 64 below: what the block was launched with
     // ---- softmax ----------------------------------------------------------------
     const int half = warp >> 2;
     const int r = tid & 127;
@@ -199,48 +208,39 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
         tc_fence_after();
         const int tok = (t0 + t) * kTile;
         const float* kf = sm.kfac[t & 3];
-        const float* vf = sm.vfac[t & 3];
-        const uint32_t have = (sm.chunks[t & 3] & 0xfu) | ((sm.chunks[t & 3] >> 4) & 0xf0u);
-        const bool whole = tok >= all_lo && tok + kTile <= all_hi && have == 0xffu;
-        // the row's scores stay in registers: scaled, then exponentiated
-        uint32_t x[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld(s_at + c * 32, x[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait(x[c]);
+        const uint32_t have = sm.have[t & 3];
+        const bool whole = tok >= all_lo && tok + kTile <= all_hi && sm.plain[t & 3] == 0xffu && p.scale_log2 > 0.f;
+        uint32_t x[4][32];  // whole: the row's scores stay in registers
+        float top = -INFINITY;
         if (whole) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float f = kf[c] * qs;
+          for (int c = 0; c < 4; ++c) tmem_ld(s_at + c * 32, x[c]);
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              uint32_t* at = &x[c >> 1][(c & 1) * 16 + e];
-              const float2 y = mul2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(f, f));
-              at[0] = __float_as_uint(y.x);
-              at[1] = __float_as_uint(y.y);
-            }
+          for (int c = 0; c < 4; ++c) tmem_wait(x[c]);
+          float tops[8];  // 16 columns share a factor, which is positive: it can wait
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint32_t* at = &x[c >> 1][(c & 1) * 16];
+            tops[c] = fmaxf(__uint_as_float(at[0]), __uint_as_float(at[1]));
+#pragma unroll
+            for (int e = 2; e < 16; e += 2) tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(at[e])), __uint_as_float(at[e + 1]));
           }
-        } else {
 #pragma unroll
+          for (int c = 0; c < 8; ++c) top = fmaxf(top, tops[c] * (kf[c] * qs));
+        } else {
+#pragma unroll 1
           for (int c = 0; c < 8; ++c) {
+            uint32_t y[16];
+            tmem_ld(s_at + c * 16, y);
+            tmem_wait(y);
             const float f = kf[c] * qs;
             // columns [from, to) of these 16 are seen
-            const int first = tok + 16 * c;
-            const int from = lo - first, to = (have >> c) & 1 ? hi - first : 0;
+            const int first = tok + 16 * c, from = lo - first, to = (have >> c) & 1 ? hi - first : 0;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              uint32_t& at = x[c >> 1][(c & 1) * 16 + e];
-              at = e >= from && e < to ? __float_as_uint(__uint_as_float(at) * f) : 0xff800000u;
-            }
+            for (int e = 0; e < 16; ++e)
+              if (e >= from && e < to) top = fmaxf(top, __uint_as_float(y[e]) * f);
           }
         }
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(x[c][e])), __uint_as_float(x[c][e + 1]));
-        const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
         if (__any_sync(0xffffffffu, grow)) {
           const float mn = fmaxf(m, top);
@@ -260,24 +260,48 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
           }
         }
         const float ms = m == -INFINITY ? 0.f : m;
-        const float2 shift = make_float2(-ms, -ms);
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        if (whole) {
+          // 2^(x f - m) b' as one power of 2; the sum of the weights without b' is taken per 16 columns
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t y[16];
+          for (int c = 0; c < 4; ++c) {
+            uint32_t y[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float w = vf[2 * c + (e >> 4)];
-            float2 a = add2(make_float2(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), shift);
-            a.x = exp2_fast(a.x);
-            a.y = exp2_fast(a.y);
-            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], a);
-            a = mul2(a, make_float2(w, w));
-            y[e >> 1] = pack_f16(a.x, a.y);
+            for (int z = 0; z < 2; ++z) {
+              const float f = kf[2 * c + z] * qs, d = sm.vlog[t & 3][2 * c + z] - ms;
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 16; e += 2) {
+                const uint32_t* at = &x[c][z * 16 + e];
+                float2 w = fma2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(f, f), make_float2(d, d));
+                w.x = exp2_fast(w.x);
+                w.y = exp2_fast(w.y);
+                sum = add2(sum, w);
+                y[(z * 16 + e) >> 1] = pack_f16(w.x, w.y);
+              }
+              l = fmaf(sum.x + sum.y, sm.vinv[t & 3][2 * c + z], l);
+            }
+            tmem_st(s_at + c * 16, y);
           }
-          tmem_st(s_at + c * 16, y);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t x16[16], y[8];
+            tmem_ld(s_at + c * 16, x16);
+            tmem_wait(x16);
+            const float f = kf[c] * qs, w = sm.vfac[t & 3][c];
+            const int first = tok + 16 * c, from = lo - first, to = (have >> c) & 1 ? hi - first : 0;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float a = exp2_fast(fmaf(__uint_as_float(x16[e]), f, -ms));
+              float b = exp2_fast(fmaf(__uint_as_float(x16[e + 1]), f, -ms));
+              a = e >= from && e < to ? a : 0.f;
+              b = e + 1 >= from && e + 1 < to ? b : 0.f;
+              l += a + b;
+              y[e >> 1] = pack_f16(a * w, b * w);
+            }
+            tmem_st(s_at + c * 8, y);
+          }
         }
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -330,113 +354,68 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
             !ok ? bad : some ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
     }
   } else if (warp < 12) {
-    regs_down<104>();
+    regs_down<80>();
     // ---- codes to f16 in shared memory -------------------------------------------
-    const int w = warp - 8;
-    const int dlo = lane & 7, chunk = (w & 1) * 4 + (lane >> 3);
-    const int d0 = (w >> 1) * (HD / 2) + dlo;
+    // Piece i of the raw codes (16 tokens of one head_dim row) is 16 bytes at 16 i: pieces of a block's
+    // line first, then rows, then blocks.
+    const int id0 = tid - 256;
+    const int per_log2 = p.bs_log2 - 4;
     constexpr int kIts = HD / 16;
-    const uint8_t* kb = p.key + head * p.k_sh + static_cast<int64_t>(d0) * bs;
-    const uint8_t* vb = p.value + head * p.v_sh + static_cast<int64_t>(d0) * bs;
-    const uint32_t to = (chunk >> 2) * (HD * 128) + d0 * 128;
-    const uint32_t c0 = ((((chunk & 3) * 2) ^ dlo) << 4), c1 = ((((chunk & 3) * 2 + 1) ^ dlo) << 4);
-    uint4 kx[kIts], vx[kIts];
-    float ks = 0.f, vs = 0.f;
-    int page = -1, next_page = -1;
-    auto find = [&](int t) {
-      const int kt = (t0 + t) * kTile + 16 * chunk;
-      int pg = -1;
-      if (t < tiles && kt < any_hi && kt + 16 > any_lo) pg = __ldg(table + (kt >> p.bs_log2));
-      return pg >= p.num_blocks ? -1 : pg;
+    auto convert = [&](uint8_t* dst, int it, uint4 z) {
+      const int id = it * 128 + id0;
+      const int d = (id >> per_log2) & (HD - 1);
+      const int chunk = ((id >> per_log2) / HD << per_log2) | (id & ((1 << per_log2) - 1));
+      uint32_t y[8];
+      codes4_to_f16<CODE>(z.x, &y[0], &y[1]);
+      codes4_to_f16<CODE>(z.y, &y[2], &y[3]);
+      codes4_to_f16<CODE>(z.z, &y[4], &y[5]);
+      codes4_to_f16<CODE>(z.w, &y[6], &y[7]);
+      uint8_t* line = dst + (chunk >> 2) * (HD * 128) + d * 128;
+      const uint32_t c0 = ((chunk & 3) * 2) ^ (d & 7);
+      *reinterpret_cast<uint4*>(line + (c0 << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint4*>(line + ((c0 ^ 1) << 4)) = make_uint4(y[4], y[5], y[6], y[7]);
     };
-    auto fetch = [&](const uint8_t* base, int64_t stride, int t, int pg, uint4(&x)[kIts]) {
-      const int kt = (t0 + t) * kTile + 16 * chunk;
-      const uint8_t* src = base + pg * stride + (kt & (bs - 1));
+    auto tile = [&](const uint8_t* src, uint8_t* dst, int t, uint64_t* raw_full, uint64_t* raw_empty, uint64_t* empty, uint64_t* full) {
+      if (!mbar_wait_warp(raw_full, t & 1, gave_up)) return false;
+      uint4 x[kIts];
 #pragma unroll
-      for (int it = 0; it < kIts; ++it) {
-        x[it] = make_uint4(0, 0, 0, 0);
-        if (pg >= 0) x[it] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<int64_t>(it * 8) * bs));
-      }
-    };
-    auto store = [&](uint8_t* dst, int t, const uint4(&x)[kIts]) {
-      const int kt = (t0 + t) * kTile + 16 * chunk;
-      uint32_t mask[4] = {~0u, ~0u, ~0u, ~0u};
-      const bool edge = kt < any_lo || kt + 16 > any_hi;
-      if (edge) {
+      for (int it = 0; it < kIts; ++it) x[it] = reinterpret_cast<const uint4*>(src)[it * 128 + id0];
+      const int tok = (t0 + t) * kTile;
+      if (tok < any_lo || tok + kTile > any_hi || sm.have[t & 3] != 0xffu) {
+        // tokens that no row sees, or without a block: their codes may be anything and become 0
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          mask[q] = 0;
+        for (int it = 0; it < kIts; ++it) {
+          const int id = it * 128 + id0;
+          const int chunk = ((id >> per_log2) / HD << per_log2) | (id & ((1 << per_log2) - 1));
+          const int first = tok + 16 * chunk;
+          uint32_t* words = &x[it].x;
 #pragma unroll
-          for (int b = 0; b < 4; ++b)
-            if (kt + 4 * q + b >= any_lo && kt + 4 * q + b < any_hi) mask[q] |= 0xffu << (8 * b);
+          for (int q = 0; q < 4; ++q) {
+            uint32_t mask = 0;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+              if (first + 4 * q + b >= any_lo && first + 4 * q + b < any_hi) mask |= 0xffu << (8 * b);
+            words[q] = (sm.have[t & 3] >> chunk) & 1 ? words[q] & mask : 0u;
+          }
         }
       }
-      auto convert = [&](int it, uint4 z) {
-        uint32_t y[8];
-        codes4_to_f16<CODE>(z.x, &y[0], &y[1]);
-        codes4_to_f16<CODE>(z.y, &y[2], &y[3]);
-        codes4_to_f16<CODE>(z.z, &y[4], &y[5]);
-        codes4_to_f16<CODE>(z.w, &y[6], &y[7]);
-        uint8_t* line = dst + to + it * 1024;
-        *reinterpret_cast<uint4*>(line + c0) = make_uint4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint4*>(line + c1) = make_uint4(y[4], y[5], y[6], y[7]);
-      };
-      if (edge) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(raw_empty);
+      if (!mbar_wait_warp(empty, ((t >> 1) & 1) ^ 1, gave_up)) return false;
 #pragma unroll
-        for (int it = 0; it < kIts; ++it)
-          convert(it, make_uint4(x[it].x & mask[0], x[it].y & mask[1], x[it].z & mask[2], x[it].w & mask[3]));
-      } else {
-#pragma unroll
-        for (int it = 0; it < kIts; ++it) convert(it, x[it]);
-      }
+      for (int it = 0; it < kIts; ++it) convert(dst, it, x[it]);
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full);
+      return true;
     };
-    auto scales = [&]() {
-      ks = vs = 0.f;
-      if (page >= 0) {
-        ks = __ldg(p.key_scale + page * p.ks_sb + head * p.ks_sh);
-        vs = __ldg(p.value_scale + page * p.vs_sb + head * p.vs_sh);
-      }
-    };
-    if (tiles > 0) {
-      page = find(0);
-      next_page = find(1);
-      fetch(kb, p.k_sb, 0, page, kx);
-      fetch(vb, p.v_sb, 0, page, vx);
-      scales();
-    }
     for (int t = 0; t < tiles; ++t) {
       const int st = t & 1;
-      const uint32_t parity = ((t >> 1) & 1) ^ 1;
-      if (!mbar_wait_warp(&sm.k_empty[st], parity, gave_up)) break;
-      // the factors of tile t - 4 were last read before tile t - 2's scores were issued
-      if (dlo == 0 && w < 2) {
-        sm.kfac[t & 3][chunk] = ks;
-        sm.vfac[t & 3][chunk] = vref > 0.f ? vs / vref * 64.f : 0.f;
-      }
-      const uint32_t votes = __ballot_sync(0xffffffffu, page >= 0);
-      if (lane == 0 && w < 2) {
-        const uint32_t bits = (votes & 1) | ((votes >> 7) & 2) | ((votes >> 14) & 4) | ((votes >> 21) & 8);
-        reinterpret_cast<uint8_t*>(&sm.chunks[t & 3])[w] = static_cast<uint8_t>(bits);
-      }
-      store(sm.k[st], t, kx);
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.k_full[st]);
-      page = next_page;
-      if (t + 1 < tiles) fetch(kb, p.k_sb, t + 1, page, kx);
-      next_page = find(t + 2);
-      if (!mbar_wait_warp(&sm.v_empty[st], parity, gave_up)) break;
-      store(sm.v[st], t, vx);
-      fence_async_shared();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.v_full[st]);
-      if (t + 1 < tiles) {
-        fetch(vb, p.v_sb, t + 1, page, vx);
-        scales();
-      }
+      if (!tile(sm.k_raw, sm.k[st], t, &sm.kr_full, &sm.kr_empty, &sm.k_empty[st], &sm.k_full[st])) break;
+      if (!tile(sm.v_raw, sm.v[st], t, &sm.vr_full, &sm.vr_empty, &sm.v_empty[st], &sm.v_full[st])) break;
     }
   } else {
-    regs_down<56>();
+    regs_down<64>();
     if (warp == 12 && lane == 0 && tiles > 0) {
       // ---- the tensor cores -------------------------------------------------------
       constexpr uint32_t kQk = instr_desc(kTile, 1, 0, false, true), kPv = instr_desc(HD, 1, 0, false, false);
@@ -485,6 +464,70 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
         for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
         }
       }
+    } else if (warp == 13 && tiles > 0) {
+      // ---- copies of the codes, a lane per 16 tokens (lanes 8 and up idle) ---------
+      const int piece = lane & 7;
+      const uint32_t per_line = bs >> 4, bytes = HD * bs;
+      const bool leads = lane < 8 && piece % per_line == 0;
+      const uint32_t k_to = smem_addr(sm.k_raw) + piece * (HD * 16), v_to = smem_addr(sm.v_raw) + piece * (HD * 16);
+      auto find = [&](int t) {
+        const int tk = ((t0 + t) * kTile + 16 * piece) & ~(bs - 1);  // the block's first token
+        int pg = -1;
+        if (lane < 8 && t < tiles && tk < any_hi && tk + bs > any_lo) pg = __ldg(table + (tk >> p.bs_log2));
+        return pg >= p.num_blocks ? -1 : pg;
+      };
+      auto scale = [&](const float* from, int pg, int64_t sb, int64_t sh) { return pg >= 0 ? __ldg(from + pg * sb + head * sh) : 0.f; };
+      int page = find(0), page1 = find(1);
+      float ks = scale(p.key_scale, page, p.ks_sb, p.ks_sh), vs = scale(p.value_scale, page, p.vs_sb, p.vs_sh);
+      uint32_t k_sent = 0, v_sent = 0;
+      for (int t = 0; t < tiles; ++t) {
+        const uint32_t parity = (t & 1) ^ 1;
+        const uint32_t led = __popc(__ballot_sync(0xffffffffu, leads && page >= 0)) * bytes;
+        if (!mbar_wait_warp(&sm.kr_empty, parity, gave_up)) break;
+        if (leads && page >= 0) {
+          if (p.bs_log2 == 4)
+            bulk_load(k_to, p.key + page * p.k_sb + head * p.k_sh, bytes, &sm.kr_full);
+          else
+            tensor_load(k_to, &kmap, head, page, &sm.kr_full);
+        }
+        // Their place was tile t - 4's.  Codes of tile t - 1 have been taken, so V of tile t - 2 has been
+        // stored, for which the products of tile t - 4 had to be done, and its factors read before them.
+        const float w = vref > 0.f ? vs / vref * 64.f : 0.f;
+        const bool fine = page >= 0 && ks > 0.f && ks < INFINITY && w > 0.f && w < INFINITY;
+        const uint32_t have = __ballot_sync(0xffffffffu, page >= 0) & 0xffu, plain = __ballot_sync(0xffffffffu, fine) & 0xffu;
+        if (lane < 8) {
+          sm.kfac[t & 3][piece] = ks;
+          sm.vfac[t & 3][piece] = w;
+          sm.vlog[t & 3][piece] = fine ? log2f(w) : 0.f;
+          sm.vinv[t & 3][piece] = fine ? 1.f / w : 0.f;
+        }
+        if (lane == 0) {
+          sm.have[t & 3] = have;
+          sm.plain[t & 3] = plain;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect(&sm.kr_full, led);
+        ++k_sent;
+        if (!mbar_wait_warp(&sm.vr_empty, parity, gave_up)) break;
+        if (leads && page >= 0) {
+          if (p.bs_log2 == 4)
+            bulk_load(v_to, p.value + page * p.v_sb + head * p.v_sh, bytes, &sm.vr_full);
+          else
+            tensor_load(v_to, &vmap, head, page, &sm.vr_full);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect(&sm.vr_full, led);
+        ++v_sent;
+        page = page1;
+        ks = scale(p.key_scale, page, p.ks_sb, p.ks_sh);
+        vs = scale(p.value_scale, page, p.vs_sb, p.vs_sh);
+        page1 = find(t + 2);
+      }
+      // copies in flight end before the block does
+      for (uint32_t z = 0; k_sent > 0 && z < kWaitLimit && !mbar_try(&sm.kr_full, (k_sent - 1) & 1); ++z) {
+      }
+      for (uint32_t z = 0; v_sent > 0 && z < kWaitLimit && !mbar_try(&sm.vr_full, (v_sent - 1) & 1); ++z) {
+      }
     }
   }
   tc_fence_before();
@@ -498,7 +541,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_attn_tc_kernel(const __grid
 
 template <int HD, int CODE>
 int launch_tc(const BlockAttnParams& p, cudaStream_t st) {
-  constexpr int kBytes = sizeof(TcSmem<HD>) + 1024;
+  constexpr int kBytes = sizeof(TcSmem<HD>);
+  static_assert(kBytes <= 227 * 1024, "shared memory of a block");
   static bool set = false;
   if (!set) {
     const cudaError_t e = cudaFuncSetAttribute(block_attn_tc_kernel<HD, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
@@ -508,10 +552,15 @@ int launch_tc(const BlockAttnParams& p, cudaStream_t st) {
     }
     set = true;
   }
+  CUtensorMap maps[2] = {};
+  if (p.bs_log2 > 4 && p.num_blocks > 0) {
+    if (int rc = cache_map(&maps[0], p.key, p.k_sb, p.k_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2, false)) return rc;
+    if (int rc = cache_map(&maps[1], p.value, p.v_sb, p.v_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2, false)) return rc;
+  }
   const int64_t items = static_cast<int64_t>(p.num_rows) * p.group / kUnitRows + p.num_seqs;
   if (items * p.nh > 0x7fffffff) return fail(MAK_E_UNSUPPORTED, "mak_block_attention: too many rows for one call");
   return launch_pdl("mak_block_attention", block_attn_tc_kernel<HD, CODE>, dim3(static_cast<unsigned>(items * p.nh)), dim3(kThreads),
-                    kBytes, st, p);
+                    kBytes, st, p, maps[0], maps[1]);
 }
 
 }  // namespace

@@ -119,18 +119,14 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&v)[16]) {
 __device__ __forceinline__ void tmem_wait(uint32_t (&v)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : MAK_RW8(v, 0), MAK_RW8(v, 8), MAK_RW8(v, 16), MAK_RW8(v, 24)::"memory");
 }
-__device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::MAK_W8(v, 0),
-      MAK_W8(v, 8), MAK_W8(v, 16), MAK_W8(v, 24), "r"(at)
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MAK_W8(v, 0),
       MAK_W8(v, 8), "r"(at)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t at, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::MAK_W8(v, 0), "r"(at) : "memory");
 }
 #undef MAK_R8
 #undef MAK_W8
