@@ -12,6 +12,7 @@ There is no fallback: if the library is missing or a call fails, a
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 from ctypes import POINTER, c_int32, c_int64, c_size_t, c_uint64, c_void_p
@@ -19,6 +20,7 @@ from ctypes import POINTER, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 import torch
 
 from . import _build
+from .dispatch import emit_native
 
 ABI_VERSION = 1
 
@@ -272,7 +274,7 @@ _PROTOTYPES = {
             c_void_p,
         ],
     ),
-    # descriptors of the calls below are packed bytes
+    # the calls below go through _mak_front
     "mak_block_attention_workspace_bytes": (c_int64, []),
     "mak_block_attention": (c_int32, [c_void_p, c_void_p]),
     "mak_block_append": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_void_p]),
@@ -315,6 +317,27 @@ def load() -> ctypes.CDLL:
             raise RuntimeError(f"musa_aiter kvcache native library ABI {version} != expected {ABI_VERSION}")
         _LIB = lib
         return lib
+
+
+_FRONT = None
+
+
+def front():
+    """The CPython module ``_mak_front`` (csrc/front.cpp), bound to this process's kernel library: the checks
+    and descriptors of the calls that are shorter than a Python argument check."""
+    global _FRONT
+    if _FRONT is None:
+        path = str(_build.FRONT_PATH)
+        if not os.path.exists(path):
+            raise RuntimeError(f"musa_aiter native front missing: {path} not found: build it with "
+                               "musa_aiter.build_native_kv_transfer()")
+        lib = load()
+        spec = importlib.util.spec_from_file_location("_mak_front", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind({name: ctypes.cast(getattr(lib, name), c_void_p).value for name in _PROTOTYPES}, emit_native)
+        _FRONT = module
+    return _FRONT
 
 
 def is_available() -> bool:
