@@ -34,44 +34,42 @@ struct AppendParams {
   int32_t num_seqs, max_blocks, num_rows, nh, bs_log2;
 };
 
-// Loads N neighbouring values of one row as float; non-finite values become 0.
+// N neighbouring values of one row as they are stored.
 template <int DT, int N>
-__device__ __forceinline__ void load_values(const void* base, int64_t at, float (&x)[N]) {
-  if constexpr (DT == MAK_DT_F32) {
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 f = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(base) + at + i));
-      x[i] = f.x;
-      x[i + 1] = f.y;
-    }
-  } else {
-    uint32_t w[N / 2];
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    if constexpr (N == 2) {
-      w[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-    } else if constexpr (N == 4) {
+struct Raw {
+  static constexpr int kWords = DT == MAK_DT_F32 ? N : N / 2;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+    const uint32_t* p = static_cast<const uint32_t*>(base) + (DT == MAK_DT_F32 ? at : at / 2);
+    if constexpr (kWords == 1) {
+      w[0] = __ldg(p);
+    } else if constexpr (kWords == 2) {
       const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
       w[0] = v.x, w[1] = v.y;
     } else {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-      w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    }
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      if constexpr (DT == MAK_DT_BF16) {
-        x[2 * i] = __uint_as_float(w[i] << 16);
-        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + i));
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
       }
     }
   }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) x[i] = 0.f;
-}
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+  }
+  // As float, non-finite values as 0.
+  __device__ __forceinline__ float get(int i) const {
+    float x;
+    if constexpr (DT == MAK_DT_F32)
+      x = __uint_as_float(w[i]);
+    else if constexpr (DT == MAK_DT_BF16)
+      x = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else
+      x = __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
+    return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0.f : x;
+  }
+};
 
 template <int CODE>
 __device__ __forceinline__ float code_value(uint32_t byte) {
@@ -162,13 +160,24 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) block_append_kernel(const
     old = *sp;
     if (!(old > 0.f) || old == INFINITY) old = 0.f;
   }
+  // 16 tokens at a time, all their loads in flight; those of the last 16 stay in registers, which for
+  // 16-token blocks is all of them
   float top = 0.f;
-#pragma unroll 4
-  for (int o = off0; o < off1; ++o) {
-    float v[kDims];
-    load_values<DT, kDims>(x, xat + o * p.x_sr[kv], v);
+  Raw<DT, kDims> raw[16];
+  int held = -1;
+  for (int c0 = off0 & ~15; c0 < off1; c0 += 16) {
 #pragma unroll
-    for (int i = 0; i < kDims; ++i) top = fmaxf(top, fabsf(v[i]));
+    for (int b = 0; b < 16; ++b) {
+      if (c0 + b >= off0 && c0 + b < off1)
+        raw[b].load(x, xat + (c0 + b) * p.x_sr[kv]);
+      else
+        raw[b].clear();
+    }
+#pragma unroll
+    for (int b = 0; b < 16; ++b)
+#pragma unroll
+      for (int i = 0; i < kDims; ++i) top = fmaxf(top, fabsf(raw[b].get(i)));
+    held = c0;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -207,16 +216,18 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) block_append_kernel(const
       }
     }
     if (fresh) {
+      if (c0 != held) {
+#pragma unroll
+        for (int b = 0; b < 16; ++b) {
+          if (c0 + b >= off0 && c0 + b < off1)
+            raw[b].load(x, xat + (c0 + b) * p.x_sr[kv]);
+          else
+            raw[b].clear();
+        }
+        held = c0;
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float v[4][kDims];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const int o = c0 + 4 * q + b;
-#pragma unroll
-          for (int i = 0; i < kDims; ++i) v[b][i] = 0.f;
-          if (o >= off0 && o < off1) load_values<DT, kDims>(x, xat + o * p.x_sr[kv], v[b]);
-        }
         uint32_t mask = 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
@@ -226,11 +237,12 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) block_append_kernel(const
           float y[4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
+            const float v = raw[4 * q + b].get(i);
             if (direct) {
-              y[b] = __fdiv_rn(v[b][i], safe);
+              y[b] = __fdiv_rn(v, safe);
             } else {
-              const float q0 = __fmul_rn(v[b][i], inv);
-              y[b] = __fmaf_rn(__fmaf_rn(-q0, safe, v[b][i]), inv, q0);
+              const float q0 = __fmul_rn(v, inv);
+              y[b] = __fmaf_rn(__fmaf_rn(-q0, safe, v), inv, q0);
             }
           }
           w[i][q] = (w[i][q] & ~mask) | (to_codes<CODE>(y) & mask);

@@ -257,11 +257,18 @@ __global__ void __launch_bounds__(kPlan) compact_plan_kernel(Pages p, int32_t* l
   }
 }
 
+// The planes of one launch in the order they are moved: first those of at least a chunk, each in
+// whole chunks of 256 vectors (its last one part empty), then the small ones, their vectors end to
+// end.  A warp moves a chunk of one page at a time, 8 vectors per lane in flight, so a page's
+// indexes cost one look-up per 4 KB.
+constexpr int kChunk = 256;
 struct Planes {
   uint64_t ptr[kMaxPagePlanes];
   int64_t stride[kMaxPagePlanes];
-  int64_t size[kMaxPagePlanes];
-  int32_t planes;
+  uint32_t vecs[kMaxPagePlanes];   // of one page
+  uint32_t start[kMaxPagePlanes];  // big: first chunk; small: first vector
+  int32_t big, planes;
+  uint32_t big_chunks, small_vecs, chunks;
 };
 
 enum { kCopyOnly = 0, kFork = 1, kCompact = 2 };
@@ -272,61 +279,61 @@ struct Moves {
   const int32_t* count;  // number of pairs on the device, or null: n
   int32_t n;
   int64_t pages;
+  int32_t table_blocks;  // leading blocks that update tables and counts instead
 };
 
+// The last plane in [lo, hi) that starts at or before x.
+__device__ __forceinline__ int plane_of(const Planes& pl, int lo, int hi, uint32_t x) {
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pl.start[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
 template <typename V>
-__device__ __forceinline__ void copy_plane(const Planes& pl, int plane, const Moves& mv, int n, int64_t first, int64_t step) {
-  const char* base = reinterpret_cast<const char*>(pl.ptr[plane]);
-  const int64_t stride = pl.stride[plane];
-  const uint32_t vecs = static_cast<uint32_t>(pl.size[plane] / sizeof(V));
-  const int64_t all = static_cast<int64_t>(n) * vecs;
-  constexpr int kDeep = 8;
-  for (int64_t v0 = first; v0 < all; v0 += step) {
-    V x[kDeep];
-    int64_t to[kDeep];
+__device__ __forceinline__ void move_pages(const Planes& pl, const Moves& mv, int n, int64_t warp, int64_t warps) {
+  const int lane = threadIdx.x & 31;
+  const int64_t units = static_cast<int64_t>(n) * pl.chunks;
+  for (int64_t u = warp; u < units; u += warps) {
+    const int64_t pair = (units >> 32) == 0 ? static_cast<uint32_t>(u) / pl.chunks : u / pl.chunks;
+    const uint32_t chunk = static_cast<uint32_t>(u - pair * pl.chunks);
+    const int s = __ldg(mv.src + pair), d = __ldg(mv.dst + pair);
+    if (s < 0 || d < 0 || s >= mv.pages || d >= mv.pages) continue;
+    V x[8];
+    if (chunk < pl.big_chunks) {
+      const int i = plane_of(pl, 0, pl.big, chunk);
+      const uint32_t first = (chunk - pl.start[i]) * kChunk, left = pl.vecs[i] - first;
+      const V* from = reinterpret_cast<const V*>(pl.ptr[i] + s * pl.stride[i]) + first;
+      V* to = reinterpret_cast<V*>(pl.ptr[i] + d * pl.stride[i]) + first;
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i) {
-      const int64_t v = v0 + i * static_cast<int64_t>(blockDim.x);
-      to[i] = -1;
-      if (v < all) {
-        const int64_t k = (all >> 31) == 0 ? static_cast<uint32_t>(v) / vecs : v / vecs;
-        const int64_t in = (v - k * vecs) * static_cast<int64_t>(sizeof(V));
-        const int s = __ldg(mv.src + k), d = __ldg(mv.dst + k);
-        if (s >= 0 && d >= 0 && s < mv.pages && d < mv.pages) {
-          to[i] = d * stride + in;
-          x[i] = *reinterpret_cast<const V*>(base + s * stride + in);
+      for (int k = 0; k < 8; ++k)
+        if (k * 32 + lane < left) x[k] = from[k * 32 + lane];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k * 32 + lane < left) to[k * 32 + lane] = x[k];
+    } else {
+      const uint32_t first = (chunk - pl.big_chunks) * kChunk;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t v = first + k * 32 + lane;
+        if (v < pl.small_vecs) {
+          const int i = plane_of(pl, pl.big, pl.planes, v);
+          const uint32_t in = v - pl.start[i];
+          reinterpret_cast<V*>(pl.ptr[i] + d * pl.stride[i])[in] = reinterpret_cast<const V*>(pl.ptr[i] + s * pl.stride[i])[in];
         }
       }
     }
-#pragma unroll
-    for (int i = 0; i < kDeep; ++i)
-      if (to[i] >= 0) *reinterpret_cast<V*>(const_cast<char*>(base) + to[i]) = x[i];
   }
 }
 
-// Block (x, y): piece x of plane y; blocks with y past the planes update tables and counts.
 template <int MODE>
-__global__ void __launch_bounds__(256) pages_move_kernel(const __grid_constant__ Planes pl, const __grid_constant__ Moves mv,
-                                                         const __grid_constant__ Pages p, const int32_t* parents,
-                                                         const int32_t* children) {
-  pdl_wait();
-  pdl_trigger();
-  const int n = mv.count != nullptr ? *mv.count : mv.n;
-  const int plane = blockIdx.y;
-  if (plane < pl.planes) {
-    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x * 8;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x * 8 + threadIdx.x;
-    const uint64_t bits = pl.ptr[plane] | static_cast<uint64_t>(pl.stride[plane]) | static_cast<uint64_t>(pl.size[plane]);
-    if ((bits & 15) == 0)
-      copy_plane<uint4>(pl, plane, mv, n, first, step);
-    else if ((bits & 3) == 0)
-      copy_plane<uint32_t>(pl, plane, mv, n, first, step);
-    else
-      copy_plane<uint8_t>(pl, plane, mv, n, first, step);
-    return;
-  }
+__device__ __forceinline__ void update_tables(const Moves& mv, const Pages& p, int n, const int32_t* parents, const int32_t* children) {
   if constexpr (MODE == kFork) {
-    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    for (int i = blockIdx.x; i < n; i += mv.table_blocks) {
       const int row = parents[i], child = children[i];
       if (row < 0 || row >= p.rows || child < 0 || child >= p.rows) continue;
       const int len = valid_len(p, row);
@@ -351,7 +358,7 @@ __global__ void __launch_bounds__(256) pages_move_kernel(const __grid_constant__
     const int32_t* rank = mv.src + 2 * mv.pages;
     const int live = mv.count[1];
     const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    const int64_t step = static_cast<int64_t>(mv.table_blocks) * blockDim.x;
     for (int64_t i = first; i < static_cast<int64_t>(p.rows) * p.max_blocks; i += step) {
       int32_t* e = p.tables + (i / p.max_blocks) * p.table_stride + i % p.max_blocks;
       const int page = *e;
@@ -364,6 +371,21 @@ __global__ void __launch_bounds__(256) pages_move_kernel(const __grid_constant__
       p.refs[mv.src[i]] = 0;
     }
   }
+}
+
+template <int MODE, typename V>
+__global__ void __launch_bounds__(256) pages_move_kernel(const __grid_constant__ Planes pl, const __grid_constant__ Moves mv,
+                                                         const __grid_constant__ Pages p, const int32_t* parents,
+                                                         const int32_t* children) {
+  pdl_wait();
+  pdl_trigger();
+  const int n = mv.count != nullptr ? *mv.count : mv.n;
+  if (static_cast<int>(blockIdx.x) < mv.table_blocks) {
+    update_tables<MODE>(mv, p, n, parents, children);
+    return;
+  }
+  const int64_t warps = static_cast<int64_t>(gridDim.x - mv.table_blocks) * 8;
+  move_pages<V>(pl, mv, n, static_cast<int64_t>(blockIdx.x - mv.table_blocks) * 8 + (threadIdx.x >> 5), warps);
 }
 
 int check_pages(const mak_pages_desc* d, const char* name, Pages* out) {
@@ -392,32 +414,85 @@ int check_planes(const mak_pages_planes* pl, const char* name) {
   return MAK_OK;
 }
 
-// Moves planes [0, num) in launches of at most kMaxPagePlanes; the last one also updates the tables.
+template <int MODE, typename V>
+int launch_move(const Planes& pl, Moves mv, const Pages& p, const int32_t* parents, const int32_t* children, int64_t most, bool tables,
+                const char* name, cudaStream_t st) {
+  const auto kernel = pages_move_kernel<MODE, V>;
+  static int per_sm = 0;
+  if (per_sm == 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, 0) != cudaSuccess || n <= 0) n = 1;
+    per_sm = n;
+  }
+  const int64_t room = static_cast<int64_t>(per_sm) * sm_count();
+  int64_t copy = (most * pl.chunks + 7) / 8;
+  copy = copy < room ? copy : room;
+  mv.table_blocks = 0;
+  if (tables && MODE == kFork) mv.table_blocks = static_cast<int32_t>(most < 256 ? most : 256);
+  if (tables && MODE == kCompact) {
+    const int64_t entries = static_cast<int64_t>(p.rows) * p.max_blocks + most;
+    mv.table_blocks = static_cast<int32_t>((entries + 1023) / 1024 < 64 ? (entries + 1023) / 1024 : 64);
+  }
+  if (copy + mv.table_blocks == 0) return MAK_OK;
+  return launch_pdl(name, kernel, dim3(static_cast<unsigned>(copy + mv.table_blocks)), dim3(256), 0, st, pl, mv, p, parents, children);
+}
+
+// Moves all planes, those of one alignment (16, 4 or 1 bytes) and at most kMaxPagePlanes to a launch;
+// the last launch also updates the tables.
 template <int MODE>
 int launch_moves(const mak_pages_planes* pl, const Moves& mv, const Pages& p, const int32_t* parents, const int32_t* children,
                  int64_t most, const char* name, cudaStream_t st) {
-  int64_t at = 0;
-  do {
-    Planes a;
-    int64_t biggest = 16;
-    a.planes = 0;
-    for (; at < pl->num_planes && a.planes < kMaxPagePlanes; ++at) {
-      a.ptr[a.planes] = pl->ptrs[at];
-      a.stride[a.planes] = pl->strides[at];
-      a.size[a.planes] = pl->sizes[at];
-      biggest = biggest > pl->sizes[at] ? biggest : pl->sizes[at];
-      ++a.planes;
+  static const int kWidths[3] = {16, 4, 1};
+  int64_t left = 0;
+  for (int64_t i = 0; i < pl->num_planes; ++i) left += pl->sizes[i] > 0;
+  Planes a;
+  a.big = a.planes = 0;
+  a.big_chunks = a.small_vecs = a.chunks = 0;
+  if (left == 0) return launch_move<MODE, uint4>(a, mv, p, parents, children, most, true, name, st);
+  for (int w = 0; w < 3 && left > 0; ++w) {
+    const int width = kWidths[w];
+    auto fits = [&](int64_t i) {
+      const uint64_t bits = pl->ptrs[i] | static_cast<uint64_t>(pl->strides[i]) | static_cast<uint64_t>(pl->sizes[i]);
+      return pl->sizes[i] > 0 && ((bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1) == width;
+    };
+    int64_t at = 0;
+    while (at < pl->num_planes) {
+      int64_t end = at;
+      int got = 0;
+      for (; end < pl->num_planes && got < kMaxPagePlanes; ++end) got += fits(end);
+      if (got == 0) break;
+      a.planes = a.big = 0;
+      a.big_chunks = a.small_vecs = 0;
+      for (int big = 1; big >= 0; --big) {
+        for (int64_t i = at; i < end; ++i) {
+          const uint32_t vecs = static_cast<uint32_t>(pl->sizes[i] / width);
+          if (!fits(i) || (vecs >= kChunk) != (big == 1)) continue;
+          a.ptr[a.planes] = pl->ptrs[i];
+          a.stride[a.planes] = pl->strides[i];
+          a.vecs[a.planes] = vecs;
+          a.start[a.planes] = big ? a.big_chunks : a.small_vecs;
+          if (big)
+            a.big_chunks += (vecs + kChunk - 1) / kChunk;
+          else
+            a.small_vecs += vecs;
+          ++a.planes;
+        }
+        if (big) a.big = a.planes;
+      }
+      a.chunks = a.big_chunks + (a.small_vecs + kChunk - 1) / kChunk;
+      left -= got;
+      const bool tables = MODE != kCopyOnly && left == 0;
+      int rc;
+      if (width == 16)
+        rc = launch_move<MODE, uint4>(a, mv, p, parents, children, most, tables, name, st);
+      else if (width == 4)
+        rc = launch_move<MODE, uint32_t>(a, mv, p, parents, children, most, tables, name, st);
+      else
+        rc = launch_move<MODE, uint8_t>(a, mv, p, parents, children, most, tables, name, st);
+      if (rc) return rc;
+      at = end;
     }
-    const bool last = at >= pl->num_planes;
-    const int extra = last && MODE != kCopyOnly ? 1 : 0;
-    if (a.planes + extra == 0) return MAK_OK;
-    // a block moves 32 KB at a time; with more of them than fit at once the last wave drains evenly
-    int64_t x = (most * biggest + 32767) / 32768;
-    x = x < 1 ? 1 : x > 4096 ? 4096 : x;
-    const dim3 grid(static_cast<unsigned>(x), static_cast<unsigned>(a.planes + extra));
-    if (int rc = launch_pdl(name, pages_move_kernel<MODE>, grid, dim3(256), 0, st, a, mv, p, parents, children)) return rc;
-    if (last) break;
-  } while (true);
+  }
   return MAK_OK;
 }
 
@@ -442,7 +517,7 @@ extern "C" int mak_pages_fork(const mak_pages_desc* pages, const mak_pages_plane
                             at == 0, src, dst))
       return rc;
     if (here == 0) break;
-    const Moves mv{src, dst, nullptr, here, p.pages};
+    const Moves mv{src, dst, nullptr, here, p.pages, 0};
     if (int rc = launch_moves<kFork>(planes, mv, p, parents + at, children + at, here, name, st)) return rc;
   }
   return MAK_OK;
@@ -482,7 +557,7 @@ extern "C" int mak_pages_compact(const mak_pages_desc* pages, const mak_pages_pl
   if (live == nullptr || scratch == nullptr) return fail(MAK_E_INVALID, "%s: null pointer", name);
   cudaStream_t st = as_stream(stream);
   if (int rc = launch_pdl(name, compact_plan_kernel, dim3(1), dim3(kPlan), 0, st, p, live, scratch)) return rc;
-  const Moves mv{scratch, scratch + p.pages, scratch + 3 * static_cast<int64_t>(p.pages), 0, p.pages};
+  const Moves mv{scratch, scratch + p.pages, scratch + 3 * static_cast<int64_t>(p.pages), 0, p.pages, 0};
   return launch_moves<kCompact>(planes, mv, p, nullptr, nullptr, p.pages / 2 + 1, name, st);
 }
 
@@ -493,6 +568,6 @@ extern "C" int mak_pages_copy(const mak_pages_planes* planes, int64_t num_pages,
   if (num_pages < 0 || num_pages > 0x3fffffff || n < 0 || n > 0x7fffffff || (n && (!src || !dst)))
     return fail(MAK_E_INVALID, "%s: bad requests", name);
   if (n == 0) return MAK_OK;
-  const Moves mv{src, dst, nullptr, static_cast<int32_t>(n), num_pages};
+  const Moves mv{src, dst, nullptr, static_cast<int32_t>(n), num_pages, 0};
   return launch_moves<kCopyOnly>(planes, mv, Pages{}, nullptr, nullptr, n, name, as_stream(stream));
 }

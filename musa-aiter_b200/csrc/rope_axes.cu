@@ -88,38 +88,51 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const __grid_constant__ 
       if (d.inverse) s[i] = -s[i];
     }
   }
-#pragma unroll 2
-  for (int h = h0; h < h1; ++h) {
-    const bool isq = h < d.q_heads;
-    const int hh = isq ? h : h - d.q_heads;
-    const uint16_t* src = static_cast<const uint16_t*>(isq ? d.q : d.k) + t * (isq ? d.q_stride_token : d.k_stride_token) +
-                          hh * (isq ? d.q_stride_head : d.k_stride_head) + at;
-    uint16_t* dst = static_cast<uint16_t*>(isq ? d.q_out : d.k_out) + t * (isq ? d.qo_stride_token : d.ko_stride_token) +
-                    hh * (isq ? d.qo_stride_head : d.ko_stride_head) + at;
-    const uint4 r0 = __ldg(reinterpret_cast<const uint4*>(src));
-    if (!rotates) {
-      *reinterpret_cast<uint4*>(dst) = r0;
-      continue;
+  // kDeep heads' loads in flight
+  constexpr int kDeep = INTER ? 8 : 4;
+  for (int h = h0; h < h1; h += kDeep) {
+    uint4 r1[kDeep], r2[kDeep];
+#pragma unroll
+    for (int z = 0; z < kDeep; ++z) {
+      if (h + z >= h1) break;
+      const bool isq = h + z < d.q_heads;
+      const int hh = isq ? h + z : h + z - d.q_heads;
+      const uint16_t* src = static_cast<const uint16_t*>(isq ? d.q : d.k) + t * (isq ? d.q_stride_token : d.k_stride_token) +
+                            hh * (isq ? d.q_stride_head : d.k_stride_head) + at;
+      r1[z] = __ldcs(reinterpret_cast<const uint4*>(src));
+      if (!INTER && rotates) r2[z] = __ldcs(reinterpret_cast<const uint4*>(src + half));
     }
-    float x[8], y[8];
-    unpack8<DT>(r0, x);
-    if constexpr (INTER) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[2 * i] = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
-        y[2 * i + 1] = x[2 * i] * s[i] + x[2 * i + 1] * c[i];
+    for (int z = 0; z < kDeep; ++z) {
+      if (h + z >= h1) break;
+      const bool isq = h + z < d.q_heads;
+      const int hh = isq ? h + z : h + z - d.q_heads;
+      uint16_t* dst = static_cast<uint16_t*>(isq ? d.q_out : d.k_out) + t * (isq ? d.qo_stride_token : d.ko_stride_token) +
+                      hh * (isq ? d.qo_stride_head : d.ko_stride_head) + at;
+      if (!rotates) {
+        __stcs(reinterpret_cast<uint4*>(dst), r1[z]);
+        continue;
       }
-      *reinterpret_cast<uint4*>(dst) = pack8<DT>(y);
-    } else {
-      float x2[8], y2[8];
-      unpack8<DT>(__ldg(reinterpret_cast<const uint4*>(src + half)), x2);
+      float x[8], y[8];
+      unpack8<DT>(r1[z], x);
+      if constexpr (INTER) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[i] = x[i] * c[i] - x2[i] * s[i];
-        y2[i] = x[i] * s[i] + x2[i] * c[i];
+        for (int i = 0; i < 4; ++i) {
+          y[2 * i] = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
+          y[2 * i + 1] = x[2 * i] * s[i] + x[2 * i + 1] * c[i];
+        }
+        __stcs(reinterpret_cast<uint4*>(dst), pack8<DT>(y));
+      } else {
+        float x2[8], y2[8];
+        unpack8<DT>(r2[z], x2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = x[i] * c[i] - x2[i] * s[i];
+          y2[i] = x[i] * s[i] + x2[i] * c[i];
+        }
+        __stcs(reinterpret_cast<uint4*>(dst), pack8<DT>(y));
+        __stcs(reinterpret_cast<uint4*>(dst + half), pack8<DT>(y2));
       }
-      *reinterpret_cast<uint4*>(dst) = pack8<DT>(y);
-      *reinterpret_cast<uint4*>(dst + half) = pack8<DT>(y2);
     }
   }
 }
