@@ -58,16 +58,43 @@ struct Raw {
 #pragma unroll
     for (int i = 0; i < kWords; ++i) w[i] = 0;
   }
-  // As float, non-finite values as 0.
-  __device__ __forceinline__ float get(int i) const {
-    float x;
+  // Magnitudes order as their bits do: the largest of those seen so far, for 16-bit types two at a time.
+  __device__ __forceinline__ void top(uint32_t& m) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      m = DT == MAK_DT_F32 ? max(m, w[i] & 0x7fffffffu) : __vmaxu2(m, w[i] & 0x7fff7fffu);
+  }
+  static constexpr uint32_t kInf = DT == MAK_DT_F32 ? 0x7f800000u : DT == MAK_DT_BF16 ? 0x7f80u : 0x7c00u;
+  // Of the two halves of m.
+  static __device__ __forceinline__ uint32_t widest(uint32_t m) { return DT == MAK_DT_F32 ? m : max(m & 0xffffu, m >> 16); }
+  static __device__ __forceinline__ float value(uint32_t bits) {
     if constexpr (DT == MAK_DT_F32)
-      x = __uint_as_float(w[i]);
+      return __uint_as_float(bits);
     else if constexpr (DT == MAK_DT_BF16)
-      x = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      return __uint_as_float(bits << 16);
     else
-      x = __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? w[i / 2] >> 16 : w[i / 2])));
-    return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0.f : x;
+      return __half2float(__ushort_as_half(static_cast<uint16_t>(bits)));
+  }
+  // Non-finite values to 0.
+  __device__ __forceinline__ void finite() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (DT == MAK_DT_F32) {
+        if ((w[i] & kInf) == kInf) w[i] = 0;
+      } else {
+        if ((w[i] & kInf) == kInf) w[i] &= 0xffff0000u;
+        if ((w[i] >> 16 & kInf) == kInf) w[i] &= 0xffffu;
+      }
+    }
+  }
+  // Values 2 i and 2 i + 1.
+  __device__ __forceinline__ float2 pair(int i) const {
+    if constexpr (DT == MAK_DT_F32)
+      return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if constexpr (DT == MAK_DT_BF16)
+      return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    else
+      return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
   }
 };
 
@@ -82,14 +109,14 @@ __device__ __forceinline__ float code_value(uint32_t byte) {
   }
 }
 
-// Four values to four code bytes.
+// Four values to four code bytes; int8: values of at most 127.5 in magnitude.
 template <int CODE>
 __device__ __forceinline__ uint32_t to_codes(const float (&v)[4]) {
   if constexpr (CODE == MAK_CODE_INT8) {
     uint32_t b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // adding 1.5 * 2^23 rounds to a whole number in the low bits
-      b[i] = __float_as_uint(fminf(fmaxf(v[i], -127.f), 127.f) + 12582912.f);
+      b[i] = __float_as_uint(v[i] + 12582912.f);
     return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   } else {
     uint32_t r;
@@ -101,20 +128,18 @@ __device__ __forceinline__ uint32_t to_codes(const float (&v)[4]) {
   }
 }
 
-template <int HD, int CODE, int DT>
-__global__ void __launch_bounds__(32 * kWarpsPerBlock) block_append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int kDims = HD / 32;
-  constexpr float kMost = CODE == MAK_CODE_INT8 ? 127.f : 448.f;
-  const int lane = threadIdx.x & 31;
-  pdl_wait();
-  pdl_trigger();
-  const int64_t unit = blockIdx.x * static_cast<int64_t>(kWarpsPerBlock) + (threadIdx.x >> 5);
-  if (unit >= p.items * p.nh * 2) return;
-  const int kv = static_cast<int>(unit & 1);
-  const int head = static_cast<int>((unit >> 1) % p.nh);
-  const int64_t item = (unit >> 1) / p.nh;
-  const int bs = 1 << p.bs_log2;
+// A block of the cache that the call writes.
+struct Target {
+  int64_t item, row;  // row: packed row of offset 0 (may lie before the sequence's first)
+  int page, off0, off1;  // offsets [off0, off1) are written; page < 0: none
+  bool begun;
+};
 
+__device__ __forceinline__ Target find_target(const AppendParams& p, int64_t item, int lane) {
+  Target t;
+  t.item = item;
+  t.page = -1;
+  const int bs = 1 << p.bs_log2;
   // Slots floor(starts[s] / bs) + 2 s ... belong to sequence s: at least as many as it
   // can touch blocks, whatever its position.
   int s, row0, rows, nth;
@@ -140,68 +165,117 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) block_append_kernel(const
   }
   const int64_t ctx = __ldg(p.ctx_lens + s);
   const int64_t first = ctx - rows;  // position of the call's first row
-  if (rows <= 0 || first < 0) return;
+  if (rows <= 0 || first < 0) return t;
   const int64_t block = (first >> p.bs_log2) + nth;
   const int64_t start = block << p.bs_log2;
-  if (start >= ctx || block >= p.max_blocks) return;
+  if (start >= ctx || block >= p.max_blocks) return t;
   const int page = __ldg(p.tables + s * p.table_stride + block);
-  if (page < 0 || page >= p.num_blocks) return;
-  const bool begun = start >= first;
-  const int off0 = begun ? 0 : static_cast<int>(first - start);  // offsets [off0, off1) are written
-  const int off1 = static_cast<int>(min(ctx - start, static_cast<int64_t>(bs)));
-  const void* x = p.x[kv];
-  // element of offset o, this lane's dims: xat + o * row stride
-  const int64_t xat = (row0 + start - first) * p.x_sr[kv] + head * p.x_sh[kv] + lane * kDims;
-  uint8_t* tile = p.cache[kv] + page * p.c_sb[kv] + head * p.c_sh[kv] + static_cast<int64_t>(lane * kDims) * bs;
-  float* sp = p.scale[kv] + page * p.s_sb[kv] + head * p.s_sh[kv];
+  if (page < 0 || page >= p.num_blocks) return t;
+  t.page = page;
+  t.begun = start >= first;
+  t.off0 = t.begun ? 0 : static_cast<int>(first - start);
+  t.off1 = static_cast<int>(min(ctx - start, static_cast<int64_t>(bs)));
+  t.row = row0 + start - first;
+  return t;
+}
 
+// Blocks per SM by the words a lane holds of a row: 16-bit rows of head_dim 64 and 128 fit five times (prompt
+// writes 24.3 us with four, 22.5 with five, 21.8 with six, 24.2 with eight; a decode step 3.95, 4.19, 4.47, 5.15).
+constexpr int blocks_per_sm_of(int words) { return words <= 2 ? 5 : words <= 4 ? 3 : 2; }
+
+// One warp, one tile: its first 16 tokens (all of them for 16-token blocks), old scale and codes are loaded
+// at once and stay in registers.
+template <int HD, int CODE, int DT>
+__global__ void __launch_bounds__(32 * kWarpsPerBlock, blocks_per_sm_of(Raw<DT, HD / 32>::kWords)) block_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kDims = HD / 32;
+  constexpr float kMost = CODE == MAK_CODE_INT8 ? 127.f : 448.f;
+  using R = Raw<DT, kDims>;
+  const int lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  const int64_t unit = blockIdx.x * static_cast<int64_t>(kWarpsPerBlock) + (threadIdx.x >> 5);
+  if (unit >= p.items * p.nh * 2) return;
+  const int kv = static_cast<int>(unit & 1);
+  const int64_t pair = unit >> 1;
+  const int64_t item = (pair >> 32) == 0 ? static_cast<uint32_t>(pair) / static_cast<uint32_t>(p.nh) : pair / p.nh;
+  const int head = static_cast<int>(pair - item * p.nh);
+  const Target t = find_target(p, item, lane);
+  if (t.page < 0) return;
+  const int bs = 1 << p.bs_log2;
+  const void* x = p.x[kv];
+  const int64_t x_step = p.x_sr[kv];
+  const int64_t x_at = t.row * x_step + head * p.x_sh[kv] + lane * kDims;  // offset 0, this lane's dims
+  uint8_t* tile = p.cache[kv] + t.page * p.c_sb[kv] + head * p.c_sh[kv] + static_cast<int64_t>(lane * kDims) * bs;
+  float* scale = p.scale[kv] + t.page * p.s_sb[kv] + head * p.s_sh[kv];
+
+  R raw[16];
+  auto load16 = [&](int c0) {
+    const int64_t at = x_at + c0 * x_step;
+    if (c0 >= t.off0 && c0 + 16 <= t.off1) {
+#pragma unroll
+      for (int b = 0; b < 16; ++b) raw[b].load(x, at + b * x_step);
+    } else {
+#pragma unroll
+      for (int b = 0; b < 16; ++b) {
+        raw[b].clear();
+        if (c0 + b >= t.off0 && c0 + b < t.off1) raw[b].load(x, at + b * x_step);
+      }
+    }
+  };
+  const int first = t.off0 & ~15;
+  load16(first);
   float old = 0.f;
-  if (!begun) {
-    old = *sp;
+  uint4 codes[kDims];
+  if (!t.begun) {
+    old = *scale;
+#pragma unroll
+    for (int i = 0; i < kDims; ++i) codes[i] = *reinterpret_cast<const uint4*>(tile + static_cast<int64_t>(i) * bs + first);
     if (!(old > 0.f) || old == INFINITY) old = 0.f;
   }
-  // 16 tokens at a time, all their loads in flight; those of the last 16 stay in registers, which for
-  // 16-token blocks is all of them
-  float top = 0.f;
-  Raw<DT, kDims> raw[16];
-  int held = -1;
-  for (int c0 = off0 & ~15; c0 < off1; c0 += 16) {
+  uint32_t most = 0;
+  int held = first;  // the 16 tokens in registers
+  bool odd = false;  // non-finite values seen
+  for (int c0 = first; c0 < t.off1; c0 += 16) {
+    if (c0 != held) load16(c0), held = c0;
+    uint32_t m = 0;
 #pragma unroll
-    for (int b = 0; b < 16; ++b) {
-      if (c0 + b >= off0 && c0 + b < off1)
-        raw[b].load(x, xat + (c0 + b) * p.x_sr[kv]);
-      else
-        raw[b].clear();
+    for (int b = 0; b < 16; ++b) raw[b].top(m);
+    if (R::widest(m) >= R::kInf) {
+      odd = true;
+      m = 0;
+#pragma unroll
+      for (int b = 0; b < 16; ++b) {
+        raw[b].finite();
+        raw[b].top(m);
+      }
     }
-#pragma unroll
-    for (int b = 0; b < 16; ++b)
-#pragma unroll
-      for (int i = 0; i < kDims; ++i) top = fmaxf(top, fabsf(raw[b].get(i)));
-    held = c0;
+    most = max(most, R::widest(m));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float top = R::value(__reduce_max_sync(0xffffffffu, most));
   const float mine = top < 0x1p-100f ? 0.f : __fdiv_rn(top, kMost);
   const float now = fmaxf(old, mine);
   const bool grew = now > old;
-  if (lane == 0 && (begun || grew || old == 0.f)) *sp = now;
+  if (lane == 0 && (t.begun || grew || old == 0.f)) *scale = now;
   const float safe = now > 0.f ? now : 1.f;
   const float ratio = grew ? __fdiv_rn(old, safe) : 1.f;
-  const float inv = __frcp_rn(safe);
-  const bool direct = safe < 0x1p-60f || safe > 0x1p60f;  // the remainder could underflow
+  // x / s as (x 2^k) / (s 2^k): away from the ends of the exponent range the remainder is exact, and what
+  // 2^-64 rounds off of an x is nothing beside an s above 2^60
+  const float adj = safe < 0x1p-60f ? 0x1p64f : safe > 0x1p60f ? 0x1p-64f : 1.f;
+  const float div = safe * adj, inv = __frcp_rn(div);
 
   for (int c0 = 0; c0 < bs; c0 += 16) {
-    const bool fresh = c0 < off1 && c0 + 16 > off0;
-    if (!fresh && !begun && !(grew)) continue;
+    const bool fresh = c0 < t.off1 && c0 + 16 > t.off0;
+    if (!fresh && !t.begun && !grew) continue;
     uint32_t w[kDims][4];
-    if (begun) {
+    if (t.begun) {
 #pragma unroll
       for (int i = 0; i < kDims; ++i) w[i][0] = w[i][1] = w[i][2] = w[i][3] = 0;
     } else {
 #pragma unroll
       for (int i = 0; i < kDims; ++i) {
-        const uint4 t = *reinterpret_cast<const uint4*>(tile + static_cast<int64_t>(i) * bs + c0);
-        w[i][0] = t.x, w[i][1] = t.y, w[i][2] = t.z, w[i][3] = t.w;
+        uint4 z = codes[i];
+        if (c0 != first) z = *reinterpret_cast<const uint4*>(tile + static_cast<int64_t>(i) * bs + c0);
+        w[i][0] = z.x, w[i][1] = z.y, w[i][2] = z.z, w[i][3] = z.w;
       }
       if (grew) {
 #pragma unroll
@@ -210,42 +284,41 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock) block_append_kernel(const
           for (int q = 0; q < 4; ++q) {
             float v[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) v[b] = __fmul_rn(code_value<CODE>((w[i][q] >> (8 * b)) & 0xffu), ratio);
+            for (int b = 0; b < 4; ++b) {
+              v[b] = __fmul_rn(code_value<CODE>((w[i][q] >> (8 * b)) & 0xffu), ratio);
+              if (CODE == MAK_CODE_INT8) v[b] = fmaxf(v[b], -127.f);  // -128 is not the writer's
+            }
             w[i][q] = to_codes<CODE>(v);
           }
       }
     }
     if (fresh) {
       if (c0 != held) {
+        load16(c0), held = c0;
+        if (odd) {
 #pragma unroll
-        for (int b = 0; b < 16; ++b) {
-          if (c0 + b >= off0 && c0 + b < off1)
-            raw[b].load(x, xat + (c0 + b) * p.x_sr[kv]);
-          else
-            raw[b].clear();
+          for (int b = 0; b < 16; ++b) raw[b].finite();
         }
-        held = c0;
       }
+      const float2 zero = make_float2(0.f, 0.f);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t mask = 0;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
-          if (c0 + 4 * q + b >= off0 && c0 + 4 * q + b < off1) mask |= 0xffu << (8 * b);
+          if (c0 + 4 * q + b >= t.off0 && c0 + 4 * q + b < t.off1) mask |= 0xffu << (8 * b);
 #pragma unroll
-        for (int i = 0; i < kDims; ++i) {
-          float y[4];
+        for (int i = 0; i < kDims; i += 2) {
+          float y[2][4];
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const float v = raw[4 * q + b].get(i);
-            if (direct) {
-              y[b] = __fdiv_rn(v, safe);
-            } else {
-              const float q0 = __fmul_rn(v, inv);
-              y[b] = __fmaf_rn(__fmaf_rn(-q0, safe, v), inv, q0);
-            }
+            const float2 v = fma2(raw[4 * q + b].pair(i / 2), make_float2(adj, adj), zero), q0 = fma2(v, make_float2(inv, inv), zero);
+            const float2 z = fma2(fma2(q0, make_float2(-div, -div), v), make_float2(inv, inv), q0);
+            y[0][b] = z.x;
+            y[1][b] = z.y;
           }
-          w[i][q] = (w[i][q] & ~mask) | (to_codes<CODE>(y) & mask);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) w[i + e][q] = (w[i + e][q] & ~mask) | (to_codes<CODE>(y[e]) & mask);
         }
       }
     }
