@@ -79,9 +79,6 @@ struct Smem {
   float lsum[4][ROWS];
   alignas(8) uint64_t k_full[C::kKs], k_empty[C::kKs], v_full[C::kVs], v_empty[C::kVs];
   uint64_t q_full, s_full[2], p_full, o_full, spare;
-  int64_t scan[4];
-  int64_t begin_base;
-  int begin_seq;
   uint32_t tmem;
   int gave_up, last;
 };
@@ -228,69 +225,65 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
   pdl_wait();
   pdl_trigger();
 
-  // ---- the run of this block ------------------------------------------------
+  // ---- the run of this block: every warp finds it for itself --------------------
   Walk walk;
   int64_t chunk;
   {
-    const int per = (p.num_seqs + kSoft - 1) / kSoft;
-    const int s0 = min(tid * per, p.num_seqs), s1 = warp < 4 ? min(s0 + per, p.num_seqs) : s0;
+    const int per = (p.num_seqs + 31) / 32;
+    const int s0 = min(lane * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
     int64_t mine = 0;
     for (int s = s0; s < s1; ++s) mine += seq_work<ROWS>(p, seq_view(p, s));
     int64_t incl = mine;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
-    if (lane == 31 && warp < 4) sm.scan[warp] = incl;
-    if (tid == kSoft) {
-      sm.gave_up = 0;
-      for (int i = 0; i < kKs; ++i) {
-        mbar_init(&sm.k_full[i], 1);
-        mbar_init(&sm.k_empty[i], 1);
-      }
-      for (int i = 0; i < kVs; ++i) {
-        mbar_init(&sm.v_full[i], 1);
-        mbar_init(&sm.v_empty[i], 1);
-      }
-      mbar_init(&sm.q_full, 4);
-      mbar_init(&sm.s_full[0], 1);
-      mbar_init(&sm.s_full[1], 1);
-      mbar_init(&sm.p_full, 4);
-      mbar_init(&sm.o_full, 1);
-      mbar_init(&sm.spare, 1);
-      mbar_init_fence();
-    }
-    __syncthreads();
-    int64_t total = 0;
-    for (int x = 0; x < 4; ++x) {
-      if (x < warp) incl += sm.scan[x];
-      total += sm.scan[x];
-    }
+    const int64_t total = __shfl_sync(0xffffffffu, incl, 31);
     chunk = (total >> 31) == 0 ? (static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x : (total + gridDim.x - 1) / gridDim.x;
     if (chunk < kMinChunk) chunk = kMinChunk;
     walk.w = blockIdx.x * chunk;
     walk.w_end = min(walk.w + chunk, total);
     if (walk.w >= walk.w_end) return;
-    if (warp < 4 && incl - mine <= walk.w && walk.w < incl) {
-      int64_t base = incl - mine;
-      for (int s = s0; s < s1; ++s) {
-        const int64_t w = seq_work<ROWS>(p, seq_view(p, s));  // zero for a sequence without rows
-        if (walk.w < base + w) {
-          sm.begin_seq = s;
-          sm.begin_base = base;
-          break;
-        }
+    const bool here = incl - mine <= walk.w && walk.w < incl;
+    int seq = 0;
+    int64_t base = incl - mine;
+    if (here) {
+      for (seq = s0;; ++seq) {
+        const int64_t w = seq_work<ROWS>(p, seq_view(p, seq));  // zero for a sequence without rows
+        if (walk.w < base + w) break;
         base += w;
       }
     }
+    const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    begin_walk<ROWS>(p, walk, __shfl_sync(0xffffffffu, seq, from), __shfl_sync(0xffffffffu, base, from));
+  }
+  const int64_t w_begin = walk.w;
+  if (tid == kSoft) {
+    sm.gave_up = 0;
+    for (int i = 0; i < kKs; ++i) {
+      mbar_init(&sm.k_full[i], 1);
+      mbar_init(&sm.k_empty[i], 1);
+    }
+    for (int i = 0; i < kVs; ++i) {
+      mbar_init(&sm.v_full[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+    }
+    mbar_init(&sm.q_full, 4);
+    mbar_init(&sm.s_full[0], 1);
+    mbar_init(&sm.s_full[1], 1);
+    mbar_init(&sm.p_full, 4);
+    mbar_init(&sm.o_full, 1);
+    mbar_init(&sm.spare, 1);
+    mbar_init_fence();
   }
   if (warp == 5) tmem_alloc<C::kTmem>(&sm.tmem);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sm.tmem;
-  begin_walk<ROWS>(p, walk, sm.begin_seq, sm.begin_base);
-  const int64_t w_begin = walk.w;
+  // Ends the set-up: what a role can load before, it does.
+  auto ready = [&]() {
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
   volatile int* gave_up = &sm.gave_up;
   const int bs = 1 << p.bs_log2;
   Unit u;
@@ -305,12 +298,26 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     uint32_t it = 0, tiles_done = 0;  // steps and tiles before this unit
     bool ok = true;
     // Rows of a unit: their places, and q as three 8-bit terms.  A row's threads are neighbours.
+    constexpr int kPer = HD * ROWS / kSoft;  // values of a thread
+    constexpr int kRowThreads = kSoft / ROWS;
+    const int r = tid / kRowThreads, d0 = tid % kRowThreads * kPer;
+    uint32_t w[kPer / 2];
+    auto fetch = [&](const Unit& u) {
+#pragma unroll
+      for (int e = 0; e < kPer / 2; ++e) w[e] = 0;
+      if (r < u.live) {
+        const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) - i * p.group;
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (u.v.first + i) * p.q_sr + j * p.q_sh + d0;
+#pragma unroll
+        for (int e = 0; e < kPer / 4; ++e) {
+          const uint2 x = __ldg(reinterpret_cast<const uint2*>(src) + e);
+          w[2 * e] = x.x, w[2 * e + 1] = x.y;
+        }
+      }
+    };
     auto stage = [&](const Unit& u, int buf) {
-      constexpr int kPer = HD * ROWS / kSoft;  // values of a thread
-      constexpr int kRowThreads = kSoft / ROWS;
-      const int r = tid / kRowThreads, d0 = tid % kRowThreads * kPer;
-      const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) - i * p.group;
       if (d0 == 0) {
+        const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) - i * p.group;
         int lo = 0, hi = 0;
         if (r < u.live) row_range(p, u.v, i, &lo, &hi);
         sm.row_lo[buf][r] = lo;
@@ -319,17 +326,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         sm.row_lse[buf][r] = static_cast<int64_t>(u.v.first + i) * p.nh * p.group + j;
       }
       if (u.t_last > u.t_first) {
-        uint32_t w[kPer / 2];
-#pragma unroll
-        for (int e = 0; e < kPer / 2; ++e) w[e] = 0;
-        if (r < u.live) {
-          const uint16_t* src = reinterpret_cast<const uint16_t*>(p.q) + (u.v.first + i) * p.q_sr + j * p.q_sh + d0;
-#pragma unroll
-          for (int e = 0; e < kPer / 4; ++e) {
-            const uint2 x = __ldg(reinterpret_cast<const uint2*>(src) + e);
-            w[2 * e] = x.x, w[2 * e + 1] = x.y;
-          }
-        }
         float x[kPer], top = 0.f;
 #pragma unroll
         for (int e = 0; e < kPer / 2; ++e) {
@@ -408,10 +404,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     open.first = -1;
     auto close = [&]() {
       if (open.first < 0) return;
-      if (tid == 0) {
-        sm.last = open.ticket == open.last - open.first;
-        __threadfence();
-      }
+      if (tid == 0) sm.last = open.ticket == open.last - open.first;
       soft_sync();
       if (sm.last) {
         for (int idx = tid; idx < open.live * (HD / 4); idx += kSoft) {
@@ -446,6 +439,9 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
 
     int buf = 0;
     bool more = next_unit<ROWS>(p, walk, u);
+    if (more) fetch(u);
+    ready();
+    const uint32_t tmem = sm.tmem;
     if (more) stage(u, 0);
     soft_sync();
     while (more) {
@@ -490,19 +486,22 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         float s[C::kStep][ROWS];
         float top[ROWS], vtop = 0.f, vs[C::kStep];
         const int tok0 = (u.t_first + t * C::kStep) * kTile;
+        uint32_t o[C::kStep][3][ROWS];
+#pragma unroll
+        for (int y = 0; y < C::kStep; ++y)
+#pragma unroll
+          for (int z = 0; z < 3; ++z) tmem_ld(tmem + lanes + C::kScores + ((x & 1) * C::kStep + y) * C::kN + z * ROWS, o[y][z]);
+#pragma unroll
+        for (int y = 0; y < C::kStep; ++y)
+#pragma unroll
+          for (int z = 0; z < 3; ++z) tmem_wait(o[y][z]);
 #pragma unroll
         for (int y = 0; y < C::kStep; ++y) {
-          uint32_t o[3][ROWS];
-          const uint32_t at = tmem + lanes + C::kScores + ((x & 1) * C::kStep + y) * C::kN;
-#pragma unroll
-          for (int z = 0; z < 3; ++z) tmem_ld(at + z * ROWS, o[z]);
-#pragma unroll
-          for (int z = 0; z < 3; ++z) tmem_wait(o[z]);
           const uint32_t k = (tile + y) & 15;
           const float ks = sm.ks[k][piece];
 #pragma unroll
           for (int z = 0; z < ROWS; ++z) {
-            const uint32_t t3[3] = {o[0][z], o[1][z], o[2][z]};
+            const uint32_t t3[3] = {o[y][0][z], o[y][1][z], o[y][2][z]};
             s[y][z] = join_terms<CODE>(t3) * (sm.row_scale[buf][z] * ks);
           }
           vs[y] = sm.vs[k][piece];
@@ -540,8 +539,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
           }
         constexpr float kFull = CODE == MAK_CODE_INT8 ? 127.f * 16777216.f : 256.f;
         const float weight = vtop > 0.f ? kFull / vtop : 0.f;
-        // The step before: its product also is the last reader of the weights' place.
-        if (t > 0) ok = ok && collect(x - 1);
+        float fade[ROWS], next_gain[ROWS];
         uint32_t words[C::kStep][4][ROWS / 4];  // weights of this thread's tokens: term, four rows
 #pragma unroll
         for (int z0 = 0; z0 < ROWS; z0 += 4) {
@@ -560,9 +558,8 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
               w[y][e] *= vs[y] * weight;
             }
             l[z] = l[z] * old + sum * add;
-#pragma unroll
-            for (int h = 0; h < C::kParts; ++h) acc[h][z] *= old;
-            gain[z] = add * vtop * (1.f / kFull);
+            fade[z] = old;
+            next_gain[z] = add * vtop * (1.f / kFull);
             m[z] = mn;
           }
 #pragma unroll
@@ -585,6 +582,14 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             }
           }
         }
+        // The step before: its product is the last reader of the weights' place, and has had until now.
+        if (t > 0) ok = ok && collect(x - 1);
+#pragma unroll
+        for (int z = 0; z < ROWS; ++z) {
+#pragma unroll
+          for (int h = 0; h < C::kParts; ++h) acc[h][z] *= fade[z];
+          gain[z] = next_gain[z];
+        }
         // 16 columns of a token are 16 bytes, the next 16 a step's tokens further on
 #pragma unroll
         for (int y = 0; y < C::kStep; ++y) {
@@ -602,11 +607,15 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             if (tk >= u.any_lo && tk + kTile <= u.any_hi && have == 0xffu) continue;
             const uint32_t slot = (tile + y) % kVs;
             ok = ok && mbar_wait_warp(&sm.v_full[slot], ((tile + y) / kVs) & 1, gave_up);
+            // pieces that are not seen whole
+            uint32_t part = ~have & 0xffu;
+            if (tk < u.any_lo) part |= (2u << ((u.any_lo - tk) >> 4)) - 1;
+            if (tk + kTile > u.any_hi) part |= 0xffu << ((u.any_hi - tk) >> 4);
             for (int d = tid; d < HD; d += kSoft)
-              for (int c = 0; c < 8; ++c) {
+              for (uint32_t left = part & 0xffu; left != 0; left &= left - 1) {
+                const int c = __ffs(left) - 1;
                 const int ct = tk + 16 * c;
                 const bool there = (have >> c) & 1;
-                if (there && ct >= u.any_lo && ct + 16 <= u.any_hi) continue;
                 const int per_line = bs >> 4;  // 16-byte pieces of a line
                 const int swz = p.bs_log2 == 7 ? d & 7 : p.bs_log2 == 6 ? (d >> 1) & 3 : p.bs_log2 == 5 ? (d >> 2) & 1 : 0;
                 uint4* at = reinterpret_cast<uint4*>(sm.v[slot] + (c / per_line) * (HD * bs) + d * bs + (((c % per_line) ^ swz) << 4));
@@ -633,21 +642,29 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       close();
       const Unit done = u;
       more = next_unit<ROWS>(p, walk, u);
-      if (more) stage(u, buf ^ 1);
+      if (more) {
+        fetch(u);
+        stage(u, buf ^ 1);
+      }
       if (ok && n > 0) ok = collect(it + steps - 1);
       it += steps;
       tiles_done += n;
 
       // ---- this block's share of the unit -----------------------------------------
+      {
+        // the rows' sums over the threads, through the weights' place
+        float* sums = reinterpret_cast<float*>(sm.p);
 #pragma unroll
-      for (int z = 0; z < ROWS; ++z) {
-        if (!ok) {  // a block that gave up leaves NaN, not stale memory
-          l[z] = __uint_as_float(0x7fffffffu);
-          m[z] = 0.f;
-        }
+        for (int z = 0; z < ROWS; z += 4)
+          *reinterpret_cast<float4*>(sums + tid * ROWS + z) = make_float4(l[z], l[z + 1], l[z + 2], l[z + 3]);
+        soft_sync();
+        const int z = tid % ROWS, part = tid / ROWS;
+        float sum = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[z] += __shfl_xor_sync(0xffffffffu, l[z], o);
-        if (lane == 0) sm.lsum[warp][z] = l[z];
+        for (int k = 0; k < ROWS; ++k) sum += sums[(part * ROWS + k) * ROWS + z];
+#pragma unroll
+        for (int o = ROWS; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane < ROWS) sm.lsum[warp][z] = ok ? sum : __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN
       }
       soft_sync();
 #pragma unroll
@@ -683,10 +700,8 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         open.buf = buf;
         open.w_tiles = done.w_tiles;
         soft_sync();
-        if (tid == 0) {
-          __threadfence();
-          open.ticket = atomicAdd(p.counters + open.slot, 1);
-        }
+        if (tid == 0)  // releases what the barrier has gathered
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(open.ticket) : "l"(p.counters + open.slot) : "memory");
       }
       buf ^= 1;
     }
@@ -725,6 +740,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       gt += next.count;
     };
     look_ahead();
+    ready();
     Batch b = next;
     next.count = 0;
     bool looked = false;
@@ -797,7 +813,10 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     for (uint32_t i = v_sent > kVs ? v_sent - kVs : 0; i < v_sent; ++i)
       for (uint32_t z = 0; z < kWaitLimit && !mbar_try(&sm.v_full[i % kVs], (i / kVs) & 1); ++z) {
       }
-  } else if (lane == 0) {
+  } else {
+    ready();
+    const uint32_t tmem = sm.tmem;
+    if (lane == 0) {
     // ---- the tensor cores ---------------------------------------------------------
     constexpr int kFmt = CODE == MAK_CODE_INT8 ? 1 : 0, kAcc = CODE == MAK_CODE_INT8 ? 2 : 1;
     constexpr uint32_t kQk = instr_desc(C::kN, kAcc, kFmt, true, false), kPv = instr_desc(C::kN, kAcc, kFmt, false, true);
@@ -876,13 +895,14 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
       }
     }
+    }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 5) {
     __syncwarp();
     tc_fence_after();
-    tmem_free<C::kTmem>(tmem);
+    tmem_free<C::kTmem>(sm.tmem);
   }
 }
 
