@@ -43,7 +43,7 @@ constexpr int kMaxRows = 16;
 constexpr int kMaxDim = 256;
 constexpr int kMinChunk = 2;  // tiles per block that are worth another block
 // A unit's beginning and end (its rows of q, its result) take a block about as long as this many tiles.
-constexpr int kUnitCost = 3;
+constexpr int kUnitCost = 4;
 
 template <int HD, int ROWS>
 struct Cfg {
@@ -979,7 +979,9 @@ int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int
   return MAK_OK;
 }
 
-int launch_block_attn_tc(const BlockAttnParams& p, int head_dim, int code, cudaStream_t st);
+int64_t block_attn_tc_partial_bytes();
+int64_t block_attn_tc_plan_bytes();
+int launch_block_attn_tc(const BlockAttnParams& p, int head_dim, int code, void* plan, cudaStream_t st);
 
 int check_block_cache(const mak_block_cache_desc& c, const char* name) {
   if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
@@ -1007,8 +1009,12 @@ int check_block_cache(const mak_block_cache_desc& c, const char* name) {
 
 using namespace mak;
 
+// counters, the plan of the many-row kernel, partial sums of either kernel
+static int64_t plan_bytes() { return (block_attn_tc_plan_bytes() + 255) / 256 * 256; }
+
 extern "C" int64_t mak_block_attention_workspace_bytes(void) {
-  return kCounterBytes + static_cast<int64_t>(2 * kMaxGrid) * kMaxRows * (kMaxDim + 2) * 4;
+  const int64_t few = static_cast<int64_t>(2 * kMaxGrid) * kMaxRows * (kMaxDim + 2) * 4, many = block_attn_tc_partial_bytes();
+  return kCounterBytes + plan_bytes() + (few > many ? few : many);
 }
 
 extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
@@ -1055,11 +1061,11 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
   p.window = d->window;
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.counters = static_cast<int32_t*>(d->workspace);
-  p.partial = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kCounterBytes);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kCounterBytes + plan_bytes());
   cudaStream_t st = as_stream(stream);
   // Rows that share a cache head, on average: more than 8 fill a second set of columns.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
-  if (rows >= 64 && c.head_dim <= 128) return launch_block_attn_tc(p, c.head_dim, c.code_type, st);
+  if (rows >= 64 && c.head_dim <= 128) return launch_block_attn_tc(p, c.head_dim, c.code_type, static_cast<char*>(d->workspace) + kCounterBytes, st);
   const bool wide = rows > 8 && c.head_dim < 256;
   if (c.head_dim == 64) return wide ? launch_rows_code<64, 16>(p, c.code_type, st) : launch_rows_code<64, 8>(p, c.code_type, st);
   if (c.head_dim == 128) return wide ? launch_rows_code<128, 16>(p, c.code_type, st) : launch_rows_code<128, 8>(p, c.code_type, st);
