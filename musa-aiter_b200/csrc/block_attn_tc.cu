@@ -10,9 +10,9 @@
 //
 // A block takes 256 rows of one cache head (heads of the group next to one another, so a K / V tile
 // serves all of them) as two tiles of 128, and walks the cache in tiles of 128 tokens.  Roles:
-//   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread per row (TMEM lane)
-//   warps 8-11       load codes, convert to f16, store to shared memory
-//   warp 12          one thread issues all tcgen05.mma
+//   warps 0-3, 4-7     softmax of row tile 0 / 1, a thread per row (TMEM lane)
+//   warps 8-11, 12-15  load codes of K / V, convert to f16, store to shared memory
+//   warp 16            one thread issues all tcgen05.mma
 // While one row tile's scores are exponentiated the tensor cores work for the other.
 //
 // Work.  All (row tile, head) units laid end to end, each as long as the tiles it sees, are cut into
@@ -24,6 +24,8 @@
 // it is, in 128-byte swizzled lines of 64 tokens: K is read from there as an MN-major operand and V as
 // a K-major one, so no element is ever transposed.  Scores and weights share TMEM columns: the product
 // with V of a tile is issued before the next scores of the same rows overwrite them.
+#include <utility>
+
 #include "block_attn.cuh"
 #include "tcgen05.cuh"
 
@@ -32,7 +34,7 @@ namespace {
 
 constexpr int kTile = 128;      // tokens per step
 constexpr int kUnitRows = 256;  // rows of a unit
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
 constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolerated
 constexpr float kLift = 6.f;    // log2 factor that weights carry
 constexpr int kUnitCost = 2;    // a unit's beginning and end, in tiles
@@ -153,11 +155,11 @@ struct TcSmem {
   alignas(16) float vlog[4][8], vinv[4][8];  // log2 and reciprocal of V's
   uint32_t have[4], plain[4];                // bit c: piece c has a block; its scales are positive and finite.  0-3 in byte 0, 4-7 in byte 1
   alignas(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], spare;
-  // Walks and units of the softmax warps, the four loading warps and the issuing thread: here, since their
+  // Walks and units of the softmax warps, the eight loading warps and the issuing thread: here, since their
   // registers are needed for scores and codes.
-  Walk walk[6];
-  Unit unit[6];
-  int more[6];
+  Walk walk[10];
+  Unit unit[10];
+  int more[10];
   uint32_t tmem;
   int gave_up, last;
 };
@@ -192,6 +194,16 @@ __device__ __forceinline__ bool next_unit(const BlockAttnParams& p, const Plan* 
     }
     if (u.tb > u.ta) return true;
   }
+}
+
+// f(0), f(1) ... f(N - 1) with the number as a constant.
+template <int N, typename F, int... I>
+__device__ __forceinline__ void steps_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void steps(F f) {
+  steps_of<N>(f, std::make_integer_sequence<int, N>());
 }
 
 __device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init_fence();
   }
-  if (warp == 12) tmem_alloc<512>(&sm.tmem);
+  if (warp == 16) tmem_alloc<512>(&sm.tmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -256,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* gave_up = &sm.gave_up;
 
   if (warp < 8) {
-    regs_up<184>();  // with 96 and 48 below: what the block was launched with
+    regs_up<128>();  // with 80 and 64 below: what the block was launched with
     // ---- softmax ----------------------------------------------------------------
     const int half = warp >> 2;
     const int r = tid & 127;
@@ -342,37 +354,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t have = (sm.have[ring] & 0xfu) | ((sm.have[ring] >> 4) & 0xf0u);
           const uint32_t plain = (sm.plain[ring] & 0xfu) | ((sm.plain[ring] >> 4) & 0xf0u);
           const bool whole = tok >= all_lo && tok + kTile <= all_hi && plain == 0xffu && p.scale_log2 > 0.f;
-          uint32_t x[4][32];  // whole: the row's scores stay in registers
-          float top = -INFINITY;
-          if (whole) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld(s_at + c * 32, x[c]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_wait(x[c]);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {  // 16 columns share their factors
-              const uint32_t* at = &x[c >> 1][(c & 1) * 16];
-              float best = fmaxf(__uint_as_float(at[0]), __uint_as_float(at[1]));
-#pragma unroll
-              for (int e = 2; e < 16; e += 2) best = fmaxf(fmaxf(best, __uint_as_float(at[e])), __uint_as_float(at[e + 1]));
-              top = fmaxf(top, fmaf(best, kf[c] * qs, vlog[c]));
-            }
-          } else {
-#pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-              uint32_t y[16];
-              tmem_ld(s_at + c * 16, y);
-              tmem_wait(y);
-              const float f = kf[c] * qs, b = vlog[c];
-              // columns [from, to) of these 16 are seen
-              const int first = tok + 16 * c, from = lo - first, to = (have >> c) & 1 ? hi - first : 0;
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (e >= from && e < to) top = fmaxf(top, fmaf(__uint_as_float(y[e]), f, b));
-            }
-          }
-          const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
-          if (__any_sync(0xffffffffu, grow)) {
+          // m moves to top for the rows of this warp: sums, accumulators and the weights of this tile's first
+          // `stored` columns follow.
+          auto raise = [&](float top, int stored) {
             const float mn = fmaxf(m, top);
             const float keep = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
             m = mn;
@@ -388,12 +372,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_st(o_at + c * 16, o);
               }
             }
-          }
-          const float ms = m == -INFINITY ? 0.f : m - kLift;
-          asm volatile("" ::: "memory");  // the factors are read again rather than kept beside the scores
+#pragma unroll 1
+            for (int c = 0; c < stored; c += 16) {
+              uint32_t y[8];
+              tc_wait_st();
+              tmem_ld(s_at + c / 2, y);
+              tmem_wait(y);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float2 w = __half22float2(*reinterpret_cast<const __half2*>(&y[e]));
+                y[e] = pack_f16(w.x * keep, w.y * keep);
+              }
+              tmem_st(s_at + c / 2, y);
+            }
+          };
           if (whole) {
+            // 32 columns at a time, the next ones on their way: their maximum, then their weights
+            uint32_t x[2][32];
+            tmem_ld(s_at, x[0]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
+              tmem_wait(x[c & 1]);
+              if (c < 3) tmem_ld(s_at + (c + 1) * 32, x[(c + 1) & 1]);
+              float top = -INFINITY;
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {  // 16 columns share their factors
+                const uint32_t* at = &x[c & 1][z * 16];
+                float best = fmaxf(__uint_as_float(at[0]), __uint_as_float(at[1]));
+#pragma unroll
+                for (int e = 2; e < 16; e += 2) best = fmaxf(fmaxf(best, __uint_as_float(at[e])), __uint_as_float(at[e + 1]));
+                top = fmaxf(top, fmaf(best, kf[2 * c + z] * qs, vlog[2 * c + z]));
+              }
+              const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
+              if (__any_sync(0xffffffffu, grow)) raise(top, c * 32);
+              const float ms = m == -INFINITY ? 0.f : m - kLift;
               uint32_t y[16];
 #pragma unroll
               for (int z = 0; z < 2; ++z) {
@@ -401,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int e = 0; e < 16; e += 2) {
-                  const uint32_t* at = &x[c][z * 16 + e];
+                  const uint32_t* at = &x[c & 1][z * 16 + e];
                   float2 w = fma2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(f, f), make_float2(d, d));
                   w.x = exp2_fast(w.x);
                   w.y = exp2_fast(w.y);
@@ -415,19 +427,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
-              uint32_t x16[16], y[8];
-              tmem_ld(s_at + c * 16, x16);
-              tmem_wait(x16);
-              const float f = kf[c] * qs, w = sm.vfac[ring][c];
+              uint32_t x[16], y[8];
+              tmem_ld(s_at + c * 16, x);
+              tmem_wait(x);
+              const float f = kf[c] * qs, b = vlog[c], w = sm.vfac[ring][c];
+              // columns [from, to) of these 16 are seen
               const int first = tok + 16 * c, from = lo - first, to = (have >> c) & 1 ? hi - first : 0;
+              float top = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (e >= from && e < to) top = fmaxf(top, fmaf(__uint_as_float(x[e]), f, b));
+              const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
+              if (__any_sync(0xffffffffu, grow)) raise(top, c * 16);
+              const float ms = m == -INFINITY ? 0.f : m - kLift;
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                float a = exp2_fast(fmaf(__uint_as_float(x16[e]), f, -ms));
-                float b = exp2_fast(fmaf(__uint_as_float(x16[e + 1]), f, -ms));
-                a = e >= from && e < to ? a : 0.f;
-                b = e + 1 >= from && e + 1 < to ? b : 0.f;
-                l += a + b;
-                y[e >> 1] = pack_f16(a * w, b * w);
+                float p0 = exp2_fast(fmaf(__uint_as_float(x[e]), f, -ms));
+                float p1 = exp2_fast(fmaf(__uint_as_float(x[e + 1]), f, -ms));
+                p0 = e >= from && e < to ? p0 : 0.f;
+                p1 = e + 1 >= from && e + 1 < to ? p1 : 0.f;
+                l += p0 + p1;
+                y[e >> 1] = pack_f16(p0 * w, p1 * w);
               }
               tmem_st(s_at + c * 8, y);
             }
@@ -548,30 +568,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       soft_sync();  // the unit is read
     }
-  } else if (warp < 12) {
-    regs_down<96>();
-    // ---- codes to f16 in shared memory -------------------------------------------
-    const int w = warp - 8;
+  } else if (warp < 16) {
+    regs_down<80>();
+    // ---- codes to f16 in shared memory: K by the first four warps, V by the others ------------------
+    const bool is_v = warp >= 12;
+    const int w = warp & 3, mine = warp - 7;
     const int dlo = lane & 7, chunk16 = (w & 1) * 4 + (lane >> 3);
     const int d0 = (w >> 1) * (HD / 2) + dlo;
     constexpr int kIts = HD / 16;
     const uint32_t to = (chunk16 >> 2) * (HD * 128) + d0 * 128;
     const uint32_t c0 = ((((chunk16 & 3) * 2) ^ dlo) << 4), c1 = ((((chunk16 & 3) * 2 + 1) ^ dlo) << 4);
-    uint4 kx[kIts], vx[kIts];
-    uint32_t g = 0;  // tiles of the units before
+    uint8_t(*const buffers)[HD * 256] = is_v ? sm.v : sm.k;
+    uint64_t *const full = is_v ? sm.v_full : sm.k_full, *const empty = is_v ? sm.v_empty : sm.k_empty;
+    const int64_t stride = is_v ? p.v_sb : p.k_sb;
+    uint4 x[kIts];
+    uint32_t g = 0;  // tiles so far
     bool ok = true;
-    if (lane == 0) sm.walk[1 + w] = walk;
-    const Unit& u = sm.unit[1 + w];
+    if (lane == 0) sm.walk[mine] = walk;
+    const Unit& u = sm.unit[mine];
     while (ok) {
       __syncwarp();
-      if (lane == 0) sm.more[1 + w] = next_unit(p, plan, sm.walk[1 + w], sm.unit[1 + w]);
+      if (lane == 0) sm.more[mine] = next_unit(p, plan, sm.walk[mine], sm.unit[mine]);
       __syncwarp();
-      if (!sm.more[1 + w]) break;
+      if (!sm.more[mine]) break;
       const int n = u.n, t_first = u.t_first, any_lo = u.any_lo, any_hi = u.any_hi, head = u.head;
-      const uint8_t* kb = p.key + head * p.k_sh + static_cast<int64_t>(d0) * bs;
-      const uint8_t* vb = p.value + head * p.v_sh + static_cast<int64_t>(d0) * bs;
+      const uint8_t* base = (is_v ? p.value + head * p.v_sh : p.key + head * p.k_sh) + d0 * bs;
       const int32_t* table = p.tables + u.seq * p.table_stride;
-      float ks = 0.f, vs = 0.f;
       auto token = [&](int t) { return (t_first + t) * kTile + 16 * chunk16; };
       auto find = [&](int t) {
         const int kt = token(t);
@@ -579,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (t < n && kt < any_hi && kt + 16 > any_lo) pg = __ldg(table + (kt >> p.bs_log2));
         return pg >= p.num_blocks ? -1 : pg;
       };
-      auto fetch = [&](const uint8_t* base, int64_t stride, int t, int pg, uint4(&x)[kIts]) {
+      auto fetch = [&](int t, int pg) {
         const uint8_t* src = base + pg * stride + (token(t) & (bs - 1));
         if (pg >= 0) {
 #pragma unroll
@@ -589,17 +611,50 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int it = 0; it < kIts; ++it) x[it] = make_uint4(0, 0, 0, 0);
         }
       };
-      auto store = [&](uint8_t* dst, int t, const uint4(&x)[kIts]) {
+      float ks = 0.f, vs = 0.f;
+      auto scales = [&](int pg) {
+        ks = vs = 0.f;
+        if (!is_v && pg >= 0) {
+          ks = __ldg(p.key_scale + pg * p.ks_sb + head * p.ks_sh);
+          vs = __ldg(p.value_scale + pg * p.vs_sb + head * p.vs_sh);
+        }
+      };
+      int page = find(0), next_page = find(1);
+      if (n > 0) {
+        fetch(0, page);
+        scales(page);
+      }
+      for (int t = 0; t < n; ++t, ++g) {
+        const int st = g & 1;
+        ok = mbar_wait_warp(&empty[st], ((g >> 1) & 1) ^ 1, gave_up);
+        if (!ok) break;
+        if (!is_v) {
+          // the factors of tile g - 4 were last read before tile g - 2's scores were issued
+          const bool fine = page >= 0 && ks > 0.f && ks < INFINITY && vs > 0.f && vs < INFINITY;
+          if (dlo == 0 && w < 2) {
+            sm.kfac[g & 3][chunk16] = ks;
+            sm.vfac[g & 3][chunk16] = vs;
+            // a scale of 0 counts as 2^-100 in the maximum: its weights go into the sum alone
+            sm.vlog[g & 3][chunk16] = vs != 0.f ? log2f(fabsf(vs)) : -100.f;
+            sm.vinv[g & 3][chunk16] = fine ? 1.f / vs : 0.f;
+          }
+          const uint32_t v1 = __ballot_sync(0xffffffffu, page >= 0), v2 = __ballot_sync(0xffffffffu, fine);
+          if (lane == 0 && w < 2) {
+            auto bits = [](uint32_t v) { return static_cast<uint8_t>((v & 1) | ((v >> 7) & 2) | ((v >> 14) & 4) | ((v >> 21) & 8)); };
+            reinterpret_cast<uint8_t*>(&sm.have[g & 3])[w] = bits(v1);
+            reinterpret_cast<uint8_t*>(&sm.plain[g & 3])[w] = bits(v2);
+          }
+        }
         const int kt = token(t);
+        uint8_t* dst = buffers[st] + to;
         auto convert = [&](int it, uint4 z) {
           uint32_t y[8];
           codes4_to_f16<CODE>(z.x, &y[0], &y[1]);
           codes4_to_f16<CODE>(z.y, &y[2], &y[3]);
           codes4_to_f16<CODE>(z.z, &y[4], &y[5]);
           codes4_to_f16<CODE>(z.w, &y[6], &y[7]);
-          uint8_t* line = dst + to + it * 1024;
-          *reinterpret_cast<uint4*>(line + c0) = make_uint4(y[0], y[1], y[2], y[3]);
-          *reinterpret_cast<uint4*>(line + c1) = make_uint4(y[4], y[5], y[6], y[7]);
+          *reinterpret_cast<uint4*>(dst + it * 1024 + c0) = make_uint4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<uint4*>(dst + it * 1024 + c1) = make_uint4(y[4], y[5], y[6], y[7]);
         };
         if (kt < any_lo || kt + 16 > any_hi) {
           // tokens that no row sees: their codes may be anything and become 0
@@ -613,67 +668,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int it = 0; it < kIts; ++it)
-            convert(it, make_uint4(x[it].x & mask[0], x[it].y & mask[1], x[it].z & mask[2], x[it].w & mask[3]));
-        } else {
+            x[it] = make_uint4(x[it].x & mask[0], x[it].y & mask[1], x[it].z & mask[2], x[it].w & mask[3]);
+        }
 #pragma unroll
-          for (int it = 0; it < kIts; ++it) convert(it, x[it]);
-        }
-      };
-      auto scales = [&](int pg) {
-        ks = vs = 0.f;
-        if (pg >= 0) {
-          ks = __ldg(p.key_scale + pg * p.ks_sb + head * p.ks_sh);
-          vs = __ldg(p.value_scale + pg * p.vs_sb + head * p.vs_sh);
-        }
-      };
-      int page = find(0), next_page = find(1);
-      if (n > 0) {
-        fetch(kb, p.k_sb, 0, page, kx);
-        fetch(vb, p.v_sb, 0, page, vx);
-        scales(page);
-      }
-      for (int t = 0; t < n; ++t, ++g) {
-        const int st = g & 1;
-        const uint32_t parity = ((g >> 1) & 1) ^ 1;
-        ok = mbar_wait_warp(&sm.k_empty[st], parity, gave_up);
-        if (!ok) break;
-        // the factors of tile g - 4 were last read before tile g - 2's scores were issued
-        const bool fine = page >= 0 && ks > 0.f && ks < INFINITY && vs > 0.f && vs < INFINITY;
-        if (dlo == 0 && w < 2) {
-          sm.kfac[g & 3][chunk16] = ks;
-          sm.vfac[g & 3][chunk16] = vs;
-          // a scale of 0 counts as 2^-100 in the maximum: its weights go into the sum alone
-          sm.vlog[g & 3][chunk16] = vs != 0.f ? log2f(fabsf(vs)) : -100.f;
-          sm.vinv[g & 3][chunk16] = fine ? 1.f / vs : 0.f;
-        }
-        const uint32_t v1 = __ballot_sync(0xffffffffu, page >= 0), v2 = __ballot_sync(0xffffffffu, fine);
-        if (lane == 0 && w < 2) {
-          auto bits = [](uint32_t v) { return static_cast<uint8_t>((v & 1) | ((v >> 7) & 2) | ((v >> 14) & 4) | ((v >> 21) & 8)); };
-          reinterpret_cast<uint8_t*>(&sm.have[g & 3])[w] = bits(v1);
-          reinterpret_cast<uint8_t*>(&sm.plain[g & 3])[w] = bits(v2);
-        }
-        store(sm.k[st], t, kx);
+        for (int it = 0; it < kIts; ++it) convert(it, x[it]);
         fence_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.k_full[st]);
+        if (lane == 0) mbar_arrive(&full[st]);
         page = next_page;
-        if (t + 1 < n) fetch(kb, p.k_sb, t + 1, page, kx);
-        next_page = find(t + 2);
-        ok = mbar_wait_warp(&sm.v_empty[st], parity, gave_up);
-        if (!ok) break;
-        store(sm.v[st], t, vx);
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.v_full[st]);
         if (t + 1 < n) {
-          fetch(vb, p.v_sb, t + 1, page, vx);
+          fetch(t + 1, page);
           scales(page);
         }
+        next_page = find(t + 2);
       }
     }
   } else {
-    regs_down<48>();
-    if (warp == 12 && lane == 0) {
+    regs_down<64>();
+    if (warp == 16 && lane == 0) {
       // ---- the tensor cores -------------------------------------------------------
       constexpr uint32_t kQk = instr_desc(kTile, 1, 0, false, true), kPv = instr_desc(HD, 1, 0, false, false);
       // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
@@ -682,16 +694,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kBuffer = HD * 256 / 16;
       auto scores = [&](int half, int st) {
         const uint64_t qd = q_desc + half * kBuffer, kd = k_desc + st * kBuffer;
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
-          mma_ss_f16(tmem + half * 128, qd + (ks >> 2) * 1024 + (ks & 3) * 2, kd + ks * 128, kQk, ks > 0);
+        steps<HD / 16>([&](auto i) {
+          constexpr int ks = decltype(i)::value;
+          mma_ss_f16<(ks >> 2) * 1024 + (ks & 3) * 2, ks * 128>(tmem + half * 128, qd, kd, kQk, ks > 0);
+        });
         tc_commit(&sm.s_full[half]);
       };
       uint32_t g = 0, mine[2] = {0, 0}, begins[2] = {0, 0};
       bool ok = true;
-      sm.walk[5] = walk;
-      const Unit& u = sm.unit[5];
-      while (ok && next_unit(p, plan, sm.walk[5], sm.unit[5])) {
+      sm.walk[9] = walk;
+      const Unit& u = sm.unit[9];
+      while (ok && next_unit(p, plan, sm.walk[9], sm.unit[9])) {
         const int n = u.n;
         if (n == 0) continue;
         const int halves = u.live > 128 ? 2 : 1;
@@ -711,9 +724,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             tc_fence_after();
             const uint64_t vd = v_desc + st * kBuffer;
-#pragma unroll
-            for (int ks = 0; ks < kTile / 16; ++ks)
-              mma_ts_f16(tmem + 256 + half * HD, tmem + half * 128 + ks * 8, vd + (ks >> 2) * (HD * 8) + (ks & 3) * 2, kPv, t > 0 || ks > 0);
+            steps<kTile / 16>([&](auto i) {
+              constexpr int ks = decltype(i)::value;
+              mma_ts_f16<ks * 8, (ks >> 2) * (HD * 8) + (ks & 3) * 2>(tmem + 256 + half * HD, tmem + half * 128, vd, kPv, t > 0 || ks > 0);
+            });
             if (half == halves - 1) tc_commit(&sm.v_empty[st]);
             if (t + 1 < n) {
               scores(half, st ^ 1);
@@ -734,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     __syncwarp();
     tc_fence_after();
     tmem_free<512>(tmem);

@@ -78,15 +78,26 @@ __device__ __forceinline__ void tmem_free(uint32_t at) {
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add)                                                               \
                  : "memory");                                                                                                  \
   }
-MAK_MMA_SS(mma_ss_f16, "f16")
 MAK_MMA_SS(mma_ss_f8, "f8f6f4")
 MAK_MMA_SS(mma_ss_i8, "i8")
 #undef MAK_MMA_SS
+// The same in f16 with constants added to the descriptors: written so that the compiler does not keep
+// every sum in a register of its own.
+template <int A, int B>
+__device__ __forceinline__ void mma_ss_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n add.u64 x, %1, %5;\n add.u64 y, %2, %6;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(add), "n"(A), "n"(B)
+      : "memory");
+}
 // D (TMEM, f32) = or += A (TMEM, f16) * B (shared memory, f16)
+template <int A, int B>
 __device__ __forceinline__ void mma_ts_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(add)
+      "{\n .reg .pred p;\n .reg .b32 x;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n add.u32 x, %1, %5;\n add.u64 y, %2, %6;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [x], y, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(add), "n"(A), "n"(B)
       : "memory");
 }
 
