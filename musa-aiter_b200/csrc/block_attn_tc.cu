@@ -5,8 +5,8 @@
 // row of q by a power of two).  The V scale b of a token goes into its exponent: with m' the running
 // maximum of S' + log2 b, the weight 2^(S' + log2 b - m') multiplies the code and, times 1 / b, joins the
 // sum, which is taken in 32 bits before the weight is rounded once to f16.  The maximum is only moved
-// when it grew by more than 2^8: weights then stay below 2^14 (they carry a factor 2^6), the result is
-// the same, and the accumulators in TMEM are rarely rescaled.
+// when it grew by more than 2^8 or so: weights then stay below 2^15 (they carry a factor 2^6), the result
+// is the same, and the accumulators in TMEM are rarely rescaled.
 //
 // A block takes 256 rows of one cache head (heads of the group next to one another, so a K / V tile
 // serves all of them) as two tiles of 128, and walks the cache in tiles of 128 tokens.  Roles:
@@ -37,7 +37,8 @@ constexpr int kUnitRows = 256;  // rows of a unit
 constexpr int kThreads = 640;
 constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolerated
 constexpr float kLift = 6.f;    // log2 factor that weights carry
-constexpr int kUnitCost = 2;    // a unit's beginning and end, in tiles
+constexpr float kSumLimit = 32768.f;  // of 16 weights, below which none of them is near f16's largest
+constexpr int kUnitCost = 4;    // a unit's beginning and end, in tiles
 constexpr int kMinChunk = 4;    // steps of work that are worth another block
 constexpr int kMaxGrid = 148;
 constexpr int kMaxItems = 1 << 16;
@@ -287,50 +288,43 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool on = half * 128 + r < u.live;
       const int64_t row = static_cast<int64_t>(u.tile) * kUnitRows + half * 128 + r;
       float qs = 0.f, m = -INFINITY, l = 0.f;
+      float ref = -1e30f;  // weights are 2^(score - ref): m - kLift, or so low that any score but -inf shows
       if (active && u.n > 0) {
         int lo = 0, hi = 0;
         {  // this row of q to f16
           const int i = on ? static_cast<int>(row / p.group) : 0, j = on ? static_cast<int>(row % p.group) : 0;
           if (on) row_range(p, u.v, i, &lo, &hi);
-          // two passes over it, four 16-byte pieces at a time: few registers are left beside the scores
           const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (u.v.first + i) * p.q_sr +
                                                             (u.head * p.group + j) * p.q_sh);
+          uint4 x[HD / 8];
+#pragma unroll
+          for (int e = 0; e < HD / 8; ++e) x[e] = on ? __ldg(src + e) : make_uint4(0, 0, 0, 0);
           int up = 0;
-          float f1 = 1.f, f2 = 1.f;
           if (p.q_bf16) {
             float top = 0.f;
-#pragma unroll 1
-            for (int e = 0; e < HD / 8; e += 4) {
 #pragma unroll
-              for (int z = 0; z < 4; ++z) {
-                const uint4 x = on ? __ldg(src + e + z) : make_uint4(0, 0, 0, 0);
+            for (int e = 0; e < HD / 8; ++e) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                  const uint32_t b = (&x.x)[w];
-                  top = fmaxf(top, fmaxf(fabsf(__uint_as_float(b << 16)), fabsf(__uint_as_float(b & 0xffff0000u))));
-                }
+              for (int w = 0; w < 4; ++w) {
+                const uint32_t b = (&x[e].x)[w];
+                top = fmaxf(top, fmaxf(fabsf(__uint_as_float(b << 16)), fabsf(__uint_as_float(b & 0xffff0000u))));
               }
             }
             if (top > 0.f && top < __uint_as_float(0x7f800000u)) up = 14 - ilogbf(top);
             const int up1 = up / 2, up2 = up - up1;
-            f1 = __uint_as_float(static_cast<uint32_t>(127 + up1) << 23);
-            f2 = __uint_as_float(static_cast<uint32_t>(127 + up2) << 23);
-          }
-#pragma unroll 1
-          for (int e = 0; e < HD / 8; e += 4) {
+            const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up1) << 23), f2 = __uint_as_float(static_cast<uint32_t>(127 + up2) << 23);
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              uint4 x = on ? __ldg(src + e + z) : make_uint4(0, 0, 0, 0);
-              if (p.q_bf16) {
+            for (int e = 0; e < HD / 8; ++e) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                  uint32_t& b = (&x.x)[w];
-                  b = pack_f16(__uint_as_float(b << 16) * f1 * f2, __uint_as_float(b & 0xffff0000u) * f1 * f2);
-                }
+              for (int w = 0; w < 4; ++w) {
+                uint32_t& b = (&x[e].x)[w];
+                b = pack_f16(__uint_as_float(b << 16) * f1 * f2, __uint_as_float(b & 0xffff0000u) * f1 * f2);
               }
-              *reinterpret_cast<uint4*>(sm.q[half] + ((e + z) >> 3) * 16384 + r * 128 + ((((e + z) & 7) ^ (r & 7)) << 4)) = x;
             }
           }
+#pragma unroll
+          for (int e = 0; e < HD / 8; ++e)
+            *reinterpret_cast<uint4*>(sm.q[half] + (e >> 3) * 16384 + r * 128 + (((e & 7) ^ (r & 7)) << 4)) = x[e];
           qs = ldexpf(p.scale_log2, -up);
           fence_async_shared();
           tc_fence_before();
@@ -353,13 +347,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float *kf = sm.kfac[ring], *vlog = sm.vlog[ring];
           const uint32_t have = (sm.have[ring] & 0xfu) | ((sm.have[ring] >> 4) & 0xf0u);
           const uint32_t plain = (sm.plain[ring] & 0xfu) | ((sm.plain[ring] >> 4) & 0xf0u);
-          const bool whole = tok >= all_lo && tok + kTile <= all_hi && plain == 0xffu && p.scale_log2 > 0.f;
+          const bool whole = tok >= all_lo && tok + kTile <= all_hi && have == 0xffu;
           // m moves to top for the rows of this warp: sums, accumulators and the weights of this tile's first
           // `stored` columns follow.
           auto raise = [&](float top, int stored) {
             const float mn = fmaxf(m, top);
             const float keep = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
             m = mn;
+            ref = m == -INFINITY ? -1e30f : m - kLift;
             l *= keep;
             if (t > 0) {
 #pragma unroll 1
@@ -386,42 +381,64 @@ __global__ void __launch_bounds__(kThreads, 1)
               tmem_st(s_at + c / 2, y);
             }
           };
-          if (whole) {
-            // 32 columns at a time, the next ones on their way: their maximum, then their weights
+          if (plain == 0xffu && p.scale_log2 > 0.f) {
+            // 32 columns at a time, the next ones on their way.  Weights are taken against the maximum so far; only when
+            // a sum of 16 of them shows that the maximum has grown too much is it looked for, and they are taken again.
+            if (!whole) {  // scores that their row does not see become -inf
+#pragma unroll 1
+              for (int c = 0; c < 8; ++c) {
+                const int first = tok + 16 * c, from = lo - first, to = (have >> c) & 1 ? hi - first : 0;
+                if (!__any_sync(0xffffffffu, from > 0 || to < 16)) continue;
+                uint32_t z[16];
+                tmem_ld(s_at + c * 16, z);
+                tmem_wait(z);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) z[e] = e >= from && e < to ? z[e] : 0xff800000u;
+                tmem_st(s_at + c * 16, z);
+              }
+              tc_wait_st();
+            }
             uint32_t x[2][32];
             tmem_ld(s_at, x[0]);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               tmem_wait(x[c & 1]);
               if (c < 3) tmem_ld(s_at + (c + 1) * 32, x[(c + 1) & 1]);
-              float top = -INFINITY;
-#pragma unroll
-              for (int z = 0; z < 2; ++z) {  // 16 columns share their factors
-                const uint32_t* at = &x[c & 1][z * 16];
-                float best = fmaxf(__uint_as_float(at[0]), __uint_as_float(at[1]));
-#pragma unroll
-                for (int e = 2; e < 16; e += 2) best = fmaxf(fmaxf(best, __uint_as_float(at[e])), __uint_as_float(at[e + 1]));
-                top = fmaxf(top, fmaf(best, kf[2 * c + z] * qs, vlog[2 * c + z]));
-              }
-              const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
-              if (__any_sync(0xffffffffu, grow)) raise(top, c * 32);
-              const float ms = m == -INFINITY ? 0.f : m - kLift;
               uint32_t y[16];
+              float2 sum[2];
+              auto weights = [&](float ms) {
 #pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                const float f = kf[2 * c + z] * qs, d = vlog[2 * c + z] - ms;
-                float2 sum = make_float2(0.f, 0.f);
+                for (int z = 0; z < 2; ++z) {  // 16 columns share their factors
+                  const float f = fmaxf(kf[2 * c + z] * qs, 1e-37f), d = vlog[2 * c + z] - ms;  // not 0: masked scores are -inf
+                  sum[z] = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                  const uint32_t* at = &x[c & 1][z * 16 + e];
-                  float2 w = fma2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(f, f), make_float2(d, d));
-                  w.x = exp2_fast(w.x);
-                  w.y = exp2_fast(w.y);
-                  sum = add2(sum, w);
-                  y[(z * 16 + e) >> 1] = pack_f16(w.x, w.y);
+                  for (int e = 0; e < 16; e += 2) {
+                    const uint32_t* at = &x[c & 1][z * 16 + e];
+                    float2 w = fma2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(f, f), make_float2(d, d));
+                    w.x = exp2_fast(w.x);
+                    w.y = exp2_fast(w.y);
+                    sum[z] = add2(sum[z], w);
+                    y[(z * 16 + e) >> 1] = pack_f16(w.x, w.y);
+                  }
+                  sum[z].x += sum[z].y;
                 }
-                l = fmaf(sum.x + sum.y, sm.vinv[ring][2 * c + z], l);
+              };
+              weights(ref);
+              if (__any_sync(0xffffffffu, fmaxf(sum[0].x, sum[1].x) > kSumLimit)) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                  const uint32_t* at = &x[c & 1][z * 16];
+                  float best = fmaxf(__uint_as_float(at[0]), __uint_as_float(at[1]));
+#pragma unroll
+                  for (int e = 2; e < 16; e += 2) best = fmaxf(fmaxf(best, __uint_as_float(at[e])), __uint_as_float(at[e + 1]));
+                  top = fmaxf(top, fmaf(best, kf[2 * c + z] * qs, vlog[2 * c + z]));
+                }
+                raise(top, c * 32);
+                weights(ref);
               }
+              l = fmaf(sum[0].x, sm.vinv[ring][2 * c], l);
+              l = fmaf(sum[1].x, sm.vinv[ring][2 * c + 1], l);
               tmem_st(s_at + c * 16, y);
             }
           } else {
@@ -613,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       float ks = 0.f, vs = 0.f;
       auto scales = [&](int pg) {
-        ks = vs = 0.f;
+        ks = vs = 1.f;  // where there is no block nothing is seen
         if (!is_v && pg >= 0) {
           ks = __ldg(p.key_scale + pg * p.ks_sb + head * p.ks_sh);
           vs = __ldg(p.value_scale + pg * p.vs_sb + head * p.vs_sh);
@@ -626,11 +643,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int t = 0; t < n; ++t, ++g) {
         const int st = g & 1;
-        ok = mbar_wait_warp(&empty[st], ((g >> 1) & 1) ^ 1, gave_up);
+        ok = mbar_wait_warp_idle(&empty[st], ((g >> 1) & 1) ^ 1, gave_up);
         if (!ok) break;
         if (!is_v) {
           // the factors of tile g - 4 were last read before tile g - 2's scores were issued
-          const bool fine = page >= 0 && ks > 0.f && ks < INFINITY && vs > 0.f && vs < INFINITY;
+          const bool fine = ks > 0.f && ks < INFINITY && vs > 0.f && vs < INFINITY;
           if (dlo == 0 && w < 2) {
             sm.kfac[g & 3][chunk16] = ks;
             sm.vfac[g & 3][chunk16] = vs;

@@ -42,6 +42,19 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity, vol
   return __all_sync(0xffffffffu, mbar_wait(b, parity, gave_up));
 }
 
+// For warps with time to spare: between looks they leave the issue slots to others.
+__device__ __forceinline__ bool mbar_wait_warp_idle(uint64_t* b, uint32_t parity, volatile int* gave_up) {
+  bool ok = false;
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    ok = mbar_try(b, parity);
+    if (ok) break;
+    __nanosleep(100);
+    if ((i & 255) == 255 && *gave_up) break;
+  }
+  if (!ok) *gave_up = 1;
+  return __all_sync(0xffffffffu, ok);
+}
+
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
