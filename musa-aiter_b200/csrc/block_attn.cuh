@@ -106,6 +106,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
   asm("{\n .reg .b64 w, x, y, z;\n mov.b64 w, {%2, %3};\n mov.b64 x, {%4, %5};\n mov.b64 y, {%6, %7};\n fma.rn.f32x2 z, w, x, y;\n"

@@ -286,13 +286,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!sm.more[0]) break;
       const bool active = half * 128 < u.live;
       const bool on = half * 128 + r < u.live;
-      const int64_t row = static_cast<int64_t>(u.tile) * kUnitRows + half * 128 + r;
+      const uint32_t row = u.tile * kUnitRows + half * 128 + r;  // below 2^24: see kMaxItems
       float qs = 0.f, m = -INFINITY, l = 0.f;
       float ref = -1e30f;  // weights are 2^(score - ref): m - kLift, or so low that any score but -inf shows
       if (active && u.n > 0) {
         int lo = 0, hi = 0;
         {  // this row of q to f16
-          const int i = on ? static_cast<int>(row / p.group) : 0, j = on ? static_cast<int>(row % p.group) : 0;
+          const int i = on ? row / p.group : 0, j = on ? row % p.group : 0;
           if (on) row_range(p, u.v, i, &lo, &hi);
           const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.q) + (u.v.first + i) * p.q_sr +
                                                             (u.head * p.group + j) * p.q_sh);
@@ -301,25 +301,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < HD / 8; ++e) x[e] = on ? __ldg(src + e) : make_uint4(0, 0, 0, 0);
           int up = 0;
           if (p.q_bf16) {
-            float top = 0.f;
+            __nv_bfloat162 tops = __float2bfloat162_rn(0.f);
 #pragma unroll
-            for (int e = 0; e < HD / 8; ++e) {
+            for (int e = 0; e < HD / 2; ++e) tops = __hmax2(tops, __habs2(reinterpret_cast<const __nv_bfloat162*>(x)[e]));
+            const float top = fmaxf(__low2float(tops), __high2float(tops));
+            // the largest comes to 2^14 or, if it is below 2^-113, less
+            if (top > 0.f && top < __uint_as_float(0x7f800000u)) up = min(14 - ilogbf(top), 127);
+            const float factor = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
 #pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint32_t b = (&x[e].x)[w];
-                top = fmaxf(top, fmaxf(fabsf(__uint_as_float(b << 16)), fabsf(__uint_as_float(b & 0xffff0000u))));
-              }
-            }
-            if (top > 0.f && top < __uint_as_float(0x7f800000u)) up = 14 - ilogbf(top);
-            const int up1 = up / 2, up2 = up - up1;
-            const float f1 = __uint_as_float(static_cast<uint32_t>(127 + up1) << 23), f2 = __uint_as_float(static_cast<uint32_t>(127 + up2) << 23);
-#pragma unroll
-            for (int e = 0; e < HD / 8; ++e) {
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                uint32_t& b = (&x[e].x)[w];
-                b = pack_f16(__uint_as_float(b << 16) * f1 * f2, __uint_as_float(b & 0xffff0000u) * f1 * f2);
-              }
+            for (int e = 0; e < HD / 2; ++e) {
+              uint32_t& b = reinterpret_cast<uint32_t*>(x)[e];
+              const float2 w = mul2(make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), make_float2(factor, factor));
+              b = pack_f16(w.x, w.y);
             }
           }
 #pragma unroll
@@ -484,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) l = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN, not stale memory
 
       // ---- this block's share of the unit -------------------------------------------
-      const int i = on ? static_cast<int>(row / p.group) : 0, j = on ? static_cast<int>(row % p.group) : 0;
+      const int i = on ? row / p.group : 0, j = on ? row % p.group : 0;
       const int64_t at = (u.v.first + i) * p.o_sr + (u.head * p.group + j) * p.o_sh;
       auto put = [&](int d, const float(&o)[16], float inv) {
         uint32_t y[8];
@@ -570,11 +563,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               float o[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = 0.f;
-              for (int b = first_block; b <= last_block; ++b) {
-                const float* src = from(b);
-                const float k = exp2_fast(__ldcg(src + HD * kUnitRows) - ms);
+#pragma unroll 1
+              for (int b = first_block; b <= last_block; b += 2) {  // two blocks' loads at a time
+                const float *src = from(b), *src2 = from(min(b + 1, last_block));
+                float x[16], x2[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = fmaf(__ldcg(src + (d + e) * kUnitRows), k, o[e]);
+                for (int e = 0; e < 16; ++e) x[e] = __ldcg(src + (d + e) * kUnitRows), x2[e] = __ldcg(src2 + (d + e) * kUnitRows);
+                const float k = exp2_fast(__ldcg(src + HD * kUnitRows) - ms), k2 = b < last_block ? exp2_fast(__ldcg(src2 + HD * kUnitRows) - ms) : 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = fmaf(x2[e], k2, fmaf(x[e], k, o[e]));
               }
               put(d, o, inv);
             }
