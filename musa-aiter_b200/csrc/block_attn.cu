@@ -911,27 +911,18 @@ int launch_rows(const BlockAttnParams& p, cudaStream_t st) {
   const auto kernel = block_attn_rows_kernel<HD, ROWS, CODE>;
   constexpr int kBytes = sizeof(Smem<HD, ROWS>);
   static_assert(kBytes <= (HD == 256 ? 227 : 113) * 1024, "blocks per SM");  // 228 KB less 1 KB per block
-  static int per_sm = 0;
-  if (per_sm == 0) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (e != cudaSuccess) {
-      (void)cudaGetLastError();
-      return cuda_fail(e, "mak_block_attention");
-    }
-    // The occupancy query answers 1 for these kernels; two blocks do run where their shared memory,
-    // registers and TMEM columns fit twice (11.7 of 12 warps active on average).
-    int n = HD == 256 ? 1 : 2;
-    // TMEM has 512 columns, and a block whose allocation has to wait for another's end gains nothing
-    if (n * Cfg<HD, ROWS>::kTmem > 512) n = 512 / Cfg<HD, ROWS>::kTmem;
-    per_sm = n;
-  }
+  // The occupancy query answers 1 for these kernels; two blocks do run where their shared memory, registers and
+  // TMEM columns fit twice (11.7 of 12 warps active on average).  TMEM has 512 columns, and a block whose allocation
+  // has to wait for another's end gains nothing.
+  constexpr int kPerSm = HD == 256 || 2 * Cfg<HD, ROWS>::kTmem > 512 ? 1 : 2;
+  static bool ready[kMaxDevices] = {};
+  if (int rc = prepare_kernel(kernel, kBytes, ready)) return rc;
   CUtensorMap maps[2] = {};
   if (p.bs_log2 > 4 && p.num_blocks > 0) {
-    if (int rc = cache_map(&maps[0], p.key, p.k_sb, p.k_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2, true)) return rc;
-    if (int rc = cache_map(&maps[1], p.value, p.v_sb, p.v_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2, true)) return rc;
+    if (int rc = cache_map(&maps[0], p.key, p.k_sb, p.k_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2)) return rc;
+    if (int rc = cache_map(&maps[1], p.value, p.v_sb, p.v_sh, p.num_blocks, p.nh, HD, 1 << p.bs_log2)) return rc;
   }
-  int64_t grid = per_sm * sm_count();
+  int64_t grid = kPerSm * sm_count();
   if (grid > kMaxGrid) grid = kMaxGrid;
   // no more blocks than there can be work for
   const int64_t seq_tiles = ((static_cast<int64_t>(p.max_blocks) << p.bs_log2) + kTile - 1) / kTile + 1 + kUnitCost;
@@ -950,8 +941,7 @@ constexpr int64_t kCounterBytes = (2 * kMaxGrid * 4 + 255) / 256 * 256;
 
 }  // namespace
 
-int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs,
-              bool swizzled) {
+int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -971,7 +961,7 @@ int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int
   const cuuint64_t strides[3] = {static_cast<cuuint64_t>(bs), static_cast<cuuint64_t>(sh), static_cast<cuuint64_t>(sb)};
   const cuuint32_t box[4] = {static_cast<cuuint32_t>(bs), static_cast<cuuint32_t>(hd), 1, 1}, steps[4] = {1, 1, 1, 1};
   const CUtensorMapSwizzle swizzle =
-      !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : bs == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bs == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
+      bs == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : bs == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
   const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, steps,
                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -981,6 +971,7 @@ int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int
 
 int64_t block_attn_tc_partial_bytes();
 int64_t block_attn_tc_plan_bytes();
+bool block_attn_tc_fits(const BlockAttnParams& p);
 int launch_block_attn_tc(const BlockAttnParams& p, int head_dim, int code, void* plan, cudaStream_t st);
 
 int check_block_cache(const mak_block_cache_desc& c, const char* name) {
@@ -1063,10 +1054,17 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
   p.counters = static_cast<int32_t*>(d->workspace);
   p.partial = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kCounterBytes + plan_bytes());
   cudaStream_t st = as_stream(stream);
-  // Rows that share a cache head, on average: more than 8 fill a second set of columns.
+  // Rows that share a cache head, on average.  Above 32 the many-row kernel costs less whatever the lengths:
+  // 16 sequences of 4096 tokens, 8 cache heads of 128: 32 rows 81.6 us here and 83.9 there, 40 rows 117 and 84, 64 rows
+  // 154 and 85; heads of 64: 32 rows 74 and 70, 64 rows 137 and 71; one sequence of 2000: 64 rows 23.3 and 25.3, 128 rows
+  // 26.6 and 28.0, of 16000: 64 rows 46 and 43, 128 rows 73 and 55.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
-  if (rows >= 64 && c.head_dim <= 128) return launch_block_attn_tc(p, c.head_dim, c.code_type, static_cast<char*>(d->workspace) + kCounterBytes, st);
-  const bool wide = rows > 8 && c.head_dim < 256;
+  if (rows > 32 && c.head_dim <= 128 && block_attn_tc_fits(p))
+    return launch_block_attn_tc(p, c.head_dim, c.code_type, static_cast<char*>(d->workspace) + kCounterBytes, st);
+  // Groups of 16 rows instead of 8, but where three of 8 hold them: the same cache, heads of 128, groups of 8 and of 16:
+  // 8 rows 36 and 50 us, 12 rows 52.2 and 51.7, 16 rows 52.8 and 52.8, 24 rows 73 and 81, 32 rows 94 and 81; heads of 64:
+  // 12 rows 50 and 45, 24 rows 67 and 73, 32 rows 87 and 74.  Heads of 256 leave shared memory for groups of 8 alone.
+  const bool wide = c.head_dim < 256 && rows > 8 && (rows <= 16 || rows > 24);
   if (c.head_dim == 64) return wide ? launch_rows_code<64, 16>(p, c.code_type, st) : launch_rows_code<64, 8>(p, c.code_type, st);
   if (c.head_dim == 128) return wide ? launch_rows_code<128, 16>(p, c.code_type, st) : launch_rows_code<128, 8>(p, c.code_type, st);
   return launch_rows_code<256, 8>(p, c.code_type, st);

@@ -87,9 +87,26 @@ __device__ __forceinline__ void codes4_to_f16(uint32_t w, uint32_t* lo, uint32_t
   }
 }
 
+// Once per device: shared memory for a kernel's blocks.
+constexpr int kMaxDevices = 64;
+template <typename K>
+int prepare_kernel(K kernel, int bytes, bool (&ready)[kMaxDevices]) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && device < kMaxDevices && ready[device]) return MAK_OK;
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return cuda_fail(e, "mak_block_attention");
+  }
+  if (device < kMaxDevices) ready[device] = true;
+  return MAK_OK;
+}
+
 // [num_blocks][num_heads][head_dim][block_size] bytes as boxes of one head of one block, lines of
-// block_size bytes swizzled or as they are.
-int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool swizzled);
+// block_size bytes swizzled.
+int cache_map(CUtensorMap* map, const uint8_t* base, int64_t sb, int64_t sh, int64_t num_blocks, int nh, int hd, int bs);
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;

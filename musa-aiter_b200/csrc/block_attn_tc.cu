@@ -477,9 +477,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) l = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN, not stale memory
 
       // ---- this block's share of the unit -------------------------------------------
-      const int i = on ? row / p.group : 0, j = on ? row % p.group : 0;
-      const int64_t at = (u.v.first + i) * p.o_sr + (u.head * p.group + j) * p.o_sh;
-      auto put = [&](int d, const float(&o)[16], float inv) {
+      auto place = [&](uint32_t row, uint16_t*& dst, float*& lse) {  // of a row's result
+        const uint32_t i = row / p.group, j = row % p.group;
+        dst = reinterpret_cast<uint16_t*>(p.out) + (u.v.first + i) * p.o_sr + (u.head * p.group + j) * p.o_sh;
+        lse = p.lse == nullptr ? nullptr : p.lse + (static_cast<int64_t>(u.v.first + i) * p.nh + u.head) * p.group + j;
+      };
+      auto put = [&](uint16_t* dst, const float(&o)[16], float inv) {
         uint32_t y[8];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
@@ -490,7 +493,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             y[e >> 1] = pack_f16(o[e] * inv, o[e + 1] * inv);
           }
         }
-        uint16_t* dst = reinterpret_cast<uint16_t*>(p.out) + at + d;
         if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
           reinterpret_cast<uint4*>(dst)[0] = make_uint4(y[0], y[1], y[2], y[3]);
           reinterpret_cast<uint4*>(dst)[1] = make_uint4(y[4], y[5], y[6], y[7]);
@@ -502,15 +504,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       };
-      auto put_lse = [&](float mx, float sum) {
-        if (p.lse != nullptr)
-          p.lse[static_cast<int64_t>(u.v.first + i) * p.nh * p.group + u.head * p.group + j] =
-              sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+      auto put_lse = [&](float* lse, float mx, float sum) {
+        if (lse != nullptr) *lse = sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
       };
       const bool split = u.ta > 0 || u.tb < u.len;
       constexpr int kFloats = kUnitRows * (HD + 2);  // of one partial sum: [HD][256], maxima, sums
       float* part = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (u.w_tiles > w_begin ? 1 : 0)) * kFloats;
       if (active) {
+        uint16_t* dst = nullptr;
+        float* lse = nullptr;
+        if (on) place(row, dst, lse);
         const float inv = l > 0.f || l != l ? 1.f / l * (1.f / (1 << static_cast<int>(kLift))) : 0.f;
 #pragma unroll 1
         for (int d = 0; d < HD; d += 16) {
@@ -526,14 +529,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) part[(d + e) * kUnitRows + tid] = o[e] * (1.f / (1 << static_cast<int>(kLift)));
           } else if (on) {
-            put(d, o, inv);
+            put(dst + d, o, inv);
           }
         }
         if (split) {
           part[HD * kUnitRows + tid] = m;
           part[HD * kUnitRows + kUnitRows + tid] = l;
         } else if (on) {
-          put_lse(m, l);
+          put_lse(lse, m, l);
         }
       }
       tc_fence_before();
@@ -548,9 +551,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         soft_sync();
         if (sm.last) {
-          if (on) {
+          // Few rows leave several threads for each, which share its columns.  Four blocks' loads at a time.
+          const int span = u.live > 128 ? 256 : u.live > 64 ? 128 : 64, mine_row = tid & (span - 1), cols = HD * span / kUnitRows;
+          if (mine_row < u.live) {
+            auto from = [&](int b) {
+              return p.partial + (2 * static_cast<int64_t>(b) + (u.w_tiles > b * chunk ? 1 : 0)) * kFloats + mine_row;
+            };
             float mx = -INFINITY, sum = 0.f;
-            auto from = [&](int b) { return p.partial + (2 * static_cast<int64_t>(b) + (u.w_tiles > b * chunk ? 1 : 0)) * kFloats + tid; };
+#pragma unroll 4
             for (int b = first_block; b <= last_block; ++b) {
               const float pm = __ldcg(from(b) + HD * kUnitRows), pl = __ldcg(from(b) + HD * kUnitRows + kUnitRows);
               const float mn = fmaxf(mx, pm), ms = mn == -INFINITY ? 0.f : mn;
@@ -558,24 +566,34 @@ __global__ void __launch_bounds__(kThreads, 1)
               mx = mn;
             }
             const float ms = mx == -INFINITY ? 0.f : mx, inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+            uint16_t* dst;
+            float* lse;
+            place(u.tile * kUnitRows + mine_row, dst, lse);
 #pragma unroll 1
-            for (int d = 0; d < HD; d += 16) {
+            for (int d = tid / span * cols, end = d + cols; d < end; d += 16) {
               float o[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = 0.f;
 #pragma unroll 1
-              for (int b = first_block; b <= last_block; b += 2) {  // two blocks' loads at a time
-                const float *src = from(b), *src2 = from(min(b + 1, last_block));
-                float x[16], x2[16];
+              for (int b = first_block; b <= last_block; b += 4) {
+                float x[4][16], k[4];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = __ldcg(src + (d + e) * kUnitRows), x2[e] = __ldcg(src2 + (d + e) * kUnitRows);
-                const float k = exp2_fast(__ldcg(src + HD * kUnitRows) - ms), k2 = b < last_block ? exp2_fast(__ldcg(src2 + HD * kUnitRows) - ms) : 0.f;
+                for (int z = 0; z < 4; ++z) {
+                  const float* src = from(min(b + z, last_block));
+                  k[z] = __ldcg(src + HD * kUnitRows);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = fmaf(x2[e], k2, fmaf(x[e], k, o[e]));
+                  for (int e = 0; e < 16; ++e) x[z][e] = __ldcg(src + (d + e) * kUnitRows);
+                }
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  k[z] = b + z <= last_block ? exp2_fast(k[z] - ms) : 0.f;
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = b + z <= last_block ? fmaf(x[z][e], k[z], o[e]) : o[e];
+                }
               }
-              put(d, o, inv);
+              put(dst + d, o, inv);
             }
-            put_lse(mx, sum);
+            if (tid < span) put_lse(lse, mx, sum);
           }
           if (tid == 0) p.counters[slot0] = 0;
         }
@@ -769,22 +787,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// Row tiles of all sequences, at most.
+int64_t row_tiles(const BlockAttnParams& p) { return static_cast<int64_t>(p.num_rows) * p.group / kUnitRows + p.num_seqs; }
+
 template <int HD, int CODE>
 int launch_tc(const BlockAttnParams& p, Plan* plan, cudaStream_t st) {
   constexpr int kBytes = sizeof(TcSmem<HD>);
   static_assert(kBytes <= 227 * 1024, "shared memory of a block");
   const auto kernel = block_attn_tc_kernel<HD, CODE>;
-  static bool set = false;
-  if (!set) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-    if (e != cudaSuccess) {
-      (void)cudaGetLastError();
-      return cuda_fail(e, "mak_block_attention");
-    }
-    set = true;
-  }
-  const int64_t items = static_cast<int64_t>(p.num_rows) * p.group / kUnitRows + p.num_seqs;
-  if (items > kMaxItems) return fail(MAK_E_UNSUPPORTED, "mak_block_attention: too many rows for one call");
+  static bool ready[kMaxDevices] = {};
+  if (int rc = prepare_kernel(kernel, kBytes, ready)) return rc;
+  const int64_t items = row_tiles(p);
   if (int rc = launch_pdl("mak_block_attention", block_attn_plan_kernel, dim3(1), dim3(1024), 0, st, p, plan, static_cast<int>(items)))
     return rc;
   const int sms = sm_count();
@@ -795,6 +808,7 @@ int launch_tc(const BlockAttnParams& p, Plan* plan, cudaStream_t st) {
 }  // namespace
 
 int64_t block_attn_tc_partial_bytes() { return static_cast<int64_t>(2 * kMaxGrid) * kUnitRows * (128 + 2) * 4; }
+bool block_attn_tc_fits(const BlockAttnParams& p) { return row_tiles(p) <= kMaxItems; }
 int64_t block_attn_tc_plan_bytes() { return sizeof(Plan); }
 
 int launch_block_attn_tc(const BlockAttnParams& p, int head_dim, int code, void* plan, cudaStream_t st) {
