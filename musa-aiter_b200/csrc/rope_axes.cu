@@ -171,10 +171,11 @@ extern "C" int mak_rope_axes(const mak_rope_axes_desc* desc, void* stream) {
   if ((addr & 15) || (strides & 7)) return fail(MAK_E_INVALID, "%s: rows need 16-byte alignment", name);
   p.rot_slots = d.rot_dim / (d.interleaved ? 8 : 16);
   p.slots = p.rot_slots + (d.head_dim - d.rot_dim) / 8;
-  // A thread takes several heads once there are enough tokens to fill the GPU without that.
+  // A thread takes up to 8 heads, as many as leave each SM 128 threads: it reads its angles once for all of them.
+  // 40 heads of 128, tokens: us with 1, 4 and 8 heads a thread: 64: 2.8, 3.4, 4.2; 256: 5.2, 3.4, 4.2;
+  // 1024: 13.0, 6.7, 6.3; 4096: 50, 19, 16.5; 16384: 202, 72, 61.
   const int64_t threads = d.tokens * p.slots * heads;
-  const int64_t full = static_cast<int64_t>(sm_count()) * 2048;
-  int64_t per = threads / (2 * full);
+  int64_t per = threads / (static_cast<int64_t>(sm_count()) * 128);
   per = per < 1 ? 1 : per > 8 ? 8 : per;
   p.per_group = static_cast<int32_t>(per);
   p.groups = (heads + p.per_group - 1) / p.per_group;
