@@ -29,6 +29,14 @@
 // alone.  A unit cut by that leaves partial sums (maximum, sum, accumulators) and the last block
 // to arrive joins them.  Roles: warps 0-3 softmax (a thread per token, then per head_dim row),
 // warp 4 copies, warp 5 issues the tensor cores; two steps are in flight between them.
+//
+// Measured (a copy runs at 6.47 TB/s).  4 sequences of 100000 to 131072 tokens, 8 cache heads of 128 with 8 query
+// heads each, E4M3, blocks of 64: 158 us, 5.8 TB/s, bound by HBM.  64 sequences of 256 to 4096, 4 query heads each,
+// blocks of 16: 77 us, 3.8 TB/s: a block gets two or three units, and between units the copies wait for some 10000
+// cycles (masks of the last step, the next rows of q, the sums), as what they run ahead by is a step of K and one of
+// V, all that shared memory holds.  Taking the next unit's rows and first scores before the last step ends: 82 us, as
+// the loop grows.  16 sequences of 300 to 4500, 16 heads of 64 on one cache head, 1 to 8 rows: 26 to 28 us, either
+// kernel.  One sequence of 777 tokens: 10.8 us, a chain of latencies (lengths, block ids, K, scores, weights, sums).
 #include "block_attn.cuh"
 #include "tcgen05.cuh"
 
@@ -41,8 +49,10 @@ constexpr int kSoft = 128;  // threads of the softmax warps
 constexpr int kMaxGrid = 148 * 4;  // blocks of the largest grid; the workspace has two partial sums for each
 constexpr int kMaxRows = 16;
 constexpr int kMaxDim = 256;
-constexpr int kMinChunk = 2;  // tiles per block that are worth another block
-// A unit's beginning and end (its rows of q, its result) take a block about as long as this many tiles.
+// Tiles per block that are worth another block.  One sequence of 777 tokens with 1, 2, 4, 8: 10.8, 10.8, 13.2, 16.6 us.
+constexpr int kMinChunk = 2;
+// A unit's beginning and end (its rows of q, its result) take a block about as long as this many tiles.  64 sequences
+// of 256 to 4096 tokens with 1, 2, 3, 4, 6: 86.7, 80.7, 76.8, 77.0, 77.4 us.
 constexpr int kUnitCost = 4;
 
 template <int HD, int ROWS>

@@ -6,6 +6,10 @@
 // order of the requests: a prefix sum over the requests meets a prefix sum over
 // the free pages); it is bound by the latency of its loads.  The second moves the
 // pages' bytes over all planes and updates tables and counts; it is bound by HBM.
+//
+// Measured.  4096 pages of 16 tokens, 8 layers (8 heads of 128, codes and scales), with holes, made dense: 94 us, 5.2
+// TB/s of a copy's 6.47; 16 requests forked 4 times each, part-filled last pages copied: 10.1 us, 3.1 TB/s, two launches
+// and the scan's loads; 64 requests freed in a pool of 32768: 3.6 us, one launch's latency.
 #include "common.cuh"
 
 namespace mak {
