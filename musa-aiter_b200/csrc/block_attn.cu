@@ -59,11 +59,11 @@ template <int HD, int ROWS>
 struct Cfg {
   static constexpr int kN = 4 * ROWS;              // columns of the products
   static constexpr int kParts = HD == 256 ? 2 : 1; // 128-row parts of head_dim
-  static constexpr int kStep = ROWS == 8 ? 2 : 1;  // tiles of one softmax step
+  static constexpr int kStep = ROWS <= 8 ? 2 : 1;  // tiles of one softmax step
   // Tiles of K and V in shared memory.  Scores are taken as soon as K is there; V waits for the
   // weights, a step of it held and a step on its way.
   static constexpr int kKs = HD == 64 ? 4 : 2;
-  static constexpr int kVs = HD == 64 ? 6 : ROWS == 8 ? 4 : 3;
+  static constexpr int kVs = HD == 64 ? 6 : ROWS <= 8 ? 4 : 3;
   static constexpr int kTileBytes = HD * kTile;
   static constexpr int kScores = 0, kOut = 2 * kStep * kN;  // TMEM columns: two steps' scores, one product
   static constexpr int kCols = kOut + kParts * kN;
@@ -77,8 +77,9 @@ struct Smem {
   alignas(1024) uint8_t v[C::kVs][C::kTileBytes];
   alignas(1024) uint8_t k[C::kKs][C::kTileBytes];
   alignas(1024) uint8_t p[C::kN * kTile * C::kStep];
-  // The products read four terms of q, of which there are three: what follows makes columns nobody reads.
-  uint8_t q[2][3 * ROWS * HD];  // of this unit and the next
+  // The products read four terms of q, of which there are three: what follows makes columns nobody reads.  Columns
+  // lie in groups of 8.
+  uint8_t q[2][(3 * ROWS + 7) / 8 * 8 * HD];  // of this unit and the next
   alignas(16) float ks[16][8], vs[16][8];  // scales per 16 tokens, tile number mod 16
   uint32_t have[16];                       // bit c: 16-token piece c has a block
   int page[16][8], head[16];               // for the copies of V, which follow those of K
@@ -1076,6 +1077,8 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
   // 12 rows 50 and 45, 24 rows 67 and 73, 32 rows 87 and 74.  Heads of 256 leave shared memory for groups of 8 alone.
   const bool wide = c.head_dim < 256 && rows > 8 && (rows <= 16 || rows > 24);
   if (c.head_dim == 64) return wide ? launch_rows_code<64, 16>(p, c.code_type, st) : launch_rows_code<64, 8>(p, c.code_type, st);
+  if (rows <= 4)
+    return c.head_dim == 128 ? launch_rows_code<128, 4>(p, c.code_type, st) : launch_rows_code<256, 4>(p, c.code_type, st);
   if (c.head_dim == 128) return wide ? launch_rows_code<128, 16>(p, c.code_type, st) : launch_rows_code<128, 8>(p, c.code_type, st);
   return launch_rows_code<256, 8>(p, c.code_type, st);
 }

@@ -118,6 +118,9 @@ __device__ __forceinline__ void mma_ts_f16(uint32_t d, uint32_t a, uint64_t b, u
 #define MAK_W8(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3]), "r"(a[i + 4]), "r"(a[i + 5]), "r"(a[i + 6]), "r"(a[i + 7])
 #define MAK_RW8(a, i) "+r"(a[i]), "+r"(a[i + 1]), "+r"(a[i + 2]), "+r"(a[i + 3]), "+r"(a[i + 4]), "+r"(a[i + 5]), "+r"(a[i + 6]), "+r"(a[i + 7])
 
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&v)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(at));
+}
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&v)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : MAK_R8(v, 0) : "r"(at));
 }
@@ -134,6 +137,9 @@ __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&v)[32]) {
       : "r"(at));
 }
 // Wait for this thread's loads from TMEM; the registers are named so that nothing uses them before.
+__device__ __forceinline__ void tmem_wait(uint32_t (&v)[4]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3])::"memory");
+}
 __device__ __forceinline__ void tmem_wait(uint32_t (&v)[8]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : MAK_RW8(v, 0)::"memory");
 }
