@@ -53,13 +53,13 @@ constexpr int kMaxDim = 256;
 constexpr int kMinChunk = 2;
 // A unit's beginning and end (its rows of q, its result) take a block about as long as this many tiles.  64 sequences
 // of 256 to 4096 tokens with 1, 2, 3, 4, 6: 86.7, 80.7, 76.8, 77.0, 77.4 us.
-constexpr int kUnitCost = 4;
+constexpr int kUnitCost = 3;
 
 template <int HD, int ROWS>
 struct Cfg {
   static constexpr int kN = 4 * ROWS;              // columns of the products
   static constexpr int kParts = HD == 256 ? 2 : 1; // 128-row parts of head_dim
-  static constexpr int kStep = ROWS <= 8 ? 2 : 1;  // tiles of one softmax step
+  static constexpr int kStep = ROWS == 8 ? 2 : 1;  // tiles of one softmax step
   // Tiles of K and V in shared memory.  Scores are taken as soon as K is there; V waits for the
   // weights, a step of it held and a step on its way.
   static constexpr int kKs = HD == 64 ? 4 : 2;
@@ -309,8 +309,8 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     uint32_t it = 0, tiles_done = 0;  // steps and tiles before this unit
     bool ok = true;
     // Rows of a unit: their places, and q as three 8-bit terms.  A row's threads are neighbours.
-    constexpr int kPer = HD * ROWS / kSoft;  // values of a thread
-    constexpr int kRowThreads = kSoft / ROWS;
+    constexpr int kPer = HD * ROWS / kSoft < 4 ? 4 : HD * ROWS / kSoft;  // values of a thread
+    constexpr int kRowThreads = HD / kPer;
     const int r = tid / kRowThreads, d0 = tid % kRowThreads * kPer;
     uint32_t w[kPer / 2];
     auto fetch = [&](const Unit& u) {
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       }
     };
     auto stage = [&](const Unit& u, int buf) {
-      if (d0 == 0) {
+      if (r < ROWS && d0 == 0) {
         const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) - i * p.group;
         int lo = 0, hi = 0;
         if (r < u.live) row_range(p, u.v, i, &lo, &hi);
@@ -383,10 +383,10 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
 #pragma unroll
           for (int z = 0; z < 3; ++z) {
             const int col = z * ROWS + r, d = d0 + e;
-            *reinterpret_cast<uint32_t*>(sm.q[buf] + (col >> 3) * (HD * 8) + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = t[z];
+            if (r < ROWS) *reinterpret_cast<uint32_t*>(sm.q[buf] + (col >> 3) * (HD * 8) + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = t[z];
           }
         }
-        if (d0 == 0) sm.row_scale[buf][r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
+        if (r < ROWS && d0 == 0) sm.row_scale[buf][r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
         fence_async_shared();
         tc_fence_before();
         __syncwarp();
@@ -1076,9 +1076,11 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
   // 8 rows 36 and 50 us, 12 rows 52.2 and 51.7, 16 rows 52.8 and 52.8, 24 rows 73 and 81, 32 rows 94 and 81; heads of 64:
   // 12 rows 50 and 45, 24 rows 67 and 73, 32 rows 87 and 74.  Heads of 256 leave shared memory for groups of 8 alone.
   const bool wide = c.head_dim < 256 && rows > 8 && (rows <= 16 || rows > 24);
-  if (c.head_dim == 64) return wide ? launch_rows_code<64, 16>(p, c.code_type, st) : launch_rows_code<64, 8>(p, c.code_type, st);
   if (rows <= 4)
-    return c.head_dim == 128 ? launch_rows_code<128, 4>(p, c.code_type, st) : launch_rows_code<256, 4>(p, c.code_type, st);
+    return c.head_dim == 64    ? launch_rows_code<64, 4>(p, c.code_type, st)
+           : c.head_dim == 128 ? launch_rows_code<128, 4>(p, c.code_type, st)
+                               : launch_rows_code<256, 4>(p, c.code_type, st);
+  if (c.head_dim == 64) return wide ? launch_rows_code<64, 16>(p, c.code_type, st) : launch_rows_code<64, 8>(p, c.code_type, st);
   if (c.head_dim == 128) return wide ? launch_rows_code<128, 16>(p, c.code_type, st) : launch_rows_code<128, 8>(p, c.code_type, st);
   return launch_rows_code<256, 8>(p, c.code_type, st);
 }
