@@ -32,11 +32,13 @@
 //
 // Measured (a copy runs at 6.47 TB/s).  4 sequences of 100000 to 131072 tokens, 8 cache heads of 128 with 8 query
 // heads each, E4M3, blocks of 64: 158 us, 5.8 TB/s, bound by HBM.  64 sequences of 256 to 4096, 4 query heads each,
-// blocks of 16: 77 us, 3.8 TB/s: a block gets two or three units, and between units the copies wait for some 10000
-// cycles (masks of the last step, the next rows of q, the sums), as what they run ahead by is a step of K and one of
-// V, all that shared memory holds.  Taking the next unit's rows and first scores before the last step ends: 82 us, as
-// the loop grows.  16 sequences of 300 to 4500, 16 heads of 64 on one cache head, 1 to 8 rows: 26 to 28 us, either
-// kernel.  One sequence of 777 tokens: 10.8 us, a chain of latencies (lengths, block ids, K, scores, weights, sums).
+// blocks of 16: 62 us, 4.7 TB/s: a block gets two or three units, and between units the copies wait for some 10000
+// cycles (masks of the last step, the next rows of q, the sums), as what they run ahead by is two tiles of K and four
+// of V, all that shared memory holds; instructions are fetched late too (1.5 of the 6 cycles between two of a warp's),
+// so less code is faster code.  Taking the next unit's rows and first scores before the last step ends: 65 us, as the
+// loop grows; three blocks per SM with fewer tiles each: 65 us.  16 sequences of 300 to 4500, 16 heads of 64 on one
+// cache head, 1 to 8 rows: 26 to 28 us, either kernel.  One sequence of 777 tokens: 10 us, a chain of latencies
+// (lengths, block ids, K, scores, weights, sums).
 #include "block_attn.cuh"
 #include "tcgen05.cuh"
 
@@ -52,14 +54,17 @@ constexpr int kMaxDim = 256;
 // Tiles per block that are worth another block.  One sequence of 777 tokens with 1, 2, 4, 8: 10.8, 10.8, 13.2, 16.6 us.
 constexpr int kMinChunk = 2;
 // A unit's beginning and end (its rows of q, its result) take a block about as long as this many tiles.  64 sequences
-// of 256 to 4096 tokens with 1, 2, 3, 4, 6: 86.7, 80.7, 76.8, 77.0, 77.4 us.
+// of 256 to 4096 tokens with 2, 3, 4: 62.2, 61.7, 62.8 us; in groups of 8 rows with 1, 2, 3, 4, 6: 86.7, 80.7, 76.8,
+// 77.0, 77.4 us.
 constexpr int kUnitCost = 3;
 
 template <int HD, int ROWS>
 struct Cfg {
   static constexpr int kN = 4 * ROWS;              // columns of the products
   static constexpr int kParts = HD == 256 ? 2 : 1; // 128-row parts of head_dim
-  static constexpr int kStep = ROWS == 8 ? 2 : 1;  // tiles of one softmax step
+  // Tiles of one softmax step: two spare groups of 8 rows half the barriers; for 4 rows the shorter code of one is
+  // faster (62.8 against 64.0 us for 64 sequences of 256 to 4096 tokens), for 16 two do not fit the registers.
+  static constexpr int kStep = ROWS == 8 ? 2 : 1;
   // Tiles of K and V in shared memory.  Scores are taken as soon as K is there; V waits for the
   // weights, a step of it held and a step on its way.
   static constexpr int kKs = HD == 64 ? 4 : 2;
@@ -1076,6 +1081,9 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
   // 8 rows 36 and 50 us, 12 rows 52.2 and 51.7, 16 rows 52.8 and 52.8, 24 rows 73 and 81, 32 rows 94 and 81; heads of 64:
   // 12 rows 50 and 45, 24 rows 67 and 73, 32 rows 87 and 74.  Heads of 256 leave shared memory for groups of 8 alone.
   const bool wide = c.head_dim < 256 && rows > 8 && (rows <= 16 || rows > 24);
+  // Groups of 4, groups of 8: one row, 4 query heads on each of 8 cache heads, 16 x 4096, 64 x 512, 1 x 777 tokens: heads
+  // of 64: 28.9 and 31.1, 23.9 and 29.9, 10.2 and 11.4 us; of 128: 33.3 and 36.1, 24.4 and 30.8, 10.9 and 11.6; of 256:
+  // 56 and 60, 39 and 49, 11.7 and 12.9.
   if (rows <= 4)
     return c.head_dim == 64    ? launch_rows_code<64, 4>(p, c.code_type, st)
            : c.head_dim == 128 ? launch_rows_code<128, 4>(p, c.code_type, st)
