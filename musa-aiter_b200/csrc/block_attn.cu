@@ -62,8 +62,9 @@ template <int HD, int ROWS>
 struct Cfg {
   static constexpr int kN = 4 * ROWS;              // columns of the products
   static constexpr int kParts = HD == 256 ? 2 : 1; // 128-row parts of head_dim
-  // Tiles of one softmax step: two spare groups of 8 rows half the barriers; for 4 rows the shorter code of one is
-  // faster (62.8 against 64.0 us for 64 sequences of 256 to 4096 tokens), for 16 two do not fit the registers.
+  // Tiles of one softmax step.  Two halve the barriers for each tile, which pays for 8 rows; for 4 rows the shorter
+  // code of one does (62.8 against 64.0 us for 64 sequences of 256 to 4096 tokens), for 16 two need more registers
+  // than there are.
   static constexpr int kStep = ROWS == 8 ? 2 : 1;
   // Tiles of K and V in shared memory.  Scores are taken as soon as K is there; V waits for the
   // weights, a step of it held and a step on its way.
