@@ -63,14 +63,15 @@ struct Plan {
   int32_t tile[kMaxItems];
 };
 
-// Tiles of row tile `tile` of a sequence (0: there is no such row tile) and the tokens they lie in.
+// Tiles of row tile `tile` of a sequence (0: there is no such row tile) and the tokens they lie in.  Numbers below the
+// first sequence's, whose rows need not begin at 0, come as negative ones.
 struct Span {
   int live, any_lo, any_hi, t0, tiles;
 };
 __device__ __forceinline__ Span span_of(const BlockAttnParams& p, const SeqView& v, int tile) {
   Span s;
   const int64_t left = static_cast<int64_t>(v.rows) * p.group - static_cast<int64_t>(tile) * kUnitRows;
-  s.live = left <= 0 ? 0 : left < kUnitRows ? static_cast<int>(left) : kUnitRows;
+  s.live = tile < 0 || left <= 0 ? 0 : left < kUnitRows ? static_cast<int>(left) : kUnitRows;
   s.any_lo = s.any_hi = s.t0 = s.tiles = 0;
   if (s.live == 0) return s;
   int unused;
@@ -86,7 +87,7 @@ __device__ __forceinline__ Span span_of(const BlockAttnParams& p, const SeqView&
 __device__ __forceinline__ int unit_len(const Span& s) { return s.live == 0 ? 0 : kUnitCost + (s.tiles > 0 ? s.tiles : 1); }
 
 // Row tiles of sequence s take the numbers floor(starts[s] * group / 256) + s and up, at least as many
-// as it has.
+// as it has; numbers before the first sequence's are nobody's.
 __device__ __forceinline__ int64_t first_item(const BlockAttnParams& p, int s) {
   const int64_t row = p.starts != nullptr ? max(__ldg(p.starts + s), 0) : s;
   return row * p.group / kUnitRows + s;

@@ -1,0 +1,92 @@
+"""Block-scaled caches at the edges of what a call may hold: rows that do not start at the packed tensors'
+first, lengths past the table, windows of any size, scales and codes that are no numbers or hardly any.
+
+Bounds as in test_gpu_block_cache: derived there, not fitted.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import musa_aiter as ma
+
+from .test_gpu_block_cache import DT, check_attention, make_cache, make_tables
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def define(q, kc, vc, ks, vs, table, ctx, starts, scale, window=0):
+    """Causal attention from its definition in 64 bits: a row's result takes the tokens it sees and no others.
+    Output, lse, and the sum of weights times magnitudes that check_attention's bound is made of."""
+    hq, hd = q.shape[1:]
+    nb, nh, _, bs = kc.shape
+    grp, room = hq // nh, table.shape[1] * bs
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    mag = torch.zeros(q.shape, dtype=torch.float64)
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
+    t = torch.arange(room)
+    for s in range(len(ctx)):
+        n = starts[s + 1] - starts[s]
+        page = table[s, t // bs].long()
+        there = (page >= 0) & (page < nb)
+        page = torch.where(there, page, 0)
+        k = kc[page, :, :, t % bs].float().double() * ks[page].double()[..., None]  # [tokens, NH, HD]
+        v = vc[page, :, :, t % bs].float().double() * vs[page].double()[..., None]
+        for i in range(n):
+            pos = ctx[s] - n + i
+            seen = there & (t <= pos) & (t > pos - window if window else t >= 0)
+            if not bool(seen.any()):
+                continue
+            row = starts[s] + i
+            x = torch.einsum("hgd,thd->hgt", q[row].double().view(nh, grp, hd), k[seen]) * scale
+            lse[row] = torch.logsumexp(x, -1).reshape(-1)
+            p = torch.softmax(x, -1)
+            out[row] = torch.einsum("hgt,thd->hgd", p, v[seen]).reshape(hq, hd)
+            mag[row] = torch.einsum("hgt,thd->hgd", p, v[seen].abs()).reshape(hq, hd)
+    return out, lse, mag
+
+
+class Case:
+    """Sequences of ctx[i] tokens whose last new[i] are rows of this call, on the CPU."""
+
+    def __init__(self, ctx, new, nh, grp, hd, bs, codes, dtype, seed=0, skip=0, after=0):
+        g = self.g = torch.Generator().manual_seed(seed)
+        self.ctx, self.codes, self.scale = list(ctx), codes, 1 / math.sqrt(hd)
+        self.table, nb, _ = make_tables(g, [max(c, 0) for c in ctx], bs)
+        self.kc, self.ks = make_cache(g, nb, nh, hd, bs, codes)
+        self.vc, self.vs = make_cache(g, nb, nh, hd, bs, codes)
+        self.starts = [skip]
+        for n in new:
+            self.starts.append(self.starts[-1] + n)
+        self.q = torch.randn((self.starts[-1] + after, nh * grp, hd), generator=g).to(DT[dtype])
+
+    def call(self, window=0, out=None):
+        args = (self.q, self.kc, self.vc, self.ks, self.vs, self.table)
+        return ma.paged_attention_block_scaled(*(x.cuda() for x in args), i32(self.ctx), i32(self.starts), window=window, scale=self.scale,
+                                               return_lse=True, out=out)
+
+    def want(self, window=0):
+        return define(self.q, self.kc, self.vc, self.ks, self.vs, self.table, self.ctx, self.starts, self.scale, window)
+
+
+# ---- rows that do not start at the packed tensors' first ---------------------------------------------
+
+
+@pytest.mark.parametrize("skip,after", [(1, 0), (130, 7), (1000, 300)])
+@pytest.mark.parametrize("new,nh,grp,hd", [((1, 1, 1), 2, 4, 64), ((3, 1, 6), 2, 1, 128), ((100, 40, 77), 2, 4, 128), ((90, 130, 300), 1, 1, 64)])
+def test_rows_of_a_slice_of_a_batch(new, nh, grp, hd, skip, after):
+    """cu_seqlens that start above 0 and end before the last row: rows of no sequence stay as they are."""
+    c = Case([40, 300, 310], new, nh, grp, hd, 16, "int8", "bf16", seed=skip, skip=skip, after=after)
+    out = torch.full_like(c.q, 7.0, device="cuda")
+    _, lse = c.call(out=out)
+    want, want_lse, mag = c.want()
+    mine = slice(c.starts[0], c.starts[-1])
+    check_attention(out[mine], lse[mine], c.q, want[mine], want_lse[mine], mag[mine])
+    assert bool((out[: mine.start] == 7).all()) and bool((out[mine.stop:] == 7).all())
