@@ -146,7 +146,8 @@ __device__ __forceinline__ Target find_target(const AppendParams& p, int64_t ite
   t.page = -1;
   const int bs = 1 << p.bs_log2;
   // Slots floor(starts[s] / bs) + 2 s ... belong to sequence s: at least as many as it
-  // can touch blocks, whatever its position.
+  // can touch blocks, whatever its position.  Slots before the first sequence's, whose rows
+  // need not begin at 0, are nobody's.
   int s, row0, rows, nth;
   if (p.starts == nullptr) {
     s = static_cast<int>(item), row0 = s, rows = 1, nth = 0;
@@ -167,6 +168,7 @@ __device__ __forceinline__ Target find_target(const AppendParams& p, int64_t ite
     row0 = max(__ldg(p.starts + s), 0);
     rows = min(__ldg(p.starts + s + 1), p.num_rows) - row0;
     nth = static_cast<int>(item - (row0 >> p.bs_log2) - 2 * static_cast<int64_t>(s));
+    if (nth < 0) return t;
   }
   const int64_t ctx = __ldg(p.ctx_lens + s);
   const int64_t first = ctx - rows;  // position of the call's first row

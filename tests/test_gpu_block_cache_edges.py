@@ -13,7 +13,7 @@ import torch
 
 import musa_aiter as ma
 
-from .test_gpu_block_cache import DT, check_attention, make_cache, make_tables
+from .test_gpu_block_cache import DT, append_reference, check_attention, make_cache, make_tables
 
 pytestmark = pytest.mark.gpu
 
@@ -90,3 +90,15 @@ def test_rows_of_a_slice_of_a_batch(new, nh, grp, hd, skip, after):
     mine = slice(c.starts[0], c.starts[-1])
     check_attention(out[mine], lse[mine], c.q, want[mine], want_lse[mine], mag[mine])
     assert bool((out[: mine.start] == 7).all()) and bool((out[mine.stop:] == 7).all())
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("skip,new", [(1, (1, 1, 2)), (40, (5, 1, 33)), (500, (64, 17, 3)), (333, (0, 20, 0))])
+def test_writer_of_a_slice_of_a_batch(codes, skip, new):
+    c = Case([70, 21, 40], new, 2, 1, 64, 16, codes, "bf16", seed=skip, skip=skip, after=9)
+    c.vs[c.table[0, 1]] = 0  # a scale of zero of a block that the call does not write, or begins
+    dev = [x.cuda() for x in (c.kc, c.vc, c.ks, c.vs)]
+    ma.kv_append_block_scaled(c.q.cuda(), c.q.cuda(), *dev, c.table.cuda(), i32(c.ctx), i32(c.starts))
+    for cache, scale, x, y in ((c.kc, c.ks, dev[0], dev[2]), (c.vc, c.vs, dev[1], dev[3])):
+        append_reference(c.q, cache, scale, c.table, c.ctx, c.starts, codes)
+        assert torch.equal(y.cpu(), scale) and torch.equal(x.cpu().float(), cache.float())
