@@ -655,7 +655,9 @@ MAK_API int64_t mak_block_attention_workspace_bytes(void);
  * position context_lens[s] - (rows of s) + that index; it sees tokens up to its
  * own position (causal) or all of them, and with window > 0 (causal only) the
  * last `window` of those.  A row that sees nothing gives zeros and lse = -inf.
- * Block ids outside [0, num_blocks) are skipped like tokens outside the sequence.
+ * Block ids outside [0, num_blocks) are skipped like tokens outside the sequence,
+ * and so are tokens past max_blocks * block_size; a length beyond that shifts no
+ * position.
  */
 MAK_API int mak_block_attention(const mak_block_attn_desc* desc, void* stream);
 

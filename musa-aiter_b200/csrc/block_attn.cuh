@@ -34,16 +34,16 @@ struct BlockAttnParams {
 };
 
 // What a sequence's rows see.  first: the row index of its first row; rows: how
-// many it has; lo..hi: tokens that at least one of them sees.
+// many it has; ctx: its length, which positions are counted from even where the
+// table holds less; lo..hi: tokens that at least one of them sees, hi within the table.
 struct SeqView {
   int first, rows, ctx, lo, hi;
 };
 
 __device__ __forceinline__ SeqView seq_view(const BlockAttnParams& p, int s) {
   SeqView v;
-  int ctx = __ldg(p.ctx_lens + s);
-  const int64_t room = static_cast<int64_t>(p.max_blocks) << p.bs_log2;
-  ctx = ctx < 0 ? 0 : (ctx > room ? static_cast<int>(room) : ctx);
+  const int ctx = max(__ldg(p.ctx_lens + s), 0);
+  const int room = p.max_blocks << p.bs_log2;
   int a = s, b = s + 1;
   if (p.starts != nullptr) {
     a = __ldg(p.starts + s);
@@ -54,7 +54,7 @@ __device__ __forceinline__ SeqView seq_view(const BlockAttnParams& p, int s) {
   v.first = a;
   v.rows = b > a ? b - a : 0;
   v.ctx = ctx;
-  v.hi = ctx;
+  v.hi = min(ctx, room);
   v.lo = 0;
   if (p.window > 0 && ctx - v.rows - p.window + 1 > 0) v.lo = ctx - v.rows - p.window + 1;
   return v;
@@ -63,7 +63,7 @@ __device__ __forceinline__ SeqView seq_view(const BlockAttnParams& p, int s) {
 // Tokens [lo, hi) that row i of the sequence sees.
 __device__ __forceinline__ void row_range(const BlockAttnParams& p, const SeqView& v, int i, int* lo, int* hi) {
   const int pos = v.ctx - v.rows + i;
-  *hi = p.causal ? (pos + 1 < 0 ? 0 : pos + 1) : v.ctx;
+  *hi = p.causal ? max(min(pos + 1, v.hi), 0) : v.hi;
   *lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
 }
 

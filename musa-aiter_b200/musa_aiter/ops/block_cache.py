@@ -9,8 +9,9 @@ from the data, block by block.
 Both calls take a sequence's pages from ``block_tables`` (int32 ``[num_seqs, max_blocks]``) and its
 length from ``context_lens`` (int32, the tokens of this call included); ``cu_seqlens`` (int32
 ``[num_seqs + 1]``) says which rows of the packed tensors are whose, None means one row per sequence.
-Nothing is read back: block ids outside the cache are skipped by the kernels, as are tokens past
-``max_blocks * block_size``.
+Rows that belong to no sequence are neither read nor written.  Nothing is read back: block ids outside
+the cache are skipped by the kernels, as are tokens past ``max_blocks * block_size`` (rows keep the
+positions that ``context_lens`` gives them).
 """
 
 from __future__ import annotations

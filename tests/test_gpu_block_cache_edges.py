@@ -75,6 +75,11 @@ class Case:
     def want(self, window=0):
         return define(self.q, self.kc, self.vc, self.ks, self.vs, self.table, self.ctx, self.starts, self.scale, window)
 
+    def check(self, window=0):
+        got, lse = self.call(window)
+        out, want_lse, mag = self.want(window)
+        check_attention(got, lse, self.q, out, want_lse, mag)
+
 
 # ---- rows that do not start at the packed tensors' first ---------------------------------------------
 
@@ -102,3 +107,35 @@ def test_writer_of_a_slice_of_a_batch(codes, skip, new):
     for cache, scale, x, y in ((c.kc, c.ks, dev[0], dev[2]), (c.vc, c.vs, dev[1], dev[3])):
         append_reference(c.q, cache, scale, c.table, c.ctx, c.starts, codes)
         assert torch.equal(y.cpu(), scale) and torch.equal(x.cpu().float(), cache.float())
+
+
+# ---- positions ------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("window", [0, 9, 200])
+@pytest.mark.parametrize("over,new", [(5, (8, 3)), (1, (1, 2)), (40, (16, 50)), (5, (120, 90)), (70, (120, 60))])
+def test_lengths_past_the_table_shift_no_position(over, new, window):
+    """A length past what the table holds: rows keep the positions that the writer gave them."""
+    c = Case([160, 96], new, 2, 4, 64, 16, "int8", "f16", seed=over)
+    c.ctx = [160 + over, 160 + over]
+    c.check(window)
+
+
+def test_writer_and_attention_agree_past_the_table():
+    g = torch.Generator().manual_seed(1)
+    nh, hd, bs, new, ctx = 2, 64, 16, 12, 53  # 48 tokens have a place
+    table = torch.tensor([[2, 0, 3]], dtype=torch.int32)
+    k, v = (torch.randn((new, nh, hd), generator=g).half() for _ in range(2))
+    kc, ks = make_cache(g, 4, nh, hd, bs, "int8")
+    vc, vs = make_cache(g, 4, nh, hd, bs, "int8")
+    dev = [x.cuda() for x in (kc, vc, ks, vs)]
+    ma.kv_append_block_scaled(k.cuda(), v.cuda(), *dev, table.cuda(), i32([ctx]), i32([0, new]))
+    kc, vc, ks, vs = (x.cpu() for x in dev)
+    q = torch.randn((new, 4, hd), generator=g).half()
+    # row i sits where the writer put token i: position ctx - new + i
+    got, lse = ma.paged_attention_block_scaled(q.cuda(), *dev, table.cuda(), i32([ctx]), i32([0, new]), window=1, return_lse=True)
+    want, want_lse, mag = define(q, kc, vc, ks, vs, table, [ctx], [0, new], 1 / math.sqrt(hd), 1)
+    check_attention(got, lse, q, want, want_lse, mag)
+    assert torch.isfinite(want_lse).sum() == 7 * 4  # the tokens at 41 to 47
+    own = v.double().repeat_interleave(2, 1)[:7]  # a window of one token gives that token's value back
+    assert float((got[:7].double().cpu() - own).abs().max()) <= 2 * float(v.abs().max()) / 127
