@@ -55,8 +55,8 @@ __device__ __forceinline__ SeqView seq_view(const BlockAttnParams& p, int s) {
   v.rows = b > a ? b - a : 0;
   v.ctx = ctx;
   v.hi = min(ctx, room);
-  v.lo = 0;
-  if (p.window > 0 && ctx - v.rows - p.window + 1 > 0) v.lo = ctx - v.rows - p.window + 1;
+  const int before = ctx - v.rows;  // the first row's position
+  v.lo = p.window > 0 && before >= p.window ? before - p.window + 1 : 0;
   return v;
 }
 
@@ -64,7 +64,7 @@ __device__ __forceinline__ SeqView seq_view(const BlockAttnParams& p, int s) {
 __device__ __forceinline__ void row_range(const BlockAttnParams& p, const SeqView& v, int i, int* lo, int* hi) {
   const int pos = v.ctx - v.rows + i;
   *hi = p.causal ? max(min(pos + 1, v.hi), 0) : v.hi;
-  *lo = p.window > 0 && pos - p.window + 1 > 0 ? pos - p.window + 1 : 0;
+  *lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;  // compared first: the difference alone may leave 32 bits
 }
 
 // Two 8-bit codes (low / high half of w as b0, b1 pairs) to two f16: every int8

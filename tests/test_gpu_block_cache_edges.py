@@ -139,3 +139,13 @@ def test_writer_and_attention_agree_past_the_table():
     assert torch.isfinite(want_lse).sum() == 7 * 4  # the tokens at 41 to 47
     own = v.double().repeat_interleave(2, 1)[:7]  # a window of one token gives that token's value back
     assert float((got[:7].double().cpu() - own).abs().max()) <= 2 * float(v.abs().max()) / 127
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 2, 2**31, 2**40, 2**31 - 200])
+@pytest.mark.parametrize("ctx,new", [((400, 3), (5, 6)), ((300, 290, 1), (310, 300, 40)), ((500, 129), (500, 135))])
+def test_windows_of_any_size(ctx, new, window):
+    """More rows than tokens and a window near the largest 32-bit number: as without a window."""
+    c = Case(ctx, new, 2, 2, 64, 16, "int8", "bf16", seed=3)
+    got, lse = c.call(window)
+    out, want_lse, mag = c.want(0)
+    check_attention(got, lse, c.q, out, want_lse, mag)
