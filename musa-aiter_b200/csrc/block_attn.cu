@@ -494,6 +494,33 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         }
         return true;
       };
+      // V scales that are infinite or NaN: the rows that see such a block get NaN, for the others it weighs nothing.
+      // An integer cannot say so, and in E4M3 a weight of 0 times NaN would say it to every row.
+      auto odd_scales = [&](uint32_t tile, int tok0, int count, float (&vs)[C::kStep], float& vtop) {
+        uint32_t seen = 0;  // bit z: row z sees one
+        vtop = 0.f;
+        for (int y = 0; y < count; ++y) {
+          const uint32_t k = (tile + y) & 15;
+          for (int c = 0; c < 8; ++c) {
+            const float v = fabsf(sm.vs[k][c]);
+            const int t0 = tok0 + y * kTile + 16 * c;
+            if (v < INFINITY) {
+              vtop = fmaxf(vtop, v);
+            } else {
+              for (int z = 0; z < ROWS; ++z)
+                if (max(sm.row_lo[buf][z], t0) < min(sm.row_hi[buf][z], t0 + 16)) seen |= 1u << z;
+            }
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < C::kStep; ++y)
+          if (!(fabsf(vs[y]) < INFINITY)) vs[y] = 0.f;
+#pragma unroll
+        for (int z = 0; z < ROWS; ++z)
+#pragma unroll
+          for (int h = 0; h < C::kParts; ++h)
+            if (seen >> z & 1) acc[h][z] = __uint_as_float(0x7fffffffu);
+      };
       // A warp that gave up goes through the same barriers as the others, without waiting for anything else.
       for (int t = 0; t < steps; ++t) {
         const uint32_t x = it + t, tile = tiles_done + t * C::kStep;
@@ -533,9 +560,10 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
           }
           if (y < count) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) vtop = fmaxf(vtop, fabsf(sm.vs[k][c]));
+            for (int c = 0; c < 8; ++c) vtop = max_or_nan(vtop, fabsf(sm.vs[k][c]));
           }
         }
+        if (!(vtop < INFINITY)) odd_scales(tile, tok0, count, vs, vtop);
 #pragma unroll
         for (int z = 0; z < ROWS; ++z) top[z] = warp_max(C::kStep == 2 ? fmaxf(s[0][z], s[C::kStep - 1][z]) : s[0][z]);
         if (lane == 0) {

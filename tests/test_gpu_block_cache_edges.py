@@ -80,6 +80,16 @@ class Case:
         out, want_lse, mag = self.want(window)
         check_attention(got, lse, self.q, out, want_lse, mag)
 
+    def check_odd(self, window=0):
+        """Where the definition gives no finite number neither may the call; everywhere else the bounds hold."""
+        got, lse = (x.cpu() for x in self.call(window))
+        out, want_lse, mag = self.want(window)
+        odd = ~torch.isfinite(out)
+        assert odd.any() and not odd.all()
+        assert torch.equal(~torch.isfinite(got), odd)
+        zero = torch.zeros((), dtype=torch.float64)
+        check_attention(torch.where(odd, zero.to(got.dtype), got), lse, self.q, torch.where(odd, zero, out), want_lse, torch.where(odd, zero, mag))
+
 
 # ---- rows that do not start at the packed tensors' first ---------------------------------------------
 
@@ -149,3 +159,19 @@ def test_windows_of_any_size(ctx, new, window):
     got, lse = c.call(window)
     out, want_lse, mag = c.want(0)
     check_attention(got, lse, c.q, out, want_lse, mag)
+
+
+# ---- scales and codes that are no numbers, or hardly any ------------------------------------------------
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("window", [0, 20])
+@pytest.mark.parametrize("new", [(1, 1), (6, 3)])
+@pytest.mark.parametrize("codes,grp", [("int8", 4), ("fp8", 2), ("fp8", 1)])
+def test_value_scales_that_are_no_numbers(codes, grp, new, window, value):
+    """Rows that see such a block give no finite number, the others are as if it were not there."""
+    c = Case([195, 135], new, 2, grp, 64, 16, codes, "f16", seed=5)
+    c.vs[c.table[0, (200 - new[0] // 2) // 16], 1] = value  # later rows see it, head 1 alone
+    if new[0] == 1:
+        c.vs[c.table[0, 11], 1] = value
+    c.check_odd(window)
