@@ -471,7 +471,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 p0 = e >= from && e < to ? p0 : 0.f;
                 p1 = e + 1 >= from && e + 1 < to ? p1 : 0.f;
                 l += p0 + p1;
-                y[e >> 1] = pack_f16(p0 * w, p1 * w);
+                // 0 where the row does not see the token, whatever its scale
+                p0 = e >= from && e < to ? p0 * w : 0.f;
+                p1 = e + 1 >= from && e + 1 < to ? p1 * w : 0.f;
+                y[e >> 1] = pack_f16(p0, p1);
               }
               tmem_st(s_at + c * 8, y);
             }
@@ -680,8 +683,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (dlo == 0 && w < 2) {
             sm.kfac[g & 3][chunk16] = ks;
             sm.vfac[g & 3][chunk16] = vs;
-            // a scale of 0 counts as 2^-100 in the maximum: its weights go into the sum alone
-            sm.vlog[g & 3][chunk16] = vs != 0.f ? log2f(fabsf(vs)) : -100.f;
+            // a scale of 0, or one that is no number, counts as 2^-100 in the maximum: its weights are right in the sum alone
+            sm.vlog[g & 3][chunk16] = vs != 0.f && fabsf(vs) < INFINITY ? log2f(fabsf(vs)) : -100.f;
             sm.vinv[g & 3][chunk16] = fine ? 1.f / vs : 0.f;
           }
           const uint32_t v1 = __ballot_sync(0xffffffffu, page >= 0), v2 = __ballot_sync(0xffffffffu, fine);

@@ -166,7 +166,7 @@ def test_windows_of_any_size(ctx, new, window):
 
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("window", [0, 20])
-@pytest.mark.parametrize("new", [(1, 1), (6, 3)])
+@pytest.mark.parametrize("new", [(1, 1), (6, 3), (100, 70)])
 @pytest.mark.parametrize("codes,grp", [("int8", 4), ("fp8", 2), ("fp8", 1)])
 def test_value_scales_that_are_no_numbers(codes, grp, new, window, value):
     """Rows that see such a block give no finite number, the others are as if it were not there."""
