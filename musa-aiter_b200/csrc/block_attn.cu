@@ -216,13 +216,14 @@ __device__ __forceinline__ uint32_t split_int8(float x) {
   return (static_cast<uint32_t>(__float2int_rn(x)) + 0x808080u) ^ 0x808080u;
 }
 
-// The terms' products to their sum: in units of the last digit (int8) or of the first term (E4M3).
+// The terms' products to their sum in units of the first: a digit is worth 1 / 256 of the one before it, an E4M3 term
+// 1 / 16.
 template <int CODE, int TERMS>
 __device__ __forceinline__ float join_terms(const uint32_t (&t)[TERMS]) {
   float x = 0.f;
   if constexpr (CODE == MAK_CODE_INT8) {
 #pragma unroll
-    for (int i = 0; i < TERMS; ++i) x = fmaf(x, 256.f, static_cast<float>(static_cast<int>(t[i])));
+    for (int i = 0; i < TERMS; ++i) x = fmaf(static_cast<float>(static_cast<int>(t[i])), 1.f / (1u << (8 * i)), x);
   } else {
 #pragma unroll
     for (int i = TERMS - 1; i >= 0; --i) x = fmaf(x, 1.f / 16.f, __uint_as_float(t[i]));
@@ -392,7 +393,8 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             if (r < ROWS) *reinterpret_cast<uint32_t*>(sm.q[buf] + (col >> 3) * (HD * 8) + (d >> 4) * 128 + (col & 7) * 16 + (d & 15)) = t[z];
           }
         }
-        if (r < ROWS && d0 == 0) sm.row_scale[buf][r] = top < INFINITY ? ldexpf(p.scale_log2, -up) : __uint_as_float(0x7fffffffu);
+        constexpr int kFirst = CODE == MAK_CODE_INT8 ? 16 : 0;  // 2^kFirst: a unit of the first term
+        if (r < ROWS && d0 == 0) sm.row_scale[buf][r] = top < INFINITY ? ldexpf(p.scale_log2, kFirst - up) : __uint_as_float(0x7fffffffu);
         fence_async_shared();
         tc_fence_before();
         __syncwarp();
@@ -582,8 +584,13 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             top[z + 2] = fmaxf(top[z + 2], o.z);
             top[z + 3] = fmaxf(top[z + 3], o.w);
           }
-        constexpr float kFull = CODE == MAK_CODE_INT8 ? 127.f * 16777216.f : 256.f;
-        const float weight = vtop > 0.f ? kFull / vtop : 0.f;
+        // The largest weight, in units of its last digit (int8) and of its first term.  Scales may be as small as there
+        // are numbers: the quotient is taken after both were lifted by 2^60.
+        constexpr float kFull = CODE == MAK_CODE_INT8 ? 127.f * 16777216.f : 256.f, kLead = CODE == MAK_CODE_INT8 ? 127.f : 256.f;
+        const float lift = vtop < 0x1p-60f ? 0x1p60f : 1.f;
+        const float weight = vtop > 0.f ? kFull / (vtop * lift) : 0.f;
+#pragma unroll
+        for (int y = 0; y < C::kStep; ++y) vs[y] *= lift;
         float fade[ROWS], next_gain[ROWS];
         uint32_t words[C::kStep][4][ROWS / 4];  // weights of this thread's tokens: term, four rows
 #pragma unroll
@@ -600,11 +607,11 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             for (int y = 0; y < C::kStep; ++y) {
               w[y][e] = exp2_fast(s[y][z] - mz);
               sum += w[y][e];
-              w[y][e] *= vs[y] * weight;
+              w[y][e] *= vs[y] * weight;  // both factors first: theirs is at most kFull
             }
             l[z] = l[z] * old + sum * add;
             fade[z] = old;
-            next_gain[z] = add * vtop * (1.f / kFull);
+            next_gain[z] = add * vtop * (1.f / kLead);
             m[z] = mn;
           }
 #pragma unroll

@@ -175,3 +175,34 @@ def test_value_scales_that_are_no_numbers(codes, grp, new, window, value):
     if new[0] == 1:
         c.vs[c.table[0, 11], 1] = value
     c.check_odd(window)
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("new", [(1, 1), (5, 4), (40, 90)])
+@pytest.mark.parametrize("power", [-50, -90, -109])
+def test_value_scales_near_the_smallest(power, new, codes):
+    """Magnitudes down to 2^-100 are stored as what they are: scales down to 2^-109.  Rows of bfloat16 hold such results."""
+    c = Case([400, 333], new, 2, 4, 128, 16, codes, "bf16", seed=7)
+    c.vs = torch.exp2(torch.rand(c.vs.shape, generator=c.g) * 2 + power)
+    got, lse = c.call()
+    out, want_lse, mag = c.want()
+    big = 2.0 ** -power
+    check_attention(got.double() * big, lse, c.q, out * big, want_lse, mag * big)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+def test_long_sequences_of_the_smallest_scales(codes, new):
+    """Scores all alike: the sum of the weights is as many as there are tokens."""
+    c = Case([40000], [new], 1, 1, 64, 128, codes, "bf16", seed=8)
+    c.q.zero_()
+    c.vs = torch.full_like(c.vs, 2.0 ** -109)
+    got, lse = c.call()
+    v = (c.vc[c.table[0].long()].float().double() * 2.0 ** -109).permute(0, 3, 1, 2).reshape(-1, 64)[:40000]
+    for i in range(new):
+        seen = v[: 40000 - new + i + 1]
+        assert abs(float(lse[i]) - math.log(len(seen))) <= 3e-5
+        off = (got[i, 0].double().cpu() - seen.mean(0)).abs() * 2.0 ** 109
+        # as in check_attention, and sums of so many terms of either sign in 32 bits
+        bound = (2.0 ** -11 + 2.0 ** -14) * seen.abs().mean(0) * 2.0 ** 109 + 2.0 ** -8 * 1.01 * seen.mean(0).abs() * 2.0 ** 109
+        assert bool((off <= bound).all())
