@@ -47,6 +47,10 @@ constexpr int kUnitRows = 256;  // rows of a unit
 constexpr int kThreads = 640;
 constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolerated
 constexpr float kLift = 6.f;    // log2 factor that weights carry
+// The sum of the weights carries 2^(kLift - kSpare): divided by the smallest scales, 2^-109 as the writer makes them, its
+// terms come to 2^114 and more.  Smaller scales count as kLeast in the maximum.
+constexpr int kSpare = 12;
+constexpr float kLeast = -110.f;  // log2
 constexpr float kSumLimit = 32768.f;  // of 16 weights, below which none of them is near f16's largest
 // A unit's beginning and end, in tiles.  The prompts below with 2, 3, 4, 5: 448, 444, 439, 440 us.
 constexpr int kUnitCost = 4;
@@ -167,8 +171,8 @@ struct TcSmem {
   alignas(1024) uint8_t k[2][HD * 256];  // 128 tokens: 2 pieces of [HD][64]
   alignas(1024) uint8_t v[2][HD * 256];
   alignas(16) float kfac[4][8], vfac[4][8];  // per 16 tokens of a tile: the scales,
-  alignas(16) float vlog[4][8], vinv[4][8];  // log2 and reciprocal of V's
-  uint32_t have[4], plain[4];                // bit c: piece c has a block; its scales are positive and finite.  0-3 in byte 0, 4-7 in byte 1
+  alignas(16) float vlog[4][8], vinv[4][8];  // log2 of V's and 2^-kSpare over V's
+  uint32_t have[4], plain[4];                // bit c: piece c has a block; its scales are positive, finite and not below 2^kLeast.  0-3 in byte 0, 4-7 in byte 1
   alignas(8) uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], spare;
   // Walks and units of the softmax warps, the eight loading warps and the issuing thread: here, since their
   // registers are needed for scores and codes.
@@ -470,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float p1 = exp2_fast(fmaf(__uint_as_float(x[e + 1]), f, -ms));
                 p0 = e >= from && e < to ? p0 : 0.f;
                 p1 = e + 1 >= from && e + 1 < to ? p1 : 0.f;
-                l += p0 + p1;
+                l = fmaf(p0 + p1, 1.f / (1 << kSpare), l);
                 // 0 where the row does not see the token, whatever its scale
                 p0 = e >= from && e < to ? p0 * w : 0.f;
                 p1 = e + 1 >= from && e + 1 < to ? p1 * w : 0.f;
@@ -490,7 +494,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++ends;
       }
       before += u.n;
-      l *= 1.f / (1 << static_cast<int>(kLift));  // both l and the accumulators carry 2^kLift
       if (!ok) l = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN, not stale memory
 
       // ---- this block's share of the unit -------------------------------------------
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       };
       auto put_lse = [&](float* lse, float mx, float sum) {
-        if (lse != nullptr) *lse = sum > 0.f || sum != sum ? (mx + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+        if (lse != nullptr) *lse = sum > 0.f || sum != sum ? (mx + (log2f(sum) + (kSpare - kLift))) * 0.69314718055994531f : -INFINITY;
       };
       const bool split = u.ta > 0 || u.tb < u.len;
       constexpr int kFloats = kUnitRows * (HD + 2);  // of one partial sum: [HD][256], maxima, sums
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint16_t* dst = nullptr;
         float* lse = nullptr;
         if (on) place(row, dst, lse);
-        const float inv = l > 0.f || l != l ? 1.f / l * (1.f / (1 << static_cast<int>(kLift))) : 0.f;
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll 1
         for (int d = 0; d < HD; d += 16) {
           uint32_t x[16];
@@ -541,10 +544,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait(x);
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = u.n > 0 ? __uint_as_float(x[e]) : 0.f;
+          for (int e = 0; e < 16; ++e)  // from 2^kLift to what l carries
+            o[e] = u.n > 0 ? __uint_as_float(x[e]) * (1.f / (1 << kSpare)) : 0.f;
           if (split) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) part[(d + e) * kUnitRows + tid] = o[e] * (1.f / (1 << static_cast<int>(kLift)));
+            for (int e = 0; e < 16; ++e) part[(d + e) * kUnitRows + tid] = o[e];
           } else if (on) {
             put(dst + d, o, inv);
           }
@@ -679,13 +683,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         if (!is_v) {
           // the factors of tile g - 4 were last read before tile g - 2's scores were issued
-          const bool fine = ks > 0.f && ks < INFINITY && vs > 0.f && vs < INFINITY;
+          const bool fine = ks > 0.f && ks < INFINITY && vs >= 0x1p-110f && vs < INFINITY;
           if (dlo == 0 && w < 2) {
             sm.kfac[g & 3][chunk16] = ks;
             sm.vfac[g & 3][chunk16] = vs;
             // a scale of 0, or one that is no number, counts as 2^-100 in the maximum: its weights are right in the sum alone
-            sm.vlog[g & 3][chunk16] = vs != 0.f && fabsf(vs) < INFINITY ? log2f(fabsf(vs)) : -100.f;
-            sm.vinv[g & 3][chunk16] = fine ? 1.f / vs : 0.f;
+            sm.vlog[g & 3][chunk16] = vs != 0.f && fabsf(vs) < INFINITY ? fmaxf(log2f(fabsf(vs)), kLeast) : -100.f;
+            sm.vinv[g & 3][chunk16] = fine ? 1.f / (1 << kSpare) / vs : 0.f;
           }
           const uint32_t v1 = __ballot_sync(0xffffffffu, page >= 0), v2 = __ballot_sync(0xffffffffu, fine);
           if (lane == 0 && w < 2) {

@@ -206,3 +206,25 @@ def test_long_sequences_of_the_smallest_scales(codes, new):
         # as in check_attention, and sums of so many terms of either sign in 32 bits
         bound = (2.0 ** -11 + 2.0 ** -14) * seen.abs().mean(0) * 2.0 ** 109 + 2.0 ** -8 * 1.01 * seen.mean(0).abs() * 2.0 ** 109
         assert bool((off <= bound).all())
+
+
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+def test_weights_of_the_smallest_scales_add_up(codes):
+    """Many rows: the first scores of each tile are low and the others are not enough above them to move the maximum."""
+    nh, hd, bs, ctx, new = 16, 64, 16, 16384, 40
+    g = torch.Generator().manual_seed(11)
+    table = torch.randperm(ctx // bs, generator=g).to(torch.int32)[None]
+    kc = torch.full((ctx // bs, nh, hd, bs), 8.0).to(torch.int8 if codes == "int8" else torch.float8_e4m3fn)
+    vc, _ = make_cache(g, ctx // bs, nh, hd, bs, codes)
+    ks, vs = torch.full((ctx // bs, nh), 4.9 * math.log(2) / 8), torch.full((ctx // bs, nh), 2.0 ** -109)
+    low = torch.arange(ctx // bs) % 8 < 2  # the first 32 of 128 tokens
+    ks[table[0, low].long()] = 1e-6
+    q = torch.ones((new, nh, hd), dtype=torch.bfloat16)
+    got, lse = ma.paged_attention_block_scaled(*(x.cuda() for x in (q, kc, vc, ks, vs, table)), i32([ctx]), i32([0, new]), scale=1 / hd,
+                                               return_lse=True)
+    weight = torch.exp(ks[table[0].long(), 0].double() * 8).repeat_interleave(bs)
+    v = vc[table[0].long()].float().double().permute(0, 3, 1, 2).reshape(ctx, nh, hd)
+    total = weight.cumsum(0)[-new:]
+    want = (weight[:, None, None] * v).cumsum(0)[-new:] / total[:, None, None]
+    mag = (weight[:, None, None] * v.abs()).cumsum(0)[-new:] / total[:, None, None]
+    check_attention(got.double() * 2.0 ** 109, lse, q, want, total.log()[:, None].expand(new, nh), mag)
