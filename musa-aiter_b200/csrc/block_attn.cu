@@ -651,28 +651,33 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             *reinterpret_cast<uint4*>(sm.p + (c * C::kStep * kTile + y * kTile + tid) * 16) =
                 make_uint4(x4[4 * c], x4[4 * c + 1], x4[4 * c + 2], x4[4 * c + 3]);
         }
-        // E4M3: codes that no row sees may be NaN, which a weight of zero does not cancel
+        // E4M3: codes may be NaN, which a weight of zero does not cancel.  What no row sees becomes 0, and so does a NaN
+        // in a piece that not every row sees whole: its dimension, this thread's, becomes NaN for the rows that see it.
         if (CODE == MAK_CODE_E4M3) {
           for (int y = 0; y < count; ++y) {
             const int tk = tok0 + y * kTile;
             const uint32_t have = sm.have[(tile + y) & 15];
-            if (tk >= u.any_lo && tk + kTile <= u.any_hi && have == 0xffu) continue;
+            if (tk >= u.all_lo && tk + kTile <= u.all_hi && have == 0xffu) continue;
             const uint32_t slot = (tile + y) % kVs;
             ok = ok && mbar_wait_warp(&sm.v_full[slot], ((tile + y) / kVs) & 1, gave_up);
-            // pieces that are not seen whole
+            // pieces that are not seen whole by every row
             uint32_t part = ~have & 0xffu;
-            if (tk < u.any_lo) part |= (2u << ((u.any_lo - tk) >> 4)) - 1;
-            if (tk + kTile > u.any_hi) part |= 0xffu << ((u.any_hi - tk) >> 4);
-            for (int d = tid; d < HD; d += kSoft)
+            if (tk < u.all_lo) part |= (2u << min((u.all_lo - tk) >> 4, 7)) - 1;
+            if (tk + kTile > u.all_hi) part |= 0xffu << (max(u.all_hi - tk, 0) >> 4);
+            const int per_line = bs >> 4;  // 16-byte pieces of a line
+#pragma unroll
+            for (int h = 0; h < C::kParts; ++h) {
+              const int d = h * 128 + tid;
+              if (HD < 128 && d >= HD) break;
+              const int swz = p.bs_log2 == 7 ? d & 7 : p.bs_log2 == 6 ? (d >> 1) & 3 : p.bs_log2 == 5 ? (d >> 2) & 1 : 0;
               for (uint32_t left = part & 0xffu; left != 0; left &= left - 1) {
                 const int c = __ffs(left) - 1;
                 const int ct = tk + 16 * c;
                 const bool there = (have >> c) & 1;
-                const int per_line = bs >> 4;  // 16-byte pieces of a line
-                const int swz = p.bs_log2 == 7 ? d & 7 : p.bs_log2 == 6 ? (d >> 1) & 3 : p.bs_log2 == 5 ? (d >> 2) & 1 : 0;
                 uint4* at = reinterpret_cast<uint4*>(sm.v[slot] + (c / per_line) * (HD * bs) + d * bs + (((c % per_line) ^ swz) << 4));
                 uint4 v = *at;
                 uint32_t* words = &v.x;
+                uint32_t bad = 0;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                   uint32_t mask = 0;
@@ -680,9 +685,25 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
                   for (int e = 0; e < 4; ++e)
                     if (there && ct + 4 * b + e >= u.any_lo && ct + 4 * b + e < u.any_hi) mask |= 0xffu << (8 * e);
                   words[b] &= mask;
+                  bad |= nan_codes(words[b]);
+                }
+                if (bad != 0) {
+#pragma unroll
+                  for (int b = 0; b < 4; ++b) {
+                    const uint32_t nan = nan_codes(words[b]);
+#pragma unroll 1
+                    for (uint32_t n = nan; n != 0; n &= n - 1) {
+                      const int t = ct + 4 * b + ((__ffs(n) - 1) >> 3);
+#pragma unroll
+                      for (int z = 0; z < ROWS; ++z)
+                        if (t >= sm.row_lo[buf][z] && t < sm.row_hi[buf][z]) acc[h][z] = __uint_as_float(0x7fffffffu);
+                    }
+                    words[b] &= ~((nan >> 7) * 0xffu);
+                  }
                 }
                 *at = v;
               }
+            }
           }
         }
         fence_async_shared();

@@ -87,6 +87,9 @@ __device__ __forceinline__ void codes4_to_f16(uint32_t w, uint32_t* lo, uint32_t
   }
 }
 
+// Bit 7 of each byte of w that is an E4M3 NaN (0x7f or 0xff).
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // Once per device: shared memory for a kernel's blocks.
 constexpr int kMaxDevices = 64;
 template <typename K>

@@ -177,6 +177,32 @@ def test_value_scales_that_are_no_numbers(codes, grp, new, window, value):
     c.check_odd(window)
 
 
+@pytest.mark.parametrize("window", [0, 20, 150])
+@pytest.mark.parametrize("hd,bs", [(64, 16), (128, 32), (128, 128), (256, 64)])
+@pytest.mark.parametrize("new,grp", [((1, 1), 4), ((6, 3), 2), ((9, 8), 1)])
+def test_codes_that_are_no_numbers(new, grp, hd, bs, window):
+    """E4M3 codes 0x7f and 0xff: a value's reaches its own dimension of the rows that see its token, a key's the whole
+    row."""
+    c = Case([310, 205], new, 2, grp, hd, bs, "fp8", "bf16", seed=6)
+    kraw, vraw = c.kc.view(torch.uint8), c.vc.view(torch.uint8)
+    at = lambda s, t: (int(c.table[s, t // bs]), t % bs)  # noqa: E731
+    for t, head, d, code in ((309, 0, 3, 0x7F), (307, 0, hd - 1, 0xFF), (310 - new[0] // 2 - 1, 0, 17, 0x7F), (306, 0, 18, 0x7F)):
+        page, off = at(0, t)
+        vraw[page, head, d, off] = code
+    page, off = at(1, 205 - (new[1] + 1) // 2)
+    kraw[page, 1, 5, off] = 0x7F
+    vraw[page, 1, :, off] = 0xFF
+    got, lse = (x.cpu() for x in c.call(window))
+    out, want_lse, mag = c.want(window)
+    odd = ~torch.isfinite(out)
+    assert odd.any() and not odd.all()
+    assert torch.equal(torch.isnan(got), odd) and torch.equal(torch.isnan(lse), torch.isnan(want_lse))
+    zero = torch.zeros((), dtype=torch.float64)
+    clean = lambda x: torch.where(odd, zero.to(x.dtype), x)  # noqa: E731
+    check_attention(clean(got), torch.nan_to_num(lse, nan=1.0, neginf=-math.inf), c.q, clean(out),
+                    torch.nan_to_num(want_lse, nan=1.0, neginf=-math.inf), clean(mag))
+
+
 @pytest.mark.parametrize("codes", ["int8", "fp8"])
 @pytest.mark.parametrize("new", [(1, 1), (5, 4), (40, 90)])
 @pytest.mark.parametrize("power", [-50, -90, -109])
