@@ -87,7 +87,7 @@ struct Smem {
   // lie in groups of 8.
   uint8_t q[2][(3 * ROWS + 7) / 8 * 8 * HD];  // of this unit and the next
   alignas(16) float ks[16][8], vs[16][8];  // scales per 16 tokens, tile number mod 16
-  uint32_t have[16];                       // bit c: 16-token piece c has a block
+  uint32_t have[16];                       // bit c: 16-token piece c has a block; bit 8 + c: whose V scale is no number
   int page[16][8], head[16];               // for the copies of V, which follow those of K
   alignas(16) float wmax[2][4][ROWS];
   alignas(16) float row_scale[2][ROWS];
@@ -496,32 +496,21 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         }
         return true;
       };
-      // V scales that are infinite or NaN: the rows that see such a block get NaN, for the others it weighs nothing.
-      // An integer cannot say so, and in E4M3 a weight of 0 times NaN would say it to every row.
-      auto odd_scales = [&](uint32_t tile, int tok0, int count, float (&vs)[C::kStep], float& vtop) {
-        uint32_t seen = 0;  // bit z: row z sees one
-        vtop = 0.f;
-        for (int y = 0; y < count; ++y) {
-          const uint32_t k = (tile + y) & 15;
-          for (int c = 0; c < 8; ++c) {
-            const float v = fabsf(sm.vs[k][c]);
-            const int t0 = tok0 + y * kTile + 16 * c;
-            if (v < INFINITY) {
-              vtop = fmaxf(vtop, v);
-            } else {
-              for (int z = 0; z < ROWS; ++z)
-                if (max(sm.row_lo[buf][z], t0) < min(sm.row_hi[buf][z], t0 + 16)) seen |= 1u << z;
-            }
+      // Blocks whose V scale is infinite or NaN (pieces of the tile at tk) come with a scale of 0: the rows that see one
+      // get NaN here.  An integer cannot say so, and in E4M3 a weight of 0 times NaN would say it to every row.
+      auto odd_scales = [&](uint32_t pieces, int tk) {
+#pragma unroll
+        for (int z = 0; z < ROWS; ++z) {
+          bool seen = false;
+#pragma unroll 1
+          for (uint32_t left = pieces; left != 0; left &= left - 1) {
+            const int t0 = tk + 16 * (__ffs(left) - 1);
+            seen |= max(sm.row_lo[buf][z], t0) < min(sm.row_hi[buf][z], t0 + 16);
           }
-        }
-#pragma unroll
-        for (int y = 0; y < C::kStep; ++y)
-          if (!(fabsf(vs[y]) < INFINITY)) vs[y] = 0.f;
-#pragma unroll
-        for (int z = 0; z < ROWS; ++z)
 #pragma unroll
           for (int h = 0; h < C::kParts; ++h)
-            if (seen >> z & 1) acc[h][z] = __uint_as_float(0x7fffffffu);
+            if (seen) acc[h][z] = __uint_as_float(0x7fffffffu);
+        }
       };
       // A warp that gave up goes through the same barriers as the others, without waiting for anything else.
       for (int t = 0; t < steps; ++t) {
@@ -556,16 +545,16 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
           if (tk < u.all_lo || tk + kTile > u.all_hi || have != 0xffu) {
             const bool there = (have >> piece) & 1;
             if (!there) vs[y] = 0.f;
+            if (have > 0xffu) odd_scales(have >> 8, tk);
 #pragma unroll
             for (int z = 0; z < ROWS; ++z)
               if (!there || tk + tid < sm.row_lo[buf][z] || tk + tid >= sm.row_hi[buf][z]) s[y][z] = -INFINITY;
           }
           if (y < count) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) vtop = max_or_nan(vtop, fabsf(sm.vs[k][c]));
+            for (int c = 0; c < 8; ++c) vtop = fmaxf(vtop, fabsf(sm.vs[k][c]));
           }
         }
-        if (!(vtop < INFINITY)) odd_scales(tile, tok0, count, vs, vtop);
 #pragma unroll
         for (int z = 0; z < ROWS; ++z) top[z] = warp_max(C::kStep == 2 ? fmaxf(s[0][z], s[C::kStep - 1][z]) : s[0][z]);
         if (lane == 0) {
@@ -787,6 +776,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     const uint32_t k_to = smem_addr(sm.k) + piece * (HD * 16), v_to = smem_addr(sm.v) + piece * (HD * 16);
     struct Batch {
       int count, head, page;
+      uint32_t odd;  // lanes whose V scale is infinite or NaN
       float ks, vs;
     } next;
     int gt = 0;
@@ -810,6 +800,9 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         next.ks = __ldg(p.key_scale + next.page * p.ks_sb + next.head * p.ks_sh);
         next.vs = __ldg(p.value_scale + next.page * p.vs_sb + next.head * p.vs_sh);
       }
+      const bool odd = !(fabsf(next.vs) < INFINITY);
+      next.odd = __ballot_sync(0xffffffffu, odd);
+      if (odd) next.vs = 0.f;
       gt += next.count;
     };
     look_ahead();
@@ -837,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
           sm.vs[ring][piece] = b.vs;
           sm.page[ring][piece] = b.page;
           if (piece == 0) {
-            sm.have[ring] = there >> (8 * j);
+            sm.have[ring] = there >> (8 * j) | (b.odd >> (8 * j) & 0xffu) << 8;
             sm.head[ring] = b.head;
           }
         }

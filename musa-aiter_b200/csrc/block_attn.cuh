@@ -117,13 +117,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// The larger, or NaN where either is.
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
 // Two 32-bit operations in one instruction, each rounded as its scalar form.
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
