@@ -573,13 +573,12 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             top[z + 2] = fmaxf(top[z + 2], o.z);
             top[z + 3] = fmaxf(top[z + 3], o.w);
           }
-        // The largest weight, in units of its last digit (int8) and of its first term.  Scales may be as small as there
-        // are numbers: the quotient is taken after both were lifted by 2^60.
+        // The largest weight, in units of its last digit (int8) and of its first term.  By the reciprocal first: kFull
+        // over a scale of 2^-109 leaves 32 bits.  Scales that have no reciprocal, below 2^-126, count as 0.
         constexpr float kFull = CODE == MAK_CODE_INT8 ? 127.f * 16777216.f : 256.f, kLead = CODE == MAK_CODE_INT8 ? 127.f : 256.f;
-        const float lift = vtop < 0x1p-60f ? 0x1p60f : 1.f;
-        const float weight = vtop > 0.f ? kFull / (vtop * lift) : 0.f;
+        const float inv = vtop >= 0x1p-126f ? 1.f / vtop : 0.f;
 #pragma unroll
-        for (int y = 0; y < C::kStep; ++y) vs[y] *= lift;
+        for (int y = 0; y < C::kStep; ++y) vs[y] = vs[y] * inv * kFull;
         float fade[ROWS], next_gain[ROWS];
         uint32_t words[C::kStep][4][ROWS / 4];  // weights of this thread's tokens: term, four rows
 #pragma unroll
@@ -596,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             for (int y = 0; y < C::kStep; ++y) {
               w[y][e] = exp2_fast(s[y][z] - mz);
               sum += w[y][e];
-              w[y][e] *= vs[y] * weight;  // both factors first: theirs is at most kFull
+              w[y][e] *= vs[y];
             }
             l[z] = l[z] * old + sum * add;
             fade[z] = old;
