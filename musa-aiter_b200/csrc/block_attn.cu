@@ -87,17 +87,19 @@ struct Smem {
   // lie in groups of 8.
   uint8_t q[2][(3 * ROWS + 7) / 8 * 8 * HD];  // of this unit and the next
   alignas(16) float ks[16][8], vs[16][8];  // scales per 16 tokens, tile number mod 16
-  uint32_t have[16];                       // bit c: 16-token piece c has a block; bit 8 + c: whose V scale is no number
+  uint32_t have[16];                       // bit c: 16-token piece c has a block
   int page[16][8], head[16];               // for the copies of V, which follow those of K
   alignas(16) float wmax[2][4][ROWS];
   alignas(16) float row_scale[2][ROWS];
   int row_lo[2][ROWS], row_hi[2][ROWS];
   alignas(8) int64_t row_out[2][ROWS], row_lse[2][ROWS];  // places of the results
+  int unit_seq[2], unit_head[2], unit_lo[2], unit_hi[2];  // tokens [lo, hi) of this block's tiles; lo on a tile's border
   float lsum[4][ROWS];
   alignas(8) uint64_t k_full[C::kKs], k_empty[C::kKs], v_full[C::kVs], v_empty[C::kVs];
   uint64_t q_full, s_full[2], p_full, o_full, spare;
   uint32_t tmem;
   int gave_up, last;
+  int odd;  // this block met a V scale that is infinite or NaN, or an E4M3 NaN
 };
 
 // Tiles of a unit of sequence v (at least one, so that empty rows are written).
@@ -231,6 +233,77 @@ __device__ __forceinline__ float join_terms(const uint32_t (&t)[TERMS]) {
   return x;
 }
 
+// E4M3 values of the tile at token tk: in its 16-token pieces `part`, codes that no row sees and NaN become 0.
+template <int HD>
+__device__ __forceinline__ void clean_tile(uint8_t* tile, int tk, uint32_t part, uint32_t have, int any_lo, int any_hi, int bs_log2,
+                                        volatile int* odd) {
+  const int bs = 1 << bs_log2, per_line = bs >> 4;  // 16-byte pieces of a line
+  for (uint32_t left = part & 0xffu; left != 0; left &= left - 1) {
+    const int c = __ffs(left) - 1;
+    const int from = have >> c & 1 ? any_lo - tk - 16 * c : 16, to = any_hi - tk - 16 * c;  // of its tokens, what some row sees
+    uint32_t mask[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      mask[b] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (4 * b + e >= from && 4 * b + e < to) mask[b] |= 0xffu << (8 * e);
+    }
+    for (int d = threadIdx.x; d < HD; d += kSoft) {
+      const int swz = bs_log2 == 7 ? d & 7 : bs_log2 == 6 ? (d >> 1) & 3 : bs_log2 == 5 ? (d >> 2) & 1 : 0;
+      uint4* at = reinterpret_cast<uint4*>(tile + (c / per_line) * (HD * bs) + d * bs + (((c % per_line) ^ swz) << 4));
+      uint4 v = *at;
+      uint32_t bad = 0;
+      auto clean = [&](uint32_t w, uint32_t m) {
+        const uint32_t nan = nan_codes(w & m);
+        bad |= nan;
+        return w & m & ~((nan >> 7) * 0xffu);
+      };
+      v = make_uint4(clean(v.x, mask[0]), clean(v.y, mask[1]), clean(v.z, mask[2]), clean(v.w, mask[3]));
+      if (bad != 0) *odd = 1;
+      *at = v;
+    }
+  }
+}
+
+// Results that are no numbers: the rows, one bit each, of the unit whose rows lie in `buf` that see a block whose V scale
+// is infinite or NaN, and in E4M3 those whose dimension d is NaN at a token that they see.  Both were 0 in the products,
+// where a weight of 0 would have brought them to every row.  Called once this block has met any; by whole warps.
+template <int HD, int ROWS, int CODE>
+__device__ __noinline__ uint32_t odd_rows(const BlockAttnParams& p, const Smem<HD, ROWS>& sm, int buf, int d) {
+  auto rows_seeing = [&](int t0, int t1) {
+    uint32_t rows = 0;
+    for (int z = 0; z < ROWS; ++z)
+      if (max(sm.row_lo[buf][z], t0) < min(sm.row_hi[buf][z], t1)) rows |= 1u << z;
+    return rows;
+  };
+  const int begin = sm.unit_lo[buf], end = sm.unit_hi[buf], bs = 1 << p.bs_log2;
+  const int64_t head = sm.unit_head[buf];
+  const int32_t* table = p.tables + sm.unit_seq[buf] * p.table_stride;
+  auto page_of = [&](int tk) {
+    const int page = __ldg(table + (tk >> p.bs_log2));
+    return page < p.num_blocks ? page : -1;
+  };
+  uint32_t rows = 0;
+  for (int tk = begin + (threadIdx.x & 31) * 16; tk < end; tk += 512) {
+    const int page = page_of(tk);
+    if (page >= 0 && !(fabsf(__ldg(p.value_scale + page * p.vs_sb + head * p.vs_sh)) < INFINITY)) rows |= rows_seeing(tk, tk + 16);
+  }
+  rows = __reduce_or_sync(0xffffffffu, rows);
+  if (CODE == MAK_CODE_E4M3 && d < HD) {
+    for (int tk = begin; tk < end; tk += 16) {
+      const int page = page_of(tk);
+      if (page < 0) continue;
+      const uint8_t* codes = p.value + page * p.v_sb + head * p.v_sh + static_cast<int64_t>(d) * bs + (tk & (bs - 1));
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(codes));
+      if ((nan_codes(v.x) | nan_codes(v.y) | nan_codes(v.z) | nan_codes(v.w)) == 0) continue;
+      for (int t = 0; t < 16; ++t)
+        if (nan_codes(__ldg(codes + t)) != 0) rows |= rows_seeing(tk + t, tk + t + 1);
+    }
+  }
+  return rows;
+}
+
 template <int HD, int ROWS, int CODE>
 __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     block_attn_rows_kernel(const __grid_constant__ BlockAttnParams p, const __grid_constant__ CUtensorMap kmap,
@@ -279,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
   const int64_t w_begin = walk.w;
   if (tid == kSoft) {
     sm.gave_up = 0;
+    sm.odd = 0;
     for (int i = 0; i < kKs; ++i) {
       mbar_init(&sm.k_full[i], 1);
       mbar_init(&sm.k_empty[i], 1);
@@ -302,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     __syncthreads();
     tc_fence_after();
   };
-  volatile int* gave_up = &sm.gave_up;
+  volatile int *gave_up = &sm.gave_up, *odd = &sm.odd;
   const int bs = 1 << p.bs_log2;
   Unit u;
   auto block_of = [&](int64_t w) {
@@ -334,6 +408,12 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
       }
     };
     auto stage = [&](const Unit& u, int buf) {
+      if (tid == 0) {
+        sm.unit_seq[buf] = u.seq;
+        sm.unit_head[buf] = u.head;
+        sm.unit_lo[buf] = u.t_first * kTile;
+        sm.unit_hi[buf] = min(u.t_last * kTile, u.any_hi);
+      }
       if (r < ROWS && d0 == 0) {
         const int i = (u.row0 + r) / p.group, j = u.head * p.group + (u.row0 + r) - i * p.group;
         int lo = 0, hi = 0;
@@ -496,22 +576,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         }
         return true;
       };
-      // Blocks whose V scale is infinite or NaN (pieces of the tile at tk) come with a scale of 0: the rows that see one
-      // get NaN here.  An integer cannot say so, and in E4M3 a weight of 0 times NaN would say it to every row.
-      auto odd_scales = [&](uint32_t pieces, int tk) {
-#pragma unroll
-        for (int z = 0; z < ROWS; ++z) {
-          bool seen = false;
-#pragma unroll 1
-          for (uint32_t left = pieces; left != 0; left &= left - 1) {
-            const int t0 = tk + 16 * (__ffs(left) - 1);
-            seen |= max(sm.row_lo[buf][z], t0) < min(sm.row_hi[buf][z], t0 + 16);
-          }
-#pragma unroll
-          for (int h = 0; h < C::kParts; ++h)
-            if (seen) acc[h][z] = __uint_as_float(0x7fffffffu);
-        }
-      };
       // A warp that gave up goes through the same barriers as the others, without waiting for anything else.
       for (int t = 0; t < steps; ++t) {
         const uint32_t x = it + t, tile = tiles_done + t * C::kStep;
@@ -545,7 +609,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
           if (tk < u.all_lo || tk + kTile > u.all_hi || have != 0xffu) {
             const bool there = (have >> piece) & 1;
             if (!there) vs[y] = 0.f;
-            if (have > 0xffu) odd_scales(have >> 8, tk);
 #pragma unroll
             for (int z = 0; z < ROWS; ++z)
               if (!there || tk + tid < sm.row_lo[buf][z] || tk + tid >= sm.row_hi[buf][z]) s[y][z] = -INFINITY;
@@ -639,8 +702,8 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             *reinterpret_cast<uint4*>(sm.p + (c * C::kStep * kTile + y * kTile + tid) * 16) =
                 make_uint4(x4[4 * c], x4[4 * c + 1], x4[4 * c + 2], x4[4 * c + 3]);
         }
-        // E4M3: codes may be NaN, which a weight of zero does not cancel.  What no row sees becomes 0, and so does a NaN
-        // in a piece that not every row sees whole: its dimension, this thread's, becomes NaN for the rows that see it.
+        // E4M3: codes may be NaN, which a weight of zero does not cancel.  They become 0 in the pieces that not every row
+        // sees whole, as does what no row sees; the rows that do see one get NaN with their results.
         if (CODE == MAK_CODE_E4M3) {
           for (int y = 0; y < count; ++y) {
             const int tk = tok0 + y * kTile;
@@ -648,56 +711,25 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
             if (tk >= u.all_lo && tk + kTile <= u.all_hi && have == 0xffu) continue;
             const uint32_t slot = (tile + y) % kVs;
             ok = ok && mbar_wait_warp(&sm.v_full[slot], ((tile + y) / kVs) & 1, gave_up);
-            // pieces that are not seen whole by every row
             uint32_t part = ~have & 0xffu;
             if (tk < u.all_lo) part |= (2u << min((u.all_lo - tk) >> 4, 7)) - 1;
             if (tk + kTile > u.all_hi) part |= 0xffu << (max(u.all_hi - tk, 0) >> 4);
-            const int per_line = bs >> 4;  // 16-byte pieces of a line
-#pragma unroll
-            for (int h = 0; h < C::kParts; ++h) {
-              const int d = h * 128 + tid;
-              if (HD < 128 && d >= HD) break;
-              const int swz = p.bs_log2 == 7 ? d & 7 : p.bs_log2 == 6 ? (d >> 1) & 3 : p.bs_log2 == 5 ? (d >> 2) & 1 : 0;
-              for (uint32_t left = part & 0xffu; left != 0; left &= left - 1) {
-                const int c = __ffs(left) - 1;
-                const int ct = tk + 16 * c;
-                const bool there = (have >> c) & 1;
-                uint4* at = reinterpret_cast<uint4*>(sm.v[slot] + (c / per_line) * (HD * bs) + d * bs + (((c % per_line) ^ swz) << 4));
-                uint4 v = *at;
-                uint32_t* words = &v.x;
-                uint32_t bad = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                  uint32_t mask = 0;
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    if (there && ct + 4 * b + e >= u.any_lo && ct + 4 * b + e < u.any_hi) mask |= 0xffu << (8 * e);
-                  words[b] &= mask;
-                  bad |= nan_codes(words[b]);
-                }
-                if (bad != 0) {
-#pragma unroll
-                  for (int b = 0; b < 4; ++b) {
-                    const uint32_t nan = nan_codes(words[b]);
-#pragma unroll 1
-                    for (uint32_t n = nan; n != 0; n &= n - 1) {
-                      const int t = ct + 4 * b + ((__ffs(n) - 1) >> 3);
-#pragma unroll
-                      for (int z = 0; z < ROWS; ++z)
-                        if (t >= sm.row_lo[buf][z] && t < sm.row_hi[buf][z]) acc[h][z] = __uint_as_float(0x7fffffffu);
-                    }
-                    words[b] &= ~((nan >> 7) * 0xffu);
-                  }
-                }
-                *at = v;
-              }
-            }
+            clean_tile<HD>(sm.v[slot], tk, part, have, u.any_lo, u.any_hi, p.bs_log2, odd);
           }
         }
         fence_async_shared();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full);
+      }
+      if (__any_sync(0xffffffffu, *odd)) {  // the last product has yet to join the sums: NaN stays NaN
+#pragma unroll
+        for (int h = 0; h < C::kParts; ++h) {
+          const uint32_t rows = odd_rows<HD, ROWS, CODE>(p, sm, buf, h * 128 + tid);
+#pragma unroll
+          for (int z = 0; z < ROWS; ++z)
+            if (rows >> z & 1) acc[h][z] = __uint_as_float(0x7fffffffu);
+        }
       }
       // The next unit's rows, so that the tensor cores begin on it while this one ends.
       close();
@@ -775,7 +807,6 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
     const uint32_t k_to = smem_addr(sm.k) + piece * (HD * 16), v_to = smem_addr(sm.v) + piece * (HD * 16);
     struct Batch {
       int count, head, page;
-      uint32_t odd;  // lanes whose V scale is infinite or NaN
       float ks, vs;
     } next;
     int gt = 0;
@@ -799,9 +830,10 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
         next.ks = __ldg(p.key_scale + next.page * p.ks_sb + next.head * p.ks_sh);
         next.vs = __ldg(p.value_scale + next.page * p.vs_sb + next.head * p.vs_sh);
       }
-      const bool odd = !(fabsf(next.vs) < INFINITY);
-      next.odd = __ballot_sync(0xffffffffu, odd);
-      if (odd) next.vs = 0.f;
+      if (!(fabsf(next.vs) < INFINITY)) {  // counts as 0 until the results: an integer weight cannot say so
+        next.vs = 0.f;
+        *odd = 1;
+      }
       gt += next.count;
     };
     look_ahead();
@@ -829,7 +861,7 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2)
           sm.vs[ring][piece] = b.vs;
           sm.page[ring][piece] = b.page;
           if (piece == 0) {
-            sm.have[ring] = there >> (8 * j) | (b.odd >> (8 * j) & 0xffu) << 8;
+            sm.have[ring] = there >> (8 * j);
             sm.head[ring] = b.head;
           }
         }
