@@ -70,18 +70,17 @@ struct Plan {
 // Tiles of row tile `tile` of a sequence (0: there is no such row tile) and the tokens they lie in.  Numbers below the
 // first sequence's, whose rows need not begin at 0, come as negative ones.
 struct Span {
-  int live, any_lo, any_hi, t0, tiles;
+  int live, any_lo, any_hi, all_lo, all_hi, t0, tiles;  // tokens that some / all rows see
 };
 __device__ __forceinline__ Span span_of(const BlockAttnParams& p, const SeqView& v, int tile) {
   Span s;
   const int64_t left = static_cast<int64_t>(v.rows) * p.group - static_cast<int64_t>(tile) * kUnitRows;
   s.live = tile < 0 || left <= 0 ? 0 : left < kUnitRows ? static_cast<int>(left) : kUnitRows;
-  s.any_lo = s.any_hi = s.t0 = s.tiles = 0;
+  s.any_lo = s.any_hi = s.all_lo = s.all_hi = s.t0 = s.tiles = 0;
   if (s.live == 0) return s;
-  int unused;
   const int64_t row0 = static_cast<int64_t>(tile) * kUnitRows;
-  row_range(p, v, static_cast<int>(row0 / p.group), &s.any_lo, &unused);
-  row_range(p, v, static_cast<int>((row0 + s.live - 1) / p.group), &unused, &s.any_hi);
+  row_range(p, v, static_cast<int>(row0 / p.group), &s.any_lo, &s.all_hi);
+  row_range(p, v, static_cast<int>((row0 + s.live - 1) / p.group), &s.all_lo, &s.any_hi);
   if (s.any_hi > s.any_lo) {
     s.t0 = s.any_lo / kTile;
     s.tiles = (s.any_hi + kTile - 1) / kTile - s.t0;
@@ -159,7 +158,7 @@ struct Walk {
   Span span;
 };
 struct Unit {
-  int seq, head, tile, live, ta, tb, any_lo, any_hi, t_first, n;  // this block has tiles [ta, tb), n of them real, from t_first on
+  int seq, head, tile, live, ta, tb, any_lo, any_hi, all_lo, all_hi, t_first, n;  // this block has tiles [ta, tb), n of them real, from t_first on
   int64_t w_tiles;
   int len;  // tiles of the whole unit, at least 1
   SeqView v;
@@ -181,7 +180,32 @@ struct TcSmem {
   int more[10];
   uint32_t tmem;
   int gave_up, last;
+  int nan_seen;  // E4M3: this block replaced a NaN
 };
+
+// E4M3: the dimensions d .. d + 16, one bit each, whose values are NaN at a token that row i of the unit sees, in the
+// pieces where the loading warps replaced NaN: those that not every row of the unit sees whole.
+__device__ __forceinline__ uint32_t nan_dims(const BlockAttnParams& p, const Unit& u, uint32_t i, int d) {
+  int lo, hi;
+  row_range(p, u.v, i, &lo, &hi);
+  lo = max(lo, u.t_first * kTile);
+  hi = min(hi, (u.t_first + u.n) * kTile);
+  const int bs = 1 << p.bs_log2;
+  uint32_t bad = 0;
+#pragma unroll 1
+  for (int kt = lo & ~15; kt < hi; kt += 16) {
+    if (kt >= u.all_lo && kt + 16 <= u.all_hi) continue;
+    const int page = __ldg(p.tables + u.seq * p.table_stride + (kt >> p.bs_log2));
+    if (page < 0 || page >= p.num_blocks) continue;
+    const uint8_t* codes = p.value + page * p.v_sb + u.head * p.v_sh + static_cast<int64_t>(d) * bs + (kt & (bs - 1));
+#pragma unroll 1
+    for (int e = 0; e < 16; ++e, codes += bs)
+#pragma unroll 1
+      for (int t = max(lo - kt, 0); t < min(hi - kt, 16); ++t)
+        if ((__ldg(codes + t) & 0x7f) == 0x7f) bad |= 1u << e;
+  }
+  return bad;
+}
 
 __device__ __forceinline__ void look_up(const BlockAttnParams& p, const Plan* plan, Walk& k) {
   k.seq = plan->seq[k.item];
@@ -198,7 +222,7 @@ __device__ __forceinline__ bool next_unit(const BlockAttnParams& p, const Plan* 
     u.tb = static_cast<int>(min(k.w_end - k.w0 - kUnitCost, static_cast<int64_t>(len)));
     u.len = len;
     u.seq = k.seq, u.head = k.head, u.tile = k.tile, u.live = k.span.live, u.v = k.v;
-    u.any_lo = k.span.any_lo, u.any_hi = k.span.any_hi;
+    u.any_lo = k.span.any_lo, u.any_hi = k.span.any_hi, u.all_lo = k.span.all_lo, u.all_hi = k.span.all_hi;
     u.w_tiles = k.w0 + kUnitCost;
     u.t_first = k.span.t0 + u.ta;
     u.n = k.span.tiles > 0 ? u.tb - u.ta : 0;
@@ -265,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (tid == 0) {
     sm.gave_up = 0;
+    sm.nan_seen = 0;
     mbar_init(&sm.spare, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.q_full[i], 4);
@@ -535,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float* lse = nullptr;
         if (on) place(row, dst, lse);
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        const bool nan_seen = CODE == MAK_CODE_E4M3 && u.n > 0 && *static_cast<volatile int*>(&sm.nan_seen);
 #pragma unroll 1
         for (int d = 0; d < HD; d += 16) {
           uint32_t x[16];
@@ -546,6 +572,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e)  // from 2^kLift to what l carries
             o[e] = u.n > 0 ? __uint_as_float(x[e]) * (1.f / (1 << kSpare)) : 0.f;
+          if (CODE == MAK_CODE_E4M3 && nan_seen && on) {
+            const uint32_t bad = nan_dims(p, u, row / p.group, d);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = bad >> e & 1 ? __uint_as_float(0x7fffffffu) : o[e];
+          }
           if (split) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) part[(d + e) * kUnitRows + tid] = o[e];
@@ -644,14 +675,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) sm.more[mine] = next_unit(p, plan, sm.walk[mine], sm.unit[mine]);
       __syncwarp();
       if (!sm.more[mine]) break;
-      const int n = u.n, t_first = u.t_first, any_lo = u.any_lo, any_hi = u.any_hi, head = u.head;
+      const int n = u.n, t_first = u.t_first, head = u.head;
+      // Pieces outside need a look at their codes: those that some row does not see where a code of V may be NaN.
+      constexpr bool kNan = CODE == MAK_CODE_E4M3;
+      const int inner_lo = kNan && is_v ? u.all_lo : u.any_lo, inner_hi = kNan && is_v ? u.all_hi : u.any_hi;
+      auto any_lo = [&]() { return kNan ? u.any_lo : inner_lo; };
+      auto any_hi = [&]() { return kNan ? u.any_hi : inner_hi; };
       const uint8_t* base = (is_v ? p.value + head * p.v_sh : p.key + head * p.k_sh) + d0 * bs;
       const int32_t* table = p.tables + u.seq * p.table_stride;
       auto token = [&](int t) { return (t_first + t) * kTile + 16 * chunk16; };
       auto find = [&](int t) {
         const int kt = token(t);
         int pg = -1;
-        if (t < n && kt < any_hi && kt + 16 > any_lo) pg = __ldg(table + (kt >> p.bs_log2));
+        if (t < n && kt < any_hi() && kt + 16 > any_lo()) pg = __ldg(table + (kt >> p.bs_log2));
         return pg >= p.num_blocks ? -1 : pg;
       };
       auto fetch = [&](int t, int pg) {
@@ -709,22 +745,39 @@ __global__ void __launch_bounds__(kThreads, 1)
           *reinterpret_cast<uint4*>(dst + it * 1024 + c0) = make_uint4(y[0], y[1], y[2], y[3]);
           *reinterpret_cast<uint4*>(dst + it * 1024 + c1) = make_uint4(y[4], y[5], y[6], y[7]);
         };
-        if (kt < any_lo || kt + 16 > any_hi) {
-          // tokens that no row sees: their codes may be anything and become 0
-          uint32_t mask[4];
+        uint32_t bad = 0;
+        if (kt < inner_lo || kt + 16 > inner_hi) {
+          if (!kNan || kt < any_lo() || kt + 16 > any_hi()) {
+            // tokens that no row sees: their codes may be anything and become 0
+            uint32_t mask[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            mask[q] = 0;
+            for (int q = 0; q < 4; ++q) {
+              mask[q] = 0;
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-              if (kt + 4 * q + b >= any_lo && kt + 4 * q + b < any_hi) mask[q] |= 0xffu << (8 * b);
+              for (int b = 0; b < 4; ++b)
+                if (kt + 4 * q + b >= any_lo() && kt + 4 * q + b < any_hi()) mask[q] |= 0xffu << (8 * b);
+            }
+#pragma unroll
+            for (int it = 0; it < kIts; ++it)
+              x[it] = make_uint4(x[it].x & mask[0], x[it].y & mask[1], x[it].z & mask[2], x[it].w & mask[3]);
           }
+          if (kNan && is_v) {
 #pragma unroll
-          for (int it = 0; it < kIts; ++it)
-            x[it] = make_uint4(x[it].x & mask[0], x[it].y & mask[1], x[it].z & mask[2], x[it].w & mask[3]);
+            for (int it = 0; it < kIts; ++it) bad |= nan_codes(x[it].x) | nan_codes(x[it].y) | nan_codes(x[it].z) | nan_codes(x[it].w);
+          }
         }
 #pragma unroll
         for (int it = 0; it < kIts; ++it) convert(it, x[it]);
+        if (kNan && bad != 0) {
+          // A weight of 0 times NaN would reach the rows that do not see the token: NaN becomes 0 here, and the rows that
+          // see it get it with their results.
+#pragma unroll 1
+          for (int e = 0; e < kIts * 16; ++e) {
+            uint16_t* h = reinterpret_cast<uint16_t*>(dst + (e >> 4) * 1024 + (e & 8 ? c1 : c0)) + (e & 7);
+            if ((*h & 0x7fffu) > 0x7c00u) *h = 0;
+          }
+          *static_cast<volatile int*>(&sm.nan_seen) = 1;
+        }
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[st]);

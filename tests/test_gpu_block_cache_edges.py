@@ -179,7 +179,7 @@ def test_value_scales_that_are_no_numbers(codes, grp, new, window, value):
 
 @pytest.mark.parametrize("window", [0, 20, 150])
 @pytest.mark.parametrize("hd,bs", [(64, 16), (128, 32), (128, 128), (256, 64)])
-@pytest.mark.parametrize("new,grp", [((1, 1), 4), ((6, 3), 2), ((9, 8), 1)])
+@pytest.mark.parametrize("new,grp", [((1, 1), 4), ((6, 3), 2), ((9, 8), 1), ((100, 70), 4), ((140, 130), 1)])
 def test_codes_that_are_no_numbers(new, grp, hd, bs, window):
     """E4M3 codes 0x7f and 0xff: a value's reaches its own dimension of the rows that see its token, a key's the whole
     row."""
