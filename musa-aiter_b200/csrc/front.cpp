@@ -136,7 +136,7 @@ at::Tensor aligned_rows(const at::Tensor& x) {
   const int64_t per = 16 / x.element_size();
   const auto st = x.strides();
   if (st[2] == 1 && st[0] % per == 0 && st[1] % per == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0) return x;
-  return x.is_contiguous() ? x.clone() : x.contiguous();
+  return x.clone(at::MemoryFormat::Contiguous);  // contiguous() would keep the stride of an axis with one entry, whatever it is
 }
 
 // ---- block-scaled caches --------------------------------------------------------------------------------
@@ -182,7 +182,10 @@ mak_block_cache_desc cache_desc(const char* name, Args a, int64_t rows, int64_t 
   for (const at::Tensor* t : {&kc, &vc, &ks, &vs, &table, &ctx}) dev.add(*t);
   d.key = kc.data_ptr(), d.value = vc.data_ptr();
   d.key_scale = static_cast<float*>(ks.data_ptr()), d.value_scale = static_cast<float*>(vs.data_ptr());
-  d.key_stride_block = kst[0], d.key_stride_head = kst[1], d.value_stride_block = vst[0], d.value_stride_head = vst[1];
+  // the stride of an axis with one entry reaches nothing: a multiple of 16 in its place
+  auto step = [&](at::IntArrayRef st, int64_t axis, int64_t size) { return size > 1 ? st[axis] : nh * hd * bs; };
+  d.key_stride_block = step(kst, 0, nb), d.key_stride_head = step(kst, 1, nh);
+  d.value_stride_block = step(vst, 0, nb), d.value_stride_head = step(vst, 1, nh);
   d.key_scale_stride_block = ks.stride(0), d.key_scale_stride_head = ks.stride(1);
   d.value_scale_stride_block = vs.stride(0), d.value_scale_stride_head = vs.stride(1);
   d.block_tables = static_cast<const int32_t*>(table.data_ptr());

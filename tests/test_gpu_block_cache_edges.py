@@ -254,3 +254,34 @@ def test_weights_of_the_smallest_scales_add_up(codes):
     want = (weight[:, None, None] * v).cumsum(0)[-new:] / total[:, None, None]
     mag = (weight[:, None, None] * v.abs()).cumsum(0)[-new:] / total[:, None, None]
     check_attention(got.double() * 2.0 ** 109, lse, q, want, total.log()[:, None].expand(new, nh), mag)
+
+
+# ---- tensors with a single row, head or block -----------------------------------------------------------
+
+
+def test_strides_of_axes_with_one_entry():
+    """A stride that no element is reached by counts for nothing."""
+    g = torch.Generator().manual_seed(9)
+    wide = torch.randn((1, 3, 132), generator=g).half().cuda()
+    one = wide[:, :1, :128]
+    assert one.stride() == (396, 132, 1)
+    cos, sin = torch.rand((5, 64), device="cuda"), torch.rand((5, 64), device="cuda")
+    pos = i32([[3], [1]])
+    plain = one.clone(memory_format=torch.contiguous_format)
+    for x, y in zip(ma.apply_rope_axes(one, one, pos, cos, sin, (32, 32)), ma.apply_rope_axes(plain, plain, pos, cos, sin, (32, 32))):
+        assert torch.equal(x, y)
+    c = Case([20], [1], 1, 1, 128, 16, "int8", "f16", seed=9)
+    want, got = ([x.cuda() for x in (c.kc, c.vc, c.ks, c.vs)] for _ in range(2))
+    ma.kv_append_block_scaled(plain, plain, *want, c.table.cuda(), i32([20]))
+    ma.kv_append_block_scaled(one, one, *got, c.table.cuda(), i32([20]))
+    for x, y in zip(want, got):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    a = ma.paged_attention_block_scaled(plain, *want, c.table.cuda(), i32([20]))
+    assert torch.equal(a, ma.paged_attention_block_scaled(one, *want, c.table.cuda(), i32([20])))
+    # caches of one head whose head stride is odd
+    odd = []
+    for x in want[:2]:
+        room = torch.zeros((x.shape[0], 128 * 16 + 16), dtype=x.dtype, device="cuda")
+        room[:, : 128 * 16] = x.view(x.shape[0], -1)
+        odd.append(room.as_strided(x.shape, (128 * 16 + 16, 7, 16, 1)))
+    assert torch.equal(a, ma.paged_attention_block_scaled(plain, *odd, *want[2:], c.table.cuda(), i32([20])))
