@@ -2,7 +2,7 @@
 
 A token has one position per axis; ``sections`` says how many of a head's pairs each axis turns.  Serving
 applies it before ``kv_append_block_scaled`` or ``copy_to_kv_cache``; ``apply_rope_axes_backward`` is its
-gradient.  Angles come as cos / sin tables indexed by position, as in ``apply_rope_to_key_cache``.
+gradient, which autograd also takes where q or k requires one.  Angles come as cos / sin tables indexed by position, as in ``apply_rope_to_key_cache``.
 """
 
 from __future__ import annotations
@@ -14,6 +14,35 @@ import torch
 from .. import _native
 
 __all__ = ["apply_rope_axes", "apply_rope_axes_backward"]
+
+
+class _Rotation(torch.autograd.Function):
+    """The rotation is linear in q and k: its gradient is the rotation by the negative angles, and so on."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse):
+        ctx.save_for_backward(positions, cos, sin)
+        ctx.how = (tuple(sections), interleaved, interleaved_axes)
+        ctx.inverse = inverse
+        return _native.front().rope(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse)
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k):
+        return (*_rotate(grad_q, grad_k, *ctx.saved_tensors, *ctx.how, not ctx.inverse), *(None,) * 7)
+
+
+def _wants_gradient(x) -> bool:
+    return getattr(x, "requires_grad", False)
+
+
+def _rotate(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse):
+    if torch.is_grad_enabled():
+        if _wants_gradient(cos) or _wants_gradient(sin):
+            name = "apply_rope_axes_backward" if inverse else "apply_rope_axes"
+            raise ValueError(f"{name}: cos and sin are tables without a gradient, detach them")
+        if _wants_gradient(q) or _wants_gradient(k):
+            return _Rotation.apply(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse)
+    return _native.front().rope(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse)
 
 
 def apply_rope_axes(
@@ -32,8 +61,9 @@ def apply_rope_axes(
     Pair j is (j, j + rot / 2), or (2 j, 2 j + 1) with ``interleaved``, of the first rot = 2 * sum(sections)
     columns; the others are copied.  Its angle is row positions[axis(j), t], column j of the tables; axes
     take their pairs one section after another, or in turn with ``interleaved_axes``.  Computed in 32 bits
-    and rounded once.  A pair whose position lies outside the tables stays as it is.  Returns new tensors."""
-    return _native.front().rope(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, False)
+    and rounded once.  A pair whose position lies outside the tables stays as it is.  Returns new tensors,
+    through which q and k get their gradients; cos and sin get none and may not require one."""
+    return _rotate(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, False)
 
 
 def apply_rope_axes_backward(
@@ -49,4 +79,4 @@ def apply_rope_axes_backward(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The gradient of ``apply_rope_axes`` in q and k from that of its outputs: the rotation by the negative
     angles."""
-    return _native.front().rope(grad_q, grad_k, positions, cos, sin, sections, interleaved, interleaved_axes, True)
+    return _rotate(grad_q, grad_k, positions, cos, sin, sections, interleaved, interleaved_axes, True)
