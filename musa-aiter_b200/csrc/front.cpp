@@ -17,6 +17,7 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "mak_kvcache.h"
@@ -198,10 +199,12 @@ mak_block_cache_desc cache_desc(const char* name, Args a, int64_t rows, int64_t 
 }
 
 // Attention workspaces, one per device and stream: the kernels leave their counters at zero, so calls that
-// follow one another on a stream share it.  Kept until the process ends.
+// follow one another on a stream share it.  The per-thread default stream is another one for each thread, under one
+// handle.  Kept until the process ends.
 at::Tensor workspace(const at::Device& device, cudaStream_t stream) {
   static std::mutex mutex;
-  static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>();
+  static thread_local char thread;
+  static auto* kept = new std::map<std::tuple<int, cudaStream_t, const void*>, at::Tensor>();
   const int64_t bytes = lib.workspace_bytes();
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
     // a graph may be replayed on any stream: it gets a workspace of its own
@@ -210,7 +213,7 @@ at::Tensor workspace(const at::Device& device, cudaStream_t stream) {
     return ws;
   }
   std::lock_guard<std::mutex> lock(mutex);
-  at::Tensor& ws = (*kept)[{device.index(), stream}];
+  at::Tensor& ws = (*kept)[{device.index(), stream, stream == cudaStreamPerThread ? &thread : nullptr}];
   if (!ws.defined()) ws = at::zeros({bytes}, at::TensorOptions().dtype(at::kByte).device(device));
   return ws;
 }

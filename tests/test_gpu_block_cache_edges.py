@@ -7,6 +7,7 @@ Bounds as in test_gpu_block_cache: derived there, not fitted.
 from __future__ import annotations
 
 import math
+import threading
 
 import pytest
 import torch
@@ -285,3 +286,38 @@ def test_strides_of_axes_with_one_entry():
         room[:, : 128 * 16] = x.view(x.shape[0], -1)
         odd.append(room.as_strided(x.shape, (128 * 16 + 16, 7, 16, 1)))
     assert torch.equal(a, ma.paged_attention_block_scaled(plain, *odd, *want[2:], c.table.cuda(), i32([20])))
+
+
+# ---- streams ----------------------------------------------------------------------------------------------
+
+
+def test_the_default_streams_of_two_threads():
+    """One handle, another stream in each thread: their partial sums must not meet."""
+    cases = [Case([9000], [1], 1, 8, 64, 64, "int8", "f16", seed=s) for s in (12, 13)]
+    args, outs, failed = [], [], []
+    for c in cases:
+        args.append([x.cuda() for x in (c.q, c.kc, c.vc, c.ks, c.vs, c.table)] + [i32(c.ctx)])
+        outs.append([torch.empty_like(args[-1][0]) for _ in range(100)])
+    want = [ma.paged_attention_block_scaled(*a) for a in args]
+    torch.cuda.synchronize()
+    start = threading.Barrier(2)
+
+    def work(i):
+        try:
+            stream = torch.cuda.ExternalStream(2)  # cudaStreamPerThread
+            with torch.cuda.stream(stream):
+                start.wait(60)
+                for out in outs[i]:
+                    ma.paged_attention_block_scaled(*args[i], out=out)
+                stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for i in range(2):
+        assert all(torch.equal(out, want[i]) for out in outs[i])
