@@ -71,6 +71,11 @@ int64_t integer(const char* name, const char* what, PyObject* o) {
   }
   return v;
 }
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v == 1;
+}
 void count(const char* name, Py_ssize_t got, Py_ssize_t want) {
   if (got != want) throw Refused{cat(name, ": ", want, " arguments, got ", got), false};
 }
@@ -228,7 +233,7 @@ PyObject* py_attend(PyObject*, Args a, Py_ssize_t n) {
     const at::ScalarType kind = q0.scalar_type();
     if (kind != at::kHalf && kind != at::kBFloat16) refuse(name, "q must be float16 or bfloat16, got ", toString(kind));
     const int64_t rows = q0.size(0), hq = q0.size(1), hd = q0.size(2);
-    const bool causal = PyObject_IsTrue(a[9]) == 1, want_lse = PyObject_IsTrue(a[11]) == 1;
+    const bool causal = truth(a[9]), want_lse = truth(a[11]);
     const int64_t window = integer(name, "window", a[10]);
     if (window < 0 || (window && !causal)) refuse(name, "window must be positive or 0 and needs causal=True");
     Device dev{name};
@@ -497,7 +502,7 @@ PyObject* py_copy(PyObject*, Args a, Py_ssize_t n) {
 // q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse
 PyObject* py_rope(PyObject*, Args a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    const bool inverse = n == 9 && PyObject_IsTrue(a[8]) == 1;
+    const bool inverse = n == 9 && truth(a[8]);
     const char* name = inverse ? "apply_rope_axes_backward" : "apply_rope_axes";
     count(name, n, 9);
     const at::Tensor &q0 = tensor(name, "q", a[0]), &k0 = tensor(name, "k", a[1]);
@@ -508,7 +513,7 @@ PyObject* py_rope(PyObject*, Args a, Py_ssize_t n) {
     if ((kind != at::kHalf && kind != at::kBFloat16) || k0.scalar_type() != kind)
       refuse(name, "q and k must both be float16 or both bfloat16");
     const int64_t tokens = q0.size(0), hq = q0.size(1), hk = k0.size(1), hd = q0.size(2);
-    const bool inter = PyObject_IsTrue(a[6]) == 1, dealt = PyObject_IsTrue(a[7]) == 1;
+    const bool inter = truth(a[6]), dealt = truth(a[7]);
     mak_rope_axes_desc d = {};
     // axis of each pair: the sections one after another, or dealt out in turn while one has pairs left
     std::vector<int64_t> sections;
