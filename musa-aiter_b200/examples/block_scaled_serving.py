@@ -2,8 +2,8 @@
 
 A few attention layers (random projections, no training) answer a handful of requests whose tokens have
 three position axes.  The scheduler's steps are page calls on device tensors; a layer's step is
-rotate, write, attend.  ``serve`` also keeps every request's keys and values in 32 bits and returns the
-largest difference between the layers' attention and plain attention over those.
+rotate, write, attend.  ``differences`` also keeps every request's keys and values as they were and holds
+the cache and the layers' attention against them; ``serve`` returns the attention's largest difference.
 
     python musa-aiter_b200/examples/block_scaled_serving.py
 """
@@ -38,6 +38,16 @@ class Layer:
     def planes(self):
         return [*self.codes, *self.scales]
 
+    def read(self, table, length):
+        """Keys and values [length, kv_heads, head_dim] of a row as the cache holds them, and the largest that each block
+        and head can hold, [length, kv_heads, 1]."""
+        block_size = self.codes[0].shape[3]
+        token = torch.arange(length, device=table.device)
+        page, at = table[token // block_size].long(), token % block_size
+        most = 127.0 if self.codes[0].dtype == torch.int8 else 448.0
+        scales = [s[page][..., None] for s in self.scales]
+        return [c[page, :, :, at].float() * s for c, s in zip(self.codes, scales)], [s * most for s in scales]
+
     def step(self, x, positions, cos, sin, tables, lens, starts):
         """One layer on packed rows x; returns the new x, the rotated q and k, v and the attention's result."""
         nq, nk, d = self.heads
@@ -59,7 +69,15 @@ def plain_attention(q, k, v):
     return torch.einsum("hit,thd->ihd", s.masked_fill(hidden, float("-inf")).softmax(-1), v)
 
 
-def serve(code=torch.int8, block_size=16, layers=2, decode_steps=6, seed=0, device="cuda"):
+def serve(*args, **kwargs):
+    """``differences`` for its first result alone."""
+    return differences(*args, **kwargs)["values"]
+
+
+def differences(code=torch.int8, block_size=16, layers=2, decode_steps=6, seed=0, device="cuda"):
+    """Serves the requests and returns the largest differences met: ``values``, of the attention from plain attention over
+    the keys and values that were written; ``cache``, from plain attention over what the cache holds of them; ``stored``,
+    of a value in the cache from the one written, as a part of the largest its block and head can hold."""
     g = torch.Generator().manual_seed(seed)
     hidden, pages, rows, max_blocks = 256, 160, 6, 24
     stack = [Layer(g, hidden, 8, 2, 128, pages, block_size, code, device) for _ in range(layers)]
@@ -72,11 +90,13 @@ def serve(code=torch.int8, block_size=16, layers=2, decode_steps=6, seed=0, devi
     refs = torch.zeros(pages, dtype=torch.int32, device=device)
     ids = lambda x: torch.tensor(x, dtype=torch.int32, device=device)
     history = {}  # (row, layer) -> its keys and values so far
-    worst = 0.0
+    worst = dict(values=0.0, cache=0.0, stored=0.0)
+
+    def note(name, x):
+        worst[name] = max(worst[name], x.abs().max().item())
 
     def forward(live, counts):
         """The rows `live` take counts[i] tokens each: pages, then every layer."""
-        nonlocal worst
         short = ma.kv_pages_grow(tables, lens, ids(live), ids(counts), refs, block_size)
         at = [0]
         for n in counts:
@@ -93,7 +113,11 @@ def serve(code=torch.int8, block_size=16, layers=2, decode_steps=6, seed=0, devi
                 s = slice(at[j], at[j + 1])
                 old = history.get((r, i))
                 history[r, i] = (k[s], v[s]) if old is None else (torch.cat((old[0], k[s])), torch.cat((old[1], v[s])))
-                worst = max(worst, (o[s].double() - plain_attention(q[s], *history[r, i])).abs().max().item())
+                note("values", o[s].double() - plain_attention(q[s], *history[r, i]))
+                held, most = layer.read(tables[r], int(lens[r]))
+                note("cache", o[s].double() - plain_attention(q[s], *held))
+                for x_held, x_most, x_old in zip(held, most, history[r, i]):
+                    note("stored", (x_held - x_old.float()) / x_most)
         assert int(short) == 0
 
     forward([0, 1, 2], list(PROMPTS))
@@ -117,4 +141,6 @@ def serve(code=torch.int8, block_size=16, layers=2, decode_steps=6, seed=0, devi
 
 if __name__ == "__main__":
     for code in (torch.int8, torch.float8_e4m3fn):
-        print(f"{code}: largest difference from 32-bit keys and values {serve(code):.4f}")
+        got = differences(code)
+        print(f"{code}: attention differs by {got['values']:.4f} from the values written, by {got['cache']:.4f} from what the cache "
+              f"holds of them; a value by {got['stored']:.4f} of its block's largest")
