@@ -120,6 +120,19 @@ def test_writer_of_a_slice_of_a_batch(codes, skip, new):
         assert torch.equal(y.cpu(), scale) and torch.equal(x.cpu().float(), cache.float())
 
 
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("codes", ["int8", "fp8"])
+@pytest.mark.parametrize("prompt,singles,grp,hd", [(300, 12, 4, 64), (200, 60, 1, 128), (70, 40, 8, 128), (90, 30, 4, 256)])
+def test_a_prompt_and_single_tokens_in_one_call(prompt, singles, grp, hd, codes, window):
+    """One kernel takes them all, by their average: a prompt among groups of few rows, single tokens among many."""
+    g = torch.Generator().manual_seed(prompt)
+    ctx = torch.randint(1, 300, (singles,), generator=g).tolist()
+    at = singles // 2
+    ctx.insert(at, prompt + 150)
+    new = [1] * at + [prompt] + [1] * (singles - at)
+    Case(ctx, new, 1, grp, hd, 16, codes, "bf16", seed=prompt).check(window)
+
+
 # ---- positions ------------------------------------------------------------------------------------------
 
 
