@@ -67,23 +67,28 @@ def sources() -> list[Path]:
     return sorted(CSRC_DIR.glob("*.cu"))
 
 
-def _fingerprint() -> str:
+def _fingerprint(front: bool) -> str:
+    """Of what the library, or the Python entry, is built from."""
     h = hashlib.sha256()
-    for path in sources() + sorted(CSRC_DIR.glob("*.cuh")) + sorted(INCLUDE_DIR.glob("*.h")):
+    headers = sorted(INCLUDE_DIR.glob("*.h"))
+    for path in [FRONT_SOURCE] + headers if front else sources() + sorted(CSRC_DIR.glob("*.cuh")) + headers:
         h.update(path.name.encode())
         h.update(path.read_bytes())
-    h.update(FRONT_SOURCE.read_bytes())
-    h.update(" ".join(ARCH_FLAGS + NVCC_FLAGS).encode())
-    h.update((importlib.metadata.version("torch") + sys.version).encode())
+    h.update(" ".join([importlib.metadata.version("torch"), sys.version] if front else ARCH_FLAGS + NVCC_FLAGS).encode())
     return h.hexdigest()
 
 
-def _stamp_path() -> Path:
-    return LIB_DIR / (LIB_NAME + ".stamp")
+def _is_current(path: Path, front: bool) -> bool:
+    stamp = _stamp_path(path)
+    return path.exists() and stamp.exists() and stamp.read_text().strip() == _fingerprint(front)
+
+
+def _stamp_path(path: Path) -> Path:
+    return path.with_name(path.name + ".stamp")
 
 
 def is_built() -> bool:
-    return LIB_PATH.exists() and FRONT_PATH.exists() and _stamp_path().exists() and _stamp_path().read_text().strip() == _fingerprint()
+    return _is_current(LIB_PATH, False) and _is_current(FRONT_PATH, True)
 
 
 def _front_command(out: Path) -> list[str]:
@@ -99,44 +104,39 @@ def _front_command(out: Path) -> list[str]:
 
 
 def build(force: bool = False, verbose: bool = False) -> BuildResult:
-    """Compile every ``csrc/*.cu`` for sm_100a, link ``lib/libmak_kvcache.so`` and build ``lib/_mak_front.so``."""
-    if not force and is_built():
+    """Compile every ``csrc/*.cu`` for sm_100a, link ``lib/libmak_kvcache.so`` and build ``lib/_mak_front.so``, each
+    where its sources changed (the latter also for another torch or Python)."""
+    with_lib, with_front = (force or not _is_current(path, front) for path, front in ((LIB_PATH, False), (FRONT_PATH, True)))
+    if not with_lib and not with_front:
         return BuildResult(True, "up to date", LIB_PATH)
     nvcc = _nvcc()
-    if nvcc is None:
+    if with_lib and nvcc is None:
         return BuildResult(False, "nvcc compiler not found", None)
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     LIB_DIR.mkdir(parents=True, exist_ok=True)
-    include = ["-I", str(INCLUDE_DIR), "-I", str(CSRC_DIR)]
 
-    def compile_one(src: Path) -> tuple[Path, subprocess.CompletedProcess]:
-        obj = BUILD_DIR / (src.stem + ".o")
-        cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, *include, "-c", str(src), "-o", str(obj)]
+    def run(cmd: list[str]) -> subprocess.CompletedProcess:
         if verbose:
             print(" ".join(cmd))
-        return obj, subprocess.run(cmd, capture_output=True, text=True)
+        return subprocess.run(cmd, capture_output=True, text=True)
 
+    objects = [BUILD_DIR / (src.stem + ".o") for src in sources()] if with_lib else []
+    front_tmp, lib_tmp = LIB_DIR / "_mak_front.so.tmp", LIB_DIR / (LIB_NAME + ".tmp")
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
-        front_tmp = LIB_DIR / "_mak_front.so.tmp"
-        front_cmd = _front_command(front_tmp)
-        if verbose:
-            print(" ".join(front_cmd))
-        front = pool.submit(subprocess.run, front_cmd, capture_output=True, text=True)
-        results = list(pool.map(compile_one, sources()))
-        front = front.result()
-    if front.returncode != 0:
-        return BuildResult(False, front.stderr, None)
-    errors = [proc.stderr for _, proc in results if proc.returncode != 0]
+        jobs = [pool.submit(run, _front_command(front_tmp))] if with_front else []
+        include = ["-I", str(INCLUDE_DIR), "-I", str(CSRC_DIR)]
+        for src, obj in zip(sources() if with_lib else [], objects):
+            jobs.append(pool.submit(run, [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, *include, "-c", str(src), "-o", str(obj)]))
+        results = [job.result() for job in jobs]
+    if with_lib and not any(proc.returncode for proc in results):
+        results.append(run([nvcc, *ARCH_FLAGS, "-shared", "-o", str(lib_tmp), *map(str, objects)]))
+    errors = [proc.stderr for proc in results if proc.returncode != 0]
     if errors:
         return BuildResult(False, "\n".join(errors), None)
-    tmp = LIB_DIR / (LIB_NAME + ".tmp")
-    cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", str(tmp), *[str(obj) for obj, _ in results]]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        return BuildResult(False, proc.stderr, None)
-    os.replace(tmp, LIB_PATH)
-    os.replace(front_tmp, FRONT_PATH)
-    _stamp_path().write_text(_fingerprint() + "\n")
+    for tmp, path, front in ((lib_tmp, LIB_PATH, False), (front_tmp, FRONT_PATH, True)):
+        if with_front if front else with_lib:
+            os.replace(tmp, path)
+            _stamp_path(path).write_text(_fingerprint(front) + "\n")
     return BuildResult(True, "built", LIB_PATH)
 
 
