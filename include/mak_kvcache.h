@@ -654,7 +654,9 @@ MAK_API int64_t mak_block_attention_workspace_bytes(void);
  * Row r of sequence s is its (r - cu_seqlens[s])-th row of this call, at
  * position context_lens[s] - (rows of s) + that index; it sees tokens up to its
  * own position (causal) or all of them, and with window > 0 (causal only) the
- * last `window` of those.  A row that sees nothing gives zeros and lse = -inf.
+ * last `window` of those.  A row that sees nothing gives zeros and lse = -inf; what
+ * it does not see reaches it in no form, NaN among it.  cu_seqlens may begin above 0
+ * and end before num_rows: rows of no sequence are neither read nor written.
  * Block ids outside [0, num_blocks) are skipped like tokens outside the sequence,
  * and so are tokens past max_blocks * block_size; a length beyond that shifts no
  * position.
@@ -669,7 +671,9 @@ MAK_API int mak_block_attention(const mak_block_attn_desc* desc, void* stream);
  * writes the block's first position, else the larger of that and the old scale,
  * and the codes that stay are rounded again to a scale that grew.  Non-finite
  * values are stored as 0.  Positions behind the last token of a block that the
- * call begins are zeroed; other positions of the block keep their value.
+ * call begins are zeroed; other positions of the block keep their value.  Tokens past
+ * max_blocks * block_size have no place, rows of no sequence are not read, and a
+ * sequence with more rows than tokens is left alone.
  */
 MAK_API int mak_block_append(const mak_block_cache_desc* cache, const void* k, const void* v, int64_t k_stride_row,
                              int64_t k_stride_head, int64_t v_stride_row, int64_t v_stride_head, int32_t dtype, void* stream);

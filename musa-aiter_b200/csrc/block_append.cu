@@ -14,9 +14,10 @@
 // row, its stores whole 16-byte pieces of the tile's rows.
 //
 // Measured.  8 prompts of 900 to 4096 tokens, 8 heads of 128, bf16 to E4M3, blocks of 16: 22.3 us, 3.5 TB/s of a copy's
-// 6.47, bound by instructions (quotient, correction, rounding and packing of each value) with the loads' latency
-// behind them; 64 requests of one token, into blocks that held some: 4.3 us, latency (length, block id, rows and old
-// codes, new codes).
+// 6.47; f16 the same, f32 29.6 us, 4.3 TB/s.  Neither instructions nor HBM bound it alone: 15 instructions for 32 values
+// keep 0.53 of the issue slots busy, and of 8.2 cycles between two of a warp's 2.6 go to loads (lengths, block id and
+// rows come one after another, a tile a warp, 17 warps per SM) and 1.8 to waits of fixed length.  64 requests of one
+// token, into blocks that held some: 4.1 to 4.3 us, latency (length, block id, rows and old codes, new codes).
 #include "block_attn.cuh"
 
 namespace mak {

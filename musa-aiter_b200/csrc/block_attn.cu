@@ -11,8 +11,8 @@
 //     A row of q is scaled to a maximum in [2^7, 2^8) (three terms), weights to at most 2^8 (four).
 //   int8: x = x1 2^16 + x2 2^8 + x3, a whole number in balanced base 256: q to a maximum in
 //     [2^21, 2^22), weights to 127 * 2^24 (four digits).  The products are summed exactly in s32.
-// So q (bf16: 8 bits, f16: 11) goes in exactly but for values below 2^-13 of its row's largest,
-// and a weight is good to 2^-12 of itself or 2^-30 of its tile's largest.  The fourth term is free:
+// So a value of q (bf16: 8 bits, f16: 11) goes in exactly, or to 2^-22 (int8) or 2^-26 (E4M3) of its row's
+// largest where it is that much smaller, and a weight is good to 2^-12 of itself or 2^-30 of its tile's largest.  The fourth term is free:
 // 8 rows with three terms would be 24 columns, and the tensor cores want a multiple of 16.
 // Each step of one or two 128-token tiles has its own maximum, largest V scale and product with V;
 // steps are joined in 32-bit registers, so the tensor cores' accumulators never need rescaling.
@@ -30,14 +30,20 @@
 // to arrive joins them.  Roles: warps 0-3 softmax (a thread per token, then per head_dim row),
 // warp 4 copies, warp 5 issues the tensor cores; two steps are in flight between them.
 //
+// Numbers that are none.  What a row does not see reaches none of its sums, whatever it holds: masked scores are set
+// apart, V scales that are infinite or NaN count as 0 in the products, and so do E4M3 codes that are NaN where not every
+// row sees their tokens.  The rows that do see them get NaN at the unit's end (odd_rows).  That code is kept out of the
+// loop: inside it 64 sequences took 1.5 % longer, 16-row groups 5 %.
+//
 // Measured (a copy runs at 6.47 TB/s).  4 sequences of 100000 to 131072 tokens, 8 cache heads of 128 with 8 query
-// heads each, E4M3, blocks of 64: 158 us, 5.8 TB/s, bound by HBM.  64 sequences of 256 to 4096, 4 query heads each,
-// blocks of 16: 62 us, 4.7 TB/s: a block gets two or three units, and between units the copies wait for some 10000
-// cycles (masks of the last step, the next rows of q, the sums), as what they run ahead by is two tiles of K and four
-// of V, all that shared memory holds; instructions are fetched late too (1.5 of the 6 cycles between two of a warp's),
-// so less code is faster code.  Taking the next unit's rows and first scores before the last step ends: 65 us, as the
+// heads each, E4M3, blocks of 64: 156 to 169 us on several GPUs, 5.4 to 5.9 TB/s, bound by HBM.  64 sequences of 256 to
+// 4096, 4 query heads each, blocks of 16: 61 to 62 us, 4.7 TB/s: a block gets two or three units, and between units the
+// copies wait for some 10000 cycles (masks of the last step, the next rows of q, the sums), as what they run ahead by is
+// two tiles of K and four of V, all that shared memory holds.  Of 8.3 cycles between two instructions of a warp 2.8 go
+// to loads, 1.6 to waits of fixed length, 0.7 to instructions that come late; with groups of 8 rows, twice the code, 1.5
+// of 6: less code is faster code.  Taking the next unit's rows and first scores before the last step ends: 65 us, as the
 // loop grows; three blocks per SM with fewer tiles each: 65 us.  16 sequences of 300 to 4500, 16 heads of 64 on one
-// cache head, 1 to 8 rows: 26 to 28 us, either kernel.  One sequence of 777 tokens: 10 us, a chain of latencies
+// cache head, 1 to 8 rows: 25 to 28 us, either kernel.  One sequence of 777 tokens: 9 to 10 us, a chain of latencies
 // (lengths, block ids, K, scores, weights, sums).
 #include "block_attn.cuh"
 #include "tcgen05.cuh"

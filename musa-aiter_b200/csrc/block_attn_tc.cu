@@ -4,9 +4,17 @@
 // Mathematics as in block_attn.cu: S = q . codes, here with q and codes in f16 (codes exactly, a bf16
 // row of q by a power of two).  The V scale b of a token goes into its exponent: with m' the running
 // maximum of S' + log2 b, the weight 2^(S' + log2 b - m') multiplies the code and, times 1 / b, joins the
-// sum, which is taken in 32 bits before the weight is rounded once to f16.  The maximum is only moved
-// when it grew by more than 2^8 or so: weights then stay below 2^15 (they carry a factor 2^6), the result
-// is the same, and the accumulators in TMEM are rarely rescaled.
+// sum, which is taken in 32 bits before the weight is rounded once to f16: the tensor cores take 16-bit
+// weights next to f16 codes, and wider ones at half the rate or less.  A weight is off by 2^-12 of
+// itself at most: an f16 result's error grows by a fifth to a third (2.1e-4 to 2.5e-4 of its norm), a bf16
+// result's rounding hides it.  The maximum is only moved when it grew by more than 2^8 or so: weights then
+// stay below 2^15 (they carry a factor 2^6), the result is the same, and the accumulators in TMEM are
+// rarely rescaled.
+//
+// Numbers that are none.  What a row does not see reaches none of its sums, whatever it holds: its weights
+// there are 0, and E4M3 codes of V that are NaN become 0 where not every row of a unit sees their tokens;
+// the rows that do see them get NaN with their results (nan_dims).  In E4M3 that costs 0.7 % of a prompt
+// chunk's time, 2.6 % with a window of 512, nothing in int8.
 //
 // A block takes 256 rows of one cache head (heads of the group next to one another, so a K / V tile
 // serves all of them) as two tiles of 128, and walks the cache in tiles of 128 tokens.  Roles:
@@ -26,8 +34,8 @@
 // with V of a tile is issued before the next scores of the same rows overwrite them.
 //
 // Measured.  Two prompts' chunks of 1500 to 2048 rows against 5000 to 8192 tokens, 32 query heads on 8 cache heads of
-// 128, int8, bf16 q: 427 to 437 us, 850 to 868 TFLOP/s of the 1678 that a bf16 matrix product reaches; heads of 64 take
-// 0.8 of the time of heads of 128.  What bounds it is the chain from scores to scores of a row tile: some 3900 cycles
+// 128, int8, bf16 q: 442 to 461 us on several GPUs, 803 to 838 TFLOP/s of the 1678 that a bf16 matrix product reaches;
+// in E4M3 438 us where int8 takes 448; heads of 64 (f16 q, blocks of 64) 384 us, in E4M3 373.  What bounds it is the chain from scores to scores of a row tile: some 3900 cycles
 // of softmax, 1100 of its two products, 350 of handing over, against 2050 that the tensor cores need for both row
 // tiles.  Four instructions for each score and 2.3 for each pair of codes converted keep the issue slots 0.44 busy, the
 // exponential unit 0.39, and 128 rows take that long because each warp waits for itself; without any softmax or

@@ -42,7 +42,7 @@ def kv_append_block_scaled(
     call writes gets the scale m / 127 (int8) or m / 448 (float8_e4m3fn), and zeros behind its last
     token; a block that held tokens gets the larger of that and its old scale, and where the scale grows
     its codes are rounded again.  Non-finite values are stored as 0.  A block must belong to one sequence
-    of the call only.  In place; returns None."""
+    of the call only; a sequence with more rows than tokens is left alone.  In place; returns None."""
     _native.front().append(k, v, key_cache, value_cache, key_scale, value_scale, block_tables, context_lens, cu_seqlens)
 
 
@@ -67,8 +67,17 @@ def paged_attention_block_scaled(
     Query head h reads cache head h // (num_q_heads // num_heads).  The last rows of a sequence sit at its
     last positions: with ``causal`` a row sees the tokens up to its own, otherwise all of its sequence; a
     ``window`` > 0 (causal only) keeps the last ``window`` of those.  ``scale`` defaults to
-    1 / sqrt(head_dim).  Sums and softmax statistics are held in 32 bits.  Returns ``out`` (q's dtype), or
-    ``(out, lse)`` with the log of each row's sum of exponentials, float32 ``[rows, num_q_heads]``.  A row
-    that sees no token gives zeros and an lse of -inf."""
+    1 / sqrt(head_dim).  Returns ``out`` (q's dtype), or ``(out, lse)`` with the log of each row's sum of
+    exponentials, float32 ``[rows, num_q_heads]``.  A row that sees no token gives zeros and an lse of -inf.
+    Nothing that a row does not see reaches its result, NaN among it; a row that sees a value scale that is
+    infinite or NaN gives NaN.
+
+    Sums and softmax statistics are held in 32 bits.  The matrix units take less: with many rows to a
+    sequence each weight is rounded to float16 (2**-12 of itself; float16 results are off by 2.5e-4 of their
+    norm instead of 2.1e-4), with few it is good to 2**-12 of itself or 2**-30 of the largest in its tile,
+    and values of q to 2**-22 of their row's largest.
+
+    For inference: no gradient flows through it.  It keeps a workspace of 40 MB per device and stream until
+    the process ends; a call captured in a graph has one of its own and zeroes its counters there."""
     return _native.front().attend(q, key_cache, value_cache, key_scale, value_scale, block_tables, context_lens, cu_seqlens, scale,
                                   causal, window, return_lse, out)
