@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -499,7 +500,7 @@ PyObject* py_copy(PyObject*, Args a, Py_ssize_t n) {
 
 // ---- rotary positions ---------------------------------------------------------------------------------------
 
-// q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse
+// q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse; None where q or k wants a gradient
 PyObject* py_rope(PyObject*, Args a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const bool inverse = n == 9 && truth(a[8]);
@@ -507,6 +508,10 @@ PyObject* py_rope(PyObject*, Args a, Py_ssize_t n) {
     count(name, n, 9);
     const at::Tensor &q0 = tensor(name, "q", a[0]), &k0 = tensor(name, "k", a[1]);
     at::Tensor pos = tensor(name, "positions", a[2]), cos = tensor(name, "cos", a[3]), sin = tensor(name, "sin", a[4]);
+    if (c10::GradMode::is_enabled()) {
+      if (cos.requires_grad() || sin.requires_grad()) refuse(name, "cos and sin are tables without a gradient, detach them");
+      if (q0.requires_grad() || k0.requires_grad()) Py_RETURN_NONE;  // the caller's autograd function calls again, with gradients off
+    }
     if (q0.dim() != 3 || k0.dim() != 3 || q0.size(0) != k0.size(0) || q0.size(2) != k0.size(2))
       refuse(name, "q and k must be [tokens, heads, head_dim] with the same tokens and head_dim");
     const at::ScalarType kind = q0.scalar_type();

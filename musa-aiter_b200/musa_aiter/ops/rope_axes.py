@@ -17,7 +17,9 @@ __all__ = ["apply_rope_axes", "apply_rope_axes_backward"]
 
 
 class _Rotation(torch.autograd.Function):
-    """The rotation is linear in q and k: its gradient is the rotation by the negative angles, and so on."""
+    """The rotation is linear in q and k: its gradient is the rotation by the negative angles, and so on.
+
+    The native call answers None where q or k wants a gradient; here it is made again with gradients off."""
 
     @staticmethod
     def forward(ctx, q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse):
@@ -28,21 +30,8 @@ class _Rotation(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_q, grad_k):
-        return (*_rotate(grad_q, grad_k, *ctx.saved_tensors, *ctx.how, not ctx.inverse), *(None,) * 7)
-
-
-def _wants_gradient(x) -> bool:
-    return getattr(x, "requires_grad", False)
-
-
-def _rotate(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse):
-    if torch.is_grad_enabled():
-        if _wants_gradient(cos) or _wants_gradient(sin):
-            name = "apply_rope_axes_backward" if inverse else "apply_rope_axes"
-            raise ValueError(f"{name}: cos and sin are tables without a gradient, detach them")
-        if _wants_gradient(q) or _wants_gradient(k):
-            return _Rotation.apply(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse)
-    return _native.front().rope(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, inverse)
+        args = (grad_q, grad_k, *ctx.saved_tensors, *ctx.how, not ctx.inverse)
+        return (*(_native.front().rope(*args) or _Rotation.apply(*args)), *(None,) * 7)
 
 
 def apply_rope_axes(
@@ -63,7 +52,8 @@ def apply_rope_axes(
     take their pairs one section after another, or in turn with ``interleaved_axes``.  Computed in 32 bits
     and rounded once.  A pair whose position lies outside the tables stays as it is.  Returns new tensors,
     through which q and k get their gradients; cos and sin get none and may not require one."""
-    return _rotate(q, k, positions, cos, sin, sections, interleaved, interleaved_axes, False)
+    args = (q, k, positions, cos, sin, sections, interleaved, interleaved_axes, False)
+    return _native.front().rope(*args) or _Rotation.apply(*args)
 
 
 def apply_rope_axes_backward(
@@ -79,4 +69,5 @@ def apply_rope_axes_backward(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """The gradient of ``apply_rope_axes`` in q and k from that of its outputs: the rotation by the negative
     angles."""
-    return _rotate(grad_q, grad_k, positions, cos, sin, sections, interleaved, interleaved_axes, True)
+    args = (grad_q, grad_k, positions, cos, sin, sections, interleaved, interleaved_axes, True)
+    return _native.front().rope(*args) or _Rotation.apply(*args)
