@@ -753,6 +753,129 @@ typedef struct mak_rope_axes_desc {
  * gradient); columns past rot_dim are copied.  Tokens with a position outside the table keep that pair unchanged. */
 MAK_API int mak_rope_axes(const mak_rope_axes_desc* desc, void* stream);
 
+/* ---- attention over paged 16-bit caches ------------------------------------- */
+
+/*
+ * A layer of a paged cache: keys and values [num_blocks][block_size][num_heads][head_dim] of 16 bits (the LMCache and
+ * SGLang layouts), head_dim contiguous, addresses and strides multiples of 16 bytes.
+ */
+typedef struct mak_paged_cache_desc {
+  const void* key;
+  const void* value; /* NULL where a call reads keys alone */
+  int64_t key_stride_block, key_stride_token, key_stride_head;       /* elements */
+  int64_t value_stride_block, value_stride_token, value_stride_head; /* elements */
+  const int32_t* block_tables; /* [num_seqs][max_blocks], row stride table_stride */
+  const int32_t* context_lens; /* tokens of each sequence, those of this call included */
+  const int32_t* cu_seqlens;   /* [num_seqs + 1] rows of each sequence in the packed tensors; NULL: one row each */
+  int64_t table_stride;
+  int64_t num_blocks, num_seqs, max_blocks, num_rows;
+  int32_t num_heads, head_dim, block_size, dtype; /* MAK_DT_F16 or MAK_DT_BF16 */
+} mak_paged_cache_desc;
+
+typedef struct mak_paged_attn_desc {
+  mak_paged_cache_desc cache;
+  const void* q;          /* [num_rows][num_q_heads][head_dim] of the cache's type, head_dim contiguous */
+  void* out;              /* same shape and type */
+  float* lse;             /* [num_rows][num_q_heads] contiguous, or NULL */
+  const int32_t* parents; /* a tree of drafted tokens: [num_rows], or NULL */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_stride_row, q_stride_head, out_stride_row, out_stride_head; /* elements */
+  int32_t num_q_heads, window, sinks; /* window 0: none */
+  float scale;
+} mak_paged_attn_desc;
+
+/* Bytes of the workspace of mak_paged_attention: independent of the call's sizes.  It is zeroed once by the caller and
+ * then kept for calls that follow one another on one stream (the kernels leave its counters at zero). */
+MAK_API int64_t mak_paged_attention_workspace_bytes(void);
+
+/*
+ * out[r, h] = softmax(scale * q[r, h] . K^T) V over the tokens that row r sees.  Row r of sequence s is its
+ * i = (r - cu_seqlens[s])-th row of this call, at position context_lens[s] - (rows of s) + i.
+ * Without parents it sees the tokens t up to its own position, with window > 0 only those with t > position - window or
+ * t < sinks.  With parents it sees the tokens before the sequence's first row, itself, its parent parents[r] (the index
+ * of an earlier row of the sequence, anything else: none), that one's parent and so on.
+ * A row that sees nothing gives zeros and lse = -inf; what it does not see reaches it in no form, NaN among it.  Rows of
+ * no sequence are neither read nor written.  Block ids outside [0, num_blocks) are skipped like tokens outside the
+ * sequence, and so are tokens past max_blocks * block_size; a length beyond that shifts no position.
+ */
+MAK_API int mak_paged_attention(const mak_paged_attn_desc* desc, void* stream);
+
+typedef struct mak_paged_weights_desc {
+  mak_paged_cache_desc cache; /* value is not read */
+  const void* q;
+  const float* lse;    /* [num_rows][num_q_heads], row stride lse_stride_row */
+  float* sums;         /* [sum_rows][num_heads][max_tokens], the last axis contiguous */
+  const int32_t* rows; /* row of sums of each sequence (distinct; out of range: none), NULL: its own number */
+  int64_t q_stride_row, q_stride_head, lse_stride_row, sum_stride_row, sum_stride_head; /* elements */
+  int64_t sum_rows, max_tokens;
+  int32_t num_q_heads, window, sinks, accumulate;
+  float scale;
+  int32_t reserved;
+} mak_paged_weights_desc;
+
+/*
+ * sums[row of s, h, t] = or += (accumulate) the sum over the rows of sequence s that see token t (as above) and over the
+ * query heads of cache head h of exp(scale * q . k_t - lse).  Without accumulate the whole row of sums is written, zeros
+ * where no row sees; with it other places are left.  Tokens at or past max_tokens have no place.
+ */
+MAK_API int mak_paged_weights(const mak_paged_weights_desc* desc, void* stream);
+
+typedef struct mak_evict_desc {
+  const uint64_t* keys;   /* HOST arrays: addresses of the layers' planes [num_pages][block_size][num_heads][head_dim], */
+  const uint64_t* values; /* 16 bits an element, all of the strides below */
+  float* sums;            /* [num_layers][rows][num_heads][max_tokens], the last axis contiguous */
+  int64_t key_stride_block, key_stride_token, key_stride_head, value_stride_block, value_stride_token, value_stride_head;
+  int64_t sum_stride_layer, sum_stride_row, sum_stride_head; /* elements */
+  int64_t num_layers, max_tokens;
+  int32_t num_heads, head_dim, keep, sinks, recent, reserved;
+} mak_evict_desc;
+
+/*
+ * Rows rows[i] of more than `keep` tokens shrink to `keep`: each layer and head keeps the first `sinks`, the last
+ * `recent` and of the others those of the largest sums (the first of equal ones; NaN counts as -inf), in their order;
+ * sums move along and become 0 behind.  Pages past the kept tokens lose a reference, their entries become -1.  left[0]
+ * counts the rows left alone: a page that would be written is shared or a page is out of range, or the row has more
+ * tokens than its table or max_tokens hold.  A row named twice shrinks once.  `state` is scratch of n int32.
+ */
+MAK_API int mak_pages_evict(const mak_pages_desc* pages, const mak_evict_desc* evict, const int32_t* rows, int64_t n, int32_t* left,
+                            int32_t* state, void* stream);
+
+/* ---- norms of queries and keys with the position rotation ------------------- */
+
+typedef struct mak_qk_norm_rope_desc {
+  const void* q; /* [tokens][q_heads][head_dim], head_dim contiguous, rows 16-byte aligned */
+  const void* k; /* [tokens][k_heads][head_dim] */
+  void* q_out;   /* the result, or the gradient of q */
+  void* k_out;
+  const void* grad_q; /* gradients of the results; NULL: forward */
+  const void* grad_k;
+  const void* q_weight; /* [head_dim], weight_dtype */
+  const void* k_weight;
+  void* grad_q_weight; /* [head_dim], weight_dtype */
+  void* grad_k_weight;
+  const void* positions; /* [tokens], pos_dtype, contiguous */
+  const float* cos;      /* [max_positions][rot_dim / 2], row stride cos_stride */
+  const float* sin;
+  float* partial; /* backward: scratch of mak_qk_norm_rope_partial_floats(head_dim) */
+  int64_t tokens, max_positions;
+  int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head; /* elements */
+  int64_t qo_stride_token, qo_stride_head, ko_stride_token, ko_stride_head;
+  int64_t gq_stride_token, gq_stride_head, gk_stride_token, gk_stride_head;
+  int64_t cos_stride, sin_stride;
+  int32_t q_heads, k_heads, head_dim, rot_dim;
+  int32_t dtype, weight_dtype, pos_dtype, interleaved;
+  float eps;
+  int32_t reserved;
+} mak_qk_norm_rope_desc;
+
+MAK_API int64_t mak_qk_norm_rope_partial_floats(int32_t head_dim);
+
+/* Each head of q and k: x / sqrt(mean(x^2) + eps) * weight, then pair j of its first rot_dim columns, (j, j + rot_dim / 2)
+ * or (2 j, 2 j + 1) interleaved, turned by the angle of row positions[t], column j (a position outside the tables turns
+ * nothing).  With gradients: those of q, k and the weights. */
+MAK_API int mak_qk_norm_rope(const mak_qk_norm_rope_desc* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

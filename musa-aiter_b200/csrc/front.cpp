@@ -1,5 +1,5 @@
 // Python entry of the calls whose kernels are shorter than a Python argument check: the block-scaled
-// cache, page and rotary operators.  Each function takes its arguments by position (the Python modules
+// cache, paged attention, page, norm and rotary operators.  Each function takes its arguments by position (the Python modules
 // under ops/ name and document them), checks them, fills the C descriptor and calls the library's entry
 // point on the current stream.  Nothing about a tensor is remembered between calls.
 #include <Python.h>
@@ -37,6 +37,12 @@ struct Library {
   decltype(&mak_pages_compact) compact = nullptr;
   decltype(&mak_pages_copy) copy = nullptr;
   decltype(&mak_rope_axes) rope = nullptr;
+  decltype(&mak_paged_attention_workspace_bytes) paged_workspace_bytes = nullptr;
+  decltype(&mak_paged_attention) paged_attention = nullptr;
+  decltype(&mak_paged_weights) paged_weights = nullptr;
+  decltype(&mak_pages_evict) evict = nullptr;
+  decltype(&mak_qk_norm_rope_partial_floats) norm_partial = nullptr;
+  decltype(&mak_qk_norm_rope) norm_rope = nullptr;
 } lib;
 PyObject* emit = nullptr;  // dispatch.emit_native
 
@@ -207,19 +213,20 @@ mak_block_cache_desc cache_desc(const char* name, Args a, int64_t rows, int64_t 
 // Attention workspaces, one per device and stream: the kernels leave their counters at zero, so calls that
 // follow one another on a stream share it.  The per-thread default stream is another one for each thread, under one
 // handle.  Kept until the process ends.
-at::Tensor workspace(const at::Device& device, cudaStream_t stream) {
-  static std::mutex mutex;
+struct Workspaces {
+  std::mutex mutex;
+  std::map<std::tuple<int, cudaStream_t, const void*>, at::Tensor> kept;
+};
+at::Tensor workspace(Workspaces& all, int64_t bytes, const at::Device& device, cudaStream_t stream) {
   static thread_local char thread;
-  static auto* kept = new std::map<std::tuple<int, cudaStream_t, const void*>, at::Tensor>();
-  const int64_t bytes = lib.workspace_bytes();
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
     // a graph may be replayed on any stream: it gets a workspace of its own
     at::Tensor ws = empty({bytes}, at::kByte, device);
     ws.narrow(0, 0, std::min<int64_t>(bytes, 1 << 16)).zero_();
     return ws;
   }
-  std::lock_guard<std::mutex> lock(mutex);
-  at::Tensor& ws = (*kept)[{device.index(), stream, stream == cudaStreamPerThread ? &thread : nullptr}];
+  std::lock_guard<std::mutex> lock(all.mutex);
+  at::Tensor& ws = all.kept[{device.index(), stream, stream == cudaStreamPerThread ? &thread : nullptr}];
   if (!ws.defined()) ws = at::zeros({bytes}, at::TensorOptions().dtype(at::kByte).device(device));
   return ws;
 }
@@ -257,7 +264,8 @@ PyObject* py_attend(PyObject*, Args a, Py_ssize_t n) {
     const at::Tensor out = given ? THPVariable_Unpack(a[12]) : empty({rows, hq, hd}, kind, q0.device());
     const at::Tensor lse = want_lse ? empty({rows, hq}, at::kFloat, q0.device()) : at::Tensor();
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev.index)).stream();
-    const at::Tensor ws = workspace(q0.device(), stream);
+    static auto* spaces = new Workspaces();
+    const at::Tensor ws = workspace(*spaces, lib.workspace_bytes(), q0.device(), stream);
     d.q = q.data_ptr(), d.out = out.data_ptr(), d.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
     d.workspace = ws.data_ptr(), d.workspace_bytes = ws.numel();
     d.q_stride_row = q.stride(0), d.q_stride_head = q.stride(1), d.out_stride_row = out.stride(0), d.out_stride_head = out.stride(1);
@@ -587,6 +595,362 @@ PyObject* py_rope(PyObject*, Args a, Py_ssize_t n) {
   });
 }
 
+// ---- paged 16-bit caches ----------------------------------------------------------------------------------
+
+// Arguments from `a`: key_cache, value_cache (where `values`), block_tables, context_lens; `cu`: cu_seqlens.
+// The tensors go to `used`: whether they are on one device is asked after all shapes.
+using Used = std::vector<const at::Tensor*>;
+mak_paged_cache_desc paged_desc(const char* name, Args a, bool values, PyObject* cu_seqlens, const at::Tensor& q, Used& used) {
+  const at::Tensor& kc = tensor(name, "key_cache", a[0]);
+  const at::Tensor& vc = values ? tensor(name, "value_cache", a[1]) : kc;
+  a += values ? 2 : 1;
+  const at::Tensor &table = tensor(name, "block_tables", a[0]), &ctx = tensor(name, "context_lens", a[1]);
+  if (q.dim() != 3) refuse(name, "q must be [rows, num_q_heads, head_dim]");
+  const at::ScalarType kind = q.scalar_type();
+  if (kind != at::kHalf && kind != at::kBFloat16) refuse(name, "q must be float16 or bfloat16, got ", toString(kind));
+  if (kc.dim() != 4 || kc.sizes() != vc.sizes())
+    refuse(name, values ? "key_cache and value_cache must both be" : "key_cache must be", " [num_blocks, block_size, num_heads, head_dim]");
+  if (kc.scalar_type() != kind || vc.scalar_type() != kind) refuse(name, "q and the caches must have one type, got ", toString(kind), " and ", toString(kc.scalar_type()));
+  const int64_t rows = q.size(0), hq = q.size(1), nb = kc.size(0), bs = kc.size(1), nh = kc.size(2), hd = kc.size(3);
+  if (hd != 64 && hd != 128) refuse(name, "head_dim must be one of (64, 128), got ", hd);
+  if (bs != 16 && bs != 32 && bs != 64 && bs != 128) refuse(name, "block_size must be one of (16, 32, 64, 128), got ", bs);
+  if (q.size(2) != hd) refuse(name, "rows have head_dim ", q.size(2), ", the cache ", hd);
+  if (nh < 1) refuse(name, "a cache needs heads");
+  if (hq < 1 || hq % nh) refuse(name, hq, " query heads do not divide over ", nh, " cache heads");
+  for (const at::Tensor* c : {&kc, &vc}) {
+    if (c->stride(3) != 1) refuse(name, "the head_dim axis of the caches must be contiguous");
+    if (nb == 0) continue;
+    for (int i = 0; i < 3; ++i)
+      if (c->size(i) > 1 && c->stride(i) % 8) refuse(name, "block, token and head strides of the caches must be multiples of 8 elements");
+    if (reinterpret_cast<uintptr_t>(c->data_ptr()) % 16) refuse(name, "caches must begin on 16 bytes");
+  }
+  if (table.dim() != 2 || ctx.dim() != 1 || table.size(0) != ctx.size(0))
+    refuse(name, "block_tables must be [num_seqs, max_blocks] and context_lens [num_seqs]");
+  if (table.scalar_type() != at::kInt || ctx.scalar_type() != at::kInt) refuse(name, "block_tables and context_lens must be int32");
+  const int64_t seqs = table.size(0), width = table.size(1);
+  if (width > 1 && table.stride(1) != 1) refuse(name, "a block table's row must be contiguous");
+  if (seqs > 1 && ctx.stride(0) != 1) refuse(name, "context_lens must be contiguous");
+  mak_paged_cache_desc d = {};
+  if (cu_seqlens == Py_None) {
+    if (rows != seqs) refuse(name, "without cu_seqlens every sequence has one row: ", rows, " rows for ", seqs, " sequences");
+  } else {
+    const at::Tensor& cu = tensor(name, "cu_seqlens", cu_seqlens);
+    if (cu.dim() != 1 || cu.size(0) != seqs + 1 || cu.scalar_type() != at::kInt) refuse(name, "cu_seqlens must be int32 [num_seqs + 1]");
+    if (!cu.is_contiguous()) refuse(name, "cu_seqlens must be contiguous");
+    used.push_back(&cu);
+    d.cu_seqlens = static_cast<const int32_t*>(cu.data_ptr());
+  }
+  for (const at::Tensor* t : {&kc, &vc, &table, &ctx, &q}) used.push_back(t);
+  d.key = kc.data_ptr(), d.value = values ? vc.data_ptr() : nullptr;
+  // the stride of an axis with one entry reaches nothing: a multiple of 8 in its place
+  auto step = [&](const at::Tensor& c, int axis) { return c.size(axis) > 1 ? c.stride(axis) : nh * hd * bs; };
+  d.key_stride_block = step(kc, 0), d.key_stride_token = step(kc, 1), d.key_stride_head = step(kc, 2);
+  d.value_stride_block = step(vc, 0), d.value_stride_token = step(vc, 1), d.value_stride_head = step(vc, 2);
+  d.block_tables = static_cast<const int32_t*>(table.data_ptr());
+  d.context_lens = static_cast<const int32_t*>(ctx.data_ptr());
+  d.table_stride = table.stride(0);
+  d.num_blocks = nb, d.num_seqs = seqs, d.max_blocks = width, d.num_rows = rows;
+  d.num_heads = static_cast<int32_t>(nh), d.head_dim = static_cast<int32_t>(hd), d.block_size = static_cast<int32_t>(bs);
+  d.dtype = float_code(kind);
+  return d;
+}
+int32_t count_of(const char* name, const char* what, PyObject* o) {
+  const int64_t v = integer(name, what, o);
+  if (v < 0) refuse(name, what, " must not be negative, got ", v);
+  return static_cast<int32_t>(std::min<int64_t>(v, 0x7fffffff));
+}
+float scale_of(PyObject* o, int64_t head_dim) {
+  if (o == Py_None) return static_cast<float>(1.0 / std::sqrt(static_cast<double>(head_dim)));
+  const double scale = PyFloat_AsDouble(o);
+  if (scale == -1.0 && PyErr_Occurred()) throw python_error();
+  return static_cast<float>(scale);
+}
+
+// q, key_cache, value_cache, block_tables, context_lens, cu_seqlens, parents (None: a window), window, sinks, scale,
+// return_lse, out
+PyObject* py_paged(PyObject*, Args a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const bool tree = n == 12 && a[6] != Py_None;
+    const char* name = tree ? "paged_attention_tree" : "paged_attention_window";
+    count(name, n, 12);
+    const at::Tensor& q0 = tensor(name, "q", a[0]);
+    Device dev{name};
+    mak_paged_attn_desc d = {};
+    d.window = count_of(name, "window", a[7]), d.sinks = count_of(name, "sinks", a[8]);
+    if (d.sinks > 0 && d.window == 0) refuse(name, "sinks need a window");
+    const bool want_lse = truth(a[10]), given = a[11] != Py_None;
+    Used used;
+    d.cache = paged_desc(name, a + 1, true, a[5], q0, used);
+    const int64_t rows = q0.size(0), hq = q0.size(1), hd = q0.size(2);
+    if (tree) {
+      const at::Tensor& up = tensor(name, "parents", a[6]);
+      if (up.dim() != 1 || up.size(0) != rows || up.scalar_type() != at::kInt) refuse(name, "parents must be int32 [rows]");
+      if (!up.is_contiguous()) refuse(name, "parents must be contiguous");
+      used.push_back(&up);
+      d.parents = static_cast<const int32_t*>(up.data_ptr());
+    }
+    if (given) {
+      const at::Tensor& o = tensor(name, "out", a[11]);
+      if (o.sizes() != q0.sizes() || o.scalar_type() != q0.scalar_type() || (o.numel() && o.stride(2) != 1))
+        refuse(name, "out must have q's shape and dtype and contiguous rows");
+      used.push_back(&o);
+    }
+    d.scale = scale_of(a[9], hd);
+    for (const at::Tensor* t : used) dev.add(*t);
+    dev.need_library();
+    const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
+    const at::Tensor q = aligned_rows(q0);
+    const at::Tensor out = given ? THPVariable_Unpack(a[11]) : empty({rows, hq, hd}, q0.scalar_type(), q0.device());
+    const at::Tensor lse = want_lse ? empty({rows, hq}, at::kFloat, q0.device()) : at::Tensor();
+    const cudaStream_t stream = stream_of(dev);
+    static auto* spaces = new Workspaces();
+    const at::Tensor ws = workspace(*spaces, lib.paged_workspace_bytes(), q0.device(), stream);
+    d.q = q.data_ptr(), d.out = out.data_ptr(), d.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
+    d.workspace = ws.data_ptr(), d.workspace_bytes = ws.numel();
+    d.q_stride_row = q.stride(0), d.q_stride_head = q.stride(1), d.out_stride_row = out.stride(0), d.out_stride_head = out.stride(1);
+    d.num_q_heads = static_cast<int32_t>(hq);
+    check(lib.paged_attention(&d, stream), name);
+    trace(name, a[0], "sm100a paged cache attention");
+    return want_lse ? wrap(out, lse) : wrap(out);
+  });
+}
+
+// q, key_cache, block_tables, context_lens, lse, sums, cu_seqlens, rows, window, sinks, scale, accumulate
+PyObject* py_weights(PyObject*, Args a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const char* name = "paged_attention_weights";
+    count(name, n, 12);
+    const at::Tensor &q0 = tensor(name, "q", a[0]), &lse = tensor(name, "lse", a[4]), &sums = tensor(name, "sums", a[5]);
+    Device dev{name};
+    mak_paged_weights_desc d = {};
+    d.window = count_of(name, "window", a[8]), d.sinks = count_of(name, "sinks", a[9]);
+    if (d.sinks > 0 && d.window == 0) refuse(name, "sinks need a window");
+    d.accumulate = truth(a[11]);
+    Used used;
+    d.cache = paged_desc(name, a + 1, false, a[6], q0, used);
+    const int64_t rows = q0.size(0), hq = q0.size(1), seqs = d.cache.num_seqs;
+    if (lse.dim() != 2 || lse.size(0) != rows || lse.size(1) != hq || lse.scalar_type() != at::kFloat)
+      refuse(name, "lse must be float32 [rows, num_q_heads]");
+    if (hq > 1 && lse.stride(1) != 1) refuse(name, "a row of lse must be contiguous");
+    if (sums.dim() != 3 || sums.size(1) != d.cache.num_heads || sums.scalar_type() != at::kFloat)
+      refuse(name, "sums must be float32 [rows of sums, num_heads, max_tokens]");
+    if (sums.size(2) > 1 && sums.stride(2) != 1) refuse(name, "the last axis of sums must be contiguous");
+    if (a[7] == Py_None) {
+      if (sums.size(0) != seqs) refuse(name, "without rows every sequence has its row of sums: ", sums.size(0), " rows for ", seqs, " sequences");
+    } else {
+      const at::Tensor& r = tensor(name, "rows", a[7]);
+      if (r.dim() != 1 || r.size(0) != seqs || r.scalar_type() != at::kInt) refuse(name, "rows must be int32 [num_seqs]");
+      if (!r.is_contiguous()) refuse(name, "rows must be contiguous");
+      used.push_back(&r);
+      d.rows = static_cast<const int32_t*>(r.data_ptr());
+    }
+    used.push_back(&lse);
+    used.push_back(&sums);
+    d.scale = scale_of(a[10], q0.size(2));
+    for (const at::Tensor* t : used) dev.add(*t);
+    dev.need_library();
+    const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
+    const at::Tensor q = aligned_rows(q0);
+    d.q = q.data_ptr(), d.lse = static_cast<const float*>(lse.data_ptr()), d.sums = static_cast<float*>(sums.data_ptr());
+    d.q_stride_row = q.stride(0), d.q_stride_head = q.stride(1), d.lse_stride_row = lse.stride(0);
+    d.sum_stride_row = sums.stride(0), d.sum_stride_head = sums.stride(1), d.sum_rows = sums.size(0), d.max_tokens = sums.size(2);
+    d.num_q_heads = static_cast<int32_t>(hq);
+    check(lib.paged_weights(&d, stream_of(dev)), name);
+    trace(name, a[0], "sm100a paged cache attention weights");
+    Py_RETURN_NONE;
+  });
+}
+
+// block_tables, context_lens, rows, ref_counts, key_caches, value_caches, sums, keep, sinks, recent
+PyObject* py_evict(PyObject*, Args a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const char* name = "kv_pages_evict";
+    count(name, n, 10);
+    const at::Tensor &table = tensor(name, "block_tables", a[0]), &lens = tensor(name, "context_lens", a[1]);
+    const at::Tensor &rows = tensor(name, "rows", a[2]), &refs = tensor(name, "ref_counts", a[3]), &sums = tensor(name, "sums", a[6]);
+    Device dev{name};
+    mak_evict_desc e = {};
+    e.keep = count_of(name, "keep", a[7]), e.sinks = count_of(name, "sinks", a[8]), e.recent = count_of(name, "recent", a[9]);
+    if (e.keep < 1 || static_cast<int64_t>(e.sinks) + e.recent > e.keep) refuse(name, "keep must be at least 1 and sinks + recent");
+    struct Held {
+      std::vector<uint64_t> at;
+      std::vector<const at::Tensor*> tensors;
+      PyObject* list = nullptr;
+      ~Held() { Py_XDECREF(list); }
+    } held[2];
+    const at::Tensor* first = nullptr;
+    for (int which = 0; which < 2; ++which) {
+      const char* what = which ? "value_caches" : "key_caches";
+      Held& h = held[which];
+      h.list = PySequence_Fast(a[4 + which], "key_caches and value_caches must be sequences of tensors");
+      if (h.list == nullptr) throw python_error();
+      for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(h.list); ++i) {
+        const at::Tensor& t = tensor(name, what, PySequence_Fast_GET_ITEM(h.list, i));
+        if (t.dim() != 4) refuse(name, what, " must be [num_blocks, block_size, num_heads, head_dim]");
+        if (first == nullptr) first = &t;
+        if (t.sizes() != first->sizes() || t.scalar_type() != first->scalar_type()) refuse(name, "all caches must have one shape and type");
+        if (!h.tensors.empty() && t.strides() != h.tensors[0]->strides()) refuse(name, what, " must have one layout");
+        if (t.stride(3) != 1) refuse(name, "the head_dim axis of the caches must be contiguous");
+        for (int x = 0; x < 3; ++x)
+          if (t.size(x) > 1 && t.stride(x) % 8) refuse(name, "block, token and head strides of the caches must be multiples of 8 elements");
+        if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) refuse(name, "caches must begin on 16 bytes");
+        h.at.push_back(reinterpret_cast<uintptr_t>(t.data_ptr()));
+        h.tensors.push_back(&t);
+      }
+    }
+    const int64_t layers = static_cast<int64_t>(held[0].at.size());
+    if (layers != static_cast<int64_t>(held[1].at.size())) refuse(name, "key_caches and value_caches must have the same length");
+    if (layers == 0) refuse(name, "key_caches must have a layer");
+    if (first->scalar_type() != at::kHalf && first->scalar_type() != at::kBFloat16) refuse(name, "caches must be float16 or bfloat16");
+    const int64_t nb = first->size(0), bs = first->size(1), nh = first->size(2), hd = first->size(3);
+    if (hd != 64 && hd != 128 && hd != 256) refuse(name, "head_dim must be one of (64, 128, 256), got ", hd);
+    if (nh < 1) refuse(name, "a cache needs heads");
+    const mak_pages_desc d = pool(name, table, &lens, refs, bs, dev);
+    if (refs.size(0) != nb) refuse(name, "ref_counts must have one entry per page of the caches");
+    const int32_t* r = index_of(name, "rows", rows, 1, dev);
+    if (sums.dim() != 4 || sums.size(0) != layers || sums.size(1) != table.size(0) || sums.size(2) != nh || sums.scalar_type() != at::kFloat)
+      refuse(name, "sums must be float32 [layers, rows of block_tables, num_heads, max_tokens]");
+    if (sums.size(3) > 1 && sums.stride(3) != 1) refuse(name, "the last axis of sums must be contiguous");
+    for (const at::Tensor* t : {&table, &lens, &rows, &refs, &sums}) dev.add(*t);
+    for (const Held& h : held)
+      for (const at::Tensor* t : h.tensors) dev.add(*t);
+    dev.need_library();
+    const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
+    auto step = [&](const at::Tensor& c, int axis) { return c.size(axis) > 1 ? c.stride(axis) : nh * hd * bs; };
+    const at::Tensor &kc = *held[0].tensors[0], &vc = *held[1].tensors[0];
+    e.keys = held[0].at.data(), e.values = held[1].at.data(), e.sums = static_cast<float*>(sums.data_ptr());
+    e.key_stride_block = step(kc, 0), e.key_stride_token = step(kc, 1), e.key_stride_head = step(kc, 2);
+    e.value_stride_block = step(vc, 0), e.value_stride_token = step(vc, 1), e.value_stride_head = step(vc, 2);
+    e.sum_stride_layer = sums.stride(0), e.sum_stride_row = sums.stride(1), e.sum_stride_head = sums.stride(2);
+    e.num_layers = layers, e.max_tokens = sums.size(3), e.num_heads = static_cast<int32_t>(nh), e.head_dim = static_cast<int32_t>(hd);
+    const int64_t want = rows.size(0);
+    const at::Tensor room = empty({want + 1}, at::kInt, table.device());  // the answer and the scratch in one allocation
+    int32_t* at = static_cast<int32_t*>(room.data_ptr());
+    check(lib.evict(&d, &e, r, want, at, at + 1, stream_of(dev)), name);
+    trace(name, a[0], "sm100a page eviction");
+    return wrap(room.narrow(0, 0, 1));
+  });
+}
+
+// ---- norms of q and k with the position rotation ----------------------------------------------------------
+
+struct NormArgs {
+  at::Tensor q, k, wq, wk, pos, cos, sin;
+};
+// Arguments from `a`: q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved
+mak_qk_norm_rope_desc norm_desc(const char* name, Args a, NormArgs& x) {
+  const at::Tensor &q = tensor(name, "q", a[0]), &k = tensor(name, "k", a[1]);
+  const at::Tensor &wq = tensor(name, "q_weight", a[2]), &wk = tensor(name, "k_weight", a[3]);
+  x.pos = tensor(name, "positions", a[4]), x.cos = tensor(name, "cos", a[5]), x.sin = tensor(name, "sin", a[6]);
+  if (q.dim() != 3 || k.dim() != 3 || q.size(0) != k.size(0) || q.size(2) != k.size(2))
+    refuse(name, "q and k must be [tokens, heads, head_dim] with the same tokens and head_dim");
+  const at::ScalarType kind = q.scalar_type();
+  if ((kind != at::kHalf && kind != at::kBFloat16) || k.scalar_type() != kind) refuse(name, "q and k must both be float16 or both bfloat16");
+  const int64_t tokens = q.size(0), hd = q.size(2);
+  if (hd < 16 || hd > 256 || hd % 16) refuse(name, "head_dim must be a multiple of 16 up to 256, got ", hd);
+  for (const at::Tensor* w : {&wq, &wk})
+    if (w->dim() != 1 || w->size(0) != hd || (w->scalar_type() != at::kFloat && w->scalar_type() != kind) || w->scalar_type() != wq.scalar_type())
+      refuse(name, "weights must both be [head_dim] in float32 or in q's type");
+  if (x.pos.dim() != 1 || x.pos.size(0) != tokens || (x.pos.scalar_type() != at::kInt && x.pos.scalar_type() != at::kLong))
+    refuse(name, "positions must be int32 or int64 [tokens]");
+  if (x.cos.dim() != 2 || x.cos.sizes() != x.sin.sizes() || x.cos.scalar_type() != at::kFloat || x.sin.scalar_type() != at::kFloat)
+    refuse(name, "cos and sin must both be float32 [max_positions, pairs]");
+  const int64_t pairs = x.cos.size(1);
+  if (pairs % 8 || 2 * pairs > hd) refuse(name, "the tables must have a multiple of 8 pairs, at most head_dim / 2, got ", pairs);
+  const double eps = PyFloat_AsDouble(a[7]);
+  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  if (!(eps >= 0.0)) refuse(name, "eps must not be negative");
+  mak_qk_norm_rope_desc d = {};
+  d.interleaved = truth(a[8]), d.eps = static_cast<float>(eps);
+  x.q = q, x.k = k, x.wq = wq, x.wk = wk;
+  d.tokens = tokens, d.max_positions = x.cos.size(0);
+  d.q_heads = static_cast<int32_t>(q.size(1)), d.k_heads = static_cast<int32_t>(k.size(1)), d.head_dim = static_cast<int32_t>(hd);
+  d.rot_dim = static_cast<int32_t>(2 * pairs), d.dtype = float_code(kind), d.weight_dtype = float_code(wq.scalar_type());
+  d.pos_dtype = x.pos.scalar_type() == at::kInt ? MAK_DT_I32 : MAK_DT_I64;
+  return d;
+}
+void norm_on(Device& dev, const NormArgs& x) {
+  for (const at::Tensor* t : {&x.q, &x.k, &x.wq, &x.wk, &x.pos, &x.cos, &x.sin}) dev.add(*t);
+  dev.need_library();
+}
+// Copies where a layout needs one, on the device that is current by now.
+void norm_inputs(mak_qk_norm_rope_desc& d, NormArgs& x) {
+  x.q = aligned_rows(x.q), x.k = aligned_rows(x.k);
+  x.wq = x.wq.contiguous(), x.wk = x.wk.contiguous(), x.pos = x.pos.contiguous();
+  if (x.cos.stride(1) != 1) x.cos = x.cos.contiguous();
+  if (x.sin.stride(1) != 1) x.sin = x.sin.contiguous();
+  d.q = x.q.data_ptr(), d.k = x.k.data_ptr(), d.q_weight = x.wq.data_ptr(), d.k_weight = x.wk.data_ptr();
+  d.positions = x.pos.data_ptr(), d.cos = static_cast<const float*>(x.cos.data_ptr()), d.sin = static_cast<const float*>(x.sin.data_ptr());
+  d.q_stride_token = x.q.stride(0), d.q_stride_head = x.q.stride(1), d.k_stride_token = x.k.stride(0), d.k_stride_head = x.k.stride(1);
+  d.cos_stride = x.cos.stride(0), d.sin_stride = x.sin.stride(0);
+  d.qo_stride_token = static_cast<int64_t>(d.q_heads) * d.head_dim, d.ko_stride_token = static_cast<int64_t>(d.k_heads) * d.head_dim;
+  d.qo_stride_head = d.ko_stride_head = d.head_dim;
+}
+
+// the nine of norm_desc; None where q, k or a weight wants a gradient
+PyObject* py_norm(PyObject*, Args a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const char* name = "apply_qk_norm_rope";
+    count(name, n, 9);
+    Device dev{name};
+    NormArgs x;
+    if (c10::GradMode::is_enabled()) {
+      for (int i : {5, 6})
+        if (tensor(name, "cos and sin", a[i]).requires_grad()) refuse(name, "cos and sin are tables without a gradient, detach them");
+      for (int i = 0; i < 4; ++i)
+        if (tensor(name, "q, k and the weights", a[i]).requires_grad()) Py_RETURN_NONE;  // the autograd function calls again, gradients off
+    }
+    mak_qk_norm_rope_desc d = norm_desc(name, a, x);
+    norm_on(dev, x);
+    const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
+    norm_inputs(d, x);
+    const at::ScalarType kind = x.q.scalar_type();
+    const at::Tensor q_out = empty(x.q.sizes(), kind, x.q.device()), k_out = empty(x.k.sizes(), kind, x.q.device());
+    d.q_out = q_out.data_ptr(), d.k_out = k_out.data_ptr();
+    check(lib.norm_rope(&d, stream_of(dev)), name);
+    trace(name, a[0], "sm100a norms and rotary positions");
+    return wrap(q_out, k_out);
+  });
+}
+
+// grad_q, grad_k, the nine of norm_desc
+PyObject* py_norm_back(PyObject*, Args a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    const char* name = "apply_qk_norm_rope_backward";
+    count(name, n, 11);
+    const at::Tensor &gq0 = tensor(name, "grad_q", a[0]), &gk0 = tensor(name, "grad_k", a[1]);
+    Device dev{name};
+    NormArgs x;
+    mak_qk_norm_rope_desc d = norm_desc(name, a + 2, x);
+    if (gq0.sizes() != x.q.sizes() || gk0.sizes() != x.k.sizes() || gq0.scalar_type() != x.q.scalar_type() || gk0.scalar_type() != x.q.scalar_type())
+      refuse(name, "grad_q and grad_k must have the shapes and type of q and k");
+    dev.add(gq0);
+    dev.add(gk0);
+    norm_on(dev, x);
+    const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
+    norm_inputs(d, x);
+    const at::Tensor gq = aligned_rows(gq0), gk = aligned_rows(gk0);
+    const at::ScalarType kind = x.q.scalar_type();
+    const at::Tensor dq = empty(x.q.sizes(), kind, x.q.device()), dk = empty(x.k.sizes(), kind, x.q.device());
+    const at::Tensor dwq = empty(x.wq.sizes(), x.wq.scalar_type(), x.q.device()), dwk = empty(x.wk.sizes(), x.wk.scalar_type(), x.q.device());
+    const at::Tensor partial = empty({lib.norm_partial(d.head_dim)}, at::kFloat, x.q.device());
+    // a tensor without elements has no address, but the call is still a backward one
+    static float none[4];
+    auto address = [](const at::Tensor& t) { return t.numel() ? t.data_ptr() : static_cast<void*>(none); };
+    d.grad_q = address(gq), d.grad_k = address(gk);
+    d.gq_stride_token = gq.stride(0), d.gq_stride_head = gq.stride(1), d.gk_stride_token = gk.stride(0), d.gk_stride_head = gk.stride(1);
+    d.q_out = dq.data_ptr(), d.k_out = dk.data_ptr(), d.grad_q_weight = dwq.data_ptr(), d.grad_k_weight = dwk.data_ptr();
+    d.partial = static_cast<float*>(partial.data_ptr());
+    check(lib.norm_rope(&d, stream_of(dev)), name);
+    trace(name, a[0], "sm100a gradient of norms and rotary positions");
+    PyObject* all = PyTuple_New(4);
+    if (all == nullptr) throw python_error();
+    const at::Tensor* got[4] = {&dq, &dk, &dwq, &dwk};
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(all, i, THPVariable_Wrap(*got[i]));
+    return all;
+  });
+}
+
 // ---- the module -----------------------------------------------------------------------------------------------
 
 // bind(addresses: dict of name -> int, emit): the library's entry points and the trace function
@@ -610,6 +974,12 @@ PyObject* py_bind(PyObject*, Args a, Py_ssize_t n) {
     MAK_BIND(compact, mak_pages_compact);
     MAK_BIND(copy, mak_pages_copy);
     MAK_BIND(rope, mak_rope_axes);
+    MAK_BIND(paged_workspace_bytes, mak_paged_attention_workspace_bytes);
+    MAK_BIND(paged_attention, mak_paged_attention);
+    MAK_BIND(paged_weights, mak_paged_weights);
+    MAK_BIND(evict, mak_pages_evict);
+    MAK_BIND(norm_partial, mak_qk_norm_rope_partial_floats);
+    MAK_BIND(norm_rope, mak_qk_norm_rope);
     MAK_BIND(attention, mak_block_attention);
 #undef MAK_BIND
     Py_INCREF(a[1]);
@@ -623,6 +993,8 @@ PyObject* py_bind(PyObject*, Args a, Py_ssize_t n) {
 PyMethodDef methods[] = {{"bind", MAK_FAST(py_bind)},       {"attend", MAK_FAST(py_attend)}, {"append", MAK_FAST(py_append)},
                          {"fork", MAK_FAST(py_fork)},       {"grow", MAK_FAST(py_grow)},     {"free", MAK_FAST(py_free)},
                          {"compact", MAK_FAST(py_compact)}, {"copy", MAK_FAST(py_copy)},     {"rope", MAK_FAST(py_rope)},
+                         {"paged", MAK_FAST(py_paged)},     {"weights", MAK_FAST(py_weights)}, {"evict", MAK_FAST(py_evict)},
+                         {"norm", MAK_FAST(py_norm)},       {"norm_back", MAK_FAST(py_norm_back)},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mak_front", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,644 @@
+// Attention over a paged 16-bit cache for few rows per sequence (single tokens, small trees), and the entry points.
+//
+// o = softmax(scale q K^T) V over the tokens that a row sees: a window and the first tokens, or the tokens before a tree
+// of drafted ones and those that a row continues.  One pass over K and V with the running maximum m and sum l of a row;
+// sums, statistics and accumulators are 32-bit.  A weight multiplies V as the sum of two 16-bit numbers, so it is good to
+// 2^-16 (bfloat16) or 2^-22 (float16; lifted by 2^15, so that weights down to 2^-39 of the largest count).
+//
+// Bound by reading K and V.  A unit is 16 rows (tokens of a sequence times the query heads of a cache head) of one
+// sequence and head, its work 16-token steps.  All units laid end to end are cut into equal runs, one per warp, whatever
+// the lengths; a warp copies its steps into a ring of its own (a page's row of 16 bytes per lane), so no warp waits for
+// another until its run ends.  A unit cut by that leaves partial sums: the block joins those of its warps, the last block
+// to arrive joins those of the blocks, both in order of position, so results do not depend on timing.
+#include "paged_attn.cuh"
+
+namespace mak {
+namespace {
+
+constexpr int kRows = 16;     // rows of a unit
+constexpr int kStep = 16;     // tokens of a step: one page holds them
+constexpr int kWarps = 8;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kMaxGrid = 148;
+constexpr int kUnitCost = 2;  // a unit's beginning and end, in steps
+constexpr int kMinRun = 4;    // steps that are worth another warp
+constexpr int kQueue = 8;     // units between a warp's copies and its products, at most
+
+struct Unit {
+  PagedSeq v;
+  Span s;
+  int seq, head, tile, live;
+  int ta, tb, len;  // this warp has steps [ta, tb) of len
+  int pad;
+  int64_t wt;       // where the unit's steps begin in all work
+};
+
+// What is left of a unit that a run's end cut.
+struct Piece {
+  int64_t wt;  // -1: none
+  const float* at;
+  int seq, head, tile, live, len, first;
+};
+
+template <int HD>
+struct Smem {
+  static constexpr int kStages = HD == 64 ? 6 : 3;
+  static constexpr int kTileBytes = kStep * HD * 2;
+  alignas(128) uint8_t ring[kWarps][kStages][2 * kTileBytes];
+  Unit queue[kWarps][kQueue];
+  Piece pieces[2 * kWarps];
+  int64_t before[kThreads + 1];  // work of the sequences of the threads before
+  int64_t sums[kWarps];
+  int last;
+};
+
+__device__ __forceinline__ int tiles_of(const PagedParams& p, const PagedSeq& v) {
+  return static_cast<int>((static_cast<int64_t>(v.rows) * p.group + kRows - 1) / kRows);
+}
+__device__ __forceinline__ Span span_of_tile(const PagedParams& p, const PagedSeq& v, int tile, int* live) {
+  const int64_t row0 = static_cast<int64_t>(tile) * kRows, left = static_cast<int64_t>(v.rows) * p.group - row0;
+  *live = left < kRows ? static_cast<int>(left) : kRows;
+  return span_of<kStep>(p, v, static_cast<int>(row0 / p.group), static_cast<int>((row0 + *live - 1) / p.group));
+}
+__device__ __forceinline__ int64_t work_of(const PagedParams& p, const PagedSeq& v) {
+  int64_t sum = 0;
+  const int tiles = tiles_of(p, v);
+  for (int i = 0; i < tiles; ++i) {
+    int live;
+    sum += kUnitCost + max(span_of_tile(p, v, i, &live).tiles, 1);
+  }
+  return sum * p.nh;
+}
+
+// A run: units one after another, the tiles of a (sequence, head) next to one another.
+struct Walk {
+  int64_t w, w_end, w0;  // w0: where the unit begins
+  PagedSeq v;
+  int seq, head, tile, tiles;
+};
+__device__ __forceinline__ bool next_unit(const PagedParams& p, Walk& k, Unit& u) {
+  while (k.w < k.w_end) {
+    int live;
+    const Span s = span_of_tile(p, k.v, k.tile, &live);
+    const int len = max(s.tiles, 1);
+    const int64_t wt = k.w0 + kUnitCost;
+    const int ta = static_cast<int>(max(k.w - wt, static_cast<int64_t>(0)));
+    const int tb = static_cast<int>(min(k.w_end - wt, static_cast<int64_t>(len)));
+    if (tb > ta) {
+      u.v = k.v, u.s = s;
+      u.seq = k.seq, u.head = k.head, u.tile = k.tile, u.live = live;
+      u.ta = ta, u.tb = tb, u.len = len, u.wt = wt;
+    }
+    k.w0 = wt + len;
+    k.w = k.w0;
+    if (++k.tile == k.tiles) {
+      k.tile = 0;
+      if (++k.head == p.nh && k.w < k.w_end) {
+        k.head = 0;
+        do {
+          k.v = paged_seq(p, ++k.seq);
+          k.tiles = tiles_of(p, k.v);
+        } while (k.tiles == 0);
+      }
+    }
+    if (tb > ta) return true;
+  }
+  return false;
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store4(uint16_t* dst, float4 o, float f) {
+  const uint32_t a = pack_two<BF16>(o.x * f, o.y * f), b = pack_two<BF16>(o.z * f, o.w * f);
+  if ((reinterpret_cast<uintptr_t>(dst) & 7) == 0) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(a, b);
+  } else {
+    dst[0] = static_cast<uint16_t>(a), dst[1] = static_cast<uint16_t>(a >> 16);
+    dst[2] = static_cast<uint16_t>(b), dst[3] = static_cast<uint16_t>(b >> 16);
+  }
+}
+
+// Partial sums: [16][HD] accumulators, 16 maxima, 16 sums.
+template <int HD>
+constexpr int kPieceFloats = kRows * (HD + 2);
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_constant__ PagedParams p) {
+  constexpr int kStages = Smem<HD>::kStages, kTileBytes = Smem<HD>::kTileBytes;
+  constexpr int kChunks = HD / 8;               // 16-byte pieces of a token
+  constexpr int kCopies = kStep * kChunks / 32; // of a lane, for K and for V
+  constexpr float kLift = BF16 ? 0.f : 15.f;    // log2 factor that weights carry
+  extern __shared__ __align__(128) uint8_t raw[];
+  Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>(raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- all work, and this warp's run ----------------------------------------------
+  const int per = (p.num_seqs + kThreads - 1) / kThreads;
+  const int s0 = min(tid * per, p.num_seqs), s1 = min(s0 + per, p.num_seqs);
+  {
+    int64_t mine = 0;
+    for (int s = s0; s < s1; ++s) mine += work_of(p, paged_seq(p, s));
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) sm.sums[warp] = incl;
+    __syncthreads();
+    int64_t at = incl - mine;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i)
+      if (i < warp) at += sm.sums[i];
+    sm.before[tid] = at;
+    if (tid == kThreads - 1) sm.before[kThreads] = at + mine;
+    if (tid < 2 * kWarps) sm.pieces[tid].wt = -1;
+    __syncthreads();
+  }
+  const int64_t total = sm.before[kThreads];
+  int64_t run = (total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps);
+  if (run < kMinRun) run = kMinRun;
+  const int64_t block_run = run * kWarps, block_begin = blockIdx.x * block_run;
+  if (block_begin >= total) return;
+
+  Walk walk;
+  walk.w = block_begin + warp * run;
+  walk.w_end = min(walk.w + run, total);
+  if (walk.w < walk.w_end) {
+    int lo = 0, n = kThreads;  // the last thread whose sequences begin at or before w
+    while (n > 1) {
+      const int step = (n + 31) >> 5, at = lo + lane * step;
+      const uint32_t votes = __ballot_sync(0xffffffffu, at < lo + n && sm.before[min(at, kThreads)] <= walk.w);
+      const int k = 31 - __clz(votes), end = lo + n;
+      lo += k * step;
+      n = min(step, end - lo);
+    }
+    int64_t at = sm.before[lo];
+    walk.seq = min(lo * per, p.num_seqs - 1);
+    for (;;) {
+      walk.v = paged_seq(p, walk.seq);
+      const int64_t work = work_of(p, walk.v);
+      if (walk.w < at + work) {
+        walk.tiles = tiles_of(p, walk.v);
+        const int64_t one = work / p.nh;
+        walk.head = static_cast<int>((walk.w - at) / one);
+        at += one * walk.head;
+        break;
+      }
+      at += work;
+      ++walk.seq;
+    }
+    walk.tile = 0;
+    for (;;) {
+      int live;
+      const int len = kUnitCost + max(span_of_tile(p, walk.v, walk.tile, &live).tiles, 1);
+      if (walk.w < at + len) break;
+      at += len;
+      ++walk.tile;
+    }
+    walk.w0 = at;
+  }
+
+  // ---- copies, some steps ahead of the products ---------------------------------------
+  const uint32_t ring = shared_at(sm.ring[warp]);
+  Unit* queue = sm.queue[warp];
+  int units_in = 0, step_in = 0, end_in = 0, page_in = -1;
+  bool more = true;
+  auto look = [&](int j) {  // page of the unit's step j
+    const Unit& u = queue[(units_in - 1) % kQueue];
+    if (j >= u.tb || j >= u.s.tiles) return -1;
+    return page_of(p, p.tables + u.seq * p.table_stride, tile_token<kStep>(u.s, j));
+  };
+  auto enter = [&]() {
+    Unit u;
+    more = more && next_unit(p, walk, u);
+    if (more) {
+      __syncwarp();
+      if (lane == 0) queue[units_in % kQueue] = u;
+      __syncwarp();
+      ++units_in;
+      step_in = u.ta, end_in = u.tb;
+      page_in = look(step_in);
+    }
+  };
+  int in = 0;  // steps copied so far
+  uint32_t there = 0;  // bit i: step i % 32 has a page
+  auto copy = [&]() {
+    if (more && step_in == end_in) enter();
+    if (more) {
+      const Unit& u = queue[(units_in - 1) % kQueue];
+      there = (there & ~(1u << (in & 31))) | (page_in >= 0 ? 1u << (in & 31) : 0u);
+      if (page_in >= 0) {
+        const int tok0 = tile_token<kStep>(u.s, step_in);
+        const uint32_t to = ring + (in % kStages) * (2 * kTileBytes);
+        const int64_t off = tok0 & ((1 << p.bs_log2) - 1);
+        const uint16_t* k = p.key + page_in * p.k_sb + off * p.k_st + u.head * p.k_sh;
+        const uint16_t* v = p.value + page_in * p.v_sb + off * p.v_st + u.head * p.v_sh;
+        // what no row sees becomes 0, whatever it holds
+        const bool edge = !(tok0 + kStep <= min(p.sinks, u.s.any_hi)) && !(tok0 >= u.s.any_lo && tok0 + kStep <= u.s.any_hi);
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int t = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
+          const int n = !edge || seen_by_any(p, u.s, tok0 + t) ? 16 : 0;
+          const uint32_t at = to + t * (HD * 2) + ((c ^ (t & 7)) << 4);
+          copy16(at, k + t * p.k_st + c * 8, n);
+          copy16(at + kTileBytes, v + t * p.v_st + c * 8, n);
+        }
+      }
+      ++step_in;
+      ++in;
+      page_in = look(step_in);
+    }
+    copies_commit();
+  };
+  if (walk.w < walk.w_end) {
+    enter();
+  } else {
+    more = false;
+  }
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) copy();
+
+  // ---- products --------------------------------------------------------------------------
+  const int r = lane >> 2, c2 = (lane & 3) * 2;  // this lane's rows r and r + 8, columns c2 and c2 + 1 of 8
+  int units_out = 0, out = 0;
+  while (units_out < units_in) {
+    const Unit& u = queue[units_out % kQueue];
+    uint32_t qf[HD / 16][4];
+    int64_t row_q[2];
+    RowView see[2];
+    int who[2];
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int x = r + 8 * z;
+      const int64_t row = static_cast<int64_t>(u.tile) * kRows + min(x, u.live - 1);
+      who[z] = static_cast<int>(row / p.group);
+      const int j = static_cast<int>(row - static_cast<int64_t>(who[z]) * p.group);
+      row_q[z] = (static_cast<int64_t>(u.v.first) + who[z]) * p.q_sr + (static_cast<int64_t>(u.head) * p.group + j) * p.q_sh;
+      see[z] = row_view(p, u.v, who[z]);
+    }
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        qf[ks][e] = __ldg(reinterpret_cast<const uint32_t*>(p.q + row_q[e & 1] + ks * 16 + (e >> 1) * 8 + c2));
+    float o[HD / 8][4];
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+    const int ta = u.ta, tb = u.tb;
+    for (int j = ta; j < tb; ++j, ++out) {
+      copy();
+      copies_wait<kStages - 1>();
+      __syncwarp();
+      if (there >> (out & 31) & 1) {
+        const int tok = tile_token<kStep>(u.s, j);
+        const uint32_t at = ring + (out % kStages) * (2 * kTileBytes);
+        float s[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        {
+          const int t = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1;
+          const uint32_t row = at + t * (HD * 2);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            uint32_t b[4];
+            load_matrix(row + (((2 * ks + half) ^ (t & 7)) << 4), b);
+            mma_16816<BF16>(s[0], qf[ks], b[0], b[1]);
+            mma_16816<BF16>(s[1], qf[ks], b[2], b[3]);
+          }
+        }
+        const bool whole = tile_whole<kStep>(u.s, tok);
+        uint32_t bits[2] = {0xffffu, 0xffffu};  // tokens that the lane's rows see
+        if (!whole) {
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            if (p.parents != nullptr) {
+              bits[z] = tree_bits(p, u.v, who[z], tok) & 0xffffu;
+            } else {
+              bits[z] = 0;
+#pragma unroll
+              for (int e = 0; e < kStep; ++e)
+                if (tok + e < see[z].hi && (tok + e >= see[z].lo || tok + e < p.sinks)) bits[z] |= 1u << e;
+            }
+          }
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int z = e >> 1, t = i * 8 + c2 + (e & 1);
+            s[i][e] = bits[z] >> t & 1 ? s[i][e] * p.scale_log2 : -INFINITY;
+            top[z] = fmaxf(top[z], s[i][e]);
+          }
+        float keep[2], ref[2];
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          top[z] = fmaxf(top[z], __shfl_xor_sync(0xffffffffu, top[z], 1));
+          top[z] = fmaxf(top[z], __shfl_xor_sync(0xffffffffu, top[z], 2));
+          const float now = fmaxf(m[z], top[z]);
+          keep[z] = now == -INFINITY ? 1.f : exp2_near(m[z] - now);
+          ref[z] = now == -INFINITY ? 0.f : now - kLift;
+          m[z] = now;
+        }
+        if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+          l[0] *= keep[0], l[1] *= keep[1];
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) o[i][0] *= keep[0], o[i][1] *= keep[0], o[i][2] *= keep[1], o[i][3] *= keep[1];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[i][e] = exp2_near(s[i][e] - ref[e >> 1]);
+            l[e >> 1] += s[i][e];
+          }
+        const uint32_t values = at + kTileBytes;
+        bool odd = false;
+        const bool alike = whole || (u.s.any_hi == u.s.all_hi && u.s.any_lo == u.s.all_lo);  // all rows see the same tokens
+        if (!alike) {
+          // Some rows see what others do not: 0 times an infinite value is not 0.
+#pragma unroll 1
+          for (int i = lane; i < kStep * kChunks; i += 32) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(values + i * 16) : "memory");
+            odd = odd || odd_two<BF16>(w[0]) || odd_two<BF16>(w[1]) || odd_two<BF16>(w[2]) || odd_two<BF16>(w[3]);
+          }
+          odd = __any_sync(0xffffffffu, odd);
+        }
+        if (!odd) {
+          // A weight is the sum of the two.  Neither is 0 where an infinite value may be seen: 0 times it is no number.
+          const uint32_t least = alike ? 0x00010001u : 0u;
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = s[e >> 1][(e & 1) * 2], b = s[e >> 1][(e & 1) * 2 + 1];
+            hi[e] = cut_two<BF16>(a, b);
+            const float2 f = unpack_two<BF16>(hi[e]);
+            lo[e] = __vmaxu2(pack_two<BF16>(a - f.x, b - f.y), least);
+            hi[e] = __vmaxu2(hi[e], least);
+          }
+          const int t = (((lane >> 3) & 1) << 3) + (lane & 7), half = lane >> 4;
+          const uint32_t row = values + t * (HD * 2);
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) {
+            uint32_t b[4];
+            load_matrix_t(row + (((2 * d + half) ^ (t & 7)) << 4), b);
+            mma_16816<BF16>(o[2 * d], hi, b[0], b[1]);
+            mma_16816<BF16>(o[2 * d + 1], hi, b[2], b[3]);
+            mma_16816<BF16>(o[2 * d], lo, b[0], b[1]);
+            mma_16816<BF16>(o[2 * d + 1], lo, b[2], b[3]);
+          }
+        } else {
+#pragma unroll
+          for (int t = 0; t < kStep; ++t) {
+            float w[2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z) w[z] = __shfl_sync(0xffffffffu, s[t >> 3][z * 2 + (t & 1)], (lane & ~3) | ((t & 7) >> 1));
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d) {
+              uint32_t x;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(values + t * (HD * 2) + ((d ^ (t & 7)) << 4) + c2 * 2) : "memory");
+              const float2 f = unpack_two<BF16>(x);
+              if (bits[0] >> t & 1) o[d][0] = fmaf(w[0], f.x, o[d][0]), o[d][1] = fmaf(w[0], f.y, o[d][1]);
+              if (bits[1] >> t & 1) o[d][2] = fmaf(w[1], f.x, o[d][2]), o[d][3] = fmaf(w[1], f.y, o[d][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();  // the stage is read
+    }
+
+    // ---- this warp's share of the unit ----------------------------------------------------
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      l[z] += __shfl_xor_sync(0xffffffffu, l[z], 1);
+      l[z] += __shfl_xor_sync(0xffffffffu, l[z], 2);
+    }
+    if (ta == 0 && tb == u.len) {
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        if (r + 8 * z >= u.live) continue;
+        const int64_t row = static_cast<int64_t>(u.tile) * kRows + r + 8 * z;
+        const int64_t i = u.v.first + row / p.group, h = static_cast<int64_t>(u.head) * p.group + row % p.group;
+        uint16_t* dst = static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh + c2;
+        const float inv = l[z] > 0.f || l[z] != l[z] ? 1.f / l[z] : 0.f;
+        const bool even = (reinterpret_cast<uintptr_t>(dst) & 3) == 0;
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) {
+          const uint32_t w = pack_two<BF16>(o[d][2 * z] * inv, o[d][2 * z + 1] * inv);
+          if (even) {
+            *reinterpret_cast<uint32_t*>(dst + d * 8) = w;
+          } else {
+            dst[d * 8] = static_cast<uint16_t>(w);
+            dst[d * 8 + 1] = static_cast<uint16_t>(w >> 16);
+          }
+        }
+        if (p.lse != nullptr && (lane & 3) == 0)
+          p.lse[i * p.nh * p.group + h] = l[z] > 0.f || l[z] != l[z] ? (m[z] - kLift + log2f(l[z])) * 0.69314718055994531f : -INFINITY;
+      }
+    } else {
+      // The last piece of a run finds its place in the ring, which is empty by then.
+      const bool final_piece = !more && units_out + 1 == units_in;
+      const int slot = ta > 0 ? 0 : 1;  // a run begins inside one unit at most, and ends inside one
+      float* part = final_piece ? reinterpret_cast<float*>(sm.ring[warp])
+                                : p.partial + (static_cast<int64_t>(blockIdx.x) * (2 * kWarps) + warp * 2 + slot) * kPieceFloats<HD>;
+      if (final_piece) {
+        copies_wait<0>();
+        __syncwarp();
+      }
+#pragma unroll
+      for (int z = 0; z < 2; ++z) {
+        if (r + 8 * z >= u.live) continue;
+        float* dst = part + (r + 8 * z) * HD + c2;
+#pragma unroll
+        for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * z], o[d][2 * z + 1]);
+        if ((lane & 3) == 0) {
+          part[kRows * HD + r + 8 * z] = m[z];
+          part[kRows * HD + kRows + r + 8 * z] = l[z];
+        }
+      }
+      if (lane == 0) {
+        Piece& x = sm.pieces[warp * 2 + slot];
+        x.wt = u.wt, x.at = part;
+        x.seq = u.seq, x.head = u.head, x.tile = u.tile, x.live = u.live, x.len = u.len, x.first = u.v.first;
+      }
+    }
+    ++units_out;
+    __syncwarp();
+  }
+  copies_wait<0>();
+  __syncthreads();
+
+  // ---- pieces of the same unit ----------------------------------------------------------------
+  auto finish = [&](const Piece& x, int row_in, int d, float4 sum, float mx, float l_sum) {
+    const int64_t row = static_cast<int64_t>(x.tile) * kRows + row_in;
+    const int64_t i = x.first + row / p.group, h = static_cast<int64_t>(x.head) * p.group + row % p.group;
+    const bool any = l_sum > 0.f || l_sum != l_sum;
+    store4<BF16>(static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh + d, sum, any ? 1.f / l_sum : 0.f);
+    if (p.lse != nullptr && d == 0)
+      p.lse[i * p.nh * p.group + h] = any ? (mx - kLift + log2f(l_sum)) * 0.69314718055994531f : -INFINITY;
+  };
+  for (int g0 = 0; g0 < 2 * kWarps;) {
+    const int64_t wt = sm.pieces[g0].wt;
+    if (wt < 0) {
+      ++g0;
+      continue;
+    }
+    int g1 = g0 + 1;  // pieces [g0, g1), some of them empty places
+    while (g1 < 2 * kWarps && (sm.pieces[g1].wt < 0 || sm.pieces[g1].wt == wt)) ++g1;
+    const Piece& x = sm.pieces[g0];
+    const int64_t first = wt / block_run, last = (wt + x.len - 1) / block_run;
+    float* mine = p.partial + (static_cast<int64_t>(gridDim.x) * (2 * kWarps) + 2 * blockIdx.x + (wt > block_begin ? 1 : 0)) * kPieceFloats<HD>;
+    for (int item = tid; item < x.live * (HD / 4); item += kThreads) {
+      const int row = item / (HD / 4), d = item % (HD / 4) * 4;
+      float mx = -INFINITY, l_sum = 0.f;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int g = g0; g < g1; ++g) {
+        if (sm.pieces[g].wt < 0) continue;
+        const float* at = sm.pieces[g].at;
+        const float pm = at[kRows * HD + row], pl = at[kRows * HD + kRows + row];
+        const float4 po = *reinterpret_cast<const float4*>(at + row * HD + d);
+        const float now = fmaxf(mx, pm);
+        const float a = now == -INFINITY ? 1.f : exp2_near(mx - now), b = now == -INFINITY ? 1.f : exp2_near(pm - now);
+        sum.x = sum.x * a + po.x * b, sum.y = sum.y * a + po.y * b, sum.z = sum.z * a + po.z * b, sum.w = sum.w * a + po.w * b;
+        l_sum = l_sum * a + pl * b;
+        mx = now;
+      }
+      if (first == last) {
+        finish(x, row, d, sum, mx, l_sum);
+      } else {
+        *reinterpret_cast<float4*>(mine + row * HD + d) = sum;
+        if (d == 0) mine[kRows * HD + row] = mx, mine[kRows * HD + kRows + row] = l_sum;
+      }
+    }
+    if (first != last) {
+      __syncthreads();
+      if (tid == 0) {  // releases what the barrier has gathered
+        int ticket;
+        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + first) : "memory");
+        sm.last = ticket == last - first;
+      }
+      __syncthreads();
+      if (sm.last) {
+        auto from = [&](int64_t b) {
+          return p.partial + (static_cast<int64_t>(gridDim.x) * (2 * kWarps) + 2 * b + (wt > b * block_run ? 1 : 0)) * kPieceFloats<HD>;
+        };
+        for (int item = tid; item < x.live * (HD / 4); item += kThreads) {
+          const int row = item / (HD / 4), d = item % (HD / 4) * 4;
+          float mx = -INFINITY, l_sum = 0.f;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int64_t b = first; b <= last; ++b) {
+            const float* at = from(b);
+            const float pm = __ldcg(at + kRows * HD + row), pl = __ldcg(at + kRows * HD + kRows + row);
+            const float4 po = __ldcg(reinterpret_cast<const float4*>(at + row * HD + d));
+            const float now = fmaxf(mx, pm);
+            const float fa = now == -INFINITY ? 1.f : exp2_near(mx - now), fb = now == -INFINITY ? 1.f : exp2_near(pm - now);
+            sum.x = sum.x * fa + po.x * fb, sum.y = sum.y * fa + po.y * fb, sum.z = sum.z * fa + po.z * fb, sum.w = sum.w * fa + po.w * fb;
+            l_sum = l_sum * fa + pl * fb;
+            mx = now;
+          }
+          finish(x, row, d, sum, mx, l_sum);
+        }
+        if (tid == 0) p.counters[first] = 0;
+      }
+    }
+    g0 = g1;
+  }
+}
+
+template <int HD, bool BF16>
+int launch_rows(const PagedParams& p, const char* name, cudaStream_t st) {
+  constexpr int kBytes = sizeof(Smem<HD>);
+  static_assert(kBytes <= 227 * 1024, "shared memory of a block");
+  static_assert(kRows * (HD + 2) * 4 <= Smem<HD>::kStages * 2 * Smem<HD>::kTileBytes, "a piece fits its warp's ring");
+  static_assert(kQueue > Smem<HD>::kStages, "units in flight");
+  const auto kernel = paged_rows_kernel<HD, BF16>;
+  static bool ready[kPagedDevices] = {};
+  if (int rc = paged_prepare(name, kernel, kBytes, ready)) return rc;
+  const int sms = sm_count();
+  return launch_pdl(name, kernel, dim3(sms < kMaxGrid ? sms : kMaxGrid), dim3(kThreads), kBytes, st, p);
+}
+
+constexpr int64_t kCounterBytes = 4096;
+static_assert(kMaxGrid * 4 <= kCounterBytes, "a counter per block");
+
+}  // namespace
+
+int check_paged_cache(const mak_paged_cache_desc& c, bool values, const char* name) {
+  if (c.head_dim != 64 && c.head_dim != 128) return fail(MAK_E_UNSUPPORTED, "%s: head_dim must be 64 or 128, got %d", name, c.head_dim);
+  if (c.block_size != 16 && c.block_size != 32 && c.block_size != 64 && c.block_size != 128)
+    return fail(MAK_E_UNSUPPORTED, "%s: block_size must be 16, 32, 64 or 128, got %d", name, c.block_size);
+  if (c.dtype != MAK_DT_F16 && c.dtype != MAK_DT_BF16) return fail(MAK_E_UNSUPPORTED, "%s: caches must be float16 or bfloat16", name);
+  if (c.num_seqs < 0 || c.num_blocks < 0 || c.max_blocks < 0 || c.num_rows < 0 || c.num_heads <= 0)
+    return fail(MAK_E_INVALID, "%s: negative size", name);
+  if (c.num_seqs > 0x7fffffff || c.num_blocks > 0x7fffffff || c.num_rows > 0x7fffffff || c.max_blocks > 0x7fffffff / c.block_size)
+    return fail(MAK_E_UNSUPPORTED, "%s: sequences, blocks, rows and tokens of a sequence are 32-bit counts", name);
+  if (c.num_seqs > 0 && (c.context_lens == nullptr || (c.max_blocks > 0 && c.block_tables == nullptr)))
+    return fail(MAK_E_INVALID, "%s: null block_tables or context_lens", name);
+  if (c.num_blocks > 0 && (c.key == nullptr || (values && c.value == nullptr))) return fail(MAK_E_INVALID, "%s: null cache", name);
+  uint64_t bits = reinterpret_cast<uintptr_t>(c.key), strides = static_cast<uint64_t>(c.key_stride_block | c.key_stride_token | c.key_stride_head);
+  if (values) {
+    bits |= reinterpret_cast<uintptr_t>(c.value);
+    strides |= static_cast<uint64_t>(c.value_stride_block | c.value_stride_token | c.value_stride_head);
+  }
+  if ((bits & 15) || (strides & 7)) return fail(MAK_E_INVALID, "%s: caches need 16-byte aligned addresses and strides", name);
+  return MAK_OK;
+}
+
+PagedParams paged_params(const mak_paged_cache_desc& c) {
+  PagedParams p = {};
+  p.key = static_cast<const uint16_t*>(c.key);
+  p.value = static_cast<const uint16_t*>(c.value);
+  p.k_sb = c.key_stride_block, p.k_st = c.key_stride_token, p.k_sh = c.key_stride_head;
+  p.v_sb = c.value_stride_block, p.v_st = c.value_stride_token, p.v_sh = c.value_stride_head;
+  p.tables = c.block_tables, p.ctx_lens = c.context_lens, p.starts = c.cu_seqlens;
+  p.table_stride = c.table_stride, p.num_blocks = c.num_blocks;
+  p.num_seqs = static_cast<int32_t>(c.num_seqs), p.max_blocks = static_cast<int32_t>(c.max_blocks);
+  p.num_rows = static_cast<int32_t>(c.num_rows);
+  p.nh = c.num_heads;
+  p.bs_log2 = c.block_size == 16 ? 4 : c.block_size == 32 ? 5 : c.block_size == 64 ? 6 : 7;
+  return p;
+}
+
+}  // namespace mak
+
+using namespace mak;
+
+extern "C" int64_t mak_paged_attention_workspace_bytes(void) {
+  return kCounterBytes + static_cast<int64_t>(kMaxGrid) * (2 * kWarps + 2) * kPieceFloats<128> * 4;
+}
+
+extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
+  const char* name = "mak_paged_attention";
+  if (d == nullptr) return fail(MAK_E_INVALID, "%s: null descriptor", name);
+  const mak_paged_cache_desc& c = d->cache;
+  if (int rc = check_paged_cache(c, true, name)) return rc;
+  if (d->num_q_heads <= 0 || d->num_q_heads % c.num_heads)
+    return fail(MAK_E_INVALID, "%s: %d query heads over %d cache heads", name, d->num_q_heads, c.num_heads);
+  if (d->window < 0 || d->sinks < 0) return fail(MAK_E_INVALID, "%s: negative window or sinks", name);
+  if (d->parents != nullptr && d->window) return fail(MAK_E_INVALID, "%s: a tree has no window", name);
+  if (c.num_seqs == 0 || c.num_rows == 0) return MAK_OK;
+  if (d->q == nullptr || d->out == nullptr) return fail(MAK_E_INVALID, "%s: null q or out", name);
+  if ((reinterpret_cast<uintptr_t>(d->q) & 15) || ((d->q_stride_row | d->q_stride_head) & 7))
+    return fail(MAK_E_INVALID, "%s: q needs 16-byte aligned rows", name);
+  if (d->workspace == nullptr || d->workspace_bytes < mak_paged_attention_workspace_bytes())
+    return fail(MAK_E_WORKSPACE, "%s: workspace missing or too small", name);
+  PagedParams p = paged_params(c);
+  p.parents = d->parents;
+  p.q = static_cast<const uint16_t*>(d->q), p.out = d->out, p.lse = d->lse;
+  p.q_sr = d->q_stride_row, p.q_sh = d->q_stride_head, p.o_sr = d->out_stride_row, p.o_sh = d->out_stride_head;
+  p.group = d->num_q_heads / c.num_heads;
+  p.window = d->window, p.sinks = d->window ? d->sinks : 0;
+  p.scale_log2 = d->scale * 1.4426950408889634f;
+  p.counters = static_cast<int32_t*>(d->workspace);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kCounterBytes);
+  cudaStream_t st = as_stream(stream);
+  const bool bf16 = c.dtype == MAK_DT_BF16;
+  if (c.head_dim == 64) return bf16 ? launch_rows<64, true>(p, name, st) : launch_rows<64, false>(p, name, st);
+  return bf16 ? launch_rows<128, true>(p, name, st) : launch_rows<128, false>(p, name, st);
+}

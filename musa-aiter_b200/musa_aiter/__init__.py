@@ -10,7 +10,9 @@ from .version import __version__
 from . import registry, dispatch
 from .ops.block_cache import kv_append_block_scaled, paged_attention_block_scaled
 from .ops.cache import apply_rope, apply_rope_to_key_cache, copy_to_kv_cache
-from .ops.pages import kv_pages_compact, kv_pages_copy, kv_pages_fork, kv_pages_free, kv_pages_grow
+from .ops.paged_attention import paged_attention_tree, paged_attention_weights, paged_attention_window
+from .ops.pages import kv_pages_compact, kv_pages_copy, kv_pages_evict, kv_pages_fork, kv_pages_free, kv_pages_grow
+from .ops.qk_norm_rope import apply_qk_norm_rope, apply_qk_norm_rope_backward
 from .ops.rope_axes import apply_rope_axes, apply_rope_axes_backward
 from .ops.kv_layout import KVFormatFacts, KVLayoutKind, KVLayoutSpec, KVOrganization, KVScaleKind
 from .ops.kv_transfer_plan import (

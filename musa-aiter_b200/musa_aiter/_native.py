@@ -284,6 +284,12 @@ _PROTOTYPES = {
     "mak_pages_compact": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mak_pages_copy": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
     "mak_rope_axes": (c_int32, [c_void_p, c_void_p]),
+    "mak_paged_attention_workspace_bytes": (c_int64, []),
+    "mak_paged_attention": (c_int32, [c_void_p, c_void_p]),
+    "mak_paged_weights": (c_int32, [c_void_p, c_void_p]),
+    "mak_pages_evict": (c_int32, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "mak_qk_norm_rope_partial_floats": (c_int64, [c_int32]),
+    "mak_qk_norm_rope": (c_int32, [c_void_p, c_void_p]),
 }
 
 _LOCK = threading.Lock()

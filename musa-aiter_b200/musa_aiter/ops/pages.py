@@ -17,7 +17,7 @@ import torch
 
 from .. import _native
 
-__all__ = ["kv_pages_compact", "kv_pages_copy", "kv_pages_fork", "kv_pages_free", "kv_pages_grow"]
+__all__ = ["kv_pages_compact", "kv_pages_copy", "kv_pages_evict", "kv_pages_fork", "kv_pages_free", "kv_pages_grow"]
 
 
 def kv_pages_copy(planes: Sequence[torch.Tensor], src_pages: torch.Tensor, dst_pages: torch.Tensor) -> None:
@@ -71,3 +71,32 @@ def kv_pages_compact(block_tables: torch.Tensor, ref_counts: torch.Tensor, plane
     Pages already among the first ``live`` stay; the others go to the holes there, in index order.  What
     lies behind is left as it was.  Returns ``live`` as an int32 ``[1]`` tensor on the device."""
     return _native.front().compact(block_tables, ref_counts, planes)
+
+
+def kv_pages_evict(
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    rows: torch.Tensor,
+    ref_counts: torch.Tensor,
+    key_caches: Sequence[torch.Tensor],
+    value_caches: Sequence[torch.Tensor],
+    sums: torch.Tensor,
+    keep: int,
+    *,
+    sinks: int = 0,
+    recent: int = 0,
+) -> torch.Tensor:
+    """Shrink rows of more than ``keep`` tokens to ``keep``, each layer and head keeping its own.
+
+    ``key_caches`` / ``value_caches``: the layers' planes ``[num_pages, block_size, num_heads, head_dim]`` (float16 or
+    bfloat16, head_dim 64, 128 or 256); ``sums``: float32 ``[layers, rows of block_tables, num_heads, max_tokens]``, what
+    ``paged_attention_weights`` has gathered.  The first ``sinks`` and the last ``recent`` tokens stay, and of the others
+    those of the largest sums (of equal ones the first; NaN counts as -inf).  Kept tokens move to the row's first places
+    in their order, their sums with them, and the sums behind become 0; pages that are left over lose one reference.
+    Keys keep the rotation they were written with: what is appended later goes on at the row's new length, so positions
+    for the rotation have to be counted apart.
+
+    Returns an int32 ``[1]`` tensor on the device: how many rows were left as they are because a page that would be
+    written is shared with another row, a page is out of range, or they have more tokens than their table or ``sums``
+    hold.  A row named twice shrinks once."""
+    return _native.front().evict(block_tables, context_lens, rows, ref_counts, key_caches, value_caches, sums, keep, sinks, recent)

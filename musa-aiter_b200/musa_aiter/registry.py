@@ -122,6 +122,8 @@ _CACHE = [
     ("apply_rope_to_key_cache", "b200", _FLOAT, "Apply RoPE in place to selected paged key-cache slots.", ()),
     ("apply_rope_axes", "b200", _HALF, "RoPE with one position per axis (time, height, width), q and k in one launch.", ()),
     ("apply_rope_axes_backward", "b200", _HALF, "Gradient of apply_rope_axes.", ()),
+    ("apply_qk_norm_rope", "b200", _HALF, "Norms of q and k for each head with RoPE, one pass.", ()),
+    ("apply_qk_norm_rope_backward", "b200", _HALF, "Gradient of apply_qk_norm_rope.", ()),
     ("kv_append_block_scaled", "b200", _FLOAT, "Quantising write into an 8-bit cache with one scale per block and head.", ()),
 ]
 for _name, _status, _dtypes, _desc, _notes in _CACHE:
@@ -130,6 +132,10 @@ for _name, _status, _dtypes, _desc, _notes in _CACHE:
 # Operators of this build on top of the reference's families.
 _EXTRA = [
     ("paged_attention_block_scaled", "attention", _HALF, "Attention over a paged 8-bit cache with one scale per block and head."),
+    ("paged_attention_window", "attention", _HALF, "Attention over a paged 16-bit cache, sliding window and first tokens that stay visible."),
+    ("paged_attention_tree", "attention", _HALF, "Attention of trees of drafted tokens over a paged 16-bit cache."),
+    ("paged_attention_weights", "eviction", _HALF, "The attention weight that each cached token gathers."),
+    ("kv_pages_evict", "eviction", _HALF, "Shrink sequences to the tokens that gathered most weight, each head its own."),
     ("kv_pages_copy", "pages", ("any",), "Copy pages within every plane of a cache, one launch."),
     ("kv_pages_fork", "pages", ("any",), "Continue sequences in new rows: full pages shared, part-filled ones copied."),
     ("kv_pages_grow", "pages", ("int32",), "Hand out pages for new tokens."),
