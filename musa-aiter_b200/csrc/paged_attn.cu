@@ -10,7 +10,7 @@
 // the lengths; a warp copies its steps into a ring of its own (a page's row of 16 bytes per lane), so no warp waits for
 // another until its run ends.  A unit cut by that leaves partial sums: the block joins those of its warps, the last block
 // to arrive joins those of the blocks, both in order of position, so results do not depend on timing.
-#include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 
 namespace mak {
 namespace {
@@ -565,6 +565,7 @@ int launch_rows(const PagedParams& p, const char* name, cudaStream_t st) {
 }
 
 constexpr int64_t kCounterBytes = 4096;
+int64_t plan_bytes() { return (paged_tc_plan_bytes() + 255) / 256 * 256; }
 static_assert(kMaxGrid * 4 <= kCounterBytes, "a counter per block");
 
 }  // namespace
@@ -610,7 +611,8 @@ PagedParams paged_params(const mak_paged_cache_desc& c) {
 using namespace mak;
 
 extern "C" int64_t mak_paged_attention_workspace_bytes(void) {
-  return kCounterBytes + static_cast<int64_t>(kMaxGrid) * (2 * kWarps + 2) * kPieceFloats<128> * 4;
+  const int64_t few = static_cast<int64_t>(kMaxGrid) * (2 * kWarps + 2) * kPieceFloats<128> * 4, many = paged_tc_partial_bytes();
+  return kCounterBytes + plan_bytes() + (few > many ? few : many);
 }
 
 extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
@@ -636,9 +638,16 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   p.window = d->window, p.sinks = d->window ? d->sinks : 0;
   p.scale_log2 = d->scale * 1.4426950408889634f;
   p.counters = static_cast<int32_t*>(d->workspace);
-  p.partial = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kCounterBytes);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kCounterBytes + plan_bytes());
   cudaStream_t st = as_stream(stream);
   const bool bf16 = c.dtype == MAK_DT_BF16;
+  // Rows that share a cache head, on average.
+  const int64_t rows = c.num_rows * p.group / c.num_seqs;
+  if (rows > 32 && paged_tc_fits(p)) {
+    bool taken = false;
+    const int rc = launch_paged_tc(p, c.head_dim, bf16, name, static_cast<char*>(d->workspace) + kCounterBytes, st, &taken);
+    if (rc != MAK_OK || taken) return rc;
+  }
   if (c.head_dim == 64) return bf16 ? launch_rows<64, true>(p, name, st) : launch_rows<64, false>(p, name, st);
   return bf16 ? launch_rows<128, true>(p, name, st) : launch_rows<128, false>(p, name, st);
 }

@@ -1,0 +1,886 @@
+// Attention over a paged 16-bit cache for many rows per sequence (prompts, trees): the products on the tcgen05 tensor
+// cores, K and V brought in by TMA as they lie in their pages.
+//
+// S = q K^T and O = P V with S, P and O in tensor memory: of each row of 128 scores the largest is found, weights
+// 2^(S c - m') are written over the scores in 16 bits and multiply V.  Sums, maxima and accumulators are 32-bit; a weight is
+// rounded once to the cache's type, which the tensor cores take next to V (wider weights at half the rate): its error, half
+// a step of itself, is what rounding a result adds too.  The running maximum is only moved where it grew by more than
+// 2^kLazy, so accumulators are rarely rescaled; the result is the same.
+//
+// Of each 32 weights some are taken by the exponential unit (16 a cycle and SM: as long as the products take for all of
+// them) and some by a polynomial on the other units: 2^y = 2^n 2^f, n the nearest whole number, 2^f of degree 4 with the
+// smallest largest relative error on [-1/2, 1/2], 2.6e-6 (coefficients by exchange of extrema, as Remez has it).
+//
+// A block takes 256 rows of one cache head (heads of the group next to one another, so a K / V tile serves all of them) as
+// two halves of 128 and walks the tokens in tiles of 128; of a unit with 128 rows or fewer each half takes every other
+// tile instead, and the two are joined.  Roles:
+//   warps 0-3, 4-7   softmax of half 0 / 1, a thread per row (TMEM lane)
+//   warp 8           page ids and TMA loads
+//   warp 9           one thread issues all tcgen05.mma
+//   warps 10, 11     values in tiles that not every row sees whole: infinite and NaN ones become 0 there
+// While one half's scores are exponentiated the tensor cores work for the other.
+//
+// What a row does not see reaches none of its sums: its weights there are 0, and 0 times a value that is no number is
+// kept out by warps 10 and 11; the rows that do see such a value get it with their results (odd_sum).
+//
+// Work.  All (row tile, head) units laid end to end, each as long as the tiles it sees, are cut into equal runs, one per
+// block; a small launch before this one adds up the lengths.  A unit cut by that leaves partial sums, and the last half to
+// arrive joins them in order of position, so results do not depend on timing.
+#include <utility>
+
+#include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
+#include "tcgen05.cuh"
+
+namespace mak {
+namespace {
+
+constexpr int kTile = 128;      // tokens per step
+constexpr int kHalf = 128;      // rows of a half
+constexpr int kUnitRows = 256;  // rows of a unit
+constexpr int kThreads = 384;
+constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolerated
+constexpr int kUnitCost = 4;    // a unit's beginning and end, in tiles
+constexpr int kMinChunk = 4;    // steps of work that are worth another block
+constexpr int kMaxGrid = 148;
+constexpr int kMaxItems = 1 << 16;
+constexpr int kHave = 8;
+
+// What the planning launch leaves: unit lengths added up over the row tiles, and whose they are.
+struct Plan {
+  int64_t base[kMaxItems + 1];  // work before row tile i, over all heads
+  int32_t seq[kMaxItems];
+  int32_t tile[kMaxItems];
+};
+
+// Rows of row tile `tile` of a sequence (numbers below the first sequence's come as negative ones) and what they see.
+__device__ __forceinline__ int live_rows(const PagedParams& p, const PagedSeq& v, int tile) {
+  const int64_t left = static_cast<int64_t>(v.rows) * p.group - static_cast<int64_t>(tile) * kUnitRows;
+  return tile < 0 || left <= 0 ? 0 : left < kUnitRows ? static_cast<int>(left) : kUnitRows;
+}
+__device__ __forceinline__ Span span_of_rows(const PagedParams& p, const PagedSeq& v, int tile, int row_a, int row_b) {
+  const int64_t row0 = static_cast<int64_t>(tile) * kUnitRows;
+  return span_of<kTile>(p, v, static_cast<int>((row0 + row_a) / p.group), static_cast<int>((row0 + row_b) / p.group));
+}
+__device__ __forceinline__ int unit_len(const PagedParams& p, const PagedSeq& v, int tile) {
+  const int live = live_rows(p, v, tile);
+  return live == 0 ? 0 : kUnitCost + max(span_of_rows(p, v, tile, 0, live - 1).tiles, 1);
+}
+
+// Row tiles of sequence s take the numbers floor(starts[s] * group / 256) + s and up, at least as many as it has; numbers
+// before the first sequence's are nobody's.
+__device__ __forceinline__ int64_t first_item(const PagedParams& p, int s) {
+  const int64_t row = p.starts != nullptr ? max(__ldg(p.starts + s), 0) : s;
+  return row * p.group / kUnitRows + s;
+}
+
+__global__ void __launch_bounds__(1024) paged_plan_kernel(const __grid_constant__ PagedParams p, Plan* plan, int items) {
+  __shared__ int64_t sums[32];
+  pdl_wait();
+  pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (items + 1023) / 1024;
+  const int i0 = min(tid * per, items), i1 = min(i0 + per, items);
+  int seq = 0;
+  if (i0 < i1) {
+    int hi = p.num_seqs;  // the last sequence whose first number is at most i0
+    while (hi - seq > 1) {
+      const int mid = (seq + hi) >> 1;
+      if (first_item(p, mid) <= i0)
+        seq = mid;
+      else
+        hi = mid;
+    }
+  }
+  int64_t mine = 0;
+  for (int i = i0; i < i1; ++i) {
+    while (seq + 1 < p.num_seqs && first_item(p, seq + 1) <= i) ++seq;
+    const int tile = static_cast<int>(i - first_item(p, seq));
+    plan->seq[i] = seq;
+    plan->tile[i] = tile;
+    mine += unit_len(p, paged_seq(p, seq), tile);
+  }
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int64_t v = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += up;
+    }
+    sums[lane] = v;
+  }
+  __syncthreads();
+  int64_t at = (warp ? sums[warp - 1] : 0) + incl - mine;
+  for (int i = i0; i < i1; ++i) {
+    plan->base[i] = at * p.nh;
+    at += unit_len(p, paged_seq(p, plan->seq[i]), plan->tile[i]);
+  }
+  if (tid == 1023) plan->base[items] = sums[31] * p.nh;
+}
+
+// The run of a block, one (row tile, head) unit after another; every role walks it for itself.
+struct Walk {
+  int64_t w, w_end, w0;  // w0: where the current unit begins
+  int item, head, seq, tile, live;
+  PagedSeq v;
+  Span s;
+};
+struct Unit {
+  PagedSeq v;
+  Span s;
+  int seq, head, tile, live;
+  int ta, tb, len;  // this block has tiles [ta, tb) of len, at least 1
+  int n;            // of these, real ones
+  int64_t wt;       // where the unit's tiles begin in all work
+  bool solo;        // each half takes every other tile
+};
+
+__device__ __forceinline__ void look_up(const PagedParams& p, const Plan* plan, Walk& k) {
+  k.seq = plan->seq[k.item];
+  k.tile = plan->tile[k.item];
+  k.v = paged_seq(p, k.seq);
+  k.live = live_rows(p, k.v, k.tile);
+  if (k.live > 0) k.s = span_of_rows(p, k.v, k.tile, 0, k.live - 1);
+}
+
+__device__ __forceinline__ bool next_unit(const PagedParams& p, const Plan* plan, Walk& k, Unit& u) {
+  for (;;) {
+    if (k.w >= k.w_end) return false;
+    const int len = max(k.s.tiles, 1);
+    u.ta = static_cast<int>(max(k.w - k.w0 - kUnitCost, static_cast<int64_t>(0)));
+    u.tb = static_cast<int>(min(k.w_end - k.w0 - kUnitCost, static_cast<int64_t>(len)));
+    u.len = len;
+    u.seq = k.seq, u.head = k.head, u.tile = k.tile, u.live = k.live, u.v = k.v, u.s = k.s;
+    u.wt = k.w0 + kUnitCost;
+    u.n = k.s.tiles > 0 ? u.tb - u.ta : 0;
+    u.solo = k.live <= kHalf;
+    k.w0 += kUnitCost + len;
+    k.w = k.w0;
+    if (k.w < k.w_end && ++k.head == p.nh) {
+      k.head = 0;
+      do {
+        ++k.item;
+        look_up(p, plan, k);
+      } while (k.live == 0);
+    }
+    if (u.tb > u.ta) return true;
+  }
+}
+
+// f(0), f(1) ... f(N - 1) with the number as a constant.
+template <int N, typename F, int... I>
+__device__ __forceinline__ void steps_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void steps(F f) {
+  steps_of<N>(f, std::make_integer_sequence<int, N>());
+}
+
+__device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 w, x, y, z;\n mov.b64 w, {%2, %3};\n mov.b64 x, {%4, %5};\n mov.b64 y, {%6, %7};\n fma.rn.f32x2 z, w, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// The larger of the three, NaN where one is NaN.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^y for y up to 2^7, without the exponential unit; below -125 it is 2^-125 or so.
+__device__ __forceinline__ float2 exp2_poly(float2 y) {
+  constexpr float kShift = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
+  y.x = fmaxf(y.x, -125.f), y.y = fmaxf(y.y, -125.f);
+  const float2 n = add2(y, both(kShift));
+  const float2 f = add2(y, fma2(n, both(-1.f), both(kShift)));
+  float2 q = fma2(both(0.009570101911f), f, both(0.05591786032f));
+  q = fma2(q, f, both(0.2402474483f));
+  q = fma2(q, f, both(0.6931218147f));
+  q = fma2(q, f, both(0.9999992614f));
+  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(n.x) << 23)),
+                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(n.y) << 23)));
+}
+
+template <int HD>
+struct TcSmem {
+  static constexpr int kBytes = kTile * HD * 2;  // of a tile of K, V or q: HD / 64 pieces of [128][64], lines of 128 bytes swizzled
+  static constexpr int kK = HD == 64 ? 4 : 2, kV = HD == 64 ? 4 : 3;  // tiles of K and of V
+  alignas(1024) uint8_t q[2][kBytes];
+  alignas(1024) uint8_t k[kK][kBytes];
+  alignas(1024) uint8_t v[kV][kBytes];
+  alignas(8) uint64_t q_full[2], k_full[kK], k_empty[kK], v_full[kV], v_clean[kV], v_empty[kV], s_full[2], p_full[2][2], o_full[2], spare;
+  Walk walk[6];
+  Unit unit[6];
+  int more[6];
+  uint32_t have[kHave];  // bit c: 16 tokens c of a tile have a page
+  uint32_t tmem;
+  int gave_up, last[2];
+  int odd_seen;  // values that are no numbers were replaced
+};
+
+// Of dimension d .. d + 16: the sum of the values that are no numbers over the tokens that row i of the unit sees, in this
+// half's tiles, where they were replaced.
+template <bool BF16>
+__device__ __noinline__ void odd_sum(const PagedParams& p, const Unit& u, int i, int d, int first, int step, float* sum) {
+  const RowView r = row_view(p, u.v, i);
+  for (int j = u.ta + first; j < u.ta + u.n; j += step) {
+    const int tok = tile_token<kTile>(u.s, j);
+    if (tile_whole<kTile>(u.s, tok)) continue;
+    for (int t = tok; t < tok + kTile; ++t) {
+      const bool seen = p.parents != nullptr ? tree_bits(p, u.v, i, t) & 1 : t < r.hi && (t >= r.lo || t < p.sinks);
+      if (!seen) continue;
+      const int page = page_of(p, p.tables + u.seq * p.table_stride, t);
+      if (page < 0) continue;
+      const uint16_t* v = p.value + page * p.v_sb + (t & ((1 << p.bs_log2) - 1)) * p.v_st + u.head * p.v_sh + d;
+      for (int e = 0; e < 16; ++e) {
+        const float x = to_float<BF16>(v[e]);
+        if (!(fabsf(x) < INFINITY)) sum[e] += x;
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void box_load(uint32_t to, const void* map, int x, int head, int token, int block, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
+      "l"(map), "r"(x), "r"(head), "r"(token), "r"(block), "r"(smem_addr(bar))
+      : "memory");
+}
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_tc_kernel(const __grid_constant__ PagedParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                    const Plan* plan, int items) {
+  using Sm = TcSmem<HD>;
+  constexpr float kLift = BF16 ? 0.f : 6.f;  // log2 factor that weights carry: those of float16 stay below 2^15
+  constexpr int kBytes = Sm::kBytes, kK = Sm::kK, kV = Sm::kV;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Sm& sm = *reinterpret_cast<Sm*>(raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- the run of this block ----------------------------------------------------
+  Walk walk;
+  const int64_t total = plan->base[items];
+  int64_t chunk = (total + gridDim.x - 1) / gridDim.x;
+  if (chunk < kMinChunk) chunk = kMinChunk;
+  walk.w = blockIdx.x * chunk;
+  walk.w_end = min(walk.w + chunk, total);
+  if (walk.w >= walk.w_end) return;
+  {
+    int lo = 0, n = items;  // the last row tile that begins at or before w
+    while (n > 1) {
+      const int step = (n + 31) >> 5;
+      const int at = lo + lane * step;
+      const uint32_t votes = __ballot_sync(0xffffffffu, at < lo + n && plan->base[at] <= walk.w);
+      const int k = 31 - __clz(votes);
+      const int end = lo + n;
+      lo += k * step;
+      n = min(step, end - lo);
+    }
+    walk.item = lo;
+    look_up(p, plan, walk);
+    const int len = kUnitCost + max(walk.s.tiles, 1);
+    const int64_t rel = walk.w - plan->base[lo];
+    walk.head = static_cast<int>(rel / len);
+    walk.w0 = plan->base[lo] + static_cast<int64_t>(walk.head) * len;
+  }
+  if (tid == 0) {
+    sm.gave_up = 0;
+    sm.odd_seen = 0;
+    mbar_init(&sm.spare, 1);
+    for (int i = 0; i < kK; ++i) mbar_init(&sm.k_full[i], 1), mbar_init(&sm.k_empty[i], 1);
+    for (int i = 0; i < kV; ++i) mbar_init(&sm.v_full[i], 1), mbar_init(&sm.v_clean[i], 2), mbar_init(&sm.v_empty[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], 4);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i][0], 4);
+      mbar_init(&sm.p_full[i][1], 4);
+      mbar_init(&sm.o_full[i], 1);
+    }
+    mbar_init_fence();
+  }
+  if (warp == 9) tmem_alloc<512>(&sm.tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  volatile int* gave_up = &sm.gave_up;
+
+  if (warp < 8) {
+    regs_up<208>();  // with 88 below: what the block was launched with
+    // ---- softmax ----------------------------------------------------------------
+    const int half = warp >> 2;
+    const int r = tid & 127;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_at = tmem + lanes + half * 128;
+    const uint32_t o_at = tmem + lanes + 256 + half * HD;
+    const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);  // not 0: masked scores are -inf
+    const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+    uint32_t before = 0, mine = 0, ends = 0;  // tiles of all units so far, of this half, and how many units had tiles for it
+    bool ok = true;
+    if (r == 0) sm.walk[half] = walk;
+    const Unit& u = sm.unit[half];
+    for (;;) {
+      if (r == 0) sm.more[half] = next_unit(p, plan, sm.walk[half], sm.unit[half]);
+      half_sync(half);
+      if (!sm.more[half]) break;
+      const bool solo = u.solo;
+      const int row_in = solo ? r : half * kHalf + r;  // of the unit
+      const bool active = solo || half * kHalf < u.live;
+      const bool on = row_in < u.live;
+      const int64_t row = static_cast<int64_t>(u.tile) * kUnitRows + (on ? row_in : 0);
+      const int who = static_cast<int>(row / p.group), head = u.head * p.group + static_cast<int>(row - static_cast<int64_t>(who) * p.group);
+      const int first = solo ? half : 0, step = solo ? 2 : 1;
+      const int n = active && u.n > first ? (u.n - first + step - 1) / step : 0;  // tiles of this half
+      float m = -INFINITY, l = 0.f;
+      if (n > 0) {
+        {  // this row of q
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + (static_cast<int64_t>(u.v.first) + who) * p.q_sr + head * p.q_sh);
+          uint4 x[HD / 8];
+#pragma unroll
+          for (int e = 0; e < HD / 8; ++e) x[e] = on ? __ldg(src + e) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < HD / 8; ++e)
+            *reinterpret_cast<uint4*>(sm.q[half] + (e >> 3) * 16384 + r * 128 + (((e & 7) ^ (r & 7)) << 4)) =
+                make_uint4(x[e].x ^ sign, x[e].y ^ sign, x[e].z ^ sign, x[e].w ^ sign);
+          fence_async_shared();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.q_full[half]);
+        }
+        const int last_row = solo ? u.live - 1 : min(u.live, half * kHalf + kHalf) - 1;
+        const Span s = span_of_rows(p, u.v, u.tile, solo ? 0 : half * kHalf, last_row);  // of this half's rows
+        const RowView see = row_view(p, u.v, who);
+        for (int t = 0; t < n; ++t) {
+          ok = ok && mbar_wait_warp(&sm.s_full[half], (mine + t) & 1, gave_up);
+          tc_fence_after();
+          const int j = first + t * step;
+          const int tok = tile_token<kTile>(u.s, u.ta + j);
+          const uint32_t have = sm.have[(before + j) % kHave];
+          const bool whole = tile_whole<kTile>(s, tok) && have == 0xffu;
+          uint32_t x[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld(s_at + c * 32, x[c]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_wait(x[c]);
+          if (!whole) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int t0 = tok + c * 32;
+              uint32_t bits;
+              if (p.parents != nullptr) {
+                bits = tree_bits(p, u.v, who, t0);
+              } else {
+                auto below = [](int k) { return k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1u; };
+                bits = below(see.hi - t0) & (~below(see.lo - t0) | below(p.sinks - t0));
+              }
+              bits &= ((have >> (2 * c)) & 1 ? 0x0000ffffu : 0u) | ((have >> (2 * c + 1)) & 1 ? 0xffff0000u : 0u);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) x[c][e] = bits >> e & 1 ? x[c][e] : 0xff800000u;
+            }
+          }
+          float tops[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tops[c] = __uint_as_float(x[c][0]);
+#pragma unroll
+            for (int e = 1; e + 1 < 32; e += 2) tops[c] = max3(tops[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+            tops[c] = max3(tops[c], __uint_as_float(x[c][31]), __uint_as_float(x[c][31]));
+          }
+          const float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]) * scale;
+          if (!(top < INFINITY)) l = __uint_as_float(0x7fffffffu);  // a score that is no number, or infinite
+          const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float mn = fmaxf(m, top);
+            const float keep = mn == m ? 1.f : exp2_near(m - mn);
+            m = mn;
+            l *= keep;
+            if (t > 0) {
+#pragma unroll 1
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld(o_at + c * 32, o);
+                tmem_wait(o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tmem_st(o_at + c * 32, reinterpret_cast<uint32_t(&)[16]>(o[0]));
+                tmem_st(o_at + c * 32 + 16, reinterpret_cast<uint32_t(&)[16]>(o[16]));
+              }
+            }
+          }
+          const float ref = m > -INFINITY && m < INFINITY ? m - kLift : 0.f;
+          float2 sum[2] = {both(0.f), both(0.f)};
+          auto weights = [&](auto all_units) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t y[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float2 w = fma2(make_float2(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), both(scale), both(-ref));
+                if (decltype(all_units)::value && e % 8 >= 5) {
+                  w = exp2_poly(w);
+                } else {
+                  w.x = exp2_near(w.x);
+                  w.y = exp2_near(w.y);
+                }
+                sum[e & 1] = add2(sum[e & 1], w);
+                y[e] = pack_two<BF16>(w.x, w.y);
+              }
+              tmem_st(s_at + c * 16, y);
+              if (c & 1) {  // half of the tile's weights: their product may begin
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_full[half][c >> 1]);
+              }
+            }
+          };
+          // Weights of masked scores are 0, which the polynomial does not give.
+          if (whole)
+            weights(std::true_type());
+          else
+            weights(std::false_type());
+          sum[0] = add2(sum[0], sum[1]);
+          l += sum[0].x + sum[0].y;
+        }
+        ok = ok && mbar_wait_warp(&sm.o_full[half], ends & 1, gave_up);
+        tc_fence_after();
+        mine += n;
+        ++ends;
+      }
+      before += u.n;
+      if (!ok) l = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN, not stale memory
+
+      // ---- this half's share of the unit -------------------------------------------
+      auto place = [&](int64_t row, uint16_t*& dst, float*& lse) {  // of a row's result
+        const int64_t i = u.v.first + row / p.group, h = static_cast<int64_t>(u.head) * p.group + row % p.group;
+        dst = static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh;
+        lse = p.lse == nullptr ? nullptr : p.lse + i * p.nh * p.group + h;
+      };
+      auto put = [&](uint16_t* dst, const float(&o)[16], float inv) {
+        uint32_t y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = pack_two<BF16>(o[2 * e] * inv, o[2 * e + 1] * inv);
+        if ((reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+          reinterpret_cast<uint4*>(dst)[0] = make_uint4(y[0], y[1], y[2], y[3]);
+          reinterpret_cast<uint4*>(dst)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            dst[2 * e] = static_cast<uint16_t>(y[e]);
+            dst[2 * e + 1] = static_cast<uint16_t>(y[e] >> 16);
+          }
+        }
+      };
+      auto put_lse = [&](float* lse, float mx, float sum) {
+        if (lse != nullptr) *lse = sum > 0.f || sum != sum ? (mx - kLift + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+      };
+      const bool cut = u.ta > 0 || u.tb < u.len, split = cut || solo;
+      constexpr int kFloats = kHalf * (HD + 2);  // of one partial sum: [HD][128], maxima, sums
+      auto piece = [&](int64_t block, int which) {
+        return p.partial + ((2 * block + (u.wt > block * chunk ? 1 : 0)) * 2 + which) * kFloats;
+      };
+      float* part = piece(blockIdx.x, half);
+      if (active) {
+        uint16_t* dst = nullptr;
+        float* lse = nullptr;
+        if (on) place(row, dst, lse);
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        const bool odd_seen = n > 0 && *static_cast<volatile int*>(&sm.odd_seen);
+#pragma unroll 1
+        for (int d = 0; d < HD; d += 16) {
+          float o[16];
+          if (n > 0) {
+            uint32_t x[16];
+            tmem_ld(o_at + d, x);
+            tmem_wait(x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(x[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0.f;
+          }
+          if (odd_seen && on) {
+            float bad[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) bad[e] = 0.f;
+            odd_sum<BF16>(p, u, who, d, first, step, bad);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] += bad[e];
+          }
+          if (split) {
+            if (on) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) part[(d + e) * kHalf + r] = o[e];
+            }
+          } else if (on) {
+            put(dst + d, o, inv);
+          }
+        }
+        if (on) {
+          if (split) {
+            part[HD * kHalf + r] = m;
+            part[HD * kHalf + kHalf + r] = l;
+          } else {
+            put_lse(lse, m, l);
+          }
+        }
+      }
+      tc_fence_before();
+      if (split && active) {
+        const int64_t first_block = u.wt / chunk, last_block = (u.wt + u.len - 1) / chunk;
+        const int64_t slot0 = (2 * first_block + (u.wt > first_block * chunk ? 1 : 0)) * 2 + (solo ? 0 : half);
+        half_sync(half);
+        if (r == 0) {  // releases what the barrier has gathered
+          int ticket;
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + slot0) : "memory");
+          sm.last[half] = ticket == (last_block - first_block + 1) * (solo ? 2 : 1) - 1;
+        }
+        half_sync(half);
+        if (sm.last[half]) {
+          // Few rows leave several threads for each, which share its columns.  Four pieces' loads at a time.
+          const int rows = solo ? u.live : min(u.live - half * kHalf, kHalf);
+          const int span = rows > 64 ? 128 : rows > 32 ? 64 : 32, mine_row = r & (span - 1), cols = HD * span / kHalf;
+          const int pieces = static_cast<int>(last_block - first_block + 1) * (solo ? 2 : 1);
+          if (mine_row < rows) {
+            auto from = [&](int i) {
+              return (solo ? piece(first_block + (i >> 1), i & 1) : piece(first_block + i, half)) + mine_row;
+            };
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll 4
+            for (int i = 0; i < pieces; ++i) {
+              const float pm = __ldcg(from(i) + HD * kHalf), pl = __ldcg(from(i) + HD * kHalf + kHalf);
+              const float mn = fmaxf(mx, pm), ms = mn == -INFINITY ? 0.f : mn;
+              sum = sum * exp2_near(mx - ms) + pl * exp2_near(pm - ms);
+              mx = mn;
+            }
+            const float ms = mx == -INFINITY ? 0.f : mx, inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+            uint16_t* dst;
+            float* lse;
+            place(static_cast<int64_t>(u.tile) * kUnitRows + (solo ? 0 : half * kHalf) + mine_row, dst, lse);
+#pragma unroll 1
+            for (int d = r / span * cols, end = d + cols; d < end; d += 16) {
+              float o[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = 0.f;
+#pragma unroll 1
+              for (int i = 0; i < pieces; i += 4) {
+                float x[4][16], k[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  const float* src = from(min(i + z, pieces - 1));
+                  k[z] = __ldcg(src + HD * kHalf);
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) x[z][e] = __ldcg(src + (d + e) * kHalf);
+                }
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  k[z] = exp2_near(k[z] - ms);
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = i + z < pieces ? fmaf(x[z][e], k[z], o[e]) : o[e];
+                }
+              }
+              put(dst + d, o, inv);
+            }
+            if (r < span) put_lse(lse, mx, sum);
+          }
+          if (r == 0) p.counters[slot0] = 0;
+        }
+      }
+      half_sync(half);  // the unit is read
+    }
+  } else {
+    regs_down<88>();
+    if (warp == 8) {
+      // ---- loads ----------------------------------------------------------------------
+      constexpr int kPieces = HD / 64;
+      const int pages = kTile >> p.bs_log2, bs = 1 << p.bs_log2;
+      uint32_t g = 0, k_issued = 0, v_issued = 0;  // tiles so far
+      bool ok = true;
+      if (lane == 0) sm.walk[2] = walk;
+      const Unit& u = sm.unit[2];
+      while (ok) {
+        __syncwarp();
+        if (lane == 0) sm.more[2] = next_unit(p, plan, sm.walk[2], sm.unit[2]);
+        __syncwarp();
+        if (!sm.more[2]) break;
+        const int n = u.n, head = u.head;
+        const int32_t* table = p.tables + u.seq * p.table_stride;
+        auto find = [&](int j) {  // page `lane` of tile j
+          int page = -1;
+          if (j < n && lane < pages) {
+            const int tok = tile_token<kTile>(u.s, u.ta + j) + (lane << p.bs_log2);
+            if (tok < u.v.room) page = page_of(p, table, tok);
+          }
+          return page;
+        };
+        int page = find(0);
+        for (int j = 0; j < n; ++j, ++g) {
+          const int next_page = find(j + 1);
+          const uint32_t votes = __ballot_sync(0xffffffffu, page >= 0);
+          const uint32_t ks = g % kK, vs = g % kV;
+          ok = mbar_wait_warp_idle(&sm.k_empty[ks], ((g / kK) & 1) ^ 1, gave_up);
+          if (!ok) break;
+          if (lane == 0) {
+            uint32_t have = 0;  // in sixteens of tokens
+            for (int c = 0; c < 8; ++c) have |= (votes >> ((c * 16) >> p.bs_log2) & 1) << c;
+            sm.have[g % kHave] = have;
+            mbar_arrive_expect(&sm.k_full[ks], kBytes);
+          }
+          __syncwarp();
+          const int mine = __shfl_sync(0xffffffffu, page, lane / kPieces), piece = lane % kPieces;
+          const uint32_t to = piece * 16384 + (lane / kPieces) * bs * 128;
+          // a block that there is not: the loads fill zeros
+          if (lane < pages * kPieces) box_load(smem_addr(sm.k[ks]) + to, &k_map, piece * 64, head, 0, mine, &sm.k_full[ks]);
+          ++k_issued;
+          ok = mbar_wait_warp_idle(&sm.v_empty[vs], ((g / kV) & 1) ^ 1, gave_up);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect(&sm.v_full[vs], kBytes);
+          __syncwarp();
+          if (lane < pages * kPieces) box_load(smem_addr(sm.v[vs]) + to, &v_map, piece * 64, head, 0, mine, &sm.v_full[vs]);
+          ++v_issued;
+          page = next_page;
+        }
+      }
+      if (!ok) {  // the copies in flight end before the block does
+        auto landed = [&](uint64_t* full, uint32_t stages, uint32_t issued) {
+          for (uint32_t t = issued > stages ? issued - stages : 0; t < issued; ++t)
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[t % stages], (t / stages) & 1); ++i) {
+            }
+        };
+        landed(sm.k_full, kK, k_issued);
+        landed(sm.v_full, kV, v_issued);
+      }
+    } else if (warp >= 10) {
+      // ---- values that are no numbers ---------------------------------------------------
+      const int mine = warp - 10;
+      uint32_t g = 0;
+      bool ok = true;
+      if (lane == 0) sm.walk[3 + mine] = walk;
+      const Unit& u = sm.unit[3 + mine];
+      while (ok) {
+        __syncwarp();
+        if (lane == 0) sm.more[3 + mine] = next_unit(p, plan, sm.walk[3 + mine], sm.unit[3 + mine]);
+        __syncwarp();
+        if (!sm.more[3 + mine]) break;
+        const int n = u.n;
+        for (int j = 0; j < n; ++j, ++g) {
+          const uint32_t vs = g % kV;
+          ok = mbar_wait_warp_idle(&sm.v_full[vs], (g / kV) & 1, gave_up);
+          if (!ok) break;
+          if (!tile_whole<kTile>(u.s, tile_token<kTile>(u.s, u.ta + j))) {
+            uint4* v = reinterpret_cast<uint4*>(sm.v[vs]) + mine * (kBytes / 32);
+            bool odd = false;
+#pragma unroll 4
+            for (int i = lane; i < kBytes / 32; i += 32) {
+              uint4 w = v[i];
+              if (odd_two<BF16>(w.x) || odd_two<BF16>(w.y) || odd_two<BF16>(w.z) || odd_two<BF16>(w.w)) {
+                odd = true;
+                auto fine = [](uint32_t a) {
+                  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+                  return a & (((a & e) == e ? 0u : 0xffffu) | ((a & (e << 16)) == (e << 16) ? 0u : 0xffff0000u));
+                };
+                v[i] = make_uint4(fine(w.x), fine(w.y), fine(w.z), fine(w.w));
+              }
+            }
+            if (odd) *static_cast<volatile int*>(&sm.odd_seen) = 1;
+            fence_async_shared();
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&sm.v_clean[vs]);
+        }
+      }
+    } else if (lane == 0) {
+      // ---- the tensor cores -------------------------------------------------------
+      constexpr int kFormat = BF16 ? 1 : 0;
+      constexpr uint32_t kQk = instr_desc(kTile, 1, kFormat, false, false), kPv = instr_desc(HD, 1, kFormat, false, true);
+      // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
+      const uint64_t q_desc = smem_desc(smem_addr(sm.q), 16, 1024, 7), k_desc = smem_desc(smem_addr(sm.k), 16, 1024, 7);
+      const uint64_t v_desc = smem_desc(smem_addr(sm.v), 16384, 1024, 7);
+      constexpr uint32_t kBuffer = kBytes / 16;
+      uint32_t g = 0, done[2] = {0, 0}, begins[2] = {0, 0};  // done: tiles of each half so far
+      bool ok = true;
+      sm.walk[5] = walk;
+      const Unit& u = sm.unit[5];
+      auto scores = [&](int half, uint32_t tile, bool free_it) {
+        const uint32_t st = tile % kK;
+        const uint64_t qd = q_desc + half * kBuffer, kd = k_desc + st * kBuffer;
+        steps<HD / 16>([&](auto i) {
+          constexpr int ks = decltype(i)::value;
+          constexpr int at = (ks >> 2) * 1024 + (ks & 3) * 2;
+          mma_ss_f16<at, at>(tmem + half * 128, qd, kd, kQk, ks > 0);
+        });
+        tc_commit(&sm.s_full[half]);
+        if (free_it) tc_commit(&sm.k_empty[st]);
+      };
+      auto values = [&](int half, uint32_t tile, bool add, bool free_it) {  // waits for the weights, a half of them at a time
+        const uint64_t vd = v_desc + (tile % kV) * kBuffer;
+        if (!mbar_wait(&sm.p_full[half][0], done[half] & 1, gave_up)) return false;
+        tc_fence_after();
+        steps<4>([&](auto i) {
+          constexpr int ks = decltype(i)::value;
+          mma_ts_f16<ks * 8, ks * 128>(tmem + 256 + half * HD, tmem + half * 128, vd, kPv, add || ks > 0);
+        });
+        if (!mbar_wait(&sm.p_full[half][1], done[half] & 1, gave_up)) return false;
+        tc_fence_after();
+        steps<4>([&](auto i) {
+          constexpr int ks = decltype(i)::value + 4;
+          mma_ts_f16<ks * 8, ks * 128>(tmem + 256 + half * HD, tmem + half * 128, vd, kPv, 1);
+        });
+        ++done[half];
+        if (free_it) tc_commit(&sm.v_empty[tile % kV]);
+        return true;
+      };
+      auto k_there = [&](uint32_t tile) {
+        const bool fine = mbar_wait(&sm.k_full[tile % kK], (tile / kK) & 1, gave_up);
+        tc_fence_after();
+        return fine;
+      };
+      auto v_there = [&](uint32_t tile) {
+        const bool fine = mbar_wait(&sm.v_full[tile % kV], (tile / kV) & 1, gave_up) && mbar_wait(&sm.v_clean[tile % kV], (tile / kV) & 1, gave_up);
+        tc_fence_after();
+        return fine;
+      };
+      while (ok && next_unit(p, plan, sm.walk[5], sm.unit[5])) {
+        const int n = u.n;
+        if (n == 0) continue;
+        if (u.solo) {
+          const int halves = n > 1 ? 2 : 1;
+          for (int half = 0; half < halves && ok; ++half) {
+            ok = mbar_wait(&sm.q_full[half], begins[half]++ & 1, gave_up) && k_there(g + half);
+            if (ok) scores(half, g + half, true);
+          }
+          for (int j = 0; j < n && ok; ++j) {
+            const int half = j & 1;
+            ok = v_there(g + j) && values(half, g + j, j > 1, true);
+            if (!ok) break;
+            if (j + 2 < n) {
+              ok = k_there(g + j + 2);
+              if (ok) scores(half, g + j + 2, true);
+            } else {
+              tc_commit(&sm.o_full[half]);
+            }
+          }
+        } else {
+          ok = k_there(g);
+          for (int half = 0; half < 2 && ok; ++half) {
+            ok = mbar_wait(&sm.q_full[half], begins[half]++ & 1, gave_up);
+            tc_fence_after();
+            if (ok) scores(half, g, half == 1);
+          }
+          for (int j = 0; j < n && ok; ++j) {
+            ok = v_there(g + j);
+            for (int half = 0; half < 2 && ok; ++half) {
+              ok = values(half, g + j, j > 0, half == 1);
+              if (!ok) break;
+              if (j + 1 < n) {
+                ok = k_there(g + j + 1);
+                if (ok) scores(half, g + j + 1, half == 1);
+              } else {
+                tc_commit(&sm.o_full[half]);
+              }
+            }
+          }
+        }
+        g += n;
+      }
+      if (!ok) {  // let what was issued end before the TMEM is given back
+        tc_commit(&sm.spare);
+        for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_free<512>(tmem);
+  }
+}
+
+// Row tiles of all sequences, at most.
+int64_t row_tiles(const PagedParams& p) { return static_cast<int64_t>(p.num_rows) * p.group / kUnitRows + p.num_seqs; }
+
+template <int HD, bool BF16>
+int launch(const PagedParams& p, const char* name, const CUtensorMap& k, const CUtensorMap& v, Plan* plan, cudaStream_t st) {
+  constexpr int kBytes = sizeof(TcSmem<HD>);
+  static_assert(kBytes <= 227 * 1024, "shared memory of a block");
+  const auto kernel = paged_tc_kernel<HD, BF16>;
+  static bool ready[kPagedDevices] = {};
+  if (int rc = paged_prepare(name, kernel, kBytes, ready)) return rc;
+  const int items = static_cast<int>(row_tiles(p));
+  if (int rc = launch_pdl(name, paged_plan_kernel, dim3(1), dim3(1024), 0, st, p, plan, items)) return rc;
+  const int sms = sm_count();
+  return launch_pdl(name, kernel, dim3(sms < kMaxGrid ? sms : kMaxGrid), dim3(kThreads), kBytes, st, p, k, v, static_cast<const Plan*>(plan), items);
+}
+
+}  // namespace
+
+int64_t paged_tc_partial_bytes() { return static_cast<int64_t>(4 * kMaxGrid) * kHalf * (128 + 2) * 4; }
+int64_t paged_tc_plan_bytes() { return sizeof(Plan); }
+int64_t paged_tc_counters() { return 4 * kMaxGrid; }
+bool paged_tc_fits(const PagedParams& p) { return row_tiles(p) <= kMaxItems; }
+
+bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool bf16,
+               int tokens) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  if (encode == nullptr) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found);
+    if (e != cudaSuccess || fn == nullptr) {
+      (void)cudaGetLastError();
+      return false;
+    }
+    encode = reinterpret_cast<Encode>(fn);
+  }
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(nh), static_cast<cuuint64_t>(bs),
+                              static_cast<cuuint64_t>(num_blocks)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(st) * 2, static_cast<cuuint64_t>(sb) * 2};
+  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(tokens), 1}, each[4] = {1, 1, 1, 1};
+  const CUresult rc = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t*>(base), dims,
+                             strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return rc == CUDA_SUCCESS;
+}
+
+int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* name, void* plan, cudaStream_t st, bool* taken) {
+  CUtensorMap k, v;
+  const int bs = 1 << p.bs_log2;
+  *taken = p.num_blocks > 0 && paged_map(&k, p.key, p.k_sb, p.k_st, p.k_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs) &&
+           paged_map(&v, p.value, p.v_sb, p.v_st, p.v_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs);
+  if (!*taken) return MAK_OK;
+  Plan* at = static_cast<Plan*>(plan);
+  if (head_dim == 64) return bf16 ? launch<64, true>(p, name, k, v, at, st) : launch<64, false>(p, name, k, v, at, st);
+  return bf16 ? launch<128, true>(p, name, k, v, at, st) : launch<128, false>(p, name, k, v, at, st);
+}
+
+}  // namespace mak

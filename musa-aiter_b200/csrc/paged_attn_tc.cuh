@@ -1,0 +1,19 @@
+// The kernel for many rows of the attention over paged 16-bit caches, as its entry point calls it.
+#pragma once
+
+#include "paged_attn.cuh"
+
+namespace mak {
+
+int64_t paged_tc_partial_bytes();
+int64_t paged_tc_plan_bytes();
+int64_t paged_tc_counters();
+bool paged_tc_fits(const PagedParams& p);
+// `taken`: false where the strides of a cache make no tensor map; nothing was launched then.
+int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* name, void* plan, cudaStream_t st, bool* taken);
+// A plane [num_blocks][block_size][num_heads][head_dim] as boxes of `tokens` tokens of one head, 64 columns of them, lines of
+// 128 bytes swizzled.
+bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool bf16,
+               int tokens);
+
+}  // namespace mak
