@@ -12,13 +12,13 @@
 // smallest largest relative error on [-1/2, 1/2], 2.6e-6 (coefficients by exchange of extrema, as Remez has it).
 //
 // A block takes 256 rows of one cache head (heads of the group next to one another, so a K / V tile serves all of them) as
-// two halves of 128 and walks the tokens in tiles of 128; of a unit with 128 rows or fewer each half takes every other
+// two halves of 128 and walks the tokens in tiles of 64, with two places for each half's scores: while those of one tile
+// are exponentiated the tensor cores make the next ones and multiply the last weights.  Of a unit with 128 rows or fewer each half takes every other
 // tile instead, and the two are joined.  Roles:
 //   warps 0-3, 4-7   softmax of half 0 / 1, a thread per row (TMEM lane)
 //   warp 8           page ids and TMA loads
 //   warp 9           one thread issues all tcgen05.mma
 //   warps 10, 11     values in tiles that not every row sees whole: infinite and NaN ones become 0 there
-// While one half's scores are exponentiated the tensor cores work for the other.
 //
 // What a row does not see reaches none of its sums: its weights there are 0, and 0 times a value that is no number is
 // kept out by warps 10 and 11; the rows that do see such a value get it with their results (odd_sum).
@@ -35,16 +35,17 @@
 namespace mak {
 namespace {
 
-constexpr int kTile = 128;      // tokens per step
+constexpr int kTile = 64;       // tokens per step
 constexpr int kHalf = 128;      // rows of a half
 constexpr int kUnitRows = 256;  // rows of a unit
 constexpr int kThreads = 384;
+constexpr int kPolyOf8 = 3;     // pairs of weights of each eight that the polynomial takes
 constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolerated
-constexpr int kUnitCost = 4;    // a unit's beginning and end, in tiles
-constexpr int kMinChunk = 4;    // steps of work that are worth another block
+constexpr int kUnitCost = 8;    // a unit's beginning and end, in tiles
+constexpr int kMinChunk = 8;    // steps of work that are worth another block
 constexpr int kMaxGrid = 148;
 constexpr int kMaxItems = 1 << 16;
-constexpr int kHave = 8;
+constexpr int kHave = 16;       // tiles whose pages are remembered
 
 // What the planning launch leaves: unit lengths added up over the row tiles, and whose they are.
 struct Plan {
@@ -185,6 +186,13 @@ __device__ __forceinline__ void steps(F f) {
   steps_of<N>(f, std::make_integer_sequence<int, N>());
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is != 0;
+}
+
 __device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -225,12 +233,12 @@ __device__ __forceinline__ float2 exp2_poly(float2 y) {
 
 template <int HD>
 struct TcSmem {
-  static constexpr int kBytes = kTile * HD * 2;  // of a tile of K, V or q: HD / 64 pieces of [128][64], lines of 128 bytes swizzled
-  static constexpr int kK = HD == 64 ? 4 : 2, kV = HD == 64 ? 4 : 3;  // tiles of K and of V
-  alignas(1024) uint8_t q[2][kBytes];
+  static constexpr int kBytes = kTile * HD * 2;      // of a tile of K or V: HD / 64 pieces of [64][64], lines of 128 bytes swizzled
+  static constexpr int kK = HD == 64 ? 8 : 5, kV = HD == 64 ? 8 : 5;  // tiles of K and of V
+  alignas(1024) uint8_t q[2][kHalf * HD * 2];  // pieces of [128][64]
   alignas(1024) uint8_t k[kK][kBytes];
   alignas(1024) uint8_t v[kV][kBytes];
-  alignas(8) uint64_t q_full[2], k_full[kK], k_empty[kK], v_full[kV], v_clean[kV], v_empty[kV], s_full[2], p_full[2][2], o_full[2], spare;
+  alignas(8) uint64_t q_full[2], k_full[kK], k_empty[kK], v_full[kV], v_clean[kV], v_empty[kV], s_full[2][2], p_full[2][2], o_full[2][2], spare;
   Walk walk[6];
   Unit unit[6];
   int more[6];
@@ -278,7 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kBytes = Sm::kBytes, kK = Sm::kK, kV = Sm::kV;
   extern __shared__ __align__(1024) uint8_t raw[];
   Sm& sm = *reinterpret_cast<Sm*>(raw);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // the same for all lanes, as the compiler sees it
   pdl_wait();
   pdl_trigger();
 
@@ -316,10 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kV; ++i) mbar_init(&sm.v_full[i], 1), mbar_init(&sm.v_clean[i], 2), mbar_init(&sm.v_empty[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.q_full[i], 4);
-      mbar_init(&sm.s_full[i], 1);
-      mbar_init(&sm.p_full[i][0], 4);
-      mbar_init(&sm.p_full[i][1], 4);
-      mbar_init(&sm.o_full[i], 1);
+      for (int b = 0; b < 2; ++b) mbar_init(&sm.s_full[i][b], 1), mbar_init(&sm.p_full[i][b], 4), mbar_init(&sm.o_full[i][b], 1);
     }
     mbar_init_fence();
   }
@@ -340,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t o_at = tmem + lanes + 256 + half * HD;
     const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);  // not 0: masked scores are -inf
     const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
-    uint32_t before = 0, mine = 0, ends = 0;  // tiles of all units so far, of this half, and how many units had tiles for it
+    uint32_t before = 0, mine = 0, ends = 0, ends2 = 0;  // tiles of all units and of this half, units with one and with two of these
     bool ok = true;
     if (r == 0) sm.walk[half] = walk;
     const Unit& u = sm.unit[half];
@@ -375,21 +381,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int last_row = solo ? u.live - 1 : min(u.live, half * kHalf + kHalf) - 1;
         const Span s = span_of_rows(p, u.v, u.tile, solo ? 0 : half * kHalf, last_row);  // of this half's rows
         const RowView see = row_view(p, u.v, who);
-        for (int t = 0; t < n; ++t) {
-          ok = ok && mbar_wait_warp(&sm.s_full[half], (mine + t) & 1, gave_up);
+        for (int t = 0; t < n; ++t, ++mine) {
+          const uint32_t place_at = s_at + (mine & 1) * 64;  // of the scores, and of the weights over them
+          ok = ok && mbar_wait_warp(&sm.s_full[half][mine & 1], (mine >> 1) & 1, gave_up);
           tc_fence_after();
           const int j = first + t * step;
           const int tok = tile_token<kTile>(u.s, u.ta + j);
           const uint32_t have = sm.have[(before + j) % kHave];
-          const bool whole = tile_whole<kTile>(s, tok) && have == 0xffu;
-          uint32_t x[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld(s_at + c * 32, x[c]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_wait(x[c]);
+          const bool whole = tile_whole<kTile>(s, tok) && have == 0xfu;
+          uint32_t x[2][32];
+          tmem_ld(place_at, x[0]);
+          tmem_ld(place_at + 32, x[1]);
+          tmem_wait(x[0]);
+          tmem_wait(x[1]);
           if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
               const int t0 = tok + c * 32;
               uint32_t bits;
               if (p.parents != nullptr) {
@@ -406,10 +413,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           float tops[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            tops[c] = __uint_as_float(x[c][0]);
+            const uint32_t* at = &x[c >> 1][(c & 1) * 16];
+            tops[c] = max3(__uint_as_float(at[0]), __uint_as_float(at[1]), __uint_as_float(at[15]));
 #pragma unroll
-            for (int e = 1; e + 1 < 32; e += 2) tops[c] = max3(tops[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
-            tops[c] = max3(tops[c], __uint_as_float(x[c][31]), __uint_as_float(x[c][31]));
+            for (int e = 2; e < 14; e += 2) tops[c] = max3(tops[c], __uint_as_float(at[e]), __uint_as_float(at[e + 1]));
+            tops[c] = max3(tops[c], __uint_as_float(at[14]), __uint_as_float(at[14]));
           }
           const float top = max3(max3(tops[0], tops[1], tops[2]), tops[3], tops[3]) * scale;
           if (!(top < INFINITY)) l = __uint_as_float(0x7fffffffu);  // a score that is no number, or infinite
@@ -420,15 +428,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             m = mn;
             l *= keep;
             if (t > 0) {
+              // The last weights' product: the next scores come after it.
+              ok = ok && (t + 1 < n ? mbar_wait_warp(&sm.s_full[half][(mine + 1) & 1], ((mine + 1) >> 1) & 1, gave_up)
+                                    : mbar_wait_warp(&sm.o_full[half][1], ends2 & 1, gave_up));
+              tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld(o_at + c * 32, o);
+              for (int c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld(o_at + c * 16, o);
                 tmem_wait(o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                tmem_st(o_at + c * 32, reinterpret_cast<uint32_t(&)[16]>(o[0]));
-                tmem_st(o_at + c * 32 + 16, reinterpret_cast<uint32_t(&)[16]>(o[16]));
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tmem_st(o_at + c * 16, o);
               }
             }
           }
@@ -436,12 +447,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           float2 sum[2] = {both(0.f), both(0.f)};
           auto weights = [&](auto all_units) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
               uint32_t y[16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 float2 w = fma2(make_float2(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), both(scale), both(-ref));
-                if (decltype(all_units)::value && e % 8 >= 5) {
+                if (decltype(all_units)::value && e % 8 >= 8 - kPolyOf8) {
                   w = exp2_poly(w);
                 } else {
                   w.x = exp2_near(w.x);
@@ -450,13 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 sum[e & 1] = add2(sum[e & 1], w);
                 y[e] = pack_two<BF16>(w.x, w.y);
               }
-              tmem_st(s_at + c * 16, y);
-              if (c & 1) {  // half of the tile's weights: their product may begin
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_full[half][c >> 1]);
-              }
+              tmem_st(place_at + c * 16, y);
             }
           };
           // Weights of masked scores are 0, which the polynomial does not give.
@@ -464,13 +469,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             weights(std::true_type());
           else
             weights(std::false_type());
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.p_full[half][mine & 1]);
           sum[0] = add2(sum[0], sum[1]);
           l += sum[0].x + sum[0].y;
         }
-        ok = ok && mbar_wait_warp(&sm.o_full[half], ends & 1, gave_up);
+        ok = ok && mbar_wait_warp(&sm.o_full[half][0], ends & 1, gave_up);
         tc_fence_after();
-        mine += n;
         ++ends;
+        if (n > 1) ++ends2;
       }
       before += u.n;
       if (!ok) l = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN, not stale memory
@@ -618,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 8) {
       // ---- loads ----------------------------------------------------------------------
       constexpr int kPieces = HD / 64;
-      const int pages = kTile >> p.bs_log2, bs = 1 << p.bs_log2;
+      const int bs = 1 << p.bs_log2, box = min(bs, kTile), pages = kTile / box;
       uint32_t g = 0, k_issued = 0, v_issued = 0;  // tiles so far
       bool ok = true;
       if (lane == 0) sm.walk[2] = walk;
@@ -633,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto find = [&](int j) {  // page `lane` of tile j
           int page = -1;
           if (j < n && lane < pages) {
-            const int tok = tile_token<kTile>(u.s, u.ta + j) + (lane << p.bs_log2);
+            const int tok = tile_token<kTile>(u.s, u.ta + j) + lane * box;
             if (tok < u.v.room) page = page_of(p, table, tok);
           }
           return page;
@@ -647,21 +656,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           if (lane == 0) {
             uint32_t have = 0;  // in sixteens of tokens
-            for (int c = 0; c < 8; ++c) have |= (votes >> ((c * 16) >> p.bs_log2) & 1) << c;
+            for (int c = 0; c < kTile / 16; ++c) have |= (votes >> (c * 16 / box) & 1) << c;
             sm.have[g % kHave] = have;
             mbar_arrive_expect(&sm.k_full[ks], kBytes);
           }
           __syncwarp();
           const int mine = __shfl_sync(0xffffffffu, page, lane / kPieces), piece = lane % kPieces;
-          const uint32_t to = piece * 16384 + (lane / kPieces) * bs * 128;
+          const uint32_t to = piece * (kTile * 128) + (lane / kPieces) * box * 128;
+          const int inside = tile_token<kTile>(u.s, u.ta + j) & (bs - 1);  // of a page that holds several tiles
           // a block that there is not: the loads fill zeros
-          if (lane < pages * kPieces) box_load(smem_addr(sm.k[ks]) + to, &k_map, piece * 64, head, 0, mine, &sm.k_full[ks]);
+          if (lane < pages * kPieces) box_load(smem_addr(sm.k[ks]) + to, &k_map, piece * 64, head, inside, mine, &sm.k_full[ks]);
           ++k_issued;
           ok = mbar_wait_warp_idle(&sm.v_empty[vs], ((g / kV) & 1) ^ 1, gave_up);
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect(&sm.v_full[vs], kBytes);
           __syncwarp();
-          if (lane < pages * kPieces) box_load(smem_addr(sm.v[vs]) + to, &v_map, piece * 64, head, 0, mine, &sm.v_full[vs]);
+          if (lane < pages * kPieces) box_load(smem_addr(sm.v[vs]) + to, &v_map, piece * 64, head, inside, mine, &sm.v_full[vs]);
           ++v_issued;
           page = next_page;
         }
@@ -708,108 +718,128 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             if (odd) *static_cast<volatile int*>(&sm.odd_seen) = 1;
-            fence_async_shared();
-            __syncwarp();
           }
+          fence_async_shared();
+          __syncwarp();
           if (lane == 0) mbar_arrive(&sm.v_clean[vs]);
         }
       }
-    } else if (lane == 0) {
+    } else {
       // ---- the tensor cores -------------------------------------------------------
+      // The whole warp walks, so that all addresses are known to be the same for its lanes; one of them issues.
       constexpr int kFormat = BF16 ? 1 : 0;
       constexpr uint32_t kQk = instr_desc(kTile, 1, kFormat, false, false), kPv = instr_desc(HD, 1, kFormat, false, true);
       // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
       const uint64_t q_desc = smem_desc(smem_addr(sm.q), 16, 1024, 7), k_desc = smem_desc(smem_addr(sm.k), 16, 1024, 7);
-      const uint64_t v_desc = smem_desc(smem_addr(sm.v), 16384, 1024, 7);
-      constexpr uint32_t kBuffer = kBytes / 16;
-      uint32_t g = 0, done[2] = {0, 0}, begins[2] = {0, 0};  // done: tiles of each half so far
+      const uint64_t v_desc = smem_desc(smem_addr(sm.v), kTile * 128, 1024, 7);
+      constexpr uint32_t kBuffer = kBytes / 16, kRows = kHalf * HD * 2 / 16;
+      struct Ring {
+        uint32_t at, phase;
+      } kr = {0, 0}, vr = {0, 0};
+      uint32_t made[2] = {0, 0}, done[2] = {0, 0}, begins[2] = {0, 0};  // scores made and weights used of each half so far
       bool ok = true;
-      sm.walk[5] = walk;
-      const Unit& u = sm.unit[5];
-      auto scores = [&](int half, uint32_t tile, bool free_it) {
-        const uint32_t st = tile % kK;
-        const uint64_t qd = q_desc + half * kBuffer, kd = k_desc + st * kBuffer;
-        steps<HD / 16>([&](auto i) {
-          constexpr int ks = decltype(i)::value;
-          constexpr int at = (ks >> 2) * 1024 + (ks & 3) * 2;
-          mma_ss_f16<at, at>(tmem + half * 128, qd, kd, kQk, ks > 0);
-        });
-        tc_commit(&sm.s_full[half]);
-        if (free_it) tc_commit(&sm.k_empty[st]);
+      if (lane == 0) sm.walk[5] = walk;
+      auto next_k = [&]() {
+        if (++kr.at == kK) kr.at = 0, kr.phase ^= 1;
       };
-      auto values = [&](int half, uint32_t tile, bool add, bool free_it) {  // waits for the weights, a half of them at a time
-        const uint64_t vd = v_desc + (tile % kV) * kBuffer;
-        if (!mbar_wait(&sm.p_full[half][0], done[half] & 1, gave_up)) return false;
+      auto next_v = [&]() {
+        if (++vr.at == kV) vr.at = 0, vr.phase ^= 1;
+      };
+      auto scores = [&](auto which, bool free_it) {
+        constexpr int half = decltype(which)::value;
+        const uint32_t at = made[half] & 1;
+        if (elect_one()) {
+          const uint64_t qd = q_desc + half * kRows, kd = k_desc + kr.at * kBuffer;
+          steps<HD / 16>([&](auto i) {
+            constexpr int ks = decltype(i)::value;
+            mma_ss_f16<(ks >> 2) * (kHalf * 8) + (ks & 3) * 2, (ks >> 2) * (kTile * 8) + (ks & 3) * 2>(tmem + half * 128 + at * 64, qd, kd, kQk, ks > 0);
+          });
+          tc_commit(&sm.s_full[half][at]);
+          if (free_it) tc_commit(&sm.k_empty[kr.at]);
+        }
+        ++made[half];
+      };
+      auto values = [&](auto which, bool add, bool free_it, bool last, bool last_but_one) {
+        constexpr int half = decltype(which)::value;
+        const uint32_t at = done[half] & 1;
+        ok = mbar_wait_warp(&sm.p_full[half][at], (done[half] >> 1) & 1, gave_up);
         tc_fence_after();
-        steps<4>([&](auto i) {
-          constexpr int ks = decltype(i)::value;
-          mma_ts_f16<ks * 8, ks * 128>(tmem + 256 + half * HD, tmem + half * 128, vd, kPv, add || ks > 0);
-        });
-        if (!mbar_wait(&sm.p_full[half][1], done[half] & 1, gave_up)) return false;
-        tc_fence_after();
-        steps<4>([&](auto i) {
-          constexpr int ks = decltype(i)::value + 4;
-          mma_ts_f16<ks * 8, ks * 128>(tmem + 256 + half * HD, tmem + half * 128, vd, kPv, 1);
-        });
+        if (!ok) return;
+        if (elect_one()) {
+          const uint64_t vd = v_desc + vr.at * kBuffer;
+          steps<kTile / 16>([&](auto i) {
+            constexpr int ks = decltype(i)::value;
+            mma_ts_f16<ks * 8, ks * 128>(tmem + 256 + half * HD, tmem + half * 128 + at * 64, vd, kPv, add || ks > 0);
+          });
+          if (last || last_but_one) tc_commit(&sm.o_full[half][last ? 0 : 1]);
+          if (free_it) tc_commit(&sm.v_empty[vr.at]);
+        }
         ++done[half];
-        if (free_it) tc_commit(&sm.v_empty[tile % kV]);
-        return true;
       };
-      auto k_there = [&](uint32_t tile) {
-        const bool fine = mbar_wait(&sm.k_full[tile % kK], (tile / kK) & 1, gave_up);
-        tc_fence_after();
-        return fine;
-      };
-      auto v_there = [&](uint32_t tile) {
-        const bool fine = mbar_wait(&sm.v_full[tile % kV], (tile / kV) & 1, gave_up) && mbar_wait(&sm.v_clean[tile % kV], (tile / kV) & 1, gave_up);
-        tc_fence_after();
-        return fine;
-      };
-      while (ok && next_unit(p, plan, sm.walk[5], sm.unit[5])) {
-        const int n = u.n;
+      using H0 = std::integral_constant<int, 0>;
+      using H1 = std::integral_constant<int, 1>;
+      while (true) {
+        __syncwarp();
+        if (lane == 0) sm.more[5] = next_unit(p, plan, sm.walk[5], sm.unit[5]);
+        __syncwarp();
+        if (!__shfl_sync(0xffffffffu, sm.more[5], 0) || !__all_sync(0xffffffffu, ok)) break;
+        // Of each half the scores of two tiles, then always the values of one and the scores of the next but one.
+        const int n = __shfl_sync(0xffffffffu, sm.unit[5].n, 0);
+        const bool solo = __shfl_sync(0xffffffffu, static_cast<int>(sm.unit[5].solo), 0);
         if (n == 0) continue;
-        if (u.solo) {
-          const int halves = n > 1 ? 2 : 1;
-          for (int half = 0; half < halves && ok; ++half) {
-            ok = mbar_wait(&sm.q_full[half], begins[half]++ & 1, gave_up) && k_there(g + half);
-            if (ok) scores(half, g + half, true);
-          }
-          for (int j = 0; j < n && ok; ++j) {
-            const int half = j & 1;
-            ok = v_there(g + j) && values(half, g + j, j > 1, true);
+        ok = mbar_wait_warp(&sm.q_full[0], begins[0]++ & 1, gave_up);
+        if (!solo || n > 1) ok = ok && mbar_wait_warp(&sm.q_full[1], begins[1]++ & 1, gave_up);
+        tc_fence_after();
+        if (solo) {
+          for (int j = 0; j < n + 4 && ok; j += 2) {  // the values of tiles j - 4 and j - 3, the scores of j and j + 1
+            if (j >= 4) {
+              ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up);
+              if (!ok) break;
+              values(H0(), j > 4, true, j - 2 >= n, j >= n && j - 2 < n);
+              next_v();
+            }
             if (!ok) break;
-            if (j + 2 < n) {
-              ok = k_there(g + j + 2);
-              if (ok) scores(half, g + j + 2, true);
-            } else {
-              tc_commit(&sm.o_full[half]);
+            if (j < n) {
+              ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
+              if (!ok) break;
+              scores(H0(), true);
+              next_k();
+            }
+            if (j >= 4 && j - 3 < n) {
+              ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up);
+              if (!ok) break;
+              values(H1(), j > 4, true, j - 1 >= n, j + 1 >= n && j - 1 < n);
+              next_v();
+            }
+            if (!ok) break;
+            if (j + 1 < n) {
+              ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
+              if (!ok) break;
+              scores(H1(), true);
+              next_k();
             }
           }
         } else {
-          ok = k_there(g);
-          for (int half = 0; half < 2 && ok; ++half) {
-            ok = mbar_wait(&sm.q_full[half], begins[half]++ & 1, gave_up);
-            tc_fence_after();
-            if (ok) scores(half, g, half == 1);
-          }
-          for (int j = 0; j < n && ok; ++j) {
-            ok = v_there(g + j);
-            for (int half = 0; half < 2 && ok; ++half) {
-              ok = values(half, g + j, j > 0, half == 1);
-              if (!ok) break;
-              if (j + 1 < n) {
-                ok = k_there(g + j + 1);
-                if (ok) scores(half, g + j + 1, half == 1);
-              } else {
-                tc_commit(&sm.o_full[half]);
-              }
-            }
+          for (int j = 0; j < n + 2; ++j) {  // the values of tile j - 2, the scores of tile j
+            const bool v = j >= 2, k = j < n;
+            if (v) ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up);
+            if (k && ok) ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
+            if (!ok) break;
+            if (v) values(H0(), j > 2, false, j - 1 >= n, !k && j - 1 < n);
+            if (!ok) break;
+            if (k) scores(H0(), false);
+            if (v) values(H1(), j > 2, true, j - 1 >= n, !k && j - 1 < n);
+            if (!ok) break;
+            if (k) scores(H1(), true);
+            if (v) next_v();
+            if (k) next_k();
           }
         }
-        g += n;
       }
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) {  // let what was issued end before the TMEM is given back
-        tc_commit(&sm.spare);
+        if (elect_one()) tc_commit(&sm.spare);
+        __syncwarp();
         for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
         }
       }
@@ -875,8 +905,8 @@ bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, i
 int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* name, void* plan, cudaStream_t st, bool* taken) {
   CUtensorMap k, v;
   const int bs = 1 << p.bs_log2;
-  *taken = p.num_blocks > 0 && paged_map(&k, p.key, p.k_sb, p.k_st, p.k_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs) &&
-           paged_map(&v, p.value, p.v_sb, p.v_st, p.v_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs);
+  *taken = p.num_blocks > 0 && paged_map(&k, p.key, p.k_sb, p.k_st, p.k_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs < kTile ? bs : kTile) &&
+           paged_map(&v, p.value, p.v_sb, p.v_st, p.v_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs < kTile ? bs : kTile);
   if (!*taken) return MAK_OK;
   Plan* at = static_cast<Plan*>(plan);
   if (head_dim == 64) return bf16 ? launch<64, true>(p, name, k, v, at, st) : launch<64, false>(p, name, k, v, at, st);
