@@ -16,12 +16,12 @@
 // are exponentiated the tensor cores make the next ones and multiply the last weights.  Of a unit with 128 rows or fewer each half takes every other
 // tile instead, and the two are joined.  Roles:
 //   warps 0-3, 4-7   softmax of half 0 / 1, a thread per row (TMEM lane)
-//   warp 8           page ids and TMA loads
-//   warp 9           one thread issues all tcgen05.mma
-//   warps 10, 11     values in tiles that not every row sees whole: infinite and NaN ones become 0 there
+//   warps 8, 9       page ids and TMA loads of K / V
+//   warps 10, 11     a thread issues all tcgen05.mma of half 0 / 1: while one waits the other's products run
+//   warps 12-15      values in tiles that not every row sees whole: infinite and NaN ones become 0 there
 //
 // What a row does not see reaches none of its sums: its weights there are 0, and 0 times a value that is no number is
-// kept out by warps 10 and 11; the rows that do see such a value get it with their results (odd_sum).
+// kept out by warps 12-15; the rows that do see such a value get it with their results (odd_sum).
 //
 // Work.  All (row tile, head) units laid end to end, each as long as the tiles it sees, are cut into equal runs, one per
 // block; a small launch before this one adds up the lengths.  A unit cut by that leaves partial sums, and the last half to
@@ -38,7 +38,7 @@ namespace {
 constexpr int kTile = 64;       // tokens per step
 constexpr int kHalf = 128;      // rows of a half
 constexpr int kUnitRows = 256;  // rows of a unit
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kPolyOf8 = 3;     // pairs of weights of each eight that the polynomial takes
 constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolerated
 constexpr int kUnitCost = 8;    // a unit's beginning and end, in tiles
@@ -238,10 +238,10 @@ struct TcSmem {
   alignas(1024) uint8_t q[2][kHalf * HD * 2];  // pieces of [128][64]
   alignas(1024) uint8_t k[kK][kBytes];
   alignas(1024) uint8_t v[kV][kBytes];
-  alignas(8) uint64_t q_full[2], k_full[kK], k_empty[kK], v_full[kV], v_clean[kV], v_empty[kV], s_full[2][2], p_full[2][2], o_full[2][2], spare;
-  Walk walk[6];
-  Unit unit[6];
-  int more[6];
+  alignas(8) uint64_t q_full[2], k_full[kK], k_empty[kK], v_full[kV], v_clean[kV], v_empty[kV], s_full[2][2], p_full[2][2], o_full[2][2], spare[2];
+  Walk walk[10];  // of the halves' softmax, the loads, the cleaning warps, the issuing ones
+  Unit unit[10];
+  int more[10];
   uint32_t have[kHave];  // bit c: 16 tokens c of a tile have a page
   uint32_t tmem;
   int gave_up, last[2];
@@ -320,16 +320,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     sm.gave_up = 0;
     sm.odd_seen = 0;
-    mbar_init(&sm.spare, 1);
-    for (int i = 0; i < kK; ++i) mbar_init(&sm.k_full[i], 1), mbar_init(&sm.k_empty[i], 1);
-    for (int i = 0; i < kV; ++i) mbar_init(&sm.v_full[i], 1), mbar_init(&sm.v_clean[i], 2), mbar_init(&sm.v_empty[i], 1);
+    for (int i = 0; i < kK; ++i) mbar_init(&sm.k_full[i], 1), mbar_init(&sm.k_empty[i], 2);
+    for (int i = 0; i < kV; ++i) mbar_init(&sm.v_full[i], 1), mbar_init(&sm.v_clean[i], 4), mbar_init(&sm.v_empty[i], 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sm.q_full[i], 4);
+      mbar_init(&sm.spare[i], 1);
       for (int b = 0; b < 2; ++b) mbar_init(&sm.s_full[i][b], 1), mbar_init(&sm.p_full[i][b], 4), mbar_init(&sm.o_full[i][b], 1);
     }
     mbar_init_fence();
   }
-  if (warp == 9) tmem_alloc<512>(&sm.tmem);
+  if (warp == 10) tmem_alloc<512>(&sm.tmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* gave_up = &sm.gave_up;
 
   if (warp < 8) {
-    regs_up<208>();  // with 88 below: what the block was launched with
+    regs_up<184>();  // with 72 below: what the block was launched with
     // ---- softmax ----------------------------------------------------------------
     const int half = warp >> 2;
     const int r = tid & 127;
@@ -623,90 +623,92 @@ __global__ void __launch_bounds__(kThreads, 1)
       half_sync(half);  // the unit is read
     }
   } else {
-    regs_down<88>();
-    if (warp == 8) {
+    regs_down<72>();
+    if (warp < 10) {
       // ---- loads ----------------------------------------------------------------------
-      constexpr int kPieces = HD / 64;
+      constexpr int kPieces = HD / 64, kStages = kK;
+      static_assert(kK == kV, "one loop for both");
+      const bool is_v = warp == 9;
+      const int role = warp - 6;
       const int bs = 1 << p.bs_log2, box = min(bs, kTile), pages = kTile / box;
-      uint32_t g = 0, k_issued = 0, v_issued = 0;  // tiles so far
+      uint64_t *const full = is_v ? sm.v_full : sm.k_full, *const empty = is_v ? sm.v_empty : sm.k_empty;
+      const uint32_t ring = smem_addr(is_v ? sm.v : sm.k);
+      const void* map = is_v ? &v_map : &k_map;
+      uint32_t g = 0, stage = 0, phase = 1;  // tiles so far
       bool ok = true;
-      if (lane == 0) sm.walk[2] = walk;
-      const Unit& u = sm.unit[2];
+      if (lane == 0) sm.walk[role] = walk;
+      const Unit& u = sm.unit[role];
       while (ok) {
         __syncwarp();
-        if (lane == 0) sm.more[2] = next_unit(p, plan, sm.walk[2], sm.unit[2]);
+        if (lane == 0) sm.more[role] = next_unit(p, plan, sm.walk[role], sm.unit[role]);
         __syncwarp();
-        if (!sm.more[2]) break;
-        const int n = u.n, head = u.head;
+        if (!__shfl_sync(0xffffffffu, sm.more[role], 0)) break;
+        const int n = __shfl_sync(0xffffffffu, u.n, 0), head = __shfl_sync(0xffffffffu, u.head, 0);
+        const int ta = u.ta, room = u.v.room;
+        const Span s = u.s;
         const int32_t* table = p.tables + u.seq * p.table_stride;
-        auto find = [&](int j) {  // page `lane` of tile j
-          int page = -1;
-          if (j < n && lane < pages) {
-            const int tok = tile_token<kTile>(u.s, u.ta + j) + lane * box;
-            if (tok < u.v.room) page = page_of(p, table, tok);
-          }
-          return page;
+        auto find = [&](int j) {  // id of page `lane` of tile j; looked at when it is needed, a tile later
+          const int tok = tile_token<kTile>(s, ta + j) + lane * box;
+          return j < n && lane < pages && tok < room ? __ldg(table + (tok >> p.bs_log2)) : -1;
         };
-        int page = find(0);
+        int next = find(0);
         for (int j = 0; j < n; ++j, ++g) {
-          const int next_page = find(j + 1);
-          const uint32_t votes = __ballot_sync(0xffffffffu, page >= 0);
-          const uint32_t ks = g % kK, vs = g % kV;
-          ok = mbar_wait_warp_idle(&sm.k_empty[ks], ((g / kK) & 1) ^ 1, gave_up);
+          const int page = next >= 0 && next < p.num_blocks ? next : -1;
+          next = find(j + 1);
+          ok = mbar_wait_warp(&empty[stage], phase, gave_up);
           if (!ok) break;
-          if (lane == 0) {
+          if (!is_v) {
+            const uint32_t votes = __ballot_sync(0xffffffffu, page >= 0);
             uint32_t have = 0;  // in sixteens of tokens
             for (int c = 0; c < kTile / 16; ++c) have |= (votes >> (c * 16 / box) & 1) << c;
-            sm.have[g % kHave] = have;
-            mbar_arrive_expect(&sm.k_full[ks], kBytes);
+            if (lane == 0) sm.have[g % kHave] = have;
+            __syncwarp();
           }
-          __syncwarp();
-          const int mine = __shfl_sync(0xffffffffu, page, lane / kPieces), piece = lane % kPieces;
-          const uint32_t to = piece * (kTile * 128) + (lane / kPieces) * box * 128;
-          const int inside = tile_token<kTile>(u.s, u.ta + j) & (bs - 1);  // of a page that holds several tiles
-          // a block that there is not: the loads fill zeros
-          if (lane < pages * kPieces) box_load(smem_addr(sm.k[ks]) + to, &k_map, piece * 64, head, inside, mine, &sm.k_full[ks]);
-          ++k_issued;
-          ok = mbar_wait_warp_idle(&sm.v_empty[vs], ((g / kV) & 1) ^ 1, gave_up);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect(&sm.v_full[vs], kBytes);
-          __syncwarp();
-          if (lane < pages * kPieces) box_load(smem_addr(sm.v[vs]) + to, &v_map, piece * 64, head, inside, mine, &sm.v_full[vs]);
-          ++v_issued;
-          page = next_page;
+          int id[kTile / 16];
+#pragma unroll
+          for (int i = 0; i < kTile / 16; ++i) id[i] = __shfl_sync(0xffffffffu, page, i);
+          const int inside = tile_token<kTile>(s, ta + j) & (bs - 1);  // of a page that holds several tiles
+          if (elect_one()) {
+            mbar_arrive_expect(&full[stage], kBytes);
+#pragma unroll
+            for (int i = 0; i < kTile / 16; ++i) {
+              if (i >= pages) break;
+              // a block that there is not: the load fills zeros
+#pragma unroll
+              for (int c = 0; c < kPieces; ++c)
+                box_load(ring + stage * kBytes + c * (kTile * 128) + i * box * 128, map, c * 64, head, inside, id[i], &full[stage]);
+            }
+          }
+          if (++stage == kStages) stage = 0, phase ^= 1;
         }
       }
       if (!ok) {  // the copies in flight end before the block does
-        auto landed = [&](uint64_t* full, uint32_t stages, uint32_t issued) {
-          for (uint32_t t = issued > stages ? issued - stages : 0; t < issued; ++t)
-            for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[t % stages], (t / stages) & 1); ++i) {
-            }
-        };
-        landed(sm.k_full, kK, k_issued);
-        landed(sm.v_full, kV, v_issued);
+        for (uint32_t t = g > kStages ? g - kStages : 0; t < g; ++t)
+          for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&full[t % kStages], (t / kStages) & 1); ++i) {
+          }
       }
-    } else if (warp >= 10) {
+    } else if (warp >= 12) {
       // ---- values that are no numbers ---------------------------------------------------
-      const int mine = warp - 10;
+      const int mine = warp - 12, role = warp - 8;
       uint32_t g = 0;
       bool ok = true;
-      if (lane == 0) sm.walk[3 + mine] = walk;
-      const Unit& u = sm.unit[3 + mine];
+      if (lane == 0) sm.walk[role] = walk;
+      const Unit& u = sm.unit[role];
       while (ok) {
         __syncwarp();
-        if (lane == 0) sm.more[3 + mine] = next_unit(p, plan, sm.walk[3 + mine], sm.unit[3 + mine]);
+        if (lane == 0) sm.more[role] = next_unit(p, plan, sm.walk[role], sm.unit[role]);
         __syncwarp();
-        if (!sm.more[3 + mine]) break;
+        if (!sm.more[role]) break;
         const int n = u.n;
         for (int j = 0; j < n; ++j, ++g) {
           const uint32_t vs = g % kV;
           ok = mbar_wait_warp_idle(&sm.v_full[vs], (g / kV) & 1, gave_up);
           if (!ok) break;
           if (!tile_whole<kTile>(u.s, tile_token<kTile>(u.s, u.ta + j))) {
-            uint4* v = reinterpret_cast<uint4*>(sm.v[vs]) + mine * (kBytes / 32);
+            uint4* v = reinterpret_cast<uint4*>(sm.v[vs]) + mine * (kBytes / 64);
             bool odd = false;
 #pragma unroll 4
-            for (int i = lane; i < kBytes / 32; i += 32) {
+            for (int i = lane; i < kBytes / 64; i += 32) {
               uint4 w = v[i];
               if (odd_two<BF16>(w.x) || odd_two<BF16>(w.y) || odd_two<BF16>(w.z) || odd_two<BF16>(w.w)) {
                 odd = true;
@@ -729,125 +731,101 @@ __global__ void __launch_bounds__(kThreads, 1)
       // The whole warp walks, so that all addresses are known to be the same for its lanes; one of them issues.
       constexpr int kFormat = BF16 ? 1 : 0;
       constexpr uint32_t kQk = instr_desc(kTile, 1, kFormat, false, false), kPv = instr_desc(HD, 1, kFormat, false, true);
-      // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
-      const uint64_t q_desc = smem_desc(smem_addr(sm.q), 16, 1024, 7), k_desc = smem_desc(smem_addr(sm.k), 16, 1024, 7);
-      const uint64_t v_desc = smem_desc(smem_addr(sm.v), kTile * 128, 1024, 7);
       constexpr uint32_t kBuffer = kBytes / 16, kRows = kHalf * HD * 2 / 16;
+      const int half = warp - 10, role = 8 + half;
+      // Descriptors differ in their addresses alone, in units of 16 bytes: no carry leaves that field.
+      const uint64_t q_desc = smem_desc(smem_addr(sm.q), 16, 1024, 7) + half * kRows, k_desc = smem_desc(smem_addr(sm.k), 16, 1024, 7);
+      const uint64_t v_desc = smem_desc(smem_addr(sm.v), kTile * 128, 1024, 7);
+      const uint32_t s_at = tmem + half * 128, o_at = tmem + 256 + half * HD;
+      uint64_t *const s_full = sm.s_full[half], *const p_full = sm.p_full[half], *const o_full = sm.o_full[half];
       struct Ring {
         uint32_t at, phase;
       } kr = {0, 0}, vr = {0, 0};
-      uint32_t made[2] = {0, 0}, done[2] = {0, 0}, begins[2] = {0, 0};  // scores made and weights used of each half so far
+      uint32_t made = 0, done = 0, begins = 0;  // scores made and weights used so far, units
       bool ok = true;
-      if (lane == 0) sm.walk[5] = walk;
-      auto next_k = [&]() {
-        if (++kr.at == kK) kr.at = 0, kr.phase ^= 1;
+      if (lane == 0) sm.walk[role] = walk;
+      auto move = [](Ring& r, uint32_t by, uint32_t size) {
+        r.at += by;
+        if (r.at >= size) r.at -= size, r.phase ^= 1;
       };
-      auto next_v = [&]() {
-        if (++vr.at == kV) vr.at = 0, vr.phase ^= 1;
+      auto back = [](Ring& r, uint32_t size) {
+        if (r.at == 0) r.at = size, r.phase ^= 1;
+        --r.at;
       };
-      auto scores = [&](auto which, bool free_it) {
-        constexpr int half = decltype(which)::value;
-        const uint32_t at = made[half] & 1;
-        if (elect_one()) {
-          const uint64_t qd = q_desc + half * kRows, kd = k_desc + kr.at * kBuffer;
-          steps<HD / 16>([&](auto i) {
-            constexpr int ks = decltype(i)::value;
-            mma_ss_f16<(ks >> 2) * (kHalf * 8) + (ks & 3) * 2, (ks >> 2) * (kTile * 8) + (ks & 3) * 2>(tmem + half * 128 + at * 64, qd, kd, kQk, ks > 0);
-          });
-          tc_commit(&sm.s_full[half][at]);
-          if (free_it) tc_commit(&sm.k_empty[kr.at]);
-        }
-        ++made[half];
-      };
-      auto values = [&](auto which, bool add, bool free_it, bool last, bool last_but_one) {
-        constexpr int half = decltype(which)::value;
-        const uint32_t at = done[half] & 1;
-        ok = mbar_wait_warp(&sm.p_full[half][at], (done[half] >> 1) & 1, gave_up);
-        tc_fence_after();
-        if (!ok) return;
-        if (elect_one()) {
-          const uint64_t vd = v_desc + vr.at * kBuffer;
-          steps<kTile / 16>([&](auto i) {
-            constexpr int ks = decltype(i)::value;
-            mma_ts_f16<ks * 8, ks * 128>(tmem + 256 + half * HD, tmem + half * 128 + at * 64, vd, kPv, add || ks > 0);
-          });
-          if (last || last_but_one) tc_commit(&sm.o_full[half][last ? 0 : 1]);
-          if (free_it) tc_commit(&sm.v_empty[vr.at]);
-        }
-        ++done[half];
-      };
-      using H0 = std::integral_constant<int, 0>;
-      using H1 = std::integral_constant<int, 1>;
-      while (true) {
+      for (;;) {
         __syncwarp();
-        if (lane == 0) sm.more[5] = next_unit(p, plan, sm.walk[5], sm.unit[5]);
+        if (lane == 0) sm.more[role] = next_unit(p, plan, sm.walk[role], sm.unit[role]);
         __syncwarp();
-        if (!__shfl_sync(0xffffffffu, sm.more[5], 0) || !__all_sync(0xffffffffu, ok)) break;
-        // Of each half the scores of two tiles, then always the values of one and the scores of the next but one.
-        const int n = __shfl_sync(0xffffffffu, sm.unit[5].n, 0);
-        const bool solo = __shfl_sync(0xffffffffu, static_cast<int>(sm.unit[5].solo), 0);
-        if (n == 0) continue;
-        ok = mbar_wait_warp(&sm.q_full[0], begins[0]++ & 1, gave_up);
-        if (!solo || n > 1) ok = ok && mbar_wait_warp(&sm.q_full[1], begins[1]++ & 1, gave_up);
-        tc_fence_after();
-        if (solo) {
-          for (int j = 0; j < n + 4 && ok; j += 2) {  // the values of tiles j - 4 and j - 3, the scores of j and j + 1
-            if (j >= 4) {
-              ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up);
-              if (!ok) break;
-              values(H0(), j > 4, true, j - 2 >= n, j >= n && j - 2 < n);
-              next_v();
-            }
+        if (!__shfl_sync(0xffffffffu, sm.more[role], 0)) break;
+        const int all = __shfl_sync(0xffffffffu, sm.unit[role].n, 0);
+        const bool solo = __shfl_sync(0xffffffffu, static_cast<int>(sm.unit[role].solo), 0);
+        const int first = solo ? half : 0, step = solo ? 2 : 1;
+        const int n = all > first ? (all - first + step - 1) / step : 0;
+        if (n > 0) {
+          move(kr, first, kK);
+          move(vr, first, kV);
+          ok = mbar_wait_warp(&sm.q_full[half], begins++ & 1, gave_up);
+          tc_fence_after();
+        }
+        // The scores of two tiles, then always the values of one and the scores of the next but one.
+        for (int t = 0; t < (n > 0 ? n + 2 : 0) && ok; ++t) {
+          if (t >= 2) {
+            const uint32_t at = done & 1;
+            ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up) && mbar_wait_warp(&p_full[at], (done >> 1) & 1, gave_up);
             if (!ok) break;
-            if (j < n) {
-              ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
-              if (!ok) break;
-              scores(H0(), true);
-              next_k();
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t vd = v_desc + vr.at * kBuffer;
+              steps<kTile / 16>([&](auto i) {
+                constexpr int ks = decltype(i)::value;
+                mma_ts_f16<ks * 8, ks * 128>(o_at, s_at + at * 64, vd, kPv, t > 2 || ks > 0);
+              });
+              if (t >= n) tc_commit(&o_full[t == n ? 1 : 0]);  // of the last two tiles
+              tc_commit(&sm.v_empty[vr.at]);
+              if (solo) tc_commit(&sm.v_empty[vr.at]);  // for the other half too
             }
-            if (j >= 4 && j - 3 < n) {
-              ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up);
-              if (!ok) break;
-              values(H1(), j > 4, true, j - 1 >= n, j + 1 >= n && j - 1 < n);
-              next_v();
-            }
-            if (!ok) break;
-            if (j + 1 < n) {
-              ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
-              if (!ok) break;
-              scores(H1(), true);
-              next_k();
-            }
+            ++done;
+            move(vr, step, kV);
           }
-        } else {
-          for (int j = 0; j < n + 2; ++j) {  // the values of tile j - 2, the scores of tile j
-            const bool v = j >= 2, k = j < n;
-            if (v) ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up);
-            if (k && ok) ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
+          if (t < n) {
+            const uint32_t at = made & 1;
+            ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
             if (!ok) break;
-            if (v) values(H0(), j > 2, false, j - 1 >= n, !k && j - 1 < n);
-            if (!ok) break;
-            if (k) scores(H0(), false);
-            if (v) values(H1(), j > 2, true, j - 1 >= n, !k && j - 1 < n);
-            if (!ok) break;
-            if (k) scores(H1(), true);
-            if (v) next_v();
-            if (k) next_k();
+            if (elect_one()) {
+              const uint64_t kd = k_desc + kr.at * kBuffer;
+              steps<HD / 16>([&](auto i) {
+                constexpr int ks = decltype(i)::value;
+                mma_ss_f16<(ks >> 2) * (kHalf * 8) + (ks & 3) * 2, (ks >> 2) * (kTile * 8) + (ks & 3) * 2>(s_at + at * 64, q_desc, kd, kQk, ks > 0);
+              });
+              tc_commit(&s_full[at]);
+              tc_commit(&sm.k_empty[kr.at]);
+              if (solo) tc_commit(&sm.k_empty[kr.at]);
+            }
+            ++made;
+            move(kr, step, kK);
           }
+        }
+        if (!ok) break;
+        // the rings go on where the unit's tiles end
+        if (n == 0) {
+          move(kr, all, kK);
+          move(vr, all, kV);
+        } else if (first + n * step > all) {  // one past it
+          back(kr, kK);
+          back(vr, kV);
         }
       }
-      ok = __all_sync(0xffffffffu, ok);
       if (!ok) {  // let what was issued end before the TMEM is given back
-        if (elect_one()) tc_commit(&sm.spare);
+        if (elect_one()) tc_commit(&sm.spare[half]);
         __syncwarp();
-        for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
+        for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare[half], 0); ++i) {
         }
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 10) {
     __syncwarp();
     tc_fence_after();
     tmem_free<512>(tmem);
