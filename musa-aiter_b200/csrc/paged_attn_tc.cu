@@ -7,10 +7,6 @@
 // a step of itself, is what rounding a result adds too.  The running maximum is only moved where it grew by more than
 // 2^kLazy, so accumulators are rarely rescaled; the result is the same.
 //
-// Of each 32 weights some are taken by the exponential unit (16 a cycle and SM: as long as the products take for all of
-// them) and some by a polynomial on the other units: 2^y = 2^n 2^f, n the nearest whole number, 2^f of degree 4 with the
-// smallest largest relative error on [-1/2, 1/2], 2.6e-6 (coefficients by exchange of extrema, as Remez has it).
-//
 // A block takes 256 rows of one cache head (heads of the group next to one another, so a K / V tile serves all of them) as
 // two halves of 128 and walks the tokens in tiles of 64, with two places for each half's scores: while those of one tile
 // are exponentiated the tensor cores make the next ones and multiply the last weights.  Of a unit with 128 rows or fewer each half takes every other
@@ -39,7 +35,6 @@ constexpr int kTile = 64;       // tokens per step
 constexpr int kHalf = 128;      // rows of a half
 constexpr int kUnitRows = 256;  // rows of a unit
 constexpr int kThreads = 512;
-constexpr int kPolyOf8 = 3;     // pairs of weights of each eight that the polynomial takes
 constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolerated
 constexpr int kUnitCost = 8;    // a unit's beginning and end, in tiles
 constexpr int kMinChunk = 8;    // steps of work that are worth another block
@@ -186,6 +181,22 @@ __device__ __forceinline__ void steps(F f) {
   steps_of<N>(f, std::make_integer_sequence<int, N>());
 }
 
+// A warp's wait for a phase of a barrier, asleep for up to 0.1 ms at a time: a loop of short looks takes issue slots from
+// the warps that compute.  False when it did not complete in a second or so, or another role gave up.
+__device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile int* gave_up) {
+  uint32_t ok = 0;
+  for (uint32_t i = 0; i < (1u << 14); ++i) {
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_addr(b)), "r"(parity), "r"(100000)
+        : "memory");
+    if (ok || *gave_up) break;
+  }
+  if (!ok) *gave_up = 1;
+  return __all_sync(0xffffffffu, ok);
+}
+
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t is;
@@ -217,20 +228,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^y for y up to 2^7, without the exponential unit; below -125 it is 2^-125 or so.
-__device__ __forceinline__ float2 exp2_poly(float2 y) {
-  constexpr float kShift = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
-  y.x = fmaxf(y.x, -125.f), y.y = fmaxf(y.y, -125.f);
-  const float2 n = add2(y, both(kShift));
-  const float2 f = add2(y, fma2(n, both(-1.f), both(kShift)));
-  float2 q = fma2(both(0.009570101911f), f, both(0.05591786032f));
-  q = fma2(q, f, both(0.2402474483f));
-  q = fma2(q, f, both(0.6931218147f));
-  q = fma2(q, f, both(0.9999992614f));
-  return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(n.x) << 23)),
-                     __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(n.y) << 23)));
-}
-
 template <int HD>
 struct TcSmem {
   static constexpr int kBytes = kTile * HD * 2;      // of a tile of K or V: HD / 64 pieces of [64][64], lines of 128 bytes swizzled
@@ -383,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const RowView see = row_view(p, u.v, who);
         for (int t = 0; t < n; ++t, ++mine) {
           const uint32_t place_at = s_at + (mine & 1) * 64;  // of the scores, and of the weights over them
-          ok = ok && mbar_wait_warp(&sm.s_full[half][mine & 1], (mine >> 1) & 1, gave_up);
+          ok = ok && wait_warp(&sm.s_full[half][mine & 1], (mine >> 1) & 1, gave_up);
           tc_fence_after();
           const int j = first + t * step;
           const int tok = tile_token<kTile>(u.s, u.ta + j);
@@ -429,8 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             l *= keep;
             if (t > 0) {
               // The last weights' product: the next scores come after it.
-              ok = ok && (t + 1 < n ? mbar_wait_warp(&sm.s_full[half][(mine + 1) & 1], ((mine + 1) >> 1) & 1, gave_up)
-                                    : mbar_wait_warp(&sm.o_full[half][1], ends2 & 1, gave_up));
+              ok = ok && (t + 1 < n ? wait_warp(&sm.s_full[half][(mine + 1) & 1], ((mine + 1) >> 1) & 1, gave_up)
+                                    : wait_warp(&sm.o_full[half][1], ends2 & 1, gave_up));
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < HD / 16; ++c) {
@@ -445,30 +442,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           const float ref = m > -INFINITY && m < INFINITY ? m - kLift : 0.f;
           float2 sum[2] = {both(0.f), both(0.f)};
-          auto weights = [&](auto all_units) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              uint32_t y[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t y[16];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                float2 w = fma2(make_float2(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), both(scale), both(-ref));
-                if (decltype(all_units)::value && e % 8 >= 8 - kPolyOf8) {
-                  w = exp2_poly(w);
-                } else {
-                  w.x = exp2_near(w.x);
-                  w.y = exp2_near(w.y);
-                }
-                sum[e & 1] = add2(sum[e & 1], w);
-                y[e] = pack_two<BF16>(w.x, w.y);
-              }
-              tmem_st(place_at + c * 16, y);
+            for (int e = 0; e < 16; ++e) {
+              float2 w = fma2(make_float2(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), both(scale), both(-ref));
+              w.x = exp2_near(w.x);
+              w.y = exp2_near(w.y);
+              sum[e & 1] = add2(sum[e & 1], w);
+              y[e] = pack_two<BF16>(w.x, w.y);
             }
-          };
-          // Weights of masked scores are 0, which the polynomial does not give.
-          if (whole)
-            weights(std::true_type());
-          else
-            weights(std::false_type());
+            tmem_st(place_at + c * 16, y);
+          }
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
@@ -476,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sum[0] = add2(sum[0], sum[1]);
           l += sum[0].x + sum[0].y;
         }
-        ok = ok && mbar_wait_warp(&sm.o_full[half][0], ends & 1, gave_up);
+        ok = ok && wait_warp(&sm.o_full[half][0], ends & 1, gave_up);
         tc_fence_after();
         ++ends;
         if (n > 1) ++ends2;
@@ -655,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < n; ++j, ++g) {
           const int page = next >= 0 && next < p.num_blocks ? next : -1;
           next = find(j + 1);
-          ok = mbar_wait_warp(&empty[stage], phase, gave_up);
+          ok = wait_warp(&empty[stage], phase, gave_up);
           if (!ok) break;
           if (!is_v) {
             const uint32_t votes = __ballot_sync(0xffffffffu, page >= 0);
@@ -702,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = u.n;
         for (int j = 0; j < n; ++j, ++g) {
           const uint32_t vs = g % kV;
-          ok = mbar_wait_warp_idle(&sm.v_full[vs], (g / kV) & 1, gave_up);
+          ok = wait_warp(&sm.v_full[vs], (g / kV) & 1, gave_up);
           if (!ok) break;
           if (!tile_whole<kTile>(u.s, tile_token<kTile>(u.s, u.ta + j))) {
             uint4* v = reinterpret_cast<uint4*>(sm.v[vs]) + mine * (kBytes / 64);
@@ -739,18 +725,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t s_at = tmem + half * 128, o_at = tmem + 256 + half * HD;
       uint64_t *const s_full = sm.s_full[half], *const p_full = sm.p_full[half], *const o_full = sm.o_full[half];
       struct Ring {
+        uint64_t *full, *empty;
         uint32_t at, phase;
-      } kr = {0, 0}, vr = {0, 0};
+      } kr = {sm.k_full, sm.k_empty, 0, 0}, vr = {sm.v_clean, sm.v_empty, 0, 0};
       uint32_t made = 0, done = 0, begins = 0;  // scores made and weights used so far, units
       bool ok = true;
       if (lane == 0) sm.walk[role] = walk;
-      auto move = [](Ring& r, uint32_t by, uint32_t size) {
-        r.at += by;
-        if (r.at >= size) r.at -= size, r.phase ^= 1;
+      static_assert(kK == kV, "one size for both");
+      auto move = [](Ring& r) {
+        if (++r.at == kK) r.at = 0, r.phase ^= 1;
       };
-      auto back = [](Ring& r, uint32_t size) {
-        if (r.at == 0) r.at = size, r.phase ^= 1;
-        --r.at;
+      auto there = [&](const Ring& r) { return wait_warp(&r.full[r.at], r.phase, gave_up); };
+      // A tile of the other half's alone: both halves wait for every tile and both give every place back.  One that
+      // skipped a wait could take an older phase for the one it wants.
+      auto pass = [&](Ring& r) {
+        ok = ok && there(r);
+        if (ok && lane == 0) mbar_arrive(&r.empty[r.at]);
+        move(r);
       };
       for (;;) {
         __syncwarp();
@@ -759,61 +750,57 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!__shfl_sync(0xffffffffu, sm.more[role], 0)) break;
         const int all = __shfl_sync(0xffffffffu, sm.unit[role].n, 0);
         const bool solo = __shfl_sync(0xffffffffu, static_cast<int>(sm.unit[role].solo), 0);
-        const int first = solo ? half : 0, step = solo ? 2 : 1;
-        const int n = all > first ? (all - first + step - 1) / step : 0;
+        const int n = !solo ? all : (all + 1 - half) / 2;  // tiles of this half, every other one of a solo unit
+        const int rounds = solo ? (all + 1) / 2 : all;
         if (n > 0) {
-          move(kr, first, kK);
-          move(vr, first, kV);
-          ok = mbar_wait_warp(&sm.q_full[half], begins++ & 1, gave_up);
+          ok = wait_warp(&sm.q_full[half], begins++ & 1, gave_up);
           tc_fence_after();
         }
         // The scores of two tiles, then always the values of one and the scores of the next but one.
-        for (int t = 0; t < (n > 0 ? n + 2 : 0) && ok; ++t) {
+        for (int t = 0; t < (rounds > 0 ? rounds + 2 : 0) && ok; ++t) {
           if (t >= 2) {
-            const uint32_t at = done & 1;
-            ok = mbar_wait_warp(&sm.v_clean[vr.at], vr.phase, gave_up) && mbar_wait_warp(&p_full[at], (done >> 1) & 1, gave_up);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t vd = v_desc + vr.at * kBuffer;
-              steps<kTile / 16>([&](auto i) {
-                constexpr int ks = decltype(i)::value;
-                mma_ts_f16<ks * 8, ks * 128>(o_at, s_at + at * 64, vd, kPv, t > 2 || ks > 0);
-              });
-              if (t >= n) tc_commit(&o_full[t == n ? 1 : 0]);  // of the last two tiles
-              tc_commit(&sm.v_empty[vr.at]);
-              if (solo) tc_commit(&sm.v_empty[vr.at]);  // for the other half too
+            if (solo && half == 1) pass(vr);
+            if (t - 2 < n) {
+              const uint32_t at = done & 1;
+              ok = ok && there(vr) && wait_warp(&p_full[at], (done >> 1) & 1, gave_up);
+              if (!ok) break;
+              tc_fence_after();
+              if (elect_one()) {
+                const uint64_t vd = v_desc + vr.at * kBuffer;
+                steps<kTile / 16>([&](auto i) {
+                  constexpr int ks = decltype(i)::value;
+                  mma_ts_f16<ks * 8, ks * 128>(o_at, s_at + at * 64, vd, kPv, t > 2 || ks > 0);
+                });
+                if (t >= n) tc_commit(&o_full[t == n ? 1 : 0]);  // of the last two tiles
+                tc_commit(&vr.empty[vr.at]);
+              }
+              ++done;
+              move(vr);
             }
-            ++done;
-            move(vr, step, kV);
+            if (solo && half == 0 && 2 * (t - 2) + 1 < all) pass(vr);
           }
-          if (t < n) {
-            const uint32_t at = made & 1;
-            ok = mbar_wait_warp(&sm.k_full[kr.at], kr.phase, gave_up);
-            if (!ok) break;
-            if (elect_one()) {
-              const uint64_t kd = k_desc + kr.at * kBuffer;
-              steps<HD / 16>([&](auto i) {
-                constexpr int ks = decltype(i)::value;
-                mma_ss_f16<(ks >> 2) * (kHalf * 8) + (ks & 3) * 2, (ks >> 2) * (kTile * 8) + (ks & 3) * 2>(s_at + at * 64, q_desc, kd, kQk, ks > 0);
-              });
-              tc_commit(&s_full[at]);
-              tc_commit(&sm.k_empty[kr.at]);
-              if (solo) tc_commit(&sm.k_empty[kr.at]);
+          if (t < rounds) {
+            if (solo && half == 1) pass(kr);
+            if (t < n) {
+              const uint32_t at = made & 1;
+              ok = ok && there(kr);
+              if (!ok) break;
+              if (elect_one()) {
+                const uint64_t kd = k_desc + kr.at * kBuffer;
+                steps<HD / 16>([&](auto i) {
+                  constexpr int ks = decltype(i)::value;
+                  mma_ss_f16<(ks >> 2) * (kHalf * 8) + (ks & 3) * 2, (ks >> 2) * (kTile * 8) + (ks & 3) * 2>(s_at + at * 64, q_desc, kd, kQk, ks > 0);
+                });
+                tc_commit(&s_full[at]);
+                tc_commit(&kr.empty[kr.at]);
+              }
+              ++made;
+              move(kr);
             }
-            ++made;
-            move(kr, step, kK);
+            if (solo && half == 0 && 2 * t + 1 < all) pass(kr);
           }
         }
         if (!ok) break;
-        // the rings go on where the unit's tiles end
-        if (n == 0) {
-          move(kr, all, kK);
-          move(vr, all, kV);
-        } else if (first + n * step > all) {  // one past it
-          back(kr, kK);
-          back(vr, kV);
-        }
       }
       if (!ok) {  // let what was issued end before the TMEM is given back
         if (elect_one()) tc_commit(&sm.spare[half]);
