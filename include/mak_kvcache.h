@@ -812,6 +812,8 @@ typedef struct mak_paged_weights_desc {
   int32_t num_q_heads, window, sinks, accumulate;
   float scale;
   int32_t reserved;
+  void* workspace; /* as of mak_paged_attention, which may be the same one on one stream */
+  int64_t workspace_bytes;
 } mak_paged_weights_desc;
 
 /*

@@ -654,6 +654,10 @@ mak_paged_cache_desc paged_desc(const char* name, Args a, bool values, PyObject*
   d.dtype = float_code(kind);
   return d;
 }
+at::Tensor paged_workspace(const at::Device& device, cudaStream_t stream) {
+  static auto* spaces = new Workspaces();
+  return workspace(*spaces, lib.paged_workspace_bytes(), device, stream);
+}
 int32_t count_of(const char* name, const char* what, PyObject* o) {
   const int64_t v = integer(name, what, o);
   if (v < 0) refuse(name, what, " must not be negative, got ", v);
@@ -703,8 +707,7 @@ PyObject* py_paged(PyObject*, Args a, Py_ssize_t n) {
     const at::Tensor out = given ? THPVariable_Unpack(a[11]) : empty({rows, hq, hd}, q0.scalar_type(), q0.device());
     const at::Tensor lse = want_lse ? empty({rows, hq}, at::kFloat, q0.device()) : at::Tensor();
     const cudaStream_t stream = stream_of(dev);
-    static auto* spaces = new Workspaces();
-    const at::Tensor ws = workspace(*spaces, lib.paged_workspace_bytes(), q0.device(), stream);
+    const at::Tensor ws = paged_workspace(q0.device(), stream);
     d.q = q.data_ptr(), d.out = out.data_ptr(), d.lse = want_lse ? static_cast<float*>(lse.data_ptr()) : nullptr;
     d.workspace = ws.data_ptr(), d.workspace_bytes = ws.numel();
     d.q_stride_row = q.stride(0), d.q_stride_head = q.stride(1), d.out_stride_row = out.stride(0), d.out_stride_head = out.stride(1);
@@ -755,7 +758,10 @@ PyObject* py_weights(PyObject*, Args a, Py_ssize_t n) {
     d.q_stride_row = q.stride(0), d.q_stride_head = q.stride(1), d.lse_stride_row = lse.stride(0);
     d.sum_stride_row = sums.stride(0), d.sum_stride_head = sums.stride(1), d.sum_rows = sums.size(0), d.max_tokens = sums.size(2);
     d.num_q_heads = static_cast<int32_t>(hq);
-    check(lib.paged_weights(&d, stream_of(dev)), name);
+    const cudaStream_t stream = stream_of(dev);
+    const at::Tensor ws = paged_workspace(q0.device(), stream);
+    d.workspace = ws.data_ptr(), d.workspace_bytes = ws.numel();
+    check(lib.paged_weights(&d, stream), name);
     trace(name, a[0], "sm100a paged cache attention weights");
     Py_RETURN_NONE;
   });

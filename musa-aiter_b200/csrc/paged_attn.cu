@@ -606,6 +606,11 @@ PagedParams paged_params(const mak_paged_cache_desc& c) {
   return p;
 }
 
+PagedSpace paged_space(void* workspace) {
+  char* at = static_cast<char*>(workspace);
+  return {static_cast<int32_t*>(workspace), at + kCounterBytes, plan_bytes(), reinterpret_cast<float*>(at + kCounterBytes + plan_bytes())};
+}
+
 }  // namespace mak
 
 using namespace mak;
@@ -637,15 +642,15 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   p.group = d->num_q_heads / c.num_heads;
   p.window = d->window, p.sinks = d->window ? d->sinks : 0;
   p.scale_log2 = d->scale * 1.4426950408889634f;
-  p.counters = static_cast<int32_t*>(d->workspace);
-  p.partial = reinterpret_cast<float*>(static_cast<char*>(d->workspace) + kCounterBytes + plan_bytes());
+  const PagedSpace space = paged_space(d->workspace);
+  p.counters = space.counters, p.partial = space.partial;
   cudaStream_t st = as_stream(stream);
   const bool bf16 = c.dtype == MAK_DT_BF16;
   // Rows that share a cache head, on average.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
   if (rows > 32 && paged_tc_fits(p)) {
     bool taken = false;
-    const int rc = launch_paged_tc(p, c.head_dim, bf16, name, static_cast<char*>(d->workspace) + kCounterBytes, st, &taken);
+    const int rc = launch_paged_tc(p, c.head_dim, bf16, name, space.plan, st, &taken);
     if (rc != MAK_OK || taken) return rc;
   }
   if (c.head_dim == 64) return bf16 ? launch_rows<64, true>(p, name, st) : launch_rows<64, false>(p, name, st);

@@ -842,8 +842,7 @@ int64_t paged_tc_plan_bytes() { return sizeof(Plan); }
 int64_t paged_tc_counters() { return 4 * kMaxGrid; }
 bool paged_tc_fits(const PagedParams& p) { return row_tiles(p) <= kMaxItems; }
 
-bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool bf16,
-               int tokens) {
+bool paged_encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims, const int64_t* strides, const uint32_t* box, bool bf16) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static Encode encode = nullptr;
@@ -857,14 +856,21 @@ bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, i
     }
     encode = reinterpret_cast<Encode>(fn);
   }
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(nh), static_cast<cuuint64_t>(bs),
-                              static_cast<cuuint64_t>(num_blocks)};
-  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(sh) * 2, static_cast<cuuint64_t>(st) * 2, static_cast<cuuint64_t>(sb) * 2};
-  const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(tokens), 1}, each[4] = {1, 1, 1, 1};
-  const CUresult rc = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<uint16_t*>(base), dims,
-                             strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  cuuint64_t size[4], step[3];
+  cuuint32_t part[4], each[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) size[i] = static_cast<cuuint64_t>(dims[i]), part[i] = box[i];
+  for (int i = 0; i + 1 < rank; ++i) step[i] = static_cast<cuuint64_t>(strides[i]);
+  const CUresult rc = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+                             const_cast<void*>(base), size, step, part, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return rc == CUDA_SUCCESS;
+}
+
+bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool bf16,
+               int tokens) {
+  const int64_t dims[4] = {hd, nh, bs, num_blocks}, strides[3] = {sh * 2, st * 2, sb * 2};
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(tokens), 1};
+  return paged_encode(map, base, 4, dims, strides, box, bf16);
 }
 
 int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* name, void* plan, cudaStream_t st, bool* taken) {

@@ -16,4 +16,18 @@ int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* n
 bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool bf16,
                int tokens);
 
+// A tensor map over 16-bit elements; strides in bytes.
+bool paged_encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims, const int64_t* strides, const uint32_t* box, bool bf16);
+
+// Of the entry points.
+int check_paged_cache(const mak_paged_cache_desc& c, bool values, const char* name);
+PagedParams paged_params(const mak_paged_cache_desc& c);
+struct PagedSpace {
+  int32_t* counters;
+  void* plan;
+  int64_t plan_bytes;
+  float* partial;
+};
+PagedSpace paged_space(void* workspace);
+
 }  // namespace mak

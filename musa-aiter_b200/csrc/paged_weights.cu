@@ -5,7 +5,7 @@
 // every warp as in the attention), keeps their K in shared memory and goes over the rows, 16 at a time; each token's sum
 // has one writer, so results do not depend on timing.  Exponents are taken of scale s - lse in natural units, one
 // rounding, which keeps a weight's error at that of its exponent.
-#include "paged_attn.cuh"
+#include "paged_weights.cuh"
 
 namespace mak {
 namespace {
@@ -18,29 +18,19 @@ constexpr int kMaxGrid = 148;
 constexpr int kMinRun = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct WeightParams {
-  PagedParams a;
-  const float* lse;     // [rows][heads], row stride lse_sr
-  float* sums;          // [sequences or more][heads][max_tokens]
-  const int32_t* rows;  // row of sums of each sequence, or null
-  int64_t lse_sr, sum_sr, sum_sh, sum_rows;
-  int32_t max_tokens, add;
-  float scale;
-};
-
 template <int HD>
 struct Smem {
   static constexpr int kStages = HD == 64 ? 8 : 4;
-  alignas(128) uint8_t ring[kWarps][kStages][kStep * HD * 2];
+  static constexpr int kStage = kStep * HD * 2 + 64;  // K of a step, its sums so far
+  alignas(128) uint8_t ring[kWarps][kStages][kStage];
   int64_t before[kThreads + 1];
   int64_t sums[kWarps];
 };
 
-// Row of sums of a sequence, -1: none.
-__device__ __forceinline__ int64_t sum_row(const WeightParams& w, int s) {
-  const int64_t r = w.rows != nullptr ? __ldg(w.rows + s) : s;
-  return r >= 0 && r < w.sum_rows ? r : -1;
+__device__ __forceinline__ void copy4(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
+
 // Steps of a (sequence, head): the tokens that some row sees, or, where sums begin, all places of the row.
 __device__ __forceinline__ Span all_rows(const PagedParams& p, const PagedSeq& v) {
   Span s = {};
@@ -54,7 +44,7 @@ __device__ __forceinline__ int steps_of(const WeightParams& w, const PagedSeq& v
 
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid_constant__ WeightParams w) {
-  constexpr int kStages = Smem<HD>::kStages, kTileBytes = kStep * HD * 2;
+  constexpr int kStages = Smem<HD>::kStages, kStage = Smem<HD>::kStage, kTileBytes = kStep * HD * 2;
   constexpr int kChunks = HD / 8, kCopies = kStep * kChunks / 32;
   extern __shared__ __align__(128) uint8_t raw[];
   Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>(raw);
@@ -150,9 +140,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
     if (copied < end) {
       const uint32_t slot = static_cast<uint32_t>(copied - begin);
       there = (there & ~(1u << (slot & 31))) | (page_in >= 0 ? 1u << (slot & 31) : 0u);
+      const int tok0 = token(in);
+      const uint32_t to = ring + (slot % kStages) * kStage;
+      if (w.add && lane < kStep) {
+        const bool has = tok0 + lane < w.max_tokens;
+        const float* old = w.sums + sum_row(w, in.seq) * w.sum_sr + in.head * w.sum_sh + tok0 + lane;
+        copy4(to + kTileBytes + lane * 4, has ? old : w.sums, has ? 4 : 0);
+      }
       if (page_in >= 0) {
-        const int tok0 = token(in);
-        const uint32_t to = ring + (slot % kStages) * kTileBytes;
         const int64_t off = tok0 & ((1 << p.bs_log2) - 1);
         const uint16_t* k = p.key + page_in * p.k_sb + off * p.k_st + in.head * p.k_sh;
 #pragma unroll
@@ -172,15 +167,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
   for (int i = 0; i < kStages - 1; ++i) copy();
 
   const int r = lane >> 2, c2 = (lane & 3) * 2;
+  uint32_t qf[HD / 16][4];
+  float lse[2];
+  RowView see[2];
+  auto fetch = [&](int64_t row0, int64_t all) {  // rows row0 + r and row0 + r + 8
+    int64_t row_q[2];
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int64_t row = min(row0 + r + 8 * z, all - 1);
+      const int i = static_cast<int>(row / p.group);
+      const int64_t h = static_cast<int64_t>(out.head) * p.group + (row - static_cast<int64_t>(i) * p.group);
+      row_q[z] = (static_cast<int64_t>(out.v.first) + i) * p.q_sr + h * p.q_sh;
+      lse[z] = __ldg(w.lse + (static_cast<int64_t>(out.v.first) + i) * w.lse_sr + h);
+      see[z] = row_view(p, out.v, i);
+      if (row0 + r + 8 * z >= all) see[z].hi = 0;
+    }
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        qf[ks][e] = __ldg(reinterpret_cast<const uint32_t*>(p.q + row_q[e & 1] + ks * 16 + (e >> 1) * 8 + c2));
+  };
+  bool fresh = true;  // another sequence or head
   for (int64_t at = begin; at < end; ++at) {
     copy();
     copies_wait<kStages - 1>();
     __syncwarp();
     const uint32_t slot = static_cast<uint32_t>(at - begin);
+    const uint32_t tile = ring + (slot % kStages) * kStage;
     const int tok = token(out);
     float sum[4] = {0.f, 0.f, 0.f, 0.f};  // tokens c2, c2 + 1, c2 + 8, c2 + 9
     if (there >> (slot & 31) & 1) {
-      const uint32_t tile = ring + (slot % kStages) * kTileBytes;
       const int64_t all = static_cast<int64_t>(out.v.rows) * p.group;
       int64_t row0 = 0;
       if (tok >= p.sinks) {  // rows before the first that sees a token of the step: the one at position tok
@@ -188,25 +205,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
         if (i > 0) row0 = i * p.group / kRows * kRows;
       }
       for (; row0 < all; row0 += kRows) {
-        uint32_t qf[HD / 16][4];
-        float lse[2];
-        RowView see[2];
-        int64_t row_q[2];
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const int64_t row = min(row0 + r + 8 * z, all - 1);
-          const int i = static_cast<int>(row / p.group);
-          const int64_t h = static_cast<int64_t>(out.head) * p.group + (row - static_cast<int64_t>(i) * p.group);
-          row_q[z] = (static_cast<int64_t>(out.v.first) + i) * p.q_sr + h * p.q_sh;
-          lse[z] = __ldg(w.lse + (static_cast<int64_t>(out.v.first) + i) * w.lse_sr + h);
-          see[z] = row_view(p, out.v, i);
-          if (row0 + r + 8 * z >= all) see[z].hi = 0;
-        }
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            qf[ks][e] = __ldg(reinterpret_cast<const uint32_t*>(p.q + row_q[e & 1] + ks * 16 + (e >> 1) * 8 + c2));
+        // 16 rows or fewer stay in registers from step to step
+        if (fresh || all > kRows) fetch(row0, all);
+        fresh = false;
         // rows of a window that have all left the step behind end the walk
         if (p.window > 0 && tok >= p.sinks && __all_sync(0xffffffffu, see[0].lo >= tok + kStep && see[1].lo >= tok + kStep)) break;
         float s[2][4];
@@ -245,11 +246,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
         const int t = tok + r * 8 + c2 + e;
         const float x = r == 0 ? sum[e] : sum[2 + e];
         const bool seen = t < out.s.any_hi && (t >= out.s.any_lo || t < p.sinks);
-        if (t < w.max_tokens && (!w.add || seen)) dst[t] = w.add ? dst[t] + x : x;
+        if (t >= w.max_tokens || (w.add && !seen)) continue;
+        float old = 0.f;
+        if (w.add) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(old) : "r"(tile + kTileBytes + (t - tok) * 4) : "memory");
+        dst[t] = old + x;
       }
     }
     __syncwarp();  // the stage is read
-    if (at + 1 < end) advance(out);
+    if (at + 1 < end) {
+      const int seq = out.seq, head = out.head;
+      advance(out);
+      fresh = fresh || out.seq != seq || out.head != head;
+    }
   }
   copies_wait<0>();
 }
@@ -266,10 +274,6 @@ int launch_few(const WeightParams& w, const char* name, cudaStream_t st) {
 }
 
 }  // namespace
-
-int check_paged_cache(const mak_paged_cache_desc& c, bool values, const char* name);
-PagedParams paged_params(const mak_paged_cache_desc& c);
-
 }  // namespace mak
 
 using namespace mak;
@@ -302,8 +306,18 @@ extern "C" int mak_paged_weights(const mak_paged_weights_desc* d, void* stream) 
   w.rows = d->rows;
   w.max_tokens = static_cast<int32_t>(d->max_tokens), w.add = d->accumulate != 0;
   w.scale = d->scale;
+  if (d->workspace == nullptr || d->workspace_bytes < mak_paged_attention_workspace_bytes())
+    return fail(MAK_E_WORKSPACE, "%s: workspace missing or too small", name);
+  const PagedSpace space = paged_space(d->workspace);
+  w.a.counters = space.counters, w.a.partial = space.partial;
   cudaStream_t st = as_stream(stream);
   const bool bf16 = c.dtype == MAK_DT_BF16;
+  // Rows that share a cache head, on average.
+  if (c.num_rows * w.a.group / c.num_seqs > 32 && c.num_seqs * 8 <= space.plan_bytes) {
+    bool taken = false;
+    const int rc = launch_weights_tc(w, c.head_dim, bf16, name, static_cast<int64_t*>(space.plan), st, &taken);
+    if (rc != MAK_OK || taken) return rc;
+  }
   if (c.head_dim == 64) return bf16 ? launch_few<64, true>(w, name, st) : launch_few<64, false>(w, name, st);
   return bf16 ? launch_few<128, true>(w, name, st) : launch_few<128, false>(w, name, st);
 }
