@@ -753,7 +753,9 @@ PyObject* py_weights(PyObject*, Args a, Py_ssize_t n) {
     for (const at::Tensor* t : used) dev.add(*t);
     dev.need_library();
     const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
-    const at::Tensor q = aligned_rows(q0);
+    // an expanded axis has no place in a tensor map
+    const bool repeats = (rows > 1 && q0.stride(0) == 0) || (hq > 1 && q0.stride(1) == 0);
+    const at::Tensor q = repeats ? q0.clone(at::MemoryFormat::Contiguous) : aligned_rows(q0);
     d.q = q.data_ptr(), d.lse = static_cast<const float*>(lse.data_ptr()), d.sums = static_cast<float*>(sums.data_ptr());
     d.q_stride_row = q.stride(0), d.q_stride_head = q.stride(1), d.lse_stride_row = lse.stride(0);
     d.sum_stride_row = sums.stride(0), d.sum_stride_head = sums.stride(1), d.sum_rows = sums.size(0), d.max_tokens = sums.size(2);

@@ -7,10 +7,11 @@
 //
 // Bound by reading K and V.  A unit is 16 rows (tokens of a sequence times the query heads of a cache head) of one
 // sequence and head, its work 16-token steps.  All units laid end to end are cut into equal runs, one per warp, whatever
-// the lengths; a warp copies its steps into a ring of its own (a page's row of 16 bytes per lane), so no warp waits for
+// the lengths; a warp has its steps brought by TMA into a ring of its own, so no warp waits for
 // another until its run ends.  A unit cut by that leaves partial sums: the block joins those of its warps, the last block
 // to arrive joins those of the blocks, both in order of position, so results do not depend on timing.
 #include "paged_attn_tc.cuh"
+#include "tcgen05.cuh"
 
 namespace mak {
 namespace {
@@ -44,12 +45,13 @@ template <int HD>
 struct Smem {
   static constexpr int kStages = HD == 64 ? 6 : 3;
   static constexpr int kTileBytes = kStep * HD * 2;
-  alignas(128) uint8_t ring[kWarps][kStages][2 * kTileBytes];
+  alignas(1024) uint8_t ring[kWarps][kStages][2 * kTileBytes];  // K, V: HD / 64 pieces of [16][64], lines of 128 bytes swizzled
+  uint64_t full[kWarps][kStages];
   Unit queue[kWarps][kQueue];
   Piece pieces[2 * kWarps];
   int64_t before[kThreads + 1];  // work of the sequences of the threads before
   int64_t sums[kWarps];
-  int last;
+  int last, gave_up;
 };
 
 __device__ __forceinline__ int tiles_of(const PagedParams& p, const PagedSeq& v) {
@@ -122,14 +124,20 @@ template <int HD>
 constexpr int kPieceFloats = kRows * (HD + 2);
 
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(kThreads, 1) 
+    paged_rows_kernel(const __grid_constant__ PagedParams p, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
   constexpr int kStages = Smem<HD>::kStages, kTileBytes = Smem<HD>::kTileBytes;
-  constexpr int kChunks = HD / 8;               // 16-byte pieces of a token
-  constexpr int kCopies = kStep * kChunks / 32; // of a lane, for K and for V
+  constexpr int kPieces = HD / 64, kPiece = kStep * 128;  // of a step's K or V
   constexpr float kLift = BF16 ? 0.f : 15.f;    // log2 factor that weights carry
-  extern __shared__ __align__(128) uint8_t raw[];
+  extern __shared__ __align__(1024) uint8_t raw[];
   Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>(raw);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  if (tid == 0) {
+    sm.gave_up = 0;
+    for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&sm.full[0][0] + i, 1);
+    mbar_init_fence();
+  }
   pdl_wait();
   pdl_trigger();
 
@@ -200,57 +208,55 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     walk.w0 = at;
   }
 
-  // ---- copies, some steps ahead of the products ---------------------------------------
+  // ---- loads, some steps ahead of the products ---------------------------------------
   const uint32_t ring = shared_at(sm.ring[warp]);
+  uint64_t* full = sm.full[warp];
+  volatile int* gave_up = &sm.gave_up;
   Unit* queue = sm.queue[warp];
-  int units_in = 0, step_in = 0, end_in = 0, page_in = -1;
+  int units_in = 0, left_in = 0;   // steps of the unit at hand that are left
+  int tok_in = 0, jump_at = 0, jump = 0, tiles_in = 0, head_in = 0, next_id = -1;
+  const int32_t* table_in = nullptr;
   bool more = true;
-  auto look = [&](int j) {  // page of the unit's step j
-    const Unit& u = queue[(units_in - 1) % kQueue];
-    if (j >= u.tb || j >= u.s.tiles) return -1;
-    return page_of(p, p.tables + u.seq * p.table_stride, tile_token<kStep>(u.s, j));
-  };
+  const int inside = (1 << p.bs_log2) - 1;
+  // Steps go up by 16 tokens, but for one jump from the first tokens to the window.
   auto enter = [&]() {
     Unit u;
     more = more && next_unit(p, walk, u);
-    if (more) {
-      __syncwarp();
-      if (lane == 0) queue[units_in % kQueue] = u;
-      __syncwarp();
-      ++units_in;
-      step_in = u.ta, end_in = u.tb;
-      page_in = look(step_in);
-    }
+    if (!more) return;
+    __syncwarp();
+    if (lane == 0) queue[units_in % kQueue] = u;
+    __syncwarp();
+    ++units_in;
+    left_in = u.tb - u.ta, tiles_in = u.s.tiles, head_in = u.head;
+    tok_in = tile_token<kStep>(u.s, u.ta);
+    jump_at = u.ta < u.s.ns ? kStep * (u.s.ns - 1) : -1, jump = kStep * u.s.t0;
+    table_in = p.tables + u.seq * p.table_stride;
+    next_id = tiles_in > 0 ? __ldg(table_in + (tok_in >> p.bs_log2)) : -1;  // looked at when it is needed, a step later
   };
-  int in = 0;  // steps copied so far
-  uint32_t there = 0;  // bit i: step i % 32 has a page
-  auto copy = [&]() {
-    if (more && step_in == end_in) enter();
-    if (more) {
-      const Unit& u = queue[(units_in - 1) % kQueue];
-      there = (there & ~(1u << (in & 31))) | (page_in >= 0 ? 1u << (in & 31) : 0u);
-      if (page_in >= 0) {
-        const int tok0 = tile_token<kStep>(u.s, step_in);
-        const uint32_t to = ring + (in % kStages) * (2 * kTileBytes);
-        const int64_t off = tok0 & ((1 << p.bs_log2) - 1);
-        const uint16_t* k = p.key + page_in * p.k_sb + off * p.k_st + u.head * p.k_sh;
-        const uint16_t* v = p.value + page_in * p.v_sb + off * p.v_st + u.head * p.v_sh;
-        // what no row sees becomes 0, whatever it holds
-        const bool edge = !(tok0 + kStep <= min(p.sinks, u.s.any_hi)) && !(tok0 >= u.s.any_lo && tok0 + kStep <= u.s.any_hi);
+  int in = 0, stage_in = 0;  // steps loaded so far
+  uint32_t there = 0;        // bit i: step i % 32 has a page
+  auto load = [&]() {
+    if (more && left_in == 0) enter();
+    if (!more) return;
+    const int page = __shfl_sync(0xffffffffu, next_id, 0), tok = __shfl_sync(0xffffffffu, tok_in, 0), head = __shfl_sync(0xffffffffu, head_in, 0);
+    const bool has = page >= 0 && page < p.num_blocks;
+    there = (there & ~(1u << (in & 31))) | (has ? 1u << (in & 31) : 0u);
+    tok_in = tok_in == jump_at ? jump : tok_in + kStep;
+    --left_in;
+    next_id = left_in > 0 && tiles_in > 0 ? __ldg(table_in + (tok_in >> p.bs_log2)) : -1;
+    if (has && elect_one()) {
+      const uint32_t to = ring + stage_in * (2 * kTileBytes);
+      uint64_t* bar = full + stage_in;
+      mbar_arrive_expect(bar, 2 * kTileBytes);
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-          const int t = (i * 32 + lane) / kChunks, c = (i * 32 + lane) % kChunks;
-          const int n = !edge || seen_by_any(p, u.s, tok0 + t) ? 16 : 0;
-          const uint32_t at = to + t * (HD * 2) + ((c ^ (t & 7)) << 4);
-          copy16(at, k + t * p.k_st + c * 8, n);
-          copy16(at + kTileBytes, v + t * p.v_st + c * 8, n);
-        }
+      for (int c = 0; c < kPieces; ++c) {
+        box_load(to + c * kPiece, &k_map, c * 64, head, tok & inside, page, bar);
+        box_load(to + kTileBytes + c * kPiece, &v_map, c * 64, head, tok & inside, page, bar);
       }
-      ++step_in;
-      ++in;
-      page_in = look(step_in);
     }
-    copies_commit();
+    __syncwarp();
+    ++in;
+    stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
   };
   if (walk.w < walk.w_end) {
     enter();
@@ -258,11 +264,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     more = false;
   }
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) copy();
+  for (int i = 0; i < kStages - 1; ++i) load();
 
   // ---- products --------------------------------------------------------------------------
   const int r = lane >> 2, c2 = (lane & 3) * 2;  // this lane's rows r and r + 8, columns c2 and c2 + 1 of 8
-  int units_out = 0, out = 0;
+  const float scale = fmaxf(fabsf(p.scale_log2), 1e-37f);  // not 0: masked scores are -inf
+  const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+  int units_out = 0, out = 0, stage = 0;
+  uint32_t phases = 0;  // bit of a stage: the parity of its next phase
+  bool ok = true;
   while (units_out < units_in) {
     const Unit& u = queue[units_out % kQueue];
     uint32_t qf[HD / 16][4];
@@ -282,35 +292,36 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        qf[ks][e] = __ldg(reinterpret_cast<const uint32_t*>(p.q + row_q[e & 1] + ks * 16 + (e >> 1) * 8 + c2));
+        qf[ks][e] = __ldg(reinterpret_cast<const uint32_t*>(p.q + row_q[e & 1] + ks * 16 + (e >> 1) * 8 + c2)) ^ sign;
     float o[HD / 8][4];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-    const int ta = u.ta, tb = u.tb;
+    const int ta = u.ta, tb = u.tb, live = u.live;
+    const Span span = u.s;
     for (int j = ta; j < tb; ++j, ++out) {
-      copy();
-      copies_wait<kStages - 1>();
-      __syncwarp();
+      load();
       if (there >> (out & 31) & 1) {
-        const int tok = tile_token<kStep>(u.s, j);
-        const uint32_t at = ring + (out % kStages) * (2 * kTileBytes);
+        ok = mbar_wait_warp(full + stage, phases >> stage & 1, gave_up) && ok;
+        phases ^= 1u << stage;
+        const int tok = tile_token<kStep>(span, j);
+        const uint32_t at = ring + stage * (2 * kTileBytes);
         float s[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
         {
           const int t = ((lane >> 4) << 3) + (lane & 7), half = (lane >> 3) & 1;
-          const uint32_t row = at + t * (HD * 2);
+          const uint32_t row = at + t * 128;
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks) {
             uint32_t b[4];
-            load_matrix(row + (((2 * ks + half) ^ (t & 7)) << 4), b);
+            load_matrix(row + (ks >> 2) * kPiece + (((2 * (ks & 3) + half) ^ (t & 7)) << 4), b);
             mma_16816<BF16>(s[0], qf[ks], b[0], b[1]);
             mma_16816<BF16>(s[1], qf[ks], b[2], b[3]);
           }
         }
-        const bool whole = tile_whole<kStep>(u.s, tok);
+        const bool whole = tile_whole<kStep>(span, tok);
         uint32_t bits[2] = {0xffffu, 0xffffu};  // tokens that the lane's rows see
         if (!whole) {
 #pragma unroll
@@ -318,29 +329,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             if (p.parents != nullptr) {
               bits[z] = tree_bits(p, u.v, who[z], tok) & 0xffffu;
             } else {
-              bits[z] = 0;
-#pragma unroll
-              for (int e = 0; e < kStep; ++e)
-                if (tok + e < see[z].hi && (tok + e >= see[z].lo || tok + e < p.sinks)) bits[z] |= 1u << e;
+              auto below = [](int k) { return k >= kStep ? 0xffffu : k <= 0 ? 0u : (1u << k) - 1u; };
+              bits[z] = below(see[z].hi - tok) & (~below(see[z].lo - tok) | below(p.sinks - tok));
             }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                s[i][2 * z + e] = bits[z] >> (i * 8 + c2 + e) & 1 ? s[i][2 * z + e] : -INFINITY;
           }
         }
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int z = e >> 1, t = i * 8 + c2 + (e & 1);
-            s[i][e] = bits[z] >> t & 1 ? s[i][e] * p.scale_log2 : -INFINITY;
-            top[z] = fmaxf(top[z], s[i][e]);
-          }
         float keep[2], ref[2];
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          top[z] = fmaxf(top[z], __shfl_xor_sync(0xffffffffu, top[z], 1));
-          top[z] = fmaxf(top[z], __shfl_xor_sync(0xffffffffu, top[z], 2));
-          const float now = fmaxf(m[z], top[z]);
-          keep[z] = now == -INFINITY ? 1.f : exp2_near(m[z] - now);
+          float top = fmaxf(fmaxf(s[0][2 * z], s[0][2 * z + 1]), fmaxf(s[1][2 * z], s[1][2 * z + 1]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale;
+          const float now = fmaxf(m[z], top);
+          keep[z] = now == m[z] ? 1.f : exp2_near(m[z] - now);
           ref[z] = now == -INFINITY ? 0.f : now - kLift;
           m[z] = now;
         }
@@ -353,16 +359,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[i][e] = exp2_near(s[i][e] - ref[e >> 1]);
+            s[i][e] = exp2_near(fmaf(s[i][e], scale, -ref[e >> 1]));
             l[e >> 1] += s[i][e];
           }
         const uint32_t values = at + kTileBytes;
         bool odd = false;
-        const bool alike = whole || (u.s.any_hi == u.s.all_hi && u.s.any_lo == u.s.all_lo);  // all rows see the same tokens
-        if (!alike) {
-          // Some rows see what others do not: 0 times an infinite value is not 0.
+        if (!whole) {  // 0 times an infinite value is not 0: such a value is kept from the rows that do not see it
 #pragma unroll 1
-          for (int i = lane; i < kStep * kChunks; i += 32) {
+          for (int i = lane; i < kTileBytes / 16; i += 32) {
             uint32_t w[4];
             asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(values + i * 16) : "memory");
             odd = odd || odd_two<BF16>(w[0]) || odd_two<BF16>(w[1]) || odd_two<BF16>(w[2]) || odd_two<BF16>(w[3]);
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         }
         if (!odd) {
           // A weight is the sum of the two.  Neither is 0 where an infinite value may be seen: 0 times it is no number.
-          const uint32_t least = alike ? 0x00010001u : 0u;
+          const uint32_t least = whole ? 0x00010001u : 0u;
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -382,11 +386,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             hi[e] = __vmaxu2(hi[e], least);
           }
           const int t = (((lane >> 3) & 1) << 3) + (lane & 7), half = lane >> 4;
-          const uint32_t row = values + t * (HD * 2);
+          const uint32_t row = values + t * 128;
 #pragma unroll
           for (int d = 0; d < HD / 16; ++d) {
             uint32_t b[4];
-            load_matrix_t(row + (((2 * d + half) ^ (t & 7)) << 4), b);
+            load_matrix_t(row + (d >> 2) * kPiece + (((2 * (d & 3) + half) ^ (t & 7)) << 4), b);
             mma_16816<BF16>(o[2 * d], hi, b[0], b[1]);
             mma_16816<BF16>(o[2 * d + 1], hi, b[2], b[3]);
             mma_16816<BF16>(o[2 * d], lo, b[0], b[1]);
@@ -401,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
             for (int d = 0; d < HD / 8; ++d) {
               uint32_t x;
-              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(values + t * (HD * 2) + ((d ^ (t & 7)) << 4) + c2 * 2) : "memory");
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(values + (d >> 3) * kPiece + t * 128 + (((d & 7) ^ (t & 7)) << 4) + c2 * 2) : "memory");
               const float2 f = unpack_two<BF16>(x);
               if (bits[0] >> t & 1) o[d][0] = fmaf(w[0], f.x, o[d][0]), o[d][1] = fmaf(w[0], f.y, o[d][1]);
               if (bits[1] >> t & 1) o[d][2] = fmaf(w[1], f.x, o[d][2]), o[d][3] = fmaf(w[1], f.y, o[d][3]);
@@ -409,8 +413,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
           }
         }
       }
+      stage = stage + 1 == kStages ? 0 : stage + 1;
       __syncwarp();  // the stage is read
     }
+    if (!ok) l[0] = l[1] = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN
 
     // ---- this warp's share of the unit ----------------------------------------------------
 #pragma unroll
@@ -421,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     if (ta == 0 && tb == u.len) {
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        if (r + 8 * z >= u.live) continue;
+        if (r + 8 * z >= live) continue;
         const int64_t row = static_cast<int64_t>(u.tile) * kRows + r + 8 * z;
         const int64_t i = u.v.first + row / p.group, h = static_cast<int64_t>(u.head) * p.group + row % p.group;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh + c2;
@@ -446,13 +452,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
       const int slot = ta > 0 ? 0 : 1;  // a run begins inside one unit at most, and ends inside one
       float* part = final_piece ? reinterpret_cast<float*>(sm.ring[warp])
                                 : p.partial + (static_cast<int64_t>(blockIdx.x) * (2 * kWarps) + warp * 2 + slot) * kPieceFloats<HD>;
-      if (final_piece) {
-        copies_wait<0>();
-        __syncwarp();
-      }
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
-        if (r + 8 * z >= u.live) continue;
+        if (r + 8 * z >= live) continue;
         float* dst = part + (r + 8 * z) * HD + c2;
 #pragma unroll
         for (int d = 0; d < HD / 8; ++d) *reinterpret_cast<float2*>(dst + d * 8) = make_float2(o[d][2 * z], o[d][2 * z + 1]);
@@ -470,7 +472,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     ++units_out;
     __syncwarp();
   }
-  copies_wait<0>();
   __syncthreads();
 
   // ---- pieces of the same unit ----------------------------------------------------------------
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 }
 
 template <int HD, bool BF16>
-int launch_rows(const PagedParams& p, const char* name, cudaStream_t st) {
+int launch_rows(const PagedParams& p, const CUtensorMap& k, const CUtensorMap& v, const char* name, cudaStream_t st) {
   constexpr int kBytes = sizeof(Smem<HD>);
   static_assert(kBytes <= 227 * 1024, "shared memory of a block");
   static_assert(kRows * (HD + 2) * 4 <= Smem<HD>::kStages * 2 * Smem<HD>::kTileBytes, "a piece fits its warp's ring");
@@ -561,7 +562,7 @@ int launch_rows(const PagedParams& p, const char* name, cudaStream_t st) {
   static bool ready[kPagedDevices] = {};
   if (int rc = paged_prepare(name, kernel, kBytes, ready)) return rc;
   const int sms = sm_count();
-  return launch_pdl(name, kernel, dim3(sms < kMaxGrid ? sms : kMaxGrid), dim3(kThreads), kBytes, st, p);
+  return launch_pdl(name, kernel, dim3(sms < kMaxGrid ? sms : kMaxGrid), dim3(kThreads), kBytes, st, p, k, v);
 }
 
 constexpr int64_t kCounterBytes = 4096;
@@ -648,11 +649,13 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   const bool bf16 = c.dtype == MAK_DT_BF16;
   // Rows that share a cache head, on average.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
-  if (rows > 32 && paged_tc_fits(p)) {
-    bool taken = false;
-    const int rc = launch_paged_tc(p, c.head_dim, bf16, name, space.plan, st, &taken);
-    if (rc != MAK_OK || taken) return rc;
-  }
-  if (c.head_dim == 64) return bf16 ? launch_rows<64, true>(p, name, st) : launch_rows<64, false>(p, name, st);
-  return bf16 ? launch_rows<128, true>(p, name, st) : launch_rows<128, false>(p, name, st);
+  const bool many = rows > 32 && paged_tc_fits(p);
+  const int tokens = many ? paged_tc_box(c.block_size) : kStep;
+  CUtensorMap k, v;
+  if (!paged_map(&k, p.key, p.k_sb, p.k_st, p.k_sh, p.num_blocks, p.nh, c.head_dim, c.block_size, bf16, tokens, d->workspace) ||
+      !paged_map(&v, p.value, p.v_sb, p.v_st, p.v_sh, p.num_blocks, p.nh, c.head_dim, c.block_size, bf16, tokens, d->workspace))
+    return fail(MAK_E_INVALID, "%s: the cache's strides make no tensor map", name);
+  if (many) return launch_paged_tc(p, c.head_dim, bf16, name, k, v, space.plan, st);
+  if (c.head_dim == 64) return bf16 ? launch_rows<64, true>(p, k, v, name, st) : launch_rows<64, false>(p, k, v, name, st);
+  return bf16 ? launch_rows<128, true>(p, k, v, name, st) : launch_rows<128, false>(p, k, v, name, st);
 }

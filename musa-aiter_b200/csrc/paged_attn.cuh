@@ -183,7 +183,7 @@ int paged_prepare(const char* name, K kernel, int bytes, bool (&ready)[kPagedDev
   return MAK_OK;
 }
 
-// ---- 16 x 8 x 16 products on fragments in registers, and 16-byte copies to shared memory --------------------
+// ---- 16 x 8 x 16 products on fragments in registers --------------------------------------------------------
 __device__ __forceinline__ uint32_t shared_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 template <bool BF16>
@@ -209,14 +209,24 @@ __device__ __forceinline__ void load_matrix_t(uint32_t at, uint32_t (&r)[4]) {
                : "r"(at)
                : "memory");
 }
-// 16 bytes, or zeros where `bytes` is 0.
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Box of a 4-dimensional tensor map; a coordinate outside fills zeros.
+__device__ __forceinline__ void box_load(uint32_t to, const void* map, int x, int y, int z, int v, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(shared_at(bar))
+      : "memory");
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is != 0;
 }
 
 }  // namespace mak

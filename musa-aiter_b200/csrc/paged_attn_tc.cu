@@ -197,13 +197,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile
   return __all_sync(0xffffffffu, ok);
 }
 
-// True in one lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t is;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
-  return is != 0;
-}
-
 __device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -265,13 +258,6 @@ __device__ __noinline__ void odd_sum(const PagedParams& p, const Unit& u, int i,
       }
     }
   }
-}
-
-__device__ __forceinline__ void box_load(uint32_t to, const void* map, int x, int head, int token, int block, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
-      "l"(map), "r"(x), "r"(head), "r"(token), "r"(block), "r"(smem_addr(bar))
-      : "memory");
 }
 
 template <int HD, bool BF16>
@@ -867,18 +853,17 @@ bool paged_encode(CUtensorMap* map, const void* base, int rank, const int64_t* d
 }
 
 bool paged_map(CUtensorMap* map, const uint16_t* base, int64_t sb, int64_t st, int64_t sh, int64_t num_blocks, int nh, int hd, int bs, bool bf16,
-               int tokens) {
-  const int64_t dims[4] = {hd, nh, bs, num_blocks}, strides[3] = {sh * 2, st * 2, sb * 2};
+               int tokens, const void* none) {
+  // a pool without pages is never loaded from, but a map needs a size and an address
+  const int64_t dims[4] = {hd, nh, bs, num_blocks > 0 ? num_blocks : 1}, strides[3] = {sh * 2, st * 2, sb * 2};
   const uint32_t box[4] = {64, 1, static_cast<uint32_t>(tokens), 1};
-  return paged_encode(map, base, 4, dims, strides, box, bf16);
+  return paged_encode(map, num_blocks > 0 ? static_cast<const void*>(base) : none, 4, dims, strides, box, bf16);
 }
 
-int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* name, void* plan, cudaStream_t st, bool* taken) {
-  CUtensorMap k, v;
-  const int bs = 1 << p.bs_log2;
-  *taken = p.num_blocks > 0 && paged_map(&k, p.key, p.k_sb, p.k_st, p.k_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs < kTile ? bs : kTile) &&
-           paged_map(&v, p.value, p.v_sb, p.v_st, p.v_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs < kTile ? bs : kTile);
-  if (!*taken) return MAK_OK;
+int paged_tc_box(int bs) { return bs < kTile ? bs : kTile; }
+
+int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* name, const CUtensorMap& k, const CUtensorMap& v, void* plan,
+                    cudaStream_t st) {
   Plan* at = static_cast<Plan*>(plan);
   if (head_dim == 64) return bf16 ? launch<64, true>(p, name, k, v, at, st) : launch<64, false>(p, name, k, v, at, st);
   return bf16 ? launch<128, true>(p, name, k, v, at, st) : launch<128, false>(p, name, k, v, at, st);

@@ -21,8 +21,8 @@ __device__ __forceinline__ int64_t sum_row(const WeightParams& w, int s) {
   return r >= 0 && r < w.sum_rows ? r : -1;
 }
 
-// `taken`: false where a group is wider than a chunk or strides make no tensor map; nothing was launched then.  `work`:
-// scratch of one number per sequence.
-int launch_weights_tc(const WeightParams& w, int head_dim, bool bf16, const char* name, int64_t* work, cudaStream_t st, bool* taken);
+bool weights_tc_fits(const WeightParams& w);
+// `work`: scratch of one number per sequence.
+int launch_weights_tc(const WeightParams& w, int head_dim, bool bf16, const char* name, const CUtensorMap& k, int64_t* work, cudaStream_t st);
 
 }  // namespace mak

@@ -173,12 +173,6 @@ __device__ __forceinline__ float2 exp2_poly(float2 y) {
   const float2 top = make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u));
   return mul2(q, top);
 }
-// True in one lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t is;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
-  return is != 0;
-}
 // A warp's wait for a phase of a barrier, asleep for up to 0.1 ms at a time.  False when it did not complete in a second or
 // so, or another role gave up.
 __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile int* gave_up) {
@@ -194,12 +188,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile
   return __all_sync(0xffffffffu, ok);
 }
 __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-__device__ __forceinline__ void box4(uint32_t to, const void* map, int x, int y, int z, int v, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(smem_addr(bar))
-      : "memory");
-}
 __device__ __forceinline__ void box3(uint32_t to, const void* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),
@@ -457,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (i >= pages) break;
           // a block that there is not: the load fills zeros
 #pragma unroll
-          for (int c = 0; c < kPieces; ++c) box4(smem_addr(sm.k[ks]) + c * 16384 + i * box * 128, &k_map, c * 64, head, 0, id[i], &sm.k_full[ks]);
+          for (int c = 0; c < kPieces; ++c) box_load(smem_addr(sm.k[ks]) + c * 16384 + i * box * 128, &k_map, c * 64, head, 0, id[i], &sm.k_full[ks]);
         }
       }
       ++units;
@@ -576,14 +564,14 @@ static bool rows_map(CUtensorMap* map, const uint16_t* base, int64_t sr, int64_t
   return paged_encode(map, base, 3, dims, strides, box, bf16);
 }
 
-int launch_weights_tc(const WeightParams& w, int head_dim, bool bf16, const char* name, int64_t* work, cudaStream_t st, bool* taken) {
+bool weights_tc_fits(const WeightParams& w) { return w.a.group <= kTile && w.a.num_rows > 0; }
+
+int launch_weights_tc(const WeightParams& w, int head_dim, bool bf16, const char* name, const CUtensorMap& k, int64_t* work, cudaStream_t st) {
   const PagedParams& p = w.a;
-  CUtensorMap k, q;
-  const int bs = 1 << p.bs_log2, per = p.group <= kTile ? kTile / p.group : 0;
-  *taken = per > 0 && p.num_blocks > 0 && p.num_rows > 0 &&
-           paged_map(&k, p.key, p.k_sb, p.k_st, p.k_sh, p.num_blocks, p.nh, head_dim, bs, bf16, bs < kTile ? bs : kTile) &&
-           rows_map(&q, p.q, p.q_sr, p.q_sh, p.num_rows, p.nh * p.group, head_dim, bf16, p.group, per);
-  if (!*taken) return MAK_OK;
+  const int per = kTile / p.group;
+  CUtensorMap q;
+  if (!rows_map(&q, p.q, p.q_sr, p.q_sh, p.num_rows, p.nh * p.group, head_dim, bf16, p.group, per))
+    return fail(MAK_E_INVALID, "%s: the strides of q make no tensor map", name);
   if (head_dim == 64) return bf16 ? launch<64, true>(w, name, k, q, work, per, st) : launch<64, false>(w, name, k, q, work, per, st);
   return bf16 ? launch<128, true>(w, name, k, q, work, per, st) : launch<128, false>(w, name, k, q, work, per, st);
 }
