@@ -51,16 +51,16 @@ struct Smem {
   Piece pieces[2 * kWarps];
   int64_t before[kThreads + 1];  // work of the sequences of the threads before
   int64_t sums[kWarps];
-  int last, gave_up;
+  int join[2], gave_up;  // pieces of the units that this block joins, -1: none
 };
 
 __device__ __forceinline__ int tiles_of(const PagedParams& p, const PagedSeq& v) {
-  return static_cast<int>((static_cast<int64_t>(v.rows) * p.group + kRows - 1) / kRows);
+  return (v.rows * p.group + kRows - 1) / kRows;
 }
 __device__ __forceinline__ Span span_of_tile(const PagedParams& p, const PagedSeq& v, int tile, int* live) {
-  const int64_t row0 = static_cast<int64_t>(tile) * kRows, left = static_cast<int64_t>(v.rows) * p.group - row0;
-  *live = left < kRows ? static_cast<int>(left) : kRows;
-  return span_of<kStep>(p, v, static_cast<int>(row0 / p.group), static_cast<int>((row0 + *live - 1) / p.group));
+  const int row0 = tile * kRows;
+  *live = min(v.rows * p.group - row0, kRows);
+  return span_of<kStep>(p, v, row0 / p.group, (row0 + *live - 1) / p.group);
 }
 __device__ __forceinline__ int64_t work_of(const PagedParams& p, const PagedSeq& v) {
   int64_t sum = 0;
@@ -70,6 +70,11 @@ __device__ __forceinline__ int64_t work_of(const PagedParams& p, const PagedSeq&
     sum += kUnitCost + max(span_of_tile(p, v, i, &live).tiles, 1);
   }
   return sum * p.nh;
+}
+
+// 64-bit division takes the time of a trip to memory; most fit 32 bits.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
 // A run: units one after another, the tiles of a (sequence, head) next to one another.
@@ -119,6 +124,19 @@ __device__ __forceinline__ void store4(uint16_t* dst, float4 o, float f) {
   }
 }
 
+// Four columns of a row's sum over some of its tokens.
+struct Sum {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(const Sum& y) {
+    const float now = fmaxf(m, y.m);
+    const float a = now == -INFINITY ? 1.f : exp2_near(m - now), b = now == -INFINITY ? 1.f : exp2_near(y.m - now);
+    o.x = o.x * a + y.o.x * b, o.y = o.y * a + y.o.y * b, o.z = o.z * a + y.o.z * b, o.w = o.w * a + y.o.w * b;
+    l = l * a + y.l * b;
+    m = now;
+  }
+};
+
 // Partial sums: [16][HD] accumulators, 16 maxima, 16 sums.
 template <int HD>
 constexpr int kPieceFloats = kRows * (HD + 2);
@@ -134,6 +152,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&v_map) : "memory");
     sm.gave_up = 0;
     for (int i = 0; i < kWarps * kStages; ++i) mbar_init(&sm.full[0][0] + i, 1);
     mbar_init_fence();
@@ -162,10 +182,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm.before[tid] = at;
     if (tid == kThreads - 1) sm.before[kThreads] = at + mine;
     if (tid < 2 * kWarps) sm.pieces[tid].wt = -1;
+    if (tid < 2) sm.join[tid] = -1;
     __syncthreads();
   }
   const int64_t total = sm.before[kThreads];
-  int64_t run = (total + gridDim.x * kWarps - 1) / (gridDim.x * kWarps);
+  int64_t run = divide(total + gridDim.x * kWarps - 1, gridDim.x * kWarps);
   if (run < kMinRun) run = kMinRun;
   const int64_t block_run = run * kWarps, block_begin = blockIdx.x * block_run;
   if (block_begin >= total) return;
@@ -189,8 +210,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t work = work_of(p, walk.v);
       if (walk.w < at + work) {
         walk.tiles = tiles_of(p, walk.v);
-        const int64_t one = work / p.nh;
-        walk.head = static_cast<int>((walk.w - at) / one);
+        const int64_t one = divide(work, p.nh);
+        walk.head = static_cast<int>(divide(walk.w - at, one));
         at += one * walk.head;
         break;
       }
@@ -282,9 +303,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
       const int x = r + 8 * z;
-      const int64_t row = static_cast<int64_t>(u.tile) * kRows + min(x, u.live - 1);
-      who[z] = static_cast<int>(row / p.group);
-      const int j = static_cast<int>(row - static_cast<int64_t>(who[z]) * p.group);
+      const int row = u.tile * kRows + min(x, u.live - 1);
+      who[z] = row / p.group;
+      const int j = row - who[z] * p.group;
       row_q[z] = (static_cast<int64_t>(u.v.first) + who[z]) * p.q_sr + (static_cast<int64_t>(u.head) * p.group + j) * p.q_sh;
       see[z] = row_view(p, u.v, who[z]);
     }
@@ -428,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int z = 0; z < 2; ++z) {
         if (r + 8 * z >= live) continue;
-        const int64_t row = static_cast<int64_t>(u.tile) * kRows + r + 8 * z;
+        const int row = u.tile * kRows + r + 8 * z;
         const int64_t i = u.v.first + row / p.group, h = static_cast<int64_t>(u.head) * p.group + row % p.group;
         uint16_t* dst = static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh + c2;
         const float inv = l[z] > 0.f || l[z] != l[z] ? 1.f / l[z] : 0.f;
@@ -474,81 +495,111 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   __syncthreads();
 
-  // ---- pieces of the same unit ----------------------------------------------------------------
-  auto finish = [&](const Piece& x, int row_in, int d, float4 sum, float mx, float l_sum) {
-    const int64_t row = static_cast<int64_t>(x.tile) * kRows + row_in;
+  // ---- pieces of the same unit: a warp for each unit, then the block for what other blocks have left ----------
+  auto finish = [&](const Piece& x, int row_in, int d, const Sum& s) {
+    const int row = x.tile * kRows + row_in;
     const int64_t i = x.first + row / p.group, h = static_cast<int64_t>(x.head) * p.group + row % p.group;
-    const bool any = l_sum > 0.f || l_sum != l_sum;
-    store4<BF16>(static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh + d, sum, any ? 1.f / l_sum : 0.f);
-    if (p.lse != nullptr && d == 0)
-      p.lse[i * p.nh * p.group + h] = any ? (mx - kLift + log2f(l_sum)) * 0.69314718055994531f : -INFINITY;
+    const bool any = s.l > 0.f || s.l != s.l;
+    store4<BF16>(static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh + d, s.o, any ? 1.f / s.l : 0.f);
+    if (p.lse != nullptr && d == 0) p.lse[i * p.nh * p.group + h] = any ? (s.m - kLift + log2f(s.l)) * 0.69314718055994531f : -INFINITY;
   };
-  for (int g0 = 0; g0 < 2 * kWarps;) {
-    const int64_t wt = sm.pieces[g0].wt;
-    if (wt < 0) {
-      ++g0;
-      continue;
-    }
-    int g1 = g0 + 1;  // pieces [g0, g1), some of them empty places
-    while (g1 < 2 * kWarps && (sm.pieces[g1].wt < 0 || sm.pieces[g1].wt == wt)) ++g1;
-    const Piece& x = sm.pieces[g0];
-    const int64_t first = wt / block_run, last = (wt + x.len - 1) / block_run;
-    float* mine = p.partial + (static_cast<int64_t>(gridDim.x) * (2 * kWarps) + 2 * blockIdx.x + (wt > block_begin ? 1 : 0)) * kPieceFloats<HD>;
-    for (int item = tid; item < x.live * (HD / 4); item += kThreads) {
-      const int row = item / (HD / 4), d = item % (HD / 4) * 4;
-      float mx = -INFINITY, l_sum = 0.f;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int g = g0; g < g1; ++g) {
-        if (sm.pieces[g].wt < 0) continue;
-        const float* at = sm.pieces[g].at;
-        const float pm = at[kRows * HD + row], pl = at[kRows * HD + kRows + row];
-        const float4 po = *reinterpret_cast<const float4*>(at + row * HD + d);
-        const float now = fmaxf(mx, pm);
-        const float a = now == -INFINITY ? 1.f : exp2_near(mx - now), b = now == -INFINITY ? 1.f : exp2_near(pm - now);
-        sum.x = sum.x * a + po.x * b, sum.y = sum.y * a + po.y * b, sum.z = sum.z * a + po.z * b, sum.w = sum.w * a + po.w * b;
-        l_sum = l_sum * a + pl * b;
-        mx = now;
-      }
-      if (first == last) {
-        finish(x, row, d, sum, mx, l_sum);
-      } else {
-        *reinterpret_cast<float4*>(mine + row * HD + d) = sum;
-        if (d == 0) mine[kRows * HD + row] = mx, mine[kRows * HD + kRows + row] = l_sum;
-      }
-    }
-    if (first != last) {
-      __syncthreads();
-      if (tid == 0) {  // releases what the barrier has gathered
-        int ticket;
-        asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + first) : "memory");
-        sm.last = ticket == last - first;
-      }
-      __syncthreads();
-      if (sm.last) {
-        auto from = [&](int64_t b) {
-          return p.partial + (static_cast<int64_t>(gridDim.x) * (2 * kWarps) + 2 * b + (wt > b * block_run ? 1 : 0)) * kPieceFloats<HD>;
-        };
-        for (int item = tid; item < x.live * (HD / 4); item += kThreads) {
-          const int row = item / (HD / 4), d = item % (HD / 4) * 4;
-          float mx = -INFINITY, l_sum = 0.f;
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int64_t b = first; b <= last; ++b) {
-            const float* at = from(b);
-            const float pm = __ldcg(at + kRows * HD + row), pl = __ldcg(at + kRows * HD + kRows + row);
-            const float4 po = __ldcg(reinterpret_cast<const float4*>(at + row * HD + d));
-            const float now = fmaxf(mx, pm);
-            const float fa = now == -INFINITY ? 1.f : exp2_near(mx - now), fb = now == -INFINITY ? 1.f : exp2_near(pm - now);
-            sum.x = sum.x * fa + po.x * fb, sum.y = sum.y * fa + po.y * fb, sum.z = sum.z * fa + po.z * fb, sum.w = sum.w * fa + po.w * fb;
-            l_sum = l_sum * fa + pl * fb;
-            mx = now;
+  auto of_block = [&](int64_t b, int64_t wt) {  // a block's sum of a unit that others share
+    return p.partial + (static_cast<int64_t>(gridDim.x) * (2 * kWarps) + 2 * b + (wt > b * block_run ? 1 : 0)) * kPieceFloats<HD>;
+  };
+  {
+    const int64_t wt_mine = lane < 2 * kWarps ? sm.pieces[lane].wt : -1;
+    const uint32_t used = __ballot_sync(0xffffffffu, wt_mine >= 0);
+    const uint32_t lower = used & ((1u << lane) - 1);
+    const int64_t wt_before = __shfl_sync(0xffffffffu, wt_mine, lower ? 31 - __clz(lower) : 0);
+    uint32_t heads = __ballot_sync(0xffffffffu, wt_mine >= 0 && (lower == 0 || wt_before != wt_mine));
+    for (int k = 0; heads != 0; ++k) {
+      const int g = __ffs(heads) - 1;
+      heads &= heads - 1;
+      if (k % kWarps != warp) continue;
+      const uint32_t members = used & (heads ? (1u << (__ffs(heads) - 1)) - 1 : 0xffffffffu) & ~((1u << g) - 1);
+      const Piece& x = sm.pieces[g];
+      const int64_t wt = x.wt, first = divide(wt, block_run), last = divide(wt + x.len - 1, block_run);
+      const int live = x.live;
+      float* mine = of_block(blockIdx.x, wt);
+      constexpr int kAcross = HD / 4, kDown = 32 / kAcross;  // lanes of a row, rows at once
+      const int d = lane % kAcross * 4;
+      for (int row0 = lane / kAcross; row0 < live; row0 += 4 * kDown) {
+        Sum sum[4];
+        for (uint32_t left = members; left != 0; left &= left - 1) {
+          const float* at = sm.pieces[__ffs(left) - 1].at;
+          Sum y[4];
+#pragma unroll
+          for (int z = 0; z < 4; ++z) {
+            const int row = min(row0 + z * kDown, live - 1);
+            y[z].m = at[kRows * HD + row], y[z].l = at[kRows * HD + kRows + row];
+            y[z].o = *reinterpret_cast<const float4*>(at + row * HD + d);
           }
-          finish(x, row, d, sum, mx, l_sum);
+#pragma unroll
+          for (int z = 0; z < 4; ++z) sum[z].add(y[z]);
         }
-        if (tid == 0) p.counters[first] = 0;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const int row = row0 + z * kDown;
+          if (row >= live) continue;
+          if (first == last) {
+            finish(x, row, d, sum[z]);
+          } else {
+            *reinterpret_cast<float4*>(mine + row * HD + d) = sum[z].o;
+            if (d == 0) mine[kRows * HD + row] = sum[z].m, mine[kRows * HD + kRows + row] = sum[z].l;
+          }
+        }
+      }
+      if (first != last) {
+        __syncwarp();
+        if (lane == 0) {  // releases what the warp has written
+          int ticket;
+          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + first) : "memory");
+          if (ticket == last - first) {
+            sm.join[wt > block_begin ? 1 : 0] = g;
+            p.counters[first] = 0;
+          }
+        }
       }
     }
-    g0 = g1;
+  }
+  __syncthreads();
+  for (int which = 0; which < 2; ++which) {
+    const int g = sm.join[which];
+    if (g < 0) continue;
+    const Piece& x = sm.pieces[g];
+    const int64_t wt = x.wt, first = divide(wt, block_run), last = divide(wt + x.len - 1, block_run);
+    const int items = x.live * (HD / 4);
+    const int parts = items < kThreads ? kThreads / items : 1;  // of the blocks, for rows too few for all threads
+    Sum* shared = reinterpret_cast<Sum*>(sm.ring);
+    for (int i = tid; i < items * parts; i += kThreads) {
+      const int item = i % items, part = i / items, row = item / (HD / 4), d = item % (HD / 4) * 4;
+      Sum sum;
+      for (int64_t b = first + part; b <= last; b += 4 * parts) {
+        Sum y[4];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const float* at = of_block(min(b + z * parts, last), wt);
+          y[z].m = __ldcg(at + kRows * HD + row), y[z].l = __ldcg(at + kRows * HD + kRows + row);
+          y[z].o = __ldcg(reinterpret_cast<const float4*>(at + row * HD + d));
+        }
+#pragma unroll
+        for (int z = 0; z < 4; ++z)
+          if (b + z * parts <= last) sum.add(y[z]);
+      }
+      if (parts == 1)
+        finish(x, row, d, sum);
+      else
+        shared[i] = sum;
+    }
+    if (parts > 1) {
+      __syncthreads();
+      if (tid < items) {
+        Sum sum;
+        for (int part = 0; part < parts; ++part) sum.add(shared[part * items + tid]);
+        finish(x, tid / (HD / 4), tid % (HD / 4) * 4, sum);
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -630,6 +681,8 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
     return fail(MAK_E_INVALID, "%s: %d query heads over %d cache heads", name, d->num_q_heads, c.num_heads);
   if (d->window < 0 || d->sinks < 0) return fail(MAK_E_INVALID, "%s: negative window or sinks", name);
   if (d->parents != nullptr && d->window) return fail(MAK_E_INVALID, "%s: a tree has no window", name);
+  if (c.num_rows * d->num_q_heads / c.num_heads > 0x7fffffff - 256)
+    return fail(MAK_E_UNSUPPORTED, "%s: rows times query heads of a cache head are a 32-bit count", name);
   if (c.num_seqs == 0 || c.num_rows == 0) return MAK_OK;
   if (d->q == nullptr || d->out == nullptr) return fail(MAK_E_INVALID, "%s: null q or out", name);
   if ((reinterpret_cast<uintptr_t>(d->q) & 15) || ((d->q_stride_row | d->q_stride_head) & 7))

@@ -51,12 +51,11 @@ struct Plan {
 
 // Rows of row tile `tile` of a sequence (numbers below the first sequence's come as negative ones) and what they see.
 __device__ __forceinline__ int live_rows(const PagedParams& p, const PagedSeq& v, int tile) {
-  const int64_t left = static_cast<int64_t>(v.rows) * p.group - static_cast<int64_t>(tile) * kUnitRows;
-  return tile < 0 || left <= 0 ? 0 : left < kUnitRows ? static_cast<int>(left) : kUnitRows;
+  return tile < 0 ? 0 : max(min(v.rows * p.group - tile * kUnitRows, kUnitRows), 0);
 }
 __device__ __forceinline__ Span span_of_rows(const PagedParams& p, const PagedSeq& v, int tile, int row_a, int row_b) {
-  const int64_t row0 = static_cast<int64_t>(tile) * kUnitRows;
-  return span_of<kTile>(p, v, static_cast<int>((row0 + row_a) / p.group), static_cast<int>((row0 + row_b) / p.group));
+  const int row0 = tile * kUnitRows;
+  return span_of<kTile>(p, v, (row0 + row_a) / p.group, (row0 + row_b) / p.group);
 }
 __device__ __forceinline__ int unit_len(const PagedParams& p, const PagedSeq& v, int tile) {
   const int live = live_rows(p, v, tile);
@@ -341,8 +340,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row_in = solo ? r : half * kHalf + r;  // of the unit
       const bool active = solo || half * kHalf < u.live;
       const bool on = row_in < u.live;
-      const int64_t row = static_cast<int64_t>(u.tile) * kUnitRows + (on ? row_in : 0);
-      const int who = static_cast<int>(row / p.group), head = u.head * p.group + static_cast<int>(row - static_cast<int64_t>(who) * p.group);
+      const int row = u.tile * kUnitRows + (on ? row_in : 0);
+      const int who = row / p.group, head = u.head * p.group + row - who * p.group;
       const int first = solo ? half : 0, step = solo ? 2 : 1;
       const int n = active && u.n > first ? (u.n - first + step - 1) / step : 0;  // tiles of this half
       float m = -INFINITY, l = 0.f;
@@ -457,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) l = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN, not stale memory
 
       // ---- this half's share of the unit -------------------------------------------
-      auto place = [&](int64_t row, uint16_t*& dst, float*& lse) {  // of a row's result
+      auto place = [&](int row, uint16_t*& dst, float*& lse) {  // of a row's result
         const int64_t i = u.v.first + row / p.group, h = static_cast<int64_t>(u.head) * p.group + row % p.group;
         dst = static_cast<uint16_t*>(p.out) + i * p.o_sr + h * p.o_sh;
         lse = p.lse == nullptr ? nullptr : p.lse + i * p.nh * p.group + h;
@@ -562,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float ms = mx == -INFINITY ? 0.f : mx, inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
             uint16_t* dst;
             float* lse;
-            place(static_cast<int64_t>(u.tile) * kUnitRows + (solo ? 0 : half * kHalf) + mine_row, dst, lse);
+            place(u.tile * kUnitRows + (solo ? 0 : half * kHalf) + mine_row, dst, lse);
 #pragma unroll 1
             for (int d = r / span * cols, end = d + cols; d < end; d += 16) {
               float o[16];

@@ -334,6 +334,8 @@ extern "C" int mak_paged_weights(const mak_paged_weights_desc* d, void* stream) 
   if (d->max_tokens < 0 || d->max_tokens > 0x7fffffff - 16 || d->sum_rows < 0)
     return fail(MAK_E_INVALID, "%s: sums of %lld rows of %lld tokens", name, static_cast<long long>(d->sum_rows),
                 static_cast<long long>(d->max_tokens));
+  if (c.num_rows * d->num_q_heads / c.num_heads > 0x7fffffff - 256)
+    return fail(MAK_E_UNSUPPORTED, "%s: rows times query heads of a cache head are a 32-bit count", name);
   if (c.num_seqs == 0 || d->max_tokens == 0 || d->sum_rows == 0) return MAK_OK;
   if (d->sums == nullptr || (c.num_rows > 0 && (d->q == nullptr || d->lse == nullptr)))
     return fail(MAK_E_INVALID, "%s: null q, lse or sums", name);
