@@ -10,12 +10,16 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <array>
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <tuple>
@@ -844,20 +848,28 @@ PyObject* py_evict(PyObject*, Args a, Py_ssize_t n) {
 
 struct NormArgs {
   at::Tensor q, k, wq, wk, pos, cos, sin;
+  double eps;
+  bool interleaved;
 };
-// Arguments from `a`: q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved
-mak_qk_norm_rope_desc norm_desc(const char* name, Args a, NormArgs& x) {
-  const at::Tensor &q = tensor(name, "q", a[0]), &k = tensor(name, "k", a[1]);
-  const at::Tensor &wq = tensor(name, "q_weight", a[2]), &wk = tensor(name, "k_weight", a[3]);
-  x.pos = tensor(name, "positions", a[4]), x.cos = tensor(name, "cos", a[5]), x.sin = tensor(name, "sin", a[6]);
+// q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved
+NormArgs norm_args(const char* name, Args a) {
+  NormArgs x{tensor(name, "q", a[0]), tensor(name, "k", a[1]), tensor(name, "q_weight", a[2]), tensor(name, "k_weight", a[3]),
+             tensor(name, "positions", a[4]), tensor(name, "cos", a[5]), tensor(name, "sin", a[6]), 0.0, false};
+  x.eps = PyFloat_AsDouble(a[7]);
+  if (x.eps == -1.0 && PyErr_Occurred()) throw python_error();
+  x.interleaved = truth(a[8]);
+  return x;
+}
+mak_qk_norm_rope_desc norm_desc(const char* name, const NormArgs& x) {
+  const at::Tensor &q = x.q, &k = x.k;
   if (q.dim() != 3 || k.dim() != 3 || q.size(0) != k.size(0) || q.size(2) != k.size(2))
     refuse(name, "q and k must be [tokens, heads, head_dim] with the same tokens and head_dim");
   const at::ScalarType kind = q.scalar_type();
   if ((kind != at::kHalf && kind != at::kBFloat16) || k.scalar_type() != kind) refuse(name, "q and k must both be float16 or both bfloat16");
   const int64_t tokens = q.size(0), hd = q.size(2);
   if (hd < 16 || hd > 256 || hd % 16) refuse(name, "head_dim must be a multiple of 16 up to 256, got ", hd);
-  for (const at::Tensor* w : {&wq, &wk})
-    if (w->dim() != 1 || w->size(0) != hd || (w->scalar_type() != at::kFloat && w->scalar_type() != kind) || w->scalar_type() != wq.scalar_type())
+  for (const at::Tensor* w : {&x.wq, &x.wk})
+    if (w->dim() != 1 || w->size(0) != hd || (w->scalar_type() != at::kFloat && w->scalar_type() != kind) || w->scalar_type() != x.wq.scalar_type())
       refuse(name, "weights must both be [head_dim] in float32 or in q's type");
   if (x.pos.dim() != 1 || x.pos.size(0) != tokens || (x.pos.scalar_type() != at::kInt && x.pos.scalar_type() != at::kLong))
     refuse(name, "positions must be int32 or int64 [tokens]");
@@ -865,15 +877,12 @@ mak_qk_norm_rope_desc norm_desc(const char* name, Args a, NormArgs& x) {
     refuse(name, "cos and sin must both be float32 [max_positions, pairs]");
   const int64_t pairs = x.cos.size(1);
   if (pairs % 8 || 2 * pairs > hd) refuse(name, "the tables must have a multiple of 8 pairs, at most head_dim / 2, got ", pairs);
-  const double eps = PyFloat_AsDouble(a[7]);
-  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
-  if (!(eps >= 0.0)) refuse(name, "eps must not be negative");
+  if (!(x.eps >= 0.0)) refuse(name, "eps must not be negative");
   mak_qk_norm_rope_desc d = {};
-  d.interleaved = truth(a[8]), d.eps = static_cast<float>(eps);
-  x.q = q, x.k = k, x.wq = wq, x.wk = wk;
+  d.interleaved = x.interleaved, d.eps = static_cast<float>(x.eps);
   d.tokens = tokens, d.max_positions = x.cos.size(0);
   d.q_heads = static_cast<int32_t>(q.size(1)), d.k_heads = static_cast<int32_t>(k.size(1)), d.head_dim = static_cast<int32_t>(hd);
-  d.rot_dim = static_cast<int32_t>(2 * pairs), d.dtype = float_code(kind), d.weight_dtype = float_code(wq.scalar_type());
+  d.rot_dim = static_cast<int32_t>(2 * pairs), d.dtype = float_code(kind), d.weight_dtype = float_code(x.wq.scalar_type());
   d.pos_dtype = x.pos.scalar_type() == at::kInt ? MAK_DT_I32 : MAK_DT_I64;
   return d;
 }
@@ -895,66 +904,113 @@ void norm_inputs(mak_qk_norm_rope_desc& d, NormArgs& x) {
   d.qo_stride_head = d.ko_stride_head = d.head_dim;
 }
 
-// the nine of norm_desc; None where q, k or a weight wants a gradient
+std::array<at::Tensor, 2> norm_forward(NormArgs x) {
+  const char* name = "apply_qk_norm_rope";
+  Device dev{name};
+  mak_qk_norm_rope_desc d = norm_desc(name, x);
+  norm_on(dev, x);
+  const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
+  norm_inputs(d, x);
+  const at::ScalarType kind = x.q.scalar_type();
+  std::array<at::Tensor, 2> y = {empty(x.q.sizes(), kind, x.q.device()), empty(x.k.sizes(), kind, x.q.device())};
+  d.q_out = y[0].data_ptr(), d.k_out = y[1].data_ptr();
+  check(lib.norm_rope(&d, stream_of(dev)), name);
+  return y;
+}
+
+std::array<at::Tensor, 4> norm_backward(const at::Tensor& gq0, const at::Tensor& gk0, NormArgs x) {
+  const char* name = "apply_qk_norm_rope_backward";
+  Device dev{name};
+  mak_qk_norm_rope_desc d = norm_desc(name, x);
+  if (gq0.sizes() != x.q.sizes() || gk0.sizes() != x.k.sizes() || gq0.scalar_type() != x.q.scalar_type() || gk0.scalar_type() != x.q.scalar_type())
+    refuse(name, "grad_q and grad_k must have the shapes and type of q and k");
+  dev.add(gq0);
+  dev.add(gk0);
+  norm_on(dev, x);
+  const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
+  norm_inputs(d, x);
+  const at::Tensor gq = aligned_rows(gq0), gk = aligned_rows(gk0);
+  const at::ScalarType kind = x.q.scalar_type(), weight = x.wq.scalar_type();
+  std::array<at::Tensor, 4> got = {empty(x.q.sizes(), kind, x.q.device()), empty(x.k.sizes(), kind, x.q.device()),
+                                   empty(x.wq.sizes(), weight, x.q.device()), empty(x.wk.sizes(), weight, x.q.device())};
+  const at::Tensor partial = empty({lib.norm_partial(d.head_dim)}, at::kFloat, x.q.device());
+  // a tensor without elements has no address, but the call is still a backward one
+  static float none[4];
+  auto address = [](const at::Tensor& t) { return t.numel() ? t.data_ptr() : static_cast<void*>(none); };
+  d.grad_q = address(gq), d.grad_k = address(gk);
+  d.gq_stride_token = gq.stride(0), d.gq_stride_head = gq.stride(1), d.gk_stride_token = gk.stride(0), d.gk_stride_head = gk.stride(1);
+  d.q_out = got[0].data_ptr(), d.k_out = got[1].data_ptr(), d.grad_q_weight = got[2].data_ptr(), d.grad_k_weight = got[3].data_ptr();
+  d.partial = static_cast<float*>(partial.data_ptr());
+  check(lib.norm_rope(&d, stream_of(dev)), name);
+  return got;
+}
+
+// The node of a call whose q, k or weights want a gradient.
+struct NormNode : torch::autograd::Function<NormNode> {
+  using Context = torch::autograd::AutogradContext;
+  using List = torch::autograd::variable_list;
+  static List forward(Context* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& pos,
+                      const at::Tensor& cos, const at::Tensor& sin, double eps, bool interleaved) {
+    ctx->save_for_backward({q, k, wq, wk, pos, cos, sin});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    const auto y = norm_forward({q, k, wq, wk, pos, cos, sin, eps, interleaved});
+    return {y[0], y[1]};
+  }
+  // Runs on a thread of autograd's: only exceptions of the standard library may leave it.
+  static List backward(Context* ctx, List grads) {
+    const List s = ctx->get_saved_variables();
+    List got;
+    try {
+      const auto g = norm_backward(grads[0], grads[1], {s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["eps"].toDouble(),
+                                                        ctx->saved_data["interleaved"].toBool()});
+      got.assign(g.begin(), g.end());
+    } catch (const Refused& r) {
+      TORCH_CHECK(false, r.text);
+    }
+    if (c10::GradMode::is_enabled()) {  // a graph of the gradient is wanted: it ends here, in an error when it is walked
+      for (at::Tensor& t : got) t.set_requires_grad(true);
+      got = std::make_shared<torch::autograd::DelayedError>("apply_qk_norm_rope: the gradient has no gradient of its own", 4)->apply(std::move(got));
+    }
+    got.resize(9);
+    return got;
+  }
+};
+
+// the nine of norm_args
 PyObject* py_norm(PyObject*, Args a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const char* name = "apply_qk_norm_rope";
     count(name, n, 9);
-    Device dev{name};
-    NormArgs x;
+    const NormArgs x = norm_args(name, a);
+    bool wants = false;
     if (c10::GradMode::is_enabled()) {
-      for (int i : {5, 6})
-        if (tensor(name, "cos and sin", a[i]).requires_grad()) refuse(name, "cos and sin are tables without a gradient, detach them");
-      for (int i = 0; i < 4; ++i)
-        if (tensor(name, "q, k and the weights", a[i]).requires_grad()) Py_RETURN_NONE;  // the autograd function calls again, gradients off
+      if (x.cos.requires_grad() || x.sin.requires_grad()) refuse(name, "cos and sin are tables without a gradient, detach them");
+      for (const at::Tensor* t : {&x.q, &x.k, &x.wq, &x.wk}) wants = wants || t->requires_grad();
     }
-    mak_qk_norm_rope_desc d = norm_desc(name, a, x);
-    norm_on(dev, x);
-    const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
-    norm_inputs(d, x);
-    const at::ScalarType kind = x.q.scalar_type();
-    const at::Tensor q_out = empty(x.q.sizes(), kind, x.q.device()), k_out = empty(x.k.sizes(), kind, x.q.device());
-    d.q_out = q_out.data_ptr(), d.k_out = k_out.data_ptr();
-    check(lib.norm_rope(&d, stream_of(dev)), name);
+    PyObject* got;
+    if (wants) {
+      const auto y = NormNode::apply(x.q, x.k, x.wq, x.wk, x.pos, x.cos, x.sin, x.eps, x.interleaved);
+      got = wrap(y[0], y[1]);
+    } else {
+      const auto y = norm_forward(x);
+      got = wrap(y[0], y[1]);
+    }
     trace(name, a[0], "sm100a norms and rotary positions");
-    return wrap(q_out, k_out);
+    return got;
   });
 }
 
-// grad_q, grad_k, the nine of norm_desc
+// grad_q, grad_k, the nine of norm_args
 PyObject* py_norm_back(PyObject*, Args a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     const char* name = "apply_qk_norm_rope_backward";
     count(name, n, 11);
-    const at::Tensor &gq0 = tensor(name, "grad_q", a[0]), &gk0 = tensor(name, "grad_k", a[1]);
-    Device dev{name};
-    NormArgs x;
-    mak_qk_norm_rope_desc d = norm_desc(name, a + 2, x);
-    if (gq0.sizes() != x.q.sizes() || gk0.sizes() != x.k.sizes() || gq0.scalar_type() != x.q.scalar_type() || gk0.scalar_type() != x.q.scalar_type())
-      refuse(name, "grad_q and grad_k must have the shapes and type of q and k");
-    dev.add(gq0);
-    dev.add(gk0);
-    norm_on(dev, x);
-    const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
-    norm_inputs(d, x);
-    const at::Tensor gq = aligned_rows(gq0), gk = aligned_rows(gk0);
-    const at::ScalarType kind = x.q.scalar_type();
-    const at::Tensor dq = empty(x.q.sizes(), kind, x.q.device()), dk = empty(x.k.sizes(), kind, x.q.device());
-    const at::Tensor dwq = empty(x.wq.sizes(), x.wq.scalar_type(), x.q.device()), dwk = empty(x.wk.sizes(), x.wk.scalar_type(), x.q.device());
-    const at::Tensor partial = empty({lib.norm_partial(d.head_dim)}, at::kFloat, x.q.device());
-    // a tensor without elements has no address, but the call is still a backward one
-    static float none[4];
-    auto address = [](const at::Tensor& t) { return t.numel() ? t.data_ptr() : static_cast<void*>(none); };
-    d.grad_q = address(gq), d.grad_k = address(gk);
-    d.gq_stride_token = gq.stride(0), d.gq_stride_head = gq.stride(1), d.gk_stride_token = gk.stride(0), d.gk_stride_head = gk.stride(1);
-    d.q_out = dq.data_ptr(), d.k_out = dk.data_ptr(), d.grad_q_weight = dwq.data_ptr(), d.grad_k_weight = dwk.data_ptr();
-    d.partial = static_cast<float*>(partial.data_ptr());
-    check(lib.norm_rope(&d, stream_of(dev)), name);
+    const auto got = norm_backward(tensor(name, "grad_q", a[0]), tensor(name, "grad_k", a[1]), norm_args(name, a + 2));
     trace(name, a[0], "sm100a gradient of norms and rotary positions");
     PyObject* all = PyTuple_New(4);
     if (all == nullptr) throw python_error();
-    const at::Tensor* got[4] = {&dq, &dk, &dwq, &dwk};
-    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(all, i, THPVariable_Wrap(*got[i]));
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(all, i, THPVariable_Wrap(got[i]));
     return all;
   });
 }

@@ -7,27 +7,10 @@ rotation.  Angles come as cos / sin tables indexed by position, as in ``apply_ro
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _native
 
 __all__ = ["apply_qk_norm_rope", "apply_qk_norm_rope_backward"]
-
-
-class _NormRotation(torch.autograd.Function):
-    """The native call answers None where an input wants a gradient; here it is made again with gradients off."""
-
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved):
-        args = (q, k, q_weight, k_weight, positions, cos, sin)
-        ctx.save_for_backward(*args)
-        ctx.how = (eps, interleaved)
-        return _native.front().norm(*args, eps, interleaved)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_q, grad_k):
-        return (*_native.front().norm_back(grad_q, grad_k, *ctx.saved_tensors, *ctx.how), *(None,) * 5)
 
 
 def apply_qk_norm_rope(
@@ -48,9 +31,10 @@ def apply_qk_norm_rope(
     ``[max_positions, pairs]``.  Pair j is (j, j + pairs), or (2 j, 2 j + 1) with ``interleaved``, of the first 2 * pairs
     columns; the others are normalised alone, and so is a token whose position lies outside the tables.  head_dim is a
     multiple of 16 up to 256, pairs a multiple of 8.  Computed in 32 bits and rounded once.  Returns new tensors,
-    through which q, k and the weights get their gradients; cos and sin get none and may not require one."""
-    args = (q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
-    return _native.front().norm(*args) or _NormRotation.apply(*args)
+    through which q, k and the weights get their gradients (these have none of their own); cos and sin get none and may
+    not require one.  A backward pass is captured into a CUDA graph like any of torch's: no eager graph of the same leaves
+    may live meanwhile."""
+    return _native.front().norm(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
 
 
 def apply_qk_norm_rope_backward(

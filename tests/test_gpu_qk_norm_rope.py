@@ -223,3 +223,42 @@ def test_captured_and_the_same_every_time():
     torch.cuda.synchronize()
     for other in (again, kept):
         assert all(torch.equal(a, b) for x, y in zip(first, other) for a, b in zip(x, y))
+
+
+def test_the_gradient_has_no_gradient():
+    """A graph of the gradient may be asked for; walking it is refused, and the process lives on."""
+    c = Case(5, 2, 1)
+    args = c.inputs()
+    args[0].requires_grad_()
+    y = ma.apply_qk_norm_rope(*args)
+    (dq,) = torch.autograd.grad(y[0].sum(), args[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        dq.float().square().sum().backward()
+    y = ma.apply_qk_norm_rope(*args)
+    with torch.no_grad():
+        args[0].zero_()  # what was saved has changed
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y[0].sum().backward()
+
+
+def test_backward_captured():
+    """Forward and backward in one graph, as torch captures any: no eager graph of the same leaves lives meanwhile."""
+    c = Case(200, 4, 2, hd=128)
+    args = c.inputs()
+    for x in args[:4]:
+        x.requires_grad_()
+    grads = (c.gq.cuda(), c.gk.cuda())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = torch.autograd.grad(ma.apply_qk_norm_rope(*args), args[:4], grads)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        kept = torch.autograd.grad(ma.apply_qk_norm_rope(*args), args[:4], grads)
+    for x in kept:
+        x.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    c.check_gradients(kept)
+    assert all(torch.equal(a, b) for a, b in zip(first, kept))
