@@ -20,7 +20,7 @@
 // kept out by warps 12-15; the rows that do see such a value get it with their results (odd_sum).
 //
 // Work.  All (row tile, head) units laid end to end, each as long as the tiles it sees, are cut into equal runs, one per
-// block; a small launch before this one adds up the lengths.  A unit cut by that leaves partial sums, and the last half to
+// block; a small launch before this one adds up the lengths.  A unit cut by that leaves partial sums, and the last block to
 // arrive joins them in order of position, so results do not depend on timing.
 #include <utility>
 
@@ -196,6 +196,7 @@ __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile
   return __all_sync(0xffffffffu, ok);
 }
 
+__device__ __forceinline__ void both_sync() { asm volatile("bar.sync 3, 256;" ::: "memory"); }
 __device__ __forceinline__ void half_sync(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
 
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
@@ -534,11 +535,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (split && active) {
         const int64_t first_block = u.wt / chunk, last_block = (u.wt + u.len - 1) / chunk;
         const int64_t slot0 = (2 * first_block + (u.wt > first_block * chunk ? 1 : 0)) * 2 + (solo ? 0 : half);
-        half_sync(half);
+        // A solo unit is both halves': the first of them joins it when both have written, and no half writes its next
+        // piece, which may have the same place, before that is done.
+        if (solo)
+          both_sync();
+        else
+          half_sync(half);
         if (r == 0) {  // releases what the barrier has gathered
-          int ticket;
-          asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + slot0) : "memory");
-          sm.last[half] = ticket == (last_block - first_block + 1) * (solo ? 2 : 1) - 1;
+          bool last = !solo || half == 0;
+          if (last && cut) {
+            int ticket;
+            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + slot0) : "memory");
+            last = ticket == last_block - first_block;
+            if (last) p.counters[slot0] = 0;
+          }
+          sm.last[half] = last;
         }
         half_sync(half);
         if (sm.last[half]) {
@@ -588,8 +599,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (r < span) put_lse(lse, mx, sum);
           }
-          if (r == 0) p.counters[slot0] = 0;
         }
+        if (solo) both_sync();
       }
       half_sync(half);  // the unit is read
     }

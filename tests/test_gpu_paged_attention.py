@@ -344,3 +344,27 @@ def test_head_dims_and_types_refused_on_the_gpu():
         ma.paged_attention_window(c.on("q").half(), *c.on("layer"), c.on("tables"), c.on("lens"))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ma.paged_attention_window(c.on("q"), *c.on("layer"), c.tables, c.on("lens"))
+
+
+@pytest.mark.parametrize("group,new,ctx", [(2, 20, 300), (4, 32, 900), (3, 100, 450), (1, 300, 500)])
+def test_many_units_to_a_block(group, new, ctx):
+    """More units than blocks, some of them cut, between calls of other values and of other kernels on the same stream: each
+    call's results are its own, from the first to the last."""
+    n = 48
+    lens = [ctx - 7 * i % 90 for i in range(n)]
+    news = [max(1, new - i % 11) for i in range(n)]
+    c, other = (Cache(lens, news, nh=8, group=group, hd=128, seed=seed) for seed in (1, 2))
+    few_rows = Cache([4000] * 3, nh=8, group=4, hd=128, seed=3)
+    want, want_lse, bound = c.attention(200, 3)
+    want_few, few_lse, few_bound = few_rows.attention()
+    p = random_parents(c)
+    want_tree, tree_lse, tree_bound = c.attention(parents=p)
+    for _ in range(4):
+        window(other, 200, 3)
+        got = window(c, 200, 3)
+        tree(other, p)
+        got_tree = tree(c, p)
+        got_few = window(few_rows)
+        check(got[0], want, got[1], want_lse, bound)
+        check(got_tree[0], want_tree, got_tree[1], tree_lse, tree_bound)
+        check(got_few[0], want_few, got_few[1], few_lse, few_bound, True)
