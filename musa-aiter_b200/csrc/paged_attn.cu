@@ -22,7 +22,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxGrid = 148;
 constexpr int kUnitCost = 2;  // a unit's beginning and end, in steps
-constexpr int kMinRun = 4;    // steps that are worth another warp
+constexpr int kMinRun = 2;    // steps that are worth another warp
 constexpr int kQueue = 8;     // units between a warp's copies and its products, at most
 
 struct Unit {
@@ -702,7 +702,7 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   const bool bf16 = c.dtype == MAK_DT_BF16;
   // Rows that share a cache head, on average.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
-  const bool many = rows > 32 && paged_tc_fits(p);
+  const bool many = rows > 16 && paged_tc_fits(p);
   const int tokens = many ? paged_tc_box(c.block_size) : kStep;
   CUtensorMap k, v;
   if (!paged_map(&k, p.key, p.k_sb, p.k_st, p.k_sh, p.num_blocks, p.nh, c.head_dim, c.block_size, bf16, tokens, d->workspace) ||

@@ -13,7 +13,7 @@ namespace {
 
 constexpr int kRows = 16;
 constexpr int kStep = 16;
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxGrid = 148;
 constexpr int kMinRun = 2;
@@ -29,7 +29,7 @@ struct Part {
 
 template <int HD>
 struct Smem {
-  static constexpr int kStages = HD == 64 ? 8 : 4;
+  static constexpr int kStages = HD == 64 ? 6 : 3;
   static constexpr int kTileBytes = kStep * HD * 2;
   alignas(1024) uint8_t ring[kWarps][kStages][kTileBytes];  // HD / 64 pieces of [16][64], lines of 128 bytes swizzled
   alignas(16) float old[kWarps][kStages][kStep];            // sums so far
@@ -360,7 +360,7 @@ extern "C" int mak_paged_weights(const mak_paged_weights_desc* d, void* stream) 
   cudaStream_t st = as_stream(stream);
   const bool bf16 = c.dtype == MAK_DT_BF16;
   // Rows that share a cache head, on average; a group has to fit the chunks of rows.
-  const bool many = c.num_rows * w.a.group / c.num_seqs > 32 && c.num_seqs * 8 <= space.plan_bytes && weights_tc_fits(w);
+  const bool many = c.num_rows * w.a.group / c.num_seqs > 16 && c.num_seqs * 8 <= space.plan_bytes && weights_tc_fits(w);
   CUtensorMap k;
   if (!paged_map(&k, w.a.key, w.a.k_sb, w.a.k_st, w.a.k_sh, w.a.num_blocks, w.a.nh, c.head_dim, c.block_size, bf16, many ? c.block_size : kStep,
                  d->workspace))

@@ -4,18 +4,15 @@
 // has a token, its sum runs over the columns and stays in a register, so no thread waits for another's maximum or sum.
 // A weight is 2^(s scale log2 e - lse log2 e): one rounding of the difference and that of lse log2 e, 2^-24 of 2^4 or so.
 //
-// Bound by the exponentials: 16 a cycle and SM take 1024 cycles for a chunk of 128 x 128, the products 512.  So some of each
-// eight pairs are taken by a polynomial on the other units instead: 2^y = 2^n 2^f, n the nearest whole number, 2^f of
-// degree 5 with the smallest largest relative error on [-1/2, 1/2], 7.5e-8 (coefficients by exchange of extrema, as Remez
-// has it).
+// Bound by the exponentials: 16 a cycle and SM take 1024 cycles for a chunk of 128 x 128, the products 512.
 //
 // A unit is a tile of 128 tokens of one cache head, its work the chunks of rows that see it; K of a unit is loaded once, the
 // rows stream by TMA.  All units laid end to end are cut into equal runs, one per block; a unit cut by that leaves partial
 // sums, and the last block to arrive adds them in order of position, so results do not depend on timing.  Roles:
-//   warps 0-7   exponentials: 64 columns of a chunk each, a thread per token (TMEM lane)
-//   warp 8      TMA loads of K and rows
-//   warp 9      one thread issues all tcgen05.mma
-//   warp 10     lse of the rows
+//   warps 0-15  exponentials: 32 columns of a chunk each, a thread per token (TMEM lane)
+//   warp 16     TMA loads of K and rows
+//   warp 17     one thread issues all tcgen05.mma
+//   warp 18     lse of the rows
 #include <utility>
 
 #include "paged_weights.cuh"
@@ -25,14 +22,16 @@ namespace mak {
 namespace {
 
 constexpr int kTile = 128;     // tokens of a unit
-constexpr int kThreads = 384;
+constexpr int kMath = 16;      // warps of the exponentials
+constexpr int kSides = kMath / 4, kCols = kTile / kSides;  // columns of a warp
+constexpr int kThreads = 32 * (kMath + 4);
 constexpr int kMaxGrid = 148;
 constexpr int kUnitCost = 2;   // a unit's beginning and end, in chunks
 constexpr int kMinRun = 4;     // chunks that are worth another block
 constexpr int kPlaces = 4;     // for scores in tensor memory
 constexpr int kQ = 4, kK = 2;  // chunks of rows and tiles of K in shared memory
+static_assert(kCols == 32, "one word of columns");
 constexpr int kHave = 16;      // units whose pages are remembered
-constexpr int kPolyOf8 = 3;    // pairs of weights of each eight that the polynomial takes
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Tiles of a sequence: those that some row sees, or, where sums begin, all places of its row of sums.
@@ -56,12 +55,16 @@ __device__ __forceinline__ void chunks_of(const WeightParams& w, const Seq& x, i
   *c0 = *c1 = 0;
   const PagedParams& p = w.a;
   if (x.v.rows == 0 || tok >= x.s.any_hi || (tok + kTile <= x.s.any_lo && tok >= p.sinks)) return;
-  const int64_t base = static_cast<int64_t>(x.v.ctx) - x.v.rows;  // position of row 0
-  int64_t i0 = max(tok - base, static_cast<int64_t>(0)), i1 = x.v.rows - 1;
-  if (p.window > 0 && tok >= p.sinks) i1 = min(i1, tok + kTile - 1 - base + p.window - 1);
+  const int base = x.v.ctx - x.v.rows;  // position of row 0
+  const int i0 = max(tok - base, 0);
+  int i1 = x.v.rows - 1;
+  if (p.window > 0 && tok >= p.sinks) {
+    const int64_t last = static_cast<int64_t>(tok) + kTile - 1 - base + p.window - 1;
+    if (last < i1) i1 = static_cast<int>(last);
+  }
   if (i0 > i1) return;
-  *c0 = static_cast<int>(i0 / per);
-  *c1 = static_cast<int>(i1 / per) + 1;
+  *c0 = i0 / per;
+  *c1 = i1 / per + 1;
 }
 
 __global__ void __launch_bounds__(256) weights_plan_kernel(const __grid_constant__ WeightParams w, int64_t* work, int per) {
@@ -146,33 +149,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-// 2^y without the exponential unit, y taken as between -126 and 128; NaN stays.
-__device__ __forceinline__ float2 exp2_poly(float2 y) {
-  constexpr float kShift = 12582912.f;  // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
-  auto within = [](float x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;\n min.NaN.f32 %0, %0, 0f43000000;" : "+f"(x));
-    return x;
-  };
-  y.x = within(y.x), y.y = within(y.y);
-  const float2 n = add2(y, both(kShift));
-  const float2 f = add2(y, fma2(n, both(-1.f), both(kShift)));
-  float2 q = fma2(both(0.001327647199f), f, both(0.009675541334f));
-  q = fma2(q, f, both(0.05550713273f));
-  q = fma2(q, f, both(0.2402211972f));
-  q = fma2(q, f, both(0.6931469671f));
-  q = fma2(q, f, both(1.000000072f));
-  // 2^n: the low bits of n's sum become an exponent, 2^128 infinity
-  const float2 top = make_float2(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u));
-  return mul2(q, top);
-}
 // A warp's wait for a phase of a barrier, asleep for up to 0.1 ms at a time.  False when it did not complete in a second or
 // so, or another role gave up.
 __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile int* gave_up) {
@@ -187,7 +164,7 @@ __device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile
   if (!ok) *gave_up = 1;
   return __all_sync(0xffffffffu, ok);
 }
-__device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 __device__ __forceinline__ void box3(uint32_t to, const void* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),
@@ -204,7 +181,7 @@ struct TcSmem {
   alignas(8) uint64_t q_full[kQ], q_empty[kQ], k_full[kK], k_empty[kK], s_full[kPlaces], s_empty[kPlaces], spare;
   int64_t before[kThreads + 1];
   int64_t sums[kThreads / 32];
-  float side[kTile];
+  float side[kSides][kTile];
   uint32_t have[kHave];  // bit c: 16 tokens c of a unit's tile have a page
   uint32_t tmem;
   int gave_up, last;
@@ -240,12 +217,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
       sm.gave_up = 0;
       mbar_init(&sm.spare, 1);
-      for (int i = 0; i < kQ; ++i) mbar_init(&sm.q_full[i], 2), mbar_init(&sm.q_empty[i], 9);
+      for (int i = 0; i < kQ; ++i) mbar_init(&sm.q_full[i], 2), mbar_init(&sm.q_empty[i], 1 + kMath);
       for (int i = 0; i < kK; ++i) mbar_init(&sm.k_full[i], 1), mbar_init(&sm.k_empty[i], 1);
-      for (int i = 0; i < kPlaces; ++i) mbar_init(&sm.s_full[i], 1), mbar_init(&sm.s_empty[i], 8);
+      for (int i = 0; i < kPlaces; ++i) mbar_init(&sm.s_full[i], 1), mbar_init(&sm.s_empty[i], kMath);
       mbar_init_fence();
     }
-    if (warp == 9) tmem_alloc<512>(&sm.tmem);
+    if (warp == kMath + 1) tmem_alloc<512>(&sm.tmem);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -309,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   Unit u;
   bool ok = true;
-  if (warp < 8) {
+  if (warp < kMath) {
     // ---- exponentials ----------------------------------------------------------------
     const int side = warp >> 2, r = tid & 127;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -319,60 +296,57 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t base = static_cast<int64_t>(u.v.ctx) - u.v.rows;
       float2 sum[2] = {both(0.f), both(0.f)};
       bool there = false;
+      // this thread adds the unit's sum of token t to what the row holds
+      float* dst = w.sums + sum_row(w, u.seq) * w.sum_sr + u.head * w.sum_sh + t;
+      const bool mine = side == 0 && t < w.max_tokens && (!w.add || (t < u.any_hi && (t >= u.any_lo || t < p.sinks)));
       for (int i = 0; i < u.n; ++i, ++g) {
         const uint32_t st = g % kPlaces, qs = g % kQ;
         static_assert(kQ == kPlaces, "one count for both");
         ok = ok && wait_warp(&sm.s_full[st], (g / kPlaces) & 1, gave_up);
         tc_fence_after();
         if (i == 0) there = sm.have[units % kHave] >> (r >> 4) & 1;
-        uint32_t x[2][32];
-        tmem_ld(tmem + lanes + st * 128 + side * 64, x[0]);
-        tmem_ld(tmem + lanes + st * 128 + side * 64 + 32, x[1]);
-        tmem_wait(x[0]);
-        tmem_wait(x[1]);
+        uint32_t x[kCols];
+        tmem_ld(tmem + lanes + st * 128 + side * kCols, x);
+        tmem_wait(x);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.s_empty[st]);
         // Columns [from, to) are rows that see token t: those from its own position on, until their window has left it.
         const int64_t i0 = static_cast<int64_t>(u.c0 + i) * per;  // the chunk's first row
-        const int live = static_cast<int>(min(static_cast<int64_t>(u.v.rows) - i0, static_cast<int64_t>(per)));
-        int64_t a = (t - base - i0) * p.group, b = static_cast<int64_t>(live) * p.group;
+        const int64_t live = min(u.v.rows - i0, static_cast<int64_t>(per));
+        int64_t a = (t - base - i0) * p.group, b = live * p.group;
         if (p.window > 0 && t >= p.sinks) b = min(b, (t - base - i0 + p.window) * p.group);
         if (!there || t >= u.v.room) b = 0;
-        const int from = static_cast<int>(min(max(a - side * 64, static_cast<int64_t>(0)), static_cast<int64_t>(64)));
-        const int to = static_cast<int>(min(max(b - side * 64, static_cast<int64_t>(0)), static_cast<int64_t>(64)));
-        ok = ok && wait_warp(&sm.q_full[qs], (g / kQ) & 1, gave_up);  // has been: for what warp 10 wrote
-        const float4* lse = reinterpret_cast<const float4*>(sm.lse[qs] + side * 64);
-        const bool whole = __all_sync(0xffffffffu, from == 0 && to == 64);
+        const int from = static_cast<int>(min(max(a - side * kCols, static_cast<int64_t>(0)), static_cast<int64_t>(kCols)));
+        const int to = static_cast<int>(min(max(b - side * kCols, static_cast<int64_t>(0)), static_cast<int64_t>(kCols)));
+        ok = ok && wait_warp(&sm.q_full[qs], (g / kQ) & 1, gave_up);  // has been: for what the last warp wrote
+        const float4* lse = reinterpret_cast<const float4*>(sm.lse[qs] + side * kCols);
+        const bool whole = __all_sync(0xffffffffu, from == 0 && to == kCols), none = __all_sync(0xffffffffu, to <= from);
         if (whole) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < kCols / 4; ++e) {
             const float4 f = lse[e];
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const int c = e * 4 + z * 2;
-              float2 y = fma2(make_float2(__uint_as_float(x[c >> 5][c & 31]), __uint_as_float(x[c >> 5][(c + 1) & 31])), both(p.scale_log2),
-                              z ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
-              if ((c >> 1) % 8 >= 8 - kPolyOf8) {
-                y = exp2_poly(y);
-              } else {
-                y.x = exp2_near(y.x);
-                y.y = exp2_near(y.y);
-              }
+              float2 y = fma2(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), both(p.scale_log2), z ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
+              y.x = exp2_near(y.x);
+              y.y = exp2_near(y.y);
               sum[z] = add2(sum[z], y);
             }
           }
-        } else {
+        } else if (!none) {
+          auto below = [](int k) { return k >= 32 ? 0xffffffffu : (1u << k) - 1u; };
+          const uint32_t bits = below(to) & ~below(from);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < kCols / 4; ++e) {
             const float4 f = lse[e];
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const int c = e * 4 + z * 2;
-              const float2 y = fma2(make_float2(__uint_as_float(x[c >> 5][c & 31]), __uint_as_float(x[c >> 5][(c + 1) & 31])), both(p.scale_log2),
-                                    z ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
-              sum[z].x += c >= from && c < to ? exp2_near(y.x) : 0.f;
-              sum[z].y += c + 1 >= from && c + 1 < to ? exp2_near(y.y) : 0.f;
+              const float2 y = fma2(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), both(p.scale_log2), z ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
+              sum[z].x += bits >> c & 1 ? exp2_near(y.x) : 0.f;
+              sum[z].y += bits >> (c + 1) & 1 ? exp2_near(y.y) : 0.f;
             }
           }
         }
@@ -383,13 +357,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       float got = sum[0].x + sum[0].y;
       if (!ok) got = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN
       if (u.n > 0) ++units;
-      if (side == 1) sm.side[r] = got;
+      if (side > 0) sm.side[side][r] = got;
       math_sync();
       const bool cut = u.ta > 0 || u.tb < u.len;
-      const int64_t first_block = u.wt / run, last_block = (u.wt + u.len - 1) / run;
+      const int64_t first_block = cut ? u.wt / run : 0, last_block = cut ? (u.wt + u.len - 1) / run : 0;
       auto piece = [&](int64_t block) { return p.partial + (2 * block + (u.wt > block * run ? 1 : 0)) * kTile + r; };
       if (side == 0) {
-        got += sm.side[r];
+#pragma unroll
+        for (int z = 1; z < kSides; ++z) got += sm.side[z][r];
         if (cut) *piece(blockIdx.x) = got;
       }
       if (cut) {
@@ -406,17 +381,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int64_t b = first_block; b <= last_block; ++b) got += __ldcg(piece(b));
         }
       }
-      if (side == 0 && (!cut || sm.last) && t < w.max_tokens) {
-        const bool seen = t < u.any_hi && (t >= u.any_lo || t < p.sinks);
-        float* dst = w.sums + sum_row(w, u.seq) * w.sum_sr + u.head * w.sum_sh + t;
-        if (!w.add)
-          *dst = got;
-        else if (seen)
-          *dst += got;
-      }
+      if (mine && (!cut || sm.last)) *dst = (w.add ? *dst : 0.f) + got;
       math_sync();  // side and last are read
     }
-  } else if (warp == 8) {
+  } else if (warp == kMath) {
     // ---- loads --------------------------------------------------------------------------
     const int bs = 1 << p.bs_log2, box = min(bs, kTile), pages = kTile / box, cols = per * p.group;
     uint32_t g = 0, units = 0;
@@ -470,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.k_full[t % kK], (t / kK) & 1); ++i) {
         }
     }
-  } else if (warp == 9) {
+  } else if (warp == kMath + 1) {
     // ---- the tensor cores -------------------------------------------------------
     constexpr uint32_t kIdesc = instr_desc(kTile, 1, BF16 ? 1 : 0, false, false);
     const uint64_t q_desc = smem_desc(smem_addr(sm.q), 16, 1024, 7), k_desc = smem_desc(smem_addr(sm.k), 16, 1024, 7);
@@ -505,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t i = 0; i < kWaitLimit && !mbar_try(&sm.spare, 0); ++i) {
       }
     }
-  } else if (warp == 10) {
+  } else if (warp == kMath + 2) {
     // ---- lse ---------------------------------------------------------------------
     const int cols = per * p.group;
     uint32_t g = 0;
@@ -536,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMath + 1) {
     __syncwarp();
     tc_fence_after();
     tmem_free<512>(tmem);
