@@ -7,9 +7,15 @@
 //
 // Bound by reading K and V.  A unit is 16 rows (tokens of a sequence times the query heads of a cache head) of one
 // sequence and head, its work 16-token steps.  All units laid end to end are cut into equal runs, one per warp, whatever
-// the lengths; a warp has its steps brought by TMA into a ring of its own, so no warp waits for
-// another until its run ends.  A unit cut by that leaves partial sums: the block joins those of its warps, the last block
-// to arrive joins those of the blocks, both in order of position, so results do not depend on timing.
+// the lengths; a warp has its steps brought by TMA into a ring of its own, so no warp waits for another until its run ends.
+// A unit cut by that leaves partial sums: the block joins those of its warps, the last block to arrive joins those of the
+// blocks, both in order of position, so results do not depend on timing.
+//
+// Measured, calls in a graph, 8 cache heads of 128 in bfloat16 for 32 query heads: 64 requests of 256 to 4096 tokens with a
+// window of 2048 85 us (5.1 TB/s of the 6.5 that a plain copy has), of which some 12 are the way to the first tile and the
+// joins; one request that sees 4100 tokens 15.3 us, a chain of latencies (lengths, block ids, tiles, the block's join, the
+// blocks'); three trees on 60000 to 100000 tokens, 4 heads, 102 us (5.1 TB/s).  12 warps with shorter rings: 98 us for the
+// first; K and V by cp.async of single lines instead of TMA: 89.
 #include "paged_attn_tc.cuh"
 #include "tcgen05.cuh"
 
@@ -700,7 +706,10 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   p.counters = space.counters, p.partial = space.partial;
   cudaStream_t st = as_stream(stream);
   const bool bf16 = c.dtype == MAK_DT_BF16;
-  // Rows that share a cache head, on average.
+  // Rows that share a cache head, on average.  Few rows read K and V again for every 16; many rows wait for a unit's
+  // longer beginning and end.  Few / many in us, 8 cache heads of 128 with 4 query heads: 16 sequences of 4096 tokens
+  // 63 / 62 for 16 rows, 110 / 62 for 32 (heads of 64: 38 / 49, 61 / 49); 64 of 512 44 / 61, 55 / 61, 76 / 70 for 48; one of
+  // 4096 25 / 27, 25 / 27, 35 / 48 for 128.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
   const bool many = rows > 16 && paged_tc_fits(p);
   const int tokens = many ? paged_tc_box(c.block_size) : kStep;

@@ -5,6 +5,10 @@
 // every warp as in the attention), keeps their K in shared memory and goes over the rows, 16 at a time; each token's sum
 // has one writer, so results do not depend on timing.  Exponents are taken of scale s - lse in natural units, one
 // rounding, which keeps a weight's error at that of its exponent.
+//
+// Measured, calls in a graph: 64 requests of 256 to 4096 tokens, one row, 8 cache heads of 128 in bfloat16 for 32 query heads
+// 58 us (5.3 TB/s of the 6.5 that a plain copy has); 8 warps with longer rings took 78: a warp's way from a part's pages to
+// its sums is latency, which more warps hide.
 #include "paged_weights.cuh"
 #include "tcgen05.cuh"
 
@@ -359,7 +363,9 @@ extern "C" int mak_paged_weights(const mak_paged_weights_desc* d, void* stream) 
   w.a.counters = space.counters, w.a.partial = space.partial;
   cudaStream_t st = as_stream(stream);
   const bool bf16 = c.dtype == MAK_DT_BF16;
-  // Rows that share a cache head, on average; a group has to fit the chunks of rows.
+  // Rows that share a cache head, on average; a group has to fit the chunks of rows.  Few / many in us, 8 cache heads of 128
+  // with 4 query heads: 16 sequences of 4096 tokens 33 / 80 for 16 rows, 97 / 80 for 32, 133 / 85 for 48 (heads of 64: 25 / 73,
+  // 58 / 73, 77 / 78); 64 of 512 19 / 44, 51 / 44; one of 4096 11 / 14, 20 / 14.
   const bool many = c.num_rows * w.a.group / c.num_seqs > 16 && c.num_seqs * 8 <= space.plan_bytes && weights_tc_fits(w);
   CUtensorMap k;
   if (!paged_map(&k, w.a.key, w.a.k_sb, w.a.k_st, w.a.k_sh, w.a.num_blocks, w.a.nh, c.head_dim, c.block_size, bf16, many ? c.block_size : kStep,
