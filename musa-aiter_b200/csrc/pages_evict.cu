@@ -9,10 +9,11 @@
 //
 // Bound by moving the kept tokens: rows of 256 bytes at places of their own, read and written.  A block per layer, row and
 // head; a second small launch returns the pages.  Measured: 16 requests of 1500 to 4096 tokens to 1024, 8 layers, 8 heads of
-// 128: 245 us (4.5 TB/s of 6.5 that a plain copy has), of which a block's search for its tokens is a seventh; one request of
-// 30000 tokens to 2000, 4 heads of 64: 81 us, four blocks' search and walk.  Batches of 64 tokens and 2 blocks on an SM were
-// the best of those tried: 32 tokens 352 to 413 us, 40 415, 48 344, 128 480; slices of 64 or 128 bytes of each token to a
-// warp, which needs no barrier, 374 and 362.
+// 128: 246 us (4.5 TB/s of 6.5 that a plain copy has), of which a block's search for its tokens is a seventh; one request of
+// 30000 tokens to 2000, 4 heads of 64: 65 us, four blocks' search (two thirds) and walk; with 8192 tokens to a list, not 4096,
+// the walk has its batches in one row (81 to 68 us, together with counts of each lane for equal first bytes).  Batches of 64
+// tokens and 2 blocks on an SM were the best of those tried: 32 tokens 352 to 413 us, 40 415, 48 344, 128 480; slices of 64
+// or 128 bytes of each token to a warp, which needs no barrier, 374 and 362.
 #include "common.cuh"
 
 namespace mak {
@@ -20,7 +21,7 @@ namespace {
 
 constexpr int kPer = 8;  // tokens of a thread that are looked at together
 // Tokens that move together, at most.
-constexpr int list_of(int threads) { return 2 * kPer * threads < 8192 ? 2 * kPer * threads : kPer * threads; }
+constexpr int list_of(int threads) { return 2 * kPer * threads; }
 constexpr int kMaxLayers = 128;
 constexpr int kMaxRequests = 8192;
 
@@ -93,14 +94,14 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1) evict_kerne
   const int lo = min(p.sinks, len), hi = max(len - p.recent, lo);  // candidates
   const int want = p.keep - (lo + len - hi);                       // of them, these many stay
 
-  // ---- sums of the row, eight loads of a thread at a time -----------------
+  // ---- sums of the row, sixteen loads of a thread at a time -----------------
   if (p.cached) {
-    for (int t0 = tid; t0 < len; t0 += 8 * kThreads) {
-      float x[8];
+    for (int t0 = tid; t0 < len; t0 += 16 * kThreads) {
+      float x[16];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = t0 + e * kThreads < len ? sums[t0 + e * kThreads] : 0.f;
+      for (int e = 0; e < 16; ++e) x[e] = t0 + e * kThreads < len ? sums[t0 + e * kThreads] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 16; ++e)
         if (t0 + e * kThreads < len) cache[t0 + e * kThreads] = x[e];
     }
     __syncthreads();
@@ -108,10 +109,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1) evict_kerne
   const float* from_sums = p.cached ? cache : sums;
 
   // ---- the want-th largest: `prefix`, and how many equal to it stay -----------------
+  // A lane has counts of its own, in a bank of its own, where the lists will be: most sums share their first byte.
   uint32_t prefix = 0;
   int left = want;
+  static_assert(2 * kList >= 256 * 32 && kThreads >= 256, "counts of each lane");
   for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) counts[tid] = 0;
+    for (int j = tid; j < 256 * 32 / 4; j += kThreads) reinterpret_cast<int4*>(shared)[j] = make_int4(0, 0, 0, 0);
     __syncthreads();
     const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
     for (int first = lo; first < hi; first += 8 * kThreads) {
@@ -123,17 +126,16 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1) evict_kerne
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // equal first bytes of a warp are counted together: most sums share their sign and exponent
         const uint32_t o = order_of(x[e]);
-        const bool mine = first + tid + e * kThreads < hi && (o & mask) == (prefix & mask);
-        const uint32_t byte = mine ? o >> shift & 255 : 256;
-        if (shift == 24) {
-          const uint32_t peers = __match_any_sync(0xffffffffu, byte);
-          if (mine && lane == __ffs(peers) - 1) atomicAdd(&counts[byte], __popc(peers));
-        } else if (mine) {
-          atomicAdd(&counts[byte], 1);
-        }
+        if (first + tid + e * kThreads < hi && (o & mask) == (prefix & mask)) atomicAdd(&shared[(o >> shift & 255) * 32 + lane], 1);
       }
+    }
+    __syncthreads();
+    if (tid < 256) {
+      int sum = 0;
+#pragma unroll
+      for (int c = 0; c < 32; ++c) sum += shared[tid * 32 + ((c + lane) & 31)];
+      counts[tid] = sum;
     }
     __syncthreads();
     if (warp == 0) {  // the byte: the largest b with at least `left` numbers at or above it
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1) evict_kerne
   // ---- the walk ------------------------------------------------------------------------
   const int32_t* table = p.tables + row * p.table_stride;
   // A kept token is HD / 8 pieces of 16 bytes of K and as many of V.
-  constexpr int kPieces = HD / 4, kDeep = kThreads == 256 ? 8 : 4, kBatch = kThreads * kDeep / kPieces;
+  constexpr int kPieces = HD / 4, kDeep = 8, kBatch = kThreads * kDeep / kPieces;
   const int piece = tid % kPieces;
   const bool is_v = piece >= kPieces / 2;
   uint16_t* base = (is_v ? p.value[layer] : p.key[layer]) + head * (is_v ? p.v_sh : p.k_sh) + (is_v ? piece - kPieces / 2 : piece) * 8;
@@ -308,6 +310,7 @@ __global__ void __launch_bounds__(kFinish) evict_finish_kernel(int32_t* tables, 
 }
 
 constexpr int kMostCached = 40960;  // next to the lists
+static_assert(kMostCached * 4 + list_of(512) * 8 + 2048 <= 227 * 1024, "shared memory of a block");
 constexpr int kMaxDevices = 64;
 
 template <int HD, int kThreads>
@@ -382,7 +385,7 @@ extern "C" int mak_pages_evict(const mak_pages_desc* d, const mak_evict_desc* e,
       p.value[i] = reinterpret_cast<uint16_t*>(e->values[at + i]);
     }
     const dim3 grid(static_cast<unsigned>(n * e->num_heads), static_cast<unsigned>(layers));
-    // Rows of up to 8192 tokens leave room for five blocks on an SM; longer ones are kept where there are few blocks.
+    // Rows of up to 8192 tokens leave room for two blocks on an SM; longer ones are kept where there are few blocks.
     const int64_t blocks = n * e->num_heads * layers;
     p.cached = e->max_tokens <= 8192 || (e->max_tokens <= kMostCached && blocks <= sm_count());
     const int bytes = p.cached ? static_cast<int>(e->max_tokens) * 4 : 0;
