@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <cstdlib>
@@ -658,6 +659,11 @@ mak_paged_cache_desc paged_desc(const char* name, Args a, bool values, PyObject*
   d.dtype = float_code(kind);
   return d;
 }
+// An expanded axis has several results at one place.
+void separate(const char* name, const char* what, const at::Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) refuse(name, what, " must not be expanded");
+}
 at::Tensor paged_workspace(const at::Device& device, cudaStream_t stream) {
   static auto* spaces = new Workspaces();
   return workspace(*spaces, lib.paged_workspace_bytes(), device, stream);
@@ -701,6 +707,7 @@ PyObject* py_paged(PyObject*, Args a, Py_ssize_t n) {
       const at::Tensor& o = tensor(name, "out", a[11]);
       if (o.sizes() != q0.sizes() || o.scalar_type() != q0.scalar_type() || (o.numel() && o.stride(2) != 1))
         refuse(name, "out must have q's shape and dtype and contiguous rows");
+      separate(name, "out", o);
       used.push_back(&o);
     }
     d.scale = scale_of(a[9], hd);
@@ -742,6 +749,7 @@ PyObject* py_weights(PyObject*, Args a, Py_ssize_t n) {
     if (sums.dim() != 3 || sums.size(1) != d.cache.num_heads || sums.scalar_type() != at::kFloat)
       refuse(name, "sums must be float32 [rows of sums, num_heads, max_tokens]");
     if (sums.size(2) > 1 && sums.stride(2) != 1) refuse(name, "the last axis of sums must be contiguous");
+    separate(name, "sums", sums);
     if (a[7] == Py_None) {
       if (sums.size(0) != seqs) refuse(name, "without rows every sequence has its row of sums: ", sums.size(0), " rows for ", seqs, " sequences");
     } else {
@@ -823,6 +831,14 @@ PyObject* py_evict(PyObject*, Args a, Py_ssize_t n) {
     if (sums.dim() != 4 || sums.size(0) != layers || sums.size(1) != table.size(0) || sums.size(2) != nh || sums.scalar_type() != at::kFloat)
       refuse(name, "sums must be float32 [layers, rows of block_tables, num_heads, max_tokens]");
     if (sums.size(3) > 1 && sums.stride(3) != 1) refuse(name, "the last axis of sums must be contiguous");
+    separate(name, "sums", sums);
+    for (int which = 0; which < 2; ++which) {
+      const char* what = which ? "value_caches" : "key_caches";
+      separate(name, what, *held[which].tensors[0]);  // one layout for all
+      std::vector<uint64_t> sorted = held[which].at;
+      std::sort(sorted.begin(), sorted.end());
+      if (nb > 0 && std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) refuse(name, what, " must not hold a layer twice");
+    }
     for (const at::Tensor* t : {&table, &lens, &rows, &refs, &sums}) dev.add(*t);
     for (const Held& h : held)
       for (const at::Tensor* t : h.tensors) dev.add(*t);

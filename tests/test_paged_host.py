@@ -152,6 +152,25 @@ def test_tables_that_require_a_gradient_are_refused():
                               torch.zeros((5, 32)))
 
 
+def test_results_on_top_of_one_another_are_refused():
+    with pytest.raises(ValueError, match="out must not be expanded"):
+        window(out=H(1, 1, 64).expand(1, 4, 64))
+    two = dict(q=H(2, 4, 64), key_cache=H(4, 16, 2, 64), block_tables=I(2, 2), context_lens=I(2), lse=torch.zeros((2, 4)))
+    with pytest.raises(ValueError, match="sums must not be expanded"):
+        ma.paged_attention_weights(**two, sums=torch.zeros((1, 2, 32)).expand(2, 2, 32))
+    plane, other = H(4, 16, 2, 64), H(4, 16, 2, 64)
+    evict = dict(block_tables=I(3, 2), context_lens=I(3), rows=I(2), ref_counts=I(4), keep=8)
+    for keys, values, text in (
+        ([plane, plane], [other, H(4, 16, 2, 64)], "key_caches must not hold a layer twice"),
+        ([plane, H(4, 16, 2, 64)], [other, other], "value_caches must not hold a layer twice"),
+        ([H(4, 16, 1, 64).expand(4, 16, 2, 64)], [other], "key_caches must not be expanded"),
+    ):
+        with pytest.raises(ValueError, match=text):
+            ma.kv_pages_evict(**evict, key_caches=keys, value_caches=values, sums=torch.zeros((len(keys), 3, 2, 32)))
+    with pytest.raises(ValueError, match="sums must not be expanded"):
+        ma.kv_pages_evict(**evict, key_caches=[plane], value_caches=[other], sums=torch.zeros((1, 1, 2, 32)).expand(1, 3, 2, 32))
+
+
 def test_registered():
     for name, family in (("paged_attention_window", "attention"), ("paged_attention_tree", "attention"), ("paged_attention_weights", "eviction"),
                          ("kv_pages_evict", "eviction"), ("apply_qk_norm_rope", "cache"), ("apply_qk_norm_rope_backward", "cache")):
