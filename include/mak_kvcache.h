@@ -45,7 +45,7 @@ extern "C" {
 #define MAK_OK 0
 #define MAK_E_INVALID (-1)     /* bad shape, stride, pointer or argument */
 #define MAK_E_UNSUPPORTED (-2) /* valid request this build does not handle */
-#define MAK_E_WORKSPACE (-3)   /* workspace missing or too small */
+#define MAK_E_WORKSPACE (-3)   /* workspace missing, too small or not aligned */
 #define MAK_E_CUDA (-4)        /* a CUDA runtime call or launch failed */
 
 /* ---- element / index type codes ----------------------------------------- */
@@ -785,8 +785,8 @@ typedef struct mak_paged_attn_desc {
   float scale;
 } mak_paged_attn_desc;
 
-/* Bytes of the workspace of mak_paged_attention: independent of the call's sizes.  It is zeroed once by the caller and
- * then kept for calls that follow one another on one stream (the kernels leave its counters at zero). */
+/* Bytes of the workspace of mak_paged_attention: independent of the call's sizes.  It begins on 16 bytes, is zeroed once by
+ * the caller and then kept for calls that follow one another on one stream (the kernels leave its counters at zero). */
 MAK_API int64_t mak_paged_attention_workspace_bytes(void);
 
 /*

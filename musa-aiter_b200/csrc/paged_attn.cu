@@ -664,6 +664,13 @@ PagedParams paged_params(const mak_paged_cache_desc& c) {
   return p;
 }
 
+int check_paged_workspace(const void* workspace, int64_t bytes, const char* name) {
+  if (workspace == nullptr || bytes < mak_paged_attention_workspace_bytes()) return fail(MAK_E_WORKSPACE, "%s: workspace missing or too small", name);
+  // partial sums are read from it 16 bytes at a time, and the map of a pool without blocks has its address
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return fail(MAK_E_WORKSPACE, "%s: the workspace must begin on 16 bytes", name);
+  return MAK_OK;
+}
+
 PagedSpace paged_space(void* workspace) {
   char* at = static_cast<char*>(workspace);
   return {static_cast<int32_t*>(workspace), at + kCounterBytes, plan_bytes(), reinterpret_cast<float*>(at + kCounterBytes + plan_bytes())};
@@ -693,8 +700,7 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   if (d->q == nullptr || d->out == nullptr) return fail(MAK_E_INVALID, "%s: null q or out", name);
   if ((reinterpret_cast<uintptr_t>(d->q) & 15) || ((d->q_stride_row | d->q_stride_head) & 7))
     return fail(MAK_E_INVALID, "%s: q needs 16-byte aligned rows", name);
-  if (d->workspace == nullptr || d->workspace_bytes < mak_paged_attention_workspace_bytes())
-    return fail(MAK_E_WORKSPACE, "%s: workspace missing or too small", name);
+  if (int rc = check_paged_workspace(d->workspace, d->workspace_bytes, name)) return rc;
   PagedParams p = paged_params(c);
   p.parents = d->parents;
   p.q = static_cast<const uint16_t*>(d->q), p.out = d->out, p.lse = d->lse;

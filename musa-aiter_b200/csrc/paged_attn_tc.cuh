@@ -21,6 +21,7 @@ bool paged_encode(CUtensorMap* map, const void* base, int rank, const int64_t* d
 
 // Of the entry points.
 int check_paged_cache(const mak_paged_cache_desc& c, bool values, const char* name);
+int check_paged_workspace(const void* workspace, int64_t bytes, const char* name);
 PagedParams paged_params(const mak_paged_cache_desc& c);
 struct PagedSpace {
   int32_t* counters;

@@ -357,8 +357,7 @@ extern "C" int mak_paged_weights(const mak_paged_weights_desc* d, void* stream) 
   w.rows = d->rows;
   w.max_tokens = static_cast<int32_t>(d->max_tokens), w.add = d->accumulate != 0;
   w.scale = d->scale;
-  if (d->workspace == nullptr || d->workspace_bytes < mak_paged_attention_workspace_bytes())
-    return fail(MAK_E_WORKSPACE, "%s: workspace missing or too small", name);
+  if (int rc = check_paged_workspace(d->workspace, d->workspace_bytes, name)) return rc;
   const PagedSpace space = paged_space(d->workspace);
   w.a.counters = space.counters, w.a.partial = space.partial;
   cudaStream_t st = as_stream(stream);
