@@ -645,8 +645,8 @@ typedef struct mak_block_attn_desc {
 } mak_block_attn_desc;
 
 /* Bytes of the workspace of mak_block_attention: independent of the call's sizes.
- * It is zeroed once by the caller and then kept for calls that follow one another
- * on one stream (the kernels leave its counters at zero). */
+ * It begins on 16 bytes, is zeroed once by the caller and then kept for calls that
+ * follow one another on one stream (the kernels leave its counters at zero). */
 MAK_API int64_t mak_block_attention_workspace_bytes(void);
 
 /*

@@ -1128,6 +1128,8 @@ extern "C" int mak_block_attention(const mak_block_attn_desc* d, void* stream) {
     return fail(MAK_E_INVALID, "%s: q needs 16-byte aligned rows", name);
   if (d->workspace == nullptr || d->workspace_bytes < mak_block_attention_workspace_bytes())
     return fail(MAK_E_WORKSPACE, "%s: workspace missing or too small", name);
+  // partial sums are read from it 16 bytes at a time
+  if (reinterpret_cast<uintptr_t>(d->workspace) & 15) return fail(MAK_E_WORKSPACE, "%s: the workspace must begin on 16 bytes", name);
   BlockAttnParams p = {};
   p.key = static_cast<const uint8_t*>(c.key);
   p.value = static_cast<const uint8_t*>(c.value);

@@ -31,6 +31,20 @@ class Attention(Structure):
                 [(n, c_int32) for n in ("num_q_heads", "window", "sinks")] + [("scale", c_float)])
 
 
+class BlockCache(Structure):
+    _fields_ = ([(n, c_void_p) for n in ("key", "value", "key_scale", "value_scale")] +
+                [(n, c_int64) for n in ("k_sb", "k_sh", "v_sb", "v_sh", "ks_sb", "ks_sh", "vs_sb", "vs_sh")] +
+                [(n, c_void_p) for n in ("block_tables", "context_lens", "cu_seqlens")] +
+                [(n, c_int64) for n in ("table_stride", "num_blocks", "num_seqs", "max_blocks", "num_rows")] +
+                [(n, c_int32) for n in ("num_heads", "head_dim", "block_size", "code_type")])
+
+
+class BlockAttention(Structure):
+    _fields_ = ([("cache", BlockCache)] + [(n, c_void_p) for n in ("q", "out", "lse", "workspace")] +
+                [(n, c_int64) for n in ("workspace_bytes", "q_sr", "q_sh", "o_sr", "o_sh")] +
+                [(n, c_int32) for n in ("num_q_heads", "q_dtype", "causal", "window")] + [("scale", c_float), ("reserved", c_int32)])
+
+
 class Weights(Structure):
     _fields_ = ([("cache", Cache)] + [(n, c_void_p) for n in ("q", "lse", "sums", "rows")] +
                 [(n, c_int64) for n in ("q_sr", "q_sh", "lse_sr", "sum_sr", "sum_sh", "sum_rows", "max_tokens")] +
@@ -44,6 +58,8 @@ def lib():
     assert result.ok, result.message
     lib = ctypes.CDLL(str(_build.LIB_PATH))
     lib.mak_paged_attention_workspace_bytes.restype = c_int64
+    lib.mak_block_attention_workspace_bytes.restype = c_int64
+    lib.mak_block_attention.argtypes = [POINTER(BlockAttention), c_void_p]
     lib.mak_paged_attention.argtypes = [POINTER(Attention), c_void_p]
     lib.mak_paged_weights.argtypes = [POINTER(Weights), c_void_p]
     return lib
@@ -72,7 +88,18 @@ def weights(lib, **change):
     return lib.mak_paged_weights(byref(d), None)
 
 
-@pytest.mark.parametrize("call", [paged, weights])
+def block_scaled(lib, **change):
+    c = BlockCache(key=ADDRESS, value=ADDRESS, key_scale=ADDRESS, value_scale=ADDRESS, k_sb=2048, k_sh=1024, v_sb=2048, v_sh=1024, ks_sb=2,
+                   ks_sh=1, vs_sb=2, vs_sh=1, block_tables=ADDRESS, context_lens=ADDRESS, table_stride=2, num_blocks=4, num_seqs=1,
+                   max_blocks=2, num_rows=1, num_heads=2, head_dim=64, block_size=16)
+    d = BlockAttention(cache=c, q=ADDRESS, out=ADDRESS, workspace=ADDRESS, workspace_bytes=lib.mak_block_attention_workspace_bytes(),
+                       q_sr=256, q_sh=64, o_sr=256, o_sh=64, num_q_heads=4, q_dtype=F16, causal=1, scale=0.125)
+    for name, x in change.items():
+        setattr(d, name, x)
+    return lib.mak_block_attention(byref(d), None)
+
+
+@pytest.mark.parametrize("call", [paged, weights, block_scaled])
 @pytest.mark.parametrize("change", [dict(workspace=None), dict(workspace_bytes=4096), dict(workspace=ADDRESS + 4),
                                     dict(workspace=ADDRESS + 8), dict(workspace=ADDRESS + 1)])
 def test_workspaces_refused(lib, call, change):
