@@ -74,7 +74,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 template <int HD, int kThreads>
 __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 2 : 1) evict_kernel(const __grid_constant__ EvictParams p) {
   constexpr int kChunk = kPer * kThreads, kList = list_of(kThreads);
-  extern __shared__ int32_t shared[];
+  extern __shared__ __align__(16) int32_t shared[];  // cleared 16 bytes at a time
   int32_t *const from = shared, *const to = shared + kList;
   float* const cache = reinterpret_cast<float*>(shared + 2 * kList);
   __shared__ int counts[256];
