@@ -622,9 +622,8 @@ int launch_rows(const PagedParams& p, const CUtensorMap& k, const CUtensorMap& v
   return launch_pdl(name, kernel, dim3(sms < kMaxGrid ? sms : kMaxGrid), dim3(kThreads), kBytes, st, p, k, v);
 }
 
-constexpr int64_t kCounterBytes = 4096;
 int64_t plan_bytes() { return (paged_tc_plan_bytes() + 255) / 256 * 256; }
-static_assert(kMaxGrid * 4 <= kCounterBytes, "a counter per block");
+static_assert(kMaxGrid * 4 <= kPagedCounterBytes, "a counter per block");
 
 }  // namespace
 
@@ -673,7 +672,7 @@ int check_paged_workspace(const void* workspace, int64_t bytes, const char* name
 
 PagedSpace paged_space(void* workspace) {
   char* at = static_cast<char*>(workspace);
-  return {static_cast<int32_t*>(workspace), at + kCounterBytes, plan_bytes(), reinterpret_cast<float*>(at + kCounterBytes + plan_bytes())};
+  return {static_cast<int32_t*>(workspace), at + kPagedCounterBytes, plan_bytes(), reinterpret_cast<float*>(at + kPagedCounterBytes + plan_bytes())};
 }
 
 }  // namespace mak
@@ -682,7 +681,7 @@ using namespace mak;
 
 extern "C" int64_t mak_paged_attention_workspace_bytes(void) {
   const int64_t few = static_cast<int64_t>(kMaxGrid) * (2 * kWarps + 2) * kPieceFloats<128> * 4, many = paged_tc_partial_bytes();
-  return kCounterBytes + plan_bytes() + (few > many ? few : many);
+  return kPagedCounterBytes + plan_bytes() + (few > many ? few : many);
 }
 
 extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {

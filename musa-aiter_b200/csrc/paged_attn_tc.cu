@@ -48,6 +48,7 @@ constexpr float kLazy = 8.f;    // log2 growth of a row's maximum that is tolera
 constexpr int kUnitCost = 8;    // a unit's beginning and end, in tiles
 constexpr int kMinChunk = 8;    // steps of work that are worth another block
 constexpr int kMaxGrid = 148;
+static_assert(4 * kMaxGrid * 4 <= kPagedCounterBytes, "a counter for each half of the two units that a block may share");
 constexpr int kMaxItems = 1 << 16;
 constexpr int kHave = 16;       // tiles whose pages are remembered
 
@@ -844,7 +845,6 @@ int launch(const PagedParams& p, const char* name, const CUtensorMap& k, const C
 
 int64_t paged_tc_partial_bytes() { return static_cast<int64_t>(4 * kMaxGrid) * kHalf * (128 + 2) * 4; }
 int64_t paged_tc_plan_bytes() { return sizeof(Plan); }
-int64_t paged_tc_counters() { return 4 * kMaxGrid; }
 bool paged_tc_fits(const PagedParams& p) { return row_tiles(p) <= kMaxItems; }
 
 bool paged_encode(CUtensorMap* map, const void* base, int rank, const int64_t* dims, const int64_t* strides, const uint32_t* box, bool bf16) {

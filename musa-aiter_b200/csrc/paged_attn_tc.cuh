@@ -5,9 +5,10 @@
 
 namespace mak {
 
+constexpr int64_t kPagedCounterBytes = 4096;  // of a workspace, at its beginning
+
 int64_t paged_tc_partial_bytes();
 int64_t paged_tc_plan_bytes();
-int64_t paged_tc_counters();
 bool paged_tc_fits(const PagedParams& p);
 int paged_tc_box(int bs);  // tokens of the boxes that it loads
 int launch_paged_tc(const PagedParams& p, int head_dim, bool bf16, const char* name, const CUtensorMap& k, const CUtensorMap& v, void* plan,

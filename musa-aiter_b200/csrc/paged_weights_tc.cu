@@ -35,6 +35,7 @@ constexpr int kMinRun = 4;     // chunks that are worth another block
 constexpr int kPlaces = 4;     // for scores in tensor memory
 constexpr int kQ = 4, kK = 2;  // chunks of rows and tiles of K in shared memory
 static_assert(kCols == 32, "one word of columns");
+static_assert(kMaxGrid * 4 <= kPagedCounterBytes, "a counter per block");
 constexpr int kHave = 16;      // units whose pages are remembered
 constexpr float kLog2e = 1.4426950408889634f;
 
