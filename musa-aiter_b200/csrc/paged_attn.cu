@@ -136,7 +136,7 @@ struct Sum {
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   __device__ __forceinline__ void add(const Sum& y) {
     const float now = fmaxf(m, y.m);
-    const float a = now == -INFINITY ? 1.f : exp2_near(m - now), b = now == -INFINITY ? 1.f : exp2_near(y.m - now);
+    const float a = now == -INFINITY ? 1.f : shrink(m - now), b = now == -INFINITY ? 1.f : shrink(y.m - now);
     o.x = o.x * a + y.o.x * b, o.y = o.y * a + y.o.y * b, o.z = o.z * a + y.o.z * b, o.w = o.w * a + y.o.w * b;
     l = l * a + y.l * b;
     m = now;
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale;
           const float now = fmaxf(m[z], top);
-          keep[z] = now == m[z] ? 1.f : exp2_near(m[z] - now);
+          keep[z] = now == m[z] ? 1.f : shrink(m[z] - now);
           ref[z] = now == -INFINITY ? 0.f : now - kLift;
           m[z] = now;
         }
@@ -428,7 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int t = 0; t < kStep; ++t) {
             float w[2];
 #pragma unroll
-            for (int z = 0; z < 2; ++z) w[z] = __shfl_sync(0xffffffffu, s[t >> 3][z * 2 + (t & 1)], (lane & ~3) | ((t & 7) >> 1));
+            for (int z = 0; z < 2; ++z)  // not 0 either
+              w[z] = fmaxf(__shfl_sync(0xffffffffu, s[t >> 3][z * 2 + (t & 1)], (lane & ~3) | ((t & 7) >> 1)), 0x1p-126f);
 #pragma unroll
             for (int d = 0; d < HD / 8; ++d) {
               uint32_t x;

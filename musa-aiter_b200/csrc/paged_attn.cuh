@@ -129,6 +129,10 @@ __device__ __forceinline__ float exp2_near(float x) {  // 2^x, 2 units in the la
   return y;
 }
 
+// 2^x for x <= 0 as a factor of sums that may hold an infinite one, which stays infinite: not 0, however far apart maxima are.
+// 2^-126 of a sum counts for nothing, and of an empty one is 0.
+__device__ __forceinline__ float shrink(float x) { return fmaxf(exp2_near(x), 0x1p-126f); }
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack_two(float a, float b) {
   if constexpr (BF16) {

@@ -17,7 +17,9 @@
 //   warps 12-15      values in tiles that not every row sees whole: infinite and NaN ones become 0 there
 //
 // What a row does not see reaches none of its sums: its weights there are 0, and 0 times a value that is no number is
-// kept out by warps 12-15; the rows that do see such a value get it with their results (odd_sum).
+// kept out by warps 12-15; the rows that do see such a value get it with their results (odd_sum).  Tiles that all rows see
+// whole are left as they are.  There a weight too light for 16 bits makes NaN of an infinite value, so a NaN in the result of a
+// row whose scores are all numbers is looked into at the unit's end: what it sees of values that are no numbers is its result.
 //
 // Work.  All (row tile, head) units laid end to end, each as long as the tiles it sees, are cut into equal runs, one per
 // block; a small launch before this one adds up the lengths.  A unit cut by that leaves partial sums, and the last block to
@@ -248,24 +250,53 @@ struct TcSmem {
   int odd_seen;  // values that are no numbers were replaced
 };
 
-// Of dimension d .. d + 16: the sum of the values that are no numbers over the tokens that row i of the unit sees, in this
-// half's tiles, where they were replaced.
+// Of dimensions d .. d + 16, those of `wanted`: the sum of the values that are no numbers over the tokens that row i of the
+// unit sees, in this half's tiles, all of them or those where they were replaced.
 template <bool BF16>
-__device__ __noinline__ void odd_sum(const PagedParams& p, const Unit& u, int i, int d, int first, int step, float* sum) {
+__device__ __noinline__ void odd_sum(const PagedParams& p, const Unit& u, int i, int d, int first, int step, bool all, uint32_t wanted, float* sum) {
   const RowView r = row_view(p, u.v, i);
-  for (int j = u.ta + first; j < u.ta + u.n; j += step) {
+#pragma unroll
+  for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+  for (int j = u.ta + first; j < u.ta + u.n && wanted != 0; j += step) {
     const int tok = tile_token<kTile>(u.s, j);
-    if (tile_whole<kTile>(u.s, tok)) continue;
+    if (!all && tile_whole<kTile>(u.s, tok)) continue;
     for (int t = tok; t < tok + kTile; ++t) {
       const bool seen = p.parents != nullptr ? tree_bits(p, u.v, i, t) & 1 : t < r.hi && (t >= r.lo || t < p.sinks);
       if (!seen) continue;
       const int page = page_of(p, p.tables + u.seq * p.table_stride, t);
       if (page < 0) continue;
       const uint16_t* v = p.value + page * p.v_sb + (t & ((1 << p.bs_log2) - 1)) * p.v_st + u.head * p.v_sh + d;
+#pragma unroll
       for (int e = 0; e < 16; ++e) {
+        if (!(wanted >> e & 1)) continue;
         const float x = to_float<BF16>(v[e]);
         if (!(fabsf(x) < INFINITY)) sum[e] += x;
+        if (sum[e] != sum[e]) wanted &= ~(1u << e);  // and stays so
       }
+    }
+  }
+}
+
+// A row whose scores are all numbers and whose results, in part [HD][128] where there is one, else in dst, have NaN among them:
+// those are the sums of the values that are no numbers.
+template <int HD, bool BF16>
+__device__ __noinline__ void look_again(const PagedParams& p, const Unit& u, int i, int first, int step, float* part, uint16_t* dst) {
+  for (int d = 0; d < HD; d += 16) {
+    uint32_t none = 0;
+    float sum[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = part != nullptr ? part[(d + e) * kHalf] : to_float<BF16>(dst[d + e]);
+      none |= x != x ? 1u << e : 0u;
+    }
+    odd_sum<BF16>(p, u, i, d, first, step, true, none, sum);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      if (!(none >> e & 1) || sum[e] == 0.f) continue;
+      if (part != nullptr)
+        part[(d + e) * kHalf] = sum[e];
+      else
+        dst[d + e] = static_cast<uint16_t>(pack_two<BF16>(sum[e], 0.f));
     }
   }
 }
@@ -417,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
           if (__any_sync(0xffffffffu, grow)) {
             const float mn = fmaxf(m, top);
-            const float keep = mn == m ? 1.f : exp2_near(m - mn);
+            const float keep = mn == m ? 1.f : shrink(m - mn);
             m = mn;
             l *= keep;
             if (t > 0) {
@@ -502,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (on) place(row, dst, lse);
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
         const bool odd_seen = n > 0 && *static_cast<volatile int*>(&sm.odd_seen);
+        float most = 0.f;  // NaN where a result is none
 #pragma unroll 1
         for (int d = 0; d < HD; d += 16) {
           float o[16];
@@ -517,9 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (odd_seen && on) {
             float bad[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) bad[e] = 0.f;
-            odd_sum<BF16>(p, u, who, d, first, step, bad);
+            odd_sum<BF16>(p, u, who, d, first, step, false, 0xffffu, bad);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] += bad[e];
           }
@@ -531,7 +561,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else if (on) {
             put(dst + d, o, inv);
           }
+          const float a = max3(o[0], o[1], o[2]), b = max3(o[3], o[4], o[5]), c = max3(o[6], o[7], o[8]), e = max3(o[9], o[10], o[11]);
+          most = max3(max3(a, b, c), max3(e, o[12], o[13]), max3(most, o[14], o[15]));
         }
+        // infinite values too light for 16 bits
+        if (on && most != most && l == l) look_again<HD, BF16>(p, u, who, first, step, split ? part + r : nullptr, dst);
         if (on) {
           if (split) {
             part[HD * kHalf + r] = m;
@@ -600,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                  k[z] = exp2_near(k[z] - ms);
+                  k[z] = shrink(k[z] - ms);
 #pragma unroll
                   for (int e = 0; e < 16; ++e) o[e] = i + z < pieces ? fmaf(x[z][e], k[z], o[e]) : o[e];
                 }
