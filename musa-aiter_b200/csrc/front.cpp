@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -19,6 +20,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -155,6 +157,13 @@ at::Tensor aligned_rows(const at::Tensor& x) {
   const auto st = x.strides();
   if (st[2] == 1 && st[0] % per == 0 && st[1] % per == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0) return x;
   return x.clone(at::MemoryFormat::Contiguous);  // contiguous() would keep the stride of an axis with one entry, whatever it is
+}
+
+// Forward-mode differentiation has no formula here: a tangent that a tensor carries would be lost in silence.
+void no_tangent(const char* name, std::initializer_list<const at::Tensor*> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(0).defined()) refuse(name, "no forward-mode derivative, but a tensor carries a tangent");
 }
 
 // ---- block-scaled caches --------------------------------------------------------------------------------
@@ -978,6 +987,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const List s = ctx->get_saved_variables();
     List got;
     try {
+      no_tangent("apply_qk_norm_rope", {&grads[0], &grads[1]});
       const auto g = norm_backward(grads[0], grads[1], {s[0], s[1], s[2], s[3], s[4], s[5], s[6], ctx->saved_data["eps"].toDouble(),
                                                         ctx->saved_data["interleaved"].toBool()});
       got.assign(g.begin(), g.end());
@@ -999,6 +1009,7 @@ PyObject* py_norm(PyObject*, Args a, Py_ssize_t n) {
     const char* name = "apply_qk_norm_rope";
     count(name, n, 9);
     const NormArgs x = norm_args(name, a);
+    no_tangent(name, {&x.q, &x.k, &x.wq, &x.wk, &x.cos, &x.sin});
     bool wants = false;
     if (c10::GradMode::is_enabled()) {
       if (x.cos.requires_grad() || x.sin.requires_grad()) refuse(name, "cos and sin are tables without a gradient, detach them");
