@@ -530,6 +530,7 @@ PyObject* py_rope(PyObject*, Args a, Py_ssize_t n) {
     count(name, n, 9);
     const at::Tensor &q0 = tensor(name, "q", a[0]), &k0 = tensor(name, "k", a[1]);
     at::Tensor pos = tensor(name, "positions", a[2]), cos = tensor(name, "cos", a[3]), sin = tensor(name, "sin", a[4]);
+    no_tangent(name, {&q0, &k0, &cos, &sin});
     if (c10::GradMode::is_enabled()) {
       if (cos.requires_grad() || sin.requires_grad()) refuse(name, "cos and sin are tables without a gradient, detach them");
       if (q0.requires_grad() || k0.requires_grad()) Py_RETURN_NONE;  // the caller's autograd function calls again, with gradients off

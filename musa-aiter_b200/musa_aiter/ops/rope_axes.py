@@ -51,7 +51,8 @@ def apply_rope_axes(
     columns; the others are copied.  Its angle is row positions[axis(j), t], column j of the tables; axes
     take their pairs one section after another, or in turn with ``interleaved_axes``.  Computed in 32 bits
     and rounded once.  A pair whose position lies outside the tables stays as it is.  Returns new tensors,
-    through which q and k get their gradients; cos and sin get none and may not require one."""
+    through which q and k get their gradients; cos and sin get none and may not require one.  There is no
+    forward-mode derivative: a tensor that carries a tangent is refused."""
     args = (q, k, positions, cos, sin, sections, interleaved, interleaved_axes, False)
     return _native.front().rope(*args) or _Rotation.apply(*args)
 

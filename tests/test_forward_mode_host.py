@@ -37,3 +37,23 @@ def test_norms(name):
             norm({})
         with forward_ad._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="no CPU fallback"):
             norm({name: dual})
+
+
+@pytest.mark.parametrize("name", ("q", "k", "cos", "sin"))
+@pytest.mark.parametrize("backward", [False, True])
+def test_rotations(backward, name):
+    a = dict(q=torch.zeros((3, 2, 64), dtype=torch.float16), k=torch.zeros((3, 1, 64), dtype=torch.float16), cos=torch.zeros((5, 32)),
+             sin=torch.zeros((5, 32)))
+
+    def call():
+        where = (torch.zeros((1, 3), dtype=torch.int32), a["cos"], a["sin"], (32,))
+        return (ma.apply_rope_axes_backward if backward else ma.apply_rope_axes)(a["q"], a["k"], *where)
+
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+        a[name] = dual(a[name])
+        with pytest.raises(ValueError, match="apply_rope_axes.*tangent"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+            call()
