@@ -683,10 +683,11 @@ int32_t count_of(const char* name, const char* what, PyObject* o) {
   if (v < 0) refuse(name, what, " must not be negative, got ", v);
   return static_cast<int32_t>(std::min<int64_t>(v, 0x7fffffff));
 }
-float scale_of(PyObject* o, int64_t head_dim) {
+float scale_of(const char* name, PyObject* o, int64_t head_dim) {
   if (o == Py_None) return static_cast<float>(1.0 / std::sqrt(static_cast<double>(head_dim)));
   const double scale = PyFloat_AsDouble(o);
   if (scale == -1.0 && PyErr_Occurred()) throw python_error();
+  if (!std::isfinite(static_cast<float>(scale) * 1.4426950408889634f)) refuse(name, "scale must be finite, in 32 bits and times log2 e");
   return static_cast<float>(scale);
 }
 
@@ -720,7 +721,7 @@ PyObject* py_paged(PyObject*, Args a, Py_ssize_t n) {
       separate(name, "out", o);
       used.push_back(&o);
     }
-    d.scale = scale_of(a[9], hd);
+    d.scale = scale_of(name, a[9], hd);
     for (const at::Tensor* t : used) dev.add(*t);
     dev.need_library();
     const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));
@@ -771,7 +772,7 @@ PyObject* py_weights(PyObject*, Args a, Py_ssize_t n) {
     }
     used.push_back(&lse);
     used.push_back(&sums);
-    d.scale = scale_of(a[10], q0.size(2));
+    d.scale = scale_of(name, a[10], q0.size(2));
     for (const at::Tensor* t : used) dev.add(*t);
     dev.need_library();
     const c10::cuda::CUDAGuard on(static_cast<c10::DeviceIndex>(dev.index));

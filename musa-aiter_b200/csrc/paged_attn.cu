@@ -693,6 +693,7 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   if (d->num_q_heads <= 0 || d->num_q_heads % c.num_heads)
     return fail(MAK_E_INVALID, "%s: %d query heads over %d cache heads", name, d->num_q_heads, c.num_heads);
   if (d->window < 0 || d->sinks < 0) return fail(MAK_E_INVALID, "%s: negative window or sinks", name);
+  if (!std::isfinite(d->scale * 1.4426950408889634f)) return fail(MAK_E_INVALID, "%s: the scale is not finite", name);
   if (d->parents != nullptr && d->window) return fail(MAK_E_INVALID, "%s: a tree has no window", name);
   if (c.num_rows * d->num_q_heads / c.num_heads > 0x7fffffff - 256)
     return fail(MAK_E_UNSUPPORTED, "%s: rows times query heads of a cache head are a 32-bit count", name);

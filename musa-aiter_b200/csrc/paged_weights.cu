@@ -335,6 +335,7 @@ extern "C" int mak_paged_weights(const mak_paged_weights_desc* d, void* stream) 
   if (d->num_q_heads <= 0 || d->num_q_heads % c.num_heads)
     return fail(MAK_E_INVALID, "%s: %d query heads over %d cache heads", name, d->num_q_heads, c.num_heads);
   if (d->window < 0 || d->sinks < 0) return fail(MAK_E_INVALID, "%s: negative window or sinks", name);
+  if (!std::isfinite(d->scale * 1.4426950408889634f)) return fail(MAK_E_INVALID, "%s: the scale is not finite", name);
   if (d->max_tokens < 0 || d->max_tokens > 0x7fffffff - 16 || d->sum_rows < 0)
     return fail(MAK_E_INVALID, "%s: sums of %lld rows of %lld tokens", name, static_cast<long long>(d->sum_rows),
                 static_cast<long long>(d->max_tokens));

@@ -10,8 +10,8 @@ sequence.  The last rows of a sequence sit at its last positions.  Rows that bel
 written.  Nothing is read back: block ids outside the cache are skipped by the kernels, as are tokens past
 ``max_blocks * block_size`` (rows keep the positions that ``context_lens`` gives them).
 
-Query head h reads cache head h // (num_q_heads // num_heads).  ``scale`` defaults to 1 / sqrt(head_dim).  For inference:
-no gradient flows through these calls.
+Query head h reads cache head h // (num_q_heads // num_heads).  ``scale`` defaults to 1 / sqrt(head_dim) and must be
+finite.  For inference: no gradient flows through these calls.
 """
 
 from __future__ import annotations
