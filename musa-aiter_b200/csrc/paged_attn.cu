@@ -36,7 +36,6 @@ struct Unit {
   Span s;
   int seq, head, tile, live;
   int ta, tb, len;  // this warp has steps [ta, tb) of len
-  int pad;
   int64_t wt;       // where the unit's steps begin in all work
 };
 

@@ -115,9 +115,6 @@ template <int T>
 __device__ __forceinline__ bool tile_whole(const Span& s, int tok) {
   return tok + T <= s.all_sinks || (tok >= s.all_lo && tok + T <= s.all_hi);
 }
-__device__ __forceinline__ bool seen_by_any(const PagedParams& p, const Span& s, int t) {
-  return t < s.any_hi && (t >= s.any_lo || t < p.sinks);
-}
 
 // Page of a token, -1 where there is none.
 __device__ __forceinline__ int page_of(const PagedParams& p, const int32_t* table, int tok) {

@@ -1,7 +1,11 @@
-// The kernel for many rows of the attention over paged 16-bit caches, as its entry point calls it.
+// The kernel for many rows of the attention over paged 16-bit caches, as its entry point calls it, and what it shares with that of
+// the attention weights.
 #pragma once
 
+#include <utility>
+
 #include "paged_attn.cuh"
+#include "tcgen05.cuh"
 
 namespace mak {
 
@@ -31,5 +35,49 @@ struct PagedSpace {
   float* partial;
 };
 PagedSpace paged_space(void* workspace);
+
+// ---- of the kernels for many rows ----------------------------------------------
+// f(0), f(1) ... f(N - 1) with the number as a constant.
+template <int N, typename F, int... I>
+__device__ __forceinline__ void steps_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void steps(F f) {
+  steps_of<N>(f, std::make_integer_sequence<int, N>());
+}
+
+// A warp's wait for a phase of a barrier, asleep for up to 0.1 ms at a time: a loop of short looks takes issue slots from
+// the warps that compute.  False when it did not complete in a second or so, or another role gave up.
+__device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile int* gave_up) {
+  uint32_t ok = 0;
+  for (uint32_t i = 0; i < (1u << 14); ++i) {
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_addr(b)), "r"(parity), "r"(100000)
+        : "memory");
+    if (ok || *gave_up) break;
+  }
+  if (!ok) *gave_up = 1;
+  return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 w, x, y, z;\n mov.b64 w, {%2, %3};\n mov.b64 x, {%4, %5};\n mov.b64 y, {%6, %7};\n fma.rn.f32x2 z, w, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 }  // namespace mak

@@ -17,8 +17,6 @@
 //   warp 16     TMA loads of K and rows
 //   warp 17     one thread issues all tcgen05.mma
 //   warp 18     lse of the rows
-#include <utility>
-
 #include "paged_weights.cuh"
 #include "tcgen05.cuh"
 
@@ -99,7 +97,7 @@ struct Walk {
 };
 struct Unit {
   PagedSeq v;
-  int seq, head, tok, any_lo, any_hi, all_lo, all_hi, all_sinks;
+  int seq, head, tok, any_lo, any_hi;
   int c0, n;       // this block has n chunks from c0 on
   int ta, tb, len; // of the unit's len, at least 1
   int64_t wt;      // where the unit's chunks begin in all work
@@ -131,44 +129,6 @@ __device__ __forceinline__ bool next_unit(const WeightParams& w, Walk& k, Unit& 
   return false;
 }
 
-template <int N, typename F, int... I>
-__device__ __forceinline__ void steps_of(F f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>()), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void steps(F f) {
-  steps_of<N>(f, std::make_integer_sequence<int, N>());
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 z, x, y;\n mov.b64 {%0, %1}, z;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n .reg .b64 w, x, y, z;\n mov.b64 w, {%2, %3};\n mov.b64 x, {%4, %5};\n mov.b64 y, {%6, %7};\n fma.rn.f32x2 z, w, x, y;\n"
-      " mov.b64 {%0, %1}, z;\n}"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-// A warp's wait for a phase of a barrier, asleep for up to 0.1 ms at a time.  False when it did not complete in a second or
-// so, or another role gave up.
-__device__ __forceinline__ bool wait_warp(uint64_t* b, uint32_t parity, volatile int* gave_up) {
-  uint32_t ok = 0;
-  for (uint32_t i = 0; i < (1u << 14); ++i) {
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok)
-                 : "r"(smem_addr(b)), "r"(parity), "r"(100000)
-                 : "memory");
-    if (ok || *gave_up) break;
-  }
-  if (!ok) *gave_up = 1;
-  return __all_sync(0xffffffffu, ok);
-}
 __device__ __forceinline__ void math_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 __device__ __forceinline__ void box3(uint32_t to, const void* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(

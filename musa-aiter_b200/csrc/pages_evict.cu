@@ -35,7 +35,7 @@ struct EvictParams {
   int64_t table_stride;
   int64_t sum_sl, sum_sr, sum_sh;
   int64_t k_sb, k_st, k_sh, v_sb, v_st, v_sh;  // elements
-  int32_t num_rows, max_blocks, pages, bs, n, nh, head_dim, max_tokens;
+  int32_t num_rows, max_blocks, pages, bs, nh, max_tokens;
   int32_t keep, sinks, recent, layer0;
   int32_t cached;   // sums of a row are kept in shared memory
   int32_t bs_log2;  // -1: no power of 2
@@ -373,7 +373,7 @@ extern "C" int mak_pages_evict(const mak_pages_desc* d, const mak_evict_desc* e,
   p.v_sb = e->value_stride_block, p.v_st = e->value_stride_token, p.v_sh = e->value_stride_head;
   p.num_rows = static_cast<int32_t>(d->num_rows), p.max_blocks = static_cast<int32_t>(d->max_blocks);
   p.pages = static_cast<int32_t>(d->num_pages), p.bs = static_cast<int32_t>(d->block_size);
-  p.n = static_cast<int32_t>(n), p.nh = e->num_heads, p.head_dim = e->head_dim;
+  p.nh = e->num_heads;
   p.max_tokens = static_cast<int32_t>(e->max_tokens);
   p.bs_log2 = (p.bs & (p.bs - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(p.bs)) : -1;
   p.keep = e->keep, p.sinks = e->sinks, p.recent = e->recent;
