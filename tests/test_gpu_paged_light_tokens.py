@@ -90,3 +90,12 @@ def test_light_weights_add_next_to_nothing(new, dtype):
     agree_all = c.attention()
     got, lse = ma.paged_attention_window(*c.args(), c.on("starts"), return_lse=True)
     check(got, agree_all[0], lse, agree_all[1], agree_all[2])
+
+
+def test_a_long_line_of_drafted_tokens_and_values_that_are_no_numbers():
+    """Every row's line goes back over 600 rows, and what it sees before them is looked through for NaN and infinite values."""
+    c = with_gap([9000], [600], torch.float16, 25.0, 70, group=1)
+    line = torch.arange(-1, 599, dtype=torch.int32)
+    agree(c, 70, line)
+    c.layer[1, c.tables[0, 8000 // 16], 8000 % 16, 0, 9] = math.nan
+    agree(c, 70, line)
