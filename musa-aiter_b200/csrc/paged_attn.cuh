@@ -73,7 +73,7 @@ __device__ __forceinline__ RowView row_view(const PagedParams& p, const PagedSeq
 __device__ __forceinline__ uint32_t tree_bits(const PagedParams& p, const PagedSeq& v, int i, int t0) {
   const int base = v.ctx - v.rows;
   uint32_t bits = t0 >= base ? 0u : base - t0 >= 32 ? 0xffffffffu : (1u << (base - t0)) - 1u;
-  for (int a = i; a >= 0 && base + a >= t0;) {
+  for (int a = base - t0 >= 32 ? -1 : i; a >= 0 && base + a >= t0;) {
     const int e = base + a - t0;
     if (e < 32) bits |= 1u << e;
     const int up = __ldg(p.parents + v.first + a);

@@ -211,14 +211,15 @@ struct TcSmem {
 template <bool BF16>
 __device__ __noinline__ void odd_sum(const PagedParams& p, const Unit& u, int i, int d, int first, int step, bool all, uint32_t wanted, float* sum) {
   const RowView r = row_view(p, u.v, i);
-  const int common = min(u.v.ctx - u.v.rows, u.v.room);  // tokens before a tree
 #pragma unroll
   for (int e = 0; e < 16; ++e) sum[e] = 0.f;
   for (int j = u.ta + first; j < u.ta + u.n && wanted != 0; j += step) {
     const int tok = tile_token<kTile>(u.s, j);
     if (!all && tile_whole<kTile>(u.s, tok)) continue;
+    uint32_t bits = 0;  // of 32 tokens of a tree
     for (int t = tok; t < tok + kTile; ++t) {
-      const bool seen = p.parents != nullptr ? t < common || (tree_bits(p, u.v, i, t) & 1) : t < r.hi && (t >= r.lo || t < p.sinks);
+      if (p.parents != nullptr && (t & 31) == 0) bits = tree_bits(p, u.v, i, t);
+      const bool seen = p.parents != nullptr ? bits >> (t & 31) & 1 : t < r.hi && (t >= r.lo || t < p.sinks);
       if (!seen) continue;
       const int page = page_of(p, p.tables + u.seq * p.table_stride, t);
       if (page < 0) continue;
