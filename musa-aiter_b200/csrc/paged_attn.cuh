@@ -101,9 +101,12 @@ __device__ __forceinline__ Span span_of(const PagedParams& p, const PagedSeq& v,
   }
   s.all_sinks = min(p.sinks, s.all_hi);
   s.t0 = s.any_lo / T;
-  s.ns = min((min(p.sinks, s.any_hi) + T - 1) / T, s.t0);
-  const int t1 = (s.any_hi + T - 1) / T;
-  s.tiles = s.ns + (s.any_hi > s.any_lo ? t1 - s.t0 : 0);
+  s.ns = (min(p.sinks, s.any_hi) + T - 1) / T;
+  s.tiles = s.ns;
+  if (s.any_hi > s.any_lo) {  // else all windows lie past the table's tokens, and the first tokens are all there is
+    s.ns = min(s.ns, s.t0);
+    s.tiles = s.ns + (s.any_hi + T - 1) / T - s.t0;
+  }
   return s;
 }
 // First token of tile j of a span.
