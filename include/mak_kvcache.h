@@ -790,7 +790,7 @@ typedef struct mak_paged_attn_desc {
 MAK_API int64_t mak_paged_attention_workspace_bytes(void);
 
 /*
- * out[r, h] = softmax(scale * q[r, h] . K^T) V over the tokens that row r sees.  Row r of sequence s is its
+ * out[r, h] = softmax(scale * q[r, h] . K^T) V over the tokens that row r sees, scale finite.  Row r of sequence s is its
  * i = (r - cu_seqlens[s])-th row of this call, at position context_lens[s] - (rows of s) + i.
  * Without parents it sees the tokens t up to its own position, with window > 0 only those with t > position - window or
  * t < sinks.  With parents it sees the tokens before the sequence's first row, itself, its parent parents[r] (the index
@@ -818,7 +818,7 @@ typedef struct mak_paged_weights_desc {
 
 /*
  * sums[row of s, h, t] = or += (accumulate) the sum over the rows of sequence s that see token t (as above) and over the
- * query heads of cache head h of exp(scale * q . k_t - lse).  Without accumulate the whole row of sums is written, zeros
+ * query heads of cache head h of exp(scale * q . k_t - lse), scale finite.  Without accumulate the whole row of sums is written, zeros
  * where no row sees; with it other places are left.  Tokens at or past max_tokens have no place.
  */
 MAK_API int mak_paged_weights(const mak_paged_weights_desc* desc, void* stream);
@@ -838,7 +838,7 @@ typedef struct mak_evict_desc {
  * `recent` and of the others those of the largest sums (the first of equal ones; NaN counts as -inf), in their order;
  * sums move along and become 0 behind.  Pages past the kept tokens lose a reference, their entries become -1.  left[0]
  * counts the rows left alone: a page that would be written is shared or a page is out of range, or the row has more
- * tokens than its table or max_tokens hold.  A row named twice shrinks once.  `state` is scratch of n int32.
+ * tokens than its table or max_tokens hold.  A row named twice shrinks once; n is at most 8192.  `state` is scratch of n int32.
  */
 MAK_API int mak_pages_evict(const mak_pages_desc* pages, const mak_evict_desc* evict, const int32_t* rows, int64_t n, int32_t* left,
                             int32_t* state, void* stream);

@@ -715,7 +715,8 @@ extern "C" int mak_paged_attention(const mak_paged_attn_desc* d, void* stream) {
   // Rows that share a cache head, on average.  Few rows read K and V again for every 16; many rows wait for a unit's
   // longer beginning and end.  Few / many in us, 8 cache heads of 128 with 4 query heads: 16 sequences of 4096 tokens
   // 63 / 62 for 16 rows, 110 / 62 for 32 (heads of 64: 38 / 49, 61 / 49); 64 of 512 44 / 61, 55 / 61, 76 / 70 for 48; one of
-  // 4096 25 / 27, 25 / 27, 35 / 48 for 128.
+  // 4096 25 / 27, 25 / 27, 35 / 48 for 128.  The average alone decides, which is not the faster kernel everywhere: one sequence's
+  // 17 to 128 rows, and 32 rows of many short sequences, are taken up to a third slower than the other kernel would.
   const int64_t rows = c.num_rows * p.group / c.num_seqs;
   const bool many = rows > 16 && paged_tc_fits(p);
   const int tokens = many ? paged_tc_box(c.block_size) : kStep;

@@ -28,8 +28,11 @@
 // Bound by the chain of scores, softmax and products within a half, and by the tensor cores' reading of shared memory: a
 // 128 x 64 x 16 product reads its operands in 48 cycles and multiplies in 32, so a pair of tiles needs 1280 cycles of the
 // tensor cores where the softmax needs some 1000.  Measured, calls in a graph, 8 cache heads of 128 in bfloat16 for 32 query
-// heads: two prompts of 1500 to 2048 rows on 5000 to 8192 tokens, window of 4096, 261 us, 903 TFLOP/s of the 1692 that a plain matrix product has; the beginnings and ends of units are a ninth of that.
-// 16 trees of 8 to 32 tokens on 300 to 4500 tokens 69 us, beginnings, ends and joins for the most part (K and V alone: 22).
+// heads: two prompts of 1500 to 2048 rows on 5000 to 8192 tokens, window of 4096, 257 us, 919 TFLOP/s of the 1692 that a plain
+// matrix product has (270 to 290 under lasting load); the beginnings and ends of units are a ninth of that.
+// 16 trees of 8 to 32 tokens on 300 to 4500 tokens 71 us, beginnings, ends and joins for the most part (K and V alone: 22).
+// Light weights of infinite values are looked for at a unit's end alone; weights kept above 0 in every tile took the prompts 4 %,
+// a look at every value on its way 2.3 %.
 // What was tried for the prompts: one thread that issues all products 531 us, one warp 314, a warp per half 263 (kept);
 // two threads to a row 347; tiles of 128 with one place for scores 302; scores fetched a tile ahead 356; some exponentials
 // by polynomial 265 to 270; weights against the old maximum without looking for the new one 291.

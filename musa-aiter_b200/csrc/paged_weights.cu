@@ -365,7 +365,8 @@ extern "C" int mak_paged_weights(const mak_paged_weights_desc* d, void* stream) 
   const bool bf16 = c.dtype == MAK_DT_BF16;
   // Rows that share a cache head, on average; a group has to fit the chunks of rows.  Few / many in us, 8 cache heads of 128
   // with 4 query heads: 16 sequences of 4096 tokens 33 / 80 for 16 rows, 97 / 80 for 32, 133 / 85 for 48 (heads of 64: 25 / 73,
-  // 58 / 73, 77 / 78); 64 of 512 19 / 44, 51 / 44; one of 4096 11 / 14, 20 / 14.
+  // 58 / 73, 77 / 78); 64 of 512 19 / 44, 51 / 44; one of 4096 11 / 14, 20 / 14.  The average alone decides: 17 to 32 rows with heads
+  // of 64 are taken up to a quarter slower than the other kernel would.
   const bool many = c.num_rows * w.a.group / c.num_seqs > 16 && c.num_seqs * 8 <= space.plan_bytes && weights_tc_fits(w);
   CUtensorMap k;
   if (!paged_map(&k, w.a.key, w.a.k_sb, w.a.k_st, w.a.k_sh, w.a.num_blocks, w.a.nh, c.head_dim, c.block_size, bf16, many ? c.block_size : kStep,

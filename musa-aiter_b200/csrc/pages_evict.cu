@@ -11,7 +11,8 @@
 // head; a second small launch returns the pages.  Measured: 16 requests of 1500 to 4096 tokens to 1024, 8 layers, 8 heads of
 // 128: 246 us (4.5 TB/s of 6.5 that a plain copy has), of which a block's search for its tokens is a seventh; one request of
 // 30000 tokens to 2000, 4 heads of 64: 65 us, four blocks' search (two thirds) and walk; with 8192 tokens to a list, not 4096,
-// the walk has its batches in one row (81 to 68 us, together with counts of each lane for equal first bytes).  Batches of 64
+// the walk has its batches in one row (81 to 68 us, together with counts of each lane for equal first bytes).  128 registers a
+// thread, of which 8 words are spilled.  Batches of 64
 // tokens and 2 blocks on an SM were the best of those tried: 32 tokens 352 to 413 us, 40 415, 48 344, 128 480; slices of 64
 // or 128 bytes of each token to a warp, which needs no barrier, 374 and 362.
 #include "common.cuh"

@@ -42,8 +42,8 @@ def paged_attention_window(
     A row at position p sees the tokens t <= p; with ``window`` > 0 only those with t > p - window, and the first
     ``sinks`` tokens.  Returns ``out`` (q's dtype), or ``(out, lse)`` with the log of each row's sum of exponentials,
     float32 ``[rows, num_q_heads]``.  A row that sees no token gives zeros and an lse of -inf.  Nothing that a row does not
-    see reaches its result, NaN among it.  A workspace is kept per device and stream until the process ends; a call
-    captured in a graph has one of its own."""
+    see reaches its result, NaN among it.  A workspace of 39 MiB is kept per device and stream until the process
+    ends; a call captured in a graph has one of its own."""
     return _native.front().paged(q, key_cache, value_cache, block_tables, context_lens, cu_seqlens, None, window, sinks, scale,
                                  return_lse, out)
 

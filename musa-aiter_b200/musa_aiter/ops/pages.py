@@ -98,5 +98,5 @@ def kv_pages_evict(
 
     Returns an int32 ``[1]`` tensor on the device: how many rows were left as they are because a page that would be
     written is shared with another row, a page is out of range, or they have more tokens than their table or ``sums``
-    hold.  A row named twice shrinks once."""
+    hold.  A row named twice shrinks once.  A call takes up to 8192 rows."""
     return _native.front().evict(block_tables, context_lens, rows, ref_counts, key_caches, value_caches, sums, keep, sinks, recent)

@@ -30,10 +30,11 @@ def apply_qk_norm_rope(
     Weights are ``[head_dim]``, float32 or of q's type; ``positions`` int32 or int64 ``[tokens]``; the tables float32
     ``[max_positions, pairs]``.  Pair j is (j, j + pairs), or (2 j, 2 j + 1) with ``interleaved``, of the first 2 * pairs
     columns; the others are normalised alone, and so is a token whose position lies outside the tables.  head_dim is a
-    multiple of 16 up to 256, pairs a multiple of 8.  Computed in 32 bits and rounded once.  Returns new tensors,
-    through which q, k and the weights get their gradients (these have none of their own); cos and sin get none and may
-    not require one.  There is no forward-mode derivative: a tensor that carries a tangent is refused.  A backward pass is captured into a CUDA graph like any of torch's: no eager graph of the same leaves
-    may live meanwhile."""
+    multiple of 16 up to 256, pairs a multiple of 8.  Computed in 32 bits (a head whose sum of squares is past their range
+    gives zeros) and rounded once.  Returns new tensors, through which q, k and the weights get their gradients (these
+    have none of their own); cos and sin get none and may not require one.  There is no forward-mode derivative: a tensor
+    that carries a tangent is refused.  A backward pass is captured into a CUDA graph like any of torch's: no eager graph
+    of the same leaves may live meanwhile."""
     return _native.front().norm(q, k, q_weight, k_weight, positions, cos, sin, eps, interleaved)
 
 
