@@ -261,11 +261,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   int in = 0, stage_in = 0;  // steps loaded so far
   uint32_t there = 0;        // bit i: step i % 32 has a page
+  bool ok = true;            // no wait has run out
   auto load = [&]() {
     if (more && left_in == 0) enter();
     if (!more) return;
     const int page = __shfl_sync(0xffffffffu, next_id, 0), tok = __shfl_sync(0xffffffffu, tok_in, 0), head = __shfl_sync(0xffffffffu, head_in, 0);
-    const bool has = page >= 0 && page < p.num_blocks;
+    const bool has = ok && page >= 0 && page < p.num_blocks;
     there = (there & ~(1u << (in & 31))) | (has ? 1u << (in & 31) : 0u);
     tok_in = tok_in == jump_at ? jump : tok_in + kStep;
     --left_in;
@@ -298,7 +299,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;
   int units_out = 0, out = 0, stage = 0;
   uint32_t phases = 0;  // bit of a stage: the parity of its next phase
-  bool ok = true;
   while (units_out < units_in) {
     const Unit& u = queue[units_out % kQueue];
     uint32_t qf[HD / 16][4];
@@ -328,8 +328,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Span span = u.s;
     for (int j = ta; j < tb; ++j, ++out) {
       load();
-      if (there >> (out & 31) & 1) {
-        ok = mbar_wait_warp(full + stage, phases >> stage & 1, gave_up) && ok;
+      bool has = there >> (out & 31) & 1;
+      if (has && !mbar_wait_warp(full + stage, phases >> stage & 1, gave_up)) {
+        land<kStages>(full, out, in, there, phases);
+        there = 0;
+        has = ok = false;
+      }
+      if (has) {
         phases ^= 1u << stage;
         const int tok = tile_token<kStep>(span, j);
         const uint32_t at = ring + stage * (2 * kTileBytes);

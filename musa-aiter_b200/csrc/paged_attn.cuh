@@ -9,6 +9,7 @@
 #include <cmath>
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace mak {
 
@@ -227,6 +228,16 @@ __device__ __forceinline__ void box_load(uint32_t to, const void* map, int x, in
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(v), "r"(shared_at(bar))
       : "memory");
+}
+// A warp's wait for the loads of steps [from, to) that have been issued (`there`, a bit for each of the last 32) ends when they
+// have landed, or with its limit: after a wait that ran out, so that none lands later.
+template <int STAGES>
+__device__ __forceinline__ void land(uint64_t* full, int from, int to, uint32_t there, uint32_t phases) {
+  for (int k = from; k < to; ++k)
+    if (there >> (k & 31) & 1)
+      for (uint32_t i = 0; i < kWaitLimit && !mbar_try(full + k % STAGES, phases >> (k % STAGES) & 1); ++i) {
+      }
+  __syncwarp();
 }
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {

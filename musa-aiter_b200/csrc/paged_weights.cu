@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
   int parts_in = 0, left_in = 0, in = 0, stage_in = 0;
   int tok_in = 0, jump_at = 0, jump = 0, any_lo = 0, any_hi = 0, head_in = 0, next_id = -1;
   uint32_t there = 0;  // bit i: step i % 32 has a page
+  bool ok = true;      // no wait has run out
   const int32_t* table_in = nullptr;
   const float* old_in = nullptr;
   const int inside = (1 << p.bs_log2) - 1;
@@ -184,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
     }
     if (more) {
       const int page = __shfl_sync(0xffffffffu, next_id, 0), tok = __shfl_sync(0xffffffffu, tok_in, 0), head = __shfl_sync(0xffffffffu, head_in, 0);
-      const bool has = page >= 0 && page < p.num_blocks;
+      const bool has = ok && page >= 0 && page < p.num_blocks;
       there = (there & ~(1u << (in & 31))) | (has ? 1u << (in & 31) : 0u);
       if (w.add && lane < kStep) {
         const bool fits = tok + lane < w.max_tokens;
@@ -213,7 +214,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
   const int r = lane >> 2, c2 = (lane & 3) * 2;
   int out = 0, stage = 0;
   uint32_t phases = 0;  // bit of a stage: the parity of its next phase
-  bool ok = true;
   for (int parts_out = 0; parts_out < parts_in; ++parts_out) {
     const Part& u = queue[parts_out % kQueue];
     const int seq = u.seq, head = u.head, ta = u.ta, tb = u.tb;
@@ -249,8 +249,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
       if (w.add) copies_wait<kStages - 1>();
       const int tok = w.add ? tile_token<kStep>(span, j) : j * kStep;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};  // tokens c2, c2 + 1, c2 + 8, c2 + 9
-      if (there >> (out & 31) & 1) {
-        ok = mbar_wait_warp(full + stage, phases >> stage & 1, gave_up) && ok;
+      bool has = there >> (out & 31) & 1;
+      if (has && !mbar_wait_warp(full + stage, phases >> stage & 1, gave_up)) {
+        land<kStages>(full, out, in, there, phases);
+        there = 0;
+        has = ok = false;
+      }
+      if (has) {
         phases ^= 1u << stage;
         const uint32_t tile = ring + stage * kTileBytes;
         int64_t row0 = 0;
@@ -291,8 +296,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_kernel(const __grid
           sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 8);
           sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 16);
         }
-        if (!ok) sum[0] = sum[1] = sum[2] = sum[3] = __uint_as_float(0x7fffffffu);  // a block that gave up leaves NaN
       }
+      if (!ok) sum[0] = sum[1] = sum[2] = sum[3] = __uint_as_float(0x7fffffffu);  // a warp that gave up leaves NaN
       __syncwarp();
       if (r < 2) {  // eight lanes, two tokens each
 #pragma unroll
